@@ -368,6 +368,60 @@ int qspec_rope_qkhad_kvcache(void* qkv, const void* cos_sin_cache, const int* po
                              void* cache_k, void* cache_v, int T, int Hq, int Hkv, int D, int S, float had_scale,
                              void* stream);
 
+/* ---- speculative decoding over a cache in pages and in 8 bits (the reference leaves paging, the cache's type and the rejection sampler to
+ * vLLM: vllm/core/block_manager.py, vllm/attention, vllm/model_executor/layers/rejection_sampler.py) ------------------------------------
+ *
+ * Cache of a layer: codes int8 [pages, G, P, D] and scales float32 [pages, G], for keys and for values; a code c stands for c * scale. P is 16, 32,
+ * 64 or 128 tokens, D 64 or 128. A slot is page * P + row. A table int32 [requests, width] names each request's pages in order.
+ *
+ * qspec_page_plan: the pages and slots of one step, from lengths on the device. lengths[b] tokens are held, counts[b] come with the step; counts[b] < 0: the
+ * request has ended, and its pages go back. state int32 [requests + 1]: pages held by each request, then the number of free pages; free_pages[0 ..
+ * number) are those. Pages that come back go behind them, in the order of the requests; pages are handed out from the end of that list, in the
+ * order of the requests. A request is refused (no pages; kv_len 0; its tokens without positions and slots) where what was asked for so
+ * far, its own pages included, is more than there is, where its row of the table is too short, or where its tokens do not fit into ntok.
+ *   q_start [requests + 1]: first token of each request; kv_len [requests]: tokens held once the step has run (0: refused or ended);
+ *   positions, seq_ids, slots [ntok]: of each token; -1 where there is none. state_out [requests + 2]: the state behind this step, then the number of
+ *   requests refused.
+ * `state` is not changed, nor is anything that it describes (table entries and list entries behind it are): a step that is given up costs nothing, one that
+ * is made is made so by copying state_out over state. state_out must not overlap state. requests <= 4096, width <= 2^18. */
+int qspec_page_plan(const int* lengths, const int* counts, int* table, int* free_pages, const int* state, int requests, int width, int npages,
+                    int page_tokens, int ntok, int* q_start, int* kv_len, int* positions, int* seq_ids, int* slots, int* state_out, void* stream);
+
+/* Rotation of queries and keys, and keys and values into their pages. qkv [ntok, ld]: rows [q (H x D) | k (G x D) | v (G x D)], not changed. cos_sin
+ * [cos_rows, D] = [cos | sin] of the rows' type (neox pairs, as in qspec_rope_kvcache). q_out [ntok, H, D] (token stride q_tok_stride; NULL: no queries).
+ * A page's scale: the largest of |x| / 127 of the rows that the call writes to it, of its scale before (unless its first row is among them) and 2^-60; codes =
+ * rint(x / scale) (infinities: +-127, NaN: 0, neither stretches the scale). Where a scale grows the page's older rows are put on the new one.
+ * Rotated values are quantised in float32, without a rounding to 16 bits in between. Tokens whose slot or position is outside the cache or
+ * the table of angles are skipped. The tokens of one page in a call must be neighbours in the batch, in consecutive rows. */
+int qspec_kv8_append(const void* qkv, long long ld, const void* cos_sin, int cos_rows, const int* positions, const int* slots, void* k, void* v, float* k_scale,
+                     float* v_scale, void* q_out, long long q_tok_stride, int ntok, int H, int G, int D, int npages, int page_tokens, int dtype, void* stream);
+
+/* Rows of the cache in 16 bits: k_out, v_out [rows, G, D] of slots[0 .. rows). A slot outside the cache gives zeros. */
+int qspec_kv8_read(const void* k, const void* v, const float* k_scale, const float* v_scale, const int* slots, void* k_out, void* v_out, int rows, int G, int D,
+                   int npages, int page_tokens, int dtype, void* stream);
+
+/* Softmax attention of a step's tokens over that cache. q [ntok, H, D] with free token / head strides; the tokens q_start[b] .. q_start[b + 1] - 1 of
+ * request b stand at the last positions of its kv_len[b] tokens and see the keys up to their own. Tokens that see no key give zeros; tokens
+ * behind q_start[requests] are not written. max_tokens: an upper bound of the tokens that any request has in the step. Scales are positive (a scale
+ * below 2^-100 counts as that); pages outside the cache make the rows that see them NaN. workspace: zero-initialised once, left ready for the next call;
+ * one for each stream that calls are made on at the same time. */
+size_t qspec_kv8_attention_workspace_bytes(void);
+int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* k_scale, const float* v_scale,
+                        const int* table, const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests,
+                        int width, int H, int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Verification of drafted tokens, and one token more. drafted int64 [requests, drafts]; draft / target float32 probabilities, row of (request b, place i) at
+ * b * seq_stride + i * place_stride, `drafts` and drafts + 1 places; uniform float32 [requests, drafts + 1] in [0, 1); draft_counts (NULL: all) int32: how
+ * many drafts a request has. Draft i is taken if uniform[b, i] * q_i(d_i) < p_i(d_i) (exactly) and all before it were. Then one token by inversion with
+ * uniform[b, drafts]: from max(p - q, 0) at the first place refused; from p at the place behind the drafts where all were taken, or where that difference
+ * is zero everywhere: the first token whose running sum (64 bits) is above uniform * total. tokens int64 [requests, drafts + 1]: what is emitted, -1 behind it;
+ * emitted int64 [requests]: how many. A row of p without any mass gives token 0; a drafted token outside the vocabulary is refused. */
+int qspec_verify_drafts_max_drafts(void);
+int qspec_verify_drafts(const long long* drafted, const float* draft, long long draft_seq_stride, long long draft_place_stride, const float* target,
+                        long long target_seq_stride, long long target_place_stride, const float* uniform, const int* draft_counts, long long* tokens,
+                        long long* emitted, int requests, int drafts, int vocab, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

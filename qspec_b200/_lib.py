@@ -92,6 +92,15 @@ SIGNATURES = {
     "qspec_seq_attention_supported": (c_int, [c_int, c_int, c_int, c_int, c_int]),
     "qspec_seq_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                     c_int, c_int, c_float, c_void_p]),
+    "qspec_page_plan": (c_int, [c_void_p] * 5 + [c_int] * 5 + [c_void_p] * 7),
+    "qspec_kv8_append": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, c_int] + [c_void_p] * 7 + [ctypes.c_longlong] + [c_int] * 7 + [c_void_p]),
+    "qspec_kv8_read": (c_int, [c_void_p] * 7 + [c_int] * 6 + [c_void_p]),
+    "qspec_kv8_attention_workspace_bytes": (ctypes.c_size_t, []),
+    "qspec_kv8_attention": (c_int, [c_void_p, ctypes.c_longlong, c_int] + [c_void_p] * 8 + [ctypes.c_longlong] + [c_int] * 10 + [c_float, c_int, c_void_p, ctypes.c_size_t,
+                                    c_void_p]),
+    "qspec_verify_drafts_max_drafts": (c_int, []),
+    "qspec_verify_drafts": (c_int, [c_void_p, c_void_p, ctypes.c_longlong, ctypes.c_longlong, c_void_p, ctypes.c_longlong, ctypes.c_longlong] + [c_void_p] * 4 +
+                            [c_int] * 3 + [c_void_p]),
     "qspec_argmax_rows_workspace_bytes": (ctypes.c_size_t, [c_int]),
     "qspec_argmax_rows_static_max_rows": (c_int, []),
     "qspec_argmax_rows_static": (c_int, [c_void_p, c_int, c_int, ctypes.c_longlong, c_void_p, c_void_p, c_void_p]),

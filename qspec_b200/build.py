@@ -14,7 +14,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_C")
 LIB_PATH = os.path.join(OUT_DIR, "libqspec_b200.so")
-SOURCES = ["capi.cu", "act_kernels.cu", "hadamard_kernels.cu", "gemm_w4_stream.cu", "attn_kernels.cu", "qwen_kernels.cu"]
+SOURCES = ["capi.cu", "act_kernels.cu", "hadamard_kernels.cu", "gemm_w4_stream.cu", "attn_kernels.cu", "qwen_kernels.cu", "kv8_kernels.cu",
+           "kv8_attention.cu", "spec_kernels.cu"]
 # The sequence-mixer kernels (include/qspec_b200_seq.h) are a library of their own, so that a model that needs only them
 # builds only them: libqspec_b200_seq.so.
 SEQ_SOURCES = ["capi.cu", "seq_kernels.cu", "seq_mma_kernels.cu", "seq_mix_kernels.cu", "seq_state_kernels.cu", "seq_head_kernels.cu",
@@ -32,7 +33,7 @@ def _nvcc() -> str:
 
 
 def _newest_source_mtime(sources=None) -> float:
-    names = [f for f in os.listdir(CSRC) if f != "fast_call.cpp"] if sources is None else list(sources) + ["common.cuh", "seq_common.cuh", "attn_tile.cuh", "gemm_w4_rows.cuh", "recurrence_mma.cuh", "smem_limit.h"]
+    names = [f for f in os.listdir(CSRC) if f != "fast_call.cpp"] if sources is None else list(sources) + ["common.cuh", "seq_common.cuh", "attn_tile.cuh", "gemm_w4_rows.cuh", "recurrence_mma.cuh", "smem_limit.h", "kv8_common.cuh"]
     paths = [os.path.join(CSRC, f) for f in names]
     paths.append(os.path.join(HERE, "..", "include", "qspec_b200.h"))
     paths.append(os.path.join(HERE, "..", "include", "qspec_b200_seq.h"))

@@ -1,0 +1,434 @@
+// A key/value cache in pages and in 8 bits: the page plan of a step, the writer of the cache and its inverse. The attention that reads it is in
+// kv8_attention.cu.
+//
+// Cache of a layer: codes int8 [pages, G, P, D] (a page's rows of one head are P * D bytes in a row) and scales float32 [pages, G] for keys and for
+// values; a code c stands for c * scale. P tokens a page: a power of two from 16 to 128. A slot is page * P + row.
+#include "kv8_common.cuh"
+
+namespace qspec {
+namespace kv8 {
+
+// ---- pages and slots of a step ----------------------------------------------------------------------------------------------------
+// Nothing here is of size: three prefix sums over the requests (tokens, pages wanted, pages given back), then one thread per token, per new table entry
+// and per page that goes back. Every CTA makes the sums for itself (4096 requests are 48 KB of reads from L2) and takes its share of the rest, so
+// that no CTA waits for another; nothing that a call reads is written by it (table entries from `held` on and list entries from n_free on mean nothing to
+// the state that came in), so that the order of the CTAs does not matter and a call can be made again.
+constexpr int PLAN_THREADS = 1024, PLAN_REQUESTS = 4096, PLAN_EACH = PLAN_REQUESTS / PLAN_THREADS;
+
+struct PlanArgs {
+  const int *lengths, *counts;
+  int* table;
+  int* free_pages;
+  const int* state;
+  int *q_start, *kv_len, *positions, *seq_ids, *slots, *state_out;
+  int n, width, npages, pshift, ntok;
+};
+
+// index of the last entry of the ascending s[0 .. n - 1] that is <= x (s[0] <= x)
+__device__ __forceinline__ int last_at_most(const int* s, int n, int x) {
+  int lo = 0;
+  for (int step = PLAN_REQUESTS; step; step >>= 1)
+    if (lo + step < n && s[lo + step] <= x) lo += step;
+  return lo;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs a) {
+  extern __shared__ int plan_smem[];
+  int* s_tok = plan_smem;                         // first token of each request, in front of it [n + 1]
+  int* s_need = s_tok + a.n + 1;                  // pages asked for before it [n + 1]
+  int* s_back = s_need + a.n + 1;                 // pages given back before it [n + 1]
+  __shared__ int s_warp[3][32], s_refused[32], s_over;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) s_over = a.n;
+  pdl_enter();
+  const int n_free = min(max(a.state[a.n], 0), a.npages);
+  int cnt[PLAN_EACH], len[PLAN_EACH], held[PLAN_EACH], need[PLAN_EACH];
+  int sum[3] = {0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < PLAN_EACH; ++e) {
+    const int b = tid * PLAN_EACH + e;
+    cnt[e] = len[e] = held[e] = need[e] = 0;
+    if (b < a.n) {
+      cnt[e] = a.counts[b];
+      len[e] = a.lengths[b];
+      held[e] = min(max(a.state[b], 0), a.width);
+      if (cnt[e] > 0) {
+        const long long want = ((long long)len[e] + cnt[e] + (1 << a.pshift) - 1) >> a.pshift;
+        if (len[e] >= 0 && want <= a.width) need[e] = max((int)want - held[e], 0);
+      }
+    }
+    // (a sum of tokens that passes the tokens there are room for says no more than that: it stays there)
+    sum[0] = (int)min((long long)sum[0] + max(cnt[e], 0), (long long)a.ntok + 1);
+    sum[1] += need[e];
+    sum[2] += cnt[e] < 0 ? held[e] : 0;
+  }
+  int pre[3];
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    int v = sum[q];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int w = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v = q ? v + w : (int)min((long long)v + w, (long long)a.ntok + 1);
+    }
+    pre[q] = v;
+    if (lane == 31) s_warp[q][warp] = v;
+  }
+  __syncthreads();
+  if (warp == 0) {
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      int v = s_warp[q][lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int w = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v = q ? v + w : (int)min((long long)v + w, (long long)a.ntok + 1);
+      }
+      s_warp[q][lane] = v;
+    }
+  }
+  __syncthreads();
+  int at[3];                                       // sums in front of this thread's first request
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    const int before = __shfl_up_sync(0xffffffffu, pre[q], 1), prev = warp ? s_warp[q][warp - 1] : 0;
+    at[q] = prev + (lane ? before : 0);
+    if (q == 0) at[q] = min(at[q], a.ntok + 1);
+  }
+  const int have = n_free + s_warp[2][31];
+  int refused = 0;
+#pragma unroll
+  for (int e = 0; e < PLAN_EACH; ++e) {
+    const int b = tid * PLAN_EACH + e;
+    if (b < a.n) {
+      const int first = at[0], last = (int)min((long long)first + max(cnt[e], 0), (long long)a.ntok + 1);
+      const bool ends = cnt[e] < 0;
+      const bool fits = cnt[e] <= 0 || (len[e] >= 0 && ((((long long)len[e] + cnt[e] + (1 << a.pshift) - 1) >> a.pshift) <= a.width) && last <= a.ntok);
+      const bool granted = !ends && fits && (need[e] == 0 || at[1] + need[e] <= have);
+      s_tok[b] = min(first, a.ntok);
+      if (cnt[e] > 0 && first <= a.ntok && last > a.ntok) s_over = b;   // the first whose tokens there is no room for
+      s_need[b] = at[1];
+      s_back[b] = at[2];
+      if (blockIdx.x == 0) {
+        a.q_start[b] = min(first, a.ntok);
+        a.kv_len[b] = granted ? len[e] + cnt[e] : 0;
+        a.state_out[b] = ends ? 0 : granted && need[e] ? held[e] + need[e] : held[e];
+        refused += !granted && !ends;
+      }
+      if (b == a.n - 1) {
+        s_tok[a.n] = min(last, a.ntok);
+        s_need[a.n] = at[1] + need[e];
+        s_back[a.n] = at[2] + (ends ? held[e] : 0);
+        if (blockIdx.x == 0) a.q_start[a.n] = min(last, a.ntok);
+      }
+      at[0] = last;
+      at[1] += need[e];
+      at[2] += ends ? held[e] : 0;
+    }
+  }
+  refused = __reduce_add_sync(0xffffffffu, refused);
+  if (lane == 0) s_refused[warp] = refused;
+  __syncthreads();
+
+  // pages handed out: those of the requests that were granted are the first ones asked for. (What lies behind the last sum that fits was not granted.)
+  const int total = s_need[a.n];
+  int taken = total;
+  if (total > have) {                              // the last request whose sum still fits
+    int lo = 0, hi = a.n;                          // s_need[lo] <= have
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_need[mid] <= have) lo = mid; else hi = mid;
+    }
+    taken = s_need[lo];
+  }
+  taken = min(taken, s_need[s_over]);
+  const int left = have - taken;
+  const int step = gridDim.x * PLAN_THREADS, first = blockIdx.x * PLAN_THREADS + tid;
+  // the nth page of those that have come back, and the nth page handed out
+  auto returned = [&](int nth) {
+    const int b = last_at_most(s_back, a.n, nth);
+    return a.table[(size_t)b * a.width + (nth - s_back[b])];
+  };
+  auto page = [&](int nth) {
+    const int src = have - 1 - nth;
+    return src < n_free ? a.free_pages[src] : returned(src - n_free);
+  };
+  for (int i = first; i < taken; i += step) {
+    const int b = last_at_most(s_need, a.n, i);
+    a.table[(size_t)b * a.width + min(max(a.state[b], 0), a.width) + (i - s_need[b])] = page(i);
+  }
+  for (int i = n_free + first; i < min(left, a.npages); i += step) a.free_pages[i] = returned(i - n_free);
+  const int tokens = s_tok[a.n];
+  for (int t = first; t < a.ntok; t += step) {
+    int pos = -1, slot = -1, req = -1;
+    if (t < tokens) {
+      req = last_at_most(s_tok, a.n, t);
+      const int c = a.counts[req], l = a.lengths[req], h = min(max(a.state[req], 0), a.width), wants = s_need[req + 1] - s_need[req];
+      const bool room = l >= 0 && ((((long long)l + c + (1 << a.pshift) - 1) >> a.pshift) <= a.width) && (long long)s_tok[req] + c <= a.ntok;
+      if (room && (wants == 0 || s_need[req + 1] <= have)) {
+        pos = l + (t - s_tok[req]);
+        const int nth = pos >> a.pshift;
+        const int pg = nth < h ? a.table[(size_t)req * a.width + nth] : page(s_need[req] + nth - h);
+        slot = (pg << a.pshift) + (pos & ((1 << a.pshift) - 1));
+      }
+    }
+    a.positions[t] = pos;
+    a.seq_ids[t] = req;
+    a.slots[t] = slot;
+  }
+  if (blockIdx.x == 0 && warp == 0) {
+    const int r = __reduce_add_sync(0xffffffffu, s_refused[lane]);
+    if (lane == 0) {
+      a.state_out[a.n] = left;
+      a.state_out[a.n + 1] = r;
+    }
+  }
+}
+
+// ---- rows into pages --------------------------------------------------------------------------------------------------------------
+// One warp per run and head, keys and values each: the consecutive tokens of one page. Eight lanes a row, four rows at a time; a lane holds sixteen of its
+// values, eight of each half, so that it has both of every pair that the rotation turns. Two walks over the rows, the second from L1: the page's scale is
+// the largest |x| of all of them. No barrier, no shared memory: a decode step's call is one load, a reduction and a store long.
+// Rotation and codes are evaluated with the roundings that their formulas have (no fused multiply-adds), so that the same codes come out of every
+// implementation in float32.
+struct AppendArgs {
+  const void* qkv; long long ld;
+  const void* cos_sin; int cos_rows;
+  const int *positions, *slots;
+  signed char *k, *v;
+  float *ks, *vs;
+  void* q; long long q_ts;
+  int ntok, H, G, npages, pshift, block;          // block: tokens of a CTA
+};
+constexpr float SCALE_FLOOR = 8.673617379884035e-19f;   // 2^-60
+constexpr int APPEND_WARPS = 8;
+
+// the slot of token t, or -1 if nothing is to be written for it
+__device__ __forceinline__ int slot_of(const AppendArgs& a, int t) {
+  if (t < 0 || t >= a.ntok) return -1;
+  const int s = a.slots[t], p = a.positions[t];
+  return s >= 0 && s < (a.npages << a.pshift) && p >= 0 && p < a.cos_rows ? s : -1;
+}
+
+// sixteen values of a row: x[0 .. 7] from column 8 c on, x[8 .. 15] the same of the second half
+template <bool BF16, int D, bool TURN>
+__device__ __forceinline__ void load_row(const AppendArgs& a, int t, int col, int c, float (&x)[16]) {
+  using T = typename Elem16<BF16>::T;
+  const T* row = (const T*)a.qkv + (size_t)t * a.ld + col + c * 8;
+  float lo[8], hi[8];
+  unpack8<BF16>(*reinterpret_cast<const uint4*>(row), lo);
+  unpack8<BF16>(*reinterpret_cast<const uint4*>(row + D / 2), hi);
+  if (TURN) {
+    const T* tab = (const T*)a.cos_sin + (size_t)a.positions[t] * D + c * 8;
+    float cs[8], sn[8];
+    unpack8<BF16>(*reinterpret_cast<const uint4*>(tab), cs);
+    unpack8<BF16>(*reinterpret_cast<const uint4*>(tab + D / 2), sn);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = __fsub_rn(__fmul_rn(lo[e], cs[e]), __fmul_rn(hi[e], sn[e]));
+      x[e + 8] = __fadd_rn(__fmul_rn(hi[e], cs[e]), __fmul_rn(lo[e], sn[e]));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { x[e] = lo[e]; x[e + 8] = hi[e]; }
+  }
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, float inv) {
+  const float r = rintf(__fmul_rn(x, inv));
+  return (uint32_t)(x == x ? (int)fminf(fmaxf(r, -127.f), 127.f) : 0) & 0xffu;
+}
+
+template <bool BF16, int D, bool TURN>
+__device__ __forceinline__ void write_run(const AppendArgs& a, int t0, int n, int slot, int g, int col, signed char* codes, float* scales) {
+  constexpr int LANES = D / 16, ROWS = 32 / LANES;          // lanes of a row, rows at a time
+  const int lane = threadIdx.x & 31, c = lane % LANES, r0 = lane / LANES;
+  const int page = slot >> a.pshift, first = slot & ((1 << a.pshift) - 1);
+  signed char* rows = codes + (((size_t)page * a.G + g) << a.pshift) * D;
+  float* scale = scales + (size_t)page * a.G + g;
+  const float before = first ? *scale : 0.f;
+  float mx = 0.f;
+  for (int r = r0; r < n; r += ROWS) {
+    float x[16];
+    load_row<BF16, D, TURN>(a, t0 + r, col, c, x);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float y = fabsf(x[e]);
+      mx = fmaxf(mx, y < INFINITY ? y : 0.f);               // (what is not finite does not stretch the page's scale)
+    }
+  }
+  mx = warp_xor_max(mx);
+  const float after = fmaxf(fmaxf(__fmul_rn(mx, 1.0f / 127.0f), before), SCALE_FLOOR);
+  const float inv = __frcp_rn(after);
+  for (int r = r0; r < n; r += ROWS) {
+    float x[16];
+    load_row<BF16, D, TURN>(a, t0 + r, col, c, x);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e >> 2] |= code_of(x[e], inv) << (8 * (e & 3));
+    signed char* to = rows + (size_t)(first + r) * D + c * 8;
+    *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(to + D / 2) = make_uint2(w[2], w[3]);
+  }
+  if (first && after > before) {                            // the older rows onto the new scale
+    const float f = __fdiv_rn(before, after);
+    for (int i = lane; i < first * (D / 16); i += 32) {
+      uint4* at = reinterpret_cast<uint4*>(rows) + i;
+      uint4 v = *at;
+      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t o = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o |= ((uint32_t)(int)rintf(__fmul_rn((float)(signed char)(w[q] >> (8 * e)), f)) & 0xffu) << (8 * e);
+        w[q] = o;
+      }
+      *at = v;
+    }
+  }
+  __syncwarp();                                             // every lane has read the scale
+  if (lane == 0 && after != before) *scale = after;
+}
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(APPEND_WARPS * 32) kv8_append_kernel(const AppendArgs a) {
+  using T = typename Elem16<BF16>::T;
+  constexpr int LANES = D / 16, ROWS = 32 / LANES;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int t0 = blockIdx.x * a.block, t1 = min(t0 + a.block, a.ntok);
+  const int units = (2 * a.G + APPEND_WARPS - 1) / APPEND_WARPS;    // CTAs in y that write pages; the others turn queries
+  pdl_enter();
+  if ((int)blockIdx.y < units) {
+    const int u = blockIdx.y * APPEND_WARPS + warp;
+    if (u >= 2 * a.G) return;
+    const int g = u >> 1;
+    const int mask = (1 << a.pshift) - 1;
+    for (int t = t0; t < t1; ++t) {
+      const int s = slot_of(a, t);
+      if (s < 0 || ((s & mask) && slot_of(a, t - 1) == s - 1)) continue;   // no row, or inside a run
+      int n = 0;                                            // the run's tokens: up to the end of the page
+      const int most = mask + 1 - (s & mask);
+      for (; n < most; n += 32) {
+        const bool in = n + lane < most && slot_of(a, t + n + lane) == s + n + lane;
+        const uint32_t out = ~__ballot_sync(0xffffffffu, in);
+        if (out) { n += __ffs(out) - 1; break; }
+      }
+      n = min(n, most);
+      if (u & 1) write_run<BF16, D, false>(a, t, n, s, g, (a.H + a.G + g) * D, a.v, a.vs);
+      else write_run<BF16, D, true>(a, t, n, s, g, (a.H + g) * D, a.k, a.ks);
+    }
+  } else {
+    const int c = lane % LANES, rows = (t1 - t0) * a.H, per = APPEND_WARPS * ROWS;
+    for (int r = ((int)blockIdx.y - units) * per + warp * ROWS + lane / LANES; r < rows; r += ((int)gridDim.y - units) * per) {
+      const int t = t0 + r / a.H, h = r % a.H;
+      const int p = a.positions[t];
+      if (p < 0 || p >= a.cos_rows) continue;
+      float x[16];
+      load_row<BF16, D, true>(a, t, h * D, c, x);
+      float lo[8], hi[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { lo[e] = x[e]; hi[e] = x[e + 8]; }
+      T* to = (T*)a.q + (size_t)t * a.q_ts + h * D + c * 8;
+      *reinterpret_cast<uint4*>(to) = pack8<BF16>(lo);
+      *reinterpret_cast<uint4*>(to + D / 2) = pack8<BF16>(hi);
+    }
+  }
+}
+
+// ---- rows back in 16 bits: out[i, g] = codes of slot i * their page's scale, keys and values. Eight values a thread; slots that are none give zeros.
+template <bool BF16>
+__global__ void __launch_bounds__(256) kv8_read_kernel(const signed char* k, const signed char* v, const float* ks, const float* vs, const int* slots, void* ko, void* vo,
+                                                       unsigned chunks, int G, int dshift, int npages, int pshift) {
+  using T = typename Elem16<BF16>::T;
+  pdl_enter();
+  const signed char* codes = blockIdx.y ? v : k;
+  const float* scales = blockIdx.y ? vs : ks;
+  T* out = (T*)(blockIdx.y ? vo : ko);
+  for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < chunks; i += gridDim.x * 256) {
+    const unsigned c = i & ((1u << (dshift - 3)) - 1u), row = i >> (dshift - 3);
+    const int g = (int)(row % (unsigned)G);
+    const int s = slots[row / (unsigned)G];
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (s >= 0 && s < npages << pshift) {
+      const int page = s >> pshift, r = s & ((1 << pshift) - 1);
+      const uint2 w = *reinterpret_cast<const uint2*>(codes + (((((size_t)page * G + g) << pshift) + r) << dshift) + c * 8);
+      const float f = scales[(size_t)page * G + g];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)(signed char)((e < 4 ? w.x : w.y) >> (8 * (e & 3))), f);
+    }
+    *reinterpret_cast<uint4*>(out + (size_t)i * 8) = pack8<BF16>(x);
+  }
+}
+
+}  // namespace kv8
+}  // namespace qspec
+
+using namespace qspec;
+using namespace qspec::kv8;
+
+extern "C" int qspec_page_plan(const int* lengths, const int* counts, int* table, int* free_pages, const int* state, int requests, int width, int npages, int page_tokens,
+                               int ntok, int* q_start, int* kv_len, int* positions, int* seq_ids, int* slots, int* state_out, void* stream) {
+  QSPEC_REQUIRE(lengths && counts && table && free_pages && state && q_start && kv_len && state_out && (ntok == 0 || (positions && seq_ids && slots)), QSPEC_ERR_INVALID_ARG,
+                "page_plan: null pointer");
+  QSPEC_REQUIRE(requests >= 1 && requests <= PLAN_REQUESTS, QSPEC_ERR_UNSUPPORTED, "page_plan: 1 to %d requests, got %d", PLAN_REQUESTS, requests);
+  QSPEC_REQUIRE(page_shift(page_tokens) > 0, QSPEC_ERR_UNSUPPORTED, "page_plan: pages of 16, 32, 64 or 128 tokens, got %d", page_tokens);
+  QSPEC_REQUIRE(width >= 1 && width <= (1 << 18) && npages >= 1 && (long long)npages * page_tokens < (1ll << 31) && ntok >= 0 && ntok < (1 << 30), QSPEC_ERR_INVALID_ARG,
+                "page_plan: width=%d pages=%d tokens=%d", width, npages, ntok);
+  PlanArgs a{lengths, counts, table, free_pages, state, q_start, kv_len, positions, seq_ids, slots, state_out, requests, width, npages, page_shift(page_tokens), ntok};
+  const size_t smem = 3 * (size_t)(requests + 1) * sizeof(int);
+  static SmemLimit limit;
+  if (smem > 40000) QSPEC_CUDA(limit.raise(page_plan_kernel, smem));
+  const int grid = min(max((ntok + PLAN_THREADS - 1) / PLAN_THREADS, 1), max(sm_count(), 1));
+  QSPEC_CUDA(launch_pdl(page_plan_kernel, dim3(grid), dim3(PLAN_THREADS), smem, (cudaStream_t)stream, a));
+  QSPEC_CHECK_LAUNCH(1);
+  return QSPEC_OK;
+}
+
+static int check_cache(const char* who, const void* k, const void* v, const float* ks, const float* vs, int npages, int G, int page_tokens, int D) {
+  QSPEC_REQUIRE(k && v && ks && vs, QSPEC_ERR_INVALID_ARG, "%s: null pointer", who);
+  QSPEC_REQUIRE(page_shift(page_tokens) > 0, QSPEC_ERR_UNSUPPORTED, "%s: pages of 16, 32, 64 or 128 tokens, got %d", who, page_tokens);
+  QSPEC_REQUIRE(D == 64 || D == 128, QSPEC_ERR_UNSUPPORTED, "%s: heads of 64 or 128, got %d", who, D);
+  QSPEC_REQUIRE(npages >= 1 && G >= 1 && G <= 1024 && (long long)npages * page_tokens < (1ll << 31), QSPEC_ERR_INVALID_ARG, "%s: pages=%d kv heads=%d", who, npages, G);
+  QSPEC_REQUIRE(((uintptr_t)k & 15) == 0 && ((uintptr_t)v & 15) == 0, QSPEC_ERR_INVALID_ARG, "%s: codes must begin on a 16-byte boundary", who);
+  return QSPEC_OK;
+}
+
+extern "C" int qspec_kv8_append(const void* qkv, long long ld, const void* cos_sin, int cos_rows, const int* positions, const int* slots, void* k, void* v, float* ks,
+                                float* vs, void* q_out, long long q_tok_stride, int ntok, int H, int G, int D, int npages, int page_tokens, int dtype, void* stream) {
+  if (int rc = check_cache("kv8_append", k, v, ks, vs, npages, G, page_tokens, D)) return rc;
+  if (ntok == 0) return QSPEC_OK;
+  QSPEC_REQUIRE(qkv && cos_sin && positions && slots, QSPEC_ERR_INVALID_ARG, "kv8_append: null pointer");
+  QSPEC_REQUIRE(dtype == QSPEC_DTYPE_F16 || dtype == QSPEC_DTYPE_BF16, QSPEC_ERR_UNSUPPORTED, "kv8_append: float16 or bfloat16 rows");
+  QSPEC_REQUIRE(ntok > 0 && ntok < (1 << 30) && H >= 1 && H <= 4096 && cos_rows >= 1, QSPEC_ERR_INVALID_ARG, "kv8_append: tokens=%d heads=%d table rows=%d", ntok, H, cos_rows);
+  QSPEC_REQUIRE(ld >= (long long)(H + 2 * G) * D && ld % 8 == 0 && (!q_out || (q_tok_stride >= (long long)H * D && q_tok_stride % 8 == 0)) && ((uintptr_t)qkv & 15) == 0 &&
+                    ((uintptr_t)cos_sin & 15) == 0 && ((uintptr_t)q_out & 15) == 0,
+                QSPEC_ERR_INVALID_ARG, "kv8_append: rows must lie on 16-byte boundaries (ld=%lld)", ld);
+  AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (signed char*)k, (signed char*)v, ks, vs, q_out, q_tok_stride, ntok, H, G, npages, page_shift(page_tokens), 1};
+  // A CTA looks at one token where there are few (each is likely to begin a run) and at eight of a prompt's, most of which are inside one.
+  a.block = ntok <= 512 ? 1 : 8;
+  const int rows = APPEND_WARPS * 32 * 16 / D;              // query rows that a CTA takes at a time
+  const int y = (2 * G + APPEND_WARPS - 1) / APPEND_WARPS + (q_out ? (a.block * H + 2 * rows - 1) / (2 * rows) : 0);
+  const dim3 grid((ntok + a.block - 1) / a.block, y);
+  auto kern = dtype == QSPEC_DTYPE_F16 ? (D == 128 ? kv8_append_kernel<false, 128> : kv8_append_kernel<false, 64>)
+                                       : (D == 128 ? kv8_append_kernel<true, 128> : kv8_append_kernel<true, 64>);
+  QSPEC_CUDA(launch_pdl(kern, grid, dim3(APPEND_WARPS * 32), 0, (cudaStream_t)stream, a));
+  QSPEC_CHECK_LAUNCH(1);
+  return QSPEC_OK;
+}
+
+extern "C" int qspec_kv8_read(const void* k, const void* v, const float* ks, const float* vs, const int* slots, void* k_out, void* v_out, int rows, int G, int D, int npages,
+                              int page_tokens, int dtype, void* stream) {
+  if (int rc = check_cache("kv8_read", k, v, ks, vs, npages, G, page_tokens, D)) return rc;
+  if (rows == 0) return QSPEC_OK;
+  QSPEC_REQUIRE(rows > 0 && slots && k_out && v_out, QSPEC_ERR_INVALID_ARG, "kv8_read: null pointer or rows=%d", rows);
+  QSPEC_REQUIRE(dtype == QSPEC_DTYPE_F16 || dtype == QSPEC_DTYPE_BF16, QSPEC_ERR_UNSUPPORTED, "kv8_read: float16 or bfloat16 rows");
+  QSPEC_REQUIRE(((uintptr_t)k_out & 15) == 0 && ((uintptr_t)v_out & 15) == 0, QSPEC_ERR_INVALID_ARG, "kv8_read: rows must lie on 16-byte boundaries");
+  const long long chunks = (long long)rows * G * (D / 8);
+  QSPEC_REQUIRE(chunks < (1ll << 31), QSPEC_ERR_UNSUPPORTED, "kv8_read: %d rows are too many for one call", rows);
+  const int grid = (int)std::min<long long>((chunks + 255) / 256, (long long)max(sm_count(), 1) * 8);
+  auto kern = dtype == QSPEC_DTYPE_F16 ? kv8_read_kernel<false> : kv8_read_kernel<true>;
+  QSPEC_CUDA(launch_pdl(kern, dim3(grid, 2), dim3(256), 0, (cudaStream_t)stream, (const signed char*)k, (const signed char*)v, ks, vs, slots, k_out, v_out, (unsigned)chunks, G,
+                        D == 128 ? 7 : 6, npages, page_shift(page_tokens)));
+  QSPEC_CHECK_LAUNCH(1);
+  return QSPEC_OK;
+}

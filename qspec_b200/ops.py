@@ -785,6 +785,197 @@ def argmax_rows(logits: torch.Tensor, out_val: Optional[torch.Tensor] = None) ->
     return out
 
 
+# ---------------------------------------------------------------------------------------------
+# speculative decoding over a cache in pages and in 8 bits: page plan, writer and reader of the cache, attention, verification of drafts
+# ---------------------------------------------------------------------------------------------
+
+_PAGE_TOKENS = (16, 32, 64, 128)
+
+
+def _here(*tensors: Optional[torch.Tensor]) -> None:
+    """All on the current device, whose current stream the call goes to."""
+    device = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"a tensor lies on {t.device}, the call goes to the current device, cuda:{device}")
+
+
+def _i32(t: torch.Tensor, name: str, *shape: int) -> None:
+    _chk(t, name, (torch.int32,))
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
+def page_plan(lengths: torch.Tensor, counts: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, state: torch.Tensor, page_tokens: int,
+              q_start: torch.Tensor, kv_len: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor, slots: torch.Tensor, state_out: torch.Tensor) -> None:
+    """The pages and slots of a step from lengths that lie on the device (all tensors int32). lengths [B]: tokens held; counts [B]: tokens that come with
+    the step, negative for a request that has ended. table [B, W], free_pages [pages] and state [B + 1] (pages held by each request, number of free
+    pages) describe the cache; q_start [B + 1], kv_len [B], positions / seq_ids / slots [tokens] and state_out [B + 2] (the state behind the step, number
+    of requests refused) are written. `state` and what it describes stay as they are until the caller copies state_out over it, so that a
+    step can be planned again. Who gets which pages, and who none: include/qspec_b200.h."""
+    if lengths.dim() != 1 or table.dim() != 2 or free_pages.dim() != 1 or positions.dim() != 1:
+        raise ValueError("page_plan: lengths [B], table [B, W], free_pages [pages], positions [tokens]")
+    B, T = lengths.shape[0], positions.shape[0]
+    _i32(lengths, "lengths", B); _i32(counts, "counts", B); _i32(table, "table", B, table.shape[1]); _i32(free_pages, "free_pages", free_pages.shape[0])
+    _i32(state, "state", B + 1); _i32(q_start, "q_start", B + 1); _i32(kv_len, "kv_len", B); _i32(positions, "positions", T)
+    _i32(seq_ids, "seq_ids", T); _i32(slots, "slots", T); _i32(state_out, "state_out", B + 2)
+    _here(lengths, counts, table, free_pages, state, q_start, kv_len, positions, seq_ids, slots, state_out)
+    if _overlap(state, state_out) or _overlap(lengths, kv_len):
+        raise ValueError("page_plan: state_out and kv_len must not lie over state and lengths (every CTA reads those)")
+    lib = _lib.load()
+    _lib.check(lib.qspec_page_plan(_ptr(lengths), _ptr(counts), _ptr(table), _ptr(free_pages), _ptr(state), B, table.shape[1], free_pages.shape[0], page_tokens, T,
+                                   _ptr(q_start), _ptr(kv_len), _ptr(positions), _ptr(seq_ids), _ptr(slots), _ptr(state_out), _stream()), "page_plan")
+
+
+def _kv8_cache(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
+    _chk(k_codes, "k_codes", (torch.int8,)); _chk(v_codes, "v_codes", (torch.int8,))
+    _chk(k_scale, "k_scale", (torch.float32,)); _chk(v_scale, "v_scale", (torch.float32,))
+    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
+        raise ValueError(f"codes must be [pages, kv heads, page tokens, head dim], keys and values alike: {tuple(k_codes.shape)}, {tuple(v_codes.shape)}")
+    if k_scale.shape != k_codes.shape[:2] or v_scale.shape != k_codes.shape[:2]:
+        raise ValueError(f"scales must be [pages, kv heads]: {tuple(k_scale.shape)}, {tuple(v_scale.shape)}")
+    return k_codes.shape
+
+
+def kv8_append(qkv: torch.Tensor, cos_sin_cache: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
+               k_scale: torch.Tensor, v_scale: torch.Tensor, q_out: Optional[torch.Tensor]) -> None:
+    """Neox RoPE on queries and keys of qkv [T, (H + 2 G) D] (float16 / bfloat16; rows may be strided, left as they are) and the step's keys and values
+    into the pages of their slots: codes int8 [pages, G, P, D], scales float32 [pages, G]. q_out [T, H, D] receives the rotated queries (None: they
+    are not wanted). A page's scale grows with its rows and its older rows follow; it starts anew when its first row is written. Tokens without
+    a slot (negative) are skipped. The tokens of a page must be neighbours in the batch."""
+    n, G, P, D = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
+    if not qkv.is_cuda or qkv.dtype not in (_F16, _BF16) or qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise ValueError("kv8_append: qkv must be a float16 / bfloat16 CUDA tensor [T, (H + 2 G) D] with unit column stride")
+    T = qkv.shape[0]
+    H = qkv.shape[1] // D - 2 * G
+    if qkv.shape[1] % D or H < 1:
+        raise ValueError(f"kv8_append: rows of {qkv.shape[1]} do not hold queries, {G} keys and {G} values of {D}")
+    _chk(cos_sin_cache, "cos_sin_cache", (qkv.dtype,))
+    if cos_sin_cache.dim() != 2 or cos_sin_cache.shape[1] != D:
+        raise ValueError(f"kv8_append: the rotary table must be [positions, {D}]")
+    _i32(positions, "positions", T); _i32(slots, "slots", T)
+    q_ts = 0
+    if q_out is not None:
+        if not q_out.is_cuda or q_out.dtype != qkv.dtype or q_out.shape != (T, H, D) or q_out.stride(2) != 1 or q_out.stride(1) != D:
+            raise ValueError(f"kv8_append: q_out must be {qkv.dtype} [{T}, {H}, {D}], heads side by side")
+        q_ts = q_out.stride(0)
+    _here(qkv, cos_sin_cache, positions, slots, k_codes, v_codes, k_scale, v_scale, q_out)
+    lib = _lib.load()
+    _lib.check(lib.qspec_kv8_append(_ptr(qkv), qkv.stride(0), _ptr(cos_sin_cache), cos_sin_cache.shape[0], _ptr(positions), _ptr(slots), _ptr(k_codes), _ptr(v_codes),
+                                    _ptr(k_scale), _ptr(v_scale), _ptr(q_out), q_ts, T, H, G, D, n, P, _dt(qkv), _stream()), "kv8_append")
+
+
+def kv8_read(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor,
+             v_out: torch.Tensor) -> None:
+    """Rows of the 8-bit cache as 16-bit values: k_out, v_out [N, G, D] (float16 / bfloat16) of slots int32 [N]; zeros for a slot outside the cache."""
+    n, G, P, D = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
+    _chk(k_out, "k_out", (_F16, _BF16)); _chk(v_out, "v_out", (k_out.dtype,))
+    _i32(slots, "slots", slots.numel())
+    if k_out.shape != (slots.numel(), G, D) or v_out.shape != k_out.shape:
+        raise ValueError(f"kv8_read: outputs must be [{slots.numel()}, {G}, {D}]")
+    _here(k_codes, v_codes, k_scale, v_scale, slots, k_out, v_out)
+    lib = _lib.load()
+    _lib.check(lib.qspec_kv8_read(_ptr(k_codes), _ptr(v_codes), _ptr(k_scale), _ptr(v_scale), _ptr(slots), _ptr(k_out), _ptr(v_out), slots.numel(), G, D, n, P, _dt(k_out),
+                                  _stream()), "kv8_read")
+
+
+def kv8_attention_workspace(device) -> torch.Tensor:
+    """Workspace for `kv8_attention` calls that are made one after the other (a model's layers, a captured step). Calls that may run at the same
+    time, on two streams or in two graphs, need one each."""
+    device = torch.device(device)
+    with torch.cuda.device(device):
+        return torch.zeros(_lib.load().qspec_kv8_attention_workspace_bytes(), dtype=torch.uint8, device=device)
+
+
+def kv8_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, table: torch.Tensor,
+                  q_start: torch.Tensor, kv_len: torch.Tensor, out: torch.Tensor, sm_scale: float, workspace: torch.Tensor,
+                  max_tokens: Optional[int] = None) -> torch.Tensor:
+    """Softmax attention of a step's tokens q [T, H, D] (float16 / bfloat16; token and head strides free) over the 8-bit cache: tokens q_start[b] ..
+    q_start[b + 1] - 1 are request b's last of kv_len[b], and see its keys up to their own. table int32 [B, W]. out [T, H, D] of q's type; rows that see no
+    key are zeros, rows behind q_start[B] are left as they are. max_tokens: an upper bound of the tokens that a request has in the step (T if not
+    given); a request with more than that is not attended to. workspace: `kv8_attention_workspace`."""
+    n, G, P, D = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
+    for t, name in ((q, "q"), (out, "out")):
+        if not t.is_cuda or t.dtype not in (_F16, _BF16) or t.dim() != 3 or t.shape[2] != D or t.stride(2) != 1:
+            raise ValueError(f"kv8_attention: {name} must be a float16 / bfloat16 CUDA tensor [T, H, {D}] with unit stride in a head")
+    T, H = q.shape[0], q.shape[1]
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("kv8_attention: out must have the shape and type of q")
+    if table.dim() != 2:
+        raise ValueError("kv8_attention: table must be [requests, pages of a request]")
+    B, W = table.shape
+    _i32(table, "table", B, W); _i32(q_start, "q_start", B + 1); _i32(kv_len, "kv_len", B)
+    _chk(workspace, "workspace", (torch.uint8,))
+    if not sm_scale > 0:
+        raise ValueError(f"kv8_attention: scale must be positive, got {sm_scale}")
+    if T == 0:
+        return out
+    _here(q, k_codes, v_codes, k_scale, v_scale, table, q_start, kv_len, out, workspace)
+    if max_tokens is None:
+        max_tokens = T
+    lib = _lib.load()
+    _lib.check(lib.qspec_kv8_attention(_ptr(q), q.stride(0), q.stride(1), _ptr(k_codes), _ptr(v_codes), _ptr(k_scale), _ptr(v_scale), _ptr(table), _ptr(q_start), _ptr(kv_len),
+                                       _ptr(out), out.stride(0), out.stride(1), T, B, W, H, G, D, n, P, min(max_tokens, T), float(sm_scale), _dt(q), _ptr(workspace),
+                                       workspace.numel(), _stream()), "kv8_attention")
+    return out
+
+
+def _probs(t: torch.Tensor, name: str, *shape: int) -> None:
+    if not t.is_cuda or t.dtype != torch.float32 or t.shape != shape or (t.stride(2) != 1 and shape[2] > 1):
+        raise ValueError(f"{name} must be a float32 CUDA tensor {shape} with unit stride over the vocabulary")
+
+
+def verify_drafts(drafted: Optional[torch.Tensor], draft_probs: Optional[torch.Tensor], target_probs: torch.Tensor, uniform: torch.Tensor, tokens: torch.Tensor,
+                  emitted: torch.Tensor, draft_counts: Optional[torch.Tensor] = None) -> None:
+    """Verification of drafted tokens [B, k] (int64) that were drawn from draft_probs [B, k, V], against target_probs [B, k + 1, V] (float32, rows may be strided),
+    with random numbers uniform [B, k + 1] in [0, 1): tokens int64 [B, k + 1] receives what is emitted (-1 behind it), emitted int64 [B] how many. Draft i is taken
+    with probability min(1, p / q); behind the taken ones comes one token from what the target has over the draft, or from the target where all were
+    taken. draft_counts int32 [B]: how many of its k drafts each request has (None: all). drafted and draft_probs None: no drafts, one token is drawn from
+    every row of target_probs [B, 1, V]. (vllm/model_executor/layers/rejection_sampler.py)"""
+    if target_probs.dim() != 3:
+        raise ValueError("verify_drafts: target_probs must be [B, k + 1, V]")
+    B, k, V = target_probs.shape[0], target_probs.shape[1] - 1, target_probs.shape[2]
+    if k < 0 or V < 1:
+        raise ValueError("verify_drafts: target_probs must have a place behind the drafts, and a vocabulary")
+    _probs(target_probs, "target_probs", B, k + 1, V)
+    if k:
+        if drafted is None or draft_probs is None:
+            raise ValueError("verify_drafts: target_probs has places for drafts, but none are given")
+        _chk(drafted, "drafted", (torch.int64,))
+        _probs(draft_probs, "draft_probs", B, k, V)
+        if drafted.shape != (B, k):
+            raise ValueError(f"drafted: shape {tuple(drafted.shape)}, expected {(B, k)}")
+    elif drafted is not None or draft_probs is not None:
+        raise ValueError("verify_drafts: drafts are given, but target_probs has one place only")
+    _chk(uniform, "uniform", (torch.float32,)); _chk(tokens, "tokens", (torch.int64,)); _chk(emitted, "emitted", (torch.int64,))
+    if uniform.shape != (B, k + 1) or tokens.shape != (B, k + 1) or emitted.shape != (B,):
+        raise ValueError(f"verify_drafts: uniform and tokens must be {(B, k + 1)}, emitted {(B,)}")
+    if draft_counts is not None:
+        _i32(draft_counts, "draft_counts", B)
+    if B == 0:
+        return
+    _here(target_probs, drafted, draft_probs, uniform, tokens, emitted, draft_counts)
+    if k and _overlap(tokens, drafted):
+        raise ValueError("verify_drafts: tokens must not lie over drafted")
+    lib = _lib.load()
+    _lib.check(lib.qspec_verify_drafts(_ptr(drafted), _ptr(draft_probs), draft_probs.stride(0) if k else 0, draft_probs.stride(1) if k else 0, _ptr(target_probs),
+                                       target_probs.stride(0), target_probs.stride(1), _ptr(uniform), _ptr(draft_counts), _ptr(tokens), _ptr(emitted), B, k, V, _stream()),
+               "verify_drafts")
+
+
+def sample_probs(probs: torch.Tensor, uniform: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
+    """One token per row of the probabilities [rows, V] (float32; rows may be strided) by inversion with uniform [rows] in [0, 1): tokens int64 [rows] receives the
+    first whose running sum is above uniform * (sum of the row). The sampling counterpart of `argmax_rows`."""
+    if probs.dim() != 2 or uniform.shape != probs.shape[:1] or tokens.shape != probs.shape[:1]:
+        raise ValueError("sample_probs: probs [rows, V], uniform [rows], tokens [rows]")
+    verify_drafts(None, None, probs.unsqueeze(1), uniform.unsqueeze(1), tokens.unsqueeze(1), torch.empty_like(tokens))
+    return tokens
+
+
 def tp_argmax_combine(local_max: torch.Tensor, local_idx: torch.Tensor, index_offset: int, peers,
                       out: Optional[torch.Tensor] = None, phases: int = 3) -> torch.Tensor:
     """Greedy token over a vocab-sharded lm_head through peer memory (no collective call): every rank pushes its

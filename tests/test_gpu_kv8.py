@@ -1,0 +1,489 @@
+"""The paged 8-bit cache on the GPU: page plan, writer and reader, attention -- against loops and 64-bit sums."""
+import math
+
+import pytest
+import torch
+
+from qspec_b200 import ops
+
+pytestmark = pytest.mark.gpu
+I32, F32, F64 = torch.int32, torch.float32, torch.float64
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def i32(x):
+    return torch.as_tensor(x, dtype=I32).cuda()
+
+
+# ---- the page plan ------------------------------------------------------------------------------------------------------------------
+def plan_by_hand(lengths, counts, table, free, held, n_free, P, T):
+    """The plan of a step, request by request."""
+    B, W = len(lengths), len(table[0])
+    stack = list(free[:n_free])
+    for b in range(B):
+        if counts[b] < 0:
+            stack += table[b][:held[b]]
+    have, asked, start = len(stack), 0, 0
+    table, held_out, taken = [list(r) for r in table], [], 0
+    q_start, kv_len, pos, seq, slots, refused = [], [], [], [], [], 0
+    for b in range(B):
+        c = max(counts[b], 0)
+        q_start.append(min(start, T))
+        wants = -(-(lengths[b] + c) // P)
+        room = c == 0 or (wants <= W and start + c <= T)
+        need = max(wants - held[b], 0) if c and wants <= W else 0
+        asked += need
+        granted = counts[b] >= 0 and room and (need == 0 or asked <= have)
+        if granted:
+            for i in range(need):
+                table[b][held[b] + i] = stack[have - 1 - taken]
+                taken += 1
+        refused += counts[b] >= 0 and not granted
+        held_out.append(0 if counts[b] < 0 else held[b] + (need if granted else 0))
+        kv_len.append(lengths[b] + c if granted else 0)
+        for i in range(c):
+            if start + i < T:
+                p = lengths[b] + i
+                pos.append(p if granted else -1)
+                seq.append(b)
+                slots.append(table[b][p // P] * P + p % P if granted else -1)
+        start += c
+    q_start.append(min(start, T))
+    pad = T - len(pos)
+    left = have - taken
+    free = list(free)
+    for i in range(n_free, left):
+        free[i] = stack[i]
+    return q_start, kv_len, pos + [-1] * pad, seq + [-1] * pad, slots + [-1] * pad, held_out + [left, refused], table, free
+
+
+def run_plan(lengths, counts, table, free, held, n_free, P, T):
+    B = len(lengths)
+    state = i32(list(held) + [n_free])
+    t, f = i32(table), i32(free)
+    out = [torch.full((n,), -7, dtype=I32, device="cuda") for n in (B + 1, B, T, T, T, B + 2)]
+    kept = state.clone()
+    ops.page_plan(i32(lengths), i32(counts), t, f, state, P, out[0], out[1], out[2], out[3], out[4], out[5])
+    assert torch.equal(state, kept)
+    return [o.tolist() for o in out] + [t.tolist(), f.tolist()]
+
+
+def random_plan(B, P, seed, scarce, W=40, extra_T=3, most=5):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda lo, hi: int(torch.randint(lo, hi + 1, (1,), generator=g))  # noqa: E731
+    lengths = [r(0, (W - 2) * P) for _ in range(B)]
+    counts = [[-1, 0, 1, r(1, most), r(1, 2 * P)][r(0, 4)] for _ in range(B)]
+    held = [min(-(-n // P) + r(0, 1), W) for n in lengths]
+    pages = torch.randperm(sum(held) + B + 3 + r(0, 2 * B), generator=g).tolist()
+    table, at = [], 0
+    for b in range(B):
+        table.append(pages[at:at + held[b]] + [0] * (W - held[b]))
+        at += held[b]
+    n_free = min(B // 3 if scarce else len(pages) - at, len(pages) - at)
+    free = pages[at:at + n_free] + [0] * (len(pages) - n_free)
+    return lengths, counts, table, free, held, n_free, P, sum(max(c, 0) for c in counts) + extra_T
+
+
+@pytest.mark.parametrize("B,P,scarce", [(1, 16, False), (2, 64, True), (31, 32, False), (33, 128, True), (64, 64, True), (500, 16, True), (1025, 16, False), (4096, 32, True)])
+def test_page_plan_is_the_plan_made_by_hand(B, P, scarce):
+    for seed in range(3):
+        case = random_plan(B, P, seed, scarce)
+        assert run_plan(*case) == list(plan_by_hand(*case))
+
+
+def test_page_plan_again_gives_the_same_and_steps_follow_each_other():
+    lengths, counts, table, free, held, n_free, P, T = random_plan(40, 16, 5, False)
+    first = run_plan(lengths, counts, table, free, held, n_free, P, T)
+    again = run_plan(lengths, counts, first[6], first[7], held, n_free, P, T)
+    assert first == again                                     # what a plan writes does not belong to the state it came from
+    for step in range(6):                                     # every page is in one place, step after step
+        q_start, kv_len, pos, seq, slots, state, table, free = run_plan(lengths, counts, table, free, held, n_free, P, T)
+        held, n_free = state[:-2], state[-2]
+        at = [p for b in range(len(held)) for p in table[b][:held[b]]] + free[:n_free]
+        assert len(set(at)) == len(at) and set(at) <= set(range(len(free))) and state[-1] == 0
+        assert all(s == table[b][p // P] * P + p % P for p, b, s in zip(pos, seq, slots) if p >= 0)
+        lengths = [k if c >= 0 else 0 for k, c in zip(kv_len, counts)]
+        counts = [(3 * b + step) % 4 - (1 if (b + step) % 7 == 0 else 0) if n < 30 * P else -1 for b, n in enumerate(lengths)]
+        T = sum(max(c, 0) for c in counts) + 2
+
+
+def test_page_plan_refuses_what_does_not_fit():
+    # the row of the table, the step's tokens, the free pages -- and the next requests are served where they can be
+    case = ([60, 5, 0, 8], [10, 3, 4, 0], [[0, 1, 2, 3], [4, 0, 0, 0], [0] * 4, [5, 0, 0, 0]], [6, 7, 8, 9, 0, 0, 0, 0, 0, 0], [4, 1, 0, 1], 4, 16, 40)
+    got = run_plan(*case)
+    assert got == list(plan_by_hand(*case)) and got[5][-1] == 1 and got[1] == [0, 8, 4, 8]
+    case = case[:-1] + (14,)                                  # the third request's tokens do not fit into the step
+    got = run_plan(*case)
+    assert got == list(plan_by_hand(*case)) and got[5][-1] == 2 and got[0] == [0, 10, 13, 14, 14]
+    case = ([15, 0], [1, 40], [[0, 0, 0], [0, 0, 0]], [1, 2, 3], [1, 0], 2, 16, 41)
+    got = run_plan(*case)
+    assert got == list(plan_by_hand(*case)) and got[5] == [1, 0, 2, 1]
+
+
+# ---- the writer and the reader ------------------------------------------------------------------------------------------------------
+def rotated(x, cs, dtype):
+    a, b = x.chunk(2, -1)
+    cos, sin = cs[:, None].to(dtype).chunk(2, -1)
+    return torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
+
+
+def write_by_hand(x, slots, codes, scales, dtype=F32):
+    """Rows x [T, G, D] into a copy of codes / scales, one run of a page after the other, in `dtype`."""
+    codes, scales, P = codes.clone(), scales.clone(), codes.shape[2]
+    t = 0
+    while t < len(slots):
+        if slots[t] < 0:
+            t += 1
+            continue
+        n = 1
+        while t + n < len(slots) and slots[t + n] == slots[t] + n and slots[t + n] % P:
+            n += 1
+        page, first = slots[t] // P, slots[t] % P
+        rows = x[t:t + n].to(dtype)
+        amax = torch.where(rows.abs() < math.inf, rows.abs(), 0.0).amax((0, 2))
+        before = scales[page].to(dtype) if first else torch.zeros_like(amax)
+        after = torch.maximum(torch.maximum(amax * torch.tensor(1.0 / 127.0, dtype=dtype, device=x.device), before), torch.tensor(2.0 ** -60, dtype=dtype, device=x.device))
+        if first:
+            codes[page, :, :first] = (codes[page, :, :first].to(dtype) * (before / after)[:, None, None]).round().to(torch.int8)
+        q = (rows * after.reciprocal()[None, :, None]).round().clamp(-127, 127)
+        codes[page, :, first:first + n] = torch.where(rows == rows, q, 0.0).to(torch.int8).transpose(0, 1)
+        scales[page] = after.to(scales.dtype)
+        t += n
+    return codes, scales
+
+
+def make_append(seed, runs, H, G, D, P, dtype, pages=40, spoil=False):
+    """runs: (first position, tokens) of each request; pages are handed out at random."""
+    g = gen(seed)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    pos, slots = [], []
+    for first, n in runs:
+        table = [order.pop() for _ in range(-(-(first + n) // P) - first // P)]
+        for p in range(first, first + n):
+            pos.append(p)
+            slots.append(table[p // P - first // P] * P + p % P)
+    T = len(pos)
+    qkv = torch.randn(T, (H + 2 * G) * D, generator=g, device="cuda").to(dtype)
+    if spoil:
+        qkv.view(-1)[::997] = math.inf
+        qkv.view(-1)[5::1499] = -math.inf
+        qkv.view(-1)[7::1201] = math.nan
+    angle = torch.rand(max(pos) + 1, D // 2, generator=g, device="cuda") * 6.28
+    cs = torch.cat((angle.cos(), angle.sin()), -1).to(dtype)
+    codes = [torch.randint(-127, 128, (pages, G, P, D), generator=g, device="cuda").to(torch.int8) for _ in range(2)]
+    scales = [2.0 ** (torch.rand(pages, G, generator=g, device="cuda") * 4 - 7.5) for _ in range(2)]
+    return qkv, cs, pos, slots, codes, scales
+
+
+RUNS = {"one": [(0, 1)], "decode": [(5, 1), (63, 1), (64, 1), (200, 1)], "verify": [(62, 4), (15, 5), (0, 3), (31, 4), (127, 2)], "prompts": [(0, 300), (100, 70), (17, 1), (48, 16)]}
+
+
+@pytest.mark.parametrize("D,P,H,G,dtype", [(128, 64, 8, 2, torch.float16), (128, 16, 4, 4, torch.bfloat16), (64, 32, 5, 1, torch.float16), (64, 128, 6, 3, torch.bfloat16)])
+@pytest.mark.parametrize("runs", list(RUNS))
+@pytest.mark.parametrize("spoil", [False, True])
+def test_append_gives_the_codes_of_its_formulas(runs, D, P, H, G, dtype, spoil):
+    qkv, cs, pos, slots, codes, scales = make_append(3, RUNS[runs], H, G, D, P, dtype, spoil=spoil)
+    T = len(pos)
+    x = qkv.float().view(T, H + 2 * G, D)
+    turned = rotated(x[:, :H + G], cs[torch.tensor(pos, device="cuda")].float(), F32)
+    want = [write_by_hand(y, slots, c, s) for y, c, s in ((turned[:, H:], codes[0], scales[0]), (x[:, H + G:], codes[1], scales[1]))]
+    k, v, ks, vs = codes[0].clone(), codes[1].clone(), scales[0].clone(), scales[1].clone()
+    q = torch.empty(T, H, D, dtype=dtype, device="cuda")
+    kept = qkv.clone()
+    ops.kv8_append(qkv, cs, i32(pos), i32(slots), k, v, ks, vs, q)
+    assert torch.equal(qkv.nan_to_num(), kept.nan_to_num())
+    torch.testing.assert_close(q, turned[:, :H].to(dtype), rtol=0, atol=0, equal_nan=True)
+    # float32 formulas, each operation rounded: the same bits (rows behind a page's last are no one's)
+    assert torch.equal(ks, want[0][1]) and torch.equal(vs, want[1][1])
+    assert torch.equal(k, want[0][0]) and torch.equal(v, want[1][0])
+    # the reader: code times scale, rounded once; none for slots outside
+    asked = slots + [-1, 40 * P]
+    ko, vo = (torch.empty(len(asked), G, D, dtype=dtype, device="cuda") for _ in range(2))
+    ops.kv8_read(k, v, ks, vs, i32(asked), ko, vo)
+    at = torch.tensor(slots, device="cuda")
+    for got, c, s in ((ko, k, ks), (vo, v, vs)):
+        assert torch.equal(got[:T], (c[at // P, :, at % P].float() * s[at // P][:, :, None]).to(dtype)) and not got[T:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_what_the_cache_holds_is_near_what_was_written(dtype):
+    """Against 64 bits: a code is off by half a step of the scale it was made with (and the rounding of x / scale: 127 * 2^-22 of a step at most), and by
+    half a step more each time that the page's scale has grown since."""
+    H, G, D, P, n = 2, 2, 128, 32, 75
+    g = gen(8)
+    qkv = (torch.randn(n, (H + 2 * G) * D, generator=g, device="cuda") * torch.linspace(0.2, 3, n, device="cuda")[:, None]).to(dtype)
+    angle = torch.rand(n, D // 2, generator=g, device="cuda")
+    cs = torch.cat((angle.cos(), angle.sin()), -1).to(dtype)
+    k, v = (torch.zeros(4, G, P, D, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros(4, G, device="cuda") for _ in range(2))
+    grown = torch.zeros(4, G, 2, device="cuda")
+    begin = 0
+    while begin < n:                                          # 1, 2, 3, 1, 2, .. tokens at a time
+        m = min(begin % 3 + 1, n - begin)
+        was = torch.stack([ks, vs], -1)
+        pos = torch.arange(begin, begin + m)
+        ops.kv8_append(qkv[begin:begin + m], cs, i32(pos), i32(pos), k, v, ks, vs, None)
+        grown += (torch.stack([ks, vs], -1) > was).float()
+        begin += m
+    x = qkv.to(F64).view(n, H + 2 * G, D)
+    want = [rotated(x[:, H:H + G], cs.to(F64), F64), x[:, H + G:]]
+    for i, (c, s) in enumerate(((k, ks), (v, vs))):
+        at = torch.arange(n, device="cuda")
+        got = c[at // P, :, at % P].to(F64) * s[at // P][:, :, None].to(F64)
+        step = s[at // P][:, :, None].to(F64)
+        often = grown[at // P][:, :, i, None].to(F64)
+        # (rotation in float32: three roundings of values up to |a| + |b| <= 2 * 127 steps)
+        assert ((got - want[i]).abs() <= step * (0.5 * often + 127 * 2.0 ** -22 + 4 * 127 * 3 * 2.0 ** -24)).all()
+
+
+def test_append_skips_tokens_without_a_place_and_leaves_the_rest():
+    H, G, D, P = 4, 2, 128, 32
+    qkv, cs, pos, slots, codes, scales = make_append(4, [(10, 4), (40, 3)], H, G, D, P, torch.float16)
+    pos2, slots2 = list(pos), list(slots)
+    slots2[3] = -1                                            # no slot (the last of its run: a page's tokens are neighbours, in consecutive rows)
+    pos2[4] = len(cs)                                         # a position that the table of angles does not have
+    slots2[6] = 40 * P                                        # a slot behind the cache
+    k, v, ks, vs = codes[0].clone(), codes[1].clone(), scales[0].clone(), scales[1].clone()
+    q = torch.full((7, H, D), 9.0, dtype=torch.float16, device="cuda")
+    ops.kv8_append(qkv, cs, i32(pos2), i32(slots2), k, v, ks, vs, q)
+    assert (q[4] == 9).all() and not (q[3] == 9).all()        # (queries go by their position alone)
+    gone = [s if i not in (3, 4, 6) else -1 for i, s in enumerate(slots)]
+    x = qkv.float().view(7, H + 2 * G, D)
+    want = write_by_hand(x[:, H + G:], gone, codes[1], scales[1])
+    assert torch.equal(v, want[0]) and torch.equal(vs, want[1])
+
+
+def test_append_of_strided_rows_and_an_empty_step():
+    H, G, D, P = 4, 2, 64, 16
+    qkv, cs, pos, slots, codes, scales = make_append(6, [(3, 20)], H, G, D, P, torch.float16)
+    outs = []
+    for rows in (qkv, torch.cat([qkv, qkv], 1)[:, :qkv.shape[1]]):
+        c = [x.clone() for x in (*codes, *scales)]
+        q = torch.empty(20, 2 * H, D, dtype=torch.float16, device="cuda")[:, :H]
+        ops.kv8_append(rows, cs, i32(pos), i32(slots), *c, q)
+        outs.append((*c, q.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    c = [x.clone() for x in (*codes, *scales)]
+    ops.kv8_append(qkv[:0], cs, i32([]), i32([]), *c, None)
+    assert all(torch.equal(a, b) for a, b in zip(c, (*codes, *scales)))
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------------------
+def make_attention(seed, lens, counts, H, G, D, P, dtype, spread=1.0, q_scale=1.5):
+    """Requests that hold `lens` tokens, `counts` of them new; random pages, garbage in the rows and pages behind them."""
+    g = gen(seed)
+    need = [-(-n // P) for n in lens]
+    order = torch.randperm(sum(need) + 4, generator=torch.Generator().manual_seed(seed)).tolist()
+    W = max(need + [1]) + 1
+    table = [[order.pop() for _ in range(n)] + [-5] * (W - n) for n in need]
+    pages = sum(need) + 4
+    k, v = ((torch.randn(pages, G, P, D, generator=g, device="cuda") * 40).round().clamp(-127, 127).to(torch.int8) for _ in range(2))
+    ks, vs = (2.0 ** (spread * (torch.rand(pages, G, generator=g, device="cuda") * 2 - 1)) / 40 for _ in range(2))
+    q = (q_scale * torch.randn(sum(counts), H, D, generator=g, device="cuda")).to(dtype)
+    start = [0]
+    for c in counts:
+        start.append(start[-1] + c)
+    return q, k, v, ks, vs, i32(table), i32(start), i32(lens)
+
+
+def attention_in_64_bits(q, k, v, ks, vs, table, start, lens, scale):
+    """(result, bound): how far float32 scores, float16 weights and the result's rounding may take it.
+    Weights are rounded to float16: 2^-11 relative, or 2^-25 absolute where the largest weight * value scale of a row is 1 (below float16's
+    normal range). A score is a sum of D exact products in float32 (at most 2^-23 of the sum of their sizes for each addition in the tensor cores,
+    which cut), times factors (3 roundings), and enters the exponential, whose own error and that of log2 of the scale are below 2^-20; sums of
+    values and weights in float32 add 2^-23 a key at most."""
+    T, H, D = q.shape
+    P, G = k.shape[2], k.shape[1]
+    rep = H // G
+    out, bound = torch.zeros(T, H, D, dtype=F64, device="cuda"), torch.zeros(T, H, D, dtype=F64, device="cuda")
+    for b, n in enumerate(lens.tolist()):
+        lo, hi = int(start[b]), int(start[b + 1])
+        if hi == lo or n == 0:
+            continue
+        at = table[b, :-(-n // P)].long()
+        for g in range(G):
+            kk, vv = (c[at, g].to(F64).reshape(-1, D)[:n] for c in (k, v))
+            fk, fv = (s[at, g].to(F64).repeat_interleave(P)[:n] for s in (ks, vs))
+            kk, vv = kk * fk[:, None], vv * fv[:, None]
+            hidden = torch.arange(n, device="cuda")[None] > torch.arange(n - (hi - lo), n, device="cuda")[:, None]
+            for h in range(g * rep, (g + 1) * rep):
+                x = q[lo:hi, h].to(F64)
+                s = (x @ kk.T * scale).masked_fill(hidden, -math.inf)
+                some = ~hidden.all(1)
+                w = torch.exp(s - s.amax(1, keepdim=True).nan_to_num(neginf=0.0))
+                total = w.sum(1, keepdim=True)
+                o = w @ vv / total.clamp(min=1e-300)
+                size = w @ vv.abs() / total.clamp(min=1e-300)
+                ds = ((x.abs() @ kk.abs().T) * scale * ((D + 4) * 2.0 ** -23) + 2.0 ** -20).masked_fill(hidden, 0.0).amax(1, keepdim=True)
+                top = (w * fv[None]).amax(1, keepdim=True)
+                small = n * 2.0 ** -25 * 127 * top / total.clamp(min=1e-300)
+                out[lo:hi, h] = torch.where(some[:, None], o, 0.0)
+                bound[lo:hi, h] = size * (2.0 ** -11 + 2 * ds + n * 2.0 ** -23) + small
+    return out, bound + (out.abs() + bound) * (torch.finfo(q.dtype).eps / 2) + (2.0 ** -25 if q.dtype == torch.float16 else 0.0)
+
+
+def check_attention(case, D, max_tokens=None, workspace=None):
+    q, k, v, ks, vs, table, start, lens = case
+    scale = D ** -0.5
+    out = torch.full_like(q, 3.0)
+    work = ops.kv8_attention_workspace("cuda") if workspace is None else workspace
+    for _ in range(2):                                        # the workspace is left as the next call needs it
+        ops.kv8_attention(q, k, v, ks, vs, table, start, lens, out, scale, work, max_tokens=max_tokens)
+    want, bound = attention_in_64_bits(q, k, v, ks, vs, table, start, lens, scale)
+    rows = int(start[-1])
+    off = (out[:rows].to(F64) - want[:rows]).abs()
+    assert torch.isfinite(out[:rows]).all()
+    assert (off <= bound[:rows]).all(), float((off / bound[:rows].clamp(min=1e-30)).max())
+    assert (out[rows:] == 3.0).all()
+    return out
+
+
+@pytest.mark.parametrize("H,G,D,dtype", [(32, 8, 128, torch.float16), (8, 8, 128, torch.bfloat16), (40, 8, 128, torch.float16), (16, 2, 64, torch.bfloat16), (7, 1, 64, torch.float16)])
+@pytest.mark.parametrize("P", [16, 32, 64, 128])
+def test_attention_of_decoding_requests(H, G, D, dtype, P):
+    lens = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 500, 1000]
+    check_attention(make_attention(1, lens, [1] * len(lens), H, G, D, P, dtype), D, max_tokens=1)
+
+
+@pytest.mark.parametrize("H,G,D,P,dtype", [(32, 8, 128, 64, torch.float16), (64, 8, 128, 16, torch.bfloat16), (40, 8, 128, 32, torch.bfloat16), (16, 16, 64, 128, torch.float16)])
+def test_attention_of_several_tokens_a_request(H, G, D, P, dtype):
+    lens = [4, 5, 64, 66, 700, 333, 129, 3]
+    counts = [4, 3, 4, 5, 1, 0, 2, 3]
+    check_attention(make_attention(2, lens, counts, H, G, D, P, dtype), D, max_tokens=5)
+
+
+@pytest.mark.parametrize("lens,counts", [([3000], [1]), ([20000, 3], [2, 1]), ([70] * 300, [1] * 300), ([1] * 64, [1] * 64)])
+def test_attention_over_stretches_of_every_kind(lens, counts):
+    check_attention(make_attention(3, lens, counts, 8, 2, 128, 64, torch.float16), 128)
+
+
+@pytest.mark.parametrize("H,G,D,P,dtype", [(32, 8, 128, 64, torch.float16), (8, 1, 128, 16, torch.bfloat16), (12, 4, 128, 128, torch.float16), (4, 2, 64, 32, torch.bfloat16),
+                                           (40, 8, 128, 32, torch.bfloat16)])
+@pytest.mark.parametrize("lens,counts", [([17], [17]), ([200], [200]), ([130, 400, 65, 300], [130, 100, 1, 300]), ([257, 9, 1000], [33, 4, 129])])
+def test_attention_of_prompts(H, G, D, P, dtype, lens, counts):
+    check_attention(make_attention(4, lens, counts, H, G, D, P, dtype), D)
+
+
+def test_attention_rows_that_see_nothing_and_rows_of_no_request():
+    q, k, v, ks, vs, table, start, lens = make_attention(5, [0, 40, 0, 300], [2, 1, 40, 3], 8, 2, 128, 32, torch.float16)
+    q = torch.cat([q, q[:9]])                                 # rows behind the last request
+    out = check_attention((q, k, v, ks, vs, table, start, lens), 128)
+    assert not out[:2].any() and not out[3:43].any() and out[2].any()
+
+
+@pytest.mark.parametrize("counts", [[1, 4, 2], [150, 4, 60]])
+def test_attention_with_scales_far_apart(counts):
+    """Pages whose scales differ by 2^20: the weights' common factor takes the value scale in, and no page loses its part of the sum."""
+    q, k, v, ks, vs, table, start, lens = make_attention(6, [500, 200, 900], counts, 8, 2, 128, 16, torch.bfloat16, spread=0.5)
+    vs.mul_(2.0 ** torch.randint(-20, 1, vs.shape, device="cuda", generator=gen(2)))
+    vs[::7] = 2.0 ** -60
+    check_attention((q, k, v, ks, vs, table, start, lens), 128)
+
+
+@pytest.mark.parametrize("q_scale", [0.0, 1e-30, 1e30])
+def test_attention_of_queries_of_any_size(q_scale):
+    case = make_attention(7, [100, 70], [2, 30], 4, 2, 128, 32, torch.bfloat16, q_scale=q_scale)
+    if q_scale > 1:                                           # one key takes all: its value, rounded
+        q, k, v, ks, vs, table, start, lens = case
+        out = torch.empty_like(q)
+        ops.kv8_attention(q, k, v, ks, vs, table, start, lens, out, 128 ** -0.5, ops.kv8_attention_workspace("cuda"))
+        want, _ = attention_in_64_bits(q, k, v, ks, vs, table, start, lens, 128 ** -0.5)
+        torch.testing.assert_close(out.to(F64), want, rtol=2.0 ** -8 + 2.0 ** -10, atol=1e-30)
+    else:
+        check_attention(case, 128)
+
+
+@pytest.mark.parametrize("counts", [[1, 2, 1], [40, 2, 70]])
+def test_attention_shows_what_is_broken_and_only_there(counts):
+    """A query that is not a number, and a table entry outside the cache, make the rows that have to do with them NaN, and no others."""
+    q, k, v, ks, vs, table, start, lens = make_attention(8, [90, 200, 150], counts, 8, 2, 128, 64, torch.float16)
+    clean = check_attention((q, k, v, ks, vs, table, start, lens), 128)
+    q2 = q.clone()
+    q2[0, 3, 5] = math.nan
+    table2 = table.clone()
+    table2[2, 1] = 10 ** 6
+    out = torch.empty_like(q)
+    ops.kv8_attention(q2, k, v, ks, vs, table2, start, lens, out, 128 ** -0.5, ops.kv8_attention_workspace("cuda"))
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    bad[0, 3] = True
+    first = int(lens[2]) - counts[2]
+    for i in range(counts[2]):
+        bad[int(start[2]) + i] = first + i >= 64
+    assert out.isnan().all(2).equal(bad) and out.isnan().any(2).equal(bad)
+    assert torch.equal(out[~bad], clean[~bad])
+
+
+def test_attention_of_strided_queries_and_outputs():
+    q, k, v, ks, vs, table, start, lens = make_attention(9, [90, 200, 300], [1, 2, 40], 8, 2, 128, 64, torch.float16)
+    want = check_attention((q, k, v, ks, vs, table, start, lens), 128)
+    wide = torch.randn(43, 12, 160, device="cuda").half()
+    wide[:, 2:10, 16:144] = q
+    out = torch.full((43, 9, 136), 5.0, dtype=torch.float16, device="cuda")
+    ops.kv8_attention(wide[:, 2:10, 16:144], k, v, ks, vs, table, start, lens, out[:, 1:, :128], 128 ** -0.5, ops.kv8_attention_workspace("cuda"))
+    assert torch.equal(out[:, 1:, :128], want) and (out[:, 0] == 5).all() and (out[:, :, 128:] == 5).all()
+
+
+def test_attention_is_the_same_every_time_and_in_a_graph():
+    case = make_attention(10, [5000, 333, 64, 1800], [4, 4, 1, 2], 32, 8, 128, 64, torch.float16)
+    q, k, v, ks, vs, table, start, lens = case
+    work = ops.kv8_attention_workspace("cuda")
+    want = check_attention(case, 128, workspace=work)
+    out = torch.empty_like(q)
+    ops.kv8_attention(q, k, v, ks, vs, table, start, lens, out, 128 ** -0.5, work)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.kv8_attention(q, k, v, ks, vs, table, start, lens, out, 128 ** -0.5, work)
+    for _ in range(20):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    lens.copy_(i32([4000, 500, 60, 65]))                      # other lengths, the same graph
+    graph.replay()
+    want, bound = attention_in_64_bits(q, k, v, ks, vs, table.clamp(min=0), start, lens, 128 ** -0.5)
+    keep = torch.ones(len(q), dtype=torch.bool, device="cuda")
+    keep[4:8] = False                                         # (the second request has no pages for 500 tokens)
+    assert ((out.to(F64) - want).abs() <= bound)[keep].all()
+
+
+def test_two_streams_with_a_workspace_each():
+    cases = [make_attention(s, [9000, 700], [1, 2], 16, 4, 128, 64, torch.float16) for s in (11, 12)]
+    want = [check_attention(c, 128) for c in cases]
+    streams, works = [torch.cuda.Stream() for _ in cases], [ops.kv8_attention_workspace("cuda") for _ in cases]
+    outs = [torch.empty_like(c[0]) for c in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for c, s, w, o in zip(cases, streams, works, outs):
+            with torch.cuda.stream(s):
+                ops.kv8_attention(*c, o, 128 ** -0.5, w)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+# ---- refusals that need tensors on the GPU -------------------------------------------------------------------------------------------
+def test_wrong_shapes_types_and_overlaps_are_refused():
+    z = lambda *s, dtype=I32: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    args = [z(2), z(2), z(2, 4), z(8), z(3), 16, z(3), z(2), z(5), z(5), z(5), z(4)]
+    for i, bad in ((0, z(2, 1)), (1, z(3)), (4, z(2)), (6, z(2)), (9, z(4)), (11, z(3)), (2, z(4, 2).t()), (0, z(2, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            ops.page_plan(*[bad if j == i else a for j, a in enumerate(args)])
+    both = z(6)
+    with pytest.raises(ValueError, match="must not lie over"):
+        ops.page_plan(*[both[:3] if j == 4 else both[2:] if j == 11 else a for j, a in enumerate(args)])
+    cache = [z(3, 2, 16, 64, dtype=torch.int8), z(3, 2, 16, 64, dtype=torch.int8), z(3, 2, dtype=F32), z(3, 2, dtype=F32)]
+    half = lambda *s: z(*s, dtype=torch.float16)  # noqa: E731
+    app = [half(3, 8 * 64), half(9, 64), z(3), z(3), *cache, half(3, 4, 64)]
+    for i, bad in ((0, half(3, 4 * 64)), (0, half(3, 8 * 64 + 1)), (1, z(9, 64, dtype=F32)), (1, half(9, 32)), (2, z(4)), (3, z(3, dtype=torch.int64)), (5, cache[0][:2]),
+                   (6, z(3, dtype=F32)), (8, half(3, 3, 64)), (8, half(4, 3, 64).transpose(0, 1)), (4, cache[0].view(torch.uint8))):
+        with pytest.raises(ValueError):
+            ops.kv8_append(*[bad if j == i else a for j, a in enumerate(app)])
+    att = [half(3, 4, 64), *cache, z(2, 4), z(3), z(2), half(3, 4, 64), 0.1, ops.kv8_attention_workspace("cuda")]
+    for i, bad in ((0, z(3, 4, 64, dtype=F32)), (0, half(3, 4, 32)), (5, z(8)), (6, z(2)), (7, z(3)), (8, half(3, 4, 64).bfloat16()), (8, half(2, 4, 64)), (9, 0.0), (9, math.nan),
+                   (10, z(9, dtype=F32)), (0, half(3, 5, 64)), (10, z(100, dtype=torch.uint8))):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.kv8_attention(*[bad if j == i else a for j, a in enumerate(att)])
+    with pytest.raises(ValueError):
+        ops.kv8_read(*cache, z(3), half(3, 2, 64), half(2, 2, 64))
