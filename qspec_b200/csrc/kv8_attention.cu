@@ -10,13 +10,16 @@
 // ends inside an item, through the workspace: the CTA that comes last adds the parts up in their order, so that results do not depend on which it is.
 //
 // Codes go from global memory into shared memory (16 bytes a lane, asynchronously, one unit of keys and one of values per warp) and from there into
-// registers as the product's operands: a byte c + 128 behind the byte 0x64 is the float16 1152 + c, and one subtraction makes it c, exactly. The order of the sum over
-// a head's dimensions is free, so that a lane's 16 bytes of a key are its operands of four products, and the queries are loaded in the same order;
-// values need their bytes of two keys interleaved (one byte permutation for two).
+// registers as the product's operands. The order of the sum over a head's dimensions is free, so that a lane's 16 bytes of a key are its operands of four products,
+// and the queries are loaded in the same order; values need their bytes of two keys interleaved (one byte permutation for two).
+//   keys: the byte c + 128 alone is the float16 (c + 128) 2^-24, a subnormal number, which the tensor cores take exactly: no arithmetic but the byte's
+//   place. What the 128 adds to a score is the same for all keys, 128 times the row's sum, and is where the sums begin (from the other side).
+//   values: the byte behind 0x64 is the float16 1152 + c, and one subtraction makes it c. (Sums over values must not carry the 128: over many keys they
+//   cancel, and what the products cut off at the accumulator's last bit would be of the size of what is left.)
 //
-// Queries are multiplied by a power of two per row that brings their largest value to 2^14 .. 2^15, exactly (float16 then holds bfloat16 queries too). A key's scale multiplies its
-// scores in float32. A value's scale v goes into the exponent: the weights 2^(s + log2 v - m) lie in (0, 1] whatever the scales are and are rounded to
-// float16 (2^-12 relative) for the product with the codes; the denominator is the sum of the unrounded weights / v.
+// bfloat16 queries are multiplied by a power of two per row that brings their largest value to 2^14 .. 2^15 and are float16 from there on, exactly. A key's scale
+// multiplies its scores in float32. A value's scale v goes into the exponent: the weights 2^(s + log2 v - m) lie below 2^8 whatever the scales are and are
+// rounded to float16 (2^-11 relative) for the product with the codes; the denominator is the sum of the unrounded weights / v.
 #include "kv8_common.cuh"
 
 namespace qspec {
@@ -54,15 +57,19 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// a scale; one that is zero or next to nothing, or no number, counts as 2^-100
+__device__ __forceinline__ float positive(float x) { return x >= 7.888609052210118e-31f ? x : 7.888609052210118e-31f; }
 // two codes (bytes + 128, chosen by sel from w) as exact float16
 __device__ __forceinline__ uint32_t codes16(uint32_t w, uint32_t sel) {
   const uint32_t m = __byte_perm(w, 0x64646464u, sel);
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));   // 1152
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+// two codes as float16 without the subtraction: c + 128 in units of 2^-24, the smallest float16
+__device__ __forceinline__ uint32_t codes_tiny(uint32_t w, uint32_t sel) { return __byte_perm(w, 0u, sel); }
 __device__ __forceinline__ uint32_t half_pair(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 
 // A request's part of the work.
@@ -81,18 +88,19 @@ __device__ __forceinline__ Req request(const AttArgs& a, int b) {
   return r;
 }
 
-// Where a unit lies: request, item of it (head major, row tiles inside), unit of that.
+// Where a unit lies: request, head and row tile (tiles inside heads), unit of that item.
 struct Place {
-  int b, item, u;
+  int b, g, tile, u;
   Req r;
   __device__ __forceinline__ void forward(const AttArgs& a, int steps) {
     u += steps;
     while (b < a.nreq && u >= r.units) {
       u -= r.units;
-      if (++item >= r.tiles * a.G) {
-        item = 0;
-        do { if (++b >= a.nreq) return; r = request(a, b); } while (r.tiles == 0);
-      }
+      if (++tile < r.tiles) continue;
+      tile = 0;
+      if (++g < a.G) continue;
+      g = 0;
+      do { if (++b >= a.nreq) return; r = request(a, b); } while (r.tiles == 0);
     }
   }
 };
@@ -102,26 +110,37 @@ __device__ __forceinline__ uint32_t k_chunk(int row, int c) { return (uint32_t)(
 template <int D>
 __device__ __forceinline__ uint32_t v_chunk(int row, int c) { return (uint32_t)(row * D + ((D == 128 ? c ^ (row & 6) : c ^ ((row >> 1) & 3)) << 4)); }
 
-// A warp's pages of the unit at `p`: lane i < 64 / P (at least one) has the unit's ith page, or a page that there is not (-1), with its scales.
+// The page that lane i has of the unit at `p`: its ith, of 64 / P (at least one); -1: one behind the last key; BROKEN: an entry that is no page of the cache.
+constexpr int BROKEN = -2;
 __device__ __forceinline__ int unit_page(const AttArgs& a, const Place& p, int lane) {
   const int n = max(UNIT >> a.pshift, 1), at = ((p.u * UNIT) >> a.pshift) + lane;
-  int page = -1;
-  if (lane < n && at < a.width && (at << a.pshift) < p.r.keys) page = a.table[(size_t)p.b * a.width + at];
-  return (unsigned)page < (unsigned)a.npages ? page : -1;
+  if (p.b >= a.nreq || lane >= n || (at << a.pshift) >= p.r.keys) return -1;
+  const int page = at < a.width ? a.table[(size_t)p.b * a.width + at] : BROKEN;
+  return (unsigned)page < (unsigned)a.npages ? page : BROKEN;
 }
+// A unit whose pages are known: where its codes are (bytes from the first page's, the same for keys and values; each lane its page's) and its keys.
+struct Unit {
+  long long at;                                   // -1: no such page
+  int key0, keys;
+};
+// 64 rows of keys or of values, 16 bytes a lane: 16 rows lie in one page, whatever its size, and rows of a group are at fixed distances. Rows behind the last key are
+// not fetched: what the buffer holds in their place are codes like any other, and meets weights of zero.
 template <int D, bool VALUES>
-__device__ __forceinline__ void fetch(const AttArgs& a, const Place& p, int pages, uint32_t dst, int lane) {
+__device__ __forceinline__ void fetch(const AttArgs& a, const Unit& n, uint32_t dst, int lane) {
   constexpr int CH = D / 16, PER = 32 / CH;       // 16-byte pieces of a row; rows per instruction
-  const int g = p.item / p.r.tiles, key0 = p.u * UNIT, in_page = key0 & ((1 << a.pshift) - 1);
-  const signed char* base = VALUES ? a.v : a.k;
-  const int c = lane % CH;
+  const int c = lane % CH, row0 = lane / CH, have = n.keys - n.key0;
+  const signed char* base = (VALUES ? a.v : a.k) + c * 16;
+  const int in_page = n.key0 & ((1 << a.pshift) - 1);       // (the second half of a page of 128)
 #pragma unroll
-  for (int i = 0; i < UNIT / PER; ++i) {
-    const int row = i * PER + lane / CH;
-    const int page = __shfl_sync(0xffffffffu, pages, (row >> a.pshift) & 31);
-    if (key0 + row < p.r.keys && page >= 0)
-      copy16(dst + (VALUES ? v_chunk<D>(row, c) : k_chunk<D>(row, c)),
-             base + (((((size_t)page * a.G + g) << a.pshift) + ((in_page + row) & ((1 << a.pshift) - 1))) * D + c * 16));
+  for (int q = 0; q < 4; ++q) {
+    const long long at = __shfl_sync(0xffffffffu, n.at, (16 * q) >> a.pshift);
+    if (at < 0) continue;
+    const signed char* src = base + at + (size_t)(((in_page + 16 * q) & ((1 << a.pshift) - 1)) + row0) * D;
+#pragma unroll
+    for (int i = 0; i < 16 / PER; ++i) {
+      const int row = q * 16 + i * PER + row0;
+      if (row < have) copy16(dst + (VALUES ? v_chunk<D>(row, c) : k_chunk<D>(row, c)), src + i * PER * D);
+    }
   }
 }
 
@@ -171,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
       const long long n = r.total(a.G);
       if (begin < at + n) {
         s_place[0] = tid * per_thread + i;
-        s_place[1] = (int)((begin - at) / r.units);
+        s_place[1] = (int)((begin - at) / r.units);       // item of the request: head * tiles + tile
         s_place[2] = (int)((begin - at) % r.units);
         break;
       }
@@ -181,41 +200,47 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
   __syncthreads();
   Place cur;                                                // the segment that all warps are in: (the rest of) one item
   cur.b = s_place[0];
-  cur.item = s_place[1];
   cur.u = s_place[2];
   cur.r = request(a, cur.b);
+  cur.g = s_place[1] / cur.r.tiles;
+  cur.tile = s_place[1] - cur.g * cur.r.tiles;
   const int todo = (int)(end - begin);                      // units of this stretch
 
   // queries of an item, 16 rows as they lie: a thread's 16 bytes of them (rows behind the last one are zeros)
   constexpr int PIECES_Q = D / 8;
   const int qr = tid / PIECES_Q, qc = tid % PIECES_Q;
   auto load_q = [&](const Place& p) {
-    const int row = (p.item % p.r.tiles) * ROWS + qr, tok = row / a.rep;
+    const int row = p.tile * ROWS + qr, tok = row / a.rep;
     if (qr >= ROWS || tok >= p.r.n) return make_uint4(0u, 0u, 0u, 0u);
-    return *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(p.r.first + tok) * a.q_ts + (size_t)((p.item / p.r.tiles) * a.rep + row - tok * a.rep) * a.q_hs + qc * 8);
+    return *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(p.r.first + tok) * a.q_ts + (size_t)(p.g * a.rep + row - tok * a.rep) * a.q_hs + qc * 8);
   };
   auto store_q = [&](const uint4& w, int buf) {
     if (qr < ROWS) *reinterpret_cast<uint4*>(s_q + (buf * ROWS + qr) * D * 2 + qc * 16) = w;
   };
 
-  // ---- the first unit of this warp is on its way before anything else
+  // ---- the first unit of this warp is on its way before anything else. Pages are looked up one unit ahead of the copies, so that these do not wait for them.
   int next = warp;                                          // index in the stretch of the unit that is fetched next
   Place np = cur;
   np.forward(a, warp);
-  int pages = -1;
-  float pks = 0.f, pvs = 1.f;                               // scales of the unit that is fetched
-  auto look = [&]() {                                       // the next unit's pages and scales
-    pages = next < todo ? unit_page(a, np, lane) : -1;
-    const int g = np.b < a.nreq ? np.item / np.r.tiles : 0;
+  int pages = next < todo ? unit_page(a, np, lane) : -1;
+  Unit unit{-1, 0, 0};                                      // the one that was fetched last, with its scales
+  float pks = 0.f, pvs = 1.f;
+  auto take = [&]() {                                       // the unit at np, and the pages of the one behind it
     const bool there = pages >= 0;
-    pks = there ? a.ks[(size_t)pages * a.G + g] : NAN;      // (a page outside the cache: every row that sees it is NaN)
-    pvs = there ? fmaxf(a.vs[(size_t)pages * a.G + g], 7.888609052210118e-31f) : 1.f;
+    const size_t block = there ? (size_t)pages * a.G + np.g : 0;
+    unit.at = there ? (long long)((block << a.pshift) * D) : -1ll;
+    unit.key0 = np.u * UNIT;
+    unit.keys = next < todo ? np.r.keys : 0;
+    pks = there ? a.ks[block] : pages == BROKEN ? NAN : 1.f;
+    pvs = there ? a.vs[block] : 1.f;
+    np.forward(a, WARPS);
+    pages = next + WARPS < todo ? unit_page(a, np, lane) : -1;
   };
   uint4 queries = load_q(cur);
-  look();
-  if (next < todo) fetch<D, false>(a, np, pages, kbuf, lane);
+  take();
+  fetch<D, false>(a, unit, kbuf, lane);
   copy_commit();
-  if (next < todo) fetch<D, true>(a, np, pages, vbuf, lane);
+  fetch<D, true>(a, unit, vbuf, lane);
   copy_commit();
   store_q(queries, 0);
   __syncthreads();
@@ -228,131 +253,163 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
     const bool more = seg0 + seg_n < todo;
     if (more) queries = load_q(after);                      // the next segment's queries, on their way beside this one's work
 
-    // ---- queries into registers, each row by a power of two
-    const int tile = cur.item % cur.r.tiles, g = cur.item / cur.r.tiles;
+    const int tile = cur.tile, g = cur.g;
+    // ---- queries into registers; bfloat16 rows by a power of two each
     uint32_t qa[KS][4];
     float rowf[2];
-    int limit[2], low;                                      // last visible position of this lane's rows; the lowest of the tile's
-    {
-      float mx[2] = {0.f, 0.f};
-      float x[2][CH / 4][16];
+    int limit[2];                                           // last visible position of this lane's rows
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const unsigned char* row = s_q + ((seg & 1) * ROWS + qi + 8 * e) * D * 2;
+    for (int e = 0; e < 2; ++e) {
+      const unsigned char* row = s_q + ((seg & 1) * ROWS + qi + 8 * e) * D * 2;
+      uint32_t x[CH / 4][8];
 #pragma unroll
-        for (int h = 0; h < CH / 4; ++h) {
-          const uint4 w0 = *reinterpret_cast<const uint4*>(row + (h * 4 + qj) * 32), w1 = *reinterpret_cast<const uint4*>(row + (h * 4 + qj) * 32 + 16);
-          float y[8];
-          unpack8<BF16>(w0, y);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[e][h][i] = y[i];
-          unpack8<BF16>(w1, y);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[e][h][8 + i] = y[i];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mx[e] = fmaxf(mx[e], fabsf(x[e][h][i]));
-        }
-        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-        // 2^(14 - exponent of the largest), from its bits; none for a row of zeros or one that is not finite, and in float32's range at both ends
-        const int ex = (int)(__float_as_uint(mx[e]) >> 23) - 127;
-        const int sh = mx[e] > 0.f && mx[e] < INFINITY ? min(max(14 - ex, -126), 126) : 0;
-        const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
-        rowf[e] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2;
+      for (int h = 0; h < CH / 4; ++h) {
+        const uint4 w0 = *reinterpret_cast<const uint4*>(row + (h * 4 + qj) * 32), w1 = *reinterpret_cast<const uint4*>(row + (h * 4 + qj) * 32 + 16);
+        x[h][0] = w0.x; x[h][1] = w0.y; x[h][2] = w0.z; x[h][3] = w0.w;
+        x[h][4] = w1.x; x[h][5] = w1.y; x[h][6] = w1.z; x[h][7] = w1.w;
+      }
+      int sh = 0;
+      if (BF16) {
+        float mx = 0.f;
 #pragma unroll
         for (int h = 0; h < CH / 4; ++h)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            qa[h * 4 + w][e] = half_pair(x[e][h][w * 4] * up, x[e][h][w * 4 + 1] * up);
-            qa[h * 4 + w][e + 2] = half_pair(x[e][h][w * 4 + 2] * up, x[e][h][w * 4 + 3] * up);
-          }
-        const int tok = (tile * ROWS + qi + 8 * e) / a.rep;
-        limit[e] = tok < cur.r.n ? min(cur.r.keys - cur.r.n + tok, cur.r.keys - 1) : -1;
+          for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[h][i] << 16)), fabsf(__uint_as_float(x[h][i] & 0xffff0000u))));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // 2^(14 - exponent of the largest), from its bits; none for a row of zeros or one that is not finite, and in float32's range at both ends
+        const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+        sh = mx > 0.f && mx < INFINITY ? min(max(14 - ex, -126), 126) : 0;
+        const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
+#pragma unroll
+        for (int h = 0; h < CH / 4; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[h][i] = half_pair(__uint_as_float(x[h][i] << 16) * up, __uint_as_float(x[h][i] & 0xffff0000u) * up);
       }
-      low = cur.r.keys - cur.r.n + tile * ROWS / a.rep;
+      rowf[e] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2;
+#pragma unroll
+      for (int h = 0; h < CH / 4; ++h)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          qa[h * 4 + w][e] = x[h][2 * w];
+          qa[h * 4 + w][e + 2] = x[h][2 * w + 1];
+        }
+      const int tok = (tile * ROWS + qi + 8 * e) / a.rep;
+      limit[e] = tok < cur.r.n ? min(cur.r.keys - cur.r.n + tok, cur.r.keys - 1) : -1;
     }
+    const int low = cur.r.keys - cur.r.n + tile * ROWS / a.rep;   // the lowest of the tile's rows
+    // What the codes' 128 adds to a row's scores, the other way round: -128 (in units of 2^-24) times the sum of the row.
+    float s0[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < KS; ++i) mma16816(s0, qa[i], 0x80808080u, 0x80808080u);
     float o[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
     float m[2] = {NONE, NONE}, l[2] = {0.f, 0.f};
 
     while (next < seg0 + seg_n) {
-      // ---- scores of 64 keys
-      const int key0 = np.u * UNIT;
+      // ---- scores of 64 keys, in units of 2^-24
+      const int key0 = unit.key0;
       const float cks = pks, cvs = pvs;
       copy_wait<1>();
       __syncwarp();
       float s[8][4];
 #pragma unroll
-      for (int nt = 0; nt < 8; ++nt) {
-        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[4][CH / 4][4];
 #pragma unroll
-        for (int h = 0; h < CH / 4; ++h) {
-          uint32_t w[4];
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(kbuf + k_chunk<D>(nt * 8 + qi, h * 4 + qj)));
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t u = w[i] ^ 0x80808080u;
-            mma16816(s[nt], qa[h * 4 + i], codes16(u, 0x4140), codes16(u, 0x4342));
-          }
-        }
+          for (int h = 0; h < CH / 4; ++h)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[n][h][0]), "=r"(w[n][h][1]), "=r"(w[n][h][2]), "=r"(w[n][h][3])
+                         : "r"(kbuf + k_chunk<D>((half * 4 + n) * 8 + qi, h * 4 + qj)));
+#pragma unroll
+        for (int n = 0; n < 4; ++n) { s[half * 4 + n][0] = s0[0]; s[half * 4 + n][1] = s0[0]; s[half * 4 + n][2] = s0[2]; s[half * 4 + n][3] = s0[2]; }
+#pragma unroll
+        for (int h = 0; h < CH / 4; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const uint32_t u = w[n][h][i] ^ 0x80808080u;
+              mma16816(s[half * 4 + n], qa[h * 4 + i], codes_tiny(u, 0x4140), codes_tiny(u, 0x4342));
+            }
       }
       __syncwarp();
       // the next unit's keys take this one's place
       next += WARPS;
-      np.forward(a, WARPS);
-      look();
-      if (next < todo) fetch<D, false>(a, np, pages, kbuf, lane);
+      take();
+      fetch<D, false>(a, unit, kbuf, lane);
       copy_commit();
       // ---- weights
-      float kf[4], lv[4], iv[4];                            // of 16 keys each
+      // Keys that a row does not see; and of a page that there is not, or whose scale is no number, what makes the rows NaN that do see it.
+      const bool odd = __any_sync(0xffffffffu, cks != cks || cvs != cvs);
+      if (key0 + UNIT - 1 > low || odd) {
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt) {
+          const int src = (8 * nt) >> a.pshift;
+          const float both = __shfl_sync(0xffffffffu, cks + cvs, src);
+          const bool none = both != both;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (none) s[nt][e] = NAN;
+            if (key0 + nt * 8 + qj * 2 + (e & 1) > limit[e >> 1]) s[nt][e] = NONE;
+          }
+        }
+      }
+      float kf[4][2], lv[4], iv[4], mx[2] = {NONE, NONE};   // of 16 keys each: factor of the scores, log2 of the value scale and its reciprocal
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int src = (16 * q) >> a.pshift;
-        kf[q] = __shfl_sync(0xffffffffu, cks, src);
-        const float v = __shfl_sync(0xffffffffu, cvs, src);
+        const float f = positive(__shfl_sync(0xffffffffu, cks, src)) * 16777216.f, v = positive(__shfl_sync(0xffffffffu, cvs, src));
         lv[q] = __log2f(v);
         iv[q] = __fdividef(1.f, v);
-      }
-      float mx[2] = {NONE, NONE};
-      const bool cut = key0 + UNIT - 1 > low;
 #pragma unroll
-      for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = fmaf(s[nt][e], rowf[e >> 1] * kf[nt >> 1], lv[nt >> 1]);
-          if (cut && key0 + nt * 8 + qj * 2 + (e & 1) > limit[e >> 1]) x = NONE;
-          s[nt][e] = x;
-          mx[e >> 1] = fmaxf(mx[e >> 1], x);
+        for (int e = 0; e < 2; ++e) {
+          kf[q][e] = f * rowf[e];
+          const float top = fmaxf(fmaxf(s[2 * q][2 * e], s[2 * q][2 * e + 1]), fmaxf(s[2 * q + 1][2 * e], s[2 * q + 1][2 * e + 1]));
+          mx[e] = fmaxf(mx[e], fmaf(top, kf[q][e], lv[q])); // (factors are positive: the largest score has the largest exponent)
         }
+      }
+      bool grown[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-        mx[e] = fmaxf(mx[e], m[e]);
+        // The reference follows the maximum only where it has fallen 2^8 behind: weights stay below 2^8, and sums are seldom multiplied again.
+        grown[e] = mx[e] > m[e] + 8.f || (m[e] == NONE && mx[e] > NONE);
       }
-      if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-        float f[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          f[e] = mx[e] > m[e] ? exp2_fast(m[e] - mx[e]) : 1.f;     // 0 for a row that has seen nothing
-          m[e] = mx[e];
-          l[e] *= f[e];
-        }
+      if (__any_sync(0xffffffffu, (grown[0] && m[0] != NONE) || (grown[1] && m[1] != NONE))) {
+        const float f[2] = {grown[0] ? exp2_fast(m[0] - mx[0]) : 1.f, grown[1] ? exp2_fast(m[1] - mx[1]) : 1.f};
+        l[0] *= f[0];
+        l[1] *= f[1];
 #pragma unroll
         for (int t = 0; t < NT; ++t) { o[t][0] *= f[0]; o[t][1] *= f[0]; o[t][2] *= f[1]; o[t][3] *= f[1]; }
       }
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (grown[e]) m[e] = mx[e];                         // (a row that had seen nothing has sums of zero)
       const float ref[2] = {m[0] == NONE ? 0.f : m[0], m[1] == NONE ? 0.f : m[1]};
+      // Exponents are taken from the products without a rounding in between, the reference has one: beyond 2^24 that alone would be a large exponent.
+      if (__any_sync(0xffffffffu, fabsf(ref[0]) > 16777216.f || fabsf(ref[1]) > 16777216.f)) {
+#pragma unroll
+        for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = fmaf(s[nt][e], kf[nt >> 1][e >> 1], lv[nt >> 1]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { kf[q][0] = kf[q][1] = 1.f; lv[q] = 0.f; }
+      }
       uint32_t pa[4][4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
+        const float at[2] = {lv[q] - ref[0], lv[q] - ref[1]};
         float part[2] = {0.f, 0.f};
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
           float w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            w[e] = exp2_fast(s[2 * q + z][e] - ref[e >> 1]);
+            w[e] = exp2_fast(fmaf(s[2 * q + z][e], kf[q][e >> 1], at[e >> 1]));
             part[e >> 1] += w[e];
           }
           pa[q][z * 2] = half_pair(w[0], w[1]);
@@ -389,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
         }
       }
       __syncwarp();
-      if (next < todo) fetch<D, true>(a, np, pages, vbuf, lane);
+      fetch<D, true>(a, unit, vbuf, lane);
       copy_commit();
     }
 
