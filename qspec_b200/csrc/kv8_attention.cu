@@ -4,18 +4,19 @@
 // A row is a (token, query head of a group) pair; 16 rows of one key/value head are a tile of mma.sync.m16n8k16, so that the heads of a group and the
 // tokens that verify a draft share every key that is read. What bounds it at these row counts is the cache: 2 D bytes a key and head.
 //
-// Work: (request, head, row tile) items of ceil(kv_len / 64) units of 64 keys, laid end to end and cut into equal stretches, one per CTA: lengths that
-// differ cost nothing, one long request uses every SM. Inside a stretch unit i is warp i % 8's. Every warp keeps a softmax of its own (maximum, sum and
+// Work: (request, head, row tile) items of units of 32 keys, laid end to end and cut into equal stretches, one per CTA: lengths that
+// differ cost nothing, one long request uses every SM. Inside a stretch unit i is warp i % WARPS's. Every warp keeps a softmax of its own (maximum, sum and
 // sums of values in registers) over the units of an item that it took; they are joined through shared memory at the item's end and, where a stretch
 // ends inside an item, through the workspace: the CTA that comes last adds the parts up in their order, so that results do not depend on which it is.
 //
 // Codes go from global memory into shared memory (16 bytes a lane, asynchronously, one unit of keys and one of values per warp) and from there into
-// registers as the product's operands. The order of the sum over a head's dimensions is free, so that a lane's 16 bytes of a key are its operands of four products,
-// and the queries are loaded in the same order; values need their bytes of two keys interleaved (one byte permutation for two).
-//   keys: the byte c + 128 alone is the float16 (c + 128) 2^-24, a subnormal number, which the tensor cores take exactly: no arithmetic but the byte's
-//   place. What the 128 adds to a score is the same for all keys, 128 times the row's sum, and is where the sums begin (from the other side).
-//   values: the byte behind 0x64 is the float16 1152 + c, and one subtraction makes it c. (Sums over values must not carry the 128: over many keys they
-//   cancel, and what the products cut off at the accumulator's last bit would be of the size of what is left.)
+// registers as the products' operands.
+//   keys: a byte c + 128 alone is the float16 (c + 128) 2^-24, a subnormal number, which the tensor cores take exactly: no arithmetic but the byte's
+//   place. What the 128 adds to a score is the same for all keys, 128 times the row's sum, and is where the sums begin, from the other side. The order of
+//   the sum over a head's dimensions is free, so that a lane's 16 bytes of a key are its operands of four products; queries lie in shared memory in that order.
+//   values: the transposing load of 16 x 16 bytes gives four keys of a column a word (the keys of the score tiles are numbered to match); the byte behind 0x64 is the
+//   float16 1152 + c, and one subtraction makes it c. (Sums over values must not carry the 128: over many keys they cancel, and what the
+//   products cut off would be of the size of what is left.)
 //
 // bfloat16 queries are multiplied by a power of two per row that brings their largest value to 2^14 .. 2^15 and are float16 from there on, exactly. A key's scale
 // multiplies its scores in float32. A value's scale v goes into the exponent: the weights 2^(s + log2 v - m) lie below 2^8 whatever the scales are and are
@@ -25,9 +26,10 @@
 namespace qspec {
 namespace kv8 {
 
-constexpr int WARPS = 8, THREADS = WARPS * 32, UNIT = 64, ROWS = 16;
-constexpr int MIN_UNITS = 8;                     // of a stretch: one for each warp
-constexpr int O_LD = 144;                        // floats of a row of sums on its way between warps (16 modulo 32: eight lanes' pieces in eight banks each)
+constexpr int WARPS = 4, THREADS = WARPS * 32, UNIT = 32, ROWS = 16;
+constexpr int MIN_UNITS = WARPS;                 // of a stretch: one for each warp
+constexpr int CTAS = 3;                          // of an SM: while one waits at a barrier the others compute
+constexpr int GRID_MOST = 480;                   // CTAs
 constexpr float NONE = -INFINITY;
 
 struct AttArgs {
@@ -44,10 +46,13 @@ struct AttArgs {
 template <int D> struct Smem {
   static constexpr int BUF = UNIT * D;                                  // one unit's keys or values
   static constexpr size_t RING = (size_t)WARPS * 2 * BUF;
-  static constexpr size_t Q = 2 * ROWS * D * 2;
-  static constexpr size_t O = (size_t)WARPS * ROWS * O_LD * 4;
+  static constexpr size_t Q = ROWS * D * 2;
+  static constexpr int LD = D + 8;                                      // floats of a row of sums on its way between warps (8 modulo 32: no bank conflicts)
+  static constexpr size_t SUMS = (size_t)WARPS * ROWS * LD * 4, FACTORS = (size_t)(GRID_MOST + 1) * ROWS * 4;
+  static constexpr size_t O = SUMS > FACTORS ? SUMS : FACTORS;          // sums on their way between warps, or a factor for every part of an item
   static constexpr size_t ML = (size_t)WARPS * ROWS * 2 * 4;
-  static constexpr size_t TOTAL = RING + Q + O + ML;
+  static constexpr size_t F = ROWS * 4;                             // factors of the rows' scores
+  static constexpr size_t TOTAL = RING + Q + O + ML + F;
 };
 template <int D> constexpr int PART = ROWS * 2 + ROWS * D;   // floats of a part: maxima, sums, sums of values
 
@@ -56,20 +61,28 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm vola
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = a b + c
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// two 16 x 16 blocks of bytes, columns first: word 2 m + h of a lane has rows 4 j .. 4 j + 3 (j = lane % 4) of column lane / 4 + 8 h of block m
+__device__ __forceinline__ void load_columns(uint32_t (&w)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
 }
 // a scale; one that is zero or next to nothing, or no number, counts as 2^-100
 __device__ __forceinline__ float positive(float x) { return x >= 7.888609052210118e-31f ? x : 7.888609052210118e-31f; }
-// two codes (bytes + 128, chosen by sel from w) as exact float16
-__device__ __forceinline__ uint32_t codes16(uint32_t w, uint32_t sel) {
+// The first two / the last two of four codes (bytes c + 128) as float16: a byte alone is (c + 128) 2^-24, a subnormal number.
+__device__ __forceinline__ uint32_t first_two(uint32_t w) { return __byte_perm(w, 0u, 0x4140); }
+__device__ __forceinline__ uint32_t last_two(uint32_t w) { return __byte_perm(w, 0u, 0x4342); }
+constexpr uint32_t MINUS_128 = 0x80808080u;      // two of -128 2^-24: what the codes' 128 adds up to, the other way round
+// The same as c, exactly: a byte behind 0x64 is 1152 + c.
+__device__ __forceinline__ uint32_t exact_two(uint32_t w, uint32_t sel) {
   const uint32_t m = __byte_perm(w, 0x64646464u, sel);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));   // 1152
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// two codes as float16 without the subtraction: c + 128 in units of 2^-24, the smallest float16
-__device__ __forceinline__ uint32_t codes_tiny(uint32_t w, uint32_t sel) { return __byte_perm(w, 0u, sel); }
 __device__ __forceinline__ uint32_t half_pair(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 
 // A request's part of the work.
@@ -105,12 +118,13 @@ struct Place {
   }
 };
 
+// Where the 16 bytes c of a row lie in a buffer, so that neither copies nor reads of eight rows meet in a bank.
 template <int D>
 __device__ __forceinline__ uint32_t k_chunk(int row, int c) { return (uint32_t)(row * D + ((D == 128 ? c ^ ((row & 1) << 2) : c) << 4)); }
 template <int D>
-__device__ __forceinline__ uint32_t v_chunk(int row, int c) { return (uint32_t)(row * D + ((D == 128 ? c ^ (row & 6) : c ^ ((row >> 1) & 3)) << 4)); }
+__device__ __forceinline__ uint32_t v_chunk(int row, int c) { return (uint32_t)(row * D + ((D == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4)); }
 
-// The page that lane i has of the unit at `p`: its ith, of 64 / P (at least one); -1: one behind the last key; BROKEN: an entry that is no page of the cache.
+// The page that lane i has of the unit at `p`: its ith, of UNIT / P (at least one); -1: one behind the last key; BROKEN: an entry that is no page of the cache.
 constexpr int BROKEN = -2;
 __device__ __forceinline__ int unit_page(const AttArgs& a, const Place& p, int lane) {
   const int n = max(UNIT >> a.pshift, 1), at = ((p.u * UNIT) >> a.pshift) + lane;
@@ -123,75 +137,145 @@ struct Unit {
   long long at;                                   // -1: no such page
   int key0, keys;
 };
-// 64 rows of keys or of values, 16 bytes a lane: 16 rows lie in one page, whatever its size, and rows of a group are at fixed distances. Rows behind the last key are
+// UNIT rows of keys or of values, 16 bytes a lane: 16 rows lie in one page, whatever its size, and rows of a group are at fixed distances. Rows behind the last key are
 // not fetched: what the buffer holds in their place are codes like any other, and meets weights of zero.
 template <int D, bool VALUES>
 __device__ __forceinline__ void fetch(const AttArgs& a, const Unit& n, uint32_t dst, int lane) {
   constexpr int CH = D / 16, PER = 32 / CH;       // 16-byte pieces of a row; rows per instruction
   const int c = lane % CH, row0 = lane / CH, have = n.keys - n.key0;
-  const signed char* base = (VALUES ? a.v : a.k) + c * 16;
-  const int in_page = n.key0 & ((1 << a.pshift) - 1);       // (the second half of a page of 128)
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const long long at = __shfl_sync(0xffffffffu, n.at, (16 * q) >> a.pshift);
-    if (at < 0) continue;
-    const signed char* src = base + at + (size_t)(((in_page + 16 * q) & ((1 << a.pshift) - 1)) + row0) * D;
+  const signed char* base = (VALUES ? a.v : a.k) + (row0 * D + c * 16);
+  auto rows = [&](int q, const signed char* src, bool all) {  // rows 16 q .. 16 q + 15
 #pragma unroll
     for (int i = 0; i < 16 / PER; ++i) {
       const int row = q * 16 + i * PER + row0;
-      if (row < have) copy16(dst + (VALUES ? v_chunk<D>(row, c) : k_chunk<D>(row, c)), src + i * PER * D);
+      if (all || row < have) copy16(dst + (VALUES ? v_chunk<D>(row, c) : k_chunk<D>(row, c)), src + i * PER * D);
+    }
+  };
+  if (a.pshift >= 5 && have >= UNIT) {            // (one page; larger ones are several units)
+    const long long at = __shfl_sync(0xffffffffu, n.at, 0);
+    if (at < 0) return;
+    const signed char* src = base + at + (size_t)(n.key0 & ((1 << a.pshift) - 1)) * D;
+#pragma unroll
+    for (int q = 0; q < UNIT / 16; ++q) rows(q, src + 16 * q * D, true);
+  } else {
+#pragma unroll
+    for (int q = 0; q < UNIT / 16; ++q) {
+      const long long at = __shfl_sync(0xffffffffu, n.at, (16 * q) >> a.pshift);
+      if (at >= 0) rows(q, base + at + (size_t)((n.key0 + 16 * q) & ((1 << a.pshift) - 1)) * D, false);
     }
   }
 }
 
 template <bool BF16, int D>
-__global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs a) {
+__global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttArgs a) {
   using T = typename Elem16<BF16>::T;
   using S = Smem<D>;
-  constexpr int KS = D / 16, NT = D / 8, CH = D / 16;       // steps of the score product, column tiles of the value product, 16-byte pieces of a key
+  constexpr int NT = D / 8, CH = D / 16, KT = UNIT / 8, QT = UNIT / 16;   // column tiles of the value product, 16-byte pieces of a key (steps of the score product), key tiles
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long s_sum[WARPS];
-  __shared__ int s_place[3];
+  __shared__ int s_place[4], s_items[WARPS], s_ctas[6][WARPS];
+  __shared__ Req s_req;
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, qi = lane >> 2, qj = lane & 3;
   unsigned char* const s_q = smem + S::RING;
   float* const s_o = reinterpret_cast<float*>(smem + S::RING + S::Q);
   float* const s_ml = reinterpret_cast<float*>(smem + S::RING + S::Q + S::O);   // [warp][maximum, sum][16]
+  float* const s_f = reinterpret_cast<float*>(smem + S::RING + S::Q + S::O + S::ML);   // [16]
   const uint32_t kbuf = shared_addr(smem) + warp * 2 * S::BUF, vbuf = kbuf + S::BUF;
   pdl_enter();
 
-  // ---- this CTA's stretch: all units, and the request that the first one lies in
-  const int per_thread = (a.nreq + THREADS - 1) / THREADS;
-  long long mine = 0;
-  for (int i = 0; i < per_thread; ++i) {
-    const int b = tid * per_thread + i;
-    if (b < a.nreq) mine += request(a, b).total(a.G);
-  }
-  long long incl = mine;
+  // ---- this CTA's stretch
+  const int per_thread = (a.nreq + THREADS - 1) / THREADS, b0 = tid * per_thread;
+  Req only{0, 0, 0, 0, 1};
+  if (per_thread == 1 && b0 < a.nreq) only = request(a, b0);
+  auto req = [&](int i) { return per_thread == 1 ? only : request(a, b0 + i); };
+  const int requests = max(min(per_thread, a.nreq - b0), 0);
+  long long before, total;                                  // of the requests of the threads in front of this one, and of all
+  auto scan = [&](long long mine) {
+    long long incl = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long w = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += w;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long w = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += w;
+    }
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+    before = incl - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) before += s_sum[w];
+      total += s_sum[w];
+    }
+  };
+  long long mine = 0;
+  int items = 0;
+  for (int i = 0; i < requests; ++i) {
+    const Req r = req(i);
+    mine += r.total(a.G);
+    items = min(items + (int)min((long long)r.tiles * a.G, (long long)GRID_MOST + 1), GRID_MOST + 1);
   }
-  if (lane == 31) s_sum[warp] = incl;
-  __syncthreads();
-  long long before = incl - mine, total = 0;
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
+  items = __reduce_add_sync(0xffffffffu, items);
+  if (lane == 0) s_items[warp] = items;
+  scan(mine);
+  const int grid = gridDim.x;
+  long long per = max(total <= 0x7fffffff ? (long long)(((int)total - 1) / grid + 1) : (total + grid - 1) / grid, (long long)MIN_UNITS);
+  // A stretch may lie over the end of an item: then the CTA joins and stores twice. With few items each gets CTAs of its own, as long as that makes no
+  // stretch much longer (by a quarter and eight units at most): 4 requests of 900, 32 / 8 heads, one token each 17.0 -> 12.1 us.
+  bool whole = false;
+  items = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) items += s_items[w];
+  if (items <= grid && per < (1 << 24)) {
+    constexpr int TRIES = 6;                                // lengths that are looked at
+    auto length = [&](int c) { const int p = (int)per; return c == 0 ? p : c == 1 ? p + 1 : c == 2 ? p + p / 32 + 1 : c == 3 ? p + p / 16 + 2 : c == 4 ? p + p / 8 + 4 : p + p / 4 + 8; };
+    int n[TRIES] = {0, 0, 0, 0, 0, 0};
+    for (int i = 0; i < requests; ++i) {
+      const Req r = req(i);
+#pragma unroll
+      for (int c = 0; c < TRIES; ++c)
+        n[c] = min(n[c] + (int)min((long long)r.tiles * a.G * ((r.units - 1) / length(c) + 1), (long long)GRID_MOST + 1), GRID_MOST + 1);
+    }
+#pragma unroll
+    for (int c = 0; c < TRIES; ++c) {
+      n[c] = __reduce_add_sync(0xffffffffu, n[c]);
+      if (lane == 0) s_ctas[c][warp] = n[c];
+    }
+    __syncthreads();
+    int len = 0;
+#pragma unroll
+    for (int c = TRIES - 1; c >= 0; --c) {
+      int sum = 0;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) sum += s_ctas[c][w];
+      if (sum <= grid) len = length(c);
+    }
+    if (len) {
+      whole = true;
+      per = len;
+      mine = 0;                                             // CTAs of this thread's requests
+      for (int i = 0; i < requests; ++i) {
+        const Req r = req(i);
+        mine += (long long)r.tiles * a.G * ((r.units - 1) / len + 1);
+      }
+      scan(mine);
+    }
   }
-  const long long per = max((total + gridDim.x - 1) / gridDim.x, (long long)MIN_UNITS);
-  const long long begin = per * blockIdx.x, end = min(begin + per, total);
-  if (begin >= end) return;
+  // (an item's units are spread evenly over its CTAs)
+  const long long begin = whole ? blockIdx.x : per * blockIdx.x;
+  if (begin >= total) return;
   if (begin >= before && begin < before + mine) {
     long long at = before;
-    for (int i = 0; i < per_thread; ++i) {
-      const Req r = request(a, min(tid * per_thread + i, a.nreq - 1));
-      const long long n = r.total(a.G);
+    for (int i = 0; i < requests; ++i) {
+      const Req r = req(i);
+      const int each = whole ? (r.units - 1) / (int)per + 1 : r.units;   // of an item: CTAs, or units
+      const long long n = (long long)r.tiles * a.G * each;
       if (begin < at + n) {
-        s_place[0] = tid * per_thread + i;
-        s_place[1] = (int)((begin - at) / r.units);       // item of the request: head * tiles + tile
-        s_place[2] = (int)((begin - at) % r.units);
+        s_place[0] = b0 + i;
+        s_place[1] = (int)((begin - at) / each);            // item of the request: head * tiles + tile
+        s_place[2] = (int)((begin - at) % each);
+        s_place[3] = each;
+        s_req = r;
         break;
       }
       at += n;
@@ -200,22 +284,54 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
   __syncthreads();
   Place cur;                                                // the segment that all warps are in: (the rest of) one item
   cur.b = s_place[0];
-  cur.u = s_place[2];
-  cur.r = request(a, cur.b);
+  cur.r = s_req;
   cur.g = s_place[1] / cur.r.tiles;
   cur.tile = s_place[1] - cur.g * cur.r.tiles;
-  const int todo = (int)(end - begin);                      // units of this stretch
+  const int share = whole ? (cur.r.units - 1) / s_place[3] + 1 : 0;
+  cur.u = whole ? min(s_place[2] * share, cur.r.units) : s_place[2];
+  const int todo = whole ? min(share, cur.r.units - cur.u) : (int)(min(begin + per, total) - begin);   // units of this stretch
+  if (todo <= 0) return;                                    // (a last share of none)
 
-  // queries of an item, 16 rows as they lie: a thread's 16 bytes of them (rows behind the last one are zeros)
-  constexpr int PIECES_Q = D / 8;
-  const int qr = tid / PIECES_Q, qc = tid % PIECES_Q;
+  // Queries of an item: a thread's pieces of 8 values (rows behind the last one are zeros), then float16 in the order in which the product takes them: word
+  // (step, lane, register) of the operand. Step 4 h + w of lane (row % 8, j) has columns 16 (4 h + j) + 4 w .. + 3.
+  constexpr int IN_ROW = D / 8, PIECES_Q = ROWS * IN_ROW / THREADS, QROWS = THREADS / IN_ROW;
+  const int qr = tid / IN_ROW, qc = tid % IN_ROW;
+  uint4 queries[PIECES_Q];
   auto load_q = [&](const Place& p) {
-    const int row = p.tile * ROWS + qr, tok = row / a.rep;
-    if (qr >= ROWS || tok >= p.r.n) return make_uint4(0u, 0u, 0u, 0u);
-    return *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(p.r.first + tok) * a.q_ts + (size_t)(p.g * a.rep + row - tok * a.rep) * a.q_hs + qc * 8);
+#pragma unroll
+    for (int i = 0; i < PIECES_Q; ++i) {
+      const int row = p.tile * ROWS + qr + i * QROWS, tok = row / a.rep;
+      queries[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (tok < p.r.n)
+        queries[i] = *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(p.r.first + tok) * a.q_ts + (size_t)(p.g * a.rep + row - tok * a.rep) * a.q_hs + qc * 8);
+    }
   };
-  auto store_q = [&](const uint4& w, int buf) {
-    if (qr < ROWS) *reinterpret_cast<uint4*>(s_q + (buf * ROWS + qr) * D * 2 + qc * 16) = w;
+  auto store_q = [&]() {
+#pragma unroll
+    for (int i = 0; i < PIECES_Q; ++i) {
+      const int row = qr + i * QROWS;
+      uint32_t x[4] = {queries[i].x, queries[i].y, queries[i].z, queries[i].w};
+      int sh = 0;
+      if (BF16) {
+        float mx = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
+#pragma unroll
+        for (int o = IN_ROW / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        // 2^(14 - exponent of the largest), from its bits; none for a row of zeros or one that is not finite, and in float32's range at both ends
+        const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+        sh = mx > 0.f && mx < INFINITY ? min(max(14 - ex, -126), 126) : 0;
+        const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = half_pair(__uint_as_float(x[e] << 16) * up, __uint_as_float(x[e] & 0xffff0000u) * up);
+      }
+      if (qc == 0) s_f[row] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2;
+      uint32_t* to = reinterpret_cast<uint32_t*>(s_q) + ((qc >> 3) * 4 + (qc & 1) * 2) * 128 + ((row & 7) * 4 + ((qc >> 1) & 3)) * 4 + (row >> 3);
+      to[0] = x[0];
+      to[2] = x[1];
+      to[128] = x[2];
+      to[130] = x[3];
+    }
   };
 
   // ---- the first unit of this warp is on its way before anything else. Pages are looked up one unit ahead of the copies, so that these do not wait for them.
@@ -236,64 +352,27 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
     np.forward(a, WARPS);
     pages = next + WARPS < todo ? unit_page(a, np, lane) : -1;
   };
-  uint4 queries = load_q(cur);
+  load_q(cur);
   take();
   fetch<D, false>(a, unit, kbuf, lane);
   copy_commit();
   fetch<D, true>(a, unit, vbuf, lane);
   copy_commit();
-  store_q(queries, 0);
+  store_q();
   __syncthreads();
 
   int seg0 = 0;                                             // index in the stretch of the segment's first unit
-  for (int seg = 0; seg0 < todo; ++seg) {
+  while (seg0 < todo) {
     const int seg_n = min(cur.r.units - cur.u, todo - seg0);
-    Place after = cur;
-    after.forward(a, seg_n);
-    const bool more = seg0 + seg_n < todo;
-    if (more) queries = load_q(after);                      // the next segment's queries, on their way beside this one's work
-
     const int tile = cur.tile, g = cur.g;
-    // ---- queries into registers; bfloat16 rows by a power of two each
-    uint32_t qa[KS][4];
-    float rowf[2];
+    const uint32_t frag = shared_addr(s_q) + lane * 16;
+    auto query = [&](uint32_t (&x)[4], int step) {
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(frag + step * 512));
+    };
+    const float rowf[2] = {s_f[qi], s_f[qi + 8]};
     int limit[2];                                           // last visible position of this lane's rows
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const unsigned char* row = s_q + ((seg & 1) * ROWS + qi + 8 * e) * D * 2;
-      uint32_t x[CH / 4][8];
-#pragma unroll
-      for (int h = 0; h < CH / 4; ++h) {
-        const uint4 w0 = *reinterpret_cast<const uint4*>(row + (h * 4 + qj) * 32), w1 = *reinterpret_cast<const uint4*>(row + (h * 4 + qj) * 32 + 16);
-        x[h][0] = w0.x; x[h][1] = w0.y; x[h][2] = w0.z; x[h][3] = w0.w;
-        x[h][4] = w1.x; x[h][5] = w1.y; x[h][6] = w1.z; x[h][7] = w1.w;
-      }
-      int sh = 0;
-      if (BF16) {
-        float mx = 0.f;
-#pragma unroll
-        for (int h = 0; h < CH / 4; ++h)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[h][i] << 16)), fabsf(__uint_as_float(x[h][i] & 0xffff0000u))));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // 2^(14 - exponent of the largest), from its bits; none for a row of zeros or one that is not finite, and in float32's range at both ends
-        const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
-        sh = mx > 0.f && mx < INFINITY ? min(max(14 - ex, -126), 126) : 0;
-        const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
-#pragma unroll
-        for (int h = 0; h < CH / 4; ++h)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[h][i] = half_pair(__uint_as_float(x[h][i] << 16) * up, __uint_as_float(x[h][i] & 0xffff0000u) * up);
-      }
-      rowf[e] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2;
-#pragma unroll
-      for (int h = 0; h < CH / 4; ++h)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          qa[h * 4 + w][e] = x[h][2 * w];
-          qa[h * 4 + w][e + 2] = x[h][2 * w + 1];
-        }
       const int tok = (tile * ROWS + qi + 8 * e) / a.rep;
       limit[e] = tok < cur.r.n ? min(cur.r.keys - cur.r.n + tok, cur.r.keys - 1) : -1;
     }
@@ -301,39 +380,41 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
     // What the codes' 128 adds to a row's scores, the other way round: -128 (in units of 2^-24) times the sum of the row.
     float s0[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < KS; ++i) mma16816(s0, qa[i], 0x80808080u, 0x80808080u);
+    for (int i = 0; i < CH; ++i) {
+      uint32_t x[4];
+      query(x, i);
+      mma16816(s0, x, MINUS_128, MINUS_128, s0);
+    }
     float o[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
     float m[2] = {NONE, NONE}, l[2] = {0.f, 0.f};
 
     while (next < seg0 + seg_n) {
-      // ---- scores of 64 keys, in units of 2^-24
+      // ---- scores of the unit's keys, in units of 2^-24
       const int key0 = unit.key0;
       const float cks = pks, cvs = pvs;
       copy_wait<1>();
       __syncwarp();
-      float s[8][4];
+      float s[KT][4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[4][CH / 4][4];
+      for (int h = 0; h < CH / 4; ++h) {
+        uint32_t w[KT][4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < KT; ++n)
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[n][0]), "=r"(w[n][1]), "=r"(w[n][2]), "=r"(w[n][3])
+                       : "r"(kbuf + k_chunk<D>((n >> 1) * 16 + (n & 1) * 2 + (qi >> 1) * 4 + (qi & 1), h * 4 + qj)));
 #pragma unroll
-          for (int h = 0; h < CH / 4; ++h)
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[n][h][0]), "=r"(w[n][h][1]), "=r"(w[n][h][2]), "=r"(w[n][h][3])
-                         : "r"(kbuf + k_chunk<D>((half * 4 + n) * 8 + qi, h * 4 + qj)));
+        for (int i = 0; i < 4; ++i) {
+          uint32_t x[4];
+          query(x, h * 4 + i);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) { s[half * 4 + n][0] = s0[0]; s[half * 4 + n][1] = s0[0]; s[half * 4 + n][2] = s0[2]; s[half * 4 + n][3] = s0[2]; }
-#pragma unroll
-        for (int h = 0; h < CH / 4; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const uint32_t u = w[n][h][i] ^ 0x80808080u;
-              mma16816(s[half * 4 + n], qa[h * 4 + i], codes_tiny(u, 0x4140), codes_tiny(u, 0x4342));
-            }
+          for (int n = 0; n < KT; ++n) {
+            const uint32_t u = w[n][i] ^ 0x80808080u;
+            if (h == 0 && i == 0) mma16816(s[n], x, first_two(u), last_two(u), s0);
+            else mma16816(s[n], x, first_two(u), last_two(u), s[n]);
+          }
+        }
       }
       __syncwarp();
       // the next unit's keys take this one's place
@@ -346,20 +427,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
       const bool odd = __any_sync(0xffffffffu, cks != cks || cvs != cvs);
       if (key0 + UNIT - 1 > low || odd) {
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt) {
-          const int src = (8 * nt) >> a.pshift;
+        for (int nt = 0; nt < KT; ++nt) {
+          const int src = (16 * (nt >> 1)) >> a.pshift;
           const float both = __shfl_sync(0xffffffffu, cks + cvs, src);
           const bool none = both != both;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if (none) s[nt][e] = NAN;
-            if (key0 + nt * 8 + qj * 2 + (e & 1) > limit[e >> 1]) s[nt][e] = NONE;
+            if (key0 + (nt >> 1) * 16 + qj * 4 + (nt & 1) * 2 + (e & 1) > limit[e >> 1]) s[nt][e] = NONE;
           }
         }
       }
-      float kf[4][2], lv[4], iv[4], mx[2] = {NONE, NONE};   // of 16 keys each: factor of the scores, log2 of the value scale and its reciprocal
+      float kf[QT][2], lv[QT], iv[QT], mx[2] = {NONE, NONE};   // of 16 keys each: factor of the scores, log2 of the value scale and its reciprocal
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < QT; ++q) {
         const int src = (16 * q) >> a.pshift;
         const float f = positive(__shfl_sync(0xffffffffu, cks, src)) * 16777216.f, v = positive(__shfl_sync(0xffffffffu, cvs, src));
         lv[q] = __log2f(v);
@@ -393,15 +474,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
       // Exponents are taken from the products without a rounding in between, the reference has one: beyond 2^24 that alone would be a large exponent.
       if (__any_sync(0xffffffffu, fabsf(ref[0]) > 16777216.f || fabsf(ref[1]) > 16777216.f)) {
 #pragma unroll
-        for (int nt = 0; nt < 8; ++nt)
+        for (int nt = 0; nt < KT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[nt][e] = fmaf(s[nt][e], kf[nt >> 1][e >> 1], lv[nt >> 1]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) { kf[q][0] = kf[q][1] = 1.f; lv[q] = 0.f; }
+        for (int q = 0; q < QT; ++q) { kf[q][0] = kf[q][1] = 1.f; lv[q] = 0.f; }
       }
-      uint32_t pa[4][4];
+      uint32_t pa[QT][4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < QT; ++q) {
         const float at[2] = {lv[q] - ref[0], lv[q] - ref[1]};
         float part[2] = {0.f, 0.f};
 #pragma unroll
@@ -422,36 +503,27 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
       copy_wait<1>();
       __syncwarp();
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        constexpr int W = D / 32;                           // 32-bit words of a lane's columns of a row
-        uint32_t r[4][W];
+      for (int c = 0; c < CH; c += 2)                       // 32 columns at a time
 #pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const int row = q * 16 + qj * 2 + (z & 1) + (z >> 1) * 8;
-          if constexpr (D == 128)
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[z][0]), "=r"(r[z][1]), "=r"(r[z][W - 2]), "=r"(r[z][W - 1]) : "r"(vbuf + v_chunk<D>(row, qi)));
-          else
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(r[z][0]), "=r"(r[z][1]) : "r"(vbuf + v_chunk<D>(row, qi >> 1) + (qi & 1) * 8));
+        for (int q = 0; q < QT; ++q) {
+          uint32_t w[4];
+          load_columns(w, vbuf + v_chunk<D>(q * 16 + (lane & 15), c + (lane >> 4)));
 #pragma unroll
-          for (int w = 0; w < W; ++w) r[z][w] ^= 0x80808080u;
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t u = w[t] ^ 0x80808080u;
+            mma16816(o[2 * c + t], pa[q], exact_two(u, 0x4140), exact_two(u, 0x4342), o[2 * c + t]);
+          }
         }
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const uint32_t x0 = __byte_perm(r[0][w], r[1][w], 0x5140), y0 = __byte_perm(r[0][w], r[1][w], 0x7362);
-          const uint32_t x1 = __byte_perm(r[2][w], r[3][w], 0x5140), y1 = __byte_perm(r[2][w], r[3][w], 0x7362);
-          mma16816(o[4 * w], pa[q], codes16(x0, 0x4140), codes16(x1, 0x4140));
-          mma16816(o[4 * w + 1], pa[q], codes16(x0, 0x4342), codes16(x1, 0x4342));
-          mma16816(o[4 * w + 2], pa[q], codes16(y0, 0x4140), codes16(y1, 0x4140));
-          mma16816(o[4 * w + 3], pa[q], codes16(y0, 0x4342), codes16(y1, 0x4342));
-        }
-      }
       __syncwarp();
       fetch<D, true>(a, unit, vbuf, lane);
       copy_commit();
     }
 
-    if (more) store_q(queries, (seg + 1) & 1);              // (the last that read them has passed two barriers)
-    // ---- the warps' sums of this item together. Column order on the way: [half of a lane's columns][t / 4][lane of the quad][t % 4].
+    Place after = cur;
+    after.forward(a, seg_n);
+    const bool more = seg0 + seg_n < todo;
+    if (more) load_q(after);                                // the next segment's queries, on their way while sums are joined
+    // ---- the warps' sums of this item together
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
@@ -462,17 +534,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
       }
       // (a warp without a unit in this segment has nothing but its maximum to tell)
       if (m[e] != NONE || l[e] != 0.f) {
-        float* row = s_o + (warp * ROWS + qi + 8 * e) * O_LD + qj * 4;
+        float* row = s_o + (warp * ROWS + qi + 8 * e) * S::LD + qj * 2;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int t = 0; t < NT / 4; ++t)
-            *reinterpret_cast<float4*>(row + (c * (NT / 4) + t) * 16) = make_float4(o[4 * t][2 * e + c], o[4 * t + 1][2 * e + c], o[4 * t + 2][2 * e + c], o[4 * t + 3][2 * e + c]);
+        for (int t = 0; t < NT; ++t) *reinterpret_cast<float2*>(row + 8 * t) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
       }
     }
     __syncthreads();
-    constexpr int PIECES = D / 64;                          // float4 of a thread: 16 threads a row
-    const int jr = tid >> 4, col = tid & 15;
+    constexpr int PER_ROW = THREADS / ROWS, PIECES = D / 4 / PER_ROW;   // threads of a row, float4 of a thread
+    const int jr = tid / PER_ROW, col = tid % PER_ROW;
     float mm = NONE, ll = 0.f;
     float4 oo[PIECES];
 #pragma unroll
@@ -490,58 +559,98 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
       }
     };
     for (int w = 0; w < WARPS; ++w)
-      join(s_ml[(w * 2) * ROWS + jr], s_ml[(w * 2 + 1) * ROWS + jr], [&](int c) { return *reinterpret_cast<const float4*>(s_o + (w * ROWS + jr) * O_LD + (col + 16 * c) * 4); });
-    const int rr = tile * ROWS + jr, tok = rr / a.rep;
-    auto store = [&]() {
-      if (tok >= cur.r.n) return;
-      const float f = ll == 0.f ? 0.f : __fdiv_rn(1.f, ll);  // no key: zeros
-      T* to = (T*)a.out + (size_t)(cur.r.first + tok) * a.out_ts + (size_t)(g * a.rep + rr - tok * a.rep) * a.out_hs;
-#pragma unroll
-      for (int c = 0; c < PIECES; ++c) {
-        const int at = col + 16 * c, q = at >> 2, half = q / (NT / 4), t = q % (NT / 4) * 4, j = at & 3;
-        const float4 p = oo[c];
-        uint2 w;
-        if (BF16) {
-          const __nv_bfloat162 x = __floats2bfloat162_rn(p.x * f, p.y * f), y = __floats2bfloat162_rn(p.z * f, p.w * f);
-          w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-        } else {
-          w = make_uint2(half_pair(p.x * f, p.y * f), half_pair(p.z * f, p.w * f));
-        }
-        *reinterpret_cast<uint2*>(to + (2 * j + half) * NT + t) = w;
+      join(s_ml[(w * 2) * ROWS + jr], s_ml[(w * 2 + 1) * ROWS + jr], [&](int c) { return *reinterpret_cast<const float4*>(s_o + (w * ROWS + jr) * S::LD + (col + PER_ROW * c) * 4); });
+    auto store_piece = [&](int r, int at, const float4& p, float f) {   // columns at .. at + 3 of the tile's row r
+      const int rr = tile * ROWS + r, tok = rr / a.rep;
+      uint2 w;
+      if (BF16) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(p.x * f, p.y * f), y = __floats2bfloat162_rn(p.z * f, p.w * f);
+        w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+      } else {
+        w = make_uint2(half_pair(p.x * f, p.y * f), half_pair(p.z * f, p.w * f));
       }
+      *reinterpret_cast<uint2*>((T*)a.out + (size_t)(cur.r.first + tok) * a.out_ts + (size_t)(g * a.rep + rr - tok * a.rep) * a.out_hs + at) = w;
     };
     const bool starts = cur.u == 0, ends = cur.u + seg_n == cur.r.units;
     if (starts && ends) {
-      store();
+      if (tile * ROWS + jr < cur.r.n * a.rep) {
+        const float f = ll == 0.f ? 0.f : __fdiv_rn(1.f, ll);   // (no key: zeros)
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) store_piece(jr, (col + PER_ROW * c) * 4, oo[c], f);
+      }
     } else {
       // ---- a part of an item: into the workspace; the item's last CTA to come adds all of them up, first part first
       const long long item0 = begin + seg0 - cur.u, item1 = item0 + cur.r.units;
-      const int c0 = (int)(item0 / per), c1 = (int)((item1 - 1) / per);
+      const int c0 = whole ? (int)blockIdx.x - cur.u / share : (int)(item0 / per), c1 = whole ? c0 + (cur.r.units - 1) / share : (int)((item1 - 1) / per);
       float* part = a.parts + (size_t)(2 * blockIdx.x + (starts ? 1 : 0)) * PART<D>;
       if (col == 0) { part[jr] = mm; part[ROWS + jr] = ll; }
 #pragma unroll
-      for (int c = 0; c < PIECES; ++c) *reinterpret_cast<float4*>(part + 2 * ROWS + jr * D + (col + 16 * c) * 4) = oo[c];
-      __threadfence();
+      for (int c = 0; c < PIECES; ++c) *reinterpret_cast<float4*>(part + 2 * ROWS + jr * D + (col + PER_ROW * c) * 4) = oo[c];
       __syncthreads();
       if (tid == 0) {
+        __threadfence();                                    // (of what the whole CTA has stored: the barrier is in front of it)
         const int n = c1 - c0 + 1, old = atomicAdd(a.counters + c0, 1);
         s_last = old == n - 1;
         if (old == n - 1) a.counters[c0] = 0;               // for the next call
       }
       __syncthreads();
       if (s_last) {
+        // All maxima and sums first (eight threads a row), which gives every part its factor, then the sums of values: loads that wait for none before them.
         __threadfence();
+        const int n = c1 - c0 + 1;
+        auto from = [&](int i) { return a.parts + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * PART<D>; };
+        float* const factor = s_o;                          // [part][row]: the sums on their way between warps have been read
         mm = NONE;
         ll = 0.f;
+        for (int i0 = col; i0 < n; i0 += 8 * PER_ROW) {
+          float mp[8], lp[8];
 #pragma unroll
-        for (int c = 0; c < PIECES; ++c) oo[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p = c0; p <= c1; ++p) {
-          const float* from = a.parts + (size_t)(2 * p + (p == c0 ? 1 : 0)) * PART<D>;
-          join(__ldcg(from + jr), __ldcg(from + ROWS + jr), [&](int c) { return __ldcg(reinterpret_cast<const float4*>(from + 2 * ROWS + jr * D + (col + 16 * c) * 4)); });
+          for (int k = 0; k < 8; ++k) {
+            const int i = i0 + k * PER_ROW;
+            mp[k] = i < n ? __ldcg(from(i) + jr) : NONE;
+            lp[k] = i < n ? __ldcg(from(i) + ROWS + jr) : 0.f;
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const bool none = mp[k] == NONE;                // nothing seen, or (a sum that is not zero) no number
+            const float mn = fmaxf(mm, mp[k]);
+            ll = (mm == NONE ? ll : ll * exp2_fast(mm - mn)) + (none ? lp[k] : lp[k] * exp2_fast(mp[k] - mn));
+            mm = mn;
+            if (i0 + k * PER_ROW < n) factor[(i0 + k * PER_ROW) * ROWS + jr] = none && lp[k] != 0.f ? INFINITY : mp[k];
+          }
         }
-        store();
+        const float own = mm;
+#pragma unroll
+        for (int x = PER_ROW / 2; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+        if (own != NONE) ll *= exp2_fast(own - mm);
+#pragma unroll
+        for (int x = PER_ROW / 2; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
+        for (int i = col; i < n; i += PER_ROW) {
+          const float f = factor[i * ROWS + jr];
+          factor[i * ROWS + jr] = f == NONE ? 0.f : f == INFINITY ? 1.f : exp2_fast(f - mm);
+        }
+        if (col == 0) factor[n * ROWS + jr] = ll == 0.f ? 0.f : __fdiv_rn(1.f, ll);   // (no key: zeros)
+        __syncthreads();
+        const int rows = min(cur.r.n * a.rep - tile * ROWS, ROWS);
+        for (int x = tid; x < rows * (D / 4); x += THREADS) {
+          const int r = x / (D / 4), at = x % (D / 4) * 4;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int i0 = 0; i0 < n; i0 += 32) {
+            float4 v[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              v[k] = i0 + k < n ? __ldcg(reinterpret_cast<const float4*>(from(i0 + k) + 2 * ROWS + r * D + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float f = i0 + k < n ? factor[(i0 + k) * ROWS + r] : 0.f;
+              sum.x = fmaf(v[k].x, f, sum.x); sum.y = fmaf(v[k].y, f, sum.y); sum.z = fmaf(v[k].z, f, sum.z); sum.w = fmaf(v[k].w, f, sum.w);
+            }
+          }
+          store_piece(r, at, sum, factor[n * ROWS + r]);
+        }
       }
     }
+    if (more) store_q();                                    // (all have passed the barrier behind their last use of this item's)
     cur = after;
     seg0 += seg_n;
     __syncthreads();                                        // the sums have been read, the next queries are there
@@ -555,7 +664,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_kernel(const AttArgs
 using namespace qspec;
 using namespace qspec::kv8;
 
-static int att_grid() { return max(sm_count(), 1); }
+static int att_grid() { return max(sm_count(), 1) * CTAS; }
 
 extern "C" size_t qspec_kv8_attention_workspace_bytes(void) { return 4096 + (size_t)att_grid() * 2 * PART<128> * sizeof(float); }
 
@@ -578,7 +687,7 @@ extern "C" int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_
   QSPEC_REQUIRE(workspace && workspace_bytes >= qspec_kv8_attention_workspace_bytes() && ((uintptr_t)workspace & 15) == 0, QSPEC_ERR_WORKSPACE,
                 "kv8_attention: %zu bytes of workspace needed, got %zu", qspec_kv8_attention_workspace_bytes(), workspace_bytes);
   const int grid = att_grid();
-  QSPEC_REQUIRE(grid <= 1024, QSPEC_ERR_UNSUPPORTED, "kv8_attention: %d SMs", grid);
+  QSPEC_REQUIRE(grid <= GRID_MOST, QSPEC_ERR_UNSUPPORTED, "kv8_attention: %d SMs", grid);
   AttArgs a{q, q_tok_stride, q_head_stride, (const signed char*)k, (const signed char*)v, ks, vs, table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok,
             G, H / G, 0x7fffffff, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)};
   auto run = [&](auto kern, size_t smem, SmemLimit& limit) -> int {

@@ -294,7 +294,8 @@ def attention_in_64_bits(q, k, v, ks, vs, table, start, lens, scale):
     Weights are rounded to float16: 2^-11 relative, or 2^-25 absolute where the largest weight * value scale of a row is 1 (below float16's
     normal range). A score is a sum of D exact products in float32 (at most 2^-23 of the sum of their sizes for each addition in the tensor cores,
     which cut), times factors (3 roundings), and enters the exponential, whose own error and that of log2 of the scale are below 2^-20; sums of
-    values and weights in float32 add 2^-23 a key at most."""
+    values and weights in float32 add 2^-23 a key at most. Codes c of keys enter the products as c + 128, and the 128 is taken out by where a sum begins:
+    D / 8 products of 16 terms, no partial sum of which is above 255 sum |q| (in units of the key's scale), each term cut at 2^-24 of that."""
     T, H, D = q.shape
     P, G = k.shape[2], k.shape[1]
     rep = H // G
@@ -317,7 +318,8 @@ def attention_in_64_bits(q, k, v, ks, vs, table, start, lens, scale):
                 total = w.sum(1, keepdim=True)
                 o = w @ vv / total.clamp(min=1e-300)
                 size = w @ vv.abs() / total.clamp(min=1e-300)
-                ds = ((x.abs() @ kk.abs().T) * scale * ((D + 4) * 2.0 ** -23) + 2.0 ** -20).masked_fill(hidden, 0.0).amax(1, keepdim=True)
+                carried = x.abs().sum(1, keepdim=True) * 255 * fk[None] * (D // 8 * 17 * 2.0 ** -24)
+                ds = (((x.abs() @ kk.abs().T) * ((D + 4) * 2.0 ** -23) + carried) * scale + 2.0 ** -20).masked_fill(hidden, 0.0).amax(1, keepdim=True)
                 top = (w * fv[None]).amax(1, keepdim=True)
                 small = n * 2.0 ** -25 * 127 * top / total.clamp(min=1e-300)
                 out[lo:hi, h] = torch.where(some[:, None], o, 0.0)
