@@ -63,7 +63,7 @@ def _ptr(t: Optional[torch.Tensor]):
 
 _I4 = (torch.int8, torch.uint8)
 
-# csrc/fast_call.cpp: the linear layers' calls without the Python below them. It takes what the functions here take without an error and
+# csrc/fast_call.cpp: the calls of the linear layers and of the paged 8-bit cache's operators without the Python below them. It takes what the functions here take without an error and
 # returns None for everything else, which then goes the ordinary way (and so does everything where it has not been built for this Python and torch).
 _fast = False                                             # loaded by the first call: False before it, None where there is none
 _addresses: dict = {}
@@ -806,6 +806,20 @@ def _i32(t: torch.Tensor, name: str, *shape: int) -> None:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
 
 
+def _fast_call(name: str, *args) -> bool:
+    """True: csrc/fast_call.cpp has made the call (it takes what the function below takes without an error)."""
+    fast = _load_fast() if _fast is False else _fast
+    fn = getattr(fast, name, None)
+    if fn is None:
+        return False
+    status = fn(_address("qspec_" + name), *args)
+    if status is None:
+        return False
+    if status:
+        _lib.check(status, name)
+    return True
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
 
@@ -817,6 +831,8 @@ def page_plan(lengths: torch.Tensor, counts: torch.Tensor, table: torch.Tensor, 
     pages) describe the cache; q_start [B + 1], kv_len [B], positions / seq_ids / slots [tokens] and state_out [B + 2] (the state behind the step, number
     of requests refused) are written. `state` and what it describes stay as they are until the caller copies state_out over it, so that a
     step can be planned again. Who gets which pages, and who none: include/qspec_b200.h."""
+    if _fast_call("page_plan", lengths, counts, table, free_pages, state, page_tokens, q_start, kv_len, positions, seq_ids, slots, state_out):
+        return
     if lengths.dim() != 1 or table.dim() != 2 or free_pages.dim() != 1 or positions.dim() != 1:
         raise ValueError("page_plan: lengths [B], table [B, W], free_pages [pages], positions [tokens]")
     B, T = lengths.shape[0], positions.shape[0]
@@ -847,6 +863,8 @@ def kv8_append(qkv: torch.Tensor, cos_sin_cache: torch.Tensor, positions: torch.
     into the pages of their slots: codes int8 [pages, G, P, D], scales float32 [pages, G]. q_out [T, H, D] receives the rotated queries (None: they
     are not wanted). A page's scale grows with its rows and its older rows follow; it starts anew when its first row is written. Tokens without
     a slot (negative) are skipped. The tokens of a page must be neighbours in the batch."""
+    if _fast_call("kv8_append", qkv, cos_sin_cache, positions, slots, k_codes, v_codes, k_scale, v_scale, q_out):
+        return
     n, G, P, D = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
     if not qkv.is_cuda or qkv.dtype not in (_F16, _BF16) or qkv.dim() != 2 or qkv.stride(1) != 1:
         raise ValueError("kv8_append: qkv must be a float16 / bfloat16 CUDA tensor [T, (H + 2 G) D] with unit column stride")
@@ -872,6 +890,8 @@ def kv8_append(qkv: torch.Tensor, cos_sin_cache: torch.Tensor, positions: torch.
 def kv8_read(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor,
              v_out: torch.Tensor) -> None:
     """Rows of the 8-bit cache as 16-bit values: k_out, v_out [N, G, D] (float16 / bfloat16) of slots int32 [N]; zeros for a slot outside the cache."""
+    if _fast_call("kv8_read", k_codes, v_codes, k_scale, v_scale, slots, k_out, v_out):
+        return
     n, G, P, D = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
     _chk(k_out, "k_out", (_F16, _BF16)); _chk(v_out, "v_out", (k_out.dtype,))
     _i32(slots, "slots", slots.numel())
@@ -898,6 +918,8 @@ def kv8_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
     q_start[b + 1] - 1 are request b's last of kv_len[b], and see its keys up to their own. table int32 [B, W]. out [T, H, D] of q's type; rows that see no
     key are zeros, rows behind q_start[B] are left as they are. max_tokens: an upper bound of the tokens that a request has in the step (T if not
     given); a request with more than that is not attended to. workspace: `kv8_attention_workspace`."""
+    if _fast_call("kv8_attention", q, k_codes, v_codes, k_scale, v_scale, table, q_start, kv_len, out, sm_scale, workspace, max_tokens):
+        return out
     n, G, P, D = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
     for t, name in ((q, "q"), (out, "out")):
         if not t.is_cuda or t.dtype not in (_F16, _BF16) or t.dim() != 3 or t.shape[2] != D or t.stride(2) != 1:
@@ -936,6 +958,8 @@ def verify_drafts(drafted: Optional[torch.Tensor], draft_probs: Optional[torch.T
     with probability min(1, p / q); behind the taken ones comes one token from what the target has over the draft, or from the target where all were
     taken. draft_counts int32 [B]: how many of its k drafts each request has (None: all). drafted and draft_probs None: no drafts, one token is drawn from
     every row of target_probs [B, 1, V]. (vllm/model_executor/layers/rejection_sampler.py)"""
+    if _fast_call("verify_drafts", drafted, draft_probs, target_probs, uniform, tokens, emitted, draft_counts):
+        return
     if target_probs.dim() != 3:
         raise ValueError("verify_drafts: target_probs must be [B, k + 1, V]")
     B, k, V = target_probs.shape[0], target_probs.shape[1] - 1, target_probs.shape[2]
