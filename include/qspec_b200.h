@@ -402,7 +402,8 @@ int qspec_kv8_read(const void* k, const void* v, const float* k_scale, const flo
 
 /* Softmax attention of a step's tokens over that cache. q [ntok, H, D] with free token / head strides; the tokens q_start[b] .. q_start[b + 1] - 1 of
  * request b stand at the last positions of its kv_len[b] tokens and see the keys up to their own. Tokens that see no key give zeros; tokens
- * behind q_start[requests] are not written. max_tokens: an upper bound of the tokens that any request has in the step. Scales are positive (a scale
+ * behind q_start[requests] are not written. max_tokens: an upper bound of the tokens that any request has in the step (it decides which
+ * forms are launched; a request with more is attended to as well, more slowly). Scales are positive (a scale
  * below 2^-100 counts as that); pages outside the cache make the rows that see them NaN. workspace: zero-initialised once, left ready for the next call;
  * one for each stream that calls are made on at the same time. */
 size_t qspec_kv8_attention_workspace_bytes(void);
@@ -410,6 +411,12 @@ int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_head_stride
                         const int* table, const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests,
                         int width, int H, int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace,
                         size_t workspace_bytes, void* stream);
+
+/* For tests: the roles of the prompt form's pipeline in the mask give_up (1 softmax, 2 codes, 4 products, 8 pages) give their first wait up at once. */
+int qspec_debug_kv8_attention_give_up(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* k_scale, const float* v_scale,
+                                      const int* table, const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok,
+                                      int requests, int width, int H, int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype,
+                                      void* workspace, size_t workspace_bytes, unsigned give_up, void* stream);
 
 /* Verification of drafted tokens, and one token more. drafted int64 [requests, drafts]; draft / target float32 probabilities, row of (request b, place i) at
  * b * seq_stride + i * place_stride, `drafts` and drafts + 1 places; uniform float32 [requests, drafts + 1] in [0, 1); draft_counts (NULL: all) int32: how

@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_C")
 LIB_PATH = os.path.join(OUT_DIR, "libqspec_b200.so")
 SOURCES = ["capi.cu", "act_kernels.cu", "hadamard_kernels.cu", "gemm_w4_stream.cu", "attn_kernels.cu", "qwen_kernels.cu", "kv8_kernels.cu",
-           "kv8_attention.cu", "spec_kernels.cu"]
+           "kv8_attention.cu", "kv8_prompt.cu", "spec_kernels.cu"]
 # The sequence-mixer kernels (include/qspec_b200_seq.h) are a library of their own, so that a model that needs only them
 # builds only them: libqspec_b200_seq.so.
 SEQ_SOURCES = ["capi.cu", "seq_kernels.cu", "seq_mma_kernels.cu", "seq_mix_kernels.cu", "seq_state_kernels.cu", "seq_head_kernels.cu",

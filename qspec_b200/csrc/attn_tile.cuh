@@ -116,7 +116,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
   return false;
 }
 // For what is under way at the end: waits, as long as any wait, whether or not the CTA has given up.
-__device__ __noinline__ void bar_drain(uint32_t bar, uint32_t parity) {
+static __device__ __noinline__ void bar_drain(uint32_t bar, uint32_t parity) {
   int none = 0;
   bar_wait(bar, parity, &none);
 }

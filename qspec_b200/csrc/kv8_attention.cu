@@ -71,19 +71,10 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void load_columns(uint32_t (&w)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
 }
-// a scale; one that is zero or next to nothing, or no number, counts as 2^-100
-__device__ __forceinline__ float positive(float x) { return x >= 7.888609052210118e-31f ? x : 7.888609052210118e-31f; }
 // The first two / the last two of four codes (bytes c + 128) as float16: a byte alone is (c + 128) 2^-24, a subnormal number.
 __device__ __forceinline__ uint32_t first_two(uint32_t w) { return __byte_perm(w, 0u, 0x4140); }
 __device__ __forceinline__ uint32_t last_two(uint32_t w) { return __byte_perm(w, 0u, 0x4342); }
 constexpr uint32_t MINUS_128 = 0x80808080u;      // two of -128 2^-24: what the codes' 128 adds up to, the other way round
-// The same as c, exactly: a byte behind 0x64 is 1152 + c.
-__device__ __forceinline__ uint32_t exact_two(uint32_t w, uint32_t sel) {
-  const uint32_t m = __byte_perm(w, 0x64646464u, sel);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t half_pair(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 
 // A request's part of the work.
 struct Req {
@@ -447,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
         iv[q] = __fdividef(1.f, v);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          kf[q][e] = f * rowf[e];
+          kf[q][e] = normal(f * rowf[e]);
           const float top = fmaxf(fmaxf(s[2 * q][2 * e], s[2 * q][2 * e + 1]), fmaxf(s[2 * q + 1][2 * e], s[2 * q + 1][2 * e + 1]));
           mx[e] = fmaxf(mx[e], fmaf(top, kf[q][e], lv[q])); // (factors are positive: the largest score has the largest exponent)
         }
@@ -668,9 +659,12 @@ static int att_grid() { return max(sm_count(), 1) * CTAS; }
 
 extern "C" size_t qspec_kv8_attention_workspace_bytes(void) { return 4096 + (size_t)att_grid() * 2 * PART<128> * sizeof(float); }
 
-extern "C" int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* ks, const float* vs, const int* table,
-                                   const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H,
-                                   int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+// Rows (tokens * heads of a group) from which a request goes to the prompt form.
+constexpr int PROMPT_ROWS = 65;
+
+static int attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* ks, const float* vs, const int* table, const int* q_start,
+                     const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H, int G, int D, int npages,
+                     int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, unsigned give_up, void* stream) {
   QSPEC_REQUIRE(k && v && ks && vs && table && q_start && kv_len, QSPEC_ERR_INVALID_ARG, "kv8_attention: null pointer");
   QSPEC_REQUIRE(page_shift(page_tokens) > 0, QSPEC_ERR_UNSUPPORTED, "kv8_attention: pages of 16, 32, 64 or 128 tokens, got %d", page_tokens);
   QSPEC_REQUIRE(D == 64 || D == 128, QSPEC_ERR_UNSUPPORTED, "kv8_attention: heads of 64 or 128, got %d", D);
@@ -687,9 +681,17 @@ extern "C" int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_
   QSPEC_REQUIRE(workspace && workspace_bytes >= qspec_kv8_attention_workspace_bytes() && ((uintptr_t)workspace & 15) == 0, QSPEC_ERR_WORKSPACE,
                 "kv8_attention: %zu bytes of workspace needed, got %zu", qspec_kv8_attention_workspace_bytes(), workspace_bytes);
   const int grid = att_grid();
-  QSPEC_REQUIRE(grid <= GRID_MOST, QSPEC_ERR_UNSUPPORTED, "kv8_attention: %d SMs", grid);
+  QSPEC_REQUIRE(grid <= GRID_MOST, QSPEC_ERR_UNSUPPORTED, "kv8_attention: %d SMs", sm_count());
+  // Requests with more rows than this kernel takes in few tiles go to the prompt form, in a launch of its own in front.
+  const int rep = H / G;
+  const bool prompts = rep <= PROMPT_REP && (long long)max_tokens * rep >= PROMPT_ROWS;
+  if (prompts) {
+    const PromptArgs pa{q, q_tok_stride, q_head_stride, (const signed char*)k, (const signed char*)v, ks, vs, table, q_start, kv_len, requests, width, npages,
+                        page_shift(page_tokens), ntok, G, rep, PROMPT_ROWS, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, give_up};
+    if (const int rc = launch_prompt(pa, D, dtype == QSPEC_DTYPE_BF16, (cudaStream_t)stream)) return rc;
+  }
   AttArgs a{q, q_tok_stride, q_head_stride, (const signed char*)k, (const signed char*)v, ks, vs, table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok,
-            G, H / G, 0x7fffffff, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)};
+            G, rep, prompts ? PROMPT_ROWS - 1 : 0x7fffffff, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)};
   auto run = [&](auto kern, size_t smem, SmemLimit& limit) -> int {
     QSPEC_CUDA(limit.raise(kern, smem));
     QSPEC_CUDA(launch_pdl(kern, dim3(grid), dim3(THREADS), smem, (cudaStream_t)stream, a));
@@ -700,4 +702,18 @@ extern "C" int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_
   if (dtype == QSPEC_DTYPE_F16)
     return D == 128 ? run(kv8_attention_kernel<false, 128>, Smem<128>::TOTAL, limits[0]) : run(kv8_attention_kernel<false, 64>, Smem<64>::TOTAL, limits[1]);
   return D == 128 ? run(kv8_attention_kernel<true, 128>, Smem<128>::TOTAL, limits[2]) : run(kv8_attention_kernel<true, 64>, Smem<64>::TOTAL, limits[3]);
+}
+
+extern "C" int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* ks, const float* vs, const int* table,
+                                   const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H,
+                                   int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return attention(q, q_tok_stride, q_head_stride, k, v, ks, vs, table, q_start, kv_len, out, out_tok_stride, out_head_stride, ntok, requests, width, H, G, D, npages, page_tokens,
+                   max_tokens, scale, dtype, workspace, workspace_bytes, 0, stream);
+}
+extern "C" int qspec_debug_kv8_attention_give_up(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* ks, const float* vs,
+                                                 const int* table, const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok,
+                                                 int requests, int width, int H, int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype,
+                                                 void* workspace, size_t workspace_bytes, unsigned give_up, void* stream) {
+  return attention(q, q_tok_stride, q_head_stride, k, v, ks, vs, table, q_start, kv_len, out, out_tok_stride, out_head_stride, ntok, requests, width, H, G, D, npages, page_tokens,
+                   max_tokens, scale, dtype, workspace, workspace_bytes, give_up, stream);
 }

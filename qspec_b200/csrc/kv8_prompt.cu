@@ -1,0 +1,530 @@
+// Softmax attention of prompt portions over the paged 8-bit cache, on the fifth-generation tensor cores (kv8_attention.cu has the layout, and the form for requests
+// with few tokens).
+//
+// One CTA = 128 rows of one request and key/value head; a row is a (token, query head of the group) pair. Keys are walked in blocks of 128:
+//   * pages: one warp looks the block's pages and scales up and leaves where the codes are and what their products are multiplied with.
+//   * codes: four warps bring a block's keys and values from global memory, make them float16 (a byte c + 128 behind 0x64 is 1152 + c, less 1152; exact)
+//     and store them as the tensor cores want them: the cache is read once, in 8 bits, and is never anywhere in 16.
+//   * S = Q K^T, accumulator [128 x 128] float32 in tensor memory, two of them: the next block's scores are computed under this block's softmax.
+//   * softmax: thread = half a row (64 columns), two warps per 32 rows, which exchange the row's maximum through shared memory. Weights go back over the
+//     scores as float16 (2^-11 relative; the result is rounded to 16 bits as well).
+//   * O += P V: weights from tensor memory, values from shared memory as they lie in the cache (operand "MN-major").
+// Queries, scales and the exponent that takes the value scale in: as in kv8_attention.cu. O is multiplied again only where a row's maximum grew by more than 2^8.
+// Bound by the tensor cores (1024 cycles a block of 128 x 128, head 128) and the exponentials (16 a cycle: 1024) at once; the conversion is 1600 warp
+// instructions beside 2300 of the softmax.
+//
+// Every wait is bounded; a CTA whose wait runs out waits (again with a limit) for its products under way, fills its rows with NaN, counts itself
+// (qspec_attn_tile_timeouts) and frees its tensor memory.
+#include "kv8_common.cuh"
+#include "attn_tile.cuh"
+
+namespace qspec {
+namespace kv8 {
+namespace prompt {
+using namespace atile;
+
+constexpr int SOFTMAX = 8, CONVERT = 4;                   // warps
+constexpr int W_CONVERT = SOFTMAX, W_MMA = W_CONVERT + CONVERT, W_PAGES = W_MMA + 1, NWARPS = W_PAGES + 1, NTHREADS = NWARPS * 32;
+constexpr int FACS = 4;                                   // blocks whose pages and factors are kept
+constexpr float NONE = -INFINITY;
+
+using Args = PromptArgs;
+
+template <int D> struct Sizes {
+  static constexpr int PART = 128 * 128;                  // 128 rows x 64 elements
+  static constexpr int OP = D / 64 * PART;                // an operand: 128 rows x D
+  static constexpr int STAGES = 2;                        // of keys and of values
+  static constexpr size_t USED = (size_t)OP * (1 + 2 * STAGES) + 1024;
+  static constexpr size_t SMEM = USED > 120 * 1024 ? USED : 120 * 1024;   // one CTA an SM: each takes all of the tensor memory
+  static constexpr int LD = D / 2 + 4;                    // floats of a row's half on its way out
+  static_assert(8 * 32 * LD * 4 <= 3 * OP, "rows on their way out, over queries and keys");
+};
+template <int D> constexpr uint32_t IDESC_S = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+template <int D> constexpr uint32_t IDESC_O = (1u << 4) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+
+struct alignas(16) Block {                                            // what the other roles have to know of a block: of each 16 of its keys
+  long long at[8];                                        // where their codes begin, -1: nowhere
+  float kf[8], lv[8], iv[8];                              // scale of the keys; log2 of the values' scale, and its reciprocal
+  unsigned bad;                                           // bit q: a page that there is not, or a scale that is no number
+};
+
+__device__ __forceinline__ void st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+               "r"(r[7]) : "memory");
+}
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
+  using T = typename Elem16<BF16>::T;
+  using Z = Sizes<D>;
+  constexpr int OP = Z::OP, PARTB = Z::PART, STAGES = Z::STAGES, COLS = D / 2;
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ __align__(8) uint64_t b_kfull[STAGES], b_kempty[STAGES], b_vfull[STAGES], b_vempty[STAGES], b_fac[FACS], b_facfree[FACS], b_q, b_s[2], b_p[2][2], b_o, b_done, b_mx[4];
+  __shared__ Block s_block[FACS];
+  __shared__ float s_mx[2][2][128], s_rowf[128];
+  __shared__ int s_sum[NWARPS], s_at[3];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_fail;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rep = a.rep, tok = 128 / rep, g = blockIdx.x;
+  if (tid == 0) {
+    s_fail = 0;
+    s_at[0] = -1;
+    for (int i = 0; i < STAGES; ++i) {
+      bar_init(smem_addr(&b_kfull[i]), CONVERT); bar_init(smem_addr(&b_kempty[i]), 1);
+      bar_init(smem_addr(&b_vfull[i]), CONVERT); bar_init(smem_addr(&b_vempty[i]), 1);
+    }
+    for (int i = 0; i < FACS; ++i) { bar_init(smem_addr(&b_fac[i]), 1); bar_init(smem_addr(&b_facfree[i]), SOFTMAX + CONVERT); }
+    for (int i = 0; i < 2; ++i) { bar_init(smem_addr(&b_s[i]), 1); bar_init(smem_addr(&b_p[i][0]), 8); bar_init(smem_addr(&b_p[i][1]), 4); }
+    bar_init(smem_addr(&b_q), SOFTMAX);
+    bar_init(smem_addr(&b_o), 1);
+    bar_init(smem_addr(&b_done), 1);
+    for (int i = 0; i < 4; ++i) bar_init(smem_addr(&b_mx[i]), 2);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  const uint32_t base = (smem_addr(raw) + 1023u) & ~1023u;
+  unsigned char* const gbase = raw + (base - smem_addr(raw));
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+
+  // ---- this CTA's request and tile: tiles of all requests in a row, the last one of a request (with the longest way) first
+  const int per_thread = (a.nreq + NTHREADS - 1) / NTHREADS, b0 = tid * per_thread, requests = max(min(per_thread, a.nreq - b0), 0);
+  auto tiles_of = [&](int b) {
+    const int first = min(max(a.q_start[b], 0), a.ntok), n = max(min(a.q_start[b + 1], a.ntok) - first, 0);
+    return (long long)n * rep >= a.min_rows ? (n + tok - 1) / tok : 0;
+  };
+  int mine = 0;
+  for (int i = 0; i < requests; ++i) mine += tiles_of(b0 + i);
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int w = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += w;
+  }
+  if (lane == 31) s_sum[warp] = incl;
+  __syncthreads();
+  int before = incl - mine;
+  for (int w = 0; w < warp; ++w) before += s_sum[w];
+  if ((int)blockIdx.y >= before && (int)blockIdx.y < before + mine) {
+    int at = before;
+    for (int i = 0; i < requests; ++i) {
+      const int n = tiles_of(b0 + i);
+      if ((int)blockIdx.y < at + n) {
+        s_at[0] = b0 + i;
+        s_at[1] = n - 1 - ((int)blockIdx.y - at);
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  if (s_at[0] < 0) return;
+  const int req = s_at[0], tile = s_at[1];
+  const int first = min(max(a.q_start[req], 0), a.ntok), n_new = max(min(a.q_start[req + 1], a.ntok) - first, 0), keys = max(a.kv_len[req], 0);
+  const int t0 = tile * tok, n2 = min(tok, n_new - t0);   // this tile's tokens
+  const int pos0 = keys - n_new + t0;                     // position of the first
+  const int seen = min(pos0 + n2, keys), blocks = seen > 0 ? (seen + 127) / 128 : 0;   // keys that any row sees
+  if (warp == W_MMA) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&s_tmem)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = s_tmem;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // (tensor memory is held)
+  const uint32_t kbuf = base + OP, vbuf = kbuf + STAGES * OP;
+
+  if (warp == W_PAGES) {
+    // ---- pages and factors of the blocks, ahead of all others
+    bool ok = !(a.give_up & 8u);
+    if (!ok) s_fail = 1;
+    for (int n = 0; ok && n < blocks; ++n) {
+      const int slot = n % FACS;
+      if (n >= FACS) ok = bar_wait(smem_addr(&b_facfree[slot]), (uint32_t)((n / FACS) - 1) & 1u, &s_fail);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const int key = n * 128 + lane * 16, at = key >> a.pshift;
+      bool bad = false;
+      long long codes = -1;
+      float k = 1.f, v = 1.f;
+      if (lane < 8 && key < keys) {
+        const int page = at < a.width ? a.table[(size_t)req * a.width + at] : -1;
+        bad = (unsigned)page >= (unsigned)a.npages;
+        if (!bad) {
+          const size_t block = (size_t)page * a.G + g;
+          codes = (long long)(((block << a.pshift) + (key & ((1 << a.pshift) - 1))) * D);
+          k = a.ks[block];
+          v = a.vs[block];
+          bad = k != k || v != v;
+        }
+      }
+      const unsigned mask = __ballot_sync(0xffffffffu, bad);
+      if (lane < 8) {
+        s_block[slot].at[lane] = codes;
+        v = positive(v);
+        s_block[slot].kf[lane] = positive(k);
+        s_block[slot].lv[lane] = __log2f(v);
+        s_block[slot].iv[lane] = __fdividef(1.f, v);
+        if (lane == 0) s_block[slot].bad = mask;
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(smem_addr(&b_fac[slot]));
+    }
+  } else if (warp == W_MMA) {
+    if (elect()) {
+      const uint32_t o = tmem + 256, bo = smem_addr(&b_o);
+      const uint64_t qd = desc_k(base);
+      bool ok = !(a.give_up & 4u), over = blocks == 0;
+      if (!ok) s_fail = 1;
+      auto scores = [&](int n) -> bool {
+        if (!bar_wait(smem_addr(&b_kfull[n % STAGES]), (uint32_t)(n / STAGES) & 1u, &s_fail)) return false;
+        // these scores take the columns of the weights of block n - 2: their product must be over
+        if (n >= 2 && !bar_wait(bo, (uint32_t)n & 1u, &s_fail)) return false;
+        fence_after();
+        const uint64_t kd = desc_k(kbuf + (n % STAGES) * OP);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const uint32_t step = (uint32_t)((i >> 2) * (PARTB >> 4) + (i & 3) * 2);
+          mma_ss(tmem + (n & 1) * 128, qd + step, kd + step, IDESC_S<D>, i ? 1u : 0u);
+        }
+        commit(smem_addr(&b_s[n & 1]));
+        commit(smem_addr(&b_kempty[n % STAGES]));
+        return true;
+      };
+      ok = ok && (blocks == 0 || (bar_wait(smem_addr(&b_q), 0, &s_fail) && scores(0)));
+      for (int n = 0; ok && n < blocks; ++n) {
+        if (n + 1 < blocks && !scores(n + 1)) break;
+        if (!bar_wait(smem_addr(&b_vfull[n % STAGES]), (uint32_t)(n / STAGES) & 1u, &s_fail)) break;
+        const uint64_t vd = desc_mn(vbuf + (n % STAGES) * OP);
+        const uint32_t p = tmem + (n & 1) * 128;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {                     // 64 keys each
+          ok = ok && bar_wait(smem_addr(&b_p[n & 1][h]), (uint32_t)(n >> 1) & 1u, &s_fail);
+          if (!ok) break;
+          fence_after();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mma_ts(o, p + h * 64 + i * 8, vd + (h * 4 + i) * (2048 >> 4), IDESC_O<D>, (n | h | i) ? 1u : 0u);
+        }
+        if (!ok) break;
+        commit(bo);
+        if (n + 1 == blocks) { commit(smem_addr(&b_done)); over = true; }
+        commit(smem_addr(&b_vempty[n % STAGES]));
+      }
+      if (!over) commit(smem_addr(&b_done));              // given up: the products issued so far
+      if (blocks) bar_drain(smem_addr(&b_done), 0);
+    }
+    __syncwarp();
+  } else if (warp >= W_CONVERT) {
+    // ---- codes: 16 bytes a lane, 16 rows (one page's) at a time
+    constexpr int CH = D / 16, ROWS = CONVERT * 32 / CH, STEPS = 128 / ROWS;   // pieces of a row, rows at a time, times
+    const int ct = tid - W_CONVERT * 32, c = ct % CH, row0 = ct / CH;
+    const uint32_t part = (uint32_t)(c >> 2) * PARTB;
+    const bool swap = c >= 4;                             // these lanes store their second piece first, so that eight stores meet in no bank
+    uint4 kw[STEPS], vw[STEPS];
+    auto load = [&](uint4 (&w)[STEPS], const signed char* codes, int n) {
+      const Block& f = s_block[n % FACS];
+      const int have = keys - n * 128;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int row = i * ROWS + row0;
+        const long long at = f.at[row >> 4];
+        w[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+        if (row < have && at >= 0) w[i] = __ldg(reinterpret_cast<const uint4*>(codes + at + (row & 15) * D + c * 16));
+      }
+    };
+    auto store = [&](const uint4 (&w)[STEPS], uint32_t dst) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int row = i * ROWS + row0;
+        const uint32_t x[4] = {(swap ? w[i].z : w[i].x) ^ 0x80808080u, (swap ? w[i].w : w[i].y) ^ 0x80808080u, (swap ? w[i].x : w[i].z) ^ 0x80808080u,
+                               (swap ? w[i].y : w[i].w) ^ 0x80808080u};
+        const uint32_t at = dst + part + row * 128;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int piece = ((c & 3) * 2 + (swap ? 1 - e : e)) ^ (row & 7);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at + (piece << 4)), "r"(exact_two(x[2 * e], 0x4140)), "r"(exact_two(x[2 * e], 0x4342)),
+                       "r"(exact_two(x[2 * e + 1], 0x4140)), "r"(exact_two(x[2 * e + 1], 0x4342)) : "memory");
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      __syncwarp();
+    };
+    bool ok = !(a.give_up & 2u);
+    if (!ok) s_fail = 1;
+    auto look = [&](int n) {
+      ok = ok && bar_wait(smem_addr(&b_fac[n % FACS]), (uint32_t)(n / FACS) & 1u, &s_fail);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    if (blocks && ok) look(0);
+    if (blocks && ok) load(kw, a.k, 0);
+    for (int n = 0; ok && n < blocks; ++n) {
+      load(vw, a.v, n);
+      if (n >= STAGES) ok = bar_wait(smem_addr(&b_kempty[n % STAGES]), (uint32_t)(n / STAGES - 1) & 1u, &s_fail);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      store(kw, kbuf + (n % STAGES) * OP);
+      if (lane == 0) {
+        bar_arrive(smem_addr(&b_kfull[n % STAGES]));
+        bar_arrive(smem_addr(&b_facfree[n % FACS]));
+      }
+      if (n + 1 < blocks) {
+        look(n + 1);
+        if (!ok) break;
+        load(kw, a.k, n + 1);
+      }
+      if (n >= STAGES) ok = bar_wait(smem_addr(&b_vempty[n % STAGES]), (uint32_t)(n / STAGES - 1) & 1u, &s_fail);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      store(vw, vbuf + (n % STAGES) * OP);
+      if (lane == 0) bar_arrive(smem_addr(&b_vfull[n % STAGES]));
+    }
+  } else {
+    // ---- queries: 16 bytes a thread at a time, bfloat16 rows by a power of two each
+    constexpr int IN_ROW = D / 8, QROWS = SOFTMAX * 32 / IN_ROW;
+    {
+      const int c = tid % IN_ROW;
+      uint4 w[128 / QROWS];
+#pragma unroll
+      for (int i = 0; i < 128 / QROWS; ++i) {
+        const int r = i * QROWS + tid / IN_ROW, tl = r / rep;
+        w[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (tl < n2 && r < tok * rep)
+          w[i] = *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(first + t0 + tl) * a.q_ts + (size_t)(g * rep + r - tl * rep) * a.q_hs + c * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < 128 / QROWS; ++i) {
+        const int r = i * QROWS + tid / IN_ROW;
+        uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        int sh = 0;
+        if (BF16) {
+          float mx = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
+#pragma unroll
+          for (int o = IN_ROW / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+          sh = mx > 0.f && mx < INFINITY ? min(max(14 - ex, -126), 126) : 0;
+          const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = half_pair(__uint_as_float(x[e] << 16) * up, __uint_as_float(x[e] & 0xffff0000u) * up);
+        }
+        if (c == 0) s_rowf[r] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2;
+        *reinterpret_cast<uint4*>(gbase + (c >> 3) * PARTB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(smem_addr(&b_q));
+    }
+    // ---- softmax: thread = 64 columns (half h) of row r
+    const int h = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int tl = r / rep, head = g * rep + r - tl * rep;
+    const bool row_in = r < tok * rep && tl < n2;
+    const int limit = row_in ? min(pos0 + tl, keys - 1) : -1;   // last visible position
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ot = tmem + lanes + 256 + h * COLS;
+    const uint32_t bmx = smem_addr(&b_mx[warp & 3]);
+    bool ok = !(a.give_up & 1u);
+    if (!ok) s_fail = 1;
+    ok = ok && bar_wait(smem_addr(&b_q), 0, &s_fail);     // (the factors of the rows)
+    ok = __all_sync(0xffffffffu, ok);
+    const float rowf = s_rowf[r];
+    float m = NONE, l = 0.f;
+    int n = 0;
+    for (; ok && n < blocks; ++n) {
+      const int j0 = n * 128 + h * 64;                    // this half block's first key
+      const bool plain = __all_sync(0xffffffffu, !row_in || j0 + 63 <= limit);   // (rows that stand for no token are never stored)
+      const uint32_t st = tmem + lanes + (n & 1) * 128 + h * 64;
+      ok = bar_wait(smem_addr(&b_fac[n % FACS]), (uint32_t)(n / FACS) & 1u, &s_fail) && bar_wait(smem_addr(&b_s[n & 1]), (uint32_t)(n >> 1) & 1u, &s_fail);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      fence_after();
+      uint32_t x[64];
+      ld32(st, x);
+      ld32(st + 32, x + 32);
+      const Block& f = s_block[n % FACS];
+      const float4 kf4 = *reinterpret_cast<const float4*>(&f.kf[h * 4]), lv4 = *reinterpret_cast<const float4*>(&f.lv[h * 4]), iv4 = *reinterpret_cast<const float4*>(&f.iv[h * 4]);
+      const unsigned bad = f.bad >> (h * 4) & 15u;
+      float kf[4] = {normal(kf4.x * rowf), normal(kf4.y * rowf), normal(kf4.z * rowf), normal(kf4.w * rowf)}, lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w};
+      const float iv[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
+      __syncwarp();
+      if (lane == 0) bar_arrive(smem_addr(&b_facfree[n % FACS]));
+      wait_ld();
+      if (!plain || bad) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+          if (bad >> (j >> 4) & 1u) x[j] = 0x7fffffffu;
+          if (j0 + j > limit) x[j] = 0xff800000u;         // hidden
+        }
+      }
+      float mine_mx = NONE;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float m2[2] = {NONE, NONE};
+#pragma unroll
+        for (int j = 0; j < 16; ++j) m2[j & 1] = fmaxf(m2[j & 1], __uint_as_float(x[q * 16 + j]));
+        mine_mx = fmaxf(mine_mx, fmaf(fmaxf(m2[0], m2[1]), kf[q], lv[q]));
+      }
+      s_mx[n & 1][h][r] = mine_mx;
+      __syncwarp();
+      if (lane == 0) bar_arrive(bmx);
+      ok = bar_wait(bmx, (uint32_t)(n & 1), &s_fail);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const float mn = fmaxf(m, fmaxf(mine_mx, s_mx[n & 1][1 - h][r]));
+      // (both warps of the rows see the same maxima and decide alike)
+      const bool grown = mn > m + RESCALE_LOG2 || (m == NONE && mn > m);
+      if (__any_sync(0xffffffffu, grown)) {
+        const float up = grown ? ex2(m - mn) : 1.f;       // 0 for a row that had seen nothing; other rows of the warp keep theirs
+        if (grown) m = mn;
+        l *= up;
+        if (n) {
+          ok = bar_wait(smem_addr(&b_o), (uint32_t)(n - 1) & 1u, &s_fail);   // the previous block's product is in O
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          fence_after();
+#pragma unroll 1
+          for (int q = 0; q < COLS / 8; ++q) {            // (eight at a time: the scores stay in registers)
+            uint32_t o[8];
+            ld8(ot + q * 8, o);
+            wait_ld();
+            landed8(o);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * up);
+            st8(ot + q * 8, o);
+          }
+          wait_st();
+        }
+      }
+      // The product of the first 64 keys adds to all columns of O, those of the second half's warps among them: b_p[.][0] counts their rescale, done or not
+      // needed, beside the first half's weights.
+      if (h) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(smem_addr(&b_p[n & 1][0]));
+      }
+      const float mu = m == NONE ? 0.f : m;
+      // Exponents are taken from the products without a rounding in between, the reference has one: beyond 2^24 that alone would be a large exponent.
+      if (__any_sync(0xffffffffu, fabsf(mu) > 16777216.f)) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]), kf[j >> 4], lv[j >> 4]));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) { kf[q] = 1.f; lv[q] = 0.f; }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t p[16];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          const int q = half * 2 + z;
+          const float at = lv[q] - mu;
+          const uint64_t f2 = pair(__float_as_uint(kf[q]), __float_as_uint(kf[q])), at2 = pair(__float_as_uint(at), __float_as_uint(at));
+          uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t p0, p1;
+            unpair(fma2(pair(x[q * 16 + 2 * j], x[q * 16 + 2 * j + 1]), f2, at2), p0, p1);
+            p0 = __float_as_uint(ex2(__uint_as_float(p0)));
+            p1 = __float_as_uint(ex2(__uint_as_float(p1)));
+            sum[j & 1] = add2(sum[j & 1], pair(p0, p1));
+            p[z * 8 + j] = half_pair(__uint_as_float(p0), __uint_as_float(p1));
+          }
+          uint32_t a0, a1;
+          unpair(add2(sum[0], sum[1]), a0, a1);
+          l = fmaf(__uint_as_float(a0) + __uint_as_float(a1), iv[q], l);
+        }
+        st16(st + half * 16, p);
+      }
+      wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(smem_addr(&b_p[n & 1][h]));
+    }
+    // ---- the last product is done: the halves' sums, division, rows out through shared memory, 16 bytes a lane
+    constexpr int LD = Z::LD, LANES = COLS / 8, AT_ONCE = 32 / LANES;
+    float* const rows = reinterpret_cast<float*>(gbase) + warp * 32 * LD;   // (queries and keys are done with)
+    // Without a block nothing has read the queries, and other warps may still be storing theirs where the rows go: then those are waited for (above).
+    if (ok && blocks) ok = bar_wait(smem_addr(&b_done), 0, &s_fail);
+    ok = __all_sync(0xffffffffu, ok);
+    fence_after();
+    if (ok) {
+      s_mx[n & 1][h][r] = l;
+      __syncwarp();
+      if (lane == 0) bar_arrive(bmx);
+      ok = bar_wait(bmx, (uint32_t)(n & 1), &s_fail);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (ok) {
+      l += s_mx[n & 1][1 - h][r];
+      const float f = l == 0.f ? 0.f : __fdiv_rn(1.f, l); // no key: zeros
+#pragma unroll 1
+      for (int q = 0; q < COLS / 8; ++q) {
+        uint32_t o[8];
+        if (blocks) {
+          ld8(ot + q * 8, o);
+          wait_ld();
+          landed8(o);
+        }
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * f;
+        *reinterpret_cast<float4*>(rows + lane * LD + q * 8) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(rows + lane * LD + q * 8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      }
+      const uint32_t stored = __ballot_sync(0xffffffffu, row_in);
+      __syncwarp();
+      const int pc = lane % LANES;
+#pragma unroll 1
+      for (int k = 0; k < 32 / AT_ONCE; ++k) {
+        const int rr = lane / LANES + AT_ONCE * k, r2 = (warp & 3) * 32 + rr, t2 = r2 / rep;
+        if (!(stored >> rr & 1u)) continue;
+        const float4 x = *reinterpret_cast<const float4*>(rows + rr * LD + pc * 8), y = *reinterpret_cast<const float4*>(rows + rr * LD + pc * 8 + 4);
+        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        *reinterpret_cast<uint4*>((T*)a.out + (size_t)(first + t0 + t2) * a.out_ts + (size_t)(g * rep + r2 - t2 * rep) * a.out_hs + h * COLS + pc * 8) = pack8<BF16>(v);
+      }
+    }
+    (void)head;
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == W_MMA) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u) : "memory");
+  }
+  if (s_fail) {                                           // (written before the barrier: uniform)
+    if (tid == 0) atomicAdd(&attn_tile_timeouts, 1u);
+    for (int i = tid; i < n2 * rep * (D / 8); i += NTHREADS) {
+      const int row = i / (D / 8), tl = row / rep;
+      *reinterpret_cast<uint4*>((T*)a.out + (size_t)(first + t0 + tl) * a.out_ts + (size_t)(g * rep + row - tl * rep) * a.out_hs + i % (D / 8) * 8) =
+          make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+    }
+  }
+}
+
+template <bool BF16, int D>
+int launch(const Args& a, cudaStream_t stream) {
+  static SmemLimit limit;
+  auto kern = kv8_prompt_kernel<BF16, D>;
+  QSPEC_CUDA(limit.raise(kern, Sizes<D>::SMEM));
+  // tiles of all requests at most: full ones, and one more for each request that is large enough
+  const int per = 128 / a.rep;
+  const long long tiles = a.ntok / per + std::min<long long>(a.nreq, (long long)a.ntok * a.rep / std::max(a.min_rows, 1) + 1);
+  QSPEC_REQUIRE(tiles <= 65535, QSPEC_ERR_UNSUPPORTED, "kv8_attention: %d tokens are too many for one call", a.ntok);
+  QSPEC_CUDA(launch_pdl(kern, dim3(a.G, (unsigned)tiles), dim3(NTHREADS), Sizes<D>::SMEM, stream, a));
+  QSPEC_CHECK_LAUNCH(1);
+  return QSPEC_OK;
+}
+
+}  // namespace prompt
+
+int launch_prompt(const PromptArgs& a, int D, bool bf16, cudaStream_t stream) {
+  return bf16 ? (D == 128 ? prompt::launch<true, 128>(a, stream) : prompt::launch<true, 64>(a, stream))
+              : (D == 128 ? prompt::launch<false, 128>(a, stream) : prompt::launch<false, 64>(a, stream));
+}
+}  // namespace kv8
+
+// CTAs of the form above that gave a wait up since the library was loaded on the current device; -1: not readable. Synchronises.
+int kv8_timeouts() {
+  unsigned n = 0;
+  return cudaMemcpyFromSymbol(&n, atile::attn_tile_timeouts, sizeof(n)) == cudaSuccess ? (int)(n & 0x1fffffffu) : -1;
+}
+}  // namespace qspec
