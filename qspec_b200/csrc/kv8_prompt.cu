@@ -1,17 +1,20 @@
 // Softmax attention of prompt portions over the paged 8-bit cache, on the fifth-generation tensor cores (kv8_attention.cu has the layout, and the form for requests
 // with few tokens).
 //
-// One CTA = 128 rows of one request and key/value head; a row is a (token, query head of the group) pair. Keys are walked in blocks of 128:
+// One CTA = 128 rows of one request and key/value head; a row is a (token, query head of the group) pair. Keys are walked in blocks of 128, which belong
+// alternately to two streams with a softmax and a sum of values of their own (joined at the end), so that one's products run under the other's softmax:
 //   * pages: one warp looks the block's pages and scales up and leaves where the codes are and what their products are multiplied with.
-//   * codes: four warps bring a block's keys and values from global memory, make them float16 (a byte c + 128 behind 0x64 is 1152 + c, less 1152; exact)
-//     and store them as the tensor cores want them: the cache is read once, in 8 bits, and is never anywhere in 16.
-//   * S = Q K^T, accumulator [128 x 128] float32 in tensor memory, two of them: the next block's scores are computed under this block's softmax.
-//   * softmax: thread = half a row (64 columns), two warps per 32 rows, which exchange the row's maximum through shared memory. Weights go back over the
-//     scores as float16 (2^-11 relative; the result is rounded to 16 bits as well).
+//   * codes: four warps bring a block's keys and values from global memory, make them float16 and store them as the tensor cores want them: the cache
+//     is read once, in 8 bits, and is never anywhere in 16. Keys are (c + 128) 2^-24, the subnormal number that a byte is by itself; what the 128 adds
+//     to a row's scores is taken out where they enter the exponent. Values are c exactly: a byte behind 0x64 is 1152 + c, less 1152.
+//   * S = Q K^T, accumulator [128 x 128] float32 in tensor memory, one for each stream.
+//   * softmax: thread = row, four warps a stream. Scores are read twice, for the maximum and for the weights (that keeps 128 of them out of the registers).
+//     Weights go back over the scores as float16 (2^-11 relative; the result is rounded to 16 bits as well).
 //   * O += P V: weights from tensor memory, values from shared memory as they lie in the cache (operand "MN-major").
-// Queries, scales and the exponent that takes the value scale in: as in kv8_attention.cu. O is multiplied again only where a row's maximum grew by more than 2^8.
-// Bound by the tensor cores (1024 cycles a block of 128 x 128, head 128) and the exponentials (16 a cycle: 1024) at once; the conversion is 1600 warp
-// instructions beside 2300 of the softmax.
+// Tensor memory: S | S | O | O = 512 columns. Scales and the exponent that takes the value scale in: as in kv8_attention.cu. O is multiplied again only
+// where a row's maximum grew by more than 2^8.
+// Bound by the tensor cores (1024 cycles a block of 128 x 128, head 128) and the exponentials (16 a cycle: 1024) at once, and nearly by the schedulers:
+// the conversion is 1600 warp instructions beside 2600 of the softmax.
 //
 // Every wait is bounded; a CTA whose wait runs out waits (again with a limit) for its products under way, fills its rows with NaN, counts itself
 // (qspec_attn_tile_timeouts) and frees its tensor memory.
@@ -53,15 +56,21 @@ __device__ __forceinline__ void st8(uint32_t addr, const uint32_t* r) {
                "r"(r[7]) : "memory");
 }
 
+// Behind wait_ld(): nothing that is done with these registers is moved in front of it.
+__device__ __forceinline__ void landed32(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) landed8(r + i * 8);
+}
+
 template <bool BF16, int D>
 __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   using T = typename Elem16<BF16>::T;
   using Z = Sizes<D>;
   constexpr int OP = Z::OP, PARTB = Z::PART, STAGES = Z::STAGES, COLS = D / 2;
   extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ __align__(8) uint64_t b_kfull[STAGES], b_kempty[STAGES], b_vfull[STAGES], b_vempty[STAGES], b_fac[FACS], b_facfree[FACS], b_q, b_s[2], b_p[2][2], b_o, b_done, b_mx[4];
+  __shared__ __align__(8) uint64_t b_kfull[STAGES], b_kempty[STAGES], b_vfull[STAGES], b_vempty[STAGES], b_fac[FACS], b_facfree[FACS], b_q, b_s[2], b_p[2][2], b_o[2], b_join;
   __shared__ Block s_block[FACS];
-  __shared__ float s_mx[2][2][128], s_rowf[128];
+  __shared__ float s_ml[2][2][128], s_rowf[128], s_sum128[128];
   __shared__ int s_sum[NWARPS], s_at[3];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_fail;
@@ -74,12 +83,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       bar_init(smem_addr(&b_kfull[i]), CONVERT); bar_init(smem_addr(&b_kempty[i]), 1);
       bar_init(smem_addr(&b_vfull[i]), CONVERT); bar_init(smem_addr(&b_vempty[i]), 1);
     }
-    for (int i = 0; i < FACS; ++i) { bar_init(smem_addr(&b_fac[i]), 1); bar_init(smem_addr(&b_facfree[i]), SOFTMAX + CONVERT); }
-    for (int i = 0; i < 2; ++i) { bar_init(smem_addr(&b_s[i]), 1); bar_init(smem_addr(&b_p[i][0]), 8); bar_init(smem_addr(&b_p[i][1]), 4); }
+    for (int i = 0; i < FACS; ++i) { bar_init(smem_addr(&b_fac[i]), 1); bar_init(smem_addr(&b_facfree[i]), SOFTMAX / 2 + CONVERT); }
+    for (int i = 0; i < 2; ++i) { bar_init(smem_addr(&b_s[i]), 1); bar_init(smem_addr(&b_p[i][0]), 4); bar_init(smem_addr(&b_p[i][1]), 4); bar_init(smem_addr(&b_o[i]), 1); }
     bar_init(smem_addr(&b_q), SOFTMAX);
-    bar_init(smem_addr(&b_o), 1);
-    bar_init(smem_addr(&b_done), 1);
-    for (int i = 0; i < 4; ++i) bar_init(smem_addr(&b_mx[i]), 2);
+    bar_init(smem_addr(&b_join), SOFTMAX);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   const uint32_t base = (smem_addr(raw) + 1023u) & ~1023u;
@@ -172,14 +179,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     }
   } else if (warp == W_MMA) {
     if (elect()) {
-      const uint32_t o = tmem + 256, bo = smem_addr(&b_o);
       const uint64_t qd = desc_k(base);
-      bool ok = !(a.give_up & 4u), over = blocks == 0;
+      bool ok = !(a.give_up & 4u);
       if (!ok) s_fail = 1;
+      int products = 0;                                   // value products that have been issued, block by block
       auto scores = [&](int n) -> bool {
         if (!bar_wait(smem_addr(&b_kfull[n % STAGES]), (uint32_t)(n / STAGES) & 1u, &s_fail)) return false;
         // these scores take the columns of the weights of block n - 2: their product must be over
-        if (n >= 2 && !bar_wait(bo, (uint32_t)n & 1u, &s_fail)) return false;
+        if (n >= 2 && !bar_wait(smem_addr(&b_o[n & 1]), (uint32_t)((n >> 1) - 1) & 1u, &s_fail)) return false;
         fence_after();
         const uint64_t kd = desc_k(kbuf + (n % STAGES) * OP);
 #pragma unroll
@@ -191,27 +198,31 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         commit(smem_addr(&b_kempty[n % STAGES]));
         return true;
       };
-      ok = ok && (blocks == 0 || (bar_wait(smem_addr(&b_q), 0, &s_fail) && scores(0)));
+      ok = ok && (blocks == 0 || (bar_wait(smem_addr(&b_q), 0, &s_fail) && scores(0) && (blocks == 1 || scores(1))));
       for (int n = 0; ok && n < blocks; ++n) {
-        if (n + 1 < blocks && !scores(n + 1)) break;
         if (!bar_wait(smem_addr(&b_vfull[n % STAGES]), (uint32_t)(n / STAGES) & 1u, &s_fail)) break;
         const uint64_t vd = desc_mn(vbuf + (n % STAGES) * OP);
-        const uint32_t p = tmem + (n & 1) * 128;
+        const uint32_t p = tmem + (n & 1) * 128, o = tmem + 256 + (n & 1) * D;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                     // 64 keys each
           ok = ok && bar_wait(smem_addr(&b_p[n & 1][h]), (uint32_t)(n >> 1) & 1u, &s_fail);
           if (!ok) break;
           fence_after();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mma_ts(o, p + h * 64 + i * 8, vd + (h * 4 + i) * (2048 >> 4), IDESC_O<D>, (n | h | i) ? 1u : 0u);
+          for (int i = 0; i < 4; ++i) mma_ts(o, p + h * 32 + i * 8, vd + (h * 4 + i) * (2048 >> 4), IDESC_O<D>, (n > 1 || h || i) ? 1u : 0u);
         }
         if (!ok) break;
-        commit(bo);
-        if (n + 1 == blocks) { commit(smem_addr(&b_done)); over = true; }
+        commit(smem_addr(&b_o[n & 1]));
         commit(smem_addr(&b_vempty[n % STAGES]));
+        products = n + 1;
+        if (n + 2 < blocks && !scores(n + 2)) break;
       }
-      if (!over) commit(smem_addr(&b_done));              // given up: the products issued so far
-      if (blocks) bar_drain(smem_addr(&b_done), 0);
+      if (products < blocks) {                            // given up: what was issued so far
+        commit(smem_addr(&b_o[products & 1]));
+        products += 1;
+      }
+      // every product of either stream is over before the CTA leaves
+      for (int n = max(products - 2, 0); n < products; ++n) bar_drain(smem_addr(&b_o[n & 1]), (uint32_t)(n >> 1) & 1u);
     }
     __syncwarp();
   } else if (warp >= W_CONVERT) {
@@ -224,15 +235,24 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     auto load = [&](uint4 (&w)[STEPS], const signed char* codes, int n) {
       const Block& f = s_block[n % FACS];
       const int have = keys - n * 128;
+      const signed char* from = codes + (row0 & 15) * D + c * 16;
+      long long at[STEPS];
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int row = i * ROWS + row0;
-        const long long at = f.at[row >> 4];
-        w[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-        if (row < have && at >= 0) w[i] = __ldg(reinterpret_cast<const uint4*>(codes + at + (row & 15) * D + c * 16));
+      for (int i = 0; i < STEPS; ++i) at[i] = f.at[(i * ROWS + row0) >> 4];
+      if (have >= 128 && !f.bad) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(from + at[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+          w[i] = make_uint4(0u, 0u, 0u, 0u);
+          if (i * ROWS + row0 < have && at[i] >= 0) w[i] = __ldg(reinterpret_cast<const uint4*>(from + at[i]));
+        }
       }
     };
-    auto store = [&](const uint4 (&w)[STEPS], uint32_t dst) {
+    auto store = [&](const uint4 (&w)[STEPS], uint32_t dst, const bool values) {
+      auto first_two = [&](uint32_t x) { return values ? exact_two(x, 0x4140) : __byte_perm(x, 0u, 0x4140); };
+      auto last_two = [&](uint32_t x) { return values ? exact_two(x, 0x4342) : __byte_perm(x, 0u, 0x4342); };
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         const int row = i * ROWS + row0;
@@ -242,8 +262,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int piece = ((c & 3) * 2 + (swap ? 1 - e : e)) ^ (row & 7);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at + (piece << 4)), "r"(exact_two(x[2 * e], 0x4140)), "r"(exact_two(x[2 * e], 0x4342)),
-                       "r"(exact_two(x[2 * e + 1], 0x4140)), "r"(exact_two(x[2 * e + 1], 0x4342)) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at + (piece << 4)), "r"(first_two(x[2 * e])), "r"(last_two(x[2 * e])),
+                       "r"(first_two(x[2 * e + 1])), "r"(last_two(x[2 * e + 1])) : "memory");
         }
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
@@ -262,7 +282,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       if (n >= STAGES) ok = bar_wait(smem_addr(&b_kempty[n % STAGES]), (uint32_t)(n / STAGES - 1) & 1u, &s_fail);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      store(kw, kbuf + (n % STAGES) * OP);
+      store(kw, kbuf + (n % STAGES) * OP, false);
       if (lane == 0) {
         bar_arrive(smem_addr(&b_kfull[n % STAGES]));
         bar_arrive(smem_addr(&b_facfree[n % FACS]));
@@ -275,7 +295,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       if (n >= STAGES) ok = bar_wait(smem_addr(&b_vempty[n % STAGES]), (uint32_t)(n / STAGES - 1) & 1u, &s_fail);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      store(vw, vbuf + (n % STAGES) * OP);
+      store(vw, vbuf + (n % STAGES) * OP, true);
       if (lane == 0) bar_arrive(smem_addr(&b_vfull[n % STAGES]));
     }
   } else {
@@ -308,165 +328,182 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[e] = half_pair(__uint_as_float(x[e] << 16) * up, __uint_as_float(x[e] & 0xffff0000u) * up);
         }
-        if (c == 0) s_rowf[r] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x[e]));
+          sum += y.x + y.y;
+        }
+#pragma unroll
+        for (int o = IN_ROW / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (c == 0) {
+          s_rowf[r] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2 * 16777216.f;   // (scores come in units of 2^-24)
+          s_sum128[r] = sum * (128.f / 16777216.f);
+        }
         *reinterpret_cast<uint4*>(gbase + (c >> 3) * PARTB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
       if (lane == 0) bar_arrive(smem_addr(&b_q));
     }
-    // ---- softmax: thread = 64 columns (half h) of row r
-    const int h = warp >> 2, r = (warp & 3) * 32 + lane;
-    const int tl = r / rep, head = g * rep + r - tl * rep;
+    // ---- softmax: thread = row r of the blocks of stream z
+    const int z = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int tl = r / rep;
     const bool row_in = r < tok * rep && tl < n2;
     const int limit = row_in ? min(pos0 + tl, keys - 1) : -1;   // last visible position
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ot = tmem + lanes + 256 + h * COLS;
-    const uint32_t bmx = smem_addr(&b_mx[warp & 3]);
+    const uint32_t st = tmem + lanes + z * 128, ot = tmem + lanes + 256 + z * D;
     bool ok = !(a.give_up & 1u);
     if (!ok) s_fail = 1;
     ok = ok && bar_wait(smem_addr(&b_q), 0, &s_fail);     // (the factors of the rows)
     ok = __all_sync(0xffffffffu, ok);
-    const float rowf = s_rowf[r];
+    const float rowf = s_rowf[r], sum128 = s_sum128[r];
     float m = NONE, l = 0.f;
-    int n = 0;
-    for (; ok && n < blocks; ++n) {
-      const int j0 = n * 128 + h * 64;                    // this half block's first key
-      const bool plain = __all_sync(0xffffffffu, !row_in || j0 + 63 <= limit);   // (rows that stand for no token are never stored)
-      const uint32_t st = tmem + lanes + (n & 1) * 128 + h * 64;
-      ok = bar_wait(smem_addr(&b_fac[n % FACS]), (uint32_t)(n / FACS) & 1u, &s_fail) && bar_wait(smem_addr(&b_s[n & 1]), (uint32_t)(n >> 1) & 1u, &s_fail);
+    int n = z;
+    for (; ok && n < blocks; n += 2) {
+      const uint32_t turn = (uint32_t)(n >> 1) & 1u;
+      const int j0 = n * 128;
+      const bool plain = __all_sync(0xffffffffu, !row_in || j0 + 127 <= limit);   // (rows that stand for no token are never stored)
+      ok = bar_wait(smem_addr(&b_fac[n % FACS]), (uint32_t)(n / FACS) & 1u, &s_fail) && bar_wait(smem_addr(&b_s[z]), turn, &s_fail);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
-      uint32_t x[64];
-      ld32(st, x);
-      ld32(st + 32, x + 32);
       const Block& f = s_block[n % FACS];
-      const float4 kf4 = *reinterpret_cast<const float4*>(&f.kf[h * 4]), lv4 = *reinterpret_cast<const float4*>(&f.lv[h * 4]), iv4 = *reinterpret_cast<const float4*>(&f.iv[h * 4]);
-      const unsigned bad = f.bad >> (h * 4) & 15u;
-      float kf[4] = {normal(kf4.x * rowf), normal(kf4.y * rowf), normal(kf4.z * rowf), normal(kf4.w * rowf)}, lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w};
-      const float iv[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
-      __syncwarp();
-      if (lane == 0) bar_arrive(smem_addr(&b_facfree[n % FACS]));
-      wait_ld();
-      if (!plain || bad) {
+      const unsigned bad = f.bad;
+      const bool odd = !plain || bad;
+      // Loops over 32 columns, not unrolled: three kinds of warps run at once, and with the block's 128 columns laid out in a row they waited for their
+      // instructions more than for anything else (4.2 of 12 cycles an instruction; prompt of 2000 after 1000, 32 / 8 heads 207 us, so @@).
+      // What a row does not see, and of a page that there is not, or whose scale is no number, what makes the rows NaN that do see it:
+      auto hide = [&](uint32_t (&x)[32], int c0) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {
-          if (bad >> (j >> 4) & 1u) x[j] = 0x7fffffffu;
-          if (j0 + j > limit) x[j] = 0xff800000u;         // hidden
+        for (int j = 0; j < 32; ++j) {
+          if (bad >> (c0 / 16 + j / 16) & 1u) x[j] = 0x7fffffffu;
+          if (j0 + c0 + j > limit) x[j] = 0xff800000u;
         }
-      }
-      float mine_mx = NONE;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float m2[2] = {NONE, NONE};
-#pragma unroll
-        for (int j = 0; j < 16; ++j) m2[j & 1] = fmaxf(m2[j & 1], __uint_as_float(x[q * 16 + j]));
-        mine_mx = fmaxf(mine_mx, fmaf(fmaxf(m2[0], m2[1]), kf[q], lv[q]));
-      }
-      s_mx[n & 1][h][r] = mine_mx;
-      __syncwarp();
-      if (lane == 0) bar_arrive(bmx);
-      ok = bar_wait(bmx, (uint32_t)(n & 1), &s_fail);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      const float mn = fmaxf(m, fmaxf(mine_mx, s_mx[n & 1][1 - h][r]));
-      // (both warps of the rows see the same maxima and decide alike)
-      const bool grown = mn > m + RESCALE_LOG2 || (m == NONE && mn > m);
-      if (__any_sync(0xffffffffu, grown)) {
-        const float up = grown ? ex2(m - mn) : 1.f;       // 0 for a row that had seen nothing; other rows of the warp keep theirs
-        if (grown) m = mn;
-        l *= up;
-        if (n) {
-          ok = bar_wait(smem_addr(&b_o), (uint32_t)(n - 1) & 1u, &s_fail);   // the previous block's product is in O
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          fence_after();
+      };
+      // ---- the largest exponent
+      float mn = NONE;
 #pragma unroll 1
-          for (int q = 0; q < COLS / 8; ++q) {            // (eight at a time: the scores stay in registers)
-            uint32_t o[8];
-            ld8(ot + q * 8, o);
-            wait_ld();
-            landed8(o);
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        uint32_t x[32];
+        ld32(st + c0, x);
+        const float2 kf = *reinterpret_cast<const float2*>(&f.kf[c0 / 16]), lv = *reinterpret_cast<const float2*>(&f.lv[c0 / 16]);
+        wait_ld();
+        landed32(x);
+        if (odd) hide(x, c0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * up);
-            st8(ot + q * 8, o);
-          }
-          wait_st();
+        for (int q = 0; q < 2; ++q) {
+          float t[2] = {__uint_as_float(x[q * 16]), __uint_as_float(x[q * 16 + 1])};
+#pragma unroll
+          for (int j = 2; j < 16; ++j) t[j & 1] = fmaxf(t[j & 1], __uint_as_float(x[q * 16 + j]));
+          const float k = normal((q ? kf.y : kf.x) * rowf);
+          mn = fmaxf(mn, fmaf(fmaxf(t[0], t[1]), k, fmaf(-sum128, k, q ? lv.y : lv.x)));
         }
       }
-      // The product of the first 64 keys adds to all columns of O, those of the second half's warps among them: b_p[.][0] counts their rescale, done or not
-      // needed, beside the first half's weights.
-      if (h) {
-        fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(smem_addr(&b_p[n & 1][0]));
+      const bool grown = mn > m + RESCALE_LOG2 || (m == NONE && mn > m);
+      const float up = grown ? ex2(m - mn) : 1.f;         // 0 for a row that had seen nothing; other rows of the warp keep theirs
+      l *= up;
+      if (n > 1 && __any_sync(0xffffffffu, grown && m != NONE)) {   // (the scores are there: the stream's product before them is over)
+#pragma unroll 1
+        for (int q = 0; q < D / 8; ++q) {
+          uint32_t o[8];
+          ld8(ot + q * 8, o);
+          wait_ld();
+          landed8(o);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * up);
+          st8(ot + q * 8, o);
+        }
       }
+      if (grown) m = mn;
       const float mu = m == NONE ? 0.f : m;
       // Exponents are taken from the products without a rounding in between, the reference has one: beyond 2^24 that alone would be a large exponent.
-      if (__any_sync(0xffffffffu, fabsf(mu) > 16777216.f)) {
+      const bool far = __any_sync(0xffffffffu, fabsf(mu) > 16777216.f);
+      // ---- weights
+#pragma unroll 1
+      for (int c0 = 0; c0 < 128; c0 += 32) {
+        uint32_t x[32], p[16];
+        ld32(st + c0, x);
+        const float2 kf = *reinterpret_cast<const float2*>(&f.kf[c0 / 16]), lv = *reinterpret_cast<const float2*>(&f.lv[c0 / 16]), iv = *reinterpret_cast<const float2*>(&f.iv[c0 / 16]);
+        float k[2] = {normal(kf.x * rowf), normal(kf.y * rowf)}, at[2] = {fmaf(-sum128, k[0], lv.x), fmaf(-sum128, k[1], lv.y)};
+        wait_ld();
+        landed32(x);
+        if (odd) hide(x, c0);
+        if (far) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]), kf[j >> 4], lv[j >> 4]));
+          for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]), k[j / 16], at[j / 16]));
+          k[0] = k[1] = 1.f;
+          at[0] = at[1] = 0.f;
+        }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) { kf[q] = 1.f; lv[q] = 0.f; }
-      }
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[16];
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int q = half * 2 + z;
-          const float at = lv[q] - mu;
-          const uint64_t f2 = pair(__float_as_uint(kf[q]), __float_as_uint(kf[q])), at2 = pair(__float_as_uint(at), __float_as_uint(at));
+        for (int q = 0; q < 2; ++q) {
+          const uint64_t k2 = pair(__float_as_uint(k[q]), __float_as_uint(k[q])), at2 = pair(__float_as_uint(at[q] - mu), __float_as_uint(at[q] - mu));
           uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             uint32_t p0, p1;
-            unpair(fma2(pair(x[q * 16 + 2 * j], x[q * 16 + 2 * j + 1]), f2, at2), p0, p1);
+            unpair(fma2(pair(x[q * 16 + 2 * j], x[q * 16 + 2 * j + 1]), k2, at2), p0, p1);
             p0 = __float_as_uint(ex2(__uint_as_float(p0)));
             p1 = __float_as_uint(ex2(__uint_as_float(p1)));
             sum[j & 1] = add2(sum[j & 1], pair(p0, p1));
-            p[z * 8 + j] = half_pair(__uint_as_float(p0), __uint_as_float(p1));
+            p[q * 8 + j] = half_pair(__uint_as_float(p0), __uint_as_float(p1));
           }
           uint32_t a0, a1;
           unpair(add2(sum[0], sum[1]), a0, a1);
-          l = fmaf(__uint_as_float(a0) + __uint_as_float(a1), iv[q], l);
+          l = fmaf(__uint_as_float(a0) + __uint_as_float(a1), q ? iv.y : iv.x, l);
         }
-        st16(st + half * 16, p);
+        st16(st + c0 / 2, p);                             // (over scores that have been read)
+        if (c0 & 32) {                                    // 64 keys' weights are there
+          wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(smem_addr(&b_p[z][c0 >> 6]));
+        }
       }
-      wait_st();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(smem_addr(&b_p[n & 1][h]));
+      if (lane == 0) bar_arrive(smem_addr(&b_facfree[n % FACS]));
     }
-    // ---- the last product is done: the halves' sums, division, rows out through shared memory, 16 bytes a lane
+    // ---- the streams together: maxima and sums through shared memory; stream z takes half z of the columns, of both sums. Rows leave through shared memory,
+    // 16 bytes a lane.
     constexpr int LD = Z::LD, LANES = COLS / 8, AT_ONCE = 32 / LANES;
     float* const rows = reinterpret_cast<float*>(gbase) + warp * 32 * LD;   // (queries and keys are done with)
-    // Without a block nothing has read the queries, and other warps may still be storing theirs where the rows go: then those are waited for (above).
-    if (ok && blocks) ok = bar_wait(smem_addr(&b_done), 0, &s_fail);
-    ok = __all_sync(0xffffffffu, ok);
-    fence_after();
+    s_ml[z][0][r] = m;
+    s_ml[z][1][r] = l;
+    __syncwarp();
+    if (lane == 0) bar_arrive(smem_addr(&b_join));
+    // the last product of either stream, and everyone's maxima
     if (ok) {
-      s_mx[n & 1][h][r] = l;
-      __syncwarp();
-      if (lane == 0) bar_arrive(bmx);
-      ok = bar_wait(bmx, (uint32_t)(n & 1), &s_fail);
+      ok = bar_wait(smem_addr(&b_join), 0, &s_fail);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (blocks > i) ok = ok && bar_wait(smem_addr(&b_o[i]), (uint32_t)((blocks - 1 - i) >> 1) & 1u, &s_fail);
       ok = __all_sync(0xffffffffu, ok);
     }
+    fence_after();
     if (ok) {
-      l += s_mx[n & 1][1 - h][r];
-      const float f = l == 0.f ? 0.f : __fdiv_rn(1.f, l); // no key: zeros
+      float f[2], sum = 0.f;
+      const float m0 = s_ml[0][0][r], m1 = s_ml[1][0][r], top = fmaxf(m0, m1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float mi = i ? m1 : m0, li = s_ml[i][1][r];
+        f[i] = mi == NONE ? (li == 0.f ? 0.f : 1.f) : ex2(mi - top);   // nothing seen, or no number
+        sum += li * f[i];
+      }
+      const float d = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);          // (no key: zeros)
+      const bool two = __any_sync(0xffffffffu, f[1] != 0.f) && blocks > 1;
 #pragma unroll 1
       for (int q = 0; q < COLS / 8; ++q) {
-        uint32_t o[8];
-        if (blocks) {
-          ld8(ot + q * 8, o);
-          wait_ld();
-          landed8(o);
-        }
+        uint32_t o0[8], o1[8];
+        if (blocks > 0) ld8(tmem + lanes + 256 + z * COLS + q * 8, o0);
+        if (blocks > 1) ld8(tmem + lanes + 256 + D + z * COLS + q * 8, o1);
+        wait_ld();
+        landed8(o0);
+        landed8(o1);
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = l == 0.f ? 0.f : __uint_as_float(o[e]) * f;
+        for (int e = 0; e < 8; ++e) {
+          const float x0 = f[0] == 0.f ? 0.f : __uint_as_float(o0[e]) * f[0], x1 = two && f[1] != 0.f ? __uint_as_float(o1[e]) * f[1] : 0.f;
+          v[e] = (x0 + x1) * d;
+        }
         *reinterpret_cast<float4*>(rows + lane * LD + q * 8) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4*>(rows + lane * LD + q * 8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
       }
@@ -479,10 +516,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         if (!(stored >> rr & 1u)) continue;
         const float4 x = *reinterpret_cast<const float4*>(rows + rr * LD + pc * 8), y = *reinterpret_cast<const float4*>(rows + rr * LD + pc * 8 + 4);
         const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-        *reinterpret_cast<uint4*>((T*)a.out + (size_t)(first + t0 + t2) * a.out_ts + (size_t)(g * rep + r2 - t2 * rep) * a.out_hs + h * COLS + pc * 8) = pack8<BF16>(v);
+        *reinterpret_cast<uint4*>((T*)a.out + (size_t)(first + t0 + t2) * a.out_ts + (size_t)(g * rep + r2 - t2 * rep) * a.out_hs + z * COLS + pc * 8) = pack8<BF16>(v);
       }
     }
-    (void)head;
   }
   fence_before();
   __syncthreads();
