@@ -8,16 +8,15 @@
 // Products, differences and sums are those of 64-bit numbers: the first two are exact, and with 150,000 terms a running sum in 32 bits would
 // move the borders between tokens by as much as small tokens are wide. That also makes the result one that every implementation finds.
 //
-// One cluster of CTAs per request; what bounds it is reading two rows of V float32. Each CTA sums a stretch of the row, tile by tile (TILE values), and
-// keeps the tiles' sums; the CTAs exchange their totals through distributed shared memory; the one in whose stretch the border lies looks for the
-// tile, reads that tile again and finds the token in it. Sums are made in the order of the row down to tiles, so that no atomics and no order of
-// CTAs enter.
+// One cluster of CTAs per request; what bounds it is reading two rows of V float32. A warp takes tiles of 1024 values, all of whose loads are on their way
+// before the first is used, and keeps each tile's sum; the CTAs exchange their totals through distributed shared memory; the one in whose stretch the border
+// lies looks for the tile, reads it again and finds the token in it. Sums are made in a fixed order, so that no atomics and no order of CTAs enter.
 #include "common.cuh"
 
 namespace qspec {
 namespace spec {
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, EACH = 8, TILE = 32 * EACH, MAX_DRAFTS = 31;
+constexpr int THREADS = 256, WARPS = THREADS / 32, PARTS = 8, PART = 128, TILE = PARTS * PART, MAX_DRAFTS = 31;   // a part: four values a lane
 constexpr int MAX_TILES = 1024;                   // of a CTA's stretch
 
 struct Args {
@@ -45,65 +44,62 @@ __device__ __forceinline__ double warp_before(double v, int lane) {
   const double w = __shfl_up_sync(0xffffffffu, incl, 1);
   return lane ? w : 0.0;
 }
-// What is left to draw from at place i. A probability that is no number, or below zero, counts as none.
+// What is left to draw from. A probability that is no number counts as none.
 __device__ __forceinline__ double rest_of(float p, float q) {
-  const double r = (double)p - (double)q;
-  return r > 0.0 ? r : 0.0;
+  return p > q ? (double)p - (double)q : 0.0;
 }
 
 template <int CLUSTER, bool VEC>
-__global__ void __launch_bounds__(THREADS) verify_drafts_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, CLUSTER == 8 ? 4 : 3) verify_drafts_kernel(const Args a) {
+  static_assert(PARTS == WARPS, "a part of a tile for each warp");
   __shared__ double s_tile[MAX_TILES], s_total[2];          // of this CTA's stretch: sums of tiles; of max(p - q, 0) and of p
+  __shared__ double s_part[PARTS], s_upto;
+  __shared__ int s_at;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
   pdl_enter();
 
   // ---- how many drafts are taken (every warp for itself)
   const int k = a.counts ? min(max(a.counts[b], 0), a.k) : a.k;
-  bool refused = lane < k;
-  if (lane < k) {
+  bool refused = true;
+  if (lane < a.k) {
     const long long d = a.drafted[(size_t)b * a.k + lane];
     if (d >= 0 && d < a.V) {
       const float q = a.draft[b * a.d_ss + lane * a.d_ps + d], p = a.target[b * a.t_ss + lane * a.t_ps + d];
       refused = !((double)a.uniform[(size_t)b * (a.k + 1) + lane] * (double)q < (double)p);
     }
   }
-  const uint32_t no = __ballot_sync(0xffffffffu, refused);
+  const uint32_t no = __ballot_sync(0xffffffffu, refused && lane < k);
   const int taken = no ? __ffs(no) - 1 : k;
   const float* p = a.target + b * a.t_ss + taken * a.t_ps;
   bool differ = taken < k;                                  // draw from max(p - q, 0)
   const float* q = differ ? a.draft + b * a.d_ss + taken * a.d_ps : p;
   const int lo = min(rank * a.span, a.V), hi = min(lo + a.span, a.V), tiles = (hi - lo + TILE - 1) / TILE;
 
-  auto load = [&](int at, float (&pv)[EACH], float (&qv)[EACH]) {   // values at .. at + EACH - 1 of the rows, zeros behind the stretch
-    if (VEC && at + EACH <= hi) {
-#pragma unroll
-      for (int e = 0; e < EACH; e += 4) {
-        *reinterpret_cast<float4*>(pv + e) = *reinterpret_cast<const float4*>(p + at + e);
-        if (differ) *reinterpret_cast<float4*>(qv + e) = *reinterpret_cast<const float4*>(q + at + e);
-      }
-      if (!differ) {
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) qv[e] = 0.f;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < EACH; ++e) {
-        pv[e] = at + e < hi ? p[at + e] : 0.f;
-        qv[e] = differ && at + e < hi ? q[at + e] : 0.f;
-      }
-    }
+  auto four = [&](const float* row, int at) -> float4 {     // values at .. at + 3 of a row, zeros behind the stretch
+    if (VEC && at + 4 <= hi) return *reinterpret_cast<const float4*>(row + at);
+    return make_float4(at < hi ? row[at] : 0.f, at + 1 < hi ? row[at + 1] : 0.f, at + 2 < hi ? row[at + 2] : 0.f, at + 3 < hi ? row[at + 3] : 0.f);
   };
+  auto rest4 = [&](const float4& x, const float4& y) { return (rest_of(x.x, y.x) + rest_of(x.y, y.y)) + (rest_of(x.z, y.z) + rest_of(x.w, y.w)); };
+  const float4 nothing = make_float4(0.f, 0.f, 0.f, 0.f);
 
   double total = 0.0, before = 0.0;
   int second = 0;
   for (int pass = 0; pass < 2; ++pass) {                    // (a second time where the difference has nothing)
     for (int t = warp; t < tiles; t += WARPS) {
-      float pv[EACH], qv[EACH];
-      load(lo + t * TILE + lane * EACH, pv, qv);
       double s = 0.0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < PARTS; i0 += 4) {               // (eight loads a lane under way; 24 warps an SM: sixteen of 16 warps took 47 us for 190 requests, these 44)
+        float4 pv[4], qv[4];
+        const int at = lo + t * TILE + i0 * PART + lane * 4;
 #pragma unroll
-      for (int e = 0; e < EACH; ++e) s += rest_of(pv[e], qv[e]);
+        for (int i = 0; i < 4; ++i) {
+          pv[i] = four(p, at + i * PART);
+          qv[i] = differ ? four(q, at + i * PART) : nothing;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += rest4(pv[i], qv[i]);
+      }
       s = warp_sum(s);
       if (lane == 0) s_tile[t] = s;
     }
@@ -142,9 +138,8 @@ __global__ void __launch_bounds__(THREADS) verify_drafts_kernel(const Args a) {
   const double border = (double)fminf(fmaxf(a.uniform[(size_t)b * (a.k + 1) + a.k], 0.f), 0.99999994f) * total;
   const bool mass = total > 0.0 && total < (double)INFINITY;
   const double after = before + s_total[second];
-  if (warp == 0 && (mass ? before <= border && border < after : rank == 0)) {
-    int token = 0;                                          // of a row without any mass
-    if (mass) {
+  if (mass ? before <= border && border < after : rank == 0) {   // (the same for all of the CTA)
+    if (warp == 0) {                                        // the tile, and the sum in front of it
       const int each = (tiles + 31) / 32;
       double s = 0.0;
       for (int i = 0; i < each; ++i)
@@ -152,11 +147,10 @@ __global__ void __launch_bounds__(THREADS) verify_drafts_kernel(const Args a) {
       double run = before + warp_before(s, lane);           // the sum in front of this lane's tiles
       // (the sums of tiles and those of stretches are added in different orders: where the border lies within their last bits, the last tile counts)
       uint32_t at = __ballot_sync(0xffffffffu, s > 0.0 && run + s > border);
-      if (!at) at = 1u << (31 - __clz(__ballot_sync(0xffffffffu, s > 0.0)));
-      const int src = __ffs(at) - 1;
-      int tile = 0;
-      double upto = run;
-      if (lane == src) {
+      if (!at) at = 0x80000000u >> __clz(__ballot_sync(0xffffffffu, s > 0.0) | 1u);
+      if (lane == __ffs(at) - 1) {
+        int tile = 0;
+        double upto = run;
         for (int i = 0; i < each && lane * each + i < tiles; ++i) {
           const double x = s_tile[lane * each + i];
           if (!(x > 0.0)) continue;
@@ -165,37 +159,52 @@ __global__ void __launch_bounds__(THREADS) verify_drafts_kernel(const Args a) {
           if (run + x > border) break;
           run += x;
         }
+        s_at = tile;
+        s_upto = upto;
       }
-      tile = __shfl_sync(0xffffffffu, tile, src);
-      run = __shfl_sync(0xffffffffu, upto, src);
-      float pv[EACH], qv[EACH];
-      const int first = lo + tile * TILE + lane * EACH;
-      load(first, pv, qv);
-      s = 0.0;
-#pragma unroll
-      for (int e = 0; e < EACH; ++e) s += rest_of(pv[e], qv[e]);
-      run += warp_before(s, lane);
-      at = __ballot_sync(0xffffffffu, s > 0.0 && run + s > border);
-      if (!at) at = 1u << (31 - __clz(__ballot_sync(0xffffffffu, s > 0.0)));
-      if (lane == __ffs(at) - 1) {
+    }
+    __syncthreads();
+    // the tile's parts, one a warp; then the values of the one that has the border
+    const int first = lo + s_at * TILE + warp * PART + lane * 4;
+    const float4 pv = four(p, first), qv = differ ? four(q, first) : nothing;
+    const double x[4] = {rest_of(pv.x, qv.x), rest_of(pv.y, qv.y), rest_of(pv.z, qv.z), rest_of(pv.w, qv.w)};
+    const double s = (x[0] + x[1]) + (x[2] + x[3]), mine = warp_sum(s);
+    if (lane == 0) s_part[warp] = mine;
+    __syncthreads();
+    double run = s_upto, upto = s_upto;
+    int where = 0;
+#pragma unroll 1
+    for (int i = 0; i < PARTS; ++i) {
+      const double y = s_part[i];
+      if (!(y > 0.0)) continue;
+      where = i;
+      upto = run;
+      if (run + y > border) break;
+      run += y;
+    }
+    if (warp == where) {
+      int token = 0;                                        // of a row without any mass
+      run = upto + warp_before(s, lane);
+      uint32_t at = __ballot_sync(0xffffffffu, s > 0.0 && run + s > border);
+      if (!at) at = 0x80000000u >> __clz(__ballot_sync(0xffffffffu, s > 0.0) | 1u);
+      if (mass && lane == __ffs(at) - 1) {
         bool over = false;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          const double x = rest_of(pv[e], qv[e]);
-          if (!over && x > 0.0) {
+        for (int e = 0; e < 4; ++e) {
+          if (!over && x[e] > 0.0) {
             token = first + e;
-            run += x;
+            run += x[e];
             over = run > border;
           }
         }
       }
       token = __shfl_sync(0xffffffffu, token, __ffs(at) - 1);
+      if (lane <= a.k) {
+        long long* to = a.tokens + (size_t)b * (a.k + 1) + lane;
+        *to = lane < taken ? a.drafted[(size_t)b * a.k + lane] : lane == taken ? (long long)token : -1ll;
+      }
+      if (lane == 0) a.emitted[b] = taken + 1;
     }
-    if (lane <= a.k) {
-      long long* to = a.tokens + (size_t)b * (a.k + 1) + lane;
-      *to = lane < taken ? a.drafted[(size_t)b * a.k + lane] : lane == taken ? (long long)token : -1ll;
-    }
-    if (lane == 0) a.emitted[b] = taken + 1;
   }
   if (CLUSTER > 1) cluster_wait_acquire();                  // the others have read this CTA's sum
 }
@@ -218,24 +227,27 @@ extern "C" int qspec_verify_drafts(const long long* drafted, const float* draft,
   QSPEC_REQUIRE(vocab <= 8 * MAX_TILES * TILE && requests <= (1 << 24), QSPEC_ERR_UNSUPPORTED, "verify_drafts: vocabulary of %d, %d requests", vocab, requests);
   QSPEC_REQUIRE((drafts == 0 || (draft_seq_stride >= 0 && draft_place_stride >= 0)) && target_seq_stride >= 0 && target_place_stride >= 0, QSPEC_ERR_INVALID_ARG,
                 "verify_drafts: negative stride");
-  constexpr int CLUSTER = 8;
   Args a{drafted, draft, target, uniform, draft_counts, draft_seq_stride, draft_place_stride, target_seq_stride, target_place_stride, tokens, emitted, drafts, vocab, 0};
-  a.span = ((vocab + CLUSTER - 1) / CLUSTER + TILE - 1) / TILE * TILE;
   const bool vec = (((uintptr_t)target | (uintptr_t)(drafts ? draft : target)) & 15) == 0 && ((target_seq_stride | target_place_stride) & 3) == 0 &&
                    (drafts == 0 || ((draft_seq_stride | draft_place_stride) & 3) == 0);
+  // CTAs of a request: eight where there are few requests (the rows' way through the GPU counts), four where they fill it by themselves.
+  const bool many = requests >= 96 && vocab <= 4 * MAX_TILES * TILE;
+  const int cluster = many ? 4 : 8;
+  a.span = ((vocab + cluster - 1) / cluster + TILE - 1) / TILE * TILE;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(requests * CLUSTER);
+  cfg.gridDim = dim3(requests * cluster);
   cfg.blockDim = dim3(THREADS);
   cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CLUSTER;
+  attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  QSPEC_CUDA(vec ? cudaLaunchKernelEx(&cfg, verify_drafts_kernel<CLUSTER, true>, a) : cudaLaunchKernelEx(&cfg, verify_drafts_kernel<CLUSTER, false>, a));
+  auto kern = many ? (vec ? verify_drafts_kernel<4, true> : verify_drafts_kernel<4, false>) : (vec ? verify_drafts_kernel<8, true> : verify_drafts_kernel<8, false>);
+  QSPEC_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
   QSPEC_CHECK_LAUNCH(1);
   return QSPEC_OK;
 }
