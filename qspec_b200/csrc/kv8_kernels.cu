@@ -13,7 +13,7 @@ namespace kv8 {
 // and per page that goes back. Every CTA makes the sums for itself (4096 requests are 48 KB of reads from L2) and takes its share of the rest, so
 // that no CTA waits for another; nothing that a call reads is written by it (table entries from `held` on and list entries from n_free on mean nothing to
 // the state that came in), so that the order of the CTAs does not matter and a call can be made again.
-constexpr int PLAN_THREADS = 1024, PLAN_REQUESTS = 4096, PLAN_EACH = PLAN_REQUESTS / PLAN_THREADS;
+constexpr int PLAN_REQUESTS = 4096, PLAN_EACH = 4, PLAN_SMALL = 256, PLAN_LARGE = PLAN_REQUESTS / PLAN_EACH;   // requests; of a thread; threads of a CTA
 
 struct PlanArgs {
   const int *lengths, *counts;
@@ -22,21 +22,26 @@ struct PlanArgs {
   const int* state;
   int *q_start, *kv_len, *positions, *seq_ids, *slots, *state_out;
   int n, width, npages, pshift, ntok;
+  int top;                                         // the largest power of two below n, or 1
 };
 
 // index of the last entry of the ascending s[0 .. n - 1] that is <= x (s[0] <= x)
-__device__ __forceinline__ int last_at_most(const int* s, int n, int x) {
+__device__ __forceinline__ int last_at_most(const int* s, int n, int top, int x) {
   int lo = 0;
-  for (int step = PLAN_REQUESTS; step; step >>= 1)
+  for (int step = top; step; step >>= 1)
     if (lo + step < n && s[lo + step] <= x) lo += step;
   return lo;
 }
 
+template <int PLAN_THREADS>
 __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs a) {
+  constexpr int PLAN_WARPS = PLAN_THREADS / 32;
   extern __shared__ int plan_smem[];
   int* s_tok = plan_smem;                         // first token of each request, in front of it [n + 1]
   int* s_need = s_tok + a.n + 1;                  // pages asked for before it [n + 1]
   int* s_back = s_need + a.n + 1;                 // pages given back before it [n + 1]
+  int* s_len = s_back + a.n + 1;                  // tokens held, or -1 for a request that has no place for its tokens [n]
+  int* s_held = s_len + a.n;                      // pages held [n]
   __shared__ int s_warp[3][32], s_refused[32], s_over;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) s_over = a.n;
@@ -78,13 +83,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
   if (warp == 0) {
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
-      int v = s_warp[q][lane];
+      int v = lane < PLAN_WARPS ? s_warp[q][lane] : 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
+      for (int o = 1; o < PLAN_WARPS; o <<= 1) {
         const int w = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v = q ? v + w : (int)min((long long)v + w, (long long)a.ntok + 1);
       }
-      s_warp[q][lane] = v;
+      if (lane < PLAN_WARPS) s_warp[q][lane] = v;
     }
   }
   __syncthreads();
@@ -95,7 +100,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
     at[q] = prev + (lane ? before : 0);
     if (q == 0) at[q] = min(at[q], a.ntok + 1);
   }
-  const int have = n_free + s_warp[2][31];
+  const int have = n_free + s_warp[2][PLAN_WARPS - 1];
   int refused = 0;
 #pragma unroll
   for (int e = 0; e < PLAN_EACH; ++e) {
@@ -109,6 +114,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
       if (cnt[e] > 0 && first <= a.ntok && last > a.ntok) s_over = b;   // the first whose tokens there is no room for
       s_need[b] = at[1];
       s_back[b] = at[2];
+      s_len[b] = granted ? len[e] : -1;
+      s_held[b] = held[e];
       if (blockIdx.x == 0) {
         a.q_start[b] = min(first, a.ntok);
         a.kv_len[b] = granted ? len[e] + cnt[e] : 0;
@@ -146,7 +153,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
   const int step = gridDim.x * PLAN_THREADS, first = blockIdx.x * PLAN_THREADS + tid;
   // the nth page of those that have come back, and the nth page handed out
   auto returned = [&](int nth) {
-    const int b = last_at_most(s_back, a.n, nth);
+    const int b = last_at_most(s_back, a.n, a.top, nth);
     return a.table[(size_t)b * a.width + (nth - s_back[b])];
   };
   auto page = [&](int nth) {
@@ -154,18 +161,17 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
     return src < n_free ? a.free_pages[src] : returned(src - n_free);
   };
   for (int i = first; i < taken; i += step) {
-    const int b = last_at_most(s_need, a.n, i);
-    a.table[(size_t)b * a.width + min(max(a.state[b], 0), a.width) + (i - s_need[b])] = page(i);
+    const int b = last_at_most(s_need, a.n, a.top, i);
+    a.table[(size_t)b * a.width + s_held[b] + (i - s_need[b])] = page(i);
   }
   for (int i = n_free + first; i < min(left, a.npages); i += step) a.free_pages[i] = returned(i - n_free);
   const int tokens = s_tok[a.n];
   for (int t = first; t < a.ntok; t += step) {
     int pos = -1, slot = -1, req = -1;
     if (t < tokens) {
-      req = last_at_most(s_tok, a.n, t);
-      const int c = a.counts[req], l = a.lengths[req], h = min(max(a.state[req], 0), a.width), wants = s_need[req + 1] - s_need[req];
-      const bool room = l >= 0 && ((((long long)l + c + (1 << a.pshift) - 1) >> a.pshift) <= a.width) && (long long)s_tok[req] + c <= a.ntok;
-      if (room && (wants == 0 || s_need[req + 1] <= have)) {
+      req = last_at_most(s_tok, a.n, a.top, t);
+      const int l = s_len[req], h = s_held[req];
+      if (l >= 0) {
         pos = l + (t - s_tok[req]);
         const int nth = pos >> a.pshift;
         const int pg = nth < h ? a.table[(size_t)req * a.width + nth] : page(s_need[req] + nth - h);
@@ -177,7 +183,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
     a.slots[t] = slot;
   }
   if (blockIdx.x == 0 && warp == 0) {
-    const int r = __reduce_add_sync(0xffffffffu, s_refused[lane]);
+    const int r = __reduce_add_sync(0xffffffffu, lane < PLAN_WARPS ? s_refused[lane] : 0);
     if (lane == 0) {
       a.state_out[a.n] = left;
       a.state_out[a.n + 1] = r;
@@ -186,9 +192,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
 }
 
 // ---- rows into pages --------------------------------------------------------------------------------------------------------------
-// One warp per run and head, keys and values each: the consecutive tokens of one page. Eight lanes a row, four rows at a time; a lane holds sixteen of its
-// values, eight of each half, so that it has both of every pair that the rotation turns. Two walks over the rows, the second from L1: the page's scale is
-// the largest |x| of all of them. No barrier, no shared memory: a decode step's call is one load, a reduction and a store long.
+// A run (the consecutive tokens of one page) is one warp's per head, for keys and values each, where there are few tokens, and a CTA's in a prompt. Eight
+// lanes a row, four rows of a warp at a time; a lane holds sixteen of its values, eight of each half, so that it has both of every pair that the rotation
+// turns. The page's scale is the largest |x| of all rows: those that fit into registers stay there between the maximum and the codes, others are read
+// again. A decode step's call is one load, a reduction and a store long: without barriers.
 // Rotation and codes are evaluated with the roundings that their formulas have (no fused multiply-adds), so that the same codes come out of every
 // implementation in float32.
 struct AppendArgs {
@@ -199,6 +206,7 @@ struct AppendArgs {
   float *ks, *vs;
   void* q; long long q_ts;
   int ntok, H, G, npages, pshift, block;          // block: tokens of a CTA
+  unsigned h_inv;                                 // r * h_inv >> 32 = r / H for the rows of a CTA's tokens
 };
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;   // 2^-60
 constexpr int APPEND_WARPS = 8;
@@ -210,21 +218,21 @@ __device__ __forceinline__ int slot_of(const AppendArgs& a, int t) {
   return s >= 0 && s < (a.npages << a.pshift) && p >= 0 && p < a.cos_rows ? s : -1;
 }
 
-// sixteen values of a row: x[0 .. 7] from column 8 c on, x[8 .. 15] the same of the second half
+// sixteen values of a row (token t, at position pos): x[0 .. 7] from column 8 c on, x[8 .. 15] the same of the second half
 template <bool BF16, int D, bool TURN>
-__device__ __forceinline__ void load_row(const AppendArgs& a, int t, int col, int c, float (&x)[16]) {
+__device__ __forceinline__ void load_row(const AppendArgs& a, int t, int pos, int col, int c, float (&x)[16]) {
   using T = typename Elem16<BF16>::T;
   const T* row = (const T*)a.qkv + (size_t)t * a.ld + col + c * 8;
   float lo[8], hi[8];
   unpack8<BF16>(*reinterpret_cast<const uint4*>(row), lo);
   unpack8<BF16>(*reinterpret_cast<const uint4*>(row + D / 2), hi);
   if (TURN) {
-    const T* tab = (const T*)a.cos_sin + (size_t)a.positions[t] * D + c * 8;
+    const T* tab = (const T*)a.cos_sin + (size_t)pos * D + c * 8;
     float cs[8], sn[8];
     unpack8<BF16>(*reinterpret_cast<const uint4*>(tab), cs);
     unpack8<BF16>(*reinterpret_cast<const uint4*>(tab + D / 2), sn);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 8; ++e) {                           // (not by pairs: mul.rn.f32x2 in front of add.rn.f32x2 became one multiply-add)
       x[e] = __fsub_rn(__fmul_rn(lo[e], cs[e]), __fmul_rn(hi[e], sn[e]));
       x[e + 8] = __fadd_rn(__fmul_rn(hi[e], cs[e]), __fmul_rn(lo[e], sn[e]));
     }
@@ -239,92 +247,158 @@ __device__ __forceinline__ uint32_t code_of(float x, float inv) {
   return (uint32_t)(x == x ? (int)fminf(fmaxf(r, -127.f), 127.f) : 0) & 0xffu;
 }
 
-template <bool BF16, int D, bool TURN>
-__device__ __forceinline__ void write_run(const AppendArgs& a, int t0, int n, int slot, int g, int col, signed char* codes, float* scales) {
-  constexpr int LANES = D / 16, ROWS = 32 / LANES;          // lanes of a row, rows at a time
-  const int lane = threadIdx.x & 31, c = lane % LANES, r0 = lane / LANES;
+__device__ __forceinline__ float finite_max(float mx, const float (&x)[16]) {   // (what is not finite does not stretch the page's scale)
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float y = fabsf(x[e]);
+    mx = fmaxf(mx, y < INFINITY ? y : 0.f);
+  }
+  return mx;
+}
+// The largest |x| so far, infinite as soon as one is not finite.
+__device__ __forceinline__ float largest(float mx, const float (&x)[16]) {
+  float z = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    mx = fmaxf(mx, fabsf(x[e]));
+    z = fmaf(x[e], 0.f, z);
+  }
+  return z == 0.f ? mx : INFINITY;
+}
+// odd: the run has values that are not finite. Where it has none, rint(x / scale) is in the last byte of x / scale + 1.5 * 2^23.
+template <int D>
+__device__ __forceinline__ void store_codes(signed char* row, int c, const float (&x)[16], float inv, bool odd) {
+  uint32_t w[4];
+  if (odd) {
+    w[0] = w[1] = w[2] = w[3] = 0u;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e >> 2] |= code_of(x[e], inv) << (8 * (e & 3));
+  } else {
+    auto bits = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.f)); };
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      w[e >> 2] = __byte_perm(__byte_perm(bits(x[e]), bits(x[e + 1]), 0x0040), __byte_perm(bits(x[e + 2]), bits(x[e + 3]), 0x0040), 0x5410);
+  }
+  *reinterpret_cast<uint2*>(row + c * 8) = make_uint2(w[0], w[1]);
+  *reinterpret_cast<uint2*>(row + c * 8 + D / 2) = make_uint2(w[2], w[3]);
+}
+// the page's rows before the run onto its new scale: codes i, i + step, .. of sixteen each
+__device__ __forceinline__ void rescale(signed char* rows, int pieces, int i, int step, float before, float after) {
+  const float f = __fdiv_rn(before, after);
+  for (; i < pieces; i += step) {
+    uint4* at = reinterpret_cast<uint4*>(rows) + i;
+    uint4 v = *at;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t o = 0u;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o |= ((uint32_t)(int)rintf(__fmul_rn((float)(signed char)(w[q] >> (8 * e)), f)) & 0xffu) << (8 * e);
+      w[q] = o;
+    }
+    *at = v;
+  }
+}
+__device__ __forceinline__ float new_scale(float mx, float before) { return fmaxf(fmaxf(__fmul_rn(mx, 1.0f / 127.0f), before), SCALE_FLOOR); }
+
+// How many tokens the run has that begins with token t, of slot s, where `known` of them are already: asked by a whole warp.
+__device__ __forceinline__ int run_of(const AppendArgs& a, int t, int s, int known) {
+  const int mask = (1 << a.pshift) - 1, lane = threadIdx.x & 31, most = mask + 1 - (s & mask);
+  for (int n = known; n < most; n += 32) {
+    const uint32_t out = ~__ballot_sync(0xffffffffu, n + lane < most && slot_of(a, t + n + lane) == s + n + lane);
+    if (out) return n + __ffs(out) - 1;
+  }
+  return most;
+}
+
+// A run by WARPS warps (one, or all of the CTA's): four rows (of 128) a warp at a time, the first of them held in registers between the maximum and the codes.
+template <bool BF16, int D, bool TURN, int WARPS>
+__device__ __forceinline__ void write_run(const AppendArgs& a, int t0, int n, int slot, int g, int col, signed char* codes, float* scales, float* s_max) {
+  constexpr int LANES = D / 16, ROWS = 32 / LANES, STEP = ROWS * WARPS;   // lanes of a row, rows of a warp, rows at a time
+  const int lane = threadIdx.x & 31, warp = WARPS > 1 ? threadIdx.x >> 5 : 0, c = lane % LANES, r0 = warp * ROWS + lane / LANES;
   const int page = slot >> a.pshift, first = slot & ((1 << a.pshift) - 1);
   signed char* rows = codes + (((size_t)page * a.G + g) << a.pshift) * D;
   float* scale = scales + (size_t)page * a.G + g;
   const float before = first ? *scale : 0.f;
+  float x[16];                                              // the first of this lane's rows
+  auto load = [&](int r) {
+    if (r < n) load_row<BF16, D, TURN>(a, t0 + r, TURN ? a.positions[t0 + r] : 0, col, c, x);
+    return r < n;
+  };
+  auto over_all = [&](float mx) {                           // (and everyone has read the scale)
+    mx = warp_xor_max(mx);
+    if (WARPS > 1) {
+      __syncthreads();
+      if (lane == 0) s_max[warp] = mx;
+      __syncthreads();
+      mx = warp_xor_max(lane < WARPS ? s_max[lane] : 0.f);
+    }
+    return mx;
+  };
   float mx = 0.f;
-  for (int r = r0; r < n; r += ROWS) {
-    float x[16];
-    load_row<BF16, D, TURN>(a, t0 + r, col, c, x);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float y = fabsf(x[e]);
-      mx = fmaxf(mx, y < INFINITY ? y : 0.f);               // (what is not finite does not stretch the page's scale)
+  for (int r = r0 + STEP; r < n; r += STEP) {
+    load(r);
+    mx = largest(mx, x);
+  }
+  if (load(r0)) mx = largest(mx, x);
+  mx = over_all(mx);
+  const bool odd = mx == INFINITY;
+  if (odd) {                                                // the largest of those that are finite
+    mx = 0.f;
+    for (int r = r0 + STEP; r < n; r += STEP) {
+      load(r);
+      mx = finite_max(mx, x);
     }
+    if (load(r0)) mx = finite_max(mx, x);
+    mx = over_all(mx);
   }
-  mx = warp_xor_max(mx);
-  const float after = fmaxf(fmaxf(__fmul_rn(mx, 1.0f / 127.0f), before), SCALE_FLOOR);
-  const float inv = __frcp_rn(after);
-  for (int r = r0; r < n; r += ROWS) {
-    float x[16];
-    load_row<BF16, D, TURN>(a, t0 + r, col, c, x);
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int e = 0; e < 16; ++e) w[e >> 2] |= code_of(x[e], inv) << (8 * (e & 3));
-    signed char* to = rows + (size_t)(first + r) * D + c * 8;
-    *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-    *reinterpret_cast<uint2*>(to + D / 2) = make_uint2(w[2], w[3]);
+  __syncwarp();
+  const float after = new_scale(mx, before), inv = __frcp_rn(after);
+  if (r0 < n) store_codes<D>(rows + (size_t)(first + r0) * D, c, x, inv, odd);
+  for (int r = r0 + STEP; r < n; r += STEP) {
+    load(r);
+    store_codes<D>(rows + (size_t)(first + r) * D, c, x, inv, odd);
   }
-  if (first && after > before) {                            // the older rows onto the new scale
-    const float f = __fdiv_rn(before, after);
-    for (int i = lane; i < first * (D / 16); i += 32) {
-      uint4* at = reinterpret_cast<uint4*>(rows) + i;
-      uint4 v = *at;
-      uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t o = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o |= ((uint32_t)(int)rintf(__fmul_rn((float)(signed char)(w[q] >> (8 * e)), f)) & 0xffu) << (8 * e);
-        w[q] = o;
-      }
-      *at = v;
-    }
-  }
-  __syncwarp();                                             // every lane has read the scale
-  if (lane == 0 && after != before) *scale = after;
+  if (first && after > before) rescale(rows, first * (D / 16), warp * 32 + lane, WARPS * 32, before, after);
+  if (warp == 0 && lane == 0 && after != before) *scale = after;
 }
 
-template <bool BF16, int D>
-__global__ void __launch_bounds__(APPEND_WARPS * 32) kv8_append_kernel(const AppendArgs a) {
+// WIDE: a CTA per run, head and side (prompts: runs of whole pages). Otherwise a warp.
+template <bool BF16, int D, bool WIDE>
+__global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const AppendArgs a) {
   using T = typename Elem16<BF16>::T;
-  constexpr int LANES = D / 16, ROWS = 32 / LANES;
+  constexpr int LANES = D / 16, ROWS = 32 / LANES, W = WIDE ? APPEND_WARPS : 1;
+  __shared__ float s_max[APPEND_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = blockIdx.x * a.block, t1 = min(t0 + a.block, a.ntok);
-  const int units = (2 * a.G + APPEND_WARPS - 1) / APPEND_WARPS;    // CTAs in y that write pages; the others turn queries
+  const int units = WIDE ? 2 * a.G : (2 * a.G + APPEND_WARPS - 1) / APPEND_WARPS;   // CTAs in y that write pages; the others turn queries
   pdl_enter();
   if ((int)blockIdx.y < units) {
-    const int u = blockIdx.y * APPEND_WARPS + warp;
+    const int u = WIDE ? blockIdx.y : blockIdx.y * APPEND_WARPS + warp;
     if (u >= 2 * a.G) return;
     const int g = u >> 1;
-    const int mask = (1 << a.pshift) - 1;
-    for (int t = t0; t < t1; ++t) {
-      const int s = slot_of(a, t);
-      if (s < 0 || ((s & mask) && slot_of(a, t - 1) == s - 1)) continue;   // no row, or inside a run
-      int n = 0;                                            // the run's tokens: up to the end of the page
-      const int most = mask + 1 - (s & mask);
-      for (; n < most; n += 32) {
-        const bool in = n + lane < most && slot_of(a, t + n + lane) == s + n + lane;
-        const uint32_t out = ~__ballot_sync(0xffffffffu, in);
-        if (out) { n += __ffs(out) - 1; break; }
-      }
-      n = min(n, most);
-      if (u & 1) write_run<BF16, D, false>(a, t, n, s, g, (a.H + a.G + g) * D, a.v, a.vs);
-      else write_run<BF16, D, true>(a, t, n, s, g, (a.H + g) * D, a.k, a.ks);
+    // slots from the token before this CTA's first on, two a lane: which begin a run, and where runs end as far as that shows
+    const int sa = slot_of(a, t0 - 1 + lane), sb = slot_of(a, t0 + 31 + lane);
+    const int before = __shfl_up_sync(0xffffffffu, sa, 1), mask = (1 << a.pshift) - 1;
+    const bool go_on = lane > 0 && sa >= 0 && (sa & mask) && before == sa - 1;          // token t0 - 1 + lane is in the run of the one before it
+    const int last = __shfl_sync(0xffffffffu, sa, 31), before_b = __shfl_up_sync(0xffffffffu, sb, 1);
+    const bool go_on_b = sb >= 0 && (sb & mask) && (lane ? before_b : last) == sb - 1;
+    const uint64_t in_run = ((uint64_t)__ballot_sync(0xffffffffu, go_on) | (uint64_t)__ballot_sync(0xffffffffu, go_on_b) << 32) >> 1;   // bit i: token t0 + i
+    for (uint32_t left = __ballot_sync(0xffffffffu, lane > 0 && t0 - 1 + lane < t1 && sa >= 0 && !go_on) >> 1; left; left &= left - 1u) {
+      const int i = __ffs(left) - 1, t = t0 + i, s = __shfl_sync(0xffffffffu, sa, i + 1);
+      int n = 1 + (__ffsll((long long)~(in_run >> (i + 1))) - 1);
+      if (t + n >= t0 + 63) n = run_of(a, t, s, n);         // (it may be longer than that)
+      if (u & 1) write_run<BF16, D, false, W>(a, t, n, s, g, (a.H + a.G + g) * D, a.v, a.vs, s_max);
+      else write_run<BF16, D, true, W>(a, t, n, s, g, (a.H + g) * D, a.k, a.ks, s_max);
     }
   } else {
     const int c = lane % LANES, rows = (t1 - t0) * a.H, per = APPEND_WARPS * ROWS;
     for (int r = ((int)blockIdx.y - units) * per + warp * ROWS + lane / LANES; r < rows; r += ((int)gridDim.y - units) * per) {
-      const int t = t0 + r / a.H, h = r % a.H;
+      const int tl = a.H == 1 ? r : (int)__umulhi((unsigned)r, a.h_inv), t = t0 + tl, h = r - tl * a.H;
       const int p = a.positions[t];
       if (p < 0 || p >= a.cos_rows) continue;
       float x[16];
-      load_row<BF16, D, true>(a, t, h * D, c, x);
+      load_row<BF16, D, true>(a, t, p, h * D, c, x);
       float lo[8], hi[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) { lo[e] = x[e]; hi[e] = x[e + 8]; }
@@ -374,12 +448,15 @@ extern "C" int qspec_page_plan(const int* lengths, const int* counts, int* table
   QSPEC_REQUIRE(page_shift(page_tokens) > 0, QSPEC_ERR_UNSUPPORTED, "page_plan: pages of 16, 32, 64 or 128 tokens, got %d", page_tokens);
   QSPEC_REQUIRE(width >= 1 && width <= (1 << 18) && npages >= 1 && (long long)npages * page_tokens < (1ll << 31) && ntok >= 0 && ntok < (1 << 30), QSPEC_ERR_INVALID_ARG,
                 "page_plan: width=%d pages=%d tokens=%d", width, npages, ntok);
-  PlanArgs a{lengths, counts, table, free_pages, state, q_start, kv_len, positions, seq_ids, slots, state_out, requests, width, npages, page_shift(page_tokens), ntok};
-  const size_t smem = 3 * (size_t)(requests + 1) * sizeof(int);
+  int top = 1;
+  while (top * 2 < requests) top *= 2;
+  const PlanArgs a{lengths, counts, table, free_pages, state, q_start, kv_len, positions, seq_ids, slots, state_out, requests, width, npages, page_shift(page_tokens), ntok, top};
+  const size_t smem = (5 * (size_t)requests + 3) * sizeof(int);
+  const bool large = requests > PLAN_SMALL * PLAN_EACH;
   static SmemLimit limit;
-  if (smem > 40000) QSPEC_CUDA(limit.raise(page_plan_kernel, smem));
-  const int grid = min(max((ntok + PLAN_THREADS - 1) / PLAN_THREADS, 1), max(sm_count(), 1));
-  QSPEC_CUDA(launch_pdl(page_plan_kernel, dim3(grid), dim3(PLAN_THREADS), smem, (cudaStream_t)stream, a));
+  if (large) QSPEC_CUDA(limit.raise(page_plan_kernel<PLAN_LARGE>, smem));
+  const int threads = large ? PLAN_LARGE : PLAN_SMALL, grid = min(max((ntok + threads - 1) / threads, 1), 2 * max(sm_count(), 1));
+  QSPEC_CUDA(launch_pdl(large ? page_plan_kernel<PLAN_LARGE> : page_plan_kernel<PLAN_SMALL>, dim3(grid), dim3(threads), smem, (cudaStream_t)stream, a));
   QSPEC_CHECK_LAUNCH(1);
   return QSPEC_OK;
 }
@@ -403,14 +480,19 @@ extern "C" int qspec_kv8_append(const void* qkv, long long ld, const void* cos_s
   QSPEC_REQUIRE(ld >= (long long)(H + 2 * G) * D && ld % 8 == 0 && (!q_out || (q_tok_stride >= (long long)H * D && q_tok_stride % 8 == 0)) && ((uintptr_t)qkv & 15) == 0 &&
                     ((uintptr_t)cos_sin & 15) == 0 && ((uintptr_t)q_out & 15) == 0,
                 QSPEC_ERR_INVALID_ARG, "kv8_append: rows must lie on 16-byte boundaries (ld=%lld)", ld);
-  AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (signed char*)k, (signed char*)v, ks, vs, q_out, q_tok_stride, ntok, H, G, npages, page_shift(page_tokens), 1};
-  // A CTA looks at one token where there are few (each is likely to begin a run) and at eight of a prompt's, most of which are inside one.
-  a.block = ntok <= 512 ? 1 : 8;
+  AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (signed char*)k, (signed char*)v, ks, vs, q_out, q_tok_stride, ntok, H, G, npages, page_shift(page_tokens), 1, (unsigned)(((1ull << 32) + H - 1) / H)};   // (31 * 4096 rows at most: r times what h_inv is too large by stays below 2^32)
+  // Few tokens: a CTA looks at one, which is likely to begin a run. A prompt: at a page's or so, with a CTA for each run, head and side
+  // (4200 tokens, 40 / 8 heads, pages of 32, rows without queries: 25.5 us with a warp for each, so 11.8).
+  const bool wide = ntok > 512;
+  a.block = wide ? std::min(page_tokens, 31) : 1;           // (with the token before them one a lane)
   const int rows = APPEND_WARPS * 32 * 16 / D;              // query rows that a CTA takes at a time
-  const int y = (2 * G + APPEND_WARPS - 1) / APPEND_WARPS + (q_out ? (a.block * H + 2 * rows - 1) / (2 * rows) : 0);
+  const int y = (wide ? 2 * G : (2 * G + APPEND_WARPS - 1) / APPEND_WARPS) + (q_out ? (a.block * H + 2 * rows - 1) / (2 * rows) : 0);
   const dim3 grid((ntok + a.block - 1) / a.block, y);
-  auto kern = dtype == QSPEC_DTYPE_F16 ? (D == 128 ? kv8_append_kernel<false, 128> : kv8_append_kernel<false, 64>)
-                                       : (D == 128 ? kv8_append_kernel<true, 128> : kv8_append_kernel<true, 64>);
+  auto pick = [&](auto few, auto many) { return wide ? many : few; };
+  auto kern = dtype == QSPEC_DTYPE_F16 ? (D == 128 ? pick(kv8_append_kernel<false, 128, false>, kv8_append_kernel<false, 128, true>)
+                                                   : pick(kv8_append_kernel<false, 64, false>, kv8_append_kernel<false, 64, true>))
+                                       : (D == 128 ? pick(kv8_append_kernel<true, 128, false>, kv8_append_kernel<true, 128, true>)
+                                                   : pick(kv8_append_kernel<true, 64, false>, kv8_append_kernel<true, 64, true>));
   QSPEC_CUDA(launch_pdl(kern, grid, dim3(APPEND_WARPS * 32), 0, (cudaStream_t)stream, a));
   QSPEC_CHECK_LAUNCH(1);
   return QSPEC_OK;

@@ -185,7 +185,18 @@ RUNS = {"one": [(0, 1)], "decode": [(5, 1), (63, 1), (64, 1), (200, 1)], "verify
 @pytest.mark.parametrize("runs", list(RUNS))
 @pytest.mark.parametrize("spoil", [False, True])
 def test_append_gives_the_codes_of_its_formulas(runs, D, P, H, G, dtype, spoil):
-    qkv, cs, pos, slots, codes, scales = make_append(3, RUNS[runs], H, G, D, P, dtype, spoil=spoil)
+    check_append(RUNS[runs], D, P, H, G, dtype, spoil)
+
+
+@pytest.mark.parametrize("D,P,H,G,dtype", [(128, 64, 8, 2, torch.float16), (128, 16, 4, 4, torch.bfloat16), (64, 32, 5, 1, torch.float16), (64, 128, 6, 3, torch.bfloat16),
+                                           (128, 128, 10, 2, torch.float16)])
+@pytest.mark.parametrize("runs", [[(0, 513)], [(100, 500), (0, 1), (130, 63), (7, 1), (8, 1), (77, 300), (63, 2)]])
+def test_append_of_long_steps(runs, D, P, H, G, dtype):
+    check_append(runs, D, P, H, G, dtype, False, 90)
+
+
+def check_append(runs, D, P, H, G, dtype, spoil, pages=40):
+    qkv, cs, pos, slots, codes, scales = make_append(3, runs, H, G, D, P, dtype, pages=pages, spoil=spoil)
     T = len(pos)
     x = qkv.float().view(T, H + 2 * G, D)
     turned = rotated(x[:, :H + G], cs[torch.tensor(pos, device="cuda")].float(), F32)
@@ -200,7 +211,7 @@ def test_append_gives_the_codes_of_its_formulas(runs, D, P, H, G, dtype, spoil):
     assert torch.equal(ks, want[0][1]) and torch.equal(vs, want[1][1])
     assert torch.equal(k, want[0][0]) and torch.equal(v, want[1][0])
     # the reader: code times scale, rounded once; none for slots outside
-    asked = slots + [-1, 40 * P]
+    asked = slots + [-1, pages * P]
     ko, vo = (torch.empty(len(asked), G, D, dtype=dtype, device="cuda") for _ in range(2))
     ops.kv8_read(k, v, ks, vs, i32(asked), ko, vo)
     at = torch.tensor(slots, device="cuda")
