@@ -1,5 +1,5 @@
 """QSpec speculative-decode loop around the dual-mode model: k draft passes in W4A4, one verify
-pass in W4A16 over the same weights and KV cache, greedy acceptance.
+pass in W4A16 over the same weights and KV cache, greedy acceptance or rejection sampling.
 
 Mirrors SpecDecodeWorker._run_speculative_decoding_step
 (vllm/spec_decode/spec_decode_worker.py:758-858: w4a4=True for the proposer :797-801, w4a4=False
@@ -22,8 +22,16 @@ from .model import QSpecLlamaModel
 
 
 class QSpecEngine:
-    def __init__(self, model: QSpecLlamaModel, batch: int, k: int = 3, use_cuda_graph: bool = True):
+    def __init__(self, model: QSpecLlamaModel, batch: int, k: int = 3, use_cuda_graph: bool = True, temperature: float = 0.0, seed: int = 0):
+        """temperature 0: greedy, a draft token is accepted iff it is the target's arg max. Above 0: tokens are drawn from softmax(logits / temperature) and draft
+        tokens accepted with probability min(1, p / q), so that what is emitted is distributed as the target's own (vllm/model_executor/layers/
+        rejection_sampler.py); `seed` decides the random numbers."""
         self.model, self.B, self.k = model, batch, k
+        if not temperature >= 0.0:
+            raise ValueError(f"temperature must be 0 (greedy) or positive, got {temperature}")
+        if temperature and model.tp_size != 1:
+            raise NotImplementedError("sampling with a vocab-sharded lm_head")
+        self.temperature = float(temperature)
         dev = model.device
         B = batch
         assert model.max_tokens >= B * (k + 1)
@@ -50,6 +58,16 @@ class QSpecEngine:
         # apart from a last-resort early-out).
         self._len_bound = 0
         self._steps = 0
+        if self.temperature:
+            V = model.cfg.vocab_size
+            self.generator = torch.Generator(device=dev).manual_seed(seed)
+            self.draft_probs = torch.empty(k, B, V, dtype=torch.float32, device=dev)
+            self.uniform = torch.empty(2, B, k + 1, dtype=torch.float32, device=dev)     # for the drafts, and for their verification
+        if model.paged is not None:
+            self.counts = torch.full((B,), k + 1, dtype=torch.int32, device=dev)
+            self.one_each = torch.arange(B + 1, dtype=torch.int32, device=dev)
+            if model.paged.requests != B:
+                raise ValueError(f"the model's cache holds {model.paged.requests} sequences, the engine has {B}")
 
     # ---------------------------------------------------------------------------------------
     @torch.no_grad()
@@ -60,46 +78,90 @@ class QSpecEngine:
         B, P = prompt_ids.shape
         assert B == self.B and P + 1 < m.cfg.max_seq_len
         pos = torch.arange(P, dtype=torch.int32, device=m.device)
+        if m.paged is not None:                                          # the sequences of before give their pages back
+            m.paged.plan(torch.zeros_like(self.seq_len), torch.full_like(self.seq_len, -1), 0)
+            m.paged.commit()
+            held = torch.zeros_like(self.seq_len)
         chunk = max(1, m.max_tokens)
         last_hidden = torch.empty(B, m.cfg.hidden_size, dtype=torch.float16, device=m.device)
         for b in range(B):
             for s in range(0, P, chunk):
                 e = min(P, s + chunk)
                 ids = prompt_ids[b, s:e].contiguous()
-                h = m.forward(ids, pos[s:e].contiguous(), torch.full((e - s,), b, dtype=torch.int32, device=m.device),
-                              w4a4=False)
+                if m.paged is not None:
+                    counts = torch.zeros_like(held)
+                    counts[b] = e - s
+                    step = m.paged.plan(held, counts, e - s)
+                    m.paged.commit()
+                    held[b] = e
+                    h = m.forward(ids, None, None, w4a4=False, step=step)
+                else:
+                    h = m.forward(ids, pos[s:e].contiguous(), torch.full((e - s,), b, dtype=torch.int32, device=m.device),
+                                  w4a4=False)
                 if e == P:
                     last_hidden[b].copy_(h[e - s - 1])
-        self.cur_tok.copy_(m.greedy_tokens(last_hidden))
+        if self.temperature:
+            self.uniform.uniform_(generator=self.generator)
+            ops.sample_probs(self._probs(last_hidden), self.uniform[0, :, 0].contiguous(), self.cur_tok)
+        else:
+            self.cur_tok.copy_(m.greedy_tokens(last_hidden))
         self.seq_len.fill_(P)
         self._len_bound = P
         self.counters.zero_()
 
     # ---------------------------------------------------------------------------------------
+    def _probs(self, hidden: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """softmax(logits / temperature), float32 [rows, V]."""
+        return torch.softmax(self.model.logits(hidden).float().mul_(1.0 / self.temperature), -1, out=out)
+
     @torch.no_grad()
     def _spec_step(self) -> None:
         m, B, k = self.model, self.B, self.k
         tok = self.cur_tok
+        vstep = None
+        if m.paged is not None:
+            # one plan for all passes of the step: pages for k + 1 tokens of each sequence, the slots of token i of all of them in row i
+            from .paged import PagedStep
+            vstep = m.paged.plan(self.seq_len, self.counts, B * (k + 1), k + 1)
+            m.paged.commit()
+            slots, positions = (t.view(B, k + 1).t().contiguous() for t in (vstep.slots, vstep.positions))
+        if self.temperature:
+            self.uniform.uniform_(generator=self.generator)
+            draws = self.uniform[0].t().contiguous()
         # ---- proposer: k draft passes, w4a4=True (spec_decode_worker.py:797-801)
         for i in range(k):
-            pos = self.seq_len + i
-            hidden = m.forward(tok, pos, self.seq_ids, w4a4=True)
-            tok = m.greedy_tokens(hidden)
+            if vstep is not None:
+                hidden = m.forward(tok, None, None, w4a4=True, step=PagedStep(self.one_each, positions[i] + 1, positions[i], slots[i], None, 1))
+            else:
+                pos = self.seq_len + i
+                hidden = m.forward(tok, pos, self.seq_ids, w4a4=True)
+            if self.temperature:
+                tok = ops.sample_probs(self._probs(hidden, self.draft_probs[i]), draws[i], torch.empty_like(tok))
+            else:
+                tok = m.greedy_tokens(hidden)
             self.draft_toks[:, i].copy_(tok)
         # ---- scorer: one verify pass over k+1 tokens / sequence, w4a4=False (:812-813)
         vt = torch.cat((self.cur_tok.unsqueeze(1), self.draft_toks), dim=1).reshape(-1)
-        vpos = (self.seq_len.unsqueeze(1) + self.arange_k1.unsqueeze(0)).reshape(-1).contiguous()
-        hidden = m.forward(vt, vpos, self.vseq_ids, w4a4=False)
-        tgt = m.greedy_tokens(hidden).view(B, k + 1)
-        # ---- greedy rejection (spec_decode_worker.py:861-915 with temperature 0)
-        match = (tgt[:, :k] == self.draft_toks).to(torch.int64)
-        n_acc = match.cumprod(dim=1).sum(dim=1)                         # accepted draft tokens per sequence
-        nxt = tgt.gather(1, n_acc.unsqueeze(1)).squeeze(1)              # correction / bonus token
-        padded = torch.cat((self.draft_toks, nxt.unsqueeze(1)), dim=1)
-        idx = self.arange_k1.unsqueeze(0).to(torch.int64)
-        emitted = torch.where(idx < n_acc.unsqueeze(1), padded, torch.where(idx == n_acc.unsqueeze(1), nxt.unsqueeze(1), -1))
-        self.out_tokens.copy_(emitted)
-        self.out_count.copy_(n_acc + 1)
+        if vstep is not None:
+            hidden = m.forward(vt, None, None, w4a4=False, step=vstep)
+        else:
+            vpos = (self.seq_len.unsqueeze(1) + self.arange_k1.unsqueeze(0)).reshape(-1).contiguous()
+            hidden = m.forward(vt, vpos, self.vseq_ids, w4a4=False)
+        if self.temperature:
+            ops.verify_drafts(self.draft_toks, self.draft_probs.transpose(0, 1), self._probs(hidden).view(B, k + 1, -1), self.uniform[1], self.out_tokens, self.out_count)
+            n_acc, emitted = self.out_count - 1, self.out_tokens
+            nxt = emitted.gather(1, n_acc.unsqueeze(1)).squeeze(1)
+        else:
+            tgt = m.greedy_tokens(hidden).view(B, k + 1)
+            # ---- greedy rejection (spec_decode_worker.py:861-915 with temperature 0)
+            match = (tgt[:, :k] == self.draft_toks).to(torch.int64)
+            n_acc = match.cumprod(dim=1).sum(dim=1)                     # accepted draft tokens per sequence
+            nxt = tgt.gather(1, n_acc.unsqueeze(1)).squeeze(1)          # correction / bonus token
+            padded = torch.cat((self.draft_toks, nxt.unsqueeze(1)), dim=1)
+            idx = self.arange_k1.unsqueeze(0).to(torch.int64)
+            emitted = torch.where(idx < n_acc.unsqueeze(1), padded, torch.where(idx == n_acc.unsqueeze(1), nxt.unsqueeze(1), -1))
+            self.out_tokens.copy_(emitted)
+            self.out_count.copy_(n_acc + 1)
         self.cur_tok.copy_(nxt)
         self.seq_len.add_((n_acc + 1).to(torch.int32))
         self.counters[0] += n_acc.sum()
@@ -113,17 +175,32 @@ class QSpecEngine:
         if not self.use_graph or self.graph is not None:
             return
         self._check_capacity()
-        state = (self.cur_tok.clone(), self.seq_len.clone(), self.counters.clone())
+        def rng(): return self.generator.get_state() if self.temperature else None
+        paged = self.model.paged
+        live = [self.cur_tok, self.seq_len, self.counters] + ([] if paged is None else [paged.state, paged.refusals])   # (tables and lists of pages beyond these mean nothing)
+        state, draws = [t.clone() for t in live], rng()
+
+        def restore():
+            for t, kept in zip(live, state):
+                t.copy_(kept)
+            if self.temperature:
+                self.generator.set_state(draws)
         self._join_caller_stream()
         with torch.cuda.stream(self.stream):
+            if paged is not None:
+                self.counts.zero_()                        # a step of no tokens: rows that are written over leave their mark in a page's scale
             self._spec_step()
+            if paged is not None:
+                self.counts.fill_(self.k + 1)
             torch.cuda.synchronize()
-            self.cur_tok.copy_(state[0]); self.seq_len.copy_(state[1]); self.counters.copy_(state[2])
+            restore()
             g = torch.cuda.CUDAGraph()
+            if self.temperature:
+                g.register_generator_state(self.generator)
             with torch.cuda.graph(g, stream=self.stream):
                 self._spec_step()
             torch.cuda.synchronize()
-            self.cur_tok.copy_(state[0]); self.seq_len.copy_(state[1]); self.counters.copy_(state[2])
+            restore()
         torch.cuda.synchronize()
         self.graph = g
 
@@ -139,10 +216,17 @@ class QSpecEngine:
             if self._len_bound + need > S:
                 raise RuntimeError(f"KV cache exhausted: a sequence holds {self._len_bound} tokens and a speculative step "
                                    f"writes {need} more, but max_seq_len is {S}")
+        if self.model.paged is not None and self._steps % 64 == 0:
+            self._check_pages()
         peers = getattr(self.model, "peers", None)
         if peers is not None and self._steps % 64 == 0 and peers.timeouts():
             raise RuntimeError(f"tensor-parallel peer time-out: {peers.timeouts()} arrival flag(s) never came "
                                "(a rank of the group is gone); the partial sums of those steps are stale")
+
+    def _check_pages(self) -> None:
+        if refused := self.model.paged.refused():
+            raise RuntimeError(f"the 8-bit cache had no page for {refused} sequence(s) of a step: their tokens of that step are lost "
+                               f"({self.model.paged.pages} pages of {self.model.paged.page_tokens} tokens)")
 
     def _join_caller_stream(self) -> None:
         """self.stream is a non-blocking stream: work the caller queued on ITS stream (prefill, state edits) is ordered before
@@ -190,6 +274,8 @@ class QSpecEngine:
         if given_up := ops.attn_tile_timeouts():
             raise RuntimeError(f"{given_up} CTA(s) or rows gave up a wait in attention, a linear layer or the rotation before one; the outputs of "
                                "those steps hold NaN")
+        if self.model.paged is not None:
+            self._check_pages()
         acc, draft, emitted = [int(v) for v in self.counters.tolist()]
         steps = draft // (self.B * self.k) if draft else 0
         max_emit = steps * self.B * (self.k + 1)

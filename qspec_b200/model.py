@@ -46,6 +46,9 @@ class QSpecLlamaConfig:
     heads_rotation: str = "sylvester"   # o_proj rotation across heads: Sylvester FHT (2^k heads) or "had40" (:269-277)
     qk_hadamard: bool = False        # per-head FHT_128 of q and k after the rotary embedding (:279-288)
     gate_first: bool = False         # merged gate_up rows [gate ; up] (vLLM SiluAndMul, :80-86) instead of Llama's [up ; gate]
+    kv_cache: str = "f16"            # "f16": [slot, position] rows; "int8": pages of 8-bit codes (paged.PagedKV8Cache)
+    kv_page: int = 64                # tokens of a page
+    kv_pages: Optional[int] = None   # pages of the whole cache (None: enough for every sequence at its longest)
 
     @staticmethod
     def llama3_8b(**kw):
@@ -161,8 +164,21 @@ class QSpecLlamaModel(torch.nn.Module):
         self.sm_scale = 1.0 / math.sqrt(D)
         # KV cache shared by draft and verify (worker.py:309-326 ref_initilize_cache)
         L, S = cfg.num_hidden_layers, cfg.max_seq_len
-        self.cache_k = torch.zeros(L, max_batch, S, self.hkv, D, dtype=torch.float16, device=self.device)
-        self.cache_v = torch.zeros_like(self.cache_k)
+        self.max_batch = max_batch
+        if cfg.kv_cache not in ("f16", "int8"):
+            raise ValueError(f'kv_cache must be "f16" or "int8", got {cfg.kv_cache!r}')
+        self.paged = None
+        if cfg.kv_cache == "int8":
+            if cfg.qk_hadamard:
+                raise ValueError("the 8-bit cache has no form with the Hadamard of queries and keys behind the rotary embedding")
+            from .paged import PagedKV8Cache
+            self.paged = PagedKV8Cache(L, self.hkv, D, max_batch, S, max_tokens, self.device, cfg.kv_page, cfg.kv_pages)
+            self.cache_k = self.cache_v = None
+            self.buf_q = torch.empty(max_tokens, self.hq, D, dtype=torch.float16, device=self.device)     # rotated queries
+            self._ended: set = set()
+        else:
+            self.cache_k = torch.zeros(L, max_batch, S, self.hkv, D, dtype=torch.float16, device=self.device)
+            self.cache_v = torch.zeros_like(self.cache_k)
         # scratch arena, allocated once
         T, H = max_tokens, cfg.hidden_size
         f16 = dict(dtype=torch.float16, device=self.device)
@@ -208,19 +224,22 @@ class QSpecLlamaModel(torch.nn.Module):
             import torch.distributed as dist
             dist.all_reduce(t, group=self.tp_group)     # RowParallelLinear.forward, layers/linear.py:1143-1144
 
-    def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor, w4a4: bool) -> torch.Tensor:
-        """input_ids/positions/seq_ids: [T] int (int32 positions/seq_ids). Returns final-norm hidden [T, H]."""
-        for _ in self.forward_stages(input_ids, positions, seq_ids, w4a4):
+    def forward(self, input_ids: torch.Tensor, positions: Optional[torch.Tensor], seq_ids: Optional[torch.Tensor], w4a4: bool, step=None) -> torch.Tensor:
+        """input_ids/positions/seq_ids: [T] int (int32 positions/seq_ids). Returns final-norm hidden [T, H]. step: the tokens' places in the 8-bit cache
+        (`paged.PagedStep`; positions and seq_ids are not read then)."""
+        for _ in self.forward_stages(input_ids, positions, seq_ids, w4a4, step):
             pass
         return self.buf_norm[: input_ids.numel()]
 
-    def forward_stages(self, input_ids: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor, w4a4: bool):
+    def forward_stages(self, input_ids: torch.Tensor, positions: Optional[torch.Tensor], seq_ids: Optional[torch.Tensor], w4a4: bool, step=None):
         """`forward` as a generator that yields after every row-parallel GEMM (the points where the ranks of a
         tensor-parallel group exchange partial sums): lets several shards that live in ONE process be advanced in lock
         step (tests: all ranks of a TP model on one GPU). The final-norm hidden state is left in `buf_norm[:T]`."""
         cfg = self.cfg
         T = input_ids.numel()
         assert T <= self.max_tokens
+        if (step is None) != (self.paged is None):
+            raise ValueError("forward: a model with the 8-bit cache takes a step of that cache, others none")
         D, H = cfg.head_dim, cfg.hidden_size
         x = self.buf_x[:T]
         torch.index_select(self.embed, 0, input_ids, out=x)
@@ -237,7 +256,7 @@ class QSpecLlamaModel(torch.nn.Module):
         sc2 = self.buf_scale2[:T]
         # int8 container for the draft path's quantised activations (same values, same results; include/qspec_b200.h "_c8")
         # (not with the one-launch attention block, which writes the packed form, nor with the two-step peer reduction)
-        attn_block_taken = (os.environ.get("QSPEC_ATTN_FUSED", "1") != "0" and not self.qwen
+        attn_block_taken = (self.paged is None and os.environ.get("QSPEC_ATTN_FUSED", "1") != "0" and not self.qwen
                             and T <= int(os.environ.get("QSPEC_ATTN_BLOCK_MAX_T", "32"))
                             and ops.attn_block_supported(T, self.hq, self.hkv, D, self.cache_k.shape[2]))
         c8 = (w4a4 and not self.qwen and T >= int(os.environ.get("QSPEC_C8_MIN_T", "48")) and not attn_block_taken
@@ -256,12 +275,12 @@ class QSpecLlamaModel(torch.nn.Module):
         sp_a = sp_m = None                                                  # pending partial sums (attention / MLP block)
         # one-launch attention block for decode-sized passes; QSPEC_ATTN_BLOCK_MAX_T caps the token count it takes (larger
         # passes go through rope_kvcache + seq_attention + hadamard_heads)
-        fused_attn = (os.environ.get("QSPEC_ATTN_FUSED", "1") != "0" and not self.qwen
+        fused_attn = (self.paged is None and os.environ.get("QSPEC_ATTN_FUSED", "1") != "0" and not self.qwen
                       and T <= int(os.environ.get("QSPEC_ATTN_BLOCK_MAX_T", "32"))
                       and ops.attn_block_supported(T, self.hq, self.hkv, D, self.cache_k.shape[2]))
         rot_heads = ops.hadamard_heads40 if cfg.heads_rotation == "had40" else ops.hadamard_heads
         # chain path (passes the one-launch block does not take): many tokens -> one CTA per (sequence, kv head)
-        seq_attn = (not fused_attn and T >= 32 and os.environ.get("QSPEC_SEQ_ATTN", "1") != "0"
+        seq_attn = (self.paged is None and not fused_attn and T >= 32 and os.environ.get("QSPEC_SEQ_ATTN", "1") != "0"
                     and ops.seq_attention_supported(T, self.hq, self.hkv, D, self.cache_k.shape[2]))
         # Single-GPU emulation of the two-step fused all-reduce (tests/tp_emulation.py): the rows a rank owns are reduced and
         # pushed by one launch, the other rows are consumed by a second one, with every rank's first launch before any rank's
@@ -278,7 +297,7 @@ class QSpecLlamaModel(torch.nn.Module):
             self._tp_phases = 3
 
         for li, layer in enumerate(self.layers):
-            ck, cv = self.cache_k[li], self.cache_v[li]
+            ck, cv = (None, None) if self.paged is not None else (self.cache_k[li], self.cache_v[li])
             # ---- attention block (quarot_llama.py:374-380)
             if w4a4:
                 first8 = c8 and pending                     # the very first norm of a pass has no producer GEMM: packed
@@ -300,12 +319,18 @@ class QSpecLlamaModel(torch.nn.Module):
                     ops.attn_block(qkv, self.cos_sin, positions, seq_ids, ck, cv, self.hq, self.hkv, D, self.sm_scale,
                                    self.scale_heads, out=had)
             else:
-                if cfg.qk_hadamard:
+                if self.paged is not None:
+                    q = self.buf_q[:T]
+                    self.paged.append(li, qkv, self.cos_sin, step, q)
+                    self.paged.attend(li, q, step, attn.view(T, self.hq, D), self.sm_scale)
+                elif cfg.qk_hadamard:
                     ops.rope_qkhad_kvcache(qkv, self.cos_sin, positions, seq_ids, ck, cv, self.hq, self.hkv, D,
                                            1.0 / math.sqrt(D))            # head_had_scale, qwen2_quarot.py:219
                 else:
                     ops.rope_kvcache(qkv, self.cos_sin, positions, seq_ids, ck, cv, self.hq, self.hkv, D)
-                if seq_attn:
+                if self.paged is not None:
+                    pass
+                elif seq_attn:
                     ops.seq_attention(qkv, ck, cv, positions, seq_ids, attn, self.hq, self.hkv, D, self.sm_scale)
                 else:
                     ops.decode_attention(qkv, ck, cv, positions, seq_ids, attn, self.hq, self.hkv, D, self.sm_scale)
@@ -355,7 +380,7 @@ class QSpecLlamaModel(torch.nn.Module):
     # ---- what `scheduler.Scheduler` drives (plain decoding through the verify-mode path) ---------------------------
     @property
     def n_slots(self) -> int:
-        return self.cache_k.shape[1]
+        return self.max_batch
 
     @property
     def max_step_tokens(self) -> int:
@@ -371,7 +396,42 @@ class QSpecLlamaModel(torch.nn.Module):
 
     def forward_batch(self, input_ids: torch.Tensor, meta) -> torch.Tensor:
         """A flat token batch described by a `state.BatchMeta` (slot and position per token) in W4A16 mode."""
+        if self.paged is not None:
+            return self._forward_batch_paged(input_ids, meta)
         return self.forward(input_ids.to(torch.int64), meta.pos.contiguous(), meta.slot.contiguous(), w4a4=False)
+
+    def release_slot(self, slot: int) -> None:
+        """The sequence in this slot has ended (`scheduler.Scheduler.release`): its pages go back with the next step."""
+        if self.paged is not None:
+            self._ended.add(slot)
+
+    def _forward_batch_paged(self, input_ids: torch.Tensor, meta) -> torch.Tensor:
+        cache, B = self.paged, self.max_batch
+        def on_device(x):
+            return torch.tensor(x, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+        if self._ended:
+            cache.plan(on_device([0] * B), on_device([-1 if b in self._ended else 0 for b in range(B)]), 0)
+            cache.commit()
+            self._ended.clear()
+        # the cache's operators take tokens in the order of the slots
+        order = sorted(range(len(meta.segments)), key=lambda i: meta.segments[i][1])
+        lengths, counts = [0] * B, [0] * B
+        for _, slot, first, n in meta.segments:
+            lengths[slot], counts[slot] = first, n
+        step = cache.plan(on_device(lengths), on_device(counts), meta.ntok, max(counts))
+        cache.commit()
+        if self.cfg.kv_pages is not None and cache.refused():        # (with the default number of pages every sequence fits)
+            raise RuntimeError(f"the 8-bit cache is full: {cache.pages} pages of {cache.page_tokens} tokens")
+        ids = input_ids.to(torch.int64)
+        if order == list(range(len(order))):
+            return self.forward(ids, None, None, w4a4=False, step=step)
+        begin = [0]
+        for _, _, _, n in meta.segments:
+            begin.append(begin[-1] + n)
+        there = [t for i in order for t in range(begin[i], begin[i + 1])]
+        back = sorted(range(len(there)), key=there.__getitem__)
+        hidden = self.forward(ids.index_select(0, on_device(there)), None, None, w4a4=False, step=step)
+        return hidden.index_select(0, on_device(back))
 
     def logits(self, hidden_rows: torch.Tensor) -> torch.Tensor:
         if self.tp_size != 1:

@@ -7,7 +7,8 @@ function proper -- given token ids per request it advances their state and retur
 `bin/trace_run` replays recorded steps through the same `feed`.
 
 A model plugs in with: `n_slots`, `max_step_tokens`, `vocab_size`, `device`, `forward_batch(input_ids, meta) -> hidden`,
-`logits(hidden_rows) -> [n, vocab]`, and optionally `max_seq_len` (models whose cache bounds the sequence length).
+`logits(hidden_rows) -> [n, vocab]`, and optionally `max_seq_len` (models whose cache bounds the sequence length) and `release_slot(slot)` (models
+whose slots hold more than their own memory).
 Sampling is the framework's greedy arg max (`ops.argmax_rows`), as in the speculative engine (`engine.QSpecEngine`).
 
 The reference delegates this layer to vLLM's scheduler (vllm/core/scheduler.py) and LLMEngine.step
@@ -111,7 +112,11 @@ class Scheduler:
     def release(self, rid: Hashable) -> None:
         """The request is finished: its slot returns to the pool."""
         if rid in self.table.slot_of:
+            slot = self.table.slot_of[rid]
             self.table.close(rid)
+            release = getattr(self.model, "release_slot", None)        # a model whose slots hold pages takes them back
+            if release is not None:
+                release(slot)
 
     # ---- generation -------------------------------------------------------------------------------------------------
     def add(self, rid: Hashable, prompt: Sequence[int], max_new_tokens: int, eos: Optional[int] = None) -> None:
