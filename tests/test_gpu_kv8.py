@@ -500,3 +500,45 @@ def test_wrong_shapes_types_and_overlaps_are_refused():
             ops.kv8_attention(*[bad if j == i else a for j, a in enumerate(att)])
     with pytest.raises(ValueError):
         ops.kv8_read(*cache, z(3), half(3, 2, 64), half(2, 2, 64))
+
+
+@pytest.mark.parametrize("counts", [[1, 2], [1, 90]])
+def test_attention_of_tiny_queries_over_tiny_scales(counts):
+    """Factors of scores below float32's normal range must not turn a hidden key's minus infinity into no number."""
+    q, k, v, ks, vs, table, start, lens = make_attention(13, [70, 200], counts, 4, 2, 128, 32, torch.bfloat16, q_scale=1e-30)
+    ks.fill_(2.0 ** -60)
+    check_attention((q, k, v, ks, vs, table, start, lens), 128)
+
+
+GIVE_UP = r"""
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+from test_gpu_kv8 import make_attention, attention_in_64_bits
+from qspec_b200 import _lib, ops
+lib = _lib.load()
+for D, dtype in ((128, torch.float16), (64, torch.bfloat16)):
+    q, k, v, ks, vs, table, start, lens = make_attention(3, [500, 900, 40], [130, 300, 1], 8, 2, D, 32, dtype)
+    work = ops.kv8_attention_workspace("cuda")
+    good = ops.kv8_attention(q, k, v, ks, vs, table, start, lens, torch.empty_like(q), D ** -0.5, work)
+    for roles in (1, 2, 4, 8, 15):
+        before, out = ops.attn_tile_timeouts(), torch.zeros_like(q)
+        _lib.check(lib.qspec_debug_kv8_attention_give_up(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(),
+                                                         start.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), len(q), 3, table.shape[1], 8, 2, D, k.shape[0],
+                                                         32, 300, D ** -0.5, int(dtype == torch.bfloat16), work.data_ptr(), work.numel(), roles,
+                                                         torch.cuda.current_stream().cuda_stream), "give up")
+        assert ops.attn_tile_timeouts() > before, roles
+        assert out[:430].isnan().all() and torch.equal(out[430:], good[430:]), roles   # the request with few rows is the other form's
+        again = ops.kv8_attention(q, k, v, ks, vs, table, start, lens, torch.empty_like(q), D ** -0.5, work)
+        assert torch.equal(again, good) and ops.attn_tile_timeouts() > before
+print("ok")
+"""
+
+
+def test_a_wait_that_is_given_up_shows_and_leaves_nothing_behind():
+    import os
+    import subprocess
+    import sys
+    tests = os.path.dirname(os.path.abspath(__file__))
+    run = subprocess.run([sys.executable, "-c", GIVE_UP.format(root=os.path.dirname(tests), tests=tests)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip().endswith("ok"), run.stdout + run.stderr
