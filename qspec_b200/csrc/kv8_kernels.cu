@@ -370,11 +370,11 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const 
   constexpr int LANES = D / 16, ROWS = 32 / LANES, W = WIDE ? APPEND_WARPS : 1;
   __shared__ float s_max[APPEND_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = blockIdx.x * a.block, t1 = min(t0 + a.block, a.ntok);
-  const int units = WIDE ? 2 * a.G : (2 * a.G + APPEND_WARPS - 1) / APPEND_WARPS;   // CTAs in y that write pages; the others turn queries
+  const int t0 = blockIdx.y * a.block, t1 = min(t0 + a.block, a.ntok);
+  const int units = WIDE ? 2 * a.G : (2 * a.G + APPEND_WARPS - 1) / APPEND_WARPS;   // CTAs in x that write pages; the others turn queries
   pdl_enter();
-  if ((int)blockIdx.y < units) {
-    const int u = WIDE ? blockIdx.y : blockIdx.y * APPEND_WARPS + warp;
+  if ((int)blockIdx.x < units) {
+    const int u = WIDE ? blockIdx.x : blockIdx.x * APPEND_WARPS + warp;
     if (u >= 2 * a.G) return;
     const int g = u >> 1;
     // slots from the token before this CTA's first on, two a lane: which begin a run, and where runs end as far as that shows
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const 
     }
   } else {
     const int c = lane % LANES, rows = (t1 - t0) * a.H, per = APPEND_WARPS * ROWS;
-    for (int r = ((int)blockIdx.y - units) * per + warp * ROWS + lane / LANES; r < rows; r += ((int)gridDim.y - units) * per) {
+    for (int r = ((int)blockIdx.x - units) * per + warp * ROWS + lane / LANES; r < rows; r += ((int)gridDim.x - units) * per) {
       const int tl = a.H == 1 ? r : (int)__umulhi((unsigned)r, a.h_inv), t = t0 + tl, h = r - tl * a.H;
       const int p = a.positions[t];
       if (p < 0 || p >= a.cos_rows) continue;
@@ -487,7 +487,8 @@ extern "C" int qspec_kv8_append(const void* qkv, long long ld, const void* cos_s
   a.block = wide ? std::min(page_tokens, 31) : 1;           // (with the token before them one a lane)
   const int rows = APPEND_WARPS * 32 * 16 / D;              // query rows that a CTA takes at a time
   const int y = (wide ? 2 * G : (2 * G + APPEND_WARPS - 1) / APPEND_WARPS) + (q_out ? (a.block * H + 2 * rows - 1) / (2 * rows) : 0);
-  const dim3 grid((ntok + a.block - 1) / a.block, y);
+  const dim3 grid(y, (ntok + a.block - 1) / a.block);       // (the parts of a block of tokens side by side: page writers wait, queries stream)
+  QSPEC_REQUIRE(grid.y <= 65535, QSPEC_ERR_UNSUPPORTED, "kv8_append: %d tokens are too many for one call", ntok);
   auto pick = [&](auto few, auto many) { return wide ? many : few; };
   auto kern = dtype == QSPEC_DTYPE_F16 ? (D == 128 ? pick(kv8_append_kernel<false, 128, false>, kv8_append_kernel<false, 128, true>)
                                                    : pick(kv8_append_kernel<false, 64, false>, kv8_append_kernel<false, 64, true>))

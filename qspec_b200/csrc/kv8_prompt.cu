@@ -228,9 +228,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   } else if (warp >= W_CONVERT) {
     // ---- codes: 16 bytes a lane, 16 rows (one page's) at a time
     constexpr int CH = D / 16, ROWS = CONVERT * 32 / CH, STEPS = 128 / ROWS;   // pieces of a row, rows at a time, times
-    const int ct = tid - W_CONVERT * 32, c = ct % CH, row0 = ct / CH;
+    const int ct = tid - W_CONVERT * 32;
+    // (eight lanes take four pieces of two rows, so that their stores meet in no bank)
+    const int c = D == 128 ? (ct >> 3 & 1) * 4 + (ct & 3) : ct & 3, row0 = D == 128 ? (ct >> 4) * 2 + (ct >> 2 & 1) : ct >> 2;
     const uint32_t part = (uint32_t)(c >> 2) * PARTB;
-    const bool swap = c >= 4;                             // these lanes store their second piece first, so that eight stores meet in no bank
     uint4 kw[STEPS], vw[STEPS];
     auto load = [&](uint4 (&w)[STEPS], const signed char* codes, int n) {
       const Block& f = s_block[n % FACS];
@@ -256,15 +257,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         const int row = i * ROWS + row0;
-        const uint32_t x[4] = {(swap ? w[i].z : w[i].x) ^ 0x80808080u, (swap ? w[i].w : w[i].y) ^ 0x80808080u, (swap ? w[i].x : w[i].z) ^ 0x80808080u,
-                               (swap ? w[i].y : w[i].w) ^ 0x80808080u};
+        const uint32_t x[4] = {w[i].x ^ 0x80808080u, w[i].y ^ 0x80808080u, w[i].z ^ 0x80808080u, w[i].w ^ 0x80808080u};
         const uint32_t at = dst + part + row * 128;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int piece = ((c & 3) * 2 + (swap ? 1 - e : e)) ^ (row & 7);
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at + (piece << 4)), "r"(first_two(x[2 * e])), "r"(last_two(x[2 * e])),
+        for (int e = 0; e < 2; ++e)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(at + ((((c & 3) * 2 + e) ^ (row0 & 7)) << 4)), "r"(first_two(x[2 * e])), "r"(last_two(x[2 * e])),
                        "r"(first_two(x[2 * e + 1])), "r"(last_two(x[2 * e + 1])) : "memory");
-        }
       }
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       __syncwarp();
@@ -372,7 +370,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       const unsigned bad = f.bad;
       const bool odd = !plain || bad;
       // Loops over 32 columns, not unrolled: three kinds of warps run at once, and with the block's 128 columns laid out in a row they waited for their
-      // instructions more than for anything else (4.2 of 12 cycles an instruction; prompt of 2000 after 1000, 32 / 8 heads 207 us, so @@).
+      // instructions more than for anything else (4.2 of 12 cycles an instruction; prompt of 2000 after 1000, 32 / 8 heads 207 us, so 137).
       // What a row does not see, and of a page that there is not, or whose scale is no number, what makes the rows NaN that do see it:
       auto hide = [&](uint32_t (&x)[32], int c0) {
 #pragma unroll
@@ -395,7 +393,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         for (int q = 0; q < 2; ++q) {
           float t[2] = {__uint_as_float(x[q * 16]), __uint_as_float(x[q * 16 + 1])};
 #pragma unroll
-          for (int j = 2; j < 16; ++j) t[j & 1] = fmaxf(t[j & 1], __uint_as_float(x[q * 16 + j]));
+          for (int j = 2; j < 16; j += 4) {               // (three operands: one instruction)
+            t[0] = fmaxf(fmaxf(t[0], __uint_as_float(x[q * 16 + j])), __uint_as_float(x[q * 16 + j + 1]));
+            if (j + 2 < 16) t[1] = fmaxf(fmaxf(t[1], __uint_as_float(x[q * 16 + j + 2])), __uint_as_float(x[q * 16 + j + 3]));
+          }
           const float k = normal((q ? kf.y : kf.x) * rowf);
           mn = fmaxf(mn, fmaf(fmaxf(t[0], t[1]), k, fmaf(-sum128, k, q ? lv.y : lv.x)));
         }
