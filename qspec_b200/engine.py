@@ -63,11 +63,12 @@ class QSpecEngine:
             self.generator = torch.Generator(device=dev).manual_seed(seed)
             self.draft_probs = torch.empty(k, B, V, dtype=torch.float32, device=dev)
             self.uniform = torch.empty(2, B, k + 1, dtype=torch.float32, device=dev)     # for the drafts, and for their verification
-        if model.paged is not None:
+        self.paged = getattr(model, "paged", None)                    # the model's 8-bit cache, if it has one
+        if self.paged is not None:
             self.counts = torch.full((B,), k + 1, dtype=torch.int32, device=dev)
             self.one_each = torch.arange(B + 1, dtype=torch.int32, device=dev)
-            if model.paged.requests != B:
-                raise ValueError(f"the model's cache holds {model.paged.requests} sequences, the engine has {B}")
+            if self.paged.requests != B:
+                raise ValueError(f"the model's cache holds {self.paged.requests} sequences, the engine has {B}")
 
     # ---------------------------------------------------------------------------------------
     @torch.no_grad()
@@ -78,9 +79,9 @@ class QSpecEngine:
         B, P = prompt_ids.shape
         assert B == self.B and P + 1 < m.cfg.max_seq_len
         pos = torch.arange(P, dtype=torch.int32, device=m.device)
-        if m.paged is not None:                                          # the sequences of before give their pages back
-            m.paged.plan(torch.zeros_like(self.seq_len), torch.full_like(self.seq_len, -1), 0)
-            m.paged.commit()
+        if self.paged is not None:                                          # the sequences of before give their pages back
+            self.paged.plan(torch.zeros_like(self.seq_len), torch.full_like(self.seq_len, -1), 0)
+            self.paged.commit()
             held = torch.zeros_like(self.seq_len)
         chunk = max(1, m.max_tokens)
         last_hidden = torch.empty(B, m.cfg.hidden_size, dtype=torch.float16, device=m.device)
@@ -88,11 +89,11 @@ class QSpecEngine:
             for s in range(0, P, chunk):
                 e = min(P, s + chunk)
                 ids = prompt_ids[b, s:e].contiguous()
-                if m.paged is not None:
+                if self.paged is not None:
                     counts = torch.zeros_like(held)
                     counts[b] = e - s
-                    step = m.paged.plan(held, counts, e - s)
-                    m.paged.commit()
+                    step = self.paged.plan(held, counts, e - s)
+                    self.paged.commit()
                     held[b] = e
                     h = m.forward(ids, None, None, w4a4=False, step=step)
                 else:
@@ -119,11 +120,11 @@ class QSpecEngine:
         m, B, k = self.model, self.B, self.k
         tok = self.cur_tok
         vstep = None
-        if m.paged is not None:
+        if self.paged is not None:
             # one plan for all passes of the step: pages for k + 1 tokens of each sequence, the slots of token i of all of them in row i
             from .paged import PagedStep
-            vstep = m.paged.plan(self.seq_len, self.counts, B * (k + 1), k + 1)
-            m.paged.commit()
+            vstep = self.paged.plan(self.seq_len, self.counts, B * (k + 1), k + 1)
+            self.paged.commit()
             slots, positions = (t.view(B, k + 1).t().contiguous() for t in (vstep.slots, vstep.positions))
         if self.temperature:
             self.uniform.uniform_(generator=self.generator)
@@ -176,7 +177,7 @@ class QSpecEngine:
             return
         self._check_capacity()
         def rng(): return self.generator.get_state() if self.temperature else None
-        paged = self.model.paged
+        paged = self.paged
         live = [self.cur_tok, self.seq_len, self.counters] + ([] if paged is None else [paged.state, paged.refusals])   # (tables and lists of pages beyond these mean nothing)
         state, draws = [t.clone() for t in live], rng()
 
@@ -216,7 +217,7 @@ class QSpecEngine:
             if self._len_bound + need > S:
                 raise RuntimeError(f"KV cache exhausted: a sequence holds {self._len_bound} tokens and a speculative step "
                                    f"writes {need} more, but max_seq_len is {S}")
-        if self.model.paged is not None and self._steps % 64 == 0:
+        if self.paged is not None and self._steps % 64 == 0:
             self._check_pages()
         peers = getattr(self.model, "peers", None)
         if peers is not None and self._steps % 64 == 0 and peers.timeouts():
@@ -224,9 +225,9 @@ class QSpecEngine:
                                "(a rank of the group is gone); the partial sums of those steps are stale")
 
     def _check_pages(self) -> None:
-        if refused := self.model.paged.refused():
+        if refused := self.paged.refused():
             raise RuntimeError(f"the 8-bit cache had no page for {refused} sequence(s) of a step: their tokens of that step are lost "
-                               f"({self.model.paged.pages} pages of {self.model.paged.page_tokens} tokens)")
+                               f"({self.paged.pages} pages of {self.paged.page_tokens} tokens)")
 
     def _join_caller_stream(self) -> None:
         """self.stream is a non-blocking stream: work the caller queued on ITS stream (prefill, state edits) is ordered before
@@ -274,7 +275,7 @@ class QSpecEngine:
         if given_up := ops.attn_tile_timeouts():
             raise RuntimeError(f"{given_up} CTA(s) or rows gave up a wait in attention, a linear layer or the rotation before one; the outputs of "
                                "those steps hold NaN")
-        if self.model.paged is not None:
+        if getattr(self.model, "paged", None) is not None:
             self._check_pages()
         acc, draft, emitted = [int(v) for v in self.counters.tolist()]
         steps = draft // (self.B * self.k) if draft else 0
