@@ -4,6 +4,7 @@
 // Cache of a layer: codes int8 [pages, G, P, D] (a page's rows of one head are P * D bytes in a row) and scales float32 [pages, G] for keys and for
 // values; a code c stands for c * scale. P tokens a page: a power of two from 16 to 128. A slot is page * P + row.
 #include "kv8_common.cuh"
+#include <type_traits>
 
 namespace qspec {
 namespace kv8 {
@@ -192,9 +193,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
 }
 
 // ---- rows into pages --------------------------------------------------------------------------------------------------------------
-// A run (the consecutive tokens of one page) is one warp's per head, for keys and values each, where there are few tokens, and a CTA's in a prompt. Eight
-// lanes a row, four rows of a warp at a time; a lane holds sixteen of its values, eight of each half, so that it has both of every pair that the rotation
-// turns. The page's scale is the largest |x| of all rows: those that fit into registers stay there between the maximum and the codes, others are read
+// A run (the consecutive tokens of one page) of up to SHORT tokens is one warp's per head, for keys and values each, a longer one a CTA's (a warp for each of
+// these, too: a prompt of 4200 tokens, 40 / 8 heads, without its queries 25.5 us, so 11; all by a CTA: 1024 requests of a token each 44 us, so 12). Eight lanes
+// a row, four rows of a warp at a time; a lane holds sixteen of its values, eight of each half, so that it has both of every pair that the rotation turns. The page's scale is the largest |x| of all rows: those that fit into registers stay there between the maximum and the codes, others are read
 // again. A decode step's call is one load, a reduction and a store long: without barriers.
 // Rotation and codes are evaluated with the roundings that their formulas have (no fused multiply-adds), so that the same codes come out of every
 // implementation in float32.
@@ -209,7 +210,7 @@ struct AppendArgs {
   unsigned h_inv;                                 // r * h_inv >> 32 = r / H for the rows of a CTA's tokens
 };
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;   // 2^-60
-constexpr int APPEND_WARPS = 8;
+constexpr int APPEND_WARPS = 8, SHORT = 8;        // warps of a CTA; tokens of a run up to which it is one warp's
 
 // the slot of token t, or -1 if nothing is to be written for it
 __device__ __forceinline__ int slot_of(const AppendArgs& a, int t) {
@@ -363,20 +364,18 @@ __device__ __forceinline__ void write_run(const AppendArgs& a, int t0, int n, in
   if (warp == 0 && lane == 0 && after != before) *scale = after;
 }
 
-// WIDE: a CTA per run, head and side (prompts: runs of whole pages). Otherwise a warp.
-template <bool BF16, int D, bool WIDE>
+// 2 G CTAs per block of tokens write the runs that begin in it: of long ones each all that belongs to a head and side, by all of its warps together; of short ones
+// every warp what belongs to a run, head and side, the heads of a run next to each other. The CTAs behind them turn the block's queries.
+template <bool BF16, int D>
 __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const AppendArgs a) {
   using T = typename Elem16<BF16>::T;
-  constexpr int LANES = D / 16, ROWS = 32 / LANES, W = WIDE ? APPEND_WARPS : 1;
+  constexpr int LANES = D / 16, ROWS = 32 / LANES;
   __shared__ float s_max[APPEND_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = blockIdx.y * a.block, t1 = min(t0 + a.block, a.ntok);
-  const int units = WIDE ? 2 * a.G : (2 * a.G + APPEND_WARPS - 1) / APPEND_WARPS;   // CTAs in x that write pages; the others turn queries
+  const int units = 2 * a.G;                                // CTAs in x that write pages
   pdl_enter();
   if ((int)blockIdx.x < units) {
-    const int u = WIDE ? blockIdx.x : blockIdx.x * APPEND_WARPS + warp;
-    if (u >= 2 * a.G) return;
-    const int g = u >> 1;
     // slots from the token before this CTA's first on, two a lane: which begin a run, and where runs end as far as that shows
     const int sa = slot_of(a, t0 - 1 + lane), sb = slot_of(a, t0 + 31 + lane);
     const int before = __shfl_up_sync(0xffffffffu, sa, 1), mask = (1 << a.pshift) - 1;
@@ -384,12 +383,27 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const 
     const int last = __shfl_sync(0xffffffffu, sa, 31), before_b = __shfl_up_sync(0xffffffffu, sb, 1);
     const bool go_on_b = sb >= 0 && (sb & mask) && (lane ? before_b : last) == sb - 1;
     const uint64_t in_run = ((uint64_t)__ballot_sync(0xffffffffu, go_on) | (uint64_t)__ballot_sync(0xffffffffu, go_on_b) << 32) >> 1;   // bit i: token t0 + i
-    for (uint32_t left = __ballot_sync(0xffffffffu, lane > 0 && t0 - 1 + lane < t1 && sa >= 0 && !go_on) >> 1; left; left &= left - 1u) {
-      const int i = __ffs(left) - 1, t = t0 + i, s = __shfl_sync(0xffffffffu, sa, i + 1);
-      int n = 1 + (__ffsll((long long)~(in_run >> (i + 1))) - 1);
-      if (t + n >= t0 + 63) n = run_of(a, t, s, n);         // (it may be longer than that)
+    const uint32_t begin = __ballot_sync(0xffffffffu, lane > 0 && t0 - 1 + lane < t1 && sa >= 0 && !go_on) >> 1;
+    uint64_t more = in_run >> 1;                            // bit i: the SHORT tokens behind t0 + i are in its run
+#pragma unroll
+    for (int o = 1; o < SHORT; o <<= 1) more &= more >> o;
+    auto write = [&](int i, int n, int u, auto warps) {     // the run of n tokens that begins with token t0 + i
+      constexpr int W = decltype(warps)::value;
+      const int t = t0 + i, s = __shfl_sync(0xffffffffu, sa, i + 1), g = u >> 1;
+      if (W > 1 && t + n >= t0 + 63) n = run_of(a, t, s, n);   // (it may be longer than that)
       if (u & 1) write_run<BF16, D, false, W>(a, t, n, s, g, (a.H + a.G + g) * D, a.v, a.vs, s_max);
       else write_run<BF16, D, true, W>(a, t, n, s, g, (a.H + g) * D, a.k, a.ks, s_max);
+    };
+    auto tokens = [&](int i) { return __ffsll((long long)~(in_run >> (i + 1))); };
+    for (uint32_t left = begin & (uint32_t)more; left; left &= left - 1u) {
+      const int i = __ffs(left) - 1;
+      write(i, tokens(i), blockIdx.x, std::integral_constant<int, APPEND_WARPS>());
+    }
+    const uint32_t brief = begin & ~(uint32_t)more;
+    const int rank = brief >> lane & 1u ? __popc(brief & ((1u << lane) - 1u)) : -1, all = __popc(brief) * units;
+    for (int id = blockIdx.x * APPEND_WARPS + warp; id < all; id += units * APPEND_WARPS) {
+      const int j = id / units, i = __ffs(__ballot_sync(0xffffffffu, rank == j)) - 1;
+      write(i, tokens(i), id - j * units, std::integral_constant<int, 1>());
     }
   } else {
     const int c = lane % LANES, rows = (t1 - t0) * a.H, per = APPEND_WARPS * ROWS;
@@ -480,20 +494,17 @@ extern "C" int qspec_kv8_append(const void* qkv, long long ld, const void* cos_s
   QSPEC_REQUIRE(ld >= (long long)(H + 2 * G) * D && ld % 8 == 0 && (!q_out || (q_tok_stride >= (long long)H * D && q_tok_stride % 8 == 0)) && ((uintptr_t)qkv & 15) == 0 &&
                     ((uintptr_t)cos_sin & 15) == 0 && ((uintptr_t)q_out & 15) == 0,
                 QSPEC_ERR_INVALID_ARG, "kv8_append: rows must lie on 16-byte boundaries (ld=%lld)", ld);
-  AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (signed char*)k, (signed char*)v, ks, vs, q_out, q_tok_stride, ntok, H, G, npages, page_shift(page_tokens), 1, (unsigned)(((1ull << 32) + H - 1) / H)};   // (31 * 4096 rows at most: r times what h_inv is too large by stays below 2^32)
-  // Few tokens: a CTA looks at one, which is likely to begin a run. A prompt: at a page's or so, with a CTA for each run, head and side
-  // (4200 tokens, 40 / 8 heads, pages of 32, rows without queries: 25.5 us with a warp for each, so 11.8).
-  const bool wide = ntok > 512;
-  a.block = wide ? std::min(page_tokens, 31) : 1;           // (with the token before them one a lane)
+  AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (signed char*)k, (signed char*)v, ks, vs, q_out, q_tok_stride, ntok, H, G, npages, page_shift(page_tokens), 1,
+               (unsigned)(((1ull << 32) + H - 1) / H)};    // (31 * 4096 rows at most: r times what h_inv is too large by stays below 2^32)
+  // Small blocks put more CTAs on a call with few tokens, large ones have fewer that find nothing to begin (32 / 8 heads of 128, pages of 16, us with blocks of 8, 16
+  // and 31: 64 requests of a token 3.0, 3.8, 5.9; 200 of 6 tokens 10.5, 9.1, 8.5; one prompt of 256 3.8, 4.3, 5.2; of 512 5.6, 5.2, 5.7; of 4200 35.8, 30.6, 29.1).
+  a.block = ntok <= 256 ? 8 : ntok <= 1024 ? 16 : 31;       // (31: with the token before them one a lane)
   const int rows = APPEND_WARPS * 32 * 16 / D;              // query rows that a CTA takes at a time
-  const int y = (wide ? 2 * G : (2 * G + APPEND_WARPS - 1) / APPEND_WARPS) + (q_out ? (a.block * H + 2 * rows - 1) / (2 * rows) : 0);
-  const dim3 grid(y, (ntok + a.block - 1) / a.block);       // (the parts of a block of tokens side by side: page writers wait, queries stream)
+  // (the parts of a block of tokens side by side: page writers wait, queries stream)
+  const dim3 grid(2 * G + (q_out ? (a.block * H + 2 * rows - 1) / (2 * rows) : 0), (ntok + a.block - 1) / a.block);
   QSPEC_REQUIRE(grid.y <= 65535, QSPEC_ERR_UNSUPPORTED, "kv8_append: %d tokens are too many for one call", ntok);
-  auto pick = [&](auto few, auto many) { return wide ? many : few; };
-  auto kern = dtype == QSPEC_DTYPE_F16 ? (D == 128 ? pick(kv8_append_kernel<false, 128, false>, kv8_append_kernel<false, 128, true>)
-                                                   : pick(kv8_append_kernel<false, 64, false>, kv8_append_kernel<false, 64, true>))
-                                       : (D == 128 ? pick(kv8_append_kernel<true, 128, false>, kv8_append_kernel<true, 128, true>)
-                                                   : pick(kv8_append_kernel<true, 64, false>, kv8_append_kernel<true, 64, true>));
+  auto kern = dtype == QSPEC_DTYPE_F16 ? (D == 128 ? kv8_append_kernel<false, 128> : kv8_append_kernel<false, 64>)
+                                       : (D == 128 ? kv8_append_kernel<true, 128> : kv8_append_kernel<true, 64>);
   QSPEC_CUDA(launch_pdl(kern, grid, dim3(APPEND_WARPS * 32), 0, (cudaStream_t)stream, a));
   QSPEC_CHECK_LAUNCH(1);
   return QSPEC_OK;
