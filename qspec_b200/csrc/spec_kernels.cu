@@ -230,8 +230,10 @@ extern "C" int qspec_verify_drafts(const long long* drafted, const float* draft,
   Args a{drafted, draft, target, uniform, draft_counts, draft_seq_stride, draft_place_stride, target_seq_stride, target_place_stride, tokens, emitted, drafts, vocab, 0};
   const bool vec = (((uintptr_t)target | (uintptr_t)(drafts ? draft : target)) & 15) == 0 && ((target_seq_stride | target_place_stride) & 3) == 0 &&
                    (drafts == 0 || ((draft_seq_stride | draft_place_stride) & 3) == 0);
-  // CTAs of a request: eight where there are few requests (the rows' way through the GPU counts), four where they fill it by themselves.
-  const bool many = requests >= 96 && vocab <= 4 * MAX_TILES * TILE;
+  // CTAs of a request: eight where two rounds of such clusters hold all requests (a row's way through the GPU counts), four where they fill it by themselves. Three
+  // drafts, us with eight (four): vocabulary of 152064, 64 requests 13.7 (16.8), 80: 20.7 (18.0), 96: 23.6 (19.2), 128: 28.0 (32.0), 190: 41.6 (38.8), 256: 53.4 (53.0);
+  // of 32000, 16: 6.2 (5.9), 64: 7.6 (7.7), 80: 10.6 (7.9), 128: 12.7 (11.0), 256: 22.6 (17.2).
+  const bool many = requests > sm_count() / 2 && vocab <= 4 * MAX_TILES * TILE;
   const int cluster = many ? 4 : 8;
   a.span = ((vocab + cluster - 1) / cluster + TILE - 1) / TILE * TILE;
   cudaLaunchConfig_t cfg = {};

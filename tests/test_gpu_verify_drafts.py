@@ -63,7 +63,7 @@ def check(*case, counts=None):
     return got
 
 
-@pytest.mark.parametrize("B,k,V", [(1, 0, 1), (1, 1, 2), (3, 2, 31), (2, 3, 255), (5, 1, 256), (4, 3, 257), (7, 4, 2049), (64, 3, 4100), (3, 31, 1000), (4, 3, 128256), (2, 5, 151643)])
+@pytest.mark.parametrize("B,k,V", [(1, 0, 1), (1, 1, 2), (3, 2, 31), (2, 3, 255), (5, 1, 256), (4, 3, 257), (7, 4, 2049), (64, 3, 4100), (3, 31, 1000), (4, 3, 128256), (2, 5, 151643), (74, 1, 5000), (75, 1, 5000), (90, 2, 128256), (130, 3, 32001)])
 def test_verified_tokens_are_those_of_the_rule(B, k, V):
     for seed in range(3):
         check(*make(seed, B, k, V, agree=0.7))
