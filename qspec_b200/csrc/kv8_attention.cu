@@ -37,7 +37,8 @@ struct AttArgs {
   const signed char *k, *v;
   const float *ks, *vs;
   const int *table, *q_start, *kv_len;
-  int nreq, width, npages, pshift, ntok, G, rep, max_rows;   // max_rows: requests with more rows than that are another kernel's
+  int nreq, width, npages, pshift, ntok, G, rep;
+  unsigned share;                                // to_prompt_form()'s; 0: there is no prompt form in this call
   float scale2;                                  // scale * log2(e)
   void* out; long long out_ts; int out_hs;
   int* counters; float* parts;
@@ -81,13 +82,13 @@ struct Req {
   int first, n, keys, tiles, units;               // first row of q, tokens, keys, row tiles, units of an item
   __device__ __forceinline__ long long total(int G) const { return (long long)tiles * G * units; }
 };
-__device__ __forceinline__ Req request(const AttArgs& a, int b) {
+__device__ __forceinline__ Req request(const AttArgs& a, int b, unsigned long long work) {
   Req r;
   r.first = min(max(a.q_start[b], 0), a.ntok);
   r.n = max(min(a.q_start[b + 1], a.ntok) - r.first, 0);
   r.keys = max(a.kv_len[b], 0);
   const long long rows = (long long)r.n * a.rep;
-  r.tiles = rows <= a.max_rows ? (int)((rows + ROWS - 1) / ROWS) : 0;
+  r.tiles = to_prompt_form(r.n, r.keys, a.rep, a.share, work) ? 0 : (int)((rows + ROWS - 1) / ROWS);
   r.units = max((r.keys + UNIT - 1) / UNIT, 1);   // a request without keys has a unit that shows its rows none
   return r;
 }
@@ -96,7 +97,7 @@ __device__ __forceinline__ Req request(const AttArgs& a, int b) {
 struct Place {
   int b, g, tile, u;
   Req r;
-  __device__ __forceinline__ void forward(const AttArgs& a, int steps) {
+  __device__ __forceinline__ void forward(const AttArgs& a, unsigned long long work, int steps) {
     u += steps;
     while (b < a.nreq && u >= r.units) {
       u -= r.units;
@@ -104,7 +105,7 @@ struct Place {
       tile = 0;
       if (++g < a.G) continue;
       g = 0;
-      do { if (++b >= a.nreq) return; r = request(a, b); } while (r.tiles == 0);
+      do { if (++b >= a.nreq) return; r = request(a, b, work); } while (r.tiles == 0);
     }
   }
 };
@@ -177,10 +178,25 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
 
   // ---- this CTA's stretch
   const int per_thread = (a.nreq + THREADS - 1) / THREADS, b0 = tid * per_thread;
-  Req only{0, 0, 0, 0, 1};
-  if (per_thread == 1 && b0 < a.nreq) only = request(a, b0);
-  auto req = [&](int i) { return per_thread == 1 ? only : request(a, b0 + i); };
   const int requests = max(min(per_thread, a.nreq - b0), 0);
+  unsigned long long work = 0;                              // that requests with rows enough for the prompt form ask for
+  if (a.share) {
+    for (int i = 0; i < requests; ++i) {
+      const Req r = request(a, b0 + i, 0);
+      work += prompt_work(r.n, r.keys, a.rep, a.G);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+    if (lane == 0) s_sum[warp] = (long long)work;
+    __syncthreads();
+    work = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) work += (unsigned long long)s_sum[w];
+    __syncthreads();
+  }
+  Req only{0, 0, 0, 0, 1};
+  if (per_thread == 1 && b0 < a.nreq) only = request(a, b0, work);
+  auto req = [&](int i) { return per_thread == 1 ? only : request(a, b0 + i, work); };
   long long before, total;                                  // of the requests of the threads in front of this one, and of all
   auto scan = [&](long long mine) {
     long long incl = mine;
@@ -328,7 +344,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
   // ---- the first unit of this warp is on its way before anything else. Pages are looked up one unit ahead of the copies, so that these do not wait for them.
   int next = warp;                                          // index in the stretch of the unit that is fetched next
   Place np = cur;
-  np.forward(a, warp);
+  np.forward(a, work, warp);
   int pages = next < todo ? unit_page(a, np, lane) : -1;
   Unit unit{-1, 0, 0};                                      // the one that was fetched last, with its scales
   float pks = 0.f, pvs = 1.f;
@@ -340,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
     unit.keys = next < todo ? np.r.keys : 0;
     pks = there ? a.ks[block] : pages == BROKEN ? NAN : 1.f;
     pvs = there ? a.vs[block] : 1.f;
-    np.forward(a, WARPS);
+    np.forward(a, work, WARPS);
     pages = next + WARPS < todo ? unit_page(a, np, lane) : -1;
   };
   load_q(cur);
@@ -511,7 +527,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
     }
 
     Place after = cur;
-    after.forward(a, seg_n);
+    after.forward(a, work, seg_n);
     const bool more = seg0 + seg_n < todo;
     if (more) load_q(after);                                // the next segment's queries, on their way while sums are joined
     // ---- the warps' sums of this item together
@@ -659,12 +675,9 @@ static int att_grid() { return max(sm_count(), 1) * CTAS; }
 
 extern "C" size_t qspec_kv8_attention_workspace_bytes(void) { return 4096 + (size_t)att_grid() * 2 * PART<128> * sizeof(float); }
 
-// Rows (tokens * heads of a group) from which a request goes to the prompt form.
-constexpr int PROMPT_ROWS = 65;
-
 static int attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* ks, const float* vs, const int* table, const int* q_start,
                      const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H, int G, int D, int npages,
-                     int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, unsigned give_up, void* stream) {
+                     int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, bool always, unsigned give_up, void* stream) {
   QSPEC_REQUIRE(k && v && ks && vs && table && q_start && kv_len, QSPEC_ERR_INVALID_ARG, "kv8_attention: null pointer");
   QSPEC_REQUIRE(page_shift(page_tokens) > 0, QSPEC_ERR_UNSUPPORTED, "kv8_attention: pages of 16, 32, 64 or 128 tokens, got %d", page_tokens);
   QSPEC_REQUIRE(D == 64 || D == 128, QSPEC_ERR_UNSUPPORTED, "kv8_attention: heads of 64 or 128, got %d", D);
@@ -682,16 +695,18 @@ static int attention(const void* q, long long q_tok_stride, int q_head_stride, c
                 "kv8_attention: %zu bytes of workspace needed, got %zu", qspec_kv8_attention_workspace_bytes(), workspace_bytes);
   const int grid = att_grid();
   QSPEC_REQUIRE(grid <= GRID_MOST, QSPEC_ERR_UNSUPPORTED, "kv8_attention: %d SMs", sm_count());
-  // Requests with more rows than this kernel takes in few tiles go to the prompt form, in a launch of its own in front.
+  // Requests with many rows may go to the prompt form (to_prompt_form()), in a launch of its own in front; none do if the call's rows are too few for a third of
+  // the SMs (always: for tests).
   const int rep = H / G;
-  const bool prompts = rep <= PROMPT_REP && (long long)max_tokens * rep >= PROMPT_ROWS;
+  const bool prompts = rep <= PROMPT_REP && (long long)max_tokens * rep >= PROMPT_ROWS && (always || (long long)ntok * H >= std::max(sm_count() / 3, 1) * 128ll);
+  const unsigned share = always ? 1u : std::max(sm_count() / 4, 1) * 128u;
   if (prompts) {
     const PromptArgs pa{q, q_tok_stride, q_head_stride, (const signed char*)k, (const signed char*)v, ks, vs, table, q_start, kv_len, requests, width, npages,
-                        page_shift(page_tokens), ntok, G, rep, PROMPT_ROWS, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, give_up};
+                        page_shift(page_tokens), ntok, G, rep, share, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, give_up};
     if (const int rc = launch_prompt(pa, D, dtype == QSPEC_DTYPE_BF16, (cudaStream_t)stream)) return rc;
   }
   AttArgs a{q, q_tok_stride, q_head_stride, (const signed char*)k, (const signed char*)v, ks, vs, table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok,
-            G, rep, prompts ? PROMPT_ROWS - 1 : 0x7fffffff, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)};
+            G, rep, prompts ? share : 0u, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)};
   auto run = [&](auto kern, size_t smem, SmemLimit& limit) -> int {
     QSPEC_CUDA(limit.raise(kern, smem));
     QSPEC_CUDA(launch_pdl(kern, dim3(grid), dim3(THREADS), smem, (cudaStream_t)stream, a));
@@ -708,12 +723,12 @@ extern "C" int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_
                                    const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H,
                                    int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   return attention(q, q_tok_stride, q_head_stride, k, v, ks, vs, table, q_start, kv_len, out, out_tok_stride, out_head_stride, ntok, requests, width, H, G, D, npages, page_tokens,
-                   max_tokens, scale, dtype, workspace, workspace_bytes, 0, stream);
+                   max_tokens, scale, dtype, workspace, workspace_bytes, false, 0, stream);
 }
 extern "C" int qspec_debug_kv8_attention_give_up(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* ks, const float* vs,
                                                  const int* table, const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok,
                                                  int requests, int width, int H, int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype,
                                                  void* workspace, size_t workspace_bytes, unsigned give_up, void* stream) {
   return attention(q, q_tok_stride, q_head_stride, k, v, ks, vs, table, q_start, kv_len, out, out_tok_stride, out_head_stride, ntok, requests, width, H, G, D, npages, page_tokens,
-                   max_tokens, scale, dtype, workspace, workspace_bytes, give_up, stream);
+                   max_tokens, scale, dtype, workspace, workspace_bytes, true, give_up, stream);
 }

@@ -21,6 +21,26 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) { const __half2 
 __device__ __forceinline__ float positive(float x) { return x >= 7.888609052210118e-31f ? x : 7.888609052210118e-31f; }
 // A factor of scores, not so small that it would make a hidden key's score (minus infinity) no number.
 __device__ __forceinline__ float normal(float x) { return fmaxf(x, 1.17549435e-38f); }
+
+// Which form of the attention a request goes to, from what all requests of the call ask for; both kernels work it out alike. The prompt form takes 128 rows (tokens *
+// heads of a group) and a head a CTA, so that a block of keys costs it the same however few requests there are; the other one spreads any request over the GPU but
+// reads the keys again for every 16 rows. A request goes to the prompt form if the call has rows for a third of the SMs, it has PROMPT_ROWS rows or more, and its way
+// through its keys is no longer than what the requests of that size have to do together would take on a quarter of the SMs (a third there, too, parted requests of
+// like lengths, and the two kernels run one after the other: 4 requests of 64 tokens after 4000 to 8000 keys 159 us, so 113).
+// Both forms measured, 32 / 8 heads of 128, us of the prompt form (of the other):
+//   1 request, 1000 keys in front of it   32 tokens 28 (19)   128: 28 (31)   256: 30 (47)   1024: 63 (196)
+//   1 request, 32000 keys                 32 tokens 444 (110)   128: 444 (343)   256: 453 (671)   512: 459 (1335)
+//   4 requests, 8000 keys                 17 tokens 111 (62)   48: 113 (113)   64: 113 (142)   128: 116 (269)
+//   16 requests, 1000 keys                17 tokens 27 (44)   64: 49 (103)   128: 89 (193)
+constexpr int PROMPT_ROWS = 65;
+__device__ __forceinline__ unsigned long long prompt_work(int n, int keys, int rep, int G) {
+  const unsigned long long rows = (unsigned long long)n * rep;
+  return rows >= PROMPT_ROWS ? rows * G * ((keys + 127ll) / 128) : 0ull;
+}
+// work: of all requests; share: rows that a quarter of the SMs have at a time (0: there is no prompt form)
+__device__ __forceinline__ bool to_prompt_form(int n, int keys, int rep, unsigned share, unsigned long long work) {
+  return share && (unsigned long long)n * rep >= PROMPT_ROWS && (unsigned long long)((keys + 127ll) / 128) * share <= work;
+}
 #endif
 
 struct PromptArgs {
@@ -28,13 +48,14 @@ struct PromptArgs {
   const signed char *k, *v;
   const float *ks, *vs;
   const int *table, *q_start, *kv_len;
-  int nreq, width, npages, pshift, ntok, G, rep, min_rows;   // min_rows: requests with fewer rows (tokens * rep) are the other kernel's
+  int nreq, width, npages, pshift, ntok, G, rep;
+  unsigned share;                                 // rows that a quarter of the SMs have at a time
   float scale2;                                   // scale * log2(e)
   void* out; long long out_ts; int out_hs;
   unsigned give_up;                               // for tests: roles that give their first wait up (1 softmax, 2 codes, 4 products, 8 pages)
 };
 constexpr int PROMPT_REP = 128;                   // heads of a group that a tile takes at most
-int launch_prompt(const PromptArgs& a, int D, bool bf16, cudaStream_t stream);   // kv8_prompt.cu
+int launch_prompt(const PromptArgs& a, int D, bool bf16, cudaStream_t stream);   // kv8_prompt.cu: the requests that to_prompt_form() names
 
 template <bool BF16> struct Elem16 { using T = __half; };
 template <> struct Elem16<true> { using T = __nv_bfloat16; };

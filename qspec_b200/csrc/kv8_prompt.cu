@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   __shared__ __align__(8) uint64_t b_kfull[STAGES], b_kempty[STAGES], b_vfull[STAGES], b_vempty[STAGES], b_fac[FACS], b_facfree[FACS], b_q, b_s[2], b_p[2][2], b_o[2], b_join;
   __shared__ Block s_block[FACS];
   __shared__ float s_ml[2][2][128], s_rowf[128], s_sum128[128];
+  __shared__ unsigned long long s_work[NWARPS];
   __shared__ int s_sum[NWARPS], s_at[3];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_fail;
@@ -95,9 +96,26 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
 
   // ---- this CTA's request and tile: tiles of all requests in a row, the last one of a request (with the longest way) first
   const int per_thread = (a.nreq + NTHREADS - 1) / NTHREADS, b0 = tid * per_thread, requests = max(min(per_thread, a.nreq - b0), 0);
+  auto load = [&](int b, int& n, int& keys) {
+    n = max(min(a.q_start[b + 1], a.ntok) - min(max(a.q_start[b], 0), a.ntok), 0);
+    keys = max(a.kv_len[b], 0);
+  };
+  int n1 = 0, keys1 = 0;
+  unsigned long long work = 0;
+  for (int i = 0; i < requests; ++i) {
+    load(b0 + i, n1, keys1);
+    work += prompt_work(n1, keys1, rep, a.G);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+  if (lane == 0) s_work[warp] = work;
+  __syncthreads();
+  work = 0;
+#pragma unroll
+  for (int w = 0; w < NWARPS; ++w) work += s_work[w];
   auto tiles_of = [&](int b) {
-    const int first = min(max(a.q_start[b], 0), a.ntok), n = max(min(a.q_start[b + 1], a.ntok) - first, 0);
-    return (long long)n * rep >= a.min_rows ? (n + tok - 1) / tok : 0;
+    if (per_thread > 1) load(b, n1, keys1);
+    return to_prompt_form(n1, keys1, rep, a.share, work) ? (n1 + tok - 1) / tok : 0;
   };
   int mine = 0;
   for (int i = 0; i < requests; ++i) mine += tiles_of(b0 + i);
@@ -544,7 +562,7 @@ int launch(const Args& a, cudaStream_t stream) {
   QSPEC_CUDA(limit.raise(kern, Sizes<D>::SMEM));
   // tiles of all requests at most: full ones, and one more for each request that is large enough
   const int per = 128 / a.rep;
-  const long long tiles = a.ntok / per + std::min<long long>(a.nreq, (long long)a.ntok * a.rep / std::max(a.min_rows, 1) + 1);
+  const long long tiles = a.ntok / per + std::min<long long>(a.nreq, (long long)a.ntok * a.rep / PROMPT_ROWS + 1);
   QSPEC_REQUIRE(tiles <= 65535, QSPEC_ERR_UNSUPPORTED, "kv8_attention: %d tokens are too many for one call", a.ntok);
   QSPEC_CUDA(launch_pdl(kern, dim3(a.G, (unsigned)tiles), dim3(NTHREADS), Sizes<D>::SMEM, stream, a));
   QSPEC_CHECK_LAUNCH(1);

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from qspec_b200 import ops
+from qspec_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 I32, F32, F64 = torch.int32, torch.float32, torch.float64
@@ -193,6 +193,14 @@ def test_append_gives_the_codes_of_its_formulas(runs, D, P, H, G, dtype, spoil):
 @pytest.mark.parametrize("runs", [[(0, 513)], [(100, 500), (0, 1), (130, 63), (7, 1), (8, 1), (77, 300), (63, 2)]])
 def test_append_of_long_steps(runs, D, P, H, G, dtype):
     check_append(runs, D, P, H, G, dtype, False, 90)
+
+
+@pytest.mark.parametrize("D,P,H,G,dtype", [(128, 64, 8, 2, torch.float16), (64, 16, 6, 3, torch.bfloat16)])
+@pytest.mark.parametrize("runs", [[(60 + i, 1) for i in range(70)], [(i * 7, 1 + i % 11) for i in range(30)], [(3, 8), (64, 9), (1, 7), (0, 40), (5, 1), (6, 1), (16, 17), (8, 8)] * 4,
+                                  [(i, 1) for i in range(1030)], [(i % 50, 2 + 17 * (i % 2)) for i in range(60)]])
+@pytest.mark.parametrize("spoil", [False, True])
+def test_append_of_runs_of_every_length_next_to_each_other(runs, D, P, H, G, dtype, spoil):
+    check_append(runs, D, P, H, G, dtype, spoil, 1100)
 
 
 def check_append(runs, D, P, H, G, dtype, spoil, pages=40):
@@ -542,3 +550,54 @@ def test_a_wait_that_is_given_up_shows_and_leaves_nothing_behind():
     tests = os.path.dirname(os.path.abspath(__file__))
     run = subprocess.run([sys.executable, "-c", GIVE_UP.format(root=os.path.dirname(tests), tests=tests)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout.strip().endswith("ok"), run.stdout + run.stderr
+
+
+# ---- the prompt form at sizes at which a call would not choose it ---------------------------------------------------------------------
+def prompt_form(q, k, v, ks, vs, table, start, lens, out, scale, work, max_tokens=None):
+    lib, T, H, D = _lib.load(), q.shape[0], q.shape[1], q.shape[2]
+    _lib.check(lib.qspec_debug_kv8_attention_give_up(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(),
+                                                     start.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), T, len(lens), table.shape[1], H, k.shape[1], D,
+                                                     k.shape[0], k.shape[2], T if max_tokens is None else max_tokens, scale, int(q.dtype == torch.bfloat16), work.data_ptr(),
+                                                     work.numel(), 0, torch.cuda.current_stream().cuda_stream), "kv8_attention")
+    return out
+
+
+FORCED = ([(test_attention_of_prompts, h + (lens, counts)) for h in ((32, 8, 128, 64, torch.float16), (8, 1, 128, 16, torch.bfloat16), (12, 4, 128, 128, torch.float16),
+                                                                     (4, 2, 64, 32, torch.bfloat16), (40, 8, 128, 32, torch.bfloat16), (128, 1, 64, 64, torch.float16))
+           for lens, counts in (([17], [17]), ([200], [200]), ([130, 400, 65, 300], [130, 100, 1, 300]), ([257, 9, 1000], [33, 4, 129]))]
+          + [(test_attention_rows_that_see_nothing_and_rows_of_no_request, ()), (test_attention_with_scales_far_apart, ([150, 4, 60],)),
+             (test_attention_of_queries_of_any_size, (0.0,)), (test_attention_of_queries_of_any_size, (1e-30,)), (test_attention_of_queries_of_any_size, (1e30,)),
+             (test_attention_shows_what_is_broken_and_only_there, ([40, 2, 70],)), (test_attention_of_strided_queries_and_outputs, ()),
+             (test_attention_of_tiny_queries_over_tiny_scales, ([1, 90],))])
+
+
+@pytest.mark.parametrize("at", range(len(FORCED)))
+def test_prompt_form_of_small_calls(monkeypatch, at):
+    monkeypatch.setattr(ops, "kv8_attention", prompt_form)
+    test, args = FORCED[at]
+    test(*args)
+
+
+# ---- which form a request goes to -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lens,counts", [([400, 2000, 130], [300, 20, 70]),       # long: its way through its keys is longer than the others', so not the prompt form
+                                         ([9000, 64, 900, 5000], [65, 64, 512, 16]), ([300] * 40 + [7] * 200, [20] * 40 + [1] * 200)])
+@pytest.mark.parametrize("H,G", [(32, 8), (10, 2), (5, 5)])
+def test_attention_of_requests_that_take_different_forms(H, G, lens, counts):
+    check_attention(make_attention(14, lens, counts, H, G, 128, 64, torch.float16), 128)
+
+
+def test_the_form_is_the_rules_and_both_kernels_agree_on_it():
+    """Rows of the prompt form and of the other one differ in their last bits: which form a request took shows in its rows."""
+    lens, counts, H, G = [900, 9000, 300, 1200, 40], [200, 30, 1, 500, 24], 32, 8
+    case = make_attention(15, lens, counts, H, G, 128, 64, torch.float16)
+    out = check_attention(case, 128)
+    work = ops.kv8_attention_workspace("cuda")
+    forced = prompt_form(*case, torch.empty_like(out), 128 ** -0.5, work)
+    share = torch.cuda.get_device_properties(0).multi_processor_count // 4 * 128
+    rows = [n * H // G for n in counts]
+    total = sum(r * G * -(-n // 128) for r, n in zip(rows, lens) if r >= 65)
+    picks = [r >= 65 and -(-n // 128) * share <= total for r, n in zip(rows, lens)]
+    assert picks == [True, False, False, True, True]
+    for b, pick in enumerate(picks):
+        at = slice(sum(counts[:b]), sum(counts[:b + 1]))
+        assert counts[b] == 1 or torch.equal(out[at], forced[at]) == pick
