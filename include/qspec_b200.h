@@ -413,7 +413,7 @@ int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_head_stride
                         size_t workspace_bytes, void* stream);
 
 /* For tests: every request with rows enough for a prompt form goes there, however few they are together; the roles of its pipeline in the mask give_up (1 softmax, 2
-   codes, 4 products, 8 pages) give their first wait up at once. */
+   codes, 4 products, 8 pages) give their first wait up at once; 16: its CTAs take two tiles of rows. */
 int qspec_debug_kv8_attention_give_up(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* k_scale, const float* v_scale,
                                       const int* table, const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok,
                                       int requests, int width, int H, int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype,

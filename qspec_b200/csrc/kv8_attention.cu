@@ -701,8 +701,12 @@ static int attention(const void* q, long long q_tok_stride, int q_head_stride, c
   const bool prompts = rep <= PROMPT_REP && (long long)max_tokens * rep >= PROMPT_ROWS && (always || (long long)ntok * H >= std::max(sm_count() / 3, 1) * 128ll);
   const unsigned share = always ? 1u : std::max(sm_count() / 4, 1) * 128u;
   if (prompts) {
+    // Two tiles a CTA where the rows are more than the SMs take at once with one, by a quarter: it is 2350 cycles a tile and block of keys instead of 2850 to 3400,
+    // with half as many CTAs. us of pairs (of single tiles), 32 / 8 heads, after 1000 tokens: 512 tokens 50 (36), 900: 60 (63), 2000: 113 (140); 16 requests
+    // of 64: 43 (51).
+    const int pair = always ? give_up >> 4 & 1 : (long long)ntok * H > 160ll * sm_count();
     const PromptArgs pa{q, q_tok_stride, q_head_stride, (const signed char*)k, (const signed char*)v, ks, vs, table, q_start, kv_len, requests, width, npages,
-                        page_shift(page_tokens), ntok, G, rep, share, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, give_up};
+                        page_shift(page_tokens), ntok, G, rep, pair, share, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, give_up};
     if (const int rc = launch_prompt(pa, D, dtype == QSPEC_DTYPE_BF16, (cudaStream_t)stream)) return rc;
   }
   AttArgs a{q, q_tok_stride, q_head_stride, (const signed char*)k, (const signed char*)v, ks, vs, table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok,

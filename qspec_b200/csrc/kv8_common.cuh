@@ -31,7 +31,7 @@ __device__ __forceinline__ float normal(float x) { return fmaxf(x, 1.17549435e-3
 //   1 request, 1000 keys in front of it   32 tokens 28 (19)   128: 28 (31)   256: 30 (47)   1024: 63 (196)
 //   1 request, 32000 keys                 32 tokens 444 (110)   128: 444 (343)   256: 453 (671)   512: 459 (1335)
 //   4 requests, 8000 keys                 17 tokens 111 (62)   48: 113 (113)   64: 113 (142)   128: 116 (269)
-//   16 requests, 1000 keys                17 tokens 27 (44)   64: 49 (103)   128: 89 (193)
+//   16 requests, 1000 keys                17 tokens 27 (44)   64: 43 (103)   128: 76 (193)
 constexpr int PROMPT_ROWS = 65;
 __device__ __forceinline__ unsigned long long prompt_work(int n, int keys, int rep, int G) {
   const unsigned long long rows = (unsigned long long)n * rep;
@@ -49,6 +49,7 @@ struct PromptArgs {
   const float *ks, *vs;
   const int *table, *q_start, *kv_len;
   int nreq, width, npages, pshift, ntok, G, rep;
+  int pair;                                       // 1: CTAs of the prompt form take two tiles of 128 rows
   unsigned share;                                 // rows that a quarter of the SMs have at a time
   float scale2;                                   // scale * log2(e)
   void* out; long long out_ts; int out_hs;

@@ -1,8 +1,9 @@
 // Softmax attention of prompt portions over the paged 8-bit cache, on the fifth-generation tensor cores (kv8_attention.cu has the layout, and the form for requests
 // with few tokens).
 //
-// One CTA = 128 rows of one request and key/value head; a row is a (token, query head of the group) pair. Keys are walked in blocks of 128, which belong
-// alternately to two streams with a softmax and a sum of values of their own (joined at the end), so that one's products run under the other's softmax:
+// One CTA = one or two tiles of 128 rows of one request and key/value head; a row is a (token, query head of the group) pair. Keys are walked in blocks of 128 by two
+// streams with a softmax and a sum of values of their own, so that one's products run under the other's softmax. Two tiles have a stream each, and every
+// block's codes are made ready once for both; a single tile's streams take the blocks in turn and are joined at the end.
 //   * pages: one warp looks the block's pages and scales up and leaves where the codes are and what their products are multiplied with.
 //   * codes: four warps bring a block's keys and values from global memory, make them float16 and store them as the tensor cores want them: the cache
 //     is read once, in 8 bits, and is never anywhere in 16. Keys are (c + 128) 2^-24, the subnormal number that a byte is by itself; what the 128 adds
@@ -13,8 +14,12 @@
 //   * O += P V: weights from tensor memory, values from shared memory as they lie in the cache (operand "MN-major").
 // Tensor memory: S | S | O | O = 512 columns. Scales and the exponent that takes the value scale in: as in kv8_attention.cu. O is multiplied again only
 // where a row's maximum grew by more than 2^8.
-// Bound by the tensor cores (1024 cycles a block of 128 x 128, head 128) and the exponentials (16 a cycle: 1024) at once, and nearly by the schedulers:
-// the conversion is 1600 warp instructions beside 2600 of the softmax.
+// What a block of 128 x 128 (head 128) asks of an SM: 1024 cycles of the tensor cores, 1024 of the exponentials (16 a cycle), and of the schedulers 720 by the softmax
+// and 400 by the codes (200 of two tiles). It takes 2350 cycles of two tiles (2850 to 3400 of one): what bounds it is a stream's way from scores to the next scores,
+// 4700 cycles, of which the softmax is 3000 (a warp's 32 exponentials and what belongs to them 570) and the products with their waits 1700; start and end of a CTA are
+// another 16000. Prompt of 2000 tokens after 1000, 32 / 8 heads, float16: 111 us, 590 TFLOP/s. Measured and not taken: sixteen softmax warps, two for
+// a row, 125 us (their common maximum and their waits cost more than they save); a warp for each stream's products 128 us (the streams fall into step);
+// scores read one chunk ahead 137 us (the copies between registers).
 //
 // Every wait is bounded; a CTA whose wait runs out waits (again with a limit) for its products under way, fills its rows with NaN, counts itself
 // (qspec_attn_tile_timeouts) and frees its tensor memory.
@@ -37,10 +42,9 @@ template <int D> struct Sizes {
   static constexpr int PART = 128 * 128;                  // 128 rows x 64 elements
   static constexpr int OP = D / 64 * PART;                // an operand: 128 rows x D
   static constexpr int STAGES = 2;                        // of keys and of values
-  static constexpr size_t USED = (size_t)OP * (1 + 2 * STAGES) + 1024;
+  static constexpr size_t USED = (size_t)OP * (2 + 2 * STAGES) + 1024;
   static constexpr size_t SMEM = USED > 120 * 1024 ? USED : 120 * 1024;   // one CTA an SM: each takes all of the tensor memory
-  static constexpr int LD = D / 2 + 4;                    // floats of a row's half on its way out
-  static_assert(8 * 32 * LD * 4 <= 3 * OP, "rows on their way out, over queries and keys");
+  static_assert(SOFTMAX * 32 * (D + 16) <= 3 * OP, "rows on their way out, over queries and keys");
 };
 template <int D> constexpr uint32_t IDESC_S = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 template <int D> constexpr uint32_t IDESC_O = (1u << 4) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
@@ -56,6 +60,11 @@ __device__ __forceinline__ void st8(uint32_t addr, const uint32_t* r) {
                "r"(r[7]) : "memory");
 }
 
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                 "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr));
+}
 // Behind wait_ld(): nothing that is done with these registers is moved in front of it.
 __device__ __forceinline__ void landed32(uint32_t (&r)[32]) {
 #pragma unroll
@@ -70,13 +79,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ __align__(8) uint64_t b_kfull[STAGES], b_kempty[STAGES], b_vfull[STAGES], b_vempty[STAGES], b_fac[FACS], b_facfree[FACS], b_q, b_s[2], b_p[2][2], b_o[2], b_join;
   __shared__ Block s_block[FACS];
-  __shared__ float s_ml[2][2][128], s_rowf[128], s_sum128[128];
+  __shared__ float s_ml[2][2][128], s_rowf[256], s_sum128[256];
   __shared__ unsigned long long s_work[NWARPS];
-  __shared__ int s_sum[NWARPS], s_at[3];
+  __shared__ int s_sum[NWARPS], s_at[5];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_fail;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rep = a.rep, tok = 128 / rep, g = blockIdx.x;
+  const int rep = a.rep, tok = 128 / rep, span = tok << a.pair, g = blockIdx.x, rep_inv = 65536 / rep + 1;   // tokens of 128 rows, and of a CTA
+  auto token_of = [&](int r) { return r * rep_inv >> 16; };   // r / rep, r < 256, rep <= 128
   if (tid == 0) {
     s_fail = 0;
     s_at[0] = -1;
@@ -84,7 +94,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       bar_init(smem_addr(&b_kfull[i]), CONVERT); bar_init(smem_addr(&b_kempty[i]), 1);
       bar_init(smem_addr(&b_vfull[i]), CONVERT); bar_init(smem_addr(&b_vempty[i]), 1);
     }
-    for (int i = 0; i < FACS; ++i) { bar_init(smem_addr(&b_fac[i]), 1); bar_init(smem_addr(&b_facfree[i]), SOFTMAX / 2 + CONVERT); }
+    for (int i = 0; i < FACS; ++i) bar_init(smem_addr(&b_fac[i]), 1);
     for (int i = 0; i < 2; ++i) { bar_init(smem_addr(&b_s[i]), 1); bar_init(smem_addr(&b_p[i][0]), 4); bar_init(smem_addr(&b_p[i][1]), 4); bar_init(smem_addr(&b_o[i]), 1); }
     bar_init(smem_addr(&b_q), SOFTMAX);
     bar_init(smem_addr(&b_join), SOFTMAX);
@@ -115,7 +125,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   for (int w = 0; w < NWARPS; ++w) work += s_work[w];
   auto tiles_of = [&](int b) {
     if (per_thread > 1) load(b, n1, keys1);
-    return to_prompt_form(n1, keys1, rep, a.share, work) ? (n1 + tok - 1) / tok : 0;
+    return to_prompt_form(n1, keys1, rep, a.share, work) ? (n1 + span - 1) / span : 0;
   };
   int mine = 0;
   for (int i = 0; i < requests; ++i) mine += tiles_of(b0 + i);
@@ -136,6 +146,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       if ((int)blockIdx.y < at + n) {
         s_at[0] = b0 + i;
         s_at[1] = n - 1 - ((int)blockIdx.y - at);
+        s_at[2] = a.q_start[b0 + i];
+        s_at[3] = n1;
+        s_at[4] = keys1;
         break;
       }
       at += n;
@@ -143,11 +156,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   }
   __syncthreads();
   if (s_at[0] < 0) return;
-  const int req = s_at[0], tile = s_at[1];
-  const int first = min(max(a.q_start[req], 0), a.ntok), n_new = max(min(a.q_start[req + 1], a.ntok) - first, 0), keys = max(a.kv_len[req], 0);
-  const int t0 = tile * tok, n2 = min(tok, n_new - t0);   // this tile's tokens
+  const int req = s_at[0], tile = s_at[1], first = min(max(s_at[2], 0), a.ntok), n_new = s_at[3], keys = s_at[4];
+  const int t0 = tile * span, n2 = min(span, n_new - t0);   // this CTA's tokens
   const int pos0 = keys - n_new + t0;                     // position of the first
-  const int seen = min(pos0 + n2, keys), blocks = seen > 0 ? (seen + 127) / 128 : 0;   // keys that any row sees
+  const bool both = n2 > tok;                             // two tiles of rows, a stream each
+  auto blocks_of = [&](int tokens) { const int seen = min(pos0 + tokens, keys); return seen > 0 ? (seen + 127) / 128 : 0; };
+  const int blocks = blocks_of(n2);                       // keys that any row sees
+  const int turns0 = both ? blocks_of(tok) : (blocks + 1) >> 1, turns1 = both ? blocks : blocks >> 1;   // blocks of the streams
+  if (tid == 0)
+    for (int i = 0; i < FACS; ++i) bar_init(smem_addr(&b_facfree[i]), (both ? SOFTMAX : SOFTMAX / 2) + CONVERT);
   if (warp == W_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&s_tmem)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -157,7 +174,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   fence_after();
   const uint32_t tmem = s_tmem;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // (tensor memory is held)
-  const uint32_t kbuf = base + OP, vbuf = kbuf + STAGES * OP;
+  const uint32_t kbuf = base + 2 * OP, vbuf = kbuf + STAGES * OP;
 
   if (warp == W_PAGES) {
     // ---- pages and factors of the blocks, ahead of all others
@@ -197,50 +214,56 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     }
   } else if (warp == W_MMA) {
     if (elect()) {
-      const uint64_t qd = desc_k(base);
       bool ok = !(a.give_up & 4u);
       if (!ok) s_fail = 1;
-      int products = 0;                                   // value products that have been issued, block by block
-      auto scores = [&](int n) -> bool {
+      int done0 = 0, done1 = 0;                           // value products that have been issued
+      // Step k: stream k % 2's turn k / 2. Pairs of tiles take every block in turn, a single tile's streams every other one.
+      const int steps = both ? 2 * blocks : blocks;
+      auto scores = [&](int k) -> bool {
+        const int z = k & 1, i = k >> 1, n = both ? i : k;
+        if (i >= (z ? turns1 : turns0)) return true;
         if (!bar_wait(smem_addr(&b_kfull[n % STAGES]), (uint32_t)(n / STAGES) & 1u, &s_fail)) return false;
-        // these scores take the columns of the weights of block n - 2: their product must be over
-        if (n >= 2 && !bar_wait(smem_addr(&b_o[n & 1]), (uint32_t)((n >> 1) - 1) & 1u, &s_fail)) return false;
+        // these scores take the columns of the weights of the turn before: its product must be over
+        if (i && !bar_wait(smem_addr(&b_o[z]), (uint32_t)(i - 1) & 1u, &s_fail)) return false;
         fence_after();
-        const uint64_t kd = desc_k(kbuf + (n % STAGES) * OP);
+        const uint64_t qd = desc_k(base + (both ? z * OP : 0)), kd = desc_k(kbuf + (n % STAGES) * OP);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const uint32_t step = (uint32_t)((i >> 2) * (PARTB >> 4) + (i & 3) * 2);
-          mma_ss(tmem + (n & 1) * 128, qd + step, kd + step, IDESC_S<D>, i ? 1u : 0u);
+        for (int d = 0; d < D / 16; ++d) {
+          const uint32_t step = (uint32_t)((d >> 2) * (PARTB >> 4) + (d & 3) * 2);
+          mma_ss(tmem + z * 128, qd + step, kd + step, IDESC_S<D>, d ? 1u : 0u);
         }
-        commit(smem_addr(&b_s[n & 1]));
-        commit(smem_addr(&b_kempty[n % STAGES]));
+        commit(smem_addr(&b_s[z]));
+        if (!both || z) commit(smem_addr(&b_kempty[n % STAGES]));   // (tile 1 sees every block that tile 0 sees)
         return true;
       };
-      ok = ok && (blocks == 0 || (bar_wait(smem_addr(&b_q), 0, &s_fail) && scores(0) && (blocks == 1 || scores(1))));
-      for (int n = 0; ok && n < blocks; ++n) {
-        if (!bar_wait(smem_addr(&b_vfull[n % STAGES]), (uint32_t)(n / STAGES) & 1u, &s_fail)) break;
+      ok = ok && (steps == 0 || (bar_wait(smem_addr(&b_q), 0, &s_fail) && scores(0) && (steps == 1 || scores(1))));
+      for (int k = 0; ok && k < steps; ++k) {
+        const int z = k & 1, i = k >> 1, n = both ? i : k;
+        if (i >= (z ? turns1 : turns0)) continue;
+        ok = bar_wait(smem_addr(&b_vfull[n % STAGES]), (uint32_t)(n / STAGES) & 1u, &s_fail);
         const uint64_t vd = desc_mn(vbuf + (n % STAGES) * OP);
-        const uint32_t p = tmem + (n & 1) * 128, o = tmem + 256 + (n & 1) * D;
+        const uint32_t p = tmem + z * 128, o = tmem + 256 + z * D;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {                     // 64 keys each
-          ok = ok && bar_wait(smem_addr(&b_p[n & 1][h]), (uint32_t)(n >> 1) & 1u, &s_fail);
+          ok = ok && bar_wait(smem_addr(&b_p[z][h]), (uint32_t)i & 1u, &s_fail);
           if (!ok) break;
           fence_after();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mma_ts(o, p + h * 32 + i * 8, vd + (h * 4 + i) * (2048 >> 4), IDESC_O<D>, (n > 1 || h || i) ? 1u : 0u);
+          for (int d = 0; d < 4; ++d) mma_ts(o, p + h * 32 + d * 8, vd + (h * 4 + d) * (2048 >> 4), IDESC_O<D>, (i || h || d) ? 1u : 0u);
         }
         if (!ok) break;
-        commit(smem_addr(&b_o[n & 1]));
-        commit(smem_addr(&b_vempty[n % STAGES]));
-        products = n + 1;
-        if (n + 2 < blocks && !scores(n + 2)) break;
+        commit(smem_addr(&b_o[z]));
+        if (!both || z) commit(smem_addr(&b_vempty[n % STAGES]));
+        (z ? done1 : done0) = i + 1;
+        ok = k + 2 >= steps || scores(k + 2);
       }
-      if (products < blocks) {                            // given up: what was issued so far
-        commit(smem_addr(&b_o[products & 1]));
-        products += 1;
+      // every product of either stream is over before the CTA leaves, those of a turn that was given up, too
+      if (done0) bar_drain(smem_addr(&b_o[0]), (uint32_t)(done0 - 1) & 1u);
+      if (done1) bar_drain(smem_addr(&b_o[1]), (uint32_t)(done1 - 1) & 1u);
+      if (!ok) {
+        commit(smem_addr(&b_o[0]));
+        bar_drain(smem_addr(&b_o[0]), (uint32_t)done0 & 1u);
       }
-      // every product of either stream is over before the CTA leaves
-      for (int n = max(products - 2, 0); n < products; ++n) bar_drain(smem_addr(&b_o[n & 1]), (uint32_t)(n >> 1) & 1u);
     }
     __syncwarp();
   } else if (warp >= W_CONVERT) {
@@ -315,56 +338,61 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       if (lane == 0) bar_arrive(smem_addr(&b_vfull[n % STAGES]));
     }
   } else {
-    // ---- queries: 16 bytes a thread at a time, bfloat16 rows by a power of two each
-    constexpr int IN_ROW = D / 8, QROWS = SOFTMAX * 32 / IN_ROW;
-    {
-      const int c = tid % IN_ROW;
-      uint4 w[128 / QROWS];
-#pragma unroll
-      for (int i = 0; i < 128 / QROWS; ++i) {
-        const int r = i * QROWS + tid / IN_ROW, tl = r / rep;
-        w[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (tl < n2 && r < tok * rep)
-          w[i] = *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(first + t0 + tl) * a.q_ts + (size_t)(g * rep + r - tl * rep) * a.q_hs + c * 8);
-      }
-#pragma unroll
-      for (int i = 0; i < 128 / QROWS; ++i) {
-        const int r = i * QROWS + tid / IN_ROW;
-        uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-        int sh = 0;
-        if (BF16) {
-          float mx = 0.f;
+    // ---- queries: as they are, 16 bytes a thread at a time; then a thread a row: bfloat16 rows times a power of two each, and the sums. (Loops that are
+    // not unrolled: every CTA comes here once, and had to wait for the instructions.)
+    constexpr int IN_ROW = D / 8;
+    const int tiles = both ? 2 : 1;
+#pragma unroll 4
+    for (int i = tid; i < tiles * 128 * IN_ROW; i += SOFTMAX * 32) {
+      const int c = i % IN_ROW, row = i / IN_ROW, r = row & 127, tl = (row >> 7) * tok + token_of(r);
+      const uint32_t to = base + (row >> 7) * OP + (c >> 3) * PARTB + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+      if (tl < n2 && r < tok * rep)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to),
+                     "l"((const T*)a.q + (size_t)(first + t0 + tl) * a.q_ts + (size_t)(g * rep + r - token_of(r) * rep) * a.q_hs + c * 8) : "memory");
+      else
+        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(to), "r"(0u) : "memory");
+    }
+    asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;\nbar.sync 1, %0;\n" ::"n"(SOFTMAX * 32) : "memory");   // (behind nothing that may be given up)
+    if (tid < tiles * 128) {
+      const int r = tid & 127;
+      unsigned char* const row = gbase + (tid >> 7) * OP + r * 128;
+      auto piece = [&](int c) { return reinterpret_cast<uint4*>(row + (c >> 3) * PARTB + (((c & 7) ^ (r & 7)) << 4)); };
+      int sh = 0;
+      if (BF16) {
+        float mx = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < IN_ROW; ++c) {
+          const uint4 w = *piece(c);
+          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
-#pragma unroll
-          for (int o = IN_ROW / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
-          sh = mx > 0.f && mx < INFINITY ? min(max(14 - ex, -126), 126) : 0;
-          const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = half_pair(__uint_as_float(x[e] << 16) * up, __uint_as_float(x[e] & 0xffff0000u) * up);
         }
-        float sum = 0.f;
+        const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+        sh = mx > 0.f && mx < INFINITY ? min(max(14 - ex, -126), 126) : 0;
+      }
+      const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
+      float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+      for (int c = 0; c < IN_ROW; ++c) {
+        const uint4 w = *piece(c);
+        uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+          if (BF16) x[e] = half_pair(__uint_as_float(x[e] << 16) * up, __uint_as_float(x[e] & 0xffff0000u) * up);
           const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&x[e]));
-          sum += y.x + y.y;
+          sums[e] += y.x + y.y;
         }
-#pragma unroll
-        for (int o = IN_ROW / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (c == 0) {
-          s_rowf[r] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2 * 16777216.f;   // (scores come in units of 2^-24)
-          s_sum128[r] = sum * (128.f / 16777216.f);
-        }
-        *reinterpret_cast<uint4*>(gbase + (c >> 3) * PARTB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+        if (BF16) *piece(c) = make_uint4(x[0], x[1], x[2], x[3]);
       }
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      __syncwarp();
-      if (lane == 0) bar_arrive(smem_addr(&b_q));
+      s_rowf[tid] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2 * 16777216.f;   // (scores come in units of 2^-24)
+      s_sum128[tid] = ((sums[0] + sums[1]) + (sums[2] + sums[3])) * (128.f / 16777216.f);
     }
-    // ---- softmax: thread = row r of the blocks of stream z
-    const int z = warp >> 2, r = (warp & 3) * 32 + lane;
-    const int tl = r / rep;
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    __syncwarp();
+    if (lane == 0) bar_arrive(smem_addr(&b_q));
+    // ---- softmax: thread = row r of stream z
+    const int z = warp >> 2, r = (warp & 3) * 32 + lane, turns = z ? turns1 : turns0, zrow = both ? z * 128 : 0, ztok = both ? z * tok : 0;
+    const int tl = ztok + token_of(r);
     const bool row_in = r < tok * rep && tl < n2;
     const int limit = row_in ? min(pos0 + tl, keys - 1) : -1;   // last visible position
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -373,11 +401,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     if (!ok) s_fail = 1;
     ok = ok && bar_wait(smem_addr(&b_q), 0, &s_fail);     // (the factors of the rows)
     ok = __all_sync(0xffffffffu, ok);
-    const float rowf = s_rowf[r], sum128 = s_sum128[r];
+    const float rowf = s_rowf[zrow + r], sum128 = s_sum128[zrow + r];
     float m = NONE, l = 0.f;
-    int n = z;
-    for (; ok && n < blocks; n += 2) {
-      const uint32_t turn = (uint32_t)(n >> 1) & 1u;
+    for (int i = 0; ok && i < turns; ++i) {
+      const int n = both ? i : 2 * i + z;
+      const uint32_t turn = (uint32_t)i & 1u;
       const int j0 = n * 128;
       const bool plain = __all_sync(0xffffffffu, !row_in || j0 + 127 <= limit);   // (rows that stand for no token are never stored)
       ok = bar_wait(smem_addr(&b_fac[n % FACS]), (uint32_t)(n / FACS) & 1u, &s_fail) && bar_wait(smem_addr(&b_s[z]), turn, &s_fail);
@@ -387,8 +415,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       const Block& f = s_block[n % FACS];
       const unsigned bad = f.bad;
       const bool odd = !plain || bad;
-      // Loops over 32 columns, not unrolled: three kinds of warps run at once, and with the block's 128 columns laid out in a row they waited for their
-      // instructions more than for anything else (4.2 of 12 cycles an instruction; prompt of 2000 after 1000, 32 / 8 heads 207 us, so 137).
+      // Loops over 32 columns (the weights' over 64), not over all: three kinds of warps run at once, and with the block's 128 columns laid out in a row they waited for
+      // their instructions more than for anything else (4.2 of 12 cycles an instruction; with one tile a CTA the prompt above took 207 us, so 137).
       // What a row does not see, and of a page that there is not, or whose scale is no number, what makes the rows NaN that do see it:
       auto hide = [&](uint32_t (&x)[32], int c0) {
 #pragma unroll
@@ -422,7 +450,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       const bool grown = mn > m + RESCALE_LOG2 || (m == NONE && mn > m);
       const float up = grown ? ex2(m - mn) : 1.f;         // 0 for a row that had seen nothing; other rows of the warp keep theirs
       l *= up;
-      if (n > 1 && __any_sync(0xffffffffu, grown && m != NONE)) {   // (the scores are there: the stream's product before them is over)
+      if (i && __any_sync(0xffffffffu, grown && m != NONE)) {   // (the scores are there: the stream's product before them is over)
 #pragma unroll 1
         for (int q = 0; q < D / 8; ++q) {
           uint32_t o[8];
@@ -439,7 +467,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       // Exponents are taken from the products without a rounding in between, the reference has one: beyond 2^24 that alone would be a large exponent.
       const bool far = __any_sync(0xffffffffu, fabsf(mu) > 16777216.f);
       // ---- weights
-#pragma unroll 1
+#pragma unroll 2
       for (int c0 = 0; c0 < 128; c0 += 32) {
         uint32_t x[32], p[16];
         ld32(st + c0, x);
@@ -481,10 +509,15 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       }
       if (lane == 0) bar_arrive(smem_addr(&b_facfree[n % FACS]));
     }
-    // ---- the streams together: maxima and sums through shared memory; stream z takes half z of the columns, of both sums. Rows leave through shared memory,
-    // 16 bytes a lane.
-    constexpr int LD = Z::LD, LANES = COLS / 8, AT_ONCE = 32 / LANES;
-    float* const rows = reinterpret_cast<float*>(gbase) + warp * 32 * LD;   // (queries and keys are done with)
+    if (both && z == 0)                                   // (blocks that tile 1 alone sees)
+      for (int n = turns; ok && n < blocks; ++n) {
+        ok = __all_sync(0xffffffffu, bar_wait(smem_addr(&b_fac[n % FACS]), (uint32_t)(n / FACS) & 1u, &s_fail));
+        if (ok && lane == 0) bar_arrive(smem_addr(&b_facfree[n % FACS]));
+      }
+    // ---- out, through shared memory, 16 bytes a lane. A single tile's streams together: maxima and sums through shared memory; stream z takes half z of the
+    // columns, of both sums. Of a pair either takes both halves of its own.
+    constexpr int LD = COLS * 2 + 16, LANES = COLS / 8;   // bytes of half a row (and 16: no bank conflicts), lanes that take it
+    unsigned char* const rows = gbase + warp * 32 * LD;   // (queries and keys are done with)
     s_ml[z][0][r] = m;
     s_ml[z][1][r] = l;
     __syncwarp();
@@ -492,50 +525,55 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     // the last product of either stream, and everyone's maxima
     if (ok) {
       ok = bar_wait(smem_addr(&b_join), 0, &s_fail);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (blocks > i) ok = ok && bar_wait(smem_addr(&b_o[i]), (uint32_t)((blocks - 1 - i) >> 1) & 1u, &s_fail);
+      if (turns0) ok = ok && bar_wait(smem_addr(&b_o[0]), (uint32_t)(turns0 - 1) & 1u, &s_fail);
+      if (turns1) ok = ok && bar_wait(smem_addr(&b_o[1]), (uint32_t)(turns1 - 1) & 1u, &s_fail);
       ok = __all_sync(0xffffffffu, ok);
     }
     fence_after();
     if (ok) {
-      float f[2], sum = 0.f;
-      const float m0 = s_ml[0][0][r], m1 = s_ml[1][0][r], top = fmaxf(m0, m1);
+      const int other = both ? z : 1 - z;
+      float f[2], sum = 0.f;                              // of this stream and the other one
+      const float top = fmaxf(m, s_ml[other][0][r]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float mi = i ? m1 : m0, li = s_ml[i][1][r];
+        const float mi = i ? s_ml[other][0][r] : m, li = i ? s_ml[other][1][r] : l;
         f[i] = mi == NONE ? (li == 0.f ? 0.f : 1.f) : ex2(mi - top);   // nothing seen, or no number
-        sum += li * f[i];
+        if (i && both) f[i] = 0.f;
+        sum += f[i] == 0.f ? 0.f : li * f[i];
       }
       const float d = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);          // (no key: zeros)
-      const bool two = __any_sync(0xffffffffu, f[1] != 0.f) && blocks > 1;
-#pragma unroll 1
-      for (int q = 0; q < COLS / 8; ++q) {
-        uint32_t o0[8], o1[8];
-        if (blocks > 0) ld8(tmem + lanes + 256 + z * COLS + q * 8, o0);
-        if (blocks > 1) ld8(tmem + lanes + 256 + D + z * COLS + q * 8, o1);
-        wait_ld();
-        landed8(o0);
-        landed8(o1);
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x0 = f[0] == 0.f ? 0.f : __uint_as_float(o0[e]) * f[0], x1 = two && f[1] != 0.f ? __uint_as_float(o1[e]) * f[1] : 0.f;
-          v[e] = (x0 + x1) * d;
-        }
-        *reinterpret_cast<float4*>(rows + lane * LD + q * 8) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(rows + lane * LD + q * 8 + 4) = make_float4(v[4], v[5], v[6], v[7]);
-      }
+      const bool one = turns > 0, two = !both && __any_sync(0xffffffffu, f[1] != 0.f) && (z ? turns0 : turns1) > 0;
       const uint32_t stored = __ballot_sync(0xffffffffu, row_in);
-      __syncwarp();
-      const int pc = lane % LANES;
+      for (int half = both ? 0 : z; half <= (both ? 1 : z); ++half) {
 #pragma unroll 1
-      for (int k = 0; k < 32 / AT_ONCE; ++k) {
-        const int rr = lane / LANES + AT_ONCE * k, r2 = (warp & 3) * 32 + rr, t2 = r2 / rep;
-        if (!(stored >> rr & 1u)) continue;
-        const float4 x = *reinterpret_cast<const float4*>(rows + rr * LD + pc * 8), y = *reinterpret_cast<const float4*>(rows + rr * LD + pc * 8 + 4);
-        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-        *reinterpret_cast<uint4*>((T*)a.out + (size_t)(first + t0 + t2) * a.out_ts + (size_t)(g * rep + r2 - t2 * rep) * a.out_hs + z * COLS + pc * 8) = pack8<BF16>(v);
+        for (int q = 0; q < COLS / 16; ++q) {
+          uint32_t o0[16], o1[16];
+          if (one) ld16(tmem + lanes + 256 + z * D + half * COLS + q * 16, o0);
+          if (two) ld16(tmem + lanes + 256 + other * D + half * COLS + q * 16, o1);
+          wait_ld();
+          landed8(o0); landed8(o0 + 8);
+          landed8(o1); landed8(o1 + 8);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float x0 = one && f[0] != 0.f ? __uint_as_float(o0[x * 8 + e]) * f[0] : 0.f, x1 = two && f[1] != 0.f ? __uint_as_float(o1[x * 8 + e]) * f[1] : 0.f;
+              v[e] = (x0 + x1) * d;
+            }
+            *reinterpret_cast<uint4*>(rows + lane * LD + q * 32 + x * 16) = pack8<BF16>(v);
+          }
+        }
+        __syncwarp();
+        const int pc = lane % LANES;
+#pragma unroll 2
+        for (int rr = lane / LANES; rr < 32; rr += 32 / LANES) {
+          const int r2 = (warp & 3) * 32 + rr, t2 = token_of(r2);
+          if (stored >> rr & 1u)
+            *reinterpret_cast<uint4*>((T*)a.out + (size_t)(first + t0 + ztok + t2) * a.out_ts + (size_t)(g * rep + r2 - t2 * rep) * a.out_hs + half * COLS + pc * 8) =
+                *reinterpret_cast<const uint4*>(rows + rr * LD + pc * 16);
+        }
+        __syncwarp();
       }
     }
   }
@@ -561,7 +599,7 @@ int launch(const Args& a, cudaStream_t stream) {
   auto kern = kv8_prompt_kernel<BF16, D>;
   QSPEC_CUDA(limit.raise(kern, Sizes<D>::SMEM));
   // tiles of all requests at most: full ones, and one more for each request that is large enough
-  const int per = 128 / a.rep;
+  const int per = (128 / a.rep) << a.pair;
   const long long tiles = a.ntok / per + std::min<long long>(a.nreq, (long long)a.ntok * a.rep / PROMPT_ROWS + 1);
   QSPEC_REQUIRE(tiles <= 65535, QSPEC_ERR_UNSUPPORTED, "kv8_attention: %d tokens are too many for one call", a.ntok);
   QSPEC_CUDA(launch_pdl(kern, dim3(a.G, (unsigned)tiles), dim3(NTHREADS), Sizes<D>::SMEM, stream, a));

@@ -529,7 +529,7 @@ for D, dtype in ((128, torch.float16), (64, torch.bfloat16)):
     q, k, v, ks, vs, table, start, lens = make_attention(3, [500, 900, 40], [130, 300, 1], 8, 2, D, 32, dtype)
     work = ops.kv8_attention_workspace("cuda")
     good = ops.kv8_attention(q, k, v, ks, vs, table, start, lens, torch.empty_like(q), D ** -0.5, work)
-    for roles in (1, 2, 4, 8, 15):
+    for roles in (1, 2, 4, 8, 15, 17, 18, 20, 24, 31):
         before, out = ops.attn_tile_timeouts(), torch.zeros_like(q)
         _lib.check(lib.qspec_debug_kv8_attention_give_up(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(),
                                                          start.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), len(q), 3, table.shape[1], 8, 2, D, k.shape[0],
@@ -553,12 +553,12 @@ def test_a_wait_that_is_given_up_shows_and_leaves_nothing_behind():
 
 
 # ---- the prompt form at sizes at which a call would not choose it ---------------------------------------------------------------------
-def prompt_form(q, k, v, ks, vs, table, start, lens, out, scale, work, max_tokens=None):
+def prompt_form(q, k, v, ks, vs, table, start, lens, out, scale, work, max_tokens=None, pairs=False):
     lib, T, H, D = _lib.load(), q.shape[0], q.shape[1], q.shape[2]
     _lib.check(lib.qspec_debug_kv8_attention_give_up(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), table.data_ptr(),
                                                      start.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), T, len(lens), table.shape[1], H, k.shape[1], D,
                                                      k.shape[0], k.shape[2], T if max_tokens is None else max_tokens, scale, int(q.dtype == torch.bfloat16), work.data_ptr(),
-                                                     work.numel(), 0, torch.cuda.current_stream().cuda_stream), "kv8_attention")
+                                                     work.numel(), 16 * pairs, torch.cuda.current_stream().cuda_stream), "kv8_attention")
     return out
 
 
@@ -571,9 +571,10 @@ FORCED = ([(test_attention_of_prompts, h + (lens, counts)) for h in ((32, 8, 128
              (test_attention_of_tiny_queries_over_tiny_scales, ([1, 90],))])
 
 
+@pytest.mark.parametrize("pairs", [False, True])
 @pytest.mark.parametrize("at", range(len(FORCED)))
-def test_prompt_form_of_small_calls(monkeypatch, at):
-    monkeypatch.setattr(ops, "kv8_attention", prompt_form)
+def test_prompt_form_of_small_calls(monkeypatch, at, pairs):
+    monkeypatch.setattr(ops, "kv8_attention", lambda *args, **kw: prompt_form(*args, pairs=pairs, **kw))
     test, args = FORCED[at]
     test(*args)
 
@@ -592,7 +593,7 @@ def test_the_form_is_the_rules_and_both_kernels_agree_on_it():
     case = make_attention(15, lens, counts, H, G, 128, 64, torch.float16)
     out = check_attention(case, 128)
     work = ops.kv8_attention_workspace("cuda")
-    forced = prompt_form(*case, torch.empty_like(out), 128 ** -0.5, work)
+    forced = prompt_form(*case, torch.empty_like(out), 128 ** -0.5, work, pairs=sum(counts) * H > 160 * torch.cuda.get_device_properties(0).multi_processor_count)
     share = torch.cuda.get_device_properties(0).multi_processor_count // 4 * 128
     rows = [n * H // G for n in counts]
     total = sum(r * G * -(-n // 128) for r, n in zip(rows, lens) if r >= 65)
