@@ -383,7 +383,8 @@ int qspec_rope_qkhad_kvcache(void* qkv, const void* cos_sin_cache, const int* po
  *   positions, seq_ids, slots [ntok]: of each token; -1 where there is none. state_out [requests + 2]: the state behind this step, then the number of
  *   requests refused.
  * `state` is not changed, nor is anything that it describes (table entries and list entries behind it are): a step that is given up costs nothing, one that
- * is made is made so by copying state_out over state. state_out must not overlap state. requests <= 4096, width <= 2^18. */
+ * is made is made so by copying state_out over state. What is
+ * written must not overlap anything else. requests <= 4096, width <= 2^18. */
 int qspec_page_plan(const int* lengths, const int* counts, int* table, int* free_pages, const int* state, int requests, int width, int npages,
                     int page_tokens, int ntok, int* q_start, int* kv_len, int* positions, int* seq_ids, int* slots, int* state_out, void* stream);
 

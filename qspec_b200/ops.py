@@ -840,8 +840,9 @@ def page_plan(lengths: torch.Tensor, counts: torch.Tensor, table: torch.Tensor, 
     _i32(state, "state", B + 1); _i32(q_start, "q_start", B + 1); _i32(kv_len, "kv_len", B); _i32(positions, "positions", T)
     _i32(seq_ids, "seq_ids", T); _i32(slots, "slots", T); _i32(state_out, "state_out", B + 2)
     _here(lengths, counts, table, free_pages, state, q_start, kv_len, positions, seq_ids, slots, state_out)
-    if _overlap(state, state_out) or _overlap(lengths, kv_len):
-        raise ValueError("page_plan: state_out and kv_len must not lie over state and lengths (every CTA reads those)")
+    tensors = (lengths, counts, table, free_pages, state, q_start, kv_len, positions, seq_ids, slots, state_out)
+    if any(_overlap(tensors[i], tensors[j]) for i in range(5, 11) for j in range(i)):
+        raise ValueError("page_plan: what is written must not lie over other tensors of the call (every CTA reads the state and the lengths)")
     lib = _lib.load()
     _lib.check(lib.qspec_page_plan(_ptr(lengths), _ptr(counts), _ptr(table), _ptr(free_pages), _ptr(state), B, table.shape[1], free_pages.shape[0], page_tokens, T,
                                    _ptr(q_start), _ptr(kv_len), _ptr(positions), _ptr(seq_ids), _ptr(slots), _ptr(state_out), _stream()), "page_plan")
@@ -862,7 +863,8 @@ def kv8_append(qkv: torch.Tensor, cos_sin_cache: torch.Tensor, positions: torch.
     """Neox RoPE on queries and keys of qkv [T, (H + 2 G) D] (float16 / bfloat16; rows may be strided, left as they are) and the step's keys and values
     into the pages of their slots: codes int8 [pages, G, P, D], scales float32 [pages, G]. q_out [T, H, D] receives the rotated queries (None: they
     are not wanted). A page's scale grows with its rows and its older rows follow; it starts anew when its first row is written. Tokens without
-    a slot (negative) are skipped. The tokens of a page must be neighbours in the batch."""
+    a slot (negative) are skipped. The tokens of a page must be neighbours in the batch, in consecutive rows of the page. q_out may be qkv's own query
+    columns."""
     if _fast_call("kv8_append", qkv, cos_sin_cache, positions, slots, k_codes, v_codes, k_scale, v_scale, q_out):
         return
     n, G, P, D = _kv8_cache(k_codes, v_codes, k_scale, v_scale)
@@ -916,8 +918,9 @@ def kv8_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
                   max_tokens: Optional[int] = None) -> torch.Tensor:
     """Softmax attention of a step's tokens q [T, H, D] (float16 / bfloat16; token and head strides free) over the 8-bit cache: tokens q_start[b] ..
     q_start[b + 1] - 1 are request b's last of kv_len[b], and see its keys up to their own. table int32 [B, W]. out [T, H, D] of q's type; rows that see no
-    key are zeros, rows behind q_start[B] are left as they are. max_tokens: an upper bound of the tokens that a request has in the step (T if not
-    given), by which the form is chosen. workspace: `kv8_attention_workspace`."""
+    key are zeros, rows behind q_start[B] are left as they are; out may be q itself. max_tokens: an upper bound of the tokens that a request has in the step (T if not
+    given). Which form a request takes follows from it and from what the call's requests ask for together, so that a row's last bits may differ with the other
+    requests. workspace: `kv8_attention_workspace`."""
     if _fast_call("kv8_attention", q, k_codes, v_codes, k_scale, v_scale, table, q_start, kv_len, out, sm_scale, workspace, max_tokens):
         return out
     n, G, P, D = _kv8_cache(k_codes, v_codes, k_scale, v_scale)

@@ -602,3 +602,51 @@ def test_the_form_is_the_rules_and_both_kernels_agree_on_it():
     for b, pick in enumerate(picks):
         at = slice(sum(counts[:b]), sum(counts[:b + 1]))
         assert counts[b] == 1 or torch.equal(out[at], forced[at]) == pick
+
+
+# ---- other calls that the documentation allows ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("pairs", [None, False, True])
+@pytest.mark.parametrize("H,G", [(8, 2), (6, 2), (16, 1)])
+def test_attention_of_requests_with_more_tokens_than_keys(H, G, pairs, monkeypatch):
+    """The first tokens stand in front of the first key and see nothing, whole tiles of them, or of one of two tiles."""
+    if pairs is not None:
+        monkeypatch.setattr(ops, "kv8_attention", lambda *args, **kw: prompt_form(*args, pairs=pairs, **kw))
+    lens, counts = [32, 40, 3, 1, 300], [64, 130, 70, 200, 310]
+    case = make_attention(16, lens, counts, H, G, 128, 32, torch.float16)
+    out = check_attention(case, 128)
+    for at, keys, n in zip(case[6].tolist(), lens, counts):
+        assert not out[at:at + n - keys].any() and out[at + n - keys].any()
+
+
+@pytest.mark.parametrize("lens,counts", [([3000, 70], [2, 4]), ([400, 300], [300, 290])])
+def test_attention_over_its_own_queries(lens, counts):
+    case = make_attention(17, lens, counts, 32, 8, 128, 64, torch.float16)
+    want = check_attention(case, 128)
+    q = case[0].clone()
+    ops.kv8_attention(q, *case[1:], q, 128 ** -0.5, ops.kv8_attention_workspace("cuda"))
+    assert torch.equal(q, want)
+
+
+def test_append_turns_queries_in_place():
+    H, G, D, P = 6, 2, 128, 16
+    qkv, cs, pos, slots, codes, scales = make_append(5, [(0, 40), (30, 1), (5, 5)], H, G, D, P, torch.float16)
+    results = []
+    for inplace in (False, True):
+        rows, k, v, ks, vs = qkv.clone(), codes[0].clone(), codes[1].clone(), scales[0].clone(), scales[1].clone()
+        q = rows[:, :H * D].unflatten(1, (H, D)) if inplace else torch.empty(len(pos), H, D, dtype=torch.float16, device="cuda")
+        ops.kv8_append(rows, cs, i32(pos), i32(slots), k, v, ks, vs, q)
+        assert torch.equal(rows[:, H * D:], qkv[:, H * D:])
+        results.append((q.clone(), k, v, ks, vs))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_page_plan_refuses_results_over_its_other_tensors():
+    z = lambda *s: torch.zeros(*s, dtype=I32, device="cuda")  # noqa: E731
+    args = [z(3), z(3), z(3, 4), z(12), z(4), 16, z(4), z(3), z(5), z(5), z(5), z(5)]
+    ops.page_plan(*args)
+    for out, over in ((7, 1), (7, 0), (8, 9), (6, 4), (10, 3), (11, 4)):
+        both = z(20)
+        bad = list(args)
+        bad[out], bad[over] = both[:args[out].numel()], both[1:1 + args[over].numel()]
+        with pytest.raises(ValueError, match="must not lie over"):
+            ops.page_plan(*bad)
