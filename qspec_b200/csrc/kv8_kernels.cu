@@ -406,19 +406,36 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const 
       write(i, tokens(i), id - j * units, std::integral_constant<int, 1>());
     }
   } else {
-    const int c = lane % LANES, rows = (t1 - t0) * a.H, per = APPEND_WARPS * ROWS;
-    for (int r = ((int)blockIdx.x - units) * per + warp * ROWS + lane / LANES; r < rows; r += ((int)gridDim.x - units) * per) {
-      const int tl = a.H == 1 ? r : (int)__umulhi((unsigned)r, a.h_inv), t = t0 + tl, h = r - tl * a.H;
-      const int p = a.positions[t];
-      if (p < 0 || p >= a.cos_rows) continue;
-      float x[16];
-      load_row<BF16, D, true>(a, t, p, h * D, c, x);
-      float lo[8], hi[8];
+    // (two rows a lane under way: a prompt of 4200 tokens 27.0 us with one, so 26.2)
+    const int c = lane % LANES, rows = (t1 - t0) * a.H, per = APPEND_WARPS * ROWS, step = ((int)gridDim.x - units) * per;
+    for (int r = ((int)blockIdx.x - units) * per + warp * ROWS + lane / LANES; r < rows; r += 2 * step) {
+      uint4 lo[2], hi[2], cs[2], sn[2];
+      T* to[2];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { lo[e] = x[e]; hi[e] = x[e + 8]; }
-      T* to = (T*)a.q + (size_t)t * a.q_ts + h * D + c * 8;
-      *reinterpret_cast<uint4*>(to) = pack8<BF16>(lo);
-      *reinterpret_cast<uint4*>(to + D / 2) = pack8<BF16>(hi);
+      for (int k = 0; k < 2; ++k) {
+        const int rr = r + k * step, tl = a.H == 1 ? rr : (int)__umulhi((unsigned)rr, a.h_inv), t = t0 + tl, h = rr - tl * a.H;
+        const int p = rr < rows ? a.positions[t] : -1;
+        to[k] = nullptr;
+        if (p < 0 || p >= a.cos_rows) continue;
+        to[k] = (T*)a.q + (size_t)t * a.q_ts + h * D + c * 8;
+        const T *row = (const T*)a.qkv + (size_t)t * a.ld + h * D + c * 8, *tab = (const T*)a.cos_sin + (size_t)p * D + c * 8;
+        lo[k] = *reinterpret_cast<const uint4*>(row);
+        hi[k] = *reinterpret_cast<const uint4*>(row + D / 2);
+        cs[k] = *reinterpret_cast<const uint4*>(tab);
+        sn[k] = *reinterpret_cast<const uint4*>(tab + D / 2);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (!to[k]) continue;
+        float x[8], y[8], u[8], v[8], o[8];
+        unpack8<BF16>(lo[k], x); unpack8<BF16>(hi[k], y); unpack8<BF16>(cs[k], u); unpack8<BF16>(sn[k], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = __fsub_rn(__fmul_rn(x[e], u[e]), __fmul_rn(y[e], v[e]));
+        *reinterpret_cast<uint4*>(to[k]) = pack8<BF16>(o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = __fadd_rn(__fmul_rn(y[e], u[e]), __fmul_rn(x[e], v[e]));
+        *reinterpret_cast<uint4*>(to[k] + D / 2) = pack8<BF16>(o);
+      }
     }
   }
 }
