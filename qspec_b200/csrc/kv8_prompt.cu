@@ -104,8 +104,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   unsigned char* const gbase = raw + (base - smem_addr(raw));
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
 
-  // ---- this CTA's request and tile: tiles of all requests in a row, the last one of a request (with the longest way) first
-  const int per_thread = (a.nreq + NTHREADS - 1) / NTHREADS, b0 = tid * per_thread, requests = max(min(per_thread, a.nreq - b0), 0);
+  // ---- this CTA's request and tile: tiles of all requests in a row, the last one of a request (with the longest way) first. Up to 32 requests every warp looks for
+  // itself, without barriers.
+  const bool few = a.nreq <= 32;
+  const int lookers = few ? 32 : NTHREADS, per_thread = (a.nreq + lookers - 1) / lookers, b0 = (few ? lane : tid) * per_thread, requests = max(min(per_thread, a.nreq - b0), 0);
   auto load = [&](int b, int& n, int& keys) {
     n = max(min(a.q_start[b + 1], a.ntok) - min(max(a.q_start[b], 0), a.ntok), 0);
     keys = max(a.kv_len[b], 0);
@@ -118,11 +120,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-  if (lane == 0) s_work[warp] = work;
-  __syncthreads();
-  work = 0;
+  if (!few) {
+    if (lane == 0) s_work[warp] = work;
+    __syncthreads();
+    work = 0;
 #pragma unroll
-  for (int w = 0; w < NWARPS; ++w) work += s_work[w];
+    for (int w = 0; w < NWARPS; ++w) work += s_work[w];
+  }
   auto tiles_of = [&](int b) {
     if (per_thread > 1) load(b, n1, keys1);
     return to_prompt_form(n1, keys1, rep, a.share, work) ? (n1 + span - 1) / span : 0;
@@ -135,28 +139,45 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     const int w = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += w;
   }
-  if (lane == 31) s_sum[warp] = incl;
-  __syncthreads();
   int before = incl - mine;
-  for (int w = 0; w < warp; ++w) before += s_sum[w];
+  if (!few) {
+    if (lane == 31) s_sum[warp] = incl;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NWARPS; ++w)
+      if (w < warp) before += s_sum[w];
+  }
+  int req = -1, tile = 0, first = 0, n_new = 0, keys = 0;
   if ((int)blockIdx.y >= before && (int)blockIdx.y < before + mine) {
     int at = before;
     for (int i = 0; i < requests; ++i) {
       const int n = tiles_of(b0 + i);
       if ((int)blockIdx.y < at + n) {
-        s_at[0] = b0 + i;
-        s_at[1] = n - 1 - ((int)blockIdx.y - at);
-        s_at[2] = a.q_start[b0 + i];
-        s_at[3] = n1;
-        s_at[4] = keys1;
+        req = b0 + i;
+        tile = n - 1 - ((int)blockIdx.y - at);
+        first = min(max(a.q_start[req], 0), a.ntok);
+        n_new = n1;
+        keys = keys1;
         break;
       }
       at += n;
     }
   }
-  __syncthreads();
-  if (s_at[0] < 0) return;
-  const int req = s_at[0], tile = s_at[1], first = min(max(s_at[2], 0), a.ntok), n_new = s_at[3], keys = s_at[4];
+  if (few) {
+    const unsigned found = __ballot_sync(0xffffffffu, req >= 0);
+    if (!found) return;
+    const int who = __ffs(found) - 1;
+    req = __shfl_sync(0xffffffffu, req, who);
+    tile = __shfl_sync(0xffffffffu, tile, who);
+    first = __shfl_sync(0xffffffffu, first, who);
+    n_new = __shfl_sync(0xffffffffu, n_new, who);
+    keys = __shfl_sync(0xffffffffu, keys, who);
+  } else {
+    if (req >= 0) { s_at[0] = req; s_at[1] = tile; s_at[2] = first; s_at[3] = n_new; s_at[4] = keys; }
+    __syncthreads();
+    if (s_at[0] < 0) return;
+    req = s_at[0]; tile = s_at[1]; first = s_at[2]; n_new = s_at[3]; keys = s_at[4];
+  }
   const int t0 = tile * span, n2 = min(span, n_new - t0);   // this CTA's tokens
   const int pos0 = keys - n_new + t0;                     // position of the first
   const bool both = n2 > tok;                             // two tiles of rows, a stream each
@@ -352,7 +373,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       else
         asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};\n" ::"r"(to), "r"(0u) : "memory");
     }
-    asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;\nbar.sync 1, %0;\n" ::"n"(SOFTMAX * 32) : "memory");   // (behind nothing that may be given up)
+    auto ready = [&] {                                    // for the products
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(smem_addr(&b_q));
+    };
+    asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;\n" ::: "memory");
+    if (!BF16) ready();                                   // (as they are)
+    asm volatile("bar.sync 1, %0;\n" ::"n"(SOFTMAX * 32) : "memory");   // (behind nothing that may be given up)
     if (tid < tiles * 128) {
       const int r = tid & 127;
       unsigned char* const row = gbase + (tid >> 7) * OP + r * 128;
@@ -387,9 +415,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       s_rowf[tid] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2 * 16777216.f;   // (scores come in units of 2^-24)
       s_sum128[tid] = ((sums[0] + sums[1]) + (sums[2] + sums[3])) * (128.f / 16777216.f);
     }
-    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    __syncwarp();
-    if (lane == 0) bar_arrive(smem_addr(&b_q));
+    if (BF16) ready();
+    asm volatile("bar.sync 1, %0;\n" ::"n"(SOFTMAX * 32) : "memory");   // (the factors of the rows)
     // ---- softmax: thread = row r of stream z
     const int z = warp >> 2, r = (warp & 3) * 32 + lane, turns = z ? turns1 : turns0, zrow = both ? z * 128 : 0, ztok = both ? z * tok : 0;
     const int tl = ztok + token_of(r);
@@ -399,8 +426,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     const uint32_t st = tmem + lanes + z * 128, ot = tmem + lanes + 256 + z * D;
     bool ok = !(a.give_up & 1u);
     if (!ok) s_fail = 1;
-    ok = ok && bar_wait(smem_addr(&b_q), 0, &s_fail);     // (the factors of the rows)
-    ok = __all_sync(0xffffffffu, ok);
     const float rowf = s_rowf[zrow + r], sum128 = s_sum128[zrow + r];
     float m = NONE, l = 0.f;
     for (int i = 0; ok && i < turns; ++i) {
