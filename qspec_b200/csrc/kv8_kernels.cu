@@ -207,7 +207,7 @@ struct AppendArgs {
   float *ks, *vs;
   void* q; long long q_ts;
   int ntok, H, G, npages, pshift, block;          // block: tokens of a CTA
-  unsigned h_inv;                                 // r * h_inv >> 32 = r / H for the rows of a CTA's tokens
+  int tshift;                                     // 2^tshift: block, or the next power of two
 };
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;   // 2^-60
 constexpr int APPEND_WARPS = 8, SHORT = 8;        // warps of a CTA; tokens of a run up to which it is one warp's
@@ -406,35 +406,38 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const 
       write(i, tokens(i), id - j * units, std::integral_constant<int, 1>());
     }
   } else {
-    // (two rows a lane under way: a prompt of 4200 tokens 27.0 us with one, so 26.2)
-    const int c = lane % LANES, rows = (t1 - t0) * a.H, per = APPEND_WARPS * ROWS, step = ((int)gridDim.x - units) * per;
-    for (int r = ((int)blockIdx.x - units) * per + warp * ROWS + lane / LANES; r < rows; r += 2 * step) {
-      uint4 lo[2], hi[2], cs[2], sn[2];
-      T* to[2];
+    // LANES lanes take a token and some of its heads, two under way at a time: one look at the position and the angles for all of them (row by row, with both
+    // for each, a prompt of 4200 tokens took 26.2 us, so 24.0).
+    const int c = lane % LANES, group = warp * ROWS + lane / LANES, t = t0 + (group & ((1 << a.tshift) - 1)), per_cta = (APPEND_WARPS * ROWS) >> a.tshift;
+    const int p = t < t1 ? a.positions[t] : -1;
+    if (p < 0 || p >= a.cos_rows) return;
+    const T *row = (const T*)a.qkv + (size_t)t * a.ld + c * 8, *tab = (const T*)a.cos_sin + (size_t)p * D + c * 8;
+    T* const to = (T*)a.q + (size_t)t * a.q_ts + c * 8;
+    float cs[8], sn[8];
+    unpack8<BF16>(*reinterpret_cast<const uint4*>(tab), cs);
+    unpack8<BF16>(*reinterpret_cast<const uint4*>(tab + D / 2), sn);
+    const int step = ((int)gridDim.x - units) * per_cta;
+    for (int h0 = ((int)blockIdx.x - units) * per_cta + (group >> a.tshift); h0 < a.H; h0 += 2 * step) {
+      uint4 lo[2], hi[2];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const int rr = r + k * step, tl = a.H == 1 ? rr : (int)__umulhi((unsigned)rr, a.h_inv), t = t0 + tl, h = rr - tl * a.H;
-        const int p = rr < rows ? a.positions[t] : -1;
-        to[k] = nullptr;
-        if (p < 0 || p >= a.cos_rows) continue;
-        to[k] = (T*)a.q + (size_t)t * a.q_ts + h * D + c * 8;
-        const T *row = (const T*)a.qkv + (size_t)t * a.ld + h * D + c * 8, *tab = (const T*)a.cos_sin + (size_t)p * D + c * 8;
-        lo[k] = *reinterpret_cast<const uint4*>(row);
-        hi[k] = *reinterpret_cast<const uint4*>(row + D / 2);
-        cs[k] = *reinterpret_cast<const uint4*>(tab);
-        sn[k] = *reinterpret_cast<const uint4*>(tab + D / 2);
+        const int h = min(h0 + k * step, a.H - 1);
+        lo[k] = *reinterpret_cast<const uint4*>(row + h * D);
+        hi[k] = *reinterpret_cast<const uint4*>(row + h * D + D / 2);
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if (!to[k]) continue;
-        float x[8], y[8], u[8], v[8], o[8];
-        unpack8<BF16>(lo[k], x); unpack8<BF16>(hi[k], y); unpack8<BF16>(cs[k], u); unpack8<BF16>(sn[k], v);
+        const int h = h0 + k * step;
+        if (h >= a.H) break;
+        float x[8], y[8], o[8];
+        unpack8<BF16>(lo[k], x);
+        unpack8<BF16>(hi[k], y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = __fsub_rn(__fmul_rn(x[e], u[e]), __fmul_rn(y[e], v[e]));
-        *reinterpret_cast<uint4*>(to[k]) = pack8<BF16>(o);
+        for (int e = 0; e < 8; ++e) o[e] = __fsub_rn(__fmul_rn(x[e], cs[e]), __fmul_rn(y[e], sn[e]));
+        *reinterpret_cast<uint4*>(to + h * D) = pack8<BF16>(o);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = __fadd_rn(__fmul_rn(y[e], u[e]), __fmul_rn(x[e], v[e]));
-        *reinterpret_cast<uint4*>(to[k] + D / 2) = pack8<BF16>(o);
+        for (int e = 0; e < 8; ++e) o[e] = __fadd_rn(__fmul_rn(y[e], cs[e]), __fmul_rn(x[e], sn[e]));
+        *reinterpret_cast<uint4*>(to + h * D + D / 2) = pack8<BF16>(o);
       }
     }
   }
@@ -511,14 +514,14 @@ extern "C" int qspec_kv8_append(const void* qkv, long long ld, const void* cos_s
   QSPEC_REQUIRE(ld >= (long long)(H + 2 * G) * D && ld % 8 == 0 && (!q_out || (q_tok_stride >= (long long)H * D && q_tok_stride % 8 == 0)) && ((uintptr_t)qkv & 15) == 0 &&
                     ((uintptr_t)cos_sin & 15) == 0 && ((uintptr_t)q_out & 15) == 0,
                 QSPEC_ERR_INVALID_ARG, "kv8_append: rows must lie on 16-byte boundaries (ld=%lld)", ld);
-  AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (signed char*)k, (signed char*)v, ks, vs, q_out, q_tok_stride, ntok, H, G, npages, page_shift(page_tokens), 1,
-               (unsigned)(((1ull << 32) + H - 1) / H)};    // (31 * 4096 rows at most: r times what h_inv is too large by stays below 2^32)
+  AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (signed char*)k, (signed char*)v, ks, vs, q_out, q_tok_stride, ntok, H, G, npages, page_shift(page_tokens), 1, 0};
   // Small blocks put more CTAs on a call with few tokens, large ones have fewer that find nothing to begin (32 / 8 heads of 128, pages of 16, us with blocks of 8, 16
   // and 31: 64 requests of a token 3.0, 3.8, 5.9; 200 of 6 tokens 10.5, 9.1, 8.5; one prompt of 256 3.8, 4.3, 5.2; of 512 5.6, 5.2, 5.7; of 4200 35.8, 30.6, 29.1).
   a.block = ntok <= 256 ? 8 : ntok <= 1024 ? 16 : 31;       // (31: with the token before them one a lane)
-  const int rows = APPEND_WARPS * 32 * 16 / D;              // query rows that a CTA takes at a time
+  a.tshift = ntok <= 256 ? 3 : ntok <= 1024 ? 4 : 5;
+  const int heads = ((APPEND_WARPS * 32 * 16 / D) >> a.tshift) * (ntok <= 256 ? 2 : 4);   // that a CTA turns of every token (that prompt with 2: 25.7, 8: 24.8)
   // (the parts of a block of tokens side by side: page writers wait, queries stream)
-  const dim3 grid(2 * G + (q_out ? (a.block * H + 2 * rows - 1) / (2 * rows) : 0), (ntok + a.block - 1) / a.block);
+  const dim3 grid(2 * G + (q_out ? (H + heads - 1) / heads : 0), (ntok + a.block - 1) / a.block);
   QSPEC_REQUIRE(grid.y <= 65535, QSPEC_ERR_UNSUPPORTED, "kv8_append: %d tokens are too many for one call", ntok);
   auto kern = dtype == QSPEC_DTYPE_F16 ? (D == 128 ? kv8_append_kernel<false, 128> : kv8_append_kernel<false, 64>)
                                        : (D == 128 ? kv8_append_kernel<true, 128> : kv8_append_kernel<true, 64>);
