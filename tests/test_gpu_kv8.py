@@ -195,7 +195,7 @@ def test_append_of_long_steps(runs, D, P, H, G, dtype):
     check_append(runs, D, P, H, G, dtype, False, 90)
 
 
-@pytest.mark.parametrize("D,P,H,G,dtype", [(128, 64, 8, 2, torch.float16), (64, 16, 6, 3, torch.bfloat16)])
+@pytest.mark.parametrize("D,P,H,G,dtype", [(128, 64, 8, 2, torch.float16), (64, 16, 6, 3, torch.bfloat16), (128, 16, 1, 1, torch.float16), (64, 32, 37, 1, torch.float16)])
 @pytest.mark.parametrize("runs", [[(60 + i, 1) for i in range(70)], [(i * 7, 1 + i % 11) for i in range(30)], [(3, 8), (64, 9), (1, 7), (0, 40), (5, 1), (6, 1), (16, 17), (8, 8)] * 4,
                                   [(i, 1) for i in range(1030)], [(i % 50, 2 + 17 * (i % 2)) for i in range(60)]])
 @pytest.mark.parametrize("spoil", [False, True])
