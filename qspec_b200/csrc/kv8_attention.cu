@@ -19,8 +19,9 @@
 //   products cut off would be of the size of what is left.)
 //
 // bfloat16 queries are multiplied by a power of two per row that brings their largest value to 2^14 .. 2^15 and are float16 from there on, exactly. A key's scale
-// multiplies its scores in float32. A value's scale v goes into the exponent: the weights 2^(s + log2 v - m) lie below 2^8 whatever the scales are and are
-// rounded to float16 (2^-11 relative) for the product with the codes; the denominator is the sum of the unrounded weights / v.
+// multiplies its scores in float32. A value's scale v goes into the exponent: the weights 2^(9 + s + log2 v - m) lie below 2^15 whatever the scales are and are
+// rounded to float16 for the product with the codes (by 2^-11 of themselves at most, or by 2^-34 of the largest: kv8_common.cuh); the denominator is the sum of the
+// unrounded weights / v.
 #include "kv8_common.cuh"
 
 namespace qspec {
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
         const int src = (16 * q) >> a.pshift;
         const float f = positive(__shfl_sync(0xffffffffu, cks, src)) * 16777216.f, v = positive(__shfl_sync(0xffffffffu, cvs, src));
         lv[q] = __log2f(v);
-        iv[q] = __fdividef(1.f, v);
+        iv[q] = __fdividef(WEIGHT_UNIT, v);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           kf[q][e] = normal(f * rowf[e]);
@@ -464,8 +465,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
       for (int e = 0; e < 2; ++e) {
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-        // The reference follows the maximum only where it has fallen 2^8 behind: weights stay below 2^8, and sums are seldom multiplied again.
-        grown[e] = mx[e] > m[e] + 8.f || (m[e] == NONE && mx[e] > NONE);
+        // The reference follows the maximum only where it has fallen behind: sums are seldom multiplied again.
+        grown[e] = mx[e] > m[e] + GROWTH_LOG2 || (m[e] == NONE && mx[e] > NONE);
       }
       if (__any_sync(0xffffffffu, (grown[0] && m[0] != NONE) || (grown[1] && m[1] != NONE))) {
         const float f[2] = {grown[0] ? exp2_fast(m[0] - mx[0]) : 1.f, grown[1] ? exp2_fast(m[1] - mx[1]) : 1.f};
@@ -478,19 +479,20 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
       for (int e = 0; e < 2; ++e)
         if (grown[e]) m[e] = mx[e];                         // (a row that had seen nothing has sums of zero)
       const float ref[2] = {m[0] == NONE ? 0.f : m[0], m[1] == NONE ? 0.f : m[1]};
-      // Exponents are taken from the products without a rounding in between, the reference has one: beyond 2^24 that alone would be a large exponent.
-      if (__any_sync(0xffffffffu, fabsf(ref[0]) > 16777216.f || fabsf(ref[1]) > 16777216.f)) {
+      // Exponents are taken from the products without a rounding in between, the reference has one: far from zero that alone would be a large exponent.
+      const bool far = __any_sync(0xffffffffu, fabsf(ref[0]) > FAR || fabsf(ref[1]) > FAR);
+      if (far) {
 #pragma unroll
         for (int nt = 0; nt < KT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] = fmaf(s[nt][e], kf[nt >> 1][e >> 1], lv[nt >> 1]);
+          for (int e = 0; e < 4; ++e) s[nt][e] = fmaf(s[nt][e], kf[nt >> 1][e >> 1], lv[nt >> 1]) - ref[e >> 1];
 #pragma unroll
-        for (int q = 0; q < QT; ++q) { kf[q][0] = kf[q][1] = 1.f; lv[q] = 0.f; }
+        for (int q = 0; q < QT; ++q) kf[q][0] = kf[q][1] = 1.f;
       }
       uint32_t pa[QT][4];
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
-        const float at[2] = {lv[q] - ref[0], lv[q] - ref[1]};
+        const float base = lv[q] + WEIGHT_LOG2, at[2] = {far ? WEIGHT_LOG2 : base - ref[0], far ? WEIGHT_LOG2 : base - ref[1]};
         float part[2] = {0.f, 0.f};
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
@@ -581,7 +583,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
     const bool starts = cur.u == 0, ends = cur.u + seg_n == cur.r.units;
     if (starts && ends) {
       if (tile * ROWS + jr < cur.r.n * a.rep) {
-        const float f = ll == 0.f ? 0.f : __fdiv_rn(1.f, ll);   // (no key: zeros)
+        const float f = ll == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, ll);   // (no key: zeros)
 #pragma unroll
         for (int c = 0; c < PIECES; ++c) store_piece(jr, (col + PER_ROW * c) * 4, oo[c], f);
       }
@@ -636,7 +638,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
           const float f = factor[i * ROWS + jr];
           factor[i * ROWS + jr] = f == NONE ? 0.f : f == INFINITY ? 1.f : exp2_fast(f - mm);
         }
-        if (col == 0) factor[n * ROWS + jr] = ll == 0.f ? 0.f : __fdiv_rn(1.f, ll);   // (no key: zeros)
+        if (col == 0) factor[n * ROWS + jr] = ll == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, ll);   // (no key: zeros)
         __syncthreads();
         const int rows = min(cur.r.n * a.rep - tile * ROWS, ROWS);
         for (int x = tid; x < rows * (D / 4); x += THREADS) {

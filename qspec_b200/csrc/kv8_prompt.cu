@@ -10,10 +10,10 @@
 //     to a row's scores is taken out where they enter the exponent. Values are c exactly: a byte behind 0x64 is 1152 + c, less 1152.
 //   * S = Q K^T, accumulator [128 x 128] float32 in tensor memory, one for each stream.
 //   * softmax: thread = row, four warps a stream. Scores are read twice, for the maximum and for the weights (that keeps 128 of them out of the registers).
-//     Weights go back over the scores as float16 (2^-11 relative; the result is rounded to 16 bits as well).
+//     Weights go back over the scores as float16 (off by 2^-11 of themselves or by 2^-34 of the largest, as in kv8_attention.cu; the result is rounded to 16 bits as well).
 //   * O += P V: weights from tensor memory, values from shared memory as they lie in the cache (operand "MN-major").
 // Tensor memory: S | S | O | O = 512 columns. Scales and the exponent that takes the value scale in: as in kv8_attention.cu. O is multiplied again only
-// where a row's maximum grew by more than 2^8.
+// where a row's maximum grew by more than 2^6.
 // What a block of 128 x 128 (head 128) asks of an SM: 1024 cycles of the tensor cores, 1024 of the exponentials (16 a cycle), and of the schedulers 720 by the softmax
 // and 400 by the codes (200 of two tiles). It takes 2350 cycles of two tiles (2850 to 3400 of one): what bounds it is a stream's way from scores to the next scores,
 // 4700 cycles, of which the softmax is 3000 (a warp's 32 exponentials and what belongs to them 570) and the products with their waits 1700; start and end of a CTA are
@@ -54,11 +54,6 @@ struct alignas(16) Block {                                            // what th
   float kf[8], lv[8], iv[8];                              // scale of the keys; log2 of the values' scale, and its reciprocal
   unsigned bad;                                           // bit q: a page that there is not, or a scale that is no number
 };
-
-__device__ __forceinline__ void st8(uint32_t addr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-               "r"(r[7]) : "memory");
-}
 
 __device__ __forceinline__ void ld16(uint32_t addr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
@@ -227,7 +222,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         v = positive(v);
         s_block[slot].kf[lane] = positive(k);
         s_block[slot].lv[lane] = __log2f(v);
-        s_block[slot].iv[lane] = __fdividef(1.f, v);
+        s_block[slot].iv[lane] = __fdividef(WEIGHT_UNIT, v);
         if (lane == 0) s_block[slot].bad = mask;
       }
       __syncwarp();
@@ -450,8 +445,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
           if (j0 + c0 + j > limit) x[j] = 0xff800000u;
         }
       };
-      // ---- the largest exponent
-      float mn = NONE;
+      // ---- the largest exponent; and the largest that is taken from a score
+      float mn = NONE, taken = 0.f;
 #pragma unroll 1
       for (int c0 = 0; c0 < 128; c0 += 32) {
         uint32_t x[32];
@@ -469,28 +464,33 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
             if (j + 2 < 16) t[1] = fmaxf(fmaxf(t[1], __uint_as_float(x[q * 16 + j + 2])), __uint_as_float(x[q * 16 + j + 3]));
           }
           const float k = normal((q ? kf.y : kf.x) * rowf);
-          mn = fmaxf(mn, fmaf(fmaxf(t[0], t[1]), k, fmaf(-sum128, k, q ? lv.y : lv.x)));
+          const float at = fmaf(-sum128, k, q ? lv.y : lv.x);
+          mn = fmaxf(mn, fmaf(fmaxf(t[0], t[1]), k, at));
+          taken = fmaxf(taken, fabsf(at));
         }
       }
-      const bool grown = mn > m + RESCALE_LOG2 || (m == NONE && mn > m);
+      const bool grown = mn > m + GROWTH_LOG2 || (m == NONE && mn > m);
       const float up = grown ? ex2(m - mn) : 1.f;         // 0 for a row that had seen nothing; other rows of the warp keep theirs
       l *= up;
       if (i && __any_sync(0xffffffffu, grown && m != NONE)) {   // (the scores are there: the stream's product before them is over)
 #pragma unroll 1
-        for (int q = 0; q < D / 8; ++q) {
-          uint32_t o[8];
-          ld8(ot + q * 8, o);
+        for (int q = 0; q < D / 32; ++q) {
+          uint32_t o[32];
+          ld32(ot + q * 32, o);
           wait_ld();
-          landed8(o);
+          landed32(o);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * up);
-          st8(ot + q * 8, o);
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * up);
+          st16(ot + q * 32, o);
+          st16(ot + q * 32 + 16, o + 16);
         }
       }
       if (grown) m = mn;
       const float mu = m == NONE ? 0.f : m;
-      // Exponents are taken from the products without a rounding in between, the reference has one: beyond 2^24 that alone would be a large exponent.
-      const bool far = __any_sync(0xffffffffu, fabsf(mu) > 16777216.f);
+      // Exponents are taken from the products without a rounding in between, the reference and what it is joined with have one: far from zero that alone would be a
+      // large exponent.
+      const bool far = __any_sync(0xffffffffu, fmaxf(fabsf(mu), taken) > FAR);
+      const float ref = (far ? 0.f : mu) - WEIGHT_LOG2;
       // ---- weights
 #pragma unroll 2
       for (int c0 = 0; c0 < 128; c0 += 32) {
@@ -503,13 +503,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         if (odd) hide(x, c0);
         if (far) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]), k[j / 16], at[j / 16]));
+          for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]), k[j / 16], at[j / 16]) - mu);
           k[0] = k[1] = 1.f;
           at[0] = at[1] = 0.f;
         }
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const uint64_t k2 = pair(__float_as_uint(k[q]), __float_as_uint(k[q])), at2 = pair(__float_as_uint(at[q] - mu), __float_as_uint(at[q] - mu));
+          const uint64_t k2 = pair(__float_as_uint(k[q]), __float_as_uint(k[q])), at2 = pair(__float_as_uint(at[q] - ref), __float_as_uint(at[q] - ref));
           uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         if (i && both) f[i] = 0.f;
         sum += f[i] == 0.f ? 0.f : li * f[i];
       }
-      const float d = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);          // (no key: zeros)
+      const float d = sum == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, sum);  // (no key: zeros)
       const bool one = turns > 0, two = !both && __any_sync(0xffffffffu, f[1] != 0.f) && (z ? turns0 : turns1) > 0;
       const uint32_t stored = __ballot_sync(0xffffffffu, row_in);
       for (int half = both ? 0 : z; half <= (both ? 1 : z); ++half) {

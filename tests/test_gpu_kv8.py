@@ -650,3 +650,60 @@ def test_page_plan_refuses_results_over_its_other_tensors():
         bad[out], bad[over] = both[:args[out].numel()], both[1:1 + args[over].numel()]
         with pytest.raises(ValueError, match="must not lie over"):
             ops.page_plan(*bad)
+
+
+# ---- a long context's many small weights ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("form", ["rows", "prompt", "pairs"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("ratio,gap", [(1, 25.05), (64, 19.1), (64, 24.0), (16, 21.1)])
+def test_attention_loses_no_keys_of_a_long_context(ratio, gap, dtype, form):
+    """Values that are all 1, whatever their weights: so is the result. The first key's score is above all others' by log2 = gap, and its page may have a value scale that
+    is `ratio` times the others'. Off by the result's rounding; 2^-11 for a weight that is a normal float16; ratio * 2^-34 for each key whose weight is not (2^-25,
+    the largest being 2^9 or more, with the value scale in it); and float32 sums: 2^-23 for every key that one accumulator takes, half of that for the denominator (the
+    tensor cores cut each term of a product at the last place of the largest, which is the sum so far: terms 2^-25 of it, as in the first case, are gone one by one, not by
+    sixteens). In the prompt form that is n keys, in the other a quarter: there so many requests (of the same pages) that each is one CTA's, of four warps."""
+    n, G, H, D, P = 131000, 2, 8, 128, 64
+    B, T = (256, 1) if form == "rows" else (1, 20) if form == "prompt" else (1, 50)
+    pages = -(-n // P)
+    k, v = torch.zeros(pages, G, P, D, dtype=torch.int8, device="cuda"), torch.full((pages, G, P, D), 64, dtype=torch.int8, device="cuda")
+    ks, vs = torch.full((pages, G), gap / 127 / math.log2(math.e), device="cuda"), torch.full((pages, G), 1 / 64, device="cuda")
+    v[0], vs[0] = 64 // ratio, ratio / 64
+    k[0, :, 0, 0] = 127
+    q = torch.zeros(B * T, H, D, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    case = (q, k, v, ks, vs, torch.arange(pages, dtype=I32, device="cuda").repeat(B, 1), i32(range(0, B * T + 1, T)), i32([n] * B))
+    work, out = ops.kv8_attention_workspace("cuda"), torch.empty_like(q)
+    if form == "rows":
+        ops.kv8_attention(*case, out, 1.0, work, max_tokens=1)
+    else:
+        prompt_form(*case, out, 1.0, work, pairs=form == "pairs")
+    chain = n / (4 if form == "rows" else 1)
+    bound = torch.finfo(dtype).eps / 2 + 2.0 ** -11 + n * ratio * 2.0 ** -34 + chain * 1.5 * 2.0 ** -23
+    assert (out.double() - 1).abs().max() <= bound, (float((out.double() - 1).abs().max()), bound)
+
+
+def test_attention_of_scores_far_from_zero():
+    """Exponents of 2^20 to 2^26, where a reference's own rounding is large: weights stay finite, and one key, or several that are alike, take all."""
+    for form in ("rows", "prompt", "pairs"):
+        n, G, D, P, T = 700, 2, 128, 32, 2 if form == "rows" else 40
+        pages = -(-n // P)
+        for log2 in (18, 20, 21.9, 22.1, 23, 23.9, 24.1, 25, 26):
+            for sign in (1.0, -1.0):
+                g = gen(int(log2 * 10))
+                k = torch.zeros(pages, G, P, D, dtype=torch.int8, device="cuda")
+                k[..., 0] = 100                                   # all scores alike, and far from zero
+                v = (torch.randn(pages, G, P, D, generator=g, device="cuda") * 40).round().clamp(-127, 127).to(torch.int8)
+                ks, vs = torch.full((pages, G), 2.0 ** log2 / 100, device="cuda"), torch.full((pages, G), 1 / 64, device="cuda")
+                q = torch.zeros(T, 8, D, dtype=torch.float16, device="cuda")
+                q[:, :, 0] = sign
+                case = (q, k, v, ks, vs, torch.arange(pages, dtype=I32, device="cuda")[None], i32([0, T]), i32([n]))
+                work, out = ops.kv8_attention_workspace("cuda"), torch.empty_like(q)
+                if form == "rows":
+                    ops.kv8_attention(*case, out, 1.0, work, max_tokens=T)
+                else:
+                    prompt_form(*case, out, 1.0, work, pairs=form == "pairs")
+                rows = v.double().permute(1, 0, 2, 3).reshape(G, -1, D) / 64
+                want = torch.stack([rows[:, :n - T + 1 + t].mean(1) for t in range(T)]).repeat_interleave(4, 1)
+                # equal weights: each off by 2^-11, sums by n / 16 * 2^-23, the result by its own rounding
+                size = rows.abs().mean(1).amax()
+                assert ((out.double() - want).abs() <= size * (2.0 ** -11 + 2.0 ** -11 + n / 16 * 2.0 ** -23) + want.abs() * 2.0 ** -11 + 2.0 ** -24).all(), (form, log2, sign)
