@@ -450,12 +450,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
         const int src = (16 * q) >> a.pshift;
-        const float f = positive(__shfl_sync(0xffffffffu, cks, src)) * 16777216.f, v = positive(__shfl_sync(0xffffffffu, cvs, src));
+        const float f = positive(__shfl_sync(0xffffffffu, cks, src)), v = positive(__shfl_sync(0xffffffffu, cvs, src));
         lv[q] = __log2f(v);
         iv[q] = __fdividef(WEIGHT_UNIT, v);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          kf[q][e] = normal(f * rowf[e]);
+          kf[q][e] = score_factor(f, rowf[e]);
           const float top = fmaxf(fmaxf(s[2 * q][2 * e], s[2 * q][2 * e + 1]), fmaxf(s[2 * q + 1][2 * e], s[2 * q + 1][2 * e + 1]));
           mx[e] = fmaxf(mx[e], fmaf(top, kf[q][e], lv[q])); // (factors are positive: the largest score has the largest exponent)
         }

@@ -27,8 +27,9 @@ __device__ __forceinline__ float positive(float x) { return x >= 7.8886090522101
 // 112 us, 2^6 114, 2^5 115, 2^4 117. 2^16 is infinite, and a reference has a rounding of its own: beyond FAR it is subtracted from the finished exponent, which was rounded
 // like it. Sums of weights / v are kept in units of 2^WEIGHT_LOG2, so that they hold for every scale that positive() leaves.
 constexpr float WEIGHT_LOG2 = 9.f, GROWTH_LOG2 = 6.f, WEIGHT_UNIT = 1.f / 512.f, FAR = 1048576.f;
-// A factor of scores, not so small that it would make a hidden key's score (minus infinity) no number.
-__device__ __forceinline__ float normal(float x) { return fmaxf(x, 1.17549435e-38f); }
+// What scores in units of 2^-24 are multiplied with, from the scale of the keys and the row's factor: these two first, since either may be as far from 1 as float32 goes and
+// the other as far on the other side. Not so small that it would make a hidden key's score (minus infinity) no number.
+__device__ __forceinline__ float score_factor(float scale, float row) { return fmaxf(scale * row * 16777216.f, 1.17549435e-38f); }
 
 // Which form of the attention a request goes to, from what all requests of the call ask for; both kernels work it out alike. The prompt form takes 128 rows (tokens *
 // heads of a group) and a head a CTA, so that a block of keys costs it the same however few requests there are; the other one spreads any request over the GPU but

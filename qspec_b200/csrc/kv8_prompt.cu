@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
       const int key = n * 128 + lane * 16, at = key >> a.pshift;
       bool bad = false;
       long long codes = -1;
-      float k = 1.f, v = 1.f;
+      float k = 0.f, v = 1.f;                             // (of keys that there are not: a factor that is next to nothing)
       if (lane < 8 && key < keys) {
         const int page = at < a.width ? a.table[(size_t)req * a.width + at] : -1;
         bad = (unsigned)page >= (unsigned)a.npages;
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         }
         if (BF16) *piece(c) = make_uint4(x[0], x[1], x[2], x[3]);
       }
-      s_rowf[tid] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2 * 16777216.f;   // (scores come in units of 2^-24)
+      s_rowf[tid] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2;
       s_sum128[tid] = ((sums[0] + sums[1]) + (sums[2] + sums[3])) * (128.f / 16777216.f);
     }
     if (BF16) ready();
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
             t[0] = fmaxf(fmaxf(t[0], __uint_as_float(x[q * 16 + j])), __uint_as_float(x[q * 16 + j + 1]));
             if (j + 2 < 16) t[1] = fmaxf(fmaxf(t[1], __uint_as_float(x[q * 16 + j + 2])), __uint_as_float(x[q * 16 + j + 3]));
           }
-          const float k = normal((q ? kf.y : kf.x) * rowf);
+          const float k = score_factor(q ? kf.y : kf.x, rowf);
           const float at = fmaf(-sum128, k, q ? lv.y : lv.x);
           mn = fmaxf(mn, fmaf(fmaxf(t[0], t[1]), k, at));
           taken = fmaxf(taken, fabsf(at));
@@ -497,16 +497,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         uint32_t x[32], p[16];
         ld32(st + c0, x);
         const float2 kf = *reinterpret_cast<const float2*>(&f.kf[c0 / 16]), lv = *reinterpret_cast<const float2*>(&f.lv[c0 / 16]), iv = *reinterpret_cast<const float2*>(&f.iv[c0 / 16]);
-        float k[2] = {normal(kf.x * rowf), normal(kf.y * rowf)}, at[2] = {fmaf(-sum128, k[0], lv.x), fmaf(-sum128, k[1], lv.y)};
+        float k[2] = {score_factor(kf.x, rowf), score_factor(kf.y, rowf)}, at[2] = {fmaf(-sum128, k[0], lv.x), fmaf(-sum128, k[1], lv.y)};
         wait_ld();
         landed32(x);
-        if (odd) hide(x, c0);
         if (far) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]), k[j / 16], at[j / 16]) - mu);
           k[0] = k[1] = 1.f;
           at[0] = at[1] = 0.f;
         }
+        if (odd) hide(x, c0);                             // (behind that: a page that a row does not see may have factors that are infinite with this row's)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const uint64_t k2 = pair(__float_as_uint(k[q]), __float_as_uint(k[q])), at2 = pair(__float_as_uint(at[q] - ref), __float_as_uint(at[q] - ref));

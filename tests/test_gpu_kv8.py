@@ -707,3 +707,33 @@ def test_attention_of_scores_far_from_zero():
                 # equal weights: each off by 2^-11, sums by n / 16 * 2^-23, the result by its own rounding
                 size = rows.abs().mean(1).amax()
                 assert ((out.double() - want).abs() <= size * (2.0 ** -11 + 2.0 ** -11 + n / 16 * 2.0 ** -23) + want.abs() * 2.0 ** -11 + 2.0 ** -24).all(), (form, log2, sign)
+
+
+@pytest.mark.parametrize("form", ["rows", "prompt", "pairs"])
+@pytest.mark.parametrize("log2", [-112, 100, 121])
+def test_attention_of_queries_and_scales_that_make_up_for_each_other(log2, form, monkeypatch):
+    """Tiny queries over keys of a huge scale, and the other way round: the factors of the scores meet before they leave float32."""
+    if form != "rows":
+        monkeypatch.setattr(ops, "kv8_attention", lambda *args, **kw: prompt_form(*args, pairs=form == "pairs", **kw))
+    counts = [1, 3] if form == "rows" else [60, 40]
+    q, k, v, ks, vs, table, start, lens = make_attention(18, [200, 333], counts, 8, 2, 128, 32, torch.bfloat16, q_scale=1.5 * 2.0 ** log2)
+    ks.mul_(2.0 ** -min(log2, 93))                            # (scales below 2^-100 count as that)
+    check_attention((q, k, v, ks, vs, table, start, lens), 128)
+
+
+@pytest.mark.parametrize("form", ["rows", "prompt", "pairs"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_rows_in_front_of_a_page_of_a_huge_scale(dtype, form, monkeypatch):
+    """Scores of the last page leave float32. The rows that do not see it are what they are without it, within the bound of either of the two ways in which exponents are taken
+    (one for all rows of a warp: those that see the page decide, so that the others' last bits may move)."""
+    if form != "rows":
+        monkeypatch.setattr(ops, "kv8_attention", lambda *args, **kw: prompt_form(*args, pairs=form == "pairs", **kw))
+    q, k, v, ks, vs, table, start, lens = make_attention(19, [200, 333], [60, 40], 8, 2, 128, 32, dtype, q_scale=1.5 * 2.0 ** (10 if dtype == torch.float16 else 30))
+    ks.mul_(2.0 ** (-10 if dtype == torch.float16 else -30))
+    check_attention((q, k, v, ks, vs, table, start, lens), 128)
+    want, bound = attention_in_64_bits(q, k, v, ks, vs, table, start, lens, 128 ** -0.5)
+    ks[int(table[0, 6])] = ks[int(table[1, 10])] = 2.0 ** 120   # positions 192 and 320 on
+    out = torch.empty_like(q)
+    ops.kv8_attention(q, k, v, ks, vs, table, start, lens, out, 128 ** -0.5, ops.kv8_attention_workspace("cuda"))
+    for rows in (slice(0, 52), slice(60, 87)):
+        assert ((out[rows].to(F64) - want[rows]).abs() <= bound[rows]).all()
