@@ -393,7 +393,8 @@ int qspec_page_plan(const int* lengths, const int* counts, int* table, int* free
  * A page's scale: the largest of |x| / 127 of the rows that the call writes to it, of its scale before (unless its first row is among them) and 2^-60; codes =
  * rint(x / scale) (infinities: +-127, NaN: 0, neither stretches the scale). Where a scale grows the page's older rows are put on the new one.
  * Rotated values are quantised in float32, without a rounding to 16 bits in between. Tokens whose slot or position is outside the cache or
- * the table of angles are skipped. The tokens of one page in a call must be neighbours in the batch, in consecutive rows. */
+ * the table of angles are skipped: their rows of the cache are left as they are. The tokens of one page in a call must be neighbours in the batch, their slots consecutive rows (a
+ * token without a slot between them breaks that; one without a position does not). Rows of the page behind them are no one's any more: they stay on the scale before. */
 int qspec_kv8_append(const void* qkv, long long ld, const void* cos_sin, int cos_rows, const int* positions, const int* slots, void* k, void* v, float* k_scale,
                      float* v_scale, void* q_out, long long q_tok_stride, int ntok, int H, int G, int D, int npages, int page_tokens, int dtype, void* stream);
 

@@ -212,12 +212,14 @@ struct AppendArgs {
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f;   // 2^-60
 constexpr int APPEND_WARPS = 8, SHORT = 8;        // warps of a CTA; tokens of a run up to which it is one warp's
 
-// the slot of token t, or -1 if nothing is to be written for it
+// the slot of token t, or -1 if it has none. Runs follow from slots alone: a token whose position the table of angles does not have is a row of its page's run for which
+// nothing is written. (With such a token as an end, a page had two runs in a call, each with a scale of its own to write.)
 __device__ __forceinline__ int slot_of(const AppendArgs& a, int t) {
   if (t < 0 || t >= a.ntok) return -1;
-  const int s = a.slots[t], p = a.positions[t];
-  return s >= 0 && s < (a.npages << a.pshift) && p >= 0 && p < a.cos_rows ? s : -1;
+  const int s = a.slots[t];
+  return s >= 0 && s < (a.npages << a.pshift) ? s : -1;
 }
+__device__ __forceinline__ bool has_angle(const AppendArgs& a, int t) { return (unsigned)a.positions[t] < (unsigned)a.cos_rows; }
 
 // sixteen values of a row (token t, at position pos): x[0 .. 7] from column 8 c on, x[8 .. 15] the same of the second half
 template <bool BF16, int D, bool TURN>
@@ -322,9 +324,12 @@ __device__ __forceinline__ void write_run(const AppendArgs& a, int t0, int n, in
   float* scale = scales + (size_t)page * a.G + g;
   const float before = first ? *scale : 0.f;
   float x[16];                                              // the first of this lane's rows
-  auto load = [&](int r) {
-    if (r < n) load_row<BF16, D, TURN>(a, t0 + r, TURN ? a.positions[t0 + r] : 0, col, c, x);
-    return r < n;
+  auto load = [&](int r) {                                  // whether there is something to write
+    if (r >= n) return false;
+    const int pos = a.positions[t0 + r];
+    const bool there = (unsigned)pos < (unsigned)a.cos_rows;   // (not waited for by the row's loads)
+    load_row<BF16, D, TURN>(a, t0 + r, there ? pos : 0, col, c, x);
+    return there;
   };
   auto over_all = [&](float mx) {                           // (and everyone has read the scale)
     mx = warp_xor_max(mx);
@@ -337,29 +342,24 @@ __device__ __forceinline__ void write_run(const AppendArgs& a, int t0, int n, in
     return mx;
   };
   float mx = 0.f;
-  for (int r = r0 + STEP; r < n; r += STEP) {
-    load(r);
-    mx = largest(mx, x);
-  }
-  if (load(r0)) mx = largest(mx, x);
+  for (int r = r0 + STEP; r < n; r += STEP)
+    if (load(r)) mx = largest(mx, x);
+  const bool there = load(r0);
+  if (there) mx = largest(mx, x);
   mx = over_all(mx);
   const bool odd = mx == INFINITY;
   if (odd) {                                                // the largest of those that are finite
     mx = 0.f;
-    for (int r = r0 + STEP; r < n; r += STEP) {
-      load(r);
-      mx = finite_max(mx, x);
-    }
+    for (int r = r0 + STEP; r < n; r += STEP)
+      if (load(r)) mx = finite_max(mx, x);
     if (load(r0)) mx = finite_max(mx, x);
     mx = over_all(mx);
   }
   __syncwarp();
   const float after = new_scale(mx, before), inv = __frcp_rn(after);
-  if (r0 < n) store_codes<D>(rows + (size_t)(first + r0) * D, c, x, inv, odd);
-  for (int r = r0 + STEP; r < n; r += STEP) {
-    load(r);
-    store_codes<D>(rows + (size_t)(first + r) * D, c, x, inv, odd);
-  }
+  if (there) store_codes<D>(rows + (size_t)(first + r0) * D, c, x, inv, odd);
+  for (int r = r0 + STEP; r < n; r += STEP)
+    if (load(r)) store_codes<D>(rows + (size_t)(first + r) * D, c, x, inv, odd);
   if (first && after > before) rescale(rows, first * (D / 16), warp * 32 + lane, WARPS * 32, before, after);
   if (warp == 0 && lane == 0 && after != before) *scale = after;
 }
@@ -389,8 +389,11 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const 
     for (int o = 1; o < SHORT; o <<= 1) more &= more >> o;
     auto write = [&](int i, int n, int u, auto warps) {     // the run of n tokens that begins with token t0 + i
       constexpr int W = decltype(warps)::value;
-      const int t = t0 + i, s = __shfl_sync(0xffffffffu, sa, i + 1), g = u >> 1;
+      int t = t0 + i, s = __shfl_sync(0xffffffffu, sa, i + 1);
+      const int g = u >> 1;
       if (W > 1 && t + n >= t0 + 63) n = run_of(a, t, s, n);   // (it may be longer than that)
+      while (n && !has_angle(a, t)) { ++t; ++s; --n; }      // (it begins with the first token that is written)
+      if (!n) return;
       if (u & 1) write_run<BF16, D, false, W>(a, t, n, s, g, (a.H + a.G + g) * D, a.v, a.vs, s_max);
       else write_run<BF16, D, true, W>(a, t, n, s, g, (a.H + g) * D, a.k, a.ks, s_max);
     };

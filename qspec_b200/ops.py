@@ -863,8 +863,9 @@ def kv8_append(qkv: torch.Tensor, cos_sin_cache: torch.Tensor, positions: torch.
     """Neox RoPE on queries and keys of qkv [T, (H + 2 G) D] (float16 / bfloat16; rows may be strided, left as they are) and the step's keys and values
     into the pages of their slots: codes int8 [pages, G, P, D], scales float32 [pages, G]. q_out [T, H, D] receives the rotated queries (None: they
     are not wanted). A page's scale grows with its rows and its older rows follow; it starts anew when its first row is written. Tokens without
-    a slot (negative) are skipped. The tokens of a page must be neighbours in the batch, in consecutive rows of the page. q_out may be qkv's own query
-    columns."""
+    a slot (negative), or with a position that the table of angles does not have, are skipped. The tokens of a page must be neighbours in the batch, their slots consecutive
+    rows of the page with none missing between them; rows of the page behind them are no one's any more. q_out may be qkv's own query columns, but lie over
+    nothing else of the call."""
     if _fast_call("kv8_append", qkv, cos_sin_cache, positions, slots, k_codes, v_codes, k_scale, v_scale, q_out):
         return
     n, G, P, D = _kv8_cache(k_codes, v_codes, k_scale, v_scale)

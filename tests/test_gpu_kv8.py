@@ -737,3 +737,39 @@ def test_attention_rows_in_front_of_a_page_of_a_huge_scale(dtype, form, monkeypa
     ops.kv8_attention(q, k, v, ks, vs, table, start, lens, out, 128 ** -0.5, ops.kv8_attention_workspace("cuda"))
     for rows in (slice(0, 52), slice(60, 87)):
         assert ((out[rows].to(F64) - want[rows]).abs() <= bound[rows]).all()
+
+
+@pytest.mark.parametrize("P", [16, 128])
+@pytest.mark.parametrize("runs", [[(3, 6), (40, 2)], [(16, 16), (0, 1), (5, 60)], [(10, 118), (250, 130), (7, 9)], [(i, 1 + i % 13) for i in range(60)]])
+def test_append_leaves_out_tokens_without_a_position_in_the_middle_of_a_page(runs, P):
+    """A page's tokens are one run whatever positions they have: one scale, of those that are written, from the first of these on."""
+    H, G, D = 4, 2, 128
+    qkv, cs, pos, slots, codes, scales = make_append(9, runs, H, G, D, P, torch.float16, pages=400)
+    T = len(pos)
+    left_out = torch.rand(T, generator=torch.Generator().manual_seed(T)) < 0.4
+    left_out[:2] = True                                       # the first of a run among them
+    given = [len(cs) + i % 5 if o and i % 2 else -1 - i % 3 if o else p for i, (p, o) in enumerate(zip(pos, left_out.tolist()))]
+    x = qkv.float().view(T, H + 2 * G, D)
+    turned = rotated(x[:, :H + G], cs[torch.tensor(pos, device="cuda")].float(), F32)
+    k, v, ks, vs = codes[0].clone(), codes[1].clone(), scales[0].clone(), scales[1].clone()
+    q = torch.full((T, H, D), 9.0, dtype=torch.float16, device="cuda")
+    ops.kv8_append(qkv, cs, i32(given), i32(slots), k, v, ks, vs, q)
+    out = left_out.cuda()
+    assert (q[out] == 9).all() and torch.equal(q[~out], turned[:, :H].half()[~out])
+    for y, c, s, got_c, got_s in ((turned[:, H:], codes[0].clone(), scales[0].clone(), k, ks), (x[:, H + G:], codes[1].clone(), scales[1].clone(), v, vs)):
+        begin = 0
+        while begin < T:
+            n = 1
+            while begin + n < T and slots[begin + n] == slots[begin] + n and slots[begin + n] % P:
+                n += 1
+            some = [t for t in range(begin, begin + n) if not left_out[t]]
+            begin += n
+            if not some:
+                continue
+            page, row = slots[some[0]] // P, [slots[t] % P for t in some]
+            before = s[page] if row[0] else torch.zeros_like(s[page])
+            after = torch.maximum(torch.maximum(y[some].abs().amax((0, 2)) * torch.tensor(1.0 / 127.0, device="cuda"), before), torch.tensor(2.0 ** -60, device="cuda"))
+            c[page, :, :row[0]] = (c[page, :, :row[0]].float() * (before / after)[:, None, None]).round().to(torch.int8)
+            c[page][:, row] = (y[some] * after.reciprocal()[None, :, None]).round().clamp(-127, 127).to(torch.int8).transpose(0, 1)
+            s[page] = after
+        assert torch.equal(got_s, s) and torch.equal(got_c, c)
