@@ -419,9 +419,10 @@ class QSpecLlamaModel(torch.nn.Module):
         for _, slot, first, n in meta.segments:
             lengths[slot], counts[slot] = first, n
         step = cache.plan(on_device(lengths), on_device(counts), meta.ntok, max(counts))
+        if self.cfg.kv_pages is not None and (refused := cache.short()):   # (with the default number of pages every sequence fits)
+            raise RuntimeError(f"the 8-bit cache is full: {cache.pages} pages of {cache.page_tokens} tokens have no room for {refused} sequence(s) of this step; none of it "
+                               "has been taken, and once sequences have been released it can be made again")
         cache.commit()
-        if self.cfg.kv_pages is not None and cache.refused():        # (with the default number of pages every sequence fits)
-            raise RuntimeError(f"the 8-bit cache is full: {cache.pages} pages of {cache.page_tokens} tokens")
         ids = input_ids.to(torch.int64)
         if order == list(range(len(order))):
             return self.forward(ids, None, None, w4a4=False, step=step)

@@ -33,7 +33,7 @@ class PagedKV8Cache:
     def __init__(self, layers: int, kv_heads: int, head_dim: int, requests: int, max_request_tokens: int, max_step_tokens: int, device, page_tokens: int = 64,
                  pages: Optional[int] = None):
         """pages: of the whole cache; default: enough for every request at its longest (fewer where memory is to be shared: a step that asks for more than
-        there is refuses requests, see `refused`)."""
+        there is refuses requests, see `short` and `refused`; nothing takes pages from one request for another)."""
         if page_tokens not in ops._PAGE_TOKENS:
             raise ValueError(f"pages of 16, 32, 64 or 128 tokens, got {page_tokens}")
         if head_dim not in (64, 128):
@@ -68,6 +68,10 @@ class PagedKV8Cache:
         ops.page_plan(lengths, counts, self.table, self.free_pages, self.state, self.page_tokens, self.q_start, self.kv_len, pos, seq, slots, self.state_out)
         return PagedStep(self.q_start, self.kv_len, pos, slots, seq, max_tokens or max(tokens, 1))
 
+    def short(self) -> int:
+        """Requests that the last plan refuses pages. Reads the device. A plan that is not committed costs nothing."""
+        return int(self.state_out[-1].item())
+
     def commit(self) -> None:
         self.state.copy_(self.state_out[:-1])
         self.refusals.add_(self.state_out[-1])
@@ -90,7 +94,7 @@ class PagedKV8Cache:
         return k, v
 
     def refused(self) -> int:
-        """Requests that committed steps have refused pages so far: their tokens of that step are in no page. Reads the device."""
+        """Requests that committed steps have refused pages, since the cache was made or `refusals` was set to zero: their tokens of that step are in no page. Reads the device."""
         return int(self.refusals.item())
 
     def free(self) -> int:

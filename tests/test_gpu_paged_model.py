@@ -201,3 +201,27 @@ def test_what_the_model_and_the_engine_refuse():
     for t in (-1.0, math.nan):
         with pytest.raises(ValueError, match="temperature"):
             QSpecEngine(model, 2, 3, temperature=t)
+
+
+def test_a_step_that_found_no_pages_is_made_again_once_there_are_some():
+    """What is refused costs nothing: neither pages nor what the other sequences hold, nor the steps behind it."""
+    texts = [list(range(40)), list(range(100, 140)), list(range(200, 220))]
+    logits = {}
+    for pages in (None, 5):
+        model = QSpecLlamaModel(config(kv_cache="int8", kv_page=16, kv_pages=pages), max_batch=3, max_tokens=64, seed=8)
+        s = Scheduler(model)
+        got = [s.feed([("a", texts[0], [39])]), s.feed([("c", texts[2], [19])])]     # three pages, two pages
+        if pages:
+            for _ in range(2):
+                with pytest.raises(RuntimeError, match="full"):
+                    s.feed([("b", texts[1], [39])])
+                assert model.paged.free() == 0 and model.paged.state.tolist() == [3, 2, 0, 0]
+        got.append(s.feed([("c", [7, 8], [1])]))              # a step that needs no page
+        if pages:
+            with pytest.raises(RuntimeError, match="full"):
+                s.feed([("c", list(range(20)), [19]), ("a", [5], [0])])
+        s.release("a")
+        got += [s.feed([("b", texts[1], [39])]), s.feed([("c", [9], [0]), ("b", [3, 4], [1])])]
+        logits[pages] = torch.cat(got)
+        assert model.paged.refused() == 0
+    assert torch.equal(logits[None], logits[5])
