@@ -110,7 +110,9 @@ class Scheduler:
         return out
 
     def release(self, rid: Hashable) -> None:
-        """The request is finished: its slot returns to the pool."""
+        """The request is finished, or given up: its slot returns to the pool, and `step` goes on without it."""
+        self.waiting = deque(r for r in self.waiting if r.rid != rid)
+        self.running = [r for r in self.running if r.rid != rid]
         if rid in self.table.slot_of:
             slot = self.table.slot_of[rid]
             self.table.close(rid)
@@ -164,7 +166,6 @@ class Scheduler:
             if len(r.output) >= r.max_new_tokens or (r.eos is not None and t == r.eos):
                 r.done = True
         for r in [r for r in self.running if r.done]:
-            self.running.remove(r)
             self.release(r.rid)
             self.finished[r.rid] = r
         return sampled
