@@ -133,9 +133,10 @@ class Scheduler:
 
     def step(self) -> List[Tuple[Hashable, int]]:
         """One scheduling step: every running request that is decoding gets its last token, then prompts are advanced
-        while token budget and slots remain. Returns the (request id, token) pairs sampled in this step."""
+        while token budget and slots remain. Returns the (request id, token) pairs sampled in this step. A step that the model
+        refuses (RuntimeError: a pool of pages that is full) leaves the requests where they were, and can be made again."""
         budget = self.model.max_step_tokens
-        entries, owners = [], []
+        entries, owners, portions = [], [], []
         for r in self.running:
             if r.fed == len(r.prompt) and budget > 0:
                 entries.append((r.rid, [r.output[-1]], [0]))
@@ -150,13 +151,15 @@ class Scheduler:
                 n = min(len(r.prompt) - r.fed, self.prefill_portion, budget)
                 last = r.fed + n == len(r.prompt)
                 entries.append((r.rid, r.prompt[r.fed:r.fed + n], [n - 1] if last else []))
-                r.fed += n
+                portions.append((r, n))
                 budget -= n
                 if last:
                     owners.append(r)
         if not entries:
             return []
         logits = self.feed(entries)
+        for r, n in portions:
+            r.fed += n
         self.steps += 1
         toks = ops.argmax_rows(logits).tolist() if logits.shape[0] else []
         sampled = []

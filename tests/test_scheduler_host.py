@@ -1,4 +1,4 @@
-"""The scheduler's bookkeeping over a model that keeps its tokens on the host."""
+"""The scheduler's bookkeeping where a model refuses a step, over a model that keeps its tokens on the host."""
 import types
 
 import pytest
@@ -46,12 +46,30 @@ def host_arg_max(monkeypatch):
 PROMPTS = [list(range(1, 30)), [5, 6, 7], list(range(3, 24))]
 
 
+@pytest.mark.parametrize("refuse", [{0}, {1}, {2, 3}, {0, 4, 6, 7}])
+def test_a_refused_step_can_be_made_again(refuse):
+    want = Scheduler(Counting()).generate(PROMPTS, 4)
+    model = Counting(refuse)
+    s = Scheduler(model, prefill_portion=9)
+    for i, p in enumerate(PROMPTS):
+        s.add(i, p, 4)
+    refusals = 0
+    while s.has_work():
+        try:
+            s.step()
+        except RuntimeError:
+            refusals += 1
+    assert refusals == len(refuse) and [s.finished[i].output for i in range(3)] == want
+
+
 def test_a_request_that_is_given_up_is_not_fed_again():
-    model = Counting()
+    model = Counting({1})
     s = Scheduler(model, prefill_portion=9)
     for i, p in enumerate(PROMPTS):
         s.add(i, p, 4)
     s.step()
+    with pytest.raises(RuntimeError):
+        s.step()
     s.release(0)                                              # one that runs, its prompt half in
     s.release(2)                                              # one that waits
     assert [r.rid for r in s.running] == [1] and not s.waiting and s.table.pool.free == 1
