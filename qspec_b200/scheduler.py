@@ -42,6 +42,10 @@ class Scheduler:
     def __init__(self, model, prefill_portion: Optional[int] = None):
         self.model = model
         self.table = SequenceTable(model.n_slots, model.device, model.max_step_tokens)
+        self._release_slot = getattr(model, "release_slot", None)      # of a model whose slots hold pages
+        if self._release_slot is not None:
+            for slot in range(model.n_slots):                          # (what the requests of a scheduler before this one were left with)
+                self._release_slot(slot)
         self.prefill_portion = min(prefill_portion or model.max_step_tokens, model.max_step_tokens)
         self.waiting: Deque[Request] = deque()
         self.running: List[Request] = []
@@ -116,9 +120,8 @@ class Scheduler:
         if rid in self.table.slot_of:
             slot = self.table.slot_of[rid]
             self.table.close(rid)
-            release = getattr(self.model, "release_slot", None)        # a model whose slots hold pages takes them back
-            if release is not None:
-                release(slot)
+            if self._release_slot is not None:
+                self._release_slot(slot)
 
     # ---- generation -------------------------------------------------------------------------------------------------
     def add(self, rid: Hashable, prompt: Sequence[int], max_new_tokens: int, eos: Optional[int] = None) -> None:

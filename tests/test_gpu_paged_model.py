@@ -225,3 +225,11 @@ def test_a_step_that_found_no_pages_is_made_again_once_there_are_some():
         logits[pages] = torch.cat(got)
         assert model.paged.refused() == 0
     assert torch.equal(logits[None], logits[5])
+
+
+def test_pages_of_requests_that_an_earlier_scheduler_left_come_back():
+    model = QSpecLlamaModel(config(kv_cache="int8", kv_page=16, kv_pages=4), max_batch=3, max_tokens=64, seed=8)
+    left = Scheduler(model)
+    left.feed([("a", list(range(10)), []), ("b", list(range(10)), []), ("c", list(range(10)), [])])   # three of the four pages
+    want = Scheduler(QSpecLlamaModel(config(kv_cache="int8", kv_page=16), max_batch=3, max_tokens=64, seed=8)).generate([list(range(50))], 6)
+    assert Scheduler(model).generate([list(range(50))], 6) == want

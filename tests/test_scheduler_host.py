@@ -77,3 +77,13 @@ def test_a_request_that_is_given_up_is_not_fed_again():
         s.step()
     assert list(s.finished) == [1] and s.finished[1].output == Scheduler(Counting()).generate(PROMPTS[1:2], 4)[0]
     assert len(model.released) >= 2
+
+
+def test_a_new_scheduler_takes_every_slot_back():
+    model = Counting()
+    first = Scheduler(model)
+    first.add("left", PROMPTS[0], 4)
+    first.step()
+    model.released.clear()
+    Scheduler(model)
+    assert sorted(model.released) == [0, 1]
