@@ -25,7 +25,10 @@ class QSpecEngine:
     def __init__(self, model: QSpecLlamaModel, batch: int, k: int = 3, use_cuda_graph: bool = True, temperature: float = 0.0, seed: int = 0):
         """temperature 0: greedy, a draft token is accepted iff it is the target's arg max. Above 0: tokens are drawn from softmax(logits / temperature) and draft
         tokens accepted with probability min(1, p / q), so that what is emitted is distributed as the target's own (vllm/model_executor/layers/
-        rejection_sampler.py); `seed` decides the random numbers."""
+        rejection_sampler.py); `seed` decides the random numbers.
+
+        Over a paged cache with fewer pages than all sequences may need, a step may find none for some of them: these emit nothing (out_count 0) and stay where they
+        are. `step` raises for that at its first call behind a `prefill` and at every 64th, `metrics` at once; the next `prefill` begins with all pages."""
         self.model, self.B, self.k = model, batch, k
         if not temperature >= 0.0:
             raise ValueError(f"temperature must be 0 (greedy) or positive, got {temperature}")
@@ -82,6 +85,8 @@ class QSpecEngine:
         if self.paged is not None:                                          # the sequences of before give their pages back
             self.paged.plan(torch.zeros_like(self.seq_len), torch.full_like(self.seq_len, -1), 0)
             self.paged.commit()
+            self.paged.refusals.zero_()
+            self._steps = 0                                                 # (the first step behind this looks whether the prompts found pages)
             held = torch.zeros_like(self.seq_len)
         chunk = max(1, m.max_tokens)
         last_hidden = torch.empty(B, m.cfg.hidden_size, dtype=torch.float16, device=m.device)
@@ -163,13 +168,22 @@ class QSpecEngine:
             emitted = torch.where(idx < n_acc.unsqueeze(1), padded, torch.where(idx == n_acc.unsqueeze(1), nxt.unsqueeze(1), -1))
             self.out_tokens.copy_(emitted)
             self.out_count.copy_(n_acc + 1)
+        if vstep is not None:
+            # a sequence that found no pages has seen nothing: it emits nothing and stays where it is, so that its step can be made again
+            served = vstep.kv_len > 0
+            nxt = torch.where(served, nxt, self.cur_tok)
+            n_acc = n_acc * served
+            emitted = emitted.masked_fill(~served.unsqueeze(1), -1)
+            self.out_tokens.copy_(emitted)
+            self.out_count.mul_(served)
+        count = self.out_count
         self.cur_tok.copy_(nxt)
-        self.seq_len.add_((n_acc + 1).to(torch.int32))
+        self.seq_len.add_(count.to(torch.int32))
         self.counters[0] += n_acc.sum()
         self.counters[1] += B * k
-        self.counters[2] += (n_acc + 1).sum()
+        self.counters[2] += count.sum()
         self.d_out_pack[:, : k + 1].copy_(emitted)
-        self.d_out_pack[:, k + 1].copy_(n_acc + 1)
+        self.d_out_pack[:, k + 1].copy_(count)
 
     def capture(self) -> None:
         """Warm up once eagerly (sets kernel attributes, sizes workspaces), then capture."""
@@ -226,8 +240,8 @@ class QSpecEngine:
 
     def _check_pages(self) -> None:
         if refused := self.paged.refused():
-            raise RuntimeError(f"the 8-bit cache had no page for {refused} sequence(s) of a step: their tokens of that step are lost "
-                               f"({self.paged.pages} pages of {self.paged.page_tokens} tokens)")
+            raise RuntimeError(f"the 8-bit cache had no page {refused} time(s) for a sequence of a step, which then emitted nothing, or for a portion of a prompt, which is not in "
+                               f"it ({self.paged.pages} pages of {self.paged.page_tokens} tokens)")
 
     def _join_caller_stream(self) -> None:
         """self.stream is a non-blocking stream: work the caller queued on ITS stream (prefill, state edits) is ordered before

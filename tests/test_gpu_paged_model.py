@@ -233,3 +233,59 @@ def test_pages_of_requests_that_an_earlier_scheduler_left_come_back():
     left.feed([("a", list(range(10)), []), ("b", list(range(10)), []), ("c", list(range(10)), [])])   # three of the four pages
     want = Scheduler(QSpecLlamaModel(config(kv_cache="int8", kv_page=16), max_batch=3, max_tokens=64, seed=8)).generate([list(range(50))], 6)
     assert Scheduler(model).generate([list(range(50))], 6) == want
+
+
+@pytest.mark.parametrize("temperature", [0.0, 0.9])
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_sequence_without_a_page_emits_nothing_and_stays_where_it_is(graph, temperature):
+    """Three pages: after a step that needs two more, the second sequence has no place for its tokens. Once there is one it goes on; a new prefill begins with all pages."""
+    B, k, P = 2, 3, 14
+    model = QSpecLlamaModel(config(kv_cache="int8", kv_page=16, kv_pages=3), max_batch=B, max_tokens=32, seed=8)
+    engine = QSpecEngine(model, B, k, use_cuda_graph=graph, temperature=temperature)
+    prompts = torch.arange(B * P, device="cuda").view(B, P)
+    engine.prefill(prompts)
+    token = engine.cur_tok.tolist()
+    before = [t.clone() for t in model.paged.read(0, 1, P)]
+    for _ in range(3):
+        engine.step()
+        engine.stream.synchronize()
+        assert engine.out_count[0] >= 1 and engine.out_count[1] == 0 and engine.out_tokens[1].tolist() == [-1] * (k + 1)
+        assert engine.seq_len[1] == P and engine.cur_tok[1] == token[1] and engine.d_out_pack[1].tolist() == [-1] * (k + 1) + [0]
+        if engine.seq_len[0] > 27:
+            break
+    assert model.paged.state.tolist() == [2, 1, 0]
+    with pytest.raises(RuntimeError, match="no page"):
+        engine.metrics()
+    assert all(torch.equal(a, b) for a, b in zip(before, model.paged.read(0, 1, P)))
+    # the first sequence ends: its pages are there for the second
+    model.paged.plan(engine.seq_len, torch.tensor([-1, 0], dtype=torch.int32, device="cuda"), 0)
+    model.paged.commit()
+    engine.seq_len[0] = 0
+    engine.step()
+    engine.stream.synchronize()
+    assert engine.out_count[1] >= 1 and engine.seq_len[1] == P + engine.out_count[1]
+    # a new prefill, with room enough
+    for e in (engine, QSpecEngine(QSpecLlamaModel(config(kv_cache="int8", kv_page=16), max_batch=B, max_tokens=32, seed=8), B, k, use_cuda_graph=graph, temperature=temperature)):
+        if temperature:
+            e.generator.manual_seed(3)
+        e.prefill(prompts[:, :6])
+        e.step()
+        e.stream.synchronize()
+        assert e.metrics()["emitted_tokens"] == int(e.out_count.sum())
+        if e is engine:
+            kept = e.out_tokens.clone()
+    assert torch.equal(kept, e.out_tokens)
+
+
+def test_a_prompt_without_pages_is_reported_by_the_next_step_whatever_came_before():
+    model = QSpecLlamaModel(config(kv_cache="int8", kv_page=16, kv_pages=3), max_batch=2, max_tokens=64, seed=8)
+    engine = QSpecEngine(model, 2, 3, use_cuda_graph=False)
+    engine.prefill(torch.arange(8, device="cuda").view(2, 4))
+    engine.step()
+    engine.prefill(torch.arange(80, device="cuda").view(2, 40))
+    with pytest.raises(RuntimeError, match="no page"):
+        engine.step()
+    engine.prefill(torch.arange(8, device="cuda").view(2, 4))
+    engine.step()
+    engine.stream.synchronize()
+    assert engine.out_count.min() >= 1 and engine.metrics()["draft_tokens"] == 6
