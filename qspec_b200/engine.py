@@ -79,6 +79,7 @@ class QSpecEngine:
         """prompt_ids [B, P] (device int64). Verify-mode (W4A16) pass, as the reference's
         _run_no_spec prefill (spec_decode_worker.py:666-720); fills the KV cache."""
         m = self.model
+        self._behind_steps()
         B, P = prompt_ids.shape
         assert B == self.B and P + 1 < m.cfg.max_seq_len
         pos = torch.arange(P, dtype=torch.int32, device=m.device)
@@ -221,6 +222,7 @@ class QSpecEngine:
 
     def sync_lengths(self) -> int:
         """Reads the true max(seq_len) back (one small D2H copy + sync) and tightens the host-side bound to it."""
+        self._behind_steps()
         self._len_bound = int(self.seq_len.max().item())
         return self._len_bound
 
@@ -239,9 +241,16 @@ class QSpecEngine:
                                "(a rank of the group is gone); the partial sums of those steps are stale")
 
     def _check_pages(self) -> None:
+        self._behind_steps()
         if refused := self.paged.refused():
             raise RuntimeError(f"the 8-bit cache had no page {refused} time(s) for a sequence of a step, which then emitted nothing, or for a portion of a prompt, which is not in "
                                f"it ({self.paged.pages} pages of {self.paged.page_tokens} tokens)")
+
+    def _behind_steps(self) -> None:
+        """What the caller's stream does from here on comes after the steps that are queued on self.stream."""
+        cur = torch.cuda.current_stream(self.model.device)
+        if cur != self.stream:
+            cur.wait_stream(self.stream)
 
     def _join_caller_stream(self) -> None:
         """self.stream is a non-blocking stream: work the caller queued on ITS stream (prefill, state edits) is ordered before
@@ -283,6 +292,8 @@ class QSpecEngine:
 
     # ---------------------------------------------------------------------------------------
     def metrics(self) -> dict:
+        if self.counters.is_cuda:
+            self._behind_steps()
         peers = getattr(self.model, "peers", None)
         if peers is not None and peers.timeouts():
             raise RuntimeError(f"tensor-parallel peer time-out: {peers.timeouts()} arrival flag(s) never came")

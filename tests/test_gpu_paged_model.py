@@ -289,3 +289,39 @@ def test_a_prompt_without_pages_is_reported_by_the_next_step_whatever_came_befor
     engine.step()
     engine.stream.synchronize()
     assert engine.out_count.min() >= 1 and engine.metrics()["draft_tokens"] == 6
+
+
+@pytest.mark.parametrize("kv_cache", ["f16", "int8"])
+def test_what_is_read_back_is_behind_the_steps_that_are_queued(kv_cache):
+    """Lengths, refusals and counters are read, and a new prefill is begun, while a step has yet to run (the engine's stream is kept busy for some tenths of a second)."""
+    kw = dict(kv_cache="int8", kv_page=16, kv_pages=3) if kv_cache == "int8" else {}
+    model = QSpecLlamaModel(config(**kw), max_batch=2, max_tokens=32, seed=8)
+    engine = QSpecEngine(model, 2, 3)
+    prompts = torch.arange(28, device="cuda").view(2, 14)
+
+    def late_step():
+        with torch.cuda.stream(engine.stream):
+            torch.cuda._sleep(400_000_000)
+        engine.step()
+
+    engine.prefill(prompts[:, :5])
+    engine.step()
+    engine.stream.synchronize()
+    before = engine.seq_len.max().item()
+    late_step()
+    assert engine.sync_lengths() > before and engine.sync_lengths() == engine.seq_len.max().item()
+    late_step()
+    steps = engine.metrics()["draft_tokens"]
+    assert steps == 3 * 2 * 3
+    late_step()
+    engine.prefill(prompts)                                   # behind that step, whose lengths and pages are not the new sequences'
+    engine.stream.synchronize()
+    torch.cuda.synchronize()
+    assert engine.seq_len.tolist() == [14, 14]
+    if kv_cache == "int8":
+        assert model.paged.state.tolist() == [1, 1, 1] and model.paged.refused() == 0
+        engine._steps = 1
+        late_step()                                           # a page for one of the two
+        engine._steps = 64
+        with pytest.raises(RuntimeError, match="no page"):
+            engine.step()
