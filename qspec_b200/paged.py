@@ -87,8 +87,8 @@ class PagedKV8Cache:
     def read(self, layer: int, request: int, tokens: int, dtype=torch.float16):
         """Keys and values [tokens, kv heads, head dim] of a request's first tokens, in 16 bits (to check a cache, or to move a sequence out of it)."""
         most = self.table.shape[1] * self.page_tokens
-        if not 0 <= tokens <= most or not 0 <= request < self.requests or not 0 <= layer < len(self.k):
-            raise ValueError(f"read: layer {layer} of {len(self.k)}, request {request} of {self.requests}, {tokens} tokens of {most} at most")
+        if not 0 <= tokens <= most:
+            raise ValueError(f"read: {tokens} tokens of a request, whose row of the table has pages for {most}")
         at = torch.arange(tokens, dtype=torch.int32, device=self.device)
         slots = (self.table[request].index_select(0, at // self.page_tokens) * self.page_tokens + at % self.page_tokens).to(torch.int32)
         shape = (tokens, self.k.shape[2], self.k.shape[4])
