@@ -426,7 +426,7 @@ int qspec_debug_kv8_attention_give_up(const void* q, long long q_tok_stride, int
  * many drafts a request has. Draft i is taken if uniform[b, i] * q_i(d_i) < p_i(d_i) (exactly) and all before it were. Then one token by inversion with
  * uniform[b, drafts]: from max(p - q, 0) at the first place refused; from p at the place behind the drafts where all were taken, or where that difference
  * is zero everywhere: the first token whose running sum (64 bits) is above uniform * total. tokens int64 [requests, drafts + 1]: what is emitted, -1 behind it;
- * emitted int64 [requests]: how many. A row of p without any mass gives token 0; a drafted token outside the vocabulary is refused. */
+ * emitted int64 [requests]: how many; neither may lie over anything else of the call. A row of p without any mass gives token 0; a drafted token outside the vocabulary is refused. */
 int qspec_verify_drafts_max_drafts(void);
 int qspec_verify_drafts(const long long* drafted, const float* draft, long long draft_seq_stride, long long draft_place_stride, const float* target,
                         long long target_seq_stride, long long target_place_stride, const float* uniform, const int* draft_counts, long long* tokens,

@@ -254,11 +254,14 @@ PyObject* verify_drafts(PyObject* const* a, Py_ssize_t n) {
   QSPEC_NOT_HERE(B < 1 || V < 1 || !fits(B) || !fits(k) || !fits(V) || !is(u, at::kFloat, {B, k + 1}) || !is(tokens, at::kLong, {B, k + 1}) || !is(emitted, at::kLong, {B}));
   if (k) {
     d = on_device(a[1], device), q = on_device(a[2], device);
-    QSPEC_NOT_HERE(!q || !is(d, at::kLong, {B, k}) || q->scalar_type() != at::kFloat || q->sizes() != at::IntArrayRef({B, k, V}) || q->stride(2) != 1 || overlap(*tokens, *d));
+    QSPEC_NOT_HERE(!q || !is(d, at::kLong, {B, k}) || q->scalar_type() != at::kFloat || q->sizes() != at::IntArrayRef({B, k, V}) || q->stride(2) != 1);
   } else {
     QSPEC_NOT_HERE(a[1] != Py_None || a[2] != Py_None);
   }
   if (a[7] != Py_None) QSPEC_NOT_HERE(!(counts = on_device(a[7], device)) || !is(counts, at::kInt, {B}));
+  for (const at::Tensor* out : {tokens, emitted})
+    for (const at::Tensor* t : {d, u, counts}) QSPEC_NOT_HERE(t && overlap(*out, *t));
+  QSPEC_NOT_HERE(overlap(*tokens, *emitted));
   const auto fn = (decltype(&qspec_verify_drafts))PyLong_AsVoidPtr(a[0]);
   if (PyErr_Occurred()) return nullptr;
   QSPEC_NOT_HERE(!fn);

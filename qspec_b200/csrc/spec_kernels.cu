@@ -44,7 +44,7 @@ __device__ __forceinline__ double warp_before(double v, int lane) {
   const double w = __shfl_up_sync(0xffffffffu, incl, 1);
   return lane ? w : 0.0;
 }
-// What is left to draw from. A probability that is no number counts as none.
+// What is left to draw from. A token one of whose two probabilities is no number has nothing.
 __device__ __forceinline__ double rest_of(float p, float q) {
   return p > q ? (double)p - (double)q : 0.0;
 }

@@ -987,8 +987,8 @@ def verify_drafts(drafted: Optional[torch.Tensor], draft_probs: Optional[torch.T
     if B == 0:
         return
     _here(target_probs, drafted, draft_probs, uniform, tokens, emitted, draft_counts)
-    if k and _overlap(tokens, drafted):
-        raise ValueError("verify_drafts: tokens must not lie over drafted")
+    if any(t is not None and _overlap(out, t) for out in (tokens, emitted) for t in (drafted, uniform, draft_counts)) or _overlap(tokens, emitted):
+        raise ValueError("verify_drafts: tokens and emitted must not lie over each other, nor over drafted, uniform and draft_counts")
     lib = _lib.load()
     _lib.check(lib.qspec_verify_drafts(_ptr(drafted), _ptr(draft_probs), draft_probs.stride(0) if k else 0, draft_probs.stride(1) if k else 0, _ptr(target_probs),
                                        target_probs.stride(0), target_probs.stride(1), _ptr(uniform), _ptr(draft_counts), _ptr(tokens), _ptr(emitted), B, k, V, _stream()),

@@ -198,3 +198,20 @@ def test_wrong_shapes_types_and_overlaps_are_refused():
         ops.verify_drafts(*args, draft_counts=torch.zeros(3, dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError):
         ops.sample_probs(target[:, 0], uniform[:, 0], emitted)   # (random numbers with a stride)
+
+
+def test_results_over_other_tensors_of_the_call_are_refused():
+    drafted, draft, target, uniform = make(1, 4, 2, 50)
+    counts = torch.full((4,), 2, dtype=torch.int32, device="cuda")
+    z = lambda n, dtype=I64: torch.zeros(n, dtype=dtype, device="cuda")  # noqa: E731
+    args = dict(drafted=drafted, draft_probs=draft, target_probs=target, uniform=uniform, tokens=z(12).view(4, 3), emitted=z(4), draft_counts=counts)
+    ops.verify_drafts(**args)
+    big = z(40)
+    for bad in (dict(tokens=big[:12].view(4, 3), emitted=big[11:15]), dict(emitted=big[:4], drafted=big[3:11].view(4, 2)), dict(tokens=big[4:16].view(4, 3), drafted=big[:8].view(4, 2)),
+                dict(emitted=big[:4], uniform=big.view(torch.float32)[7:19].view(4, 3)), dict(tokens=big[:12].view(4, 3), draft_counts=big.view(torch.int32)[20:24])):
+        with pytest.raises(ValueError, match="must not lie over"):
+            ops.verify_drafts(**{**args, **bad})
+    side = dict(tokens=big[:12].view(4, 3), emitted=big[12:16], drafted=big[16:24].view(4, 2))
+    side["drafted"].copy_(drafted)
+    ops.verify_drafts(**{**args, **side})
+    assert torch.equal(side["tokens"], args["tokens"]) and torch.equal(side["emitted"], args["emitted"])
