@@ -685,6 +685,7 @@ static int attention(const void* q, long long q_tok_stride, int q_head_stride, c
   QSPEC_REQUIRE(D == 64 || D == 128, QSPEC_ERR_UNSUPPORTED, "kv8_attention: heads of 64 or 128, got %d", D);
   QSPEC_REQUIRE(dtype == QSPEC_DTYPE_F16 || dtype == QSPEC_DTYPE_BF16, QSPEC_ERR_UNSUPPORTED, "kv8_attention: float16 or bfloat16 queries");
   QSPEC_REQUIRE(G >= 1 && H >= G && H % G == 0 && H <= 4096, QSPEC_ERR_INVALID_ARG, "kv8_attention: %d query heads, %d key/value heads", H, G);
+  QSPEC_REQUIRE(scale > 0.f && scale < INFINITY, QSPEC_ERR_INVALID_ARG, "kv8_attention: scale must be positive and finite, got %g", (double)scale);
   QSPEC_REQUIRE(ntok >= 0 && ntok < (1 << 24) && requests >= 1 && width >= 1 && npages >= 1 && max_tokens >= 1 && (long long)npages * page_tokens < (1ll << 31) &&
                     (long long)width * page_tokens < (1ll << 31),
                 QSPEC_ERR_INVALID_ARG, "kv8_attention: tokens=%d requests=%d width=%d pages=%d", ntok, requests, width, npages);

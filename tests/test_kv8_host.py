@@ -1,5 +1,7 @@
 """Refusals of the paged 8-bit cache's entry points and of the draft verification, which need no GPU: the C entries look at their arguments before they
 touch the device, and the Python functions at their tensors before that."""
+import math
+
 import pytest
 import torch
 
@@ -105,3 +107,9 @@ def test_python_functions_refuse_tensors_that_are_not_on_a_gpu():
         ops.verify_drafts(None, None, z(2, 1, 10), z(2, 1), z(2, 1, dtype=torch.int64), z(2, dtype=torch.int64))
     with pytest.raises(ValueError, match="rows"):
         ops.sample_probs(z(2, 10), z(3), z(2, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, math.inf, math.nan, 1e-60])
+def test_attention_refuses_a_scale_that_is_none(lib, scale):
+    assert lib.qspec_kv8_attention(P, 1024, 128, P, P, P, P, P, P, P, P, 1024, 128, 3, 2, 4, 8, 2, 128, 9, 64, 2, scale, 0, P, 1 << 30, None) == 1
+    assert "scale must be" in lib.qspec_last_error().decode()
