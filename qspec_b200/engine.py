@@ -32,6 +32,8 @@ class QSpecEngine:
         self.model, self.B, self.k = model, batch, k
         if not temperature >= 0.0:
             raise ValueError(f"temperature must be 0 (greedy) or positive, got {temperature}")
+        if 0.0 < temperature < 1e-33:                                 # (float16 logits, up to 65504, divided by it: beyond float32, and the probabilities no numbers)
+            raise ValueError(f"temperature must be 0 (greedy) or at least 1e-33, got {temperature}")
         if temperature and model.tp_size != 1:
             raise NotImplementedError("sampling with a vocab-sharded lm_head")
         self.temperature = float(temperature)

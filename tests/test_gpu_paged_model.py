@@ -336,3 +336,18 @@ def test_reading_more_of_a_request_than_it_can_hold_is_refused_on_the_host():
         k, v = cache.read(-1, 2, tokens)
         assert k.shape == v.shape == (tokens, 2, 64)
     torch.cuda.synchronize()
+
+
+def test_temperatures_next_to_zero():
+    model = QSpecLlamaModel(config(), max_batch=2, max_tokens=8, seed=6)
+    for t in (1e-34, 5e-324):
+        with pytest.raises(ValueError, match="temperature"):
+            QSpecEngine(model, 2, 3, temperature=t)
+    tokens = []
+    for t in (0.0, 1e-33, 1e30):
+        engine = QSpecEngine(model, 2, 3, use_cuda_graph=False, temperature=t)
+        engine.prefill(torch.arange(12, device="cuda").view(2, 6))
+        engine.step()
+        engine.stream.synchronize()
+        tokens.append([engine.cur_tok.tolist(), engine.out_tokens.tolist()])
+    assert tokens[0] == tokens[1] and tokens[2] != tokens[0]
