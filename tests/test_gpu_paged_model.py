@@ -351,3 +351,19 @@ def test_temperatures_next_to_zero():
         engine.stream.synchronize()
         tokens.append([engine.cur_tok.tolist(), engine.out_tokens.tolist()])
     assert tokens[0] == tokens[1] and tokens[2] != tokens[0]
+
+
+@pytest.mark.parametrize("kv_cache", ["f16", "int8"])
+@pytest.mark.parametrize("temperature", [0.0, 1e-4])
+def test_an_engine_without_drafts_decodes_token_by_token(kv_cache, temperature):
+    model = QSpecLlamaModel(config(kv_cache=kv_cache, kv_page=16), max_batch=2, max_tokens=8, seed=6)
+    engine = QSpecEngine(model, 2, 0, temperature=temperature)
+    engine.prefill(torch.arange(12, device="cuda").view(2, 6))
+    got = [engine.cur_tok.tolist()]
+    for _ in range(4):
+        engine.step()
+        engine.stream.synchronize()
+        assert engine.out_count.tolist() == [1, 1]
+        got.append(engine.out_tokens[:, 0].tolist())
+    want = Scheduler(QSpecLlamaModel(config(kv_cache=kv_cache, kv_page=16), max_batch=2, max_tokens=8, seed=6)).generate([list(range(6)), list(range(6, 12))], 5)
+    assert [list(t) for t in zip(*got)] == want
