@@ -431,14 +431,14 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
       fetch<D, false>(a, unit, kbuf, lane);
       copy_commit();
       // ---- weights
-      // Keys that a row does not see; and of a page that there is not, or whose scale is no number, what makes the rows NaN that do see it.
-      const bool odd = __any_sync(0xffffffffu, cks != cks || cvs != cvs);
+      // Keys that a row does not see; and of a page that there is not, or whose scale is infinite or no number, what makes the rows NaN that do see it.
+      const float both = cks + cvs;
+      const bool odd = __any_sync(0xffffffffu, !(both < INFINITY));
       if (key0 + UNIT - 1 > low || odd) {
 #pragma unroll
         for (int nt = 0; nt < KT; ++nt) {
           const int src = (16 * (nt >> 1)) >> a.pshift;
-          const float both = __shfl_sync(0xffffffffu, cks + cvs, src);
-          const bool none = both != both;
+          const bool none = !(__shfl_sync(0xffffffffu, both, src) < INFINITY);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if (none) s[nt][e] = NAN;
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
         const int src = (16 * q) >> a.pshift;
-        const float f = positive(__shfl_sync(0xffffffffu, cks, src)), v = positive(__shfl_sync(0xffffffffu, cvs, src));
+        const float f = positive(__shfl_sync(0xffffffffu, cks, src)), v = fminf(positive(__shfl_sync(0xffffffffu, cvs, src)), 8.507059e37f);   // (not infinite: beside a hidden key's minus infinity that would be no number)
         lv[q] = __log2f(v);
         iv[q] = __fdividef(WEIGHT_UNIT, v);
 #pragma unroll
@@ -478,21 +478,21 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         if (grown[e]) m[e] = mx[e];                         // (a row that had seen nothing has sums of zero)
-      const float ref[2] = {m[0] == NONE ? 0.f : m[0], m[1] == NONE ? 0.f : m[1]};
+      const float ref[2] = {m[0] == NONE ? 0.f : m[0] - WEIGHT_LOG2, m[1] == NONE ? 0.f : m[1] - WEIGHT_LOG2};
       // Exponents are taken from the products without a rounding in between, the reference has one: far from zero that alone would be a large exponent.
       const bool far = __any_sync(0xffffffffu, fabsf(ref[0]) > FAR || fabsf(ref[1]) > FAR);
       if (far) {
 #pragma unroll
         for (int nt = 0; nt < KT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] = fmaf(s[nt][e], kf[nt >> 1][e >> 1], lv[nt >> 1]) - ref[e >> 1];
+          for (int e = 0; e < 4; ++e) s[nt][e] = fmaf(s[nt][e], kf[nt >> 1][e >> 1], lv[nt >> 1]) - (m[e >> 1] == NONE ? 0.f : m[e >> 1]);
 #pragma unroll
         for (int q = 0; q < QT; ++q) kf[q][0] = kf[q][1] = 1.f;
       }
       uint32_t pa[QT][4];
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
-        const float base = lv[q] + WEIGHT_LOG2, at[2] = {far ? WEIGHT_LOG2 : base - ref[0], far ? WEIGHT_LOG2 : base - ref[1]};
+        const float at[2] = {far ? WEIGHT_LOG2 : lv[q] - ref[0], far ? WEIGHT_LOG2 : lv[q] - ref[1]};
         float part[2] = {0.f, 0.f};
 #pragma unroll
         for (int z = 0; z < 2; ++z) {

@@ -27,6 +27,8 @@ __device__ __forceinline__ float positive(float x) { return x >= 7.8886090522101
 // 112 us, 2^6 114, 2^5 115, 2^4 117. 2^16 is infinite, and a reference has a rounding of its own: beyond FAR it is subtracted from the finished exponent, which was rounded
 // like it. Sums of weights / v are kept in units of 2^WEIGHT_LOG2, so that they hold for every scale that positive() leaves.
 constexpr float WEIGHT_LOG2 = 9.f, GROWTH_LOG2 = 6.f, WEIGHT_UNIT = 1.f / 512.f, FAR = 1048576.f;
+// An infinite one is no number either: beside a hidden key's minus infinity it would be one in rows that do not see the page.
+__device__ __forceinline__ float finite_scale(float x) { return x < INFINITY ? x : NAN; }
 // What scores in units of 2^-24 are multiplied with, from the scale of the keys and the row's factor: these two first, since either may be as far from 1 as float32 goes and
 // the other as far on the other side. Not so small that it would make a hidden key's score (minus infinity) no number.
 __device__ __forceinline__ float score_factor(float scale, float row) { return fmaxf(scale * row * 16777216.f, 1.17549435e-38f); }

@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         if (!bad) {
           const size_t block = (size_t)page * a.G + g;
           codes = (long long)(((block << a.pshift) + (key & ((1 << a.pshift) - 1))) * D);
-          k = a.ks[block];
-          v = a.vs[block];
+          k = finite_scale(a.ks[block]);
+          v = finite_scale(a.vs[block]);
           bad = k != k || v != v;
         }
       }

@@ -773,3 +773,22 @@ def test_append_leaves_out_tokens_without_a_position_in_the_middle_of_a_page(run
             c[page][:, row] = (y[some] * after.reciprocal()[None, :, None]).round().clamp(-127, 127).to(torch.int8).transpose(0, 1)
             s[page] = after
         assert torch.equal(got_s, s) and torch.equal(got_c, c)
+
+
+@pytest.mark.parametrize("form", ["rows", "prompt", "pairs"])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("side", ["keys", "values"])
+def test_attention_shows_a_scale_that_is_no_number_and_only_where_it_is_seen(side, value, form, monkeypatch):
+    if form != "rows":
+        monkeypatch.setattr(ops, "kv8_attention", lambda *args, **kw: prompt_form(*args, pairs=form == "pairs", **kw))
+    q, k, v, ks, vs, table, start, lens = make_attention(20, [200, 333], [60, 40], 8, 2, 128, 32, torch.float16)
+    clean = check_attention((q, k, v, ks, vs, table, start, lens), 128)
+    for page in (int(table[0, 5]), int(table[1, 9])):         # positions 160 .. 191 and 288 .. 319 of one head
+        (ks if side == "keys" else vs)[page, 1] = value
+    out = torch.empty_like(q)
+    ops.kv8_attention(q, k, v, ks, vs, table, start, lens, out, 128 ** -0.5, ops.kv8_attention_workspace("cuda"))
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    bad[20:60, 4:] = True                                     # tokens at 140 .. 199
+    bad[60:, 4:] = True                                       # tokens at 293 .. 332
+    assert out.isnan().all(2).equal(bad) and out.isnan().any(2).equal(bad)
+    assert torch.equal(out[~bad], clean[~bad])
