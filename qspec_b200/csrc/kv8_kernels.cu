@@ -378,12 +378,14 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const 
   if ((int)blockIdx.x < units) {
     // slots from the token before this CTA's first on, two a lane: which begin a run, and where runs end as far as that shows
     const int sa = slot_of(a, t0 - 1 + lane), sb = slot_of(a, t0 + 31 + lane);
+    const bool turned = t0 - 1 + lane >= 0 && t0 - 1 + lane < a.ntok && has_angle(a, t0 - 1 + lane);
     const int before = __shfl_up_sync(0xffffffffu, sa, 1), mask = (1 << a.pshift) - 1;
     const bool go_on = lane > 0 && sa >= 0 && (sa & mask) && before == sa - 1;          // token t0 - 1 + lane is in the run of the one before it
     const int last = __shfl_sync(0xffffffffu, sa, 31), before_b = __shfl_up_sync(0xffffffffu, sb, 1);
     const bool go_on_b = sb >= 0 && (sb & mask) && (lane ? before_b : last) == sb - 1;
     const uint64_t in_run = ((uint64_t)__ballot_sync(0xffffffffu, go_on) | (uint64_t)__ballot_sync(0xffffffffu, go_on_b) << 32) >> 1;   // bit i: token t0 + i
     const uint32_t begin = __ballot_sync(0xffffffffu, lane > 0 && t0 - 1 + lane < t1 && sa >= 0 && !go_on) >> 1;
+    const uint32_t written = __ballot_sync(0xffffffffu, turned) >> 1;   // bit i: token t0 + i has an angle
     uint64_t more = in_run >> 1;                            // bit i: the SHORT tokens behind t0 + i are in its run
 #pragma unroll
     for (int o = 1; o < SHORT; o <<= 1) more &= more >> o;
@@ -392,8 +394,10 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const 
       int t = t0 + i, s = __shfl_sync(0xffffffffu, sa, i + 1);
       const int g = u >> 1;
       if (W > 1 && t + n >= t0 + 63) n = run_of(a, t, s, n);   // (it may be longer than that)
-      while (n && !has_angle(a, t)) { ++t; ++s; --n; }      // (it begins with the first token that is written)
-      if (!n) return;
+      if (!(written >> i & 1u)) {                           // (it begins with the first token that is written)
+        do { ++t; ++s; --n; } while (n && !has_angle(a, t));
+        if (!n) return;
+      }
       if (u & 1) write_run<BF16, D, false, W>(a, t, n, s, g, (a.H + a.G + g) * D, a.v, a.vs, s_max);
       else write_run<BF16, D, true, W>(a, t, n, s, g, (a.H + g) * D, a.k, a.ks, s_max);
     };
