@@ -380,7 +380,7 @@ int qspec_rope_qkhad_kvcache(void* qkv, const void* cos_sin_cache, const int* po
  * order of the requests. A request is refused (no pages; kv_len 0; its tokens without positions and slots) where what was asked for so
  * far, its own pages included, is more than there is, where its row of the table is too short, or where its tokens do not fit into ntok.
  *   q_start [requests + 1]: first token of each request; kv_len [requests]: tokens held once the step has run (0: refused or ended);
- *   positions, seq_ids, slots [ntok]: of each token; -1 where there is none. state_out [requests + 2]: the state behind this step, then the number of
+ *   positions, seq_ids, slots [ntok]: of each token; -1 where there is none (no slot either where the table or the list names no page of the cache). state_out [requests + 2]: the state behind this step, then the number of
  *   requests refused.
  * `state` is not changed, nor is anything that it describes (table entries and list entries behind it are): a step that is given up costs nothing, one that
  * is made is made so by copying state_out over state. What is

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(const PlanArgs 
         pos = l + (t - s_tok[req]);
         const int nth = pos >> a.pshift;
         const int pg = nth < h ? a.table[(size_t)req * a.width + nth] : page(s_need[req] + nth - h);
-        slot = (pg << a.pshift) + (pos & ((1 << a.pshift) - 1));
+        if ((unsigned)pg < (unsigned)a.npages) slot = (pg << a.pshift) + (pos & ((1 << a.pshift) - 1));   // (an entry that is no page: no slot)
       }
     }
     a.positions[t] = pos;

@@ -792,3 +792,15 @@ def test_attention_shows_a_scale_that_is_no_number_and_only_where_it_is_seen(sid
     bad[60:, 4:] = True                                       # tokens at 293 .. 332
     assert out.isnan().all(2).equal(bad) and out.isnan().any(2).equal(bad)
     assert torch.equal(out[~bad], clean[~bad])
+
+
+def test_page_plan_gives_no_slot_in_what_is_no_page():
+    """Entries of the table and of the list of free pages outside the cache: 2^26 pages of 64 tokens on is where a slot's number would begin again."""
+    table = [[1 << 26, 3], [-1, 0], [2, 0], [0, 0]]
+    free = [(1 << 26) + 1, 8, -7, 1, 5, 0, 0, 0]
+    lengths, counts, held = [64, 10, 60, 0], [2, 1, 8, 1], [2, 1, 1, 0]
+    got = run_plan(lengths, counts, table, free, held, 3, 64, 12)
+    assert got[2] == [64, 65, 10, 60, 61, 62, 63, 64, 65, 66, 67, 0]
+    assert got[4] == [3 * 64, 3 * 64 + 1, -1] + [2 * 64 + r for r in (60, 61, 62, 63)] + [-1] * 5
+    lengths[0] = 10                                           # the page behind the cache
+    assert run_plan(lengths, counts, table, free, held, 3, 64, 12)[4][:2] == [-1, -1]
