@@ -90,7 +90,8 @@ __device__ __forceinline__ Req request(const AttArgs& a, int b, unsigned long lo
   r.keys = max(a.kv_len[b], 0);
   const long long rows = (long long)r.n * a.rep;
   r.tiles = to_prompt_form(r.n, r.keys, a.rep, a.share, work) ? 0 : (int)((rows + ROWS - 1) / ROWS);
-  r.units = max((r.keys + UNIT - 1) / UNIT, 1);   // a request without keys has a unit that shows its rows none
+  // A request without keys has a unit that shows its rows none. Behind the table's last page is nothing but a page that there is not: one unit shows that.
+  r.units = max((min(r.keys, keys_at_most(a.width, a.pshift)) + UNIT - 1) / UNIT, 1);
   return r;
 }
 

@@ -33,6 +33,9 @@ __device__ __forceinline__ float finite_scale(float x) { return x < INFINITY ? x
 // the other as far on the other side. Not so small that it would make a hidden key's score (minus infinity) no number.
 __device__ __forceinline__ float score_factor(float scale, float row) { return fmaxf(scale * row * 16777216.f, 1.17549435e-38f); }
 
+// Keys that are walked at most: those that a row of the table has pages for, and one that it has none for (less than what would leave an int when it is rounded up).
+__device__ __forceinline__ int keys_at_most(int width, int pshift) { return (int)min(((unsigned)width << pshift) + 1u, 0x7fffff80u); }
+
 // Which form of the attention a request goes to, from what all requests of the call ask for; both kernels work it out alike. The prompt form takes 128 rows (tokens *
 // heads of a group) and a head a CTA, so that a block of keys costs it the same however few requests there are; the other one spreads any request over the GPU but
 // reads the keys again for every 16 rows. A request goes to the prompt form if the call has rows for a third of the SMs, it has PROMPT_ROWS rows or more, and its way

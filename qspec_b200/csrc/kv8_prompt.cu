@@ -126,6 +126,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     if (per_thread > 1) load(b, n1, keys1);
     return to_prompt_form(n1, keys1, rep, a.share, work) ? (n1 + span - 1) / span : 0;
   };
+  const int most = keys_at_most(a.width, a.pshift);
   int mine = 0;
   for (int i = 0; i < requests; ++i) mine += tiles_of(b0 + i);
   int incl = mine;
@@ -176,7 +177,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
   const int t0 = tile * span, n2 = min(span, n_new - t0);   // this CTA's tokens
   const int pos0 = keys - n_new + t0;                     // position of the first
   const bool both = n2 > tok;                             // two tiles of rows, a stream each
-  auto blocks_of = [&](int tokens) { const int seen = min(pos0 + tokens, keys); return seen > 0 ? (seen + 127) / 128 : 0; };
+  const int reach = min(keys, most);
+  auto blocks_of = [&](int tokens) { const int seen = min(pos0 + tokens, reach); return seen > 0 ? (seen + 127) / 128 : 0; };
   const int blocks = blocks_of(n2);                       // keys that any row sees
   const int turns0 = both ? blocks_of(tok) : (blocks + 1) >> 1, turns1 = both ? blocks : blocks >> 1;   // blocks of the streams
   if (tid == 0)

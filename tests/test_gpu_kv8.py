@@ -804,3 +804,22 @@ def test_page_plan_gives_no_slot_in_what_is_no_page():
     assert got[4] == [3 * 64, 3 * 64 + 1, -1] + [2 * 64 + r for r in (60, 61, 62, 63)] + [-1] * 5
     lengths[0] = 10                                           # the page behind the cache
     assert run_plan(lengths, counts, table, free, held, 3, 64, 12)[4][:2] == [-1, -1]
+
+
+@pytest.mark.parametrize("form", ["rows", "prompt", "pairs"])
+def test_attention_walks_no_further_than_the_table(form, monkeypatch):
+    """Lengths beyond the table's pages, up to the largest number there is: the rows that see such keys are NaN, soon; others are what they are."""
+    if form != "rows":
+        monkeypatch.setattr(ops, "kv8_attention", lambda *args, **kw: prompt_form(*args, pairs=form == "pairs", **kw))
+    q, k, v, ks, vs, table, start, lens = make_attention(21, [200, 256, 100], [40, 20, 40], 8, 2, 128, 32, torch.float16)
+    clean = check_attention((q, k, v, ks, vs, table, start, lens), 128)
+    work = ops.kv8_attention_workspace("cuda")
+    short = table[:, :4].contiguous()                         # 128 keys
+    for large in (129, 300, 10 ** 6, 2 ** 31 - 1):
+        far = i32([large, 256, 100])
+        out = ops.kv8_attention(q, k, v, ks, vs, short, start, far, torch.zeros_like(q), 128 ** -0.5, work)
+        first = large - 40
+        bad = [first + i >= 128 for i in range(40)] + [True] * 20 + [False] * 40
+        bad = torch.tensor(bad, device="cuda")
+        assert out[bad].isnan().all() and not out[~bad].isnan().any()
+        assert torch.equal(out[60:], clean[60:])
