@@ -36,6 +36,8 @@ class QSpecEngine:
             raise ValueError(f"temperature must be 0 (greedy) or at least 1e-33, got {temperature}")
         if temperature and model.tp_size != 1:
             raise NotImplementedError("sampling with a vocab-sharded lm_head")
+        if temperature and k > (most := ops.max_verified_drafts()):
+            raise ValueError(f"sampling verifies at most {most} draft tokens a step, got k = {k}")
         self.temperature = float(temperature)
         dev = model.device
         B = batch

@@ -955,6 +955,11 @@ def _probs(t: torch.Tensor, name: str, *shape: int) -> None:
         raise ValueError(f"{name} must be a float32 CUDA tensor {shape} with unit stride over the vocabulary")
 
 
+def max_verified_drafts() -> int:
+    """Drafts of a request that `verify_drafts` takes."""
+    return _lib.load().qspec_verify_drafts_max_drafts()
+
+
 def verify_drafts(drafted: Optional[torch.Tensor], draft_probs: Optional[torch.Tensor], target_probs: torch.Tensor, uniform: torch.Tensor, tokens: torch.Tensor,
                   emitted: torch.Tensor, draft_counts: Optional[torch.Tensor] = None) -> None:
     """Verification of drafted tokens [B, k] (int64) that were drawn from draft_probs [B, k, V], against target_probs [B, k + 1, V] (float32, rows may be strided),

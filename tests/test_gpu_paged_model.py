@@ -367,3 +367,15 @@ def test_an_engine_without_drafts_decodes_token_by_token(kv_cache, temperature):
         got.append(engine.out_tokens[:, 0].tolist())
     want = Scheduler(QSpecLlamaModel(config(kv_cache=kv_cache, kv_page=16), max_batch=2, max_tokens=8, seed=6)).generate([list(range(6)), list(range(6, 12))], 5)
     assert [list(t) for t in zip(*got)] == want
+
+
+def test_more_drafts_than_are_verified_are_refused_when_the_engine_is_made():
+    model = QSpecLlamaModel(config(), max_batch=1, max_tokens=40, seed=6)
+    with pytest.raises(ValueError, match="at most 31"):
+        QSpecEngine(model, 1, 32, temperature=0.5)
+    QSpecEngine(model, 1, 32)
+    engine = QSpecEngine(model, 1, 31, use_cuda_graph=False, temperature=0.5)
+    engine.prefill(torch.arange(6, device="cuda").view(1, 6))
+    engine.step()
+    engine.stream.synchronize()
+    assert 1 <= int(engine.out_count) <= 32
