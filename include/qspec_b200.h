@@ -404,7 +404,7 @@ int qspec_kv8_read(const void* k, const void* v, const float* k_scale, const flo
 
 /* Softmax attention of a step's tokens over that cache. q [ntok, H, D] with free token / head strides; the tokens q_start[b] .. q_start[b + 1] - 1 of
  * request b stand at the last positions of its kv_len[b] tokens and see the keys up to their own. Tokens that see no key give zeros; tokens
- * behind q_start[requests] are not written. max_tokens: an upper bound of the tokens that any request has in the step (it decides which
+ * behind q_start[requests] are not written. out may be q itself (same strides), but lie over nothing else of the call. max_tokens: an upper bound of the tokens that any request has in the step (it decides which
  * forms are launched; a request with more is attended to as well, more slowly). scale is positive and finite. Scales are positive (a scale
  * below 2^-100 counts as that); pages outside the cache, and scales that are infinite or no number, make the rows that see them NaN, and no others. workspace: zero-initialised once, left ready for the next call;
  * one for each stream that calls are made on at the same time. */

@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv8_append_kernel(const 
     }
   } else {
     // LANES lanes take a token and some of its heads, two under way at a time: one look at the position and the angles for all of them (row by row, with both
-    // for each, a prompt of 4200 tokens took 26.2 us, so 24.0).
+    // for each, a prompt of 4200 tokens took 26.2 us, so 24.3).
     const int c = lane % LANES, group = warp * ROWS + lane / LANES, t = t0 + (group & ((1 << a.tshift) - 1)), per_cta = (APPEND_WARPS * ROWS) >> a.tshift;
     const int p = t < t1 ? a.positions[t] : -1;
     if (p < 0 || p >= a.cos_rows) return;

@@ -17,7 +17,7 @@
 // What a block of 128 x 128 (head 128) asks of an SM: 1024 cycles of the tensor cores, 1024 of the exponentials (16 a cycle), and of the schedulers 720 by the softmax
 // and 400 by the codes (200 of two tiles). It takes 2350 cycles of two tiles (2850 to 3400 of one): what bounds it is a stream's way from scores to the next scores,
 // 4700 cycles, of which the softmax is 3000 (a warp's 32 exponentials and what belongs to them 570) and the products with their waits 1700; start and end of a CTA are
-// another 16000. Prompt of 2000 tokens after 1000, 32 / 8 heads, float16: 111 us, 590 TFLOP/s. Measured and not taken: sixteen softmax warps, two for
+// another 16000. Prompt of 2000 tokens after 1000, 32 / 8 heads, float16: 112 us, 586 TFLOP/s. Measured and not taken: sixteen softmax warps, two for
 // a row, 125 us (their common maximum and their waits cost more than they save); a warp for each stream's products 128 us (the streams fall into step);
 // scores read one chunk ahead 137 us (the copies between registers).
 //

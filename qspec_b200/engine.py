@@ -25,7 +25,8 @@ class QSpecEngine:
     def __init__(self, model: QSpecLlamaModel, batch: int, k: int = 3, use_cuda_graph: bool = True, temperature: float = 0.0, seed: int = 0):
         """temperature 0: greedy, a draft token is accepted iff it is the target's arg max. Above 0: tokens are drawn from softmax(logits / temperature) and draft
         tokens accepted with probability min(1, p / q), so that what is emitted is distributed as the target's own (vllm/model_executor/layers/
-        rejection_sampler.py); `seed` decides the random numbers.
+        rejection_sampler.py); `seed` decides the random numbers. (Over the 8-bit cache the target depends on the drafts a little: a page's scale does not shrink while its
+        first row stands, so that rows of a draft that was refused, or that verification wrote over, may leave the page coarser than without them.)
 
         Over a paged cache with fewer pages than all sequences may need, a step may find none for some of them: these emit nothing (out_count 0) and stay where they
         are. `step` raises for that at its first call behind a `prefill` and at every 64th, `metrics` at once; the next `prefill` begins with all pages."""

@@ -57,7 +57,8 @@ class Scheduler:
     def feed(self, entries: Sequence[Tuple[Hashable, Sequence[int], Sequence[int]]]) -> torch.Tensor:
         """entries: (request id, its next tokens, indices among these tokens whose logits are wanted). Runs the tokens
         from the state earlier calls left and returns float32-or-model-typed logits [total wanted, vocab] in the order of
-        the entries and of their wanted lists. Entries longer than the model's step size are cut into several passes."""
+        the entries and of their wanted lists. Entries longer than the model's step size are cut into several passes; if the model refuses one
+        (RuntimeError), the tokens of the passes before it are consumed, and no others (`table.pos`)."""
         model, cap = self.model, self.model.max_step_tokens
         limit = getattr(model, "max_seq_len", None)
         seen = set()
