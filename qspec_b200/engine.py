@@ -287,6 +287,7 @@ class QSpecEngine:
         reference engine does); returns host [B, k+2] = emitted tokens (-1 padded) + count.
         H2D of the inputs and D2H of the result are part of the call."""
         self.h_in.copy_(host_tokens)
+        self._join_caller_stream()                        # (a prefill that has yet to run writes cur_tok, too)
         with torch.cuda.stream(self.stream):
             self.cur_tok.copy_(self.h_in, non_blocking=True)
         self.step()

@@ -379,3 +379,22 @@ def test_more_drafts_than_are_verified_are_refused_when_the_engine_is_made():
     engine.step()
     engine.stream.synchronize()
     assert 1 <= int(engine.out_count) <= 32
+
+
+def test_tokens_from_the_host_come_behind_what_the_caller_has_queued():
+    """A prefill that has yet to run must not write its own last tokens over those that `step_host` brings."""
+    results = []
+    for late in (False, True):
+        model = QSpecLlamaModel(config(), max_batch=2, max_tokens=32, seed=8)
+        engine = QSpecEngine(model, 2, 3)
+        prompts = torch.arange(12, device="cuda").view(2, 6)
+        engine.prefill(prompts)
+        engine.capture()                                      # (waits for everything, once)
+        tokens = torch.tensor([400, 500])
+        if late:
+            torch.cuda._sleep(400_000_000)
+        engine.prefill(prompts)
+        if not late:
+            torch.cuda.synchronize()
+        results.append(engine.step_host(tokens).clone())
+    assert torch.equal(*results)
