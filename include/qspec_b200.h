@@ -380,7 +380,8 @@ int qspec_rope_qkhad_kvcache(void* qkv, const void* cos_sin_cache, const int* po
  * order of the requests. A request is refused (no pages; kv_len 0; its tokens without positions and slots) where what was asked for so
  * far, its own pages included, is more than there is, where its row of the table is too short, or where its tokens do not fit into ntok.
  *   q_start [requests + 1]: first token of each request; kv_len [requests]: tokens held once the step has run (0: refused or ended);
- *   positions, seq_ids, slots [ntok]: of each token; -1 where there is none (no slot either where the table or the list names no page of the cache). state_out [requests + 2]: the state behind this step, then the number of
+ *   positions, seq_ids, slots [ntok]: of each token; -1 where there is none (no slot either where the table or the list names no page of the
+ *   cache). state_out [requests + 2]: the state behind this step, then the number of
  *   requests refused.
  * `state` is not changed, nor is anything that it describes (table entries and list entries behind it are): a step that is given up costs nothing, one that
  * is made is made so by copying state_out over state. What is
@@ -393,8 +394,9 @@ int qspec_page_plan(const int* lengths, const int* counts, int* table, int* free
  * A page's scale: the largest of |x| / 127 of the rows that the call writes to it, of its scale before (unless its first row is among them) and 2^-60; codes =
  * rint(x / scale) (infinities: +-127, NaN: 0, neither stretches the scale). Where a scale grows the page's older rows are put on the new one.
  * Rotated values are quantised in float32, without a rounding to 16 bits in between. Tokens whose slot or position is outside the cache or
- * the table of angles are skipped: their rows of the cache are left as they are. The tokens of one page in a call must be neighbours in the batch, their slots consecutive rows (a
- * token without a slot between them breaks that; one without a position does not). Rows of the page behind them are no one's any more: they stay on the scale before. */
+ * the table of angles are skipped: their rows of the cache are left as they are. The tokens of one page in a call must be neighbours in the batch, their slots
+ * consecutive rows (a token without a slot between them breaks that; one without a position does not). Rows of the page behind them are no one's any more: they
+ * stay on the scale before. */
 int qspec_kv8_append(const void* qkv, long long ld, const void* cos_sin, int cos_rows, const int* positions, const int* slots, void* k, void* v, float* k_scale,
                      float* v_scale, void* q_out, long long q_tok_stride, int ntok, int H, int G, int D, int npages, int page_tokens, int dtype, void* stream);
 
@@ -404,9 +406,10 @@ int qspec_kv8_read(const void* k, const void* v, const float* k_scale, const flo
 
 /* Softmax attention of a step's tokens over that cache. q [ntok, H, D] with free token / head strides; the tokens q_start[b] .. q_start[b + 1] - 1 of
  * request b stand at the last positions of its kv_len[b] tokens and see the keys up to their own. Tokens that see no key give zeros; tokens
- * behind q_start[requests] are not written. out may be q itself (same strides), but lie over nothing else of the call. max_tokens: an upper bound of the tokens that any request has in the step (it decides which
- * forms are launched; a request with more is attended to as well, more slowly). scale is positive and finite. Scales are positive (a scale
- * below 2^-100 counts as that); pages outside the cache, and scales that are infinite or no number, make the rows that see them NaN, and no others. workspace: zero-initialised once, left ready for the next call;
+ * behind q_start[requests] are not written. out may be q itself (same strides), but lie over nothing else of the call. max_tokens: an upper bound of
+ * the tokens that any request has in the step (it decides which forms are launched; a request with more is attended to as well, more slowly). scale is positive and
+ * finite. Scales of pages are positive (one below 2^-100 counts as that); pages outside the cache, and scales that are infinite or no number, make the rows
+ * that see them NaN, and no others. workspace: zero-initialised once, left ready for the next call;
  * one for each stream that calls are made on at the same time. */
 size_t qspec_kv8_attention_workspace_bytes(void);
 int qspec_kv8_attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const float* k_scale, const float* v_scale,

@@ -451,7 +451,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
         const int src = (16 * q) >> a.pshift;
-        const float f = positive(__shfl_sync(0xffffffffu, cks, src)), v = fminf(positive(__shfl_sync(0xffffffffu, cvs, src)), 8.507059e37f);   // (not infinite: beside a hidden key's minus infinity that would be no number)
+        const float f = positive(__shfl_sync(0xffffffffu, cks, src)), v = fminf(positive(__shfl_sync(0xffffffffu, cvs, src)), 8.507059e37f);
+        // (2^126, not infinite: beside a hidden key's minus infinity that would be no number)
         lv[q] = __log2f(v);
         iv[q] = __fdividef(WEIGHT_UNIT, v);
 #pragma unroll

@@ -23,9 +23,10 @@ __device__ __forceinline__ float positive(float x) { return x >= 7.8886090522101
 // ones: what float16 cannot hold is lost to the one and not to the other, always to the same side, and over a long context that adds up. So weights begin at
 // 2^WEIGHT_LOG2 where the reference stands, and it follows the maximum as soon as that is 2^GROWTH_LOG2 above it: the largest is at most 2^15, what is above 2^-23 of it
 // is rounded by 2^-11 of itself at most, and below that a key is off by 2^-25 of 2^9 at most. (While weights began at 1, behind a key that leads in a page whose value
-// scale is 64 times the others', 131,000 keys at 2^-19.1 of its weight, 19 % of all there is, came to nothing in the sum of values.) A reference that follows sooner costs the prompt form: 2000 tokens after 1000, with growth by 2^8
-// 112 us, 2^6 114, 2^5 115, 2^4 117. 2^16 is infinite, and a reference has a rounding of its own: beyond FAR it is subtracted from the finished exponent, which was rounded
-// like it. Sums of weights / v are kept in units of 2^WEIGHT_LOG2, so that they hold for every scale that positive() leaves.
+// scale is 64 times the others', 131,000 keys at 2^-19.1 of its weight, 19 % of all there is, came to nothing in the sum of values.) A reference that follows
+// sooner costs the prompt form: 2000 tokens after 1000, with growth by 2^8 112 us, 2^6 114, 2^5 115, 2^4 117. 2^16 is infinite, and a reference has a rounding of its
+// own: beyond FAR it is subtracted from the finished exponent, which was rounded like it. Sums of weights / v are kept in units of 2^WEIGHT_LOG2, so that they
+// hold for every scale that positive() leaves.
 constexpr float WEIGHT_LOG2 = 9.f, GROWTH_LOG2 = 6.f, WEIGHT_UNIT = 1.f / 512.f, FAR = 1048576.f;
 // An infinite one is no number either: beside a hidden key's minus infinity it would be one in rows that do not see the page.
 __device__ __forceinline__ float finite_scale(float x) { return x < INFINITY ? x : NAN; }

@@ -233,7 +233,7 @@ extern "C" int qspec_verify_drafts(const long long* drafted, const float* draft,
   // CTAs of a request: eight where two rounds of such clusters hold all requests (a row's way through the GPU counts), four where they fill it by themselves. Three
   // drafts, us with eight (four): vocabulary of 152064, 64 requests 13.7 (16.8), 80: 20.7 (18.0), 96: 23.6 (19.2), 128: 28.0 (32.0), 190: 41.6 (38.8), 256: 53.4 (53.0);
   // of 32000, 16: 6.2 (5.9), 64: 7.6 (7.7), 80: 10.6 (7.9), 128: 12.7 (11.0), 256: 22.6 (17.2). (128 of the larger vocabulary is the one that the rule takes the slower
-  // way: there eight CTAs fill their last round.) Rows that do not begin on 16 bytes are loaded value by value: of 151643, 64 requests 18.4 (152064: 13.9), 190 of five
+  // way: 512 CTAs, three an SM, leave a second round nearly empty.) Rows that do not begin on 16 bytes are loaded value by value: of 151643, 64 requests 18.4 (152064: 13.9), 190 of five
   // drafts 48.0 (39.9). Without drafts, of 128256: 4 rows 6.6, 64 rows 11.9; 190 rows of 152064 32.1.
   const bool many = requests > sm_count() / 2 && vocab <= 4 * MAX_TILES * TILE;
   const int cluster = many ? 4 : 8;

@@ -160,7 +160,8 @@ class QSpecEngine:
             vpos = (self.seq_len.unsqueeze(1) + self.arange_k1.unsqueeze(0)).reshape(-1).contiguous()
             hidden = m.forward(vt, vpos, self.vseq_ids, w4a4=False)
         if self.temperature:
-            ops.verify_drafts(self.draft_toks if k else None, self.draft_probs.transpose(0, 1) if k else None, self._probs(hidden).view(B, k + 1, -1), self.uniform[1], self.out_tokens, self.out_count)
+            drafts = (self.draft_toks, self.draft_probs.transpose(0, 1)) if k else (None, None)
+            ops.verify_drafts(*drafts, self._probs(hidden).view(B, k + 1, -1), self.uniform[1], self.out_tokens, self.out_count)
             n_acc, emitted = self.out_count - 1, self.out_tokens
             nxt = emitted.gather(1, n_acc.unsqueeze(1)).squeeze(1)
         else:

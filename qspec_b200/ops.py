@@ -919,8 +919,8 @@ def kv8_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
                   max_tokens: Optional[int] = None) -> torch.Tensor:
     """Softmax attention of a step's tokens q [T, H, D] (float16 / bfloat16; token and head strides free) over the 8-bit cache: tokens q_start[b] ..
     q_start[b + 1] - 1 are request b's last of kv_len[b], and see its keys up to their own. table int32 [B, W]. out [T, H, D] of q's type; rows that see no
-    key are zeros, rows behind q_start[B] are left as they are; out may be q itself, but lie over nothing else of the call. max_tokens: an upper bound of the tokens that a request has in the step (T if not
-    given). Which form a request takes follows from it and from what the call's requests ask for together, so that a row's last bits may differ with the other
+    key are zeros, rows behind q_start[B] are left as they are; out may be q itself, but lie over nothing else of the call. max_tokens: an upper
+    bound of the tokens that a request has in the step (T if not given). Which form a request takes follows from it and from what the call's requests ask for together, so that a row's last bits may differ with the other
     requests. workspace: `kv8_attention_workspace`."""
     if _fast_call("kv8_attention", q, k_codes, v_codes, k_scale, v_scale, table, q_start, kv_len, out, sm_scale, workspace, max_tokens):
         return out
