@@ -4,10 +4,7 @@
 // A row is a (token, query head of a group) pair; 16 rows of one key/value head are a tile of mma.sync.m16n8k16, so that the heads of a group and the
 // tokens that verify a draft share every key that is read. What bounds it at these row counts is the cache: 2 D bytes a key and head.
 //
-// Work: (request, head, row tile) items of units of 32 keys, laid end to end and cut into equal stretches, one per CTA: lengths that
-// differ cost nothing, one long request uses every SM. Inside a stretch unit i is warp i % WARPS's. Every warp keeps a softmax of its own (maximum, sum and
-// sums of values in registers) over the units of an item that it took; they are joined through shared memory at the item's end and, where a stretch
-// ends inside an item, through the workspace: the CTA that comes last adds the parts up in their order, so that results do not depend on which it is.
+// How the work is spread over the GPU, and the parts joined: kv_stretch.cuh.
 //
 // Codes go from global memory into shared memory (16 bytes a lane, asynchronously, one unit of keys and one of values per warp) and from there into
 // registers as the products' operands.
@@ -22,27 +19,16 @@
 // multiplies its scores in float32. A value's scale v goes into the exponent: the weights 2^(9 + s + log2 v - m) lie below 2^15 whatever the scales are and are
 // rounded to float16 for the product with the codes (by 2^-11 of themselves at most, or by 2^-34 of the largest: kv8_common.cuh); the denominator is the sum of the
 // unrounded weights / v.
-#include "kv8_common.cuh"
+#include "kv_stretch.cuh"
 
 namespace qspec {
 namespace kv8 {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, UNIT = 32, ROWS = 16;
-constexpr int MIN_UNITS = WARPS;                 // of a stretch: one for each warp
-constexpr int CTAS = 3;                          // of an SM: while one waits at a barrier the others compute
-constexpr int GRID_MOST = 480;                   // CTAs
-constexpr float NONE = -INFINITY;
-
-struct AttArgs {
+struct AttArgs : Step, Out {
   const void* q; long long q_ts; int q_hs;
   const signed char *k, *v;
   const float *ks, *vs;
-  const int *table, *q_start, *kv_len;
-  int nreq, width, npages, pshift, ntok, G, rep;
-  unsigned share;                                // to_prompt_form()'s; 0: there is no prompt form in this call
   float scale2;                                  // scale * log2(e)
-  void* out; long long out_ts; int out_hs;
-  int* counters; float* parts;
 };
 
 template <int D> struct Smem {
@@ -56,13 +42,11 @@ template <int D> struct Smem {
   static constexpr size_t F = ROWS * 4;                             // factors of the rows' scores
   static constexpr size_t TOTAL = RING + Q + O + ML + F;
 };
-template <int D> constexpr int PART = ROWS * 2 + ROWS * D;   // floats of a part: maxima, sums, sums of values
 
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
-__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
 // d = a b + c
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
@@ -78,59 +62,12 @@ __device__ __forceinline__ uint32_t first_two(uint32_t w) { return __byte_perm(w
 __device__ __forceinline__ uint32_t last_two(uint32_t w) { return __byte_perm(w, 0u, 0x4342); }
 constexpr uint32_t MINUS_128 = 0x80808080u;      // two of -128 2^-24: what the codes' 128 adds up to, the other way round
 
-// A request's part of the work.
-struct Req {
-  int first, n, keys, tiles, units;               // first row of q, tokens, keys, row tiles, units of an item
-  __device__ __forceinline__ long long total(int G) const { return (long long)tiles * G * units; }
-};
-__device__ __forceinline__ Req request(const AttArgs& a, int b, unsigned long long work) {
-  Req r;
-  r.first = min(max(a.q_start[b], 0), a.ntok);
-  r.n = max(min(a.q_start[b + 1], a.ntok) - r.first, 0);
-  r.keys = max(a.kv_len[b], 0);
-  const long long rows = (long long)r.n * a.rep;
-  r.tiles = to_prompt_form(r.n, r.keys, a.rep, a.share, work) ? 0 : (int)((rows + ROWS - 1) / ROWS);
-  // A request without keys has a unit that shows its rows none. Behind the table's last page is nothing but a page that there is not: one unit shows that.
-  r.units = max((min(r.keys, keys_at_most(a.width, a.pshift)) + UNIT - 1) / UNIT, 1);
-  return r;
-}
-
-// Where a unit lies: request, head and row tile (tiles inside heads), unit of that item.
-struct Place {
-  int b, g, tile, u;
-  Req r;
-  __device__ __forceinline__ void forward(const AttArgs& a, unsigned long long work, int steps) {
-    u += steps;
-    while (b < a.nreq && u >= r.units) {
-      u -= r.units;
-      if (++tile < r.tiles) continue;
-      tile = 0;
-      if (++g < a.G) continue;
-      g = 0;
-      do { if (++b >= a.nreq) return; r = request(a, b, work); } while (r.tiles == 0);
-    }
-  }
-};
-
 // Where the 16 bytes c of a row lie in a buffer, so that neither copies nor reads of eight rows meet in a bank.
 template <int D>
 __device__ __forceinline__ uint32_t k_chunk(int row, int c) { return (uint32_t)(row * D + ((D == 128 ? c ^ ((row & 1) << 2) : c) << 4)); }
 template <int D>
 __device__ __forceinline__ uint32_t v_chunk(int row, int c) { return (uint32_t)(row * D + ((D == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3)) << 4)); }
 
-// The page that lane i has of the unit at `p`: its ith, of UNIT / P (at least one); -1: one behind the last key; BROKEN: an entry that is no page of the cache.
-constexpr int BROKEN = -2;
-__device__ __forceinline__ int unit_page(const AttArgs& a, const Place& p, int lane) {
-  const int n = max(UNIT >> a.pshift, 1), at = ((p.u * UNIT) >> a.pshift) + lane;
-  if (p.b >= a.nreq || lane >= n || (at << a.pshift) >= p.r.keys) return -1;
-  const int page = at < a.width ? a.table[(size_t)p.b * a.width + at] : BROKEN;
-  return (unsigned)page < (unsigned)a.npages ? page : BROKEN;
-}
-// A unit whose pages are known: where its codes are (bytes from the first page's, the same for keys and values; each lane its page's) and its keys.
-struct Unit {
-  long long at;                                   // -1: no such page
-  int key0, keys;
-};
 // UNIT rows of keys or of values, 16 bytes a lane: 16 rows lie in one page, whatever its size, and rows of a group are at fixed distances. Rows behind the last key are
 // not fetched: what the buffer holds in their place are codes like any other, and meets weights of zero.
 template <int D, bool VALUES>
@@ -166,10 +103,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
   using S = Smem<D>;
   constexpr int NT = D / 8, CH = D / 16, KT = UNIT / 8, QT = UNIT / 16;   // column tiles of the value product, 16-byte pieces of a key (steps of the score product), key tiles
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long s_sum[WARPS];
-  __shared__ int s_place[4], s_items[WARPS], s_ctas[6][WARPS];
-  __shared__ Req s_req;
-  __shared__ int s_last;
+  __shared__ Shared s_sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, qi = lane >> 2, qj = lane & 3;
   unsigned char* const s_q = smem + S::RING;
   float* const s_o = reinterpret_cast<float*>(smem + S::RING + S::Q);
@@ -178,128 +112,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
   const uint32_t kbuf = shared_addr(smem) + warp * 2 * S::BUF, vbuf = kbuf + S::BUF;
   pdl_enter();
 
-  // ---- this CTA's stretch
-  const int per_thread = (a.nreq + THREADS - 1) / THREADS, b0 = tid * per_thread;
-  const int requests = max(min(per_thread, a.nreq - b0), 0);
-  unsigned long long work = 0;                              // that requests with rows enough for the prompt form ask for
-  if (a.share) {
-    for (int i = 0; i < requests; ++i) {
-      const Req r = request(a, b0 + i, 0);
-      work += prompt_work(r.n, r.keys, a.rep, a.G);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-    if (lane == 0) s_sum[warp] = (long long)work;
-    __syncthreads();
-    work = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) work += (unsigned long long)s_sum[w];
-    __syncthreads();
-  }
-  Req only{0, 0, 0, 0, 1};
-  if (per_thread == 1 && b0 < a.nreq) only = request(a, b0, work);
-  auto req = [&](int i) { return per_thread == 1 ? only : request(a, b0 + i, work); };
-  long long before, total;                                  // of the requests of the threads in front of this one, and of all
-  auto scan = [&](long long mine) {
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long w = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += w;
-    }
-    if (lane == 31) s_sum[warp] = incl;
-    __syncthreads();
-    before = incl - mine;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      if (w < warp) before += s_sum[w];
-      total += s_sum[w];
-    }
-  };
-  long long mine = 0;
-  int items = 0;
-  for (int i = 0; i < requests; ++i) {
-    const Req r = req(i);
-    mine += r.total(a.G);
-    items = min(items + (int)min((long long)r.tiles * a.G, (long long)GRID_MOST + 1), GRID_MOST + 1);
-  }
-  items = __reduce_add_sync(0xffffffffu, items);
-  if (lane == 0) s_items[warp] = items;
-  scan(mine);
-  const int grid = gridDim.x;
-  long long per = max(total <= 0x7fffffff ? (long long)(((int)total - 1) / grid + 1) : (total + grid - 1) / grid, (long long)MIN_UNITS);
-  // A stretch may lie over the end of an item: then the CTA joins and stores twice. With few items each gets CTAs of its own, as long as that makes no
-  // stretch much longer (by a quarter and eight units at most): 4 requests of 900, 32 / 8 heads, one token each 17.0 -> 12.1 us.
-  bool whole = false;
-  items = 0;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) items += s_items[w];
-  if (items <= grid && per < (1 << 24)) {
-    constexpr int TRIES = 6;                                // lengths that are looked at
-    auto length = [&](int c) { const int p = (int)per; return c == 0 ? p : c == 1 ? p + 1 : c == 2 ? p + p / 32 + 1 : c == 3 ? p + p / 16 + 2 : c == 4 ? p + p / 8 + 4 : p + p / 4 + 8; };
-    int n[TRIES] = {0, 0, 0, 0, 0, 0};
-    for (int i = 0; i < requests; ++i) {
-      const Req r = req(i);
-#pragma unroll
-      for (int c = 0; c < TRIES; ++c)
-        n[c] = min(n[c] + (int)min((long long)r.tiles * a.G * ((r.units - 1) / length(c) + 1), (long long)GRID_MOST + 1), GRID_MOST + 1);
-    }
-#pragma unroll
-    for (int c = 0; c < TRIES; ++c) {
-      n[c] = __reduce_add_sync(0xffffffffu, n[c]);
-      if (lane == 0) s_ctas[c][warp] = n[c];
-    }
-    __syncthreads();
-    int len = 0;
-#pragma unroll
-    for (int c = TRIES - 1; c >= 0; --c) {
-      int sum = 0;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) sum += s_ctas[c][w];
-      if (sum <= grid) len = length(c);
-    }
-    if (len) {
-      whole = true;
-      per = len;
-      mine = 0;                                             // CTAs of this thread's requests
-      for (int i = 0; i < requests; ++i) {
-        const Req r = req(i);
-        mine += (long long)r.tiles * a.G * ((r.units - 1) / len + 1);
-      }
-      scan(mine);
-    }
-  }
-  // (an item's units are spread evenly over its CTAs)
-  const long long begin = whole ? blockIdx.x : per * blockIdx.x;
-  if (begin >= total) return;
-  if (begin >= before && begin < before + mine) {
-    long long at = before;
-    for (int i = 0; i < requests; ++i) {
-      const Req r = req(i);
-      const int each = whole ? (r.units - 1) / (int)per + 1 : r.units;   // of an item: CTAs, or units
-      const long long n = (long long)r.tiles * a.G * each;
-      if (begin < at + n) {
-        s_place[0] = b0 + i;
-        s_place[1] = (int)((begin - at) / each);            // item of the request: head * tiles + tile
-        s_place[2] = (int)((begin - at) % each);
-        s_place[3] = each;
-        s_req = r;
-        break;
-      }
-      at += n;
-    }
-  }
-  __syncthreads();
-  Place cur;                                                // the segment that all warps are in: (the rest of) one item
-  cur.b = s_place[0];
-  cur.r = s_req;
-  cur.g = s_place[1] / cur.r.tiles;
-  cur.tile = s_place[1] - cur.g * cur.r.tiles;
-  const int share = whole ? (cur.r.units - 1) / s_place[3] + 1 : 0;
-  cur.u = whole ? min(s_place[2] * share, cur.r.units) : s_place[2];
-  const int todo = whole ? min(share, cur.r.units - cur.u) : (int)(min(begin + per, total) - begin);   // units of this stretch
-  if (todo <= 0) return;                                    // (a last share of none)
+  unsigned long long work;
+  Stretch stretch;
+  if (!find_stretch(a, s_sh, work, stretch)) return;
+  Place cur = stretch.cur;                                  // the segment that all warps are in: (the rest of) one item
+  const int todo = stretch.todo;
 
   // Queries of an item: a thread's pieces of 8 values (rows behind the last one are zeros), then float16 in the order in which the product takes them: word
   // (step, lane, register) of the operand. Step 4 h + w of lane (row % 8, j) has columns 16 (4 h + j) + 4 w .. + 3.
@@ -373,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
   int seg0 = 0;                                             // index in the stretch of the segment's first unit
   while (seg0 < todo) {
     const int seg_n = min(cur.r.units - cur.u, todo - seg0);
-    const int tile = cur.tile, g = cur.g;
+    const int tile = cur.tile;
     const uint32_t frag = shared_addr(s_q) + lane * 16;
     auto query = [&](uint32_t (&x)[4], int step) {
       asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(frag + step * 512));
@@ -550,117 +367,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
         for (int t = 0; t < NT; ++t) *reinterpret_cast<float2*>(row + 8 * t) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
       }
     }
-    __syncthreads();
-    constexpr int PER_ROW = THREADS / ROWS, PIECES = D / 4 / PER_ROW;   // threads of a row, float4 of a thread
-    const int jr = tid / PER_ROW, col = tid % PER_ROW;
-    float mm = NONE, ll = 0.f;
-    float4 oo[PIECES];
-#pragma unroll
-    for (int c = 0; c < PIECES; ++c) oo[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto join = [&](float mw, float lw, auto&& piece) {
-      // (a part that saw nothing has no sums; one that saw NaN has a sum that is not zero)
-      if (mw == NONE && lw == 0.f) return;
-      const float mn = fmaxf(mm, mw), f = mm == NONE ? 0.f : exp2_fast(mm - mn), h = mw == NONE ? 1.f : exp2_fast(mw - mn);
-      mm = mn;
-      ll = ll * f + lw * h;
-#pragma unroll
-      for (int c = 0; c < PIECES; ++c) {
-        const float4 p = piece(c);
-        oo[c].x = oo[c].x * f + p.x * h; oo[c].y = oo[c].y * f + p.y * h; oo[c].z = oo[c].z * f + p.z * h; oo[c].w = oo[c].w * f + p.w * h;
-      }
-    };
-    for (int w = 0; w < WARPS; ++w)
-      join(s_ml[(w * 2) * ROWS + jr], s_ml[(w * 2 + 1) * ROWS + jr], [&](int c) { return *reinterpret_cast<const float4*>(s_o + (w * ROWS + jr) * S::LD + (col + PER_ROW * c) * 4); });
-    auto store_piece = [&](int r, int at, const float4& p, float f) {   // columns at .. at + 3 of the tile's row r
-      const int rr = tile * ROWS + r, tok = rr / a.rep;
-      uint2 w;
-      if (BF16) {
-        const __nv_bfloat162 x = __floats2bfloat162_rn(p.x * f, p.y * f), y = __floats2bfloat162_rn(p.z * f, p.w * f);
-        w = make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-      } else {
-        w = make_uint2(half_pair(p.x * f, p.y * f), half_pair(p.z * f, p.w * f));
-      }
-      *reinterpret_cast<uint2*>((T*)a.out + (size_t)(cur.r.first + tok) * a.out_ts + (size_t)(g * a.rep + rr - tok * a.rep) * a.out_hs + at) = w;
-    };
-    const bool starts = cur.u == 0, ends = cur.u + seg_n == cur.r.units;
-    if (starts && ends) {
-      if (tile * ROWS + jr < cur.r.n * a.rep) {
-        const float f = ll == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, ll);   // (no key: zeros)
-#pragma unroll
-        for (int c = 0; c < PIECES; ++c) store_piece(jr, (col + PER_ROW * c) * 4, oo[c], f);
-      }
-    } else {
-      // ---- a part of an item: into the workspace; the item's last CTA to come adds all of them up, first part first
-      const long long item0 = begin + seg0 - cur.u, item1 = item0 + cur.r.units;
-      const int c0 = whole ? (int)blockIdx.x - cur.u / share : (int)(item0 / per), c1 = whole ? c0 + (cur.r.units - 1) / share : (int)((item1 - 1) / per);
-      float* part = a.parts + (size_t)(2 * blockIdx.x + (starts ? 1 : 0)) * PART<D>;
-      if (col == 0) { part[jr] = mm; part[ROWS + jr] = ll; }
-#pragma unroll
-      for (int c = 0; c < PIECES; ++c) *reinterpret_cast<float4*>(part + 2 * ROWS + jr * D + (col + PER_ROW * c) * 4) = oo[c];
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();                                    // (of what the whole CTA has stored: the barrier is in front of it)
-        const int n = c1 - c0 + 1, old = atomicAdd(a.counters + c0, 1);
-        s_last = old == n - 1;
-        if (old == n - 1) a.counters[c0] = 0;               // for the next call
-      }
-      __syncthreads();
-      if (s_last) {
-        // All maxima and sums first (eight threads a row), which gives every part its factor, then the sums of values: loads that wait for none before them.
-        __threadfence();
-        const int n = c1 - c0 + 1;
-        auto from = [&](int i) { return a.parts + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * PART<D>; };
-        float* const factor = s_o;                          // [part][row]: the sums on their way between warps have been read
-        mm = NONE;
-        ll = 0.f;
-        for (int i0 = col; i0 < n; i0 += 8 * PER_ROW) {
-          float mp[8], lp[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int i = i0 + k * PER_ROW;
-            mp[k] = i < n ? __ldcg(from(i) + jr) : NONE;
-            lp[k] = i < n ? __ldcg(from(i) + ROWS + jr) : 0.f;
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const bool none = mp[k] == NONE;                // nothing seen, or (a sum that is not zero) no number
-            const float mn = fmaxf(mm, mp[k]);
-            ll = (mm == NONE ? ll : ll * exp2_fast(mm - mn)) + (none ? lp[k] : lp[k] * exp2_fast(mp[k] - mn));
-            mm = mn;
-            if (i0 + k * PER_ROW < n) factor[(i0 + k * PER_ROW) * ROWS + jr] = none && lp[k] != 0.f ? INFINITY : mp[k];
-          }
-        }
-        const float own = mm;
-#pragma unroll
-        for (int x = PER_ROW / 2; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
-        if (own != NONE) ll *= exp2_fast(own - mm);
-#pragma unroll
-        for (int x = PER_ROW / 2; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
-        for (int i = col; i < n; i += PER_ROW) {
-          const float f = factor[i * ROWS + jr];
-          factor[i * ROWS + jr] = f == NONE ? 0.f : f == INFINITY ? 1.f : exp2_fast(f - mm);
-        }
-        if (col == 0) factor[n * ROWS + jr] = ll == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, ll);   // (no key: zeros)
-        __syncthreads();
-        const int rows = min(cur.r.n * a.rep - tile * ROWS, ROWS);
-        for (int x = tid; x < rows * (D / 4); x += THREADS) {
-          const int r = x / (D / 4), at = x % (D / 4) * 4;
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int i0 = 0; i0 < n; i0 += 32) {
-            float4 v[32];
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              v[k] = i0 + k < n ? __ldcg(reinterpret_cast<const float4*>(from(i0 + k) + 2 * ROWS + r * D + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float f = i0 + k < n ? factor[(i0 + k) * ROWS + r] : 0.f;
-              sum.x = fmaf(v[k].x, f, sum.x); sum.y = fmaf(v[k].y, f, sum.y); sum.z = fmaf(v[k].z, f, sum.z); sum.w = fmaf(v[k].w, f, sum.w);
-            }
-          }
-          store_piece(r, at, sum, factor[n * ROWS + r]);
-        }
-      }
-    }
+    finish_segment<BF16, D, S::LD>(a, a, stretch, cur, seg0, seg_n, s_ml, s_o, s_sh);
     if (more) store_q();                                    // (all have passed the barrier behind their last use of this item's)
     cur = after;
     seg0 += seg_n;
@@ -714,8 +421,9 @@ static int attention(const void* q, long long q_tok_stride, int q_head_stride, c
                         page_shift(page_tokens), ntok, G, rep, pair, share, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, give_up};
     if (const int rc = launch_prompt(pa, D, dtype == QSPEC_DTYPE_BF16, (cudaStream_t)stream)) return rc;
   }
-  AttArgs a{q, q_tok_stride, q_head_stride, (const signed char*)k, (const signed char*)v, ks, vs, table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok,
-            G, rep, prompts ? share : 0u, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)};
+  AttArgs a{{table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok, G, rep, prompts ? share : 0u},
+            {out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)}, q, q_tok_stride, q_head_stride, (const signed char*)k, (const signed char*)v, ks, vs,
+            scale * 1.4426950408889634f};
   auto run = [&](auto kern, size_t smem, SmemLimit& limit) -> int {
     QSPEC_CUDA(limit.raise(kern, smem));
     QSPEC_CUDA(launch_pdl(kern, dim3(grid), dim3(THREADS), smem, (cudaStream_t)stream, a));
