@@ -424,6 +424,29 @@ int qspec_debug_kv8_attention_give_up(const void* q, long long q_tok_stride, int
                                       int requests, int width, int H, int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype,
                                       void* workspace, size_t workspace_bytes, unsigned give_up, void* stream);
 
+/* The same cache in 4 bits. Per layer, for keys and for values: codes uint8 [pages, G, P, D / 2], two to a byte, the even column in the low half, and a word of 16 bits for each
+ * row, [pages, G, P]: its scale s, a float32 of five significant bits (exponent in the upper eight bits, mantissa in the next four), and its zero point z in the lowest four. A code
+ * c stands for (c - z) s. Pages, tables, slots and plans are those of the 8-bit cache.
+ *
+ * qspec_kv4_append: as qspec_kv8_append; with hadamard != 0 rotated queries and keys are multiplied by the Hadamard matrix of D / sqrt(D) besides (both, so that their
+ * products stay what they are, and channels that are large in all keys are spread over a row; butterflies of strides 1, 2 .. D / 2 in float32). Of a row of keys or values:
+ * hi = max(largest, 0), lo = min(smallest, 0) of its finite values, which count as +-2^126 beyond that; s = max((hi - lo) / 15, 2^-60) rounded to five significant bits,
+ * halves up; z = rint(-lo / s) (15 at most); c = clamp(rint(x / s) + z, 0, 15) (infinities: 15 and 0; NaN counts as 0). Rows do not depend on one another; tokens without a slot, or
+ * with a position that the table of angles does not have, are skipped. The slots of a call differ from each other. */
+int qspec_kv4_append(const void* qkv, long long ld, const void* cos_sin, int cos_rows, const int* positions, const int* slots, void* k, void* v, void* k_word, void* v_word,
+                     void* q_out, long long q_tok_stride, int ntok, int H, int G, int D, int npages, int page_tokens, int hadamard, int dtype, void* stream);
+
+/* Rows of the cache in 16 bits: k_out, v_out [rows, G, D] of slots[0 .. rows). A slot outside the cache gives zeros. */
+int qspec_kv4_read(const void* k, const void* v, const void* k_word, const void* v_word, const int* slots, void* k_out, void* v_out, int rows, int G, int D, int npages,
+                   int page_tokens, int dtype, void* stream);
+
+/* Softmax attention over that cache: as qspec_kv8_attention. Pages outside the cache, and scales that are infinite or no number, make the rows that see their keys NaN, and no
+ * others; a scale below 2^-100 counts as that. */
+size_t qspec_kv4_attention_workspace_bytes(void);
+int qspec_kv4_attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const void* k_word, const void* v_word, const int* table,
+                        const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H, int G, int D,
+                        int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Verification of drafted tokens, and one token more. drafted int64 [requests, drafts]; draft / target float32 probabilities, row of (request b, place i) at
  * b * seq_stride + i * place_stride, `drafts` and drafts + 1 places; uniform float32 [requests, drafts + 1] in [0, 1); draft_counts (NULL: all) int32: how
  * many drafts a request has. Draft i is taken if uniform[b, i] * q_i(d_i) < p_i(d_i) (exactly) and all before it were. Then one token by inversion with

@@ -497,6 +497,18 @@ int qspec_seq_glu(const void* gu, int ld, void* out, int ntok, int F, int act, i
 int qspec_seq_argmax_rows(const void* logits, int rows, int V, long long row_stride, long long* out_idx, int dtype,
                           void* stream);
 
+/* Log probabilities under softmax(logits / temperature), logits [rows, V] float16 / bfloat16 / float32 (row_stride >= V elements). tokens [rows] int64, or NULL (logprobs and ranks
+ * are then NULL as well). Any of the results may be NULL:
+ *   logprobs [rows]: of the given tokens; 0 where the token is negative (there is none), minus infinity where it is not in the vocabulary
+ *   ranks [rows] int64: 1 + how many logits are larger than the token's; 0 where there is no token, or none of the vocabulary
+ *   entropy [rows]: - sum p ln p, in nats
+ *   top_logprobs, top_tokens [rows, top]: the largest log probabilities and their tokens (int64), equal ones by the lower token; top <= 32 (and <= V)
+ * Rows that hold NaN or plus infinity have no log probabilities and no entropy (NaN); their best tokens are the largest logits all the same, NaN before all others. A row of
+ * minus infinities alone gives minus infinity, and an entropy of 0. Results lie over nothing else of the call. */
+int qspec_seq_token_logprobs_max_top(void);
+int qspec_seq_token_logprobs(const void* logits, long long row_stride, const long long* tokens, float* logprobs, float* entropy, long long* ranks, float* top_logprobs,
+                             long long* top_tokens, int rows, int V, int top, float temperature, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

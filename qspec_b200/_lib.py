@@ -100,6 +100,11 @@ SIGNATURES = {
                                     c_void_p]),
     "qspec_debug_kv8_attention_give_up": (c_int, [c_void_p, ctypes.c_longlong, c_int] + [c_void_p] * 8 + [ctypes.c_longlong] + [c_int] * 10 + [c_float, c_int, c_void_p,
                                                   ctypes.c_size_t, ctypes.c_uint, c_void_p]),
+    "qspec_kv4_append": (c_int, [c_void_p, ctypes.c_longlong, c_void_p, c_int] + [c_void_p] * 7 + [ctypes.c_longlong] + [c_int] * 8 + [c_void_p]),
+    "qspec_kv4_read": (c_int, [c_void_p] * 7 + [c_int] * 6 + [c_void_p]),
+    "qspec_kv4_attention_workspace_bytes": (ctypes.c_size_t, []),
+    "qspec_kv4_attention": (c_int, [c_void_p, ctypes.c_longlong, c_int] + [c_void_p] * 8 + [ctypes.c_longlong] + [c_int] * 10 + [c_float, c_int, c_void_p, ctypes.c_size_t,
+                                                                                                                           c_void_p]),
     "qspec_verify_drafts_max_drafts": (c_int, []),
     "qspec_verify_drafts": (c_int, [c_void_p, c_void_p, ctypes.c_longlong, ctypes.c_longlong, c_void_p, ctypes.c_longlong, ctypes.c_longlong] + [c_void_p] * 4 +
                             [c_int] * 3 + [c_void_p]),
@@ -138,6 +143,8 @@ SEQ_SIGNATURES = {
     "qspec_moe_route": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "qspec_moe_expert_tokens": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                         c_float, c_int, c_void_p]),
+    "qspec_seq_token_logprobs_max_top": (c_int, []),
+    "qspec_seq_token_logprobs": (c_int, [c_void_p, c_ll] + [c_void_p] * 6 + [c_int] * 3 + [c_float, c_int, c_void_p]),
     "qspec_seq_argmax_rows": (c_int, [c_void_p, c_int, c_int, c_ll, c_void_p, c_int, c_void_p]),
     "qspec_seq_chunk_attention_mma_supported": (c_int, [c_int, c_int, c_int, c_int]),
     "qspec_seq_chunk_attention_mma": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,

@@ -15,11 +15,11 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_C")
 LIB_PATH = os.path.join(OUT_DIR, "libqspec_b200.so")
 SOURCES = ["capi.cu", "act_kernels.cu", "hadamard_kernels.cu", "gemm_w4_stream.cu", "attn_kernels.cu", "qwen_kernels.cu", "kv8_kernels.cu",
-           "kv8_attention.cu", "kv8_prompt.cu", "spec_kernels.cu"]
+           "kv8_attention.cu", "kv8_prompt.cu", "kv4_kernels.cu", "kv4_attention.cu", "spec_kernels.cu"]
 # The sequence-mixer kernels (include/qspec_b200_seq.h) are a library of their own, so that a model that needs only them
 # builds only them: libqspec_b200_seq.so.
 SEQ_SOURCES = ["capi.cu", "seq_kernels.cu", "seq_mma_kernels.cu", "seq_mix_kernels.cu", "seq_state_kernels.cu", "seq_head_kernels.cu",
-               "seq_scan_kernels.cu"]
+               "seq_scan_kernels.cu", "seq_logprob_kernels.cu"]
 SEQ_LIB_PATH = os.path.join(OUT_DIR, "libqspec_b200_seq.so")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default"]
@@ -33,7 +33,7 @@ def _nvcc() -> str:
 
 
 def _newest_source_mtime(sources=None) -> float:
-    names = [f for f in os.listdir(CSRC) if f != "fast_call.cpp"] if sources is None else list(sources) + ["common.cuh", "seq_common.cuh", "attn_tile.cuh", "gemm_w4_rows.cuh", "recurrence_mma.cuh", "smem_limit.h", "kv8_common.cuh"]
+    names = [f for f in os.listdir(CSRC) if f != "fast_call.cpp"] if sources is None else list(sources) + ["common.cuh", "seq_common.cuh", "attn_tile.cuh", "gemm_w4_rows.cuh", "recurrence_mma.cuh", "smem_limit.h", "kv8_common.cuh", "kv4_common.cuh", "kv_stretch.cuh"]
     paths = [os.path.join(CSRC, f) for f in names]
     paths.append(os.path.join(HERE, "..", "include", "qspec_b200.h"))
     paths.append(os.path.join(HERE, "..", "include", "qspec_b200_seq.h"))
@@ -84,7 +84,7 @@ def build_fast(force: bool = False) -> str:
     """The linear layers' call path (csrc/fast_call.cpp), against the headers of the torch that is installed."""
     src, path = os.path.join(CSRC, "fast_call.cpp"), fast_path()
     os.makedirs(OUT_DIR, exist_ok=True)
-    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(HERE, "..", "include", "qspec_b200.h")))
+    newest = max(os.path.getmtime(p) for p in (src, os.path.join(HERE, "..", "include", "qspec_b200.h"), os.path.join(HERE, "..", "include", "qspec_b200_seq.h")))
     if not force and os.path.exists(path) and os.path.getmtime(path) >= newest:
         return path
     import sysconfig

@@ -1,4 +1,4 @@
-// The call path in native code of the linear layers and of the operators around the paged 8-bit cache: checks and one C call, for a product of a few microseconds that a Python path of ten would hide.
+// The call path in native code of the linear layers, of the operators around the paged caches and of the log probabilities of tokens: checks and one C call, for a product of a few microseconds that a Python path of ten would hide.
 // Takes exactly the calls that the Python functions in ops.py take without an error; everything else (another type or layout, sizes that do not
 // match, an empty batch, a workspace that is missing or too small) it leaves to them: returns None, nothing launched.
 // 4 tokens, 4096 x 4096, W4A4, through nn.Linear4bit in a row of calls: 11.1 -> 6.3 us (the kernel 2.7).
@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include "../../include/qspec_b200.h"
+#include "../../include/qspec_b200_seq.h"
 
 namespace {
 
@@ -94,7 +95,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
 }
 
-// ---- the paged 8-bit cache and the verification of drafts -----------------------------------------------------------------------------
+// ---- the paged caches, the verification of drafts, log probabilities -----------------------------------------------------------------------------
 // The same bargain: what ops.py takes without an error, on the current device.
 // Host time of a call: page_plan 15.1 -> 5.3 us, kv8_append 11.4 -> 5.0, kv8_attention 16.5 -> 3.9, verify_drafts 10.7 -> 3.9 (the kernels 3 to 12 at the
 // smallest sizes).
@@ -243,6 +244,135 @@ PyObject* kv8_attention(PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// The cache in 4 bits: codes [pages, G, P, D / 2], words [pages, G, P].
+struct Cache4 {
+  const at::Tensor *k, *v, *kw, *vw;
+  int64_t pages, G, P, D;
+  bool take(PyObject* const* a, c10::DeviceIndex device) {
+    k = on_device(a[0], device), v = on_device(a[1], device), kw = on_device(a[2], device), vw = on_device(a[3], device);
+    if (!k || !v || k->dim() != 4) return false;
+    pages = k->size(0), G = k->size(1), P = k->size(2), D = 2 * k->size(3);
+    return is(k, at::kByte, {pages, G, P, D / 2}) && is(v, at::kByte, {pages, G, P, D / 2}) && is(kw, at::kShort, {pages, G, P}) && is(vw, at::kShort, {pages, G, P}) && fits(pages) &&
+           fits(G) && fits(P) && fits(D);
+  }
+  void *kp() const { return k->mutable_data_ptr(); }
+  void *vp() const { return v->mutable_data_ptr(); }
+  void *kwp() const { return kw->mutable_data_ptr(); }
+  void *vwp() const { return vw->mutable_data_ptr(); }
+};
+
+// kv4_append(address, qkv, cos_sin_cache, positions, slots, k_codes, v_codes, k_words, v_words, q_out, hadamard)
+PyObject* kv4_append(PyObject* const* a, Py_ssize_t n) {
+  QSPEC_NOT_HERE(n != 11 || !PyBool_Check(a[10]));
+  const auto device = c10::cuda::current_device();
+  const at::Tensor *qkv = on_device(a[1], device), *cs = on_device(a[2], device), *pos = on_device(a[3], device), *slots = on_device(a[4], device), *q = nullptr;
+  Cache4 c;
+  QSPEC_NOT_HERE(!qkv || !cs || !c.take(a + 5, device) || qkv->dim() != 2 || qkv->stride(1) != 1 || element(qkv->scalar_type()) < 0 || c.D < 1);
+  const int64_t T = qkv->size(0), H = qkv->size(1) / c.D - 2 * c.G;
+  QSPEC_NOT_HERE(!fits(T) || H < 1 || !fits(H) || qkv->size(1) % c.D || cs->dim() != 2 || !fits(cs->size(0)) || !is(cs, qkv->scalar_type(), {cs->size(0), c.D}) ||
+                 !is(pos, at::kInt, {T}) || !is(slots, at::kInt, {T}));
+  if (a[9] != Py_None) {
+    q = on_device(a[9], device);
+    QSPEC_NOT_HERE(!q || q->scalar_type() != qkv->scalar_type() || q->sizes() != at::IntArrayRef({T, H, c.D}) || q->stride(2) != 1 || q->stride(1) != c.D);
+  }
+  const auto fn = (decltype(&qspec_kv4_append))PyLong_AsVoidPtr(a[0]);
+  if (PyErr_Occurred()) return nullptr;
+  QSPEC_NOT_HERE(!fn);
+  const int hadamard = a[10] == Py_True;
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  const void *x = qkv->const_data_ptr(), *table = cs->const_data_ptr();
+  const int *pp = (const int*)pos->const_data_ptr(), *sp = (const int*)slots->const_data_ptr();
+  void* out = q ? q->mutable_data_ptr() : nullptr;
+  return called([&] {
+    return fn(x, qkv->stride(0), table, (int)cs->size(0), pp, sp, c.kp(), c.vp(), c.kwp(), c.vwp(), out, q ? q->stride(0) : 0, (int)T, (int)H, (int)c.G, (int)c.D, (int)c.pages,
+              (int)c.P, hadamard, element(qkv->scalar_type()), stream);
+  });
+}
+
+// kv4_read(address, k_codes, v_codes, k_words, v_words, slots, k_out, v_out)
+PyObject* kv4_read(PyObject* const* a, Py_ssize_t n) {
+  QSPEC_NOT_HERE(n != 8);
+  const auto device = c10::cuda::current_device();
+  const at::Tensor *slots = on_device(a[5], device), *ko = on_device(a[6], device), *vo = on_device(a[7], device);
+  Cache4 c;
+  QSPEC_NOT_HERE(!slots || !ko || !c.take(a + 1, device));
+  const int64_t N = slots->numel();
+  const auto type = ko->scalar_type();
+  QSPEC_NOT_HERE(!fits(N) || element(type) < 0 || !is(slots, at::kInt, {N}) || !is(ko, type, {N, c.G, c.D}) || !is(vo, type, {N, c.G, c.D}));
+  const auto fn = (decltype(&qspec_kv4_read))PyLong_AsVoidPtr(a[0]);
+  if (PyErr_Occurred()) return nullptr;
+  QSPEC_NOT_HERE(!fn);
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  const int* sp = (const int*)slots->const_data_ptr();
+  void *kp = ko->mutable_data_ptr(), *vp = vo->mutable_data_ptr();
+  return called([&] { return fn(c.kp(), c.vp(), c.kwp(), c.vwp(), sp, kp, vp, (int)N, (int)c.G, (int)c.D, (int)c.pages, (int)c.P, element(type), stream); });
+}
+
+// kv4_attention(address, q, k_codes, v_codes, k_words, v_words, table, q_start, kv_len, out, scale, workspace, max_tokens)
+PyObject* kv4_attention(PyObject* const* a, Py_ssize_t n) {
+  QSPEC_NOT_HERE(n != 13 || !PyFloat_Check(a[10]) || !(a[12] == Py_None || PyLong_Check(a[12])));
+  const auto device = c10::cuda::current_device();
+  const at::Tensor *q = on_device(a[1], device), *table = on_device(a[6], device), *start = on_device(a[7], device), *lens = on_device(a[8], device), *out = on_device(a[9], device),
+                   *work = on_device(a[11], device);
+  Cache4 c;
+  QSPEC_NOT_HERE(!q || !table || !out || !work || !c.take(a + 2, device) || q->dim() != 3 || table->dim() != 2);
+  const int64_t T = q->size(0), H = q->size(1), B = table->size(0), W = table->size(1);
+  const auto type = q->scalar_type();
+  QSPEC_NOT_HERE(element(type) < 0 || q->size(2) != c.D || q->stride(2) != 1 || out->scalar_type() != type || out->sizes() != q->sizes() || out->stride(2) != 1 || !fits(T) || T < 1 ||
+                 !fits(H) || !fits(B) || !fits(W) || !fits(q->stride(1)) || !fits(out->stride(1)) || !is(table, at::kInt, {B, W}) || !is(start, at::kInt, {B + 1}) ||
+                 !is(lens, at::kInt, {B}) || work->scalar_type() != at::kByte || !work->is_contiguous());
+  const auto fn = (decltype(&qspec_kv4_attention))PyLong_AsVoidPtr(a[0]);
+  const double scale = PyFloat_AsDouble(a[10]);
+  const long most = a[12] == Py_None ? (long)T : PyLong_AsLong(a[12]);
+  if (PyErr_Occurred()) return nullptr;
+  QSPEC_NOT_HERE(!fn || !(scale > 0));
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  const void* qp = q->const_data_ptr();
+  const int *tp = (const int*)table->const_data_ptr(), *sp = (const int*)start->const_data_ptr(), *lp = (const int*)lens->const_data_ptr();
+  void *op = out->mutable_data_ptr(), *wp = work->mutable_data_ptr();
+  return called([&] {
+    return fn(qp, q->stride(0), (int)q->stride(1), c.kp(), c.vp(), c.kwp(), c.vwp(), tp, sp, lp, op, out->stride(0), (int)out->stride(1), (int)T, (int)B, (int)W, (int)H, (int)c.G,
+              (int)c.D, (int)c.pages, (int)c.P, (int)(most < T ? most : T), (float)scale, element(type), wp, work->nbytes(), stream);
+  });
+}
+
+// seq_token_logprobs(address, logits, tokens, logprobs, entropy, ranks, top_logprobs, top_tokens, temperature)
+PyObject* seq_token_logprobs(PyObject* const* a, Py_ssize_t n) {
+  QSPEC_NOT_HERE(n != 9 || !PyFloat_Check(a[8]));
+  const auto device = c10::cuda::current_device();
+  const at::Tensor* x = on_device(a[1], device);
+  QSPEC_NOT_HERE(!x || x->dim() != 2 || x->size(0) < 1 || x->size(1) < 1 || (x->stride(1) != 1 && x->size(1) > 1));
+  const auto type = x->scalar_type();
+  const int64_t rows = x->size(0), V = x->size(1), stride = rows > 1 ? x->stride(0) : std::max(x->stride(0), V);
+  const int dtype = type == at::kFloat ? QSPEC_DTYPE_F32 : element(type);
+  const at::Tensor* t[8] = {};
+  for (int i = 2; i < 8; ++i)
+    if (a[i] != Py_None) QSPEC_NOT_HERE(!(t[i] = on_device(a[i], device)) || !t[i]->is_contiguous());
+  const int64_t top = t[6] && t[6]->dim() == 2 ? t[6]->size(1) : 0;
+  QSPEC_NOT_HERE(dtype < 0 || !fits(rows) || !fits(V) || !fits(top) || (t[2] && !is(t[2], at::kLong, {rows})) || (t[3] && !is(t[3], at::kFloat, {rows})) ||
+                 (t[4] && !is(t[4], at::kFloat, {rows})) || (t[5] && !is(t[5], at::kLong, {rows})) || (t[6] && !is(t[6], at::kFloat, {rows, top})) ||
+                 (t[7] && !is(t[7], at::kLong, {rows, top})) || (!t[2] && (t[3] || t[5])) || !t[6] != !t[7]);
+  const char* begin = (const char*)x->const_data_ptr();
+  const char* end = begin + ((rows - 1) * stride + V) * x->element_size();
+  for (int i = 3; i < 8; ++i) {
+    if (!t[i] || !t[i]->numel()) continue;
+    for (int j = 2; j < i; ++j) QSPEC_NOT_HERE(t[j] && t[j]->numel() && overlap(*t[i], *t[j]));
+    const char* p = (const char*)t[i]->const_data_ptr();
+    QSPEC_NOT_HERE(p < end && begin < p + t[i]->nbytes());
+  }
+  const auto fn = (decltype(&qspec_seq_token_logprobs))PyLong_AsVoidPtr(a[0]);
+  const double temperature = PyFloat_AsDouble(a[8]);
+  if (PyErr_Occurred()) return nullptr;
+  QSPEC_NOT_HERE(!fn || !(temperature > 0));
+  void* stream = c10::cuda::getCurrentCUDAStream().stream();
+  void* p[8] = {};
+  for (int i = 2; i < 8; ++i) p[i] = t[i] && t[i]->numel() ? t[i]->mutable_data_ptr() : nullptr;
+  return called([&] {
+    return fn(begin, stride, (const long long*)p[2], (float*)p[3], (float*)p[4], (long long*)p[5], (float*)p[6], (long long*)p[7], (int)rows, (int)V, (int)top, (float)temperature, dtype,
+              stream);
+  });
+}
+
 // verify_drafts(address, drafted, draft_probs, target_probs, uniform, tokens, emitted, draft_counts)
 PyObject* verify_drafts(PyObject* const* a, Py_ssize_t n) {
   QSPEC_NOT_HERE(n != 8);
@@ -277,7 +407,8 @@ PyObject* verify_drafts(PyObject* const* a, Py_ssize_t n) {
 
 #define QSPEC_METHOD(name) {#name, (PyCFunction)(void (*)(void))guarded<name>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, nullptr}, QSPEC_METHOD(page_plan), QSPEC_METHOD(kv8_append), QSPEC_METHOD(kv8_read),
-                         QSPEC_METHOD(kv8_attention), QSPEC_METHOD(verify_drafts), {nullptr, nullptr, 0, nullptr}};
+                         QSPEC_METHOD(kv8_attention), QSPEC_METHOD(kv4_append), QSPEC_METHOD(kv4_read),
+                         QSPEC_METHOD(kv4_attention), QSPEC_METHOD(seq_token_logprobs), QSPEC_METHOD(verify_drafts), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,436 @@
+// Log probabilities: of each row x of logits, with the temperature T and c = log2(e) / T,
+//   y_i = c (x_i - max x),   S = sum 2^y_i,   U = sum 2^y_i y_i
+// the given token's log probability ln2 (y_t - log2 S), its rank 1 + #{i: x_i > x_t}, the entropy ln2 (log2 S - U / S), and the `top` largest log probabilities with their
+// tokens, equal ones by the lower token.
+//
+// What bounds it is reading the row, once, and the exponentials. One CTA, or a cluster of up to eight, takes a row; a CTA walks its span in batches of 1024 vectors of 16 bytes, the
+// next batch's loads under way. The first batch's maximum is where exponents are counted from; only if a value is 2^60 above it the sums are multiplied again. Candidates for
+// the best are, of the first batch, the values that reach the smallest of as many groups' maxima as are asked for, or more (at least that many do, and hardly more than some
+// hundred), and later on those above the worst of the best so far, which is brought up to date whenever four times as much has been seen: a few at a time. Where there are more than there
+// is room for (rows that rise, rows of one value), the span is looked through once for each one that is asked for. Whichever way, values are ordered together with their
+// tokens as whole numbers of 64 bits, so that there is one result. Sums are made in a fixed order in float32.
+#include "seq_common.cuh"
+#include "../../include/qspec_b200_seq.h"
+#include <algorithm>
+
+namespace qspec {
+namespace logprob {
+
+constexpr int THREADS = 256, WARPS = THREADS / 32, MOST_TOP = 32, CANDIDATES = 512, EACH = 4;   // EACH: vectors of a thread in a batch
+constexpr float AHEAD = 60.f;                     // a value 2^AHEAD above the reference moves it
+typedef unsigned long long u64;
+
+struct Args {
+  const void* logits; long long stride;
+  const long long* tokens;
+  float *logprobs, *entropy; long long* ranks;
+  float* top_logprobs; long long* top_tokens;
+  int V, span, top;                               // span: values of a CTA
+  float c;
+};
+struct Partial {                                  // of a span: what its exponents are counted from, sums, values above the given token's, how many of the best there are
+  float ref, S, U;
+  int above, best;
+};
+
+template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
+__device__ __forceinline__ float value(float x) { return x; }
+__device__ __forceinline__ float value(__half x) { return __half2float(x); }
+__device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T lowest();   // minus infinity
+template <> __device__ __forceinline__ float lowest<float>() { return -INFINITY; }
+template <> __device__ __forceinline__ __half lowest<__half>() { return __ushort_as_half(0xfc00); }
+template <> __device__ __forceinline__ __nv_bfloat16 lowest<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ u64 add2(u64 a, u64 b) { u64 r; asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) { u64 r; asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
+// A vector's values: the largest (no number if one is none), all of them, how many are above `given`.
+template <typename T> struct Lanes;
+template <> struct Lanes<float> {
+  static __device__ __forceinline__ float largest(const uint4& w) {
+    return max_nan(max_nan(__uint_as_float(w.x), __uint_as_float(w.y)), max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  static __device__ __forceinline__ void values(const uint4& w, float (&x)[4]) {
+    x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
+  }
+  static __device__ __forceinline__ int above(const uint4& w, float given) {
+    return (__uint_as_float(w.x) > given) + (__uint_as_float(w.y) > given) + (__uint_as_float(w.z) > given) + (__uint_as_float(w.w) > given);
+  }
+};
+#define QSPEC_LANES16(T, T2, SUFFIX, UNPACK, FROM)                                                                                                               \
+  template <> struct Lanes<T> {                                                                                                                                  \
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { uint32_t r; asm("max.NaN." SUFFIX " %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b)); return r; } \
+    static __device__ __forceinline__ float largest(const uint4& w) {                                                                                            \
+      const uint32_t m = max2(max2(w.x, w.y), max2(w.z, w.w));                                                                                                   \
+      const T2 h = *reinterpret_cast<const T2*>(&m);                                                                                                             \
+      return max_nan(value(h.x), value(h.y));                                                                                                                    \
+    }                                                                                                                                                            \
+    static __device__ __forceinline__ void values(const uint4& w, float (&x)[8]) { UNPACK(w, x); }                                                                \
+    static __device__ __forceinline__ int above(const uint4& w, float given) {   /* (given is one of the row's values: exact) */                                 \
+      const T2 g = FROM(given);                                                                                                                                  \
+      const T2* h = reinterpret_cast<const T2*>(&w);                                                                                                             \
+      const T2 n = __hadd2(__hadd2(__hgt2(h[0], g), __hgt2(h[1], g)), __hadd2(__hgt2(h[2], g), __hgt2(h[3], g)));                                                \
+      return (int)(value(n.x) + value(n.y));                                                                                                                     \
+    }                                                                                                                                                            \
+  };
+QSPEC_LANES16(__half, __half2, "f16x2", unpack_h8, __float2half2_rn)
+QSPEC_LANES16(__nv_bfloat16, __nv_bfloat162, "bf16x2", unpack_b8, __float2bfloat162_rn)
+#undef QSPEC_LANES16
+
+// Larger values first, no numbers before all, equal ones by the lower index; never 0.
+__device__ __forceinline__ u64 key_of(float x, int index) {
+  const uint32_t u = __float_as_uint(x + 0.f);              // (-0 is 0)
+  const uint32_t v = x != x ? 0xffffffffu : u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (u64)v << 32 | (uint32_t)~index;
+}
+__device__ __forceinline__ float value_of(u64 key) {
+  const uint32_t v = (uint32_t)(key >> 32);
+  return v == 0xffffffffu ? NAN : __uint_as_float(v & 0x80000000u ? v ^ 0x80000000u : ~v);
+}
+__device__ __forceinline__ int index_of(u64 key) { return (int)~(uint32_t)key; }
+
+// The n best of the keys s_key[0 .. count) in their order to s_best, and back to the begin of s_key. All threads of the CTA call it, with everything written.
+__device__ __forceinline__ int select(u64* s_key, u64* s_best, int count, int n) {
+  for (int i = threadIdx.x; i < count; i += THREADS) {
+    const u64 key = s_key[i];
+    int larger = 0;
+    for (int j = 0; j < count; ++j) larger += s_key[j] > key;
+    if (larger < n) s_best[larger] = key;
+  }
+  __syncthreads();
+  const int best = min(count, n);
+  if (threadIdx.x < best) s_key[threadIdx.x] = s_best[threadIdx.x];
+  return best;
+}
+
+template <typename T, int CLUSTER>
+__global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a) {
+  constexpr int E = Vec<T>::N;
+  using L = Lanes<T>;
+  __shared__ Partial s_part;
+  __shared__ u64 s_best[MOST_TOP], s_key[CANDIDATES], s_most[WARPS];
+  __shared__ float s_max[WARPS], s_low[WARPS], s_ref[WARPS], s_sum[2][WARPS];
+  __shared__ int s_above[WARPS], s_count;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
+  if (tid == 0) s_count = 0;
+  pdl_enter();
+  const T* const x_row = (const T*)a.logits + (size_t)row * a.stride;
+  const int lo = min(rank * a.span, a.V), n = min(a.span, a.V - lo);
+  const T* const from = x_row + lo;
+  // Vectors lie on 16-byte boundaries, the first and the last may lie over the span's ends: what stands there is minus infinity instead.
+  const int shift = (int)(((uintptr_t)from & 15) / sizeof(T)), vectors = n > 0 ? (n + shift + E - 1) / E : 0;
+  auto load = [&](int v) {
+    const int first = v * E - shift;
+    uint4 w;
+    if (first >= 0 && first + E <= n) {
+      w = __ldg(reinterpret_cast<const uint4*>(from + first));
+    } else {
+      T* const x = reinterpret_cast<T*>(&w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = first + e >= 0 && first + e < n ? from[first + e] : lowest<T>();
+    }
+    return w;
+  };
+  const int batches = (vectors + THREADS * EACH - 1) / (THREADS * EACH);
+  uint4 next[EACH];
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) next[j] = load(j * THREADS + tid);
+  const long long token = a.tokens ? a.tokens[row] : -1;
+  const bool there = token >= 0 && token < a.V;
+  const float given = there ? value(x_row[token]) : INFINITY;   // (nothing is above it)
+
+  float ref = -INFINITY, reach = INFINITY;                  // what exponents are counted from; what a candidate has to reach (of the first batch) or to exceed
+  bool none = true;                                         // nothing but minus infinity so far: there is nothing to count from
+  float limit = -INFINITY;                                  // what a value that is looked at more closely reaches
+  auto set_limit = [&]() { limit = none ? -INFINITY : fminf(reach, ref + AHEAD / a.c); };
+  u64 S2 = 0, U2 = 0;
+  int above = 0, best = 0, check = 0;                       // check: the batch behind which the best are brought up to date
+  bool odd = false;                                         // there is something that is no number
+  for (int b = 0; b < batches; ++b) {
+    uint4 w[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) w[j] = next[j];
+    if (b + 1 < batches) {
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) next[j] = load(((b + 1) * EACH + j) * THREADS + tid);
+    }
+    float big[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) big[j] = L::largest(w[j]);
+    if (b == 0) {
+      // ---- the first batch's maximum, and what the best have to reach: maxima of groups of eight lanes, or, of up to eight, those of the warps
+      float g = max_nan(max_nan(big[0], big[1]), max_nan(big[2], big[3]));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
+      float low = g;
+#pragma unroll
+      for (int o = 8; o < 32; o <<= 1) {
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+        g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
+      }
+      if (lane == 0) {
+        s_max[warp] = g;
+        s_low[warp] = a.top > WARPS ? low : g;
+      }
+      __syncthreads();
+      ref = s_max[0];
+      reach = s_low[0];
+#pragma unroll
+      for (int i = 1; i < WARPS; ++i) {
+        ref = max_nan(ref, s_max[i]);
+        reach = fminf(reach, s_low[i]);
+      }
+      if (!a.top) reach = INFINITY;
+      none = ref == -INFINITY;
+      if (none) ref = 0.f;                                  // (weights of minus infinity are zero wherever they are counted from)
+      set_limit();
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      if (!(big[j] < limit)) {                              // seldom: candidates, a value far above all before it, no numbers
+        odd |= big[j] != big[j];
+        if (none ? big[j] > -INFINITY : big[j] > ref + AHEAD / a.c) {
+          const float d = fmaxf((ref - big[j]) * a.c, -16384.f), f = none ? 0.f : ex2(d);
+          const float2 S = unpack_f2(S2), U = unpack_f2(U2);
+          U2 = pack_f2(fmaf(S.x, d, U.x) * f, fmaf(S.y, d, U.y) * f);
+          S2 = pack_f2(S.x * f, S.y * f);
+          ref = big[j];
+          none = false;
+          set_limit();
+        }
+        if (b == 0 ? big[j] >= reach : big[j] > reach) {
+          const int first = ((b * EACH + j) * THREADS + tid) * E - shift;
+          const T* const x = reinterpret_cast<const T*>(&w[j]);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float y = value(x[e]);
+            const int i = first + e;
+            if ((b == 0 ? y >= reach : y > reach) && i >= 0 && i < n) {
+              const int at = atomicAdd(&s_count, 1);        // (in any order: they are put in theirs)
+              if (at < CANDIDATES) s_key[at] = key_of(y, lo + i);
+            }
+          }
+        }
+      }
+      float x[E];
+      L::values(w[j], x);
+      const u64 minus = pack_f2(-ref, -ref), c2 = pack_f2(a.c, a.c);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        float2 y = unpack_f2(mul2(add2(pack_f2(x[e], x[e + 1]), minus), c2));
+        y = make_float2(max_nan(y.x, -16384.f), max_nan(y.y, -16384.f));   // (a weight of zero times minus infinity is no number)
+        const u64 y2 = pack_f2(y.x, y.y);
+        const u64 w2 = pack_f2(ex2(y.x), ex2(y.y));
+        S2 = add2(S2, w2);
+        U2 = ffma2_rn(w2, y2, U2);
+      }
+      if (a.ranks) above += L::above(w[j], given);
+    }
+    if (a.top && (b == check || b + 1 == batches)) {
+      check = 4 * b + 3;
+      __syncthreads();
+      const int count = s_count;
+      if (count <= CANDIDATES) {                            // (the same for all)
+        best = select(s_key, s_best, count, a.top);
+        __syncthreads();
+        if (tid == 0) s_count = best;
+        if (best == a.top) reach = value_of(s_best[best - 1]);
+        __syncthreads();
+      } else {
+        reach = INFINITY;                                   // too many: all of them are looked for at the end
+      }
+      set_limit();
+    }
+  }
+  // ---- the threads' sums together
+  float m = none ? -INFINITY : ref;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) s_ref[warp] = m;
+  odd = __syncthreads_or(odd);
+  m = s_ref[0];
+#pragma unroll
+  for (int i = 1; i < WARPS; ++i) m = max_nan(m, s_ref[i]);
+  float S, U;
+  {
+    const float2 s = unpack_f2(S2), u = unpack_f2(U2);
+    const float d = fmaxf((ref - m) * a.c, -16384.f), f = none ? 0.f : ref == m ? 1.f : ex2(d);
+    S = (s.x + s.y) * f;
+    U = ref == m ? u.x + u.y : none ? 0.f : fmaf(s.x + s.y, d, u.x + u.y) * f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    S += __shfl_xor_sync(0xffffffffu, S, o);
+    U += __shfl_xor_sync(0xffffffffu, U, o);
+  }
+  above = __reduce_add_sync(0xffffffffu, above);
+  if (lane == 0) { s_sum[0][warp] = S; s_sum[1][warp] = U; s_above[warp] = above; }
+  if (a.top && (odd || s_count > CANDIDATES)) {             // (the same for all: the barrier above)
+    u64 before = ~0ull;                                     // (no key is that large)
+    for (best = 0; best < a.top; ++best) {
+      u64 most = 0;
+      for (int v = tid; v < vectors; v += THREADS) {
+        const uint4 w = load(v);
+        const T* const x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int i = v * E - shift + e;
+          const u64 key = key_of(value(x[e]), lo + i);
+          if (i >= 0 && i < n && key < before && key > most) most = key;
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const u64 other = __shfl_xor_sync(0xffffffffu, most, o);
+        most = other > most ? other : most;
+      }
+      if (lane == 0) s_most[warp] = most;
+      __syncthreads();
+      most = s_most[0];
+#pragma unroll
+      for (int i = 1; i < WARPS; ++i) most = s_most[i] > most ? s_most[i] : most;
+      __syncthreads();
+      if (!most) break;
+      if (tid == 0) s_best[best] = most;
+      before = most;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    Partial p{m, 0.f, 0.f, 0, best};
+    for (int i = 0; i < WARPS; ++i) { p.S += s_sum[0][i]; p.U += s_sum[1][i]; p.above += s_above[i]; }
+    s_part = p;
+  }
+  if (CLUSTER > 1) cluster_sync_all(); else __syncthreads();
+
+  // ---- the first CTA joins the spans
+  if (rank == 0) {
+    Partial p[CLUSTER];
+    p[0] = s_part;
+    if (CLUSTER > 1) {
+#pragma unroll
+      for (int r = 1; r < CLUSTER; ++r) {
+        const uint32_t at = mapa_shared((uint32_t)__cvta_generic_to_shared(&s_part), r);
+        p[r].ref = __uint_as_float(ld_dsmem_u32(at));
+        p[r].S = __uint_as_float(ld_dsmem_u32(at + 4));
+        p[r].U = __uint_as_float(ld_dsmem_u32(at + 8));
+        p[r].above = (int)ld_dsmem_u32(at + 12);
+        p[r].best = (int)ld_dsmem_u32(at + 16);
+      }
+    }
+    float M = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < CLUSTER; ++r)
+      if (p[r].S != 0.f) M = max_nan(M, p[r].ref);          // (a span of minus infinities counts from nowhere)
+    S = U = 0.f;
+    above = 0;
+#pragma unroll
+    for (int r = 0; r < CLUSTER; ++r) {
+      above += p[r].above;
+      if (p[r].S == 0.f) continue;
+      const float d = fmaxf((p[r].ref - M) * a.c, -16384.f), f = p[r].ref == M ? 1.f : ex2(d);
+      S = fmaf(p[r].S, f, S);
+      U = fmaf(p[r].ref == M ? p[r].U : fmaf(p[r].S, d, p[r].U), f, U);
+    }
+    const float ln2 = 0.69314718055994531f, lse = log2f(S);
+    const bool nothing = M == -INFINITY;                    // no token has any probability
+    auto logprob = [&](float x) { return nothing ? -INFINITY : ((x - M) * a.c - lse) * ln2; };
+    if (tid == 0) {
+      if (a.logprobs) a.logprobs[row] = token < 0 ? 0.f : there ? logprob(given) : lse != lse ? NAN : -INFINITY;
+      if (a.ranks) a.ranks[row] = there ? 1 + above : 0;
+      if (a.entropy) a.entropy[row] = nothing ? 0.f : lse != lse ? NAN : fmaxf((lse - U / S) * ln2, 0.f);
+    }
+    if (a.top) {
+      int all = 0, mine = -1;                               // of the slices' best, one behind the other: how many, and which slice's this thread's is
+      int first[CLUSTER];
+#pragma unroll
+      for (int r = 0; r < CLUSTER; ++r) {
+        first[r] = all;
+        all += p[r].best;
+      }
+      __syncthreads();                                      // (candidates make room)
+#pragma unroll
+      for (int r = 0; r < CLUSTER; ++r)
+        if (tid >= first[r] && tid < first[r] + p[r].best) mine = r;
+      u64 key = 0;
+      if (mine >= 0) {
+        int skip = tid;
+#pragma unroll
+        for (int r = 0; r < CLUSTER; ++r)
+          if (r == mine) skip = tid - first[r];
+        if (CLUSTER > 1) {
+          const uint32_t at = mapa_shared((uint32_t)__cvta_generic_to_shared(s_best + skip), mine);
+          key = (u64)ld_dsmem_u32(at) | (u64)ld_dsmem_u32(at + 4) << 32;
+        } else {
+          key = s_best[skip];
+        }
+        s_key[tid] = key;
+      }
+      __syncthreads();
+      if (mine >= 0) {
+        int larger = 0;
+        for (int j = 0; j < all; ++j) larger += s_key[j] > key;
+        if (larger < a.top) {
+          a.top_logprobs[(size_t)row * a.top + larger] = logprob(value_of(key));
+          a.top_tokens[(size_t)row * a.top + larger] = index_of(key);
+        }
+      }
+    }
+  }
+  if (CLUSTER > 1) cluster_sync_all();                      // the first CTA has read the others' results
+}
+
+}  // namespace logprob
+}  // namespace qspec
+
+using namespace qspec;
+using namespace qspec::logprob;
+
+extern "C" int qspec_seq_token_logprobs_max_top(void) { return MOST_TOP; }
+
+extern "C" int qspec_seq_token_logprobs(const void* logits, long long row_stride, const long long* tokens, float* logprobs, float* entropy, long long* ranks, float* top_logprobs,
+                                        long long* top_tokens, int rows, int V, int top, float temperature, int dtype, void* stream) {
+  QSPEC_REQUIRE(rows >= 0 && V >= 1 && row_stride >= V, QSPEC_ERR_INVALID_ARG, "token_logprobs: rows=%d vocabulary=%d row stride=%lld", rows, V, row_stride);
+  QSPEC_REQUIRE(dtype == QSPEC_DTYPE_F16 || dtype == QSPEC_DTYPE_BF16 || dtype == QSPEC_DTYPE_F32, QSPEC_ERR_UNSUPPORTED, "token_logprobs: float16, bfloat16 or float32 logits");
+  QSPEC_REQUIRE(top >= 0 && top <= MOST_TOP && top <= V, QSPEC_ERR_UNSUPPORTED, "token_logprobs: the best 0 to %d of %d tokens, got %d", std::min(MOST_TOP, V), V, top);
+  const float c = 1.4426950408889634f / temperature;
+  QSPEC_REQUIRE(temperature > 0.f && c > 0.f && c < INFINITY, QSPEC_ERR_INVALID_ARG, "token_logprobs: the temperature must be positive and finite, got %g", (double)temperature);
+  if (rows == 0) return QSPEC_OK;
+  const int size = dtype == QSPEC_DTYPE_F32 ? 4 : 2;
+  QSPEC_REQUIRE(logits && (!top || (top_logprobs && top_tokens)) && (tokens || (!logprobs && !ranks)), QSPEC_ERR_INVALID_ARG, "token_logprobs: null pointer");
+  QSPEC_REQUIRE((uintptr_t)logits % size == 0 && ((uintptr_t)tokens & 7) == 0, QSPEC_ERR_INVALID_ARG, "token_logprobs: logits and tokens must lie on their types' boundaries");
+  // CTAs of a row
+  const int sms = std::max(sm_count(), 1), batch = THREADS * EACH * 16 / size;
+  int cluster = 1;
+  while (cluster < 8 && (long long)rows * cluster < 4ll * sms && V > cluster * batch) cluster *= 2;
+  const int span = ((V + cluster - 1) / cluster + 7) / 8 * 8;
+  QSPEC_REQUIRE(V <= (1 << 24), QSPEC_ERR_UNSUPPORTED, "token_logprobs: a vocabulary of %d is too large", V);
+  QSPEC_REQUIRE((long long)rows * cluster < (1ll << 31), QSPEC_ERR_UNSUPPORTED, "token_logprobs: %d rows are too many for one call", rows);
+  const Args a{logits, row_stride, tokens, logprobs, entropy, ranks, top_logprobs, top_tokens, V, span, top, c};
+  auto run = [&](auto kern) -> int {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * cluster));
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    QSPEC_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+    QSPEC_CHECK_LAUNCH(1);
+    return QSPEC_OK;
+  };
+#define QSPEC_LOGPROB(T)                                                                                                                                         \
+  (cluster == 8 ? run(token_logprobs_kernel<T, 8>) : cluster == 4 ? run(token_logprobs_kernel<T, 4>)                                                            \
+                                                                  : cluster == 2 ? run(token_logprobs_kernel<T, 2>) : run(token_logprobs_kernel<T, 1>))
+  return dtype == QSPEC_DTYPE_F32 ? QSPEC_LOGPROB(float) : dtype == QSPEC_DTYPE_BF16 ? QSPEC_LOGPROB(__nv_bfloat16) : QSPEC_LOGPROB(__half);
+#undef QSPEC_LOGPROB
+}

@@ -63,7 +63,7 @@ def _ptr(t: Optional[torch.Tensor]):
 
 _I4 = (torch.int8, torch.uint8)
 
-# csrc/fast_call.cpp: the calls of the linear layers and of the paged 8-bit cache's operators without the Python below them. It takes what the functions here take without an error and
+# csrc/fast_call.cpp: the calls of the linear layers and of the paged caches' operators without the Python below them. It takes what the functions here take without an error and
 # returns None for everything else, which then goes the ordinary way (and so does everything where it has not been built for this Python and torch).
 _fast = False                                             # loaded by the first call: False before it, None where there is none
 _addresses: dict = {}
@@ -87,7 +87,7 @@ def _load_fast():
 def _address(name: str) -> int:
     found = _addresses.get(name)
     if found is None:
-        lib = _lib.load()
+        lib = _lib.load_seq() if name.startswith("qspec_seq_") else _lib.load()
         found = ctypes.cast(getattr(lib, name), ctypes.c_void_p).value if isinstance(lib, ctypes.CDLL) else 0
         _addresses[name] = found
     return found
@@ -816,12 +816,18 @@ def _fast_call(name: str, *args) -> bool:
     if status is None:
         return False
     if status:
-        _lib.check(status, name)
+        _lib.check(status, name, _lib.load_seq() if name.startswith("seq_") else None)
     return True
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
+def _overlap_rows(a: torch.Tensor, rows: torch.Tensor) -> bool:
+    """`a` is contiguous, rows [n, V] may be strided: whether `a` lies over anything from the first row's begin to the last one's end."""
+    end = rows.data_ptr() + ((rows.shape[0] - 1) * rows.stride(0) + rows.shape[1]) * rows.element_size()
+    return a.data_ptr() < end and rows.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
 
 
 def page_plan(lengths: torch.Tensor, counts: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, state: torch.Tensor, page_tokens: int,
@@ -950,6 +956,108 @@ def kv8_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
     return out
 
 
+# ---- the same cache in 4 bits -------------------------------------------------------------------------------------------------------
+def _kv4_cache(k_codes: torch.Tensor, v_codes: torch.Tensor, k_words: torch.Tensor, v_words: torch.Tensor):
+    """(pages, heads, page tokens, head dim) of a 4-bit cache."""
+    _chk(k_codes, "k_codes", (torch.uint8,)); _chk(v_codes, "v_codes", (torch.uint8,))
+    _chk(k_words, "k_words", (torch.int16,)); _chk(v_words, "v_words", (torch.int16,))
+    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
+        raise ValueError(f"codes must be [pages, kv heads, page tokens, head dim / 2], keys and values alike: {tuple(k_codes.shape)}, {tuple(v_codes.shape)}")
+    if k_words.shape != k_codes.shape[:3] or v_words.shape != k_codes.shape[:3]:
+        raise ValueError(f"words must be [pages, kv heads, page tokens]: {tuple(k_words.shape)}, {tuple(v_words.shape)}")
+    return (*k_codes.shape[:3], 2 * k_codes.shape[3])
+
+
+def kv4_append(qkv: torch.Tensor, cos_sin_cache: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor,
+               k_words: torch.Tensor, v_words: torch.Tensor, q_out: Optional[torch.Tensor], hadamard: bool = False) -> None:
+    """Neox RoPE on queries and keys of qkv [T, (H + 2 G) D] (float16 / bfloat16; rows may be strided, left as they are) and the step's keys and values
+    into their slots: codes uint8 [pages, G, P, D / 2], two to a byte, and words int16 [pages, G, P], a row's scale and zero point (include/qspec_b200.h has their
+    bits; `kv4_read` gives the values back). hadamard: rotated queries and keys are multiplied by the Hadamard matrix / sqrt(D) as well, which leaves their products as they are
+    and keeps channels that are large in all keys from taking a row's few codes. q_out [T, H, D] receives the rotated queries (None: they are not
+    wanted); it may be qkv's own query columns, but lie over nothing else of the call. Every row has a scale of its own, so that no other rows change. Tokens without a slot
+    (negative), or with a position that the table of angles does not have, are skipped; the slots of a call differ from each other."""
+    if _fast_call("kv4_append", qkv, cos_sin_cache, positions, slots, k_codes, v_codes, k_words, v_words, q_out, hadamard):
+        return
+    n, G, P, D = _kv4_cache(k_codes, v_codes, k_words, v_words)
+    if not qkv.is_cuda or qkv.dtype not in (_F16, _BF16) or qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise ValueError("kv4_append: qkv must be a float16 / bfloat16 CUDA tensor [T, (H + 2 G) D] with unit column stride")
+    T = qkv.shape[0]
+    H = qkv.shape[1] // D - 2 * G if D else 0
+    if H < 1 or qkv.shape[1] % D:
+        raise ValueError(f"kv4_append: rows of {qkv.shape[1]} do not hold queries, {G} keys and {G} values of {D}")
+    _chk(cos_sin_cache, "cos_sin_cache", (qkv.dtype,))
+    if cos_sin_cache.dim() != 2 or cos_sin_cache.shape[1] != D:
+        raise ValueError(f"kv4_append: the rotary table must be [positions, {D}]")
+    _i32(positions, "positions", T); _i32(slots, "slots", T)
+    q_ts = 0
+    if q_out is not None:
+        if not q_out.is_cuda or q_out.dtype != qkv.dtype or q_out.shape != (T, H, D) or q_out.stride(2) != 1 or q_out.stride(1) != D:
+            raise ValueError(f"kv4_append: q_out must be {qkv.dtype} [{T}, {H}, {D}], heads side by side")
+        q_ts = q_out.stride(0)
+    _here(qkv, cos_sin_cache, positions, slots, k_codes, v_codes, k_words, v_words, q_out)
+    lib = _lib.load()
+    _lib.check(lib.qspec_kv4_append(_ptr(qkv), qkv.stride(0), _ptr(cos_sin_cache), cos_sin_cache.shape[0], _ptr(positions), _ptr(slots), _ptr(k_codes), _ptr(v_codes),
+                                    _ptr(k_words), _ptr(v_words), _ptr(q_out), q_ts, T, H, G, D, n, P, int(bool(hadamard)), _dt(qkv), _stream()), "kv4_append")
+
+
+def kv4_read(k_codes: torch.Tensor, v_codes: torch.Tensor, k_words: torch.Tensor, v_words: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor,
+             v_out: torch.Tensor) -> None:
+    """Rows of the 4-bit cache as 16-bit values: k_out, v_out [N, G, D] (float16 / bfloat16) of slots int32 [N]; zeros for a slot outside the cache. (Keys as they lie in
+    it: behind the Hadamard matrix, if they were written with it.)"""
+    if _fast_call("kv4_read", k_codes, v_codes, k_words, v_words, slots, k_out, v_out):
+        return
+    n, G, P, D = _kv4_cache(k_codes, v_codes, k_words, v_words)
+    _chk(k_out, "k_out", (_F16, _BF16)); _chk(v_out, "v_out", (k_out.dtype,))
+    _i32(slots, "slots", slots.numel())
+    if k_out.shape != (slots.numel(), G, D) or v_out.shape != k_out.shape:
+        raise ValueError(f"kv4_read: outputs must be [{slots.numel()}, {G}, {D}]")
+    _here(k_codes, v_codes, k_words, v_words, slots, k_out, v_out)
+    lib = _lib.load()
+    _lib.check(lib.qspec_kv4_read(_ptr(k_codes), _ptr(v_codes), _ptr(k_words), _ptr(v_words), _ptr(slots), _ptr(k_out), _ptr(v_out), slots.numel(), G, D, n, P, _dt(k_out),
+                                  _stream()), "kv4_read")
+
+
+def kv4_attention_workspace(device) -> torch.Tensor:
+    """Workspace for `kv4_attention` calls that are made one after the other (a model's layers, a captured step). Calls that may run at the same
+    time, on two streams or in two graphs, need one each."""
+    device = torch.device(device)
+    with torch.cuda.device(device):
+        return torch.zeros(_lib.load().qspec_kv4_attention_workspace_bytes(), dtype=torch.uint8, device=device)
+
+
+def kv4_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_words: torch.Tensor, v_words: torch.Tensor, table: torch.Tensor,
+                  q_start: torch.Tensor, kv_len: torch.Tensor, out: torch.Tensor, sm_scale: float, workspace: torch.Tensor,
+                  max_tokens: Optional[int] = None) -> torch.Tensor:
+    """Softmax attention of a step's tokens q [T, H, D] over the 4-bit cache: as `kv8_attention`, with the cache of `kv4_append` (and queries that have gone through the
+    same rotation as its keys). workspace: `kv4_attention_workspace`."""
+    if _fast_call("kv4_attention", q, k_codes, v_codes, k_words, v_words, table, q_start, kv_len, out, sm_scale, workspace, max_tokens):
+        return out
+    n, G, P, D = _kv4_cache(k_codes, v_codes, k_words, v_words)
+    for t, name in ((q, "q"), (out, "out")):
+        if not t.is_cuda or t.dtype not in (_F16, _BF16) or t.dim() != 3 or t.shape[2] != D or t.stride(2) != 1:
+            raise ValueError(f"kv4_attention: {name} must be a float16 / bfloat16 CUDA tensor [T, H, {D}] with unit stride in a head")
+    T, H = q.shape[0], q.shape[1]
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError("kv4_attention: out must have the shape and type of q")
+    if table.dim() != 2:
+        raise ValueError("kv4_attention: table must be [requests, pages of a request]")
+    B, Wd = table.shape
+    _i32(table, "table", B, Wd); _i32(q_start, "q_start", B + 1); _i32(kv_len, "kv_len", B)
+    _chk(workspace, "workspace", (torch.uint8,))
+    if not sm_scale > 0:
+        raise ValueError(f"kv4_attention: scale must be positive, got {sm_scale}")
+    if T == 0:
+        return out
+    _here(q, k_codes, v_codes, k_words, v_words, table, q_start, kv_len, out, workspace)
+    if max_tokens is None:
+        max_tokens = T
+    lib = _lib.load()
+    _lib.check(lib.qspec_kv4_attention(_ptr(q), q.stride(0), q.stride(1), _ptr(k_codes), _ptr(v_codes), _ptr(k_words), _ptr(v_words), _ptr(table), _ptr(q_start), _ptr(kv_len),
+                                       _ptr(out), out.stride(0), out.stride(1), T, B, Wd, H, G, D, n, P, min(max_tokens, T), float(sm_scale), _dt(q), _ptr(workspace),
+                                       workspace.numel(), _stream()), "kv4_attention")
+    return out
+
+
 def _probs(t: torch.Tensor, name: str, *shape: int) -> None:
     if not t.is_cuda or t.dtype != torch.float32 or t.shape != shape or (t.stride(2) != 1 and shape[2] > 1):
         raise ValueError(f"{name} must be a float32 CUDA tensor {shape} with unit stride over the vocabulary")
@@ -1007,6 +1115,49 @@ def sample_probs(probs: torch.Tensor, uniform: torch.Tensor, tokens: torch.Tenso
         raise ValueError("sample_probs: probs [rows, V], uniform [rows], tokens [rows]")
     verify_drafts(None, None, probs.unsqueeze(1), uniform.unsqueeze(1), tokens.unsqueeze(1), torch.empty_like(tokens))
     return tokens
+
+
+def max_top_logprobs() -> int:
+    """The most alternatives that `token_logprobs` gives."""
+    return _lib.load_seq().qspec_seq_token_logprobs_max_top()
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor], logprobs: Optional[torch.Tensor] = None, entropy: Optional[torch.Tensor] = None,
+                   ranks: Optional[torch.Tensor] = None, top_logprobs: Optional[torch.Tensor] = None, top_tokens: Optional[torch.Tensor] = None,
+                   temperature: float = 1.0) -> None:
+    """What softmax(logits / temperature) says of given tokens, logits [rows, V] (float16 / bfloat16 / float32; rows may be strided), tokens int64 [rows]: logprobs float32 [rows], ranks
+    int64 [rows] (1: no logit is larger); and of every row entropy float32 [rows] (nats), and the best alternatives, top_logprobs float32 and top_tokens int64 [rows, n]
+    (n <= `max_top_logprobs()`; equal ones by the lower token). Results that are None are not wanted; without tokens there are neither logprobs nor ranks. A negative token is none: log
+    probability 0, rank 0; one behind the vocabulary has minus infinity, and rank 0. Rows of minus infinities alone: minus infinity, entropy 0; rows with NaN or plus infinity: NaN.
+    (The reference: vllm/model_executor/layers/sampler.py, log_softmax over all logits and a sort.)"""
+    if _fast_call("seq_token_logprobs", logits, tokens, logprobs, entropy, ranks, top_logprobs, top_tokens, float(temperature)):
+        return
+    if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in (_F16, _BF16, torch.float32) or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("token_logprobs: logits must be a float16 / bfloat16 / float32 CUDA tensor [rows, V] with unit column stride")
+    rows, V = logits.shape
+    if tokens is None and (logprobs is not None or ranks is not None):
+        raise ValueError("token_logprobs: log probabilities and ranks are those of given tokens")
+    if (top_logprobs is None) != (top_tokens is None):
+        raise ValueError("token_logprobs: top_logprobs and top_tokens belong together")
+    results = (logprobs, entropy, ranks, top_logprobs, top_tokens)
+    top = top_logprobs.shape[-1] if top_logprobs is not None else 0
+    for t, name, dtype, shape in ((tokens, "tokens", torch.int64, (rows,)), (logprobs, "logprobs", torch.float32, (rows,)), (entropy, "entropy", torch.float32, (rows,)),
+                                  (ranks, "ranks", torch.int64, (rows,)), (top_logprobs, "top_logprobs", torch.float32, (rows, top)), (top_tokens, "top_tokens", torch.int64, (rows, top))):
+        _chk(t, name, (dtype,), allow_none=True)
+        if t is not None and t.shape != shape:
+            raise ValueError(f"token_logprobs: {name} must be {shape}, got {tuple(t.shape)}")
+    if rows == 0:
+        return
+    if V == 0 or not temperature > 0:
+        raise ValueError(f"token_logprobs: a vocabulary and a positive temperature are needed, got {V} and {temperature}")
+    _here(logits, tokens, *results)
+    there = [t for t in results if t is not None and t.numel()]
+    if any(_overlap(t, u) for i, t in enumerate(there) for u in (*there[:i], *((tokens,) if tokens is not None else ()))) or any(_overlap_rows(t, logits) for t in there):
+        raise ValueError("token_logprobs: results must not lie over each other, nor over other tensors of the call")
+    seq = _lib.load_seq()
+    stride = logits.stride(0) if rows > 1 else max(logits.stride(0), V)
+    _lib.check(seq.qspec_seq_token_logprobs(_ptr(logits), stride, _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(ranks), _ptr(top_logprobs), _ptr(top_tokens), rows, V, top,
+                                            float(temperature), {_F16: _lib.DTYPE_F16, _BF16: _lib.DTYPE_BF16}.get(logits.dtype, _lib.DTYPE_F32), _stream()), "token_logprobs", seq)
 
 
 def tp_argmax_combine(local_max: torch.Tensor, local_idx: torch.Tensor, index_offset: int, peers,

@@ -1,0 +1,174 @@
+"""Log probabilities of given tokens, entropy, ranks and best alternatives on the GPU, against 64 bits and sorts."""
+import math
+
+import pytest
+import torch
+
+from qspec_b200 import ops
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32, F64, I64 = torch.float16, torch.bfloat16, torch.float32, torch.float64, torch.int64
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def call(logits, tokens, top, temperature=1.0):
+    n = logits.shape[0]
+    lp, h = torch.full((n,), 7.0, device="cuda"), torch.full((n,), 7.0, device="cuda")
+    rank = torch.full((n,), -7, device="cuda")
+    tlp, tt = torch.full((n, top), 7.0, device="cuda"), torch.full((n, top), -7, device="cuda")
+    ops.token_logprobs(logits, tokens, lp, h, rank, *((tlp, tt) if top else (None, None)), temperature=temperature)
+    return lp, h, rank, tlp, tt
+
+
+def check(logits, tokens, top, temperature=1.0):
+    """A value y = c (x - max) is rounded once, by 2^-24 |y|, c by 2^-24 of itself, and so is what a weight's exponent gets; weights are off by 2^-22 (ex2.approx) and that; sums of V
+    terms in float32, in trees over V / 2048 terms at most one after the other, by (V / 2048 + 16) 2^-24; the logarithm by 2^-22. So a log probability is off by 2^-22 |lp| and
+    what log S is off by; the entropy by that and, U / S being an average of |y| <= Y, by the weights' errors times Y (terms beyond e^-40 of the largest have none)."""
+    lp, h, rank, tlp, tt = call(logits, tokens, top, temperature)
+    z = logits.double() / temperature
+    p = torch.log_softmax(z, -1)
+    V = logits.shape[1]
+    off = (V / 2048 + 16) * 2.0 ** -24 + 2.0 ** -21 + 40 * 2.0 ** -23
+    want = p.gather(1, tokens[:, None])[:, 0]
+    assert ((lp - want).abs() <= want.abs() * 2.0 ** -22 + off).all(), float((lp - want).abs().max())
+    entropy = -torch.special.xlogy(p.exp(), p.exp()).sum(-1)
+    assert ((h - entropy).abs() <= entropy * 2.0 ** -20 + off * 41).all(), float((h - entropy).abs().max())
+    assert torch.equal(rank, (logits > logits.gather(1, tokens[:, None])).sum(-1) + 1)
+    best = logits.sort(dim=-1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(tt, best)
+    want = p.gather(1, best)
+    assert ((tlp - want).abs() <= want.abs() * 2.0 ** -22 + off).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,V", [(1, 1), (3, 2), (2, 33), (5, 1024), (1, 4096), (7, 8193), (4, 32001), (33, 50257), (2, 128256), (3, 151643), (1, 262144)])
+@pytest.mark.parametrize("top", [0, 1, 5, 8, 9, 32])
+def test_of_logits_as_models_give_them(rows, V, dtype, top):
+    logits = (torch.randn(rows, V, generator=gen(V), device="cuda") * 3).to(dtype)
+    check(logits, torch.randint(0, V, (rows,), generator=gen(1), device="cuda"), min(top, V), 0.7 if top == 5 else 1.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("shape", ["up", "down", "equal", "two", "steep", "masked", "blocks"])
+@pytest.mark.parametrize("V", [1000, 40000, 130001])
+def test_of_rows_that_are_out_of_the_ordinary(shape, V, dtype):
+    at = torch.arange(V, device="cuda")
+    x = {"up": at / V, "down": -at / V, "equal": torch.full((V,), 2.5, device="cuda"), "two": (at % 2).float(), "steep": -at.float().clamp(max=60000),
+         "masked": torch.where(at % 7000 == 17, at / V, -math.inf), "blocks": torch.where(at < V // 2, 0.0, torch.where(at > V * 3 // 4, -math.inf, 4.0))}[shape]
+    logits = x.to(dtype).repeat(3, 1)
+    lp, h, rank, tlp, tt = call(logits, torch.tensor([17, 17, 17], device="cuda"), 20)
+    best = logits.sort(dim=-1, descending=True, stable=True).indices[:, :20]
+    assert torch.equal(tt, best)
+    p = torch.log_softmax(logits.double(), -1)
+    want = p.gather(1, best)
+    # (sums of V equal terms, V / 2048 of them one after the other)
+    torch.testing.assert_close(tlp.double(), want, rtol=2.0 ** -20, atol=(V / 2048 + 60) * 2.0 ** -23)
+    torch.testing.assert_close(lp.double(), p[:, 17], rtol=2.0 ** -20, atol=(V / 2048 + 60) * 2.0 ** -23)
+    torch.testing.assert_close(h.double(), -torch.special.xlogy(p.exp(), p.exp()).sum(-1), rtol=2.0 ** -18, atol=(V / 2048 + 60) * 2.0 ** -20)
+    assert torch.equal(rank, (logits > logits[:, 17:18]).sum(-1) + 1)
+
+
+def test_zeros_of_either_sign_are_equal():
+    logits = torch.zeros(2, 5000, device="cuda")
+    logits[0, ::2] = -0.0
+    logits[1, 1::2] = -0.0
+    assert call(logits, torch.zeros(2, dtype=I64, device="cuda"), 6)[4].tolist() == [list(range(6))] * 2
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("V", [100, 70000])
+def test_rows_of_nothing_of_infinity_and_of_no_numbers(dtype, V):
+    logits = torch.randn(6, V, generator=gen(3), device="cuda").to(dtype)
+    logits[1] = -math.inf
+    logits[2, 50] = math.inf
+    logits[3, 60] = math.nan
+    logits[4, :] = -math.inf
+    logits[4, 99] = 3.0
+    tokens = torch.tensor([7, 7, 50, 7, 99, 7], device="cuda")
+    clean = call(logits[5:], tokens[5:], 4)
+    lp, h, rank, tlp, tt = call(logits, tokens, 4)
+    assert lp[1] == -math.inf and h[1] == 0 and (tlp[1] == -math.inf).all() and tt[1].tolist() == [0, 1, 2, 3] and rank[1] == 1
+    for row, first in ((2, 50), (3, 60)):
+        assert lp[row].isnan() and h[row].isnan() and tlp[row].isnan().all() and tt[row, 0] == first
+        assert tt[row].tolist() == logits[row].sort(descending=True, stable=True).indices[:4].tolist()
+    assert lp[4] == 0 and h[4] == 0 and rank[4] == 1 and tt[4].tolist() == [99, 0, 1, 2] and (tlp[4, 1:] == -math.inf).all()
+    assert all(torch.equal(a[5:], b) for a, b in zip((lp, h, rank, tlp, tt), clean))
+
+
+def test_tokens_that_are_none():
+    logits = torch.randn(4, 3000, generator=gen(4), device="cuda").half()
+    lp, h, rank, _, _ = call(logits, torch.tensor([-1, 3000, 2999, -100], device="cuda"), 0)
+    assert lp[0] == 0 and lp[3] == 0 and lp[1] == -math.inf and lp[2] < 0 and rank.tolist()[0:2] == [0, 0] and rank[2] > 0 and rank[3] == 0 and (h > 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("V,stride,shift", [(5001, 5001, 0), (5001, 5003, 1), (70001, 70007, 3), (70000, 70016, 8), (128, 1000, 5)])
+def test_rows_that_begin_anywhere(V, stride, shift, dtype):
+    wide = torch.full((7, stride + 16), 100.0, device="cuda").to(dtype)   # what stands beside a row is larger than all in it
+    logits = wide.view(-1)[shift:shift + 6 * stride].view(6, stride)[:, :V]
+    logits.copy_(torch.randn(6, V, generator=gen(5), device="cuda"))
+    check(logits, torch.randint(0, V, (6,), generator=gen(6), device="cuda"), 10)
+
+
+@pytest.mark.parametrize("temperature", [1e-3, 0.1, 1.0, 30.0])
+def test_temperatures(temperature):
+    logits = torch.randn(5, 33000, generator=gen(7), device="cuda")
+    lp, h, rank, tlp, tt = call(logits, logits.argmax(-1), 3, temperature)
+    p = torch.log_softmax(logits.double() / temperature, -1)
+    # (c is rounded by 2^-24, products by as much: relative errors of log probabilities)
+    torch.testing.assert_close(tlp.double(), p.topk(3).values, rtol=2.0 ** -21, atol=80 * 2.0 ** -23)
+    assert (rank == 1).all()
+
+
+def test_results_that_are_not_wanted_and_calls_of_nothing():
+    logits = torch.randn(9, 20000, generator=gen(8), device="cuda").half()
+    tokens = torch.randint(0, 20000, (9,), generator=gen(9), device="cuda")
+    lp, h, rank, tlp, tt = call(logits, tokens, 5)
+    for only in range(4):
+        out = [torch.zeros_like(t) for t in (lp, h, rank, tlp, tt)]
+        want = (lp, h, rank, tlp, tt)
+        wanted = [(0,), (1,), (2,), (3, 4)][only]
+        ops.token_logprobs(logits, tokens if only in (0, 2) else None, *[out[i] if i in wanted else None for i in range(5)])
+        assert all(torch.equal(out[i], want[i]) for i in wanted)
+    ops.token_logprobs(logits[:0], tokens[:0], lp[:0])
+    ops.token_logprobs(logits, tokens)
+
+
+def test_the_same_every_time_in_a_graph_and_on_other_streams():
+    logits = (torch.randn(70, 128256, generator=gen(10), device="cuda") * 3).half()
+    tokens = logits.argmax(-1)
+    want = call(logits, tokens, 20)
+    out = [torch.zeros_like(t) for t in want]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.token_logprobs(logits, tokens, *out)
+    for _ in range(5):
+        for t in out:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [[torch.zeros_like(t) for t in want] for _ in range(2)]
+    torch.cuda.synchronize()
+    for s, o in zip(streams, outs):
+        with torch.cuda.stream(s):
+            ops.token_logprobs(logits, tokens, *o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
+
+
+def test_what_is_refused():
+    x, t = torch.zeros(3, 100, device="cuda"), torch.zeros(3, dtype=I64, device="cuda")
+    lp, tlp, tt = torch.zeros(3, device="cuda"), torch.zeros(3, 4, device="cuda"), torch.zeros(3, 4, dtype=I64, device="cuda")
+    ops.token_logprobs(x, t, lp, lp.clone(), t.clone(), tlp, tt)
+    for args, kw in (((x.double(), t, lp), {}), ((x.t(), t, lp), {}), ((x[0], t, lp), {}), ((x, t.int(), lp), {}), ((x, t[:2], lp), {}), ((x, t, lp.half()), {}), ((x, t, lp[:2]), {}),
+                     ((x, None, lp), {}), ((x, None, None, None, t), {}), ((x, t, lp, None, None, tlp), {}), ((x, t, lp, None, None, tlp, tt[:, :3].contiguous()), {}),
+                     ((x, t, lp), dict(temperature=0.0)), ((x, t, lp), dict(temperature=-1.0)), ((x, t, lp), dict(temperature=math.nan)), ((x, t, lp), dict(temperature=math.inf)),
+                     ((x, t, lp), dict(temperature=1e-40)), ((x, t, lp, lp), {}), ((x, t, x[0, :3]), {}), ((x, t, None, None, t), {}),
+                     ((x, t, None, None, None, torch.zeros(3, 33, device="cuda"), torch.zeros(3, 33, dtype=I64, device="cuda")), {}),
+                     ((x[:, :3].contiguous(), t, None, None, None, tlp, tt), {}), ((x[:, :0], t, lp), {})):
+        with pytest.raises(ValueError):
+            ops.token_logprobs(*args, **kw)
