@@ -16,7 +16,8 @@
 namespace qspec {
 namespace logprob {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32, MOST_TOP = 32, CANDIDATES = 512, EACH = 4;   // EACH: vectors of a thread in a batch
+constexpr int THREADS = 256, WARPS = THREADS / 32, MOST_TOP = 32, EACH = 4;   // EACH: vectors of a thread in a batch
+constexpr int GROUPS = 64, GROUP = THREADS / GROUPS, HITS = 256, CANDIDATES = 512;   // groups of neighbouring threads; vectors with candidates, candidates in them
 constexpr float AHEAD = 60.f;                     // a value 2^AHEAD above the reference moves it
 typedef unsigned long long u64;
 
@@ -92,18 +93,20 @@ __device__ __forceinline__ float value_of(u64 key) {
 }
 __device__ __forceinline__ int index_of(u64 key) { return (int)~(uint32_t)key; }
 
-// The n best of the keys s_key[0 .. count) in their order to s_best, and back to the begin of s_key. All threads of the CTA call it, with everything written.
-__device__ __forceinline__ int select(u64* s_key, u64* s_best, int count, int n) {
-  for (int i = threadIdx.x; i < count; i += THREADS) {
-    const u64 key = s_key[i];
-    int larger = 0;
-    for (int j = 0; j < count; ++j) larger += s_key[j] > key;
-    if (larger < n) s_best[larger] = key;
+// The n-th largest of the groups' maxima (n <= GROUPS): as many values reach it, or more. Every warp finds it for itself.
+__device__ __forceinline__ float nth_largest(const float* s_group, int n) {
+  const int lane = threadIdx.x & 31;
+  const float mine[2] = {s_group[lane], s_group[lane + 32]};
+  int larger[2] = {0, 0};
+#pragma unroll 4
+  for (int j = 0; j < GROUPS; ++j) {
+    const float x = s_group[j];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) larger[e] += x > mine[e] || (x == mine[e] && j < lane + 32 * e);
   }
-  __syncthreads();
-  const int best = min(count, n);
-  if (threadIdx.x < best) s_key[threadIdx.x] = s_best[threadIdx.x];
-  return best;
+  const uint32_t first = __ballot_sync(0xffffffffu, larger[0] == n - 1), second = __ballot_sync(0xffffffffu, larger[1] == n - 1);
+  const float x = __shfl_sync(0xffffffffu, mine[0], __ffs(first | 0x80000000u) - 1), y = __shfl_sync(0xffffffffu, mine[1], __ffs(second | 0x80000000u) - 1);
+  return first ? x : second ? y : -INFINITY;
 }
 
 template <typename T, int CLUSTER>
@@ -112,11 +115,12 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
   using L = Lanes<T>;
   __shared__ Partial s_part;
   __shared__ u64 s_best[MOST_TOP], s_key[CANDIDATES], s_most[WARPS];
-  __shared__ float s_max[WARPS], s_low[WARPS], s_ref[WARPS], s_sum[2][WARPS];
-  __shared__ int s_above[WARPS], s_count;
+  __shared__ uint4 s_hit[HITS];
+  __shared__ float s_group[GROUPS], s_ref[WARPS], s_sum[2][WARPS];
+  __shared__ int s_above[WARPS], s_where[HITS], s_hits, s_count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
-  if (tid == 0) s_count = 0;
+  if (tid == 0) s_hits = s_count = 0;
   pdl_enter();
   const T* const x_row = (const T*)a.logits + (size_t)row * a.stride;
   const int lo = min(rank * a.span, a.V), n = min(a.span, a.V - lo);
@@ -162,60 +166,44 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
 #pragma unroll
     for (int j = 0; j < EACH; ++j) big[j] = L::largest(w[j]);
     if (b == 0) {
-      // ---- the first batch's maximum, and what the best have to reach: maxima of groups of eight lanes, or, of up to eight, those of the warps
+      // ---- the first batch's maximum, and what the best have to reach
       float g = max_nan(max_nan(big[0], big[1]), max_nan(big[2], big[3]));
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
-      float low = g;
-#pragma unroll
-      for (int o = 8; o < 32; o <<= 1) {
-        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-        g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
-      }
-      if (lane == 0) {
-        s_max[warp] = g;
-        s_low[warp] = a.top > WARPS ? low : g;
-      }
+      for (int o = 1; o < GROUP; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if (tid % GROUP == 0) s_group[tid / GROUP] = g;
       __syncthreads();
-      ref = s_max[0];
-      reach = s_low[0];
+      ref = max_nan(s_group[lane], s_group[lane + 32]);
 #pragma unroll
-      for (int i = 1; i < WARPS; ++i) {
-        ref = max_nan(ref, s_max[i]);
-        reach = fminf(reach, s_low[i]);
-      }
-      if (!a.top) reach = INFINITY;
+      for (int o = 16; o > 0; o >>= 1) ref = max_nan(ref, __shfl_xor_sync(0xffffffffu, ref, o));
+      if (a.top) reach = nth_largest(s_group, a.top);
       none = ref == -INFINITY;
       if (none) ref = 0.f;                                  // (weights of minus infinity are zero wherever they are counted from)
       set_limit();
     }
+    const float most = max_nan(max_nan(big[0], big[1]), max_nan(big[2], big[3]));
+    if (!(most < limit)) {                                  // seldom: candidates, a value far above all before it, no numbers. (Code that is short, and there once: it is cold)
+      odd |= most != most;
+      if (none ? most > -INFINITY : most > ref + AHEAD / a.c) {
+        const float d = fmaxf((ref - most) * a.c, -16384.f), f = none ? 0.f : ex2(d);
+        const float2 S = unpack_f2(S2), U = unpack_f2(U2);
+        U2 = pack_f2(fmaf(S.x, d, U.x) * f, fmaf(S.y, d, U.y) * f);
+        S2 = pack_f2(S.x * f, S.y * f);
+        ref = most;
+        none = false;
+        set_limit();
+      }
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      if (!(big[j] < limit)) {                              // seldom: candidates, a value far above all before it, no numbers
-        odd |= big[j] != big[j];
-        if (none ? big[j] > -INFINITY : big[j] > ref + AHEAD / a.c) {
-          const float d = fmaxf((ref - big[j]) * a.c, -16384.f), f = none ? 0.f : ex2(d);
-          const float2 S = unpack_f2(S2), U = unpack_f2(U2);
-          U2 = pack_f2(fmaf(S.x, d, U.x) * f, fmaf(S.y, d, U.y) * f);
-          S2 = pack_f2(S.x * f, S.y * f);
-          ref = big[j];
-          none = false;
-          set_limit();
-        }
+      for (int j = 0; j < EACH; ++j)
         if (b == 0 ? big[j] >= reach : big[j] > reach) {
-          const int first = ((b * EACH + j) * THREADS + tid) * E - shift;
-          const T* const x = reinterpret_cast<const T*>(&w[j]);
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float y = value(x[e]);
-            const int i = first + e;
-            if ((b == 0 ? y >= reach : y > reach) && i >= 0 && i < n) {
-              const int at = atomicAdd(&s_count, 1);        // (in any order: they are put in theirs)
-              if (at < CANDIDATES) s_key[at] = key_of(y, lo + i);
-            }
+          const int at = atomicAdd(&s_hits, 1);             // (in any order: they are put in theirs)
+          if (at < HITS) {
+            s_hit[at] = w[j];
+            s_where[at] = ((b * EACH + j) * THREADS + tid) * E - shift;
           }
         }
-      }
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
       float x[E];
       L::values(w[j], x);
       const u64 minus = pack_f2(-ref, -ref), c2 = pack_f2(a.c, a.c);
@@ -231,19 +219,42 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
       if (a.ranks) above += L::above(w[j], given);
     }
     if (a.top && (b == check || b + 1 == batches)) {
-      check = 4 * b + 3;
+      // ---- the best so far: of those of before, which are the first keys, and of the candidates
       __syncthreads();
-      const int count = s_count;
-      if (count <= CANDIDATES) {                            // (the same for all)
-        best = select(s_key, s_best, count, a.top);
+      const int hits = s_hits;
+      if (hits <= HITS) {                                   // (the same for all)
+        for (int i = tid; i < hits * E; i += THREADS) {
+          const float y = value(reinterpret_cast<const T*>(s_hit)[i]);
+          const int at = s_where[i / E] + i % E;
+          if ((check == 0 ? y >= reach : y > reach) && at >= 0 && at < n) {
+            const int k = atomicAdd(&s_count, 1);
+            if (k < CANDIDATES) s_key[k] = key_of(y, lo + at);
+          }
+        }
         __syncthreads();
-        if (tid == 0) s_count = best;
-        if (best == a.top) reach = value_of(s_best[best - 1]);
-        __syncthreads();
+        const int count = s_count;
+        if (count <= CANDIDATES) {
+          for (int i = tid; i < count; i += THREADS) {
+            const u64 key = s_key[i];
+            int larger = 0;
+#pragma unroll 4
+            for (int j = 0; j < count; ++j) larger += s_key[j] > key;
+            if (larger < a.top) s_best[larger] = key;
+          }
+          __syncthreads();
+          best = min(count, a.top);
+          if (tid < best) s_key[tid] = s_best[tid];
+          if (tid == 0) { s_count = best; s_hits = 0; }
+          if (best == a.top) reach = value_of(s_best[best - 1]);
+        } else {
+          reach = INFINITY;                                 // too many: all of them are looked for at the end
+        }
       } else {
-        reach = INFINITY;                                   // too many: all of them are looked for at the end
+        reach = INFINITY;
       }
+      check = 4 * b + 3;
       set_limit();
+      __syncthreads();
     }
   }
   // ---- the threads' sums together
@@ -269,18 +280,16 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
   }
   above = __reduce_add_sync(0xffffffffu, above);
   if (lane == 0) { s_sum[0][warp] = S; s_sum[1][warp] = U; s_above[warp] = above; }
-  if (a.top && (odd || s_count > CANDIDATES)) {             // (the same for all: the barrier above)
+  if (a.top && (odd || s_hits > HITS || s_count > CANDIDATES)) {             // (the same for all: the barrier above)
     u64 before = ~0ull;                                     // (no key is that large)
     for (best = 0; best < a.top; ++best) {
       u64 most = 0;
       for (int v = tid; v < vectors; v += THREADS) {
-        const uint4 w = load(v);
-        const T* const x = reinterpret_cast<const T*>(&w);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int i = v * E - shift + e;
-          const u64 key = key_of(value(x[e]), lo + i);
-          if (i >= 0 && i < n && key < before && key > most) most = key;
+        const int first = v * E - shift;
+#pragma unroll 1
+        for (int i = max(first, 0); i < min(first + E, n); ++i) {
+          const u64 key = key_of(value(from[i]), lo + i);
+          if (key < before && key > most) most = key;
         }
       }
 #pragma unroll
@@ -406,7 +415,7 @@ extern "C" int qspec_seq_token_logprobs(const void* logits, long long row_stride
   // CTAs of a row
   const int sms = std::max(sm_count(), 1), batch = THREADS * EACH * 16 / size;
   int cluster = 1;
-  while (cluster < 8 && (long long)rows * cluster < 4ll * sms && V > cluster * batch) cluster *= 2;
+  while (cluster < 8 && (long long)rows * cluster <= 2 * sms && V > cluster * batch) cluster *= 2;
   const int span = ((V + cluster - 1) / cluster + 7) / 8 * 8;
   QSPEC_REQUIRE(V <= (1 << 24), QSPEC_ERR_UNSUPPORTED, "token_logprobs: a vocabulary of %d is too large", V);
   QSPEC_REQUIRE((long long)rows * cluster < (1ll << 31), QSPEC_ERR_UNSUPPORTED, "token_logprobs: %d rows are too many for one call", rows);
