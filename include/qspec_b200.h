@@ -447,6 +447,12 @@ int qspec_kv4_attention(const void* q, long long q_tok_stride, int q_head_stride
                         const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H, int G, int D,
                         int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* For tests, as qspec_debug_kv8_attention_give_up. */
+int qspec_debug_kv4_attention_give_up(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const void* k_word, const void* v_word,
+                                      const int* table, const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests,
+                                      int width, int H, int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                      unsigned give_up, void* stream);
+
 /* Verification of drafted tokens, and one token more. drafted int64 [requests, drafts]; draft / target float32 probabilities, row of (request b, place i) at
  * b * seq_stride + i * place_stride, `drafts` and drafts + 1 places; uniform float32 [requests, drafts + 1] in [0, 1); draft_counts (NULL: all) int32: how
  * many drafts a request has. Draft i is taken if uniform[b, i] * q_i(d_i) < p_i(d_i) (exactly) and all before it were. Then one token by inversion with

@@ -105,6 +105,8 @@ SIGNATURES = {
     "qspec_kv4_attention_workspace_bytes": (ctypes.c_size_t, []),
     "qspec_kv4_attention": (c_int, [c_void_p, ctypes.c_longlong, c_int] + [c_void_p] * 8 + [ctypes.c_longlong] + [c_int] * 10 + [c_float, c_int, c_void_p, ctypes.c_size_t,
                                                                                                                            c_void_p]),
+    "qspec_debug_kv4_attention_give_up": (c_int, [c_void_p, ctypes.c_longlong, c_int] + [c_void_p] * 8 + [ctypes.c_longlong] + [c_int] * 10 + [c_float, c_int, c_void_p,
+                                                                                                                                          ctypes.c_size_t, ctypes.c_uint, c_void_p]),
     "qspec_verify_drafts_max_drafts": (c_int, []),
     "qspec_verify_drafts": (c_int, [c_void_p, c_void_p, ctypes.c_longlong, ctypes.c_longlong, c_void_p, ctypes.c_longlong, ctypes.c_longlong] + [c_void_p] * 4 +
                             [c_int] * 3 + [c_void_p]),

@@ -19,6 +19,7 @@ void count_launch(int n = 1);                    // bumps qspec_launch_count()
 int  sm_count();
 int  gemm_rows_timeouts();                         // CTAs of the few-token GEMM that gave a wait up; -1: not readable
 int  kv8_timeouts();                               // CTAs of the prompt attention over the 8-bit cache that gave a wait up; -1: not readable
+int  kv4_timeouts();                               // the same over the 4-bit cache
 int  rotation_timeouts();                          // rows of the cluster rotation with a wait given up; -1: not readable
 
 #define QSPEC_REQUIRE(cond, code, ...)                                                       \

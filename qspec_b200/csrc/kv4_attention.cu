@@ -409,9 +409,9 @@ static int att_grid() { return max(sm_count(), 1) * CTAS; }
 
 extern "C" size_t qspec_kv4_attention_workspace_bytes(void) { return 4096 + (size_t)att_grid() * 2 * PART<128> * sizeof(float); }
 
-extern "C" int qspec_kv4_attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const void* k_word, const void* v_word, const int* table,
-                                   const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H,
-                                   int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+static int attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const void* k_word, const void* v_word, const int* table,
+                     const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H, int G, int D, int npages,
+                     int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, bool always, unsigned give_up, void* stream) {
   QSPEC_REQUIRE(k && v && k_word && v_word && table && q_start && kv_len, QSPEC_ERR_INVALID_ARG, "kv4_attention: null pointer");
   QSPEC_REQUIRE(page_shift(page_tokens) > 0, QSPEC_ERR_UNSUPPORTED, "kv4_attention: pages of 16, 32, 64 or 128 tokens, got %d", page_tokens);
   QSPEC_REQUIRE(D == 64 || D == 128, QSPEC_ERR_UNSUPPORTED, "kv4_attention: heads of 64 or 128, got %d", D);
@@ -431,7 +431,19 @@ extern "C" int qspec_kv4_attention(const void* q, long long q_tok_stride, int q_
                 "kv4_attention: %zu bytes of workspace needed, got %zu", qspec_kv4_attention_workspace_bytes(), workspace_bytes);
   const int grid = att_grid();
   QSPEC_REQUIRE(grid <= GRID_MOST, QSPEC_ERR_UNSUPPORTED, "kv4_attention: %d SMs", sm_count());
-  const AttArgs a{{table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok, G, H / G, 0u},
+  // Requests with many rows may go to the prompt form (to_prompt_form()), in a launch of its own in front; none do if the call's rows are too few for a third of
+  // the SMs (always: for tests).
+  const int rep = H / G;
+  const bool prompts = rep <= PROMPT_REP && (long long)max_tokens * rep >= PROMPT_ROWS && (always || (long long)ntok * H >= std::max(sm_count() / 3, 1) * 128ll);
+  const unsigned share = always ? 1u : std::max(sm_count() / 4, 1) * 128u;
+  if (prompts) {
+    // Two tiles a CTA where the rows are more than the SMs take at once with one, by a quarter.
+    const int pair = always ? give_up >> 4 & 1 : (long long)ntok * H > 160ll * sm_count();
+    const PromptArgs4 pa{q, q_tok_stride, q_head_stride, (const uint8_t*)k, (const uint8_t*)v, (const uint16_t*)k_word, (const uint16_t*)v_word, table, q_start, kv_len, requests, width,
+                         npages, page_shift(page_tokens), ntok, G, rep, pair, share, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, give_up};
+    if (const int rc = launch_prompt(pa, D, dtype == QSPEC_DTYPE_BF16, (cudaStream_t)stream)) return rc;
+  }
+  const AttArgs a{{table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok, G, rep, prompts ? share : 0u},
                   {out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)}, q, q_tok_stride, q_head_stride, (const uint8_t*)k, (const uint8_t*)v,
                   (const uint16_t*)k_word, (const uint16_t*)v_word, scale * 1.4426950408889634f};
   auto run = [&](auto kern, size_t smem, SmemLimit& limit) -> int {
@@ -444,4 +456,18 @@ extern "C" int qspec_kv4_attention(const void* q, long long q_tok_stride, int q_
   if (dtype == QSPEC_DTYPE_F16)
     return D == 128 ? run(kv4_attention_kernel<false, 128>, Smem<128>::TOTAL, limits[0]) : run(kv4_attention_kernel<false, 64>, Smem<64>::TOTAL, limits[1]);
   return D == 128 ? run(kv4_attention_kernel<true, 128>, Smem<128>::TOTAL, limits[2]) : run(kv4_attention_kernel<true, 64>, Smem<64>::TOTAL, limits[3]);
+}
+
+extern "C" int qspec_kv4_attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const void* k_word, const void* v_word, const int* table,
+                                   const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H,
+                                   int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return attention(q, q_tok_stride, q_head_stride, k, v, k_word, v_word, table, q_start, kv_len, out, out_tok_stride, out_head_stride, ntok, requests, width, H, G, D, npages,
+                   page_tokens, max_tokens, scale, dtype, workspace, workspace_bytes, false, 0, stream);
+}
+extern "C" int qspec_debug_kv4_attention_give_up(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const void* k_word, const void* v_word,
+                                                 const int* table, const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok,
+                                                 int requests, int width, int H, int G, int D, int npages, int page_tokens, int max_tokens, float scale, int dtype,
+                                                 void* workspace, size_t workspace_bytes, unsigned give_up, void* stream) {
+  return attention(q, q_tok_stride, q_head_stride, k, v, k_word, v_word, table, q_start, kv_len, out, out_tok_stride, out_head_stride, ntok, requests, width, H, G, D, npages,
+                   page_tokens, max_tokens, scale, dtype, workspace, workspace_bytes, true, give_up, stream);
 }

@@ -20,5 +20,19 @@ using kv8::page_shift;
 __device__ __forceinline__ float word_scale(uint32_t w) { return __uint_as_float((w & 0xfff0u) << 15); }
 #endif
 
+struct PromptArgs4 {
+  const void* q; long long q_ts; int q_hs;
+  const uint8_t *k, *v;
+  const uint16_t *kw, *vw;
+  const int *table, *q_start, *kv_len;
+  int nreq, width, npages, pshift, ntok, G, rep;
+  int pair;                                       // 1: CTAs of the prompt form take two tiles of 128 rows
+  unsigned share;                                 // rows that a quarter of the SMs have at a time
+  float scale2;                                   // scale * log2(e)
+  void* out; long long out_ts; int out_hs;
+  unsigned give_up;                               // for tests: roles that give their first wait up (1 softmax, 2 codes, 4 products, 8 pages)
+};
+int launch_prompt(const PromptArgs4& a, int D, bool bf16, cudaStream_t stream);   // kv4_prompt.cu: the requests that to_prompt_form() names
+
 }  // namespace kv4
 }  // namespace qspec

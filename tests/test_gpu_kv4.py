@@ -4,11 +4,11 @@ import math
 import pytest
 import torch
 
-from qspec_b200 import ops
+from qspec_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
 I16, I32, F32, F64, U8 = torch.int16, torch.int32, torch.float32, torch.float64, torch.uint8
-FORMS = ["rows"]
+FORMS = ["rows", "prompt", "pairs"]
 
 
 def gen(seed):
@@ -268,9 +268,16 @@ def attention_in_64_bits(q, k, v, kw, vw, table, start, lens, scale):
     return out, bound + (out.abs() + bound) * (torch.finfo(q.dtype).eps / 2) + (2.0 ** -25 if q.dtype == torch.float16 else 0.0)
 
 
-def attend(form, q, k, v, kw, vw, table, start, lens, out, scale, work, max_tokens=None):
-    assert form == "rows"
-    return ops.kv4_attention(q, k, v, kw, vw, table, start, lens, out, scale, work, max_tokens=max_tokens)
+def attend(form, q, k, v, kw, vw, table, start, lens, out, scale, work, max_tokens=None, roles=0):
+    """rows: the call as it is; prompt, pairs: every request with rows enough goes to the prompt form, with one or two tiles of rows a CTA."""
+    if form == "rows":
+        return ops.kv4_attention(q, k, v, kw, vw, table, start, lens, out, scale, work, max_tokens=max_tokens)
+    lib, T, H, D = _lib.load(), q.shape[0], q.shape[1], q.shape[2]
+    _lib.check(lib.qspec_debug_kv4_attention_give_up(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), v.data_ptr(), kw.data_ptr(), vw.data_ptr(), table.data_ptr(),
+                                                     start.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), T, len(lens), table.shape[1], H, k.shape[1], D,
+                                                     k.shape[0], k.shape[2], T if max_tokens is None else max_tokens, scale, int(q.dtype == torch.bfloat16), work.data_ptr(),
+                                                     work.numel(), 16 * (form == "pairs") + roles, torch.cuda.current_stream().cuda_stream), "kv4_attention")
+    return out
 
 
 def check_attention(case, D, max_tokens=None, workspace=None, form="rows"):
@@ -529,6 +536,59 @@ def test_attention_walks_no_further_than_the_table(form):
         bad = torch.tensor([first + i >= 128 for i in range(40)] + [True] * 20 + [False] * 40, device="cuda")
         assert out[bad].isnan().all() and not out[~bad].isnan().any()
         assert torch.equal(out[60:], clean[60:])
+
+
+GIVE_UP = r"""
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+from test_gpu_kv4 import make_attention, attend
+from qspec_b200 import ops
+for D, dtype in ((128, torch.float16), (64, torch.bfloat16)):
+    case = make_attention(3, [500, 900, 40], [130, 300, 1], 8, 2, D, 32, dtype)
+    q, work = case[0], ops.kv4_attention_workspace("cuda")
+    good = ops.kv4_attention(*case, torch.empty_like(q), D ** -0.5, work)
+    for form in ("prompt", "pairs"):
+        for roles in (1, 2, 4, 8, 15):
+            before = ops.attn_tile_timeouts()
+            out = attend(form, *case, torch.zeros_like(q), D ** -0.5, work, 300, roles)
+            assert ops.attn_tile_timeouts() > before, roles
+            assert out[:430].isnan().all() and torch.equal(out[430:], good[430:]), roles   # the request with few rows is the other form's
+            again = ops.kv4_attention(*case, torch.empty_like(q), D ** -0.5, work)
+            assert torch.equal(again, good)
+print("ok")
+"""
+
+
+def test_a_wait_that_is_given_up_shows_and_leaves_nothing_behind():
+    import os
+    import subprocess
+    import sys
+    tests = os.path.dirname(os.path.abspath(__file__))
+    run = subprocess.run([sys.executable, "-c", GIVE_UP.format(root=os.path.dirname(tests), tests=tests)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip().endswith("ok"), run.stdout + run.stderr
+
+
+@pytest.mark.parametrize("lens,counts", [([400, 2000, 130], [300, 20, 70]),       # long: its way through its keys is longer than the others', so not the prompt form
+                                         ([9000, 64, 900, 5000], [65, 64, 512, 16]), ([300] * 40 + [7] * 200, [20] * 40 + [1] * 200)])
+@pytest.mark.parametrize("H,G", [(32, 8), (10, 2), (5, 5)])
+def test_attention_of_requests_that_take_different_forms(H, G, lens, counts):
+    check_attention(make_attention(14, lens, counts, H, G, 128, 64, torch.float16), 128)
+
+
+def test_the_form_is_the_rules_and_both_kernels_agree_on_it():
+    """Rows of the prompt form and of the other one differ in their last bits: which form a request took shows in its rows."""
+    lens, counts, H, G = [900, 9000, 300, 1200, 40], [200, 30, 1, 500, 24], 32, 8
+    case = make_attention(15, lens, counts, H, G, 128, 64, torch.float16)
+    out, sms = check_attention(case, 128), torch.cuda.get_device_properties(0).multi_processor_count
+    forced = attend("pairs" if sum(counts) * H > 160 * sms else "prompt", *case, torch.empty_like(out), 128 ** -0.5, ops.kv4_attention_workspace("cuda"))
+    rows = [n * H // G for n in counts]
+    total = sum(r * G * -(-n // 128) for r, n in zip(rows, lens) if r >= 65)
+    picks = [r >= 65 and -(-n // 128) * (sms // 4 * 128) <= total for r, n in zip(rows, lens)]
+    assert picks == [True, False, False, True, True]
+    for b, pick in enumerate(picks):
+        at = slice(sum(counts[:b]), sum(counts[:b + 1]))
+        assert counts[b] == 1 or torch.equal(out[at], forced[at]) == pick
 
 
 def test_cache_whose_offsets_pass_32_bits():
