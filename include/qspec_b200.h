@@ -430,8 +430,8 @@ int qspec_debug_kv8_attention_give_up(const void* q, long long q_tok_stride, int
  *
  * qspec_kv4_append: as qspec_kv8_append; with hadamard != 0 rotated queries and keys are multiplied by the Hadamard matrix of D / sqrt(D) besides (both, so that their
  * products stay what they are, and channels that are large in all keys are spread over a row; butterflies of strides 1, 2 .. D / 2 in float32). Of a row of keys or values:
- * hi = max(largest, 0), lo = min(smallest, 0) of its finite values, which count as +-2^126 beyond that; s = max((hi - lo) / 15, 2^-60) rounded to five significant bits,
- * halves up; z = rint(-lo / s) (15 at most); c = clamp(rint(x / s) + z, 0, 15) (infinities: 15 and 0; NaN counts as 0). Rows do not depend on one another; tokens without a slot, or
+ * hi = max(largest, 0), lo = min(smallest, 0) of its finite values, which count as +-2^126 beyond that; s = max((hi - lo) * (1 / 15 as float32 has it), 2^-60) rounded to five significant
+ * bits, halves up; z = rint(-lo / s) (15 at most); c = clamp(rint(x / s) + z, 0, 15) (infinities: 15 and 0; NaN counts as 0). Rows do not depend on one another; tokens without a slot, or
  * with a position that the table of angles does not have, are skipped. The slots of a call differ from each other. */
 int qspec_kv4_append(const void* qkv, long long ld, const void* cos_sin, int cos_rows, const int* positions, const int* slots, void* k, void* v, void* k_word, void* v_word,
                      void* q_out, long long q_tok_stride, int ntok, int H, int G, int D, int npages, int page_tokens, int hadamard, int dtype, void* stream);

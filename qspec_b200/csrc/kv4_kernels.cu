@@ -9,8 +9,9 @@ namespace kv4 {
 // y = the rotation of x (neox pairs; queries and keys), then, if `hadamard`, y H / sqrt(D) with the Hadamard matrix of D (which leaves every product of a query and a key as it
 // is, and spreads a channel that is large in all keys over a row's columns). Of a row of keys or values, in float32:
 //   hi = max(largest, 0), lo = min(smallest, 0)   of the values that are finite; beyond 2^126 they count as 2^126
-//   s = max((hi - lo) / 15, 2^-60), rounded to five significant bits, halves up;   z = rint(-lo / s);   c = clamp(rint(x / s) + z, 0, 15)
-// All with the roundings that the formulas have (no fused multiply-adds, quotients correctly rounded), so that the same codes come out of every implementation in
+//   s = max((hi - lo) * (1 / 15), 2^-60), rounded to five significant bits, halves up;   z = rint(-lo / s);   c = clamp(rint(x / s) + z, 0, 15)
+// All with the roundings that the formulas have (no fused multiply-adds, quotients by s correctly rounded, 1 / 15 as float32 has it, which is a little more: halves stay halves or
+// above), so that the same codes come out of every implementation in
 // float32: scales of five bits and values of eight or eleven make quotients that lie halfway between two codes common.
 //
 // D / 16 lanes take a row; a lane holds sixteen of its values, eight of each half, so that it has both of every pair that the rotation turns, and the butterflies of the
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv4_append_kernel(const App
     }
     top = fmaxf(top, 0.f);
     low = fminf(low, 0.f);
-    const uint32_t bits = (__float_as_uint(fmaxf(__fdiv_rn(__fsub_rn(top, low), 15.f), SCALE_FLOOR)) + (1u << 18)) >> 19;
+    const uint32_t bits = (__float_as_uint(fmaxf(__fmul_rn(__fsub_rn(top, low), 1.f / 15.f), SCALE_FLOOR)) + (1u << 18)) >> 19;
     const float s = __uint_as_float(bits << 19), inv = __frcp_rn(s);
     const int zero = (int)fminf(rintf(__fdiv_rn(-low, s)), 15.f);
     uint32_t w[2] = {0u, 0u};

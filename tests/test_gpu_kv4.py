@@ -633,3 +633,24 @@ def test_wrong_shapes_and_types_are_refused():
             ops.kv4_attention(*[bad if j == i else a for j, a in enumerate(att)])
     with pytest.raises(ValueError):
         ops.kv4_read(*cache, z(3), half(3, 2, 64), half(2, 2, 64))
+
+
+def test_scales_next_to_a_half_are_those_of_the_formula():
+    """(hi - lo) * float32(1 / 15) within a few units of the last place of a border between two scales, on either side: a million rows, most of whose ranges lie there."""
+    G, D, P, n = 8, 64, 128, 128 * 1024
+    g = gen(30)
+    border = (16.5 + torch.randint(0, 16, (n, G), generator=g, device="cuda")) / 16 * 2.0 ** torch.randint(-6, 6, (n, G), generator=g, device="cuda") * 15
+    x = torch.randn(n, 3 * G, D, generator=g, device="cuda").clamp(-0.4, 0.4) * border.repeat(1, 3)[..., None] * 0.1
+    x[:, 2 * G:, 0] = border * 0.6
+    x[:, 2 * G:, 1] = -border * 0.4
+    x = x.bfloat16()                                          # (values: as they lie in the rows)
+    lo = x[:, 2 * G:].amin(-1).float()
+    x[:, 2 * G:, 0] = (border + lo).bfloat16()
+    k, v = (torch.zeros(n // P, G, P, D // 2, dtype=U8, device="cuda") for _ in range(2))
+    kw, vw = (torch.zeros(n // P, G, P, dtype=I16, device="cuda") for _ in range(2))
+    at = i32(range(n))
+    cs = torch.cat((torch.ones(n, D // 2), torch.zeros(n, D // 2)), 1).bfloat16().cuda()
+    ops.kv4_append(x.flatten(1), cs, at, at, k, v, kw, vw, None)
+    for got_c, got_w, rows in ((k, kw, x[:, G:2 * G]), (v, vw, x[:, 2 * G:])):
+        c, w = quantised(rows.float())
+        assert torch.equal(got_w, w.view(n // P, P, G).transpose(1, 2)) and torch.equal(got_c, c.view(n // P, P, G, D // 2).transpose(1, 2))
