@@ -22,11 +22,16 @@ from .model import QSpecLlamaModel
 
 
 class QSpecEngine:
-    def __init__(self, model: QSpecLlamaModel, batch: int, k: int = 3, use_cuda_graph: bool = True, temperature: float = 0.0, seed: int = 0):
+    def __init__(self, model: QSpecLlamaModel, batch: int, k: int = 3, use_cuda_graph: bool = True, temperature: float = 0.0, seed: int = 0, logprobs: Optional[int] = None):
         """temperature 0: greedy, a draft token is accepted iff it is the target's arg max. Above 0: tokens are drawn from softmax(logits / temperature) and draft
         tokens accepted with probability min(1, p / q), so that what is emitted is distributed as the target's own (vllm/model_executor/layers/
         rejection_sampler.py); `seed` decides the random numbers. (Over the 8-bit cache the target depends on the drafts a little: a page's scale does not shrink while its
         first row stands, so that rows of a draft that was refused, or that verification wrote over, may leave the page coarser than without them.)
+
+        logprobs: every step also leaves, on the device, what the target says of the tokens that it emits, under the distribution that they are drawn from (that of the logits if
+        greedy): `out_logprobs`, `out_entropy` float32 and `out_ranks` int64 [B, k + 1], and of every place the `logprobs` best tokens, `out_top_logprobs` float32 and
+        `out_top_tokens` int64 [B, k + 1, logprobs] (0: none of these; None: nothing). Behind what is emitted (out_count) the log probability and the rank are 0. (The reference gives them
+        with its sampler's output, vllm/spec_decode/spec_decode_worker.py.)
 
         Over a paged cache with fewer pages than all sequences may need, a step may find none for some of them: these emit nothing (out_count 0) and stay where they
         are. `step` raises for that at its first call behind a `prefill` and at every 64th, `metrics` at once; the next `prefill` begins with all pages."""
@@ -39,7 +44,13 @@ class QSpecEngine:
             raise NotImplementedError("sampling with a vocab-sharded lm_head")
         if temperature and k > (most := ops.max_verified_drafts()):
             raise ValueError(f"sampling verifies at most {most} draft tokens a step, got k = {k}")
-        self.temperature = float(temperature)
+        if logprobs is not None:
+            if model.tp_size != 1:
+                raise NotImplementedError("log probabilities with a vocab-sharded lm_head")
+            most = min(ops.max_top_logprobs(), model.cfg.vocab_size)
+            if not 0 <= logprobs <= most:
+                raise ValueError(f"logprobs: the best 0 to {most} tokens, got {logprobs}")
+        self.temperature, self.n_logprobs = float(temperature), logprobs
         dev = model.device
         B = batch
         assert model.max_tokens >= B * (k + 1)
@@ -54,6 +65,11 @@ class QSpecEngine:
         self.out_count = torch.zeros(B, dtype=torch.int64, device=dev)
         # SpecDecodeWorkerMetrics counters (metrics.py): accepted, draft, emitted
         self.counters = torch.zeros(3, dtype=torch.int64, device=dev)
+        if logprobs is not None:
+            self.out_logprobs, self.out_entropy = torch.zeros(B, k + 1, device=dev), torch.zeros(B, k + 1, device=dev)
+            self.out_ranks = torch.zeros(B, k + 1, dtype=torch.int64, device=dev)
+            self.out_top_logprobs = torch.zeros(B, k + 1, logprobs, device=dev)
+            self.out_top_tokens = torch.zeros(B, k + 1, logprobs, dtype=torch.int64, device=dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.stream = torch.cuda.Stream(device=dev)
         # pinned host mirrors for the end-to-end API
@@ -71,7 +87,7 @@ class QSpecEngine:
             self.generator = torch.Generator(device=dev).manual_seed(seed)
             self.draft_probs = torch.empty(k, B, V, dtype=torch.float32, device=dev)
             self.uniform = torch.empty(2, B, k + 1, dtype=torch.float32, device=dev)     # for the drafts, and for their verification
-        self.paged = getattr(model, "paged", None)                    # the model's 8-bit cache, if it has one
+        self.paged = getattr(model, "paged", None)                    # the model's paged cache, if it has one
         if self.paged is not None:
             self.counts = torch.full((B,), k + 1, dtype=torch.int32, device=dev)
             self.one_each = torch.arange(B + 1, dtype=torch.int32, device=dev)
@@ -122,9 +138,9 @@ class QSpecEngine:
         self.counters.zero_()
 
     # ---------------------------------------------------------------------------------------
-    def _probs(self, hidden: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def _probs(self, hidden: torch.Tensor, out: Optional[torch.Tensor] = None, logits: Optional[torch.Tensor] = None) -> torch.Tensor:
         """softmax(logits / temperature), float32 [rows, V]."""
-        return torch.softmax(self.model.logits(hidden).float().mul_(1.0 / self.temperature), -1, out=out)
+        return torch.softmax((self.model.logits(hidden) if logits is None else logits).float().mul_(1.0 / self.temperature), -1, out=out)
 
     @torch.no_grad()
     def _spec_step(self) -> None:
@@ -159,13 +175,14 @@ class QSpecEngine:
         else:
             vpos = (self.seq_len.unsqueeze(1) + self.arange_k1.unsqueeze(0)).reshape(-1).contiguous()
             hidden = m.forward(vt, vpos, self.vseq_ids, w4a4=False)
+        logits = m.logits(hidden) if self.n_logprobs is not None else None
         if self.temperature:
             drafts = (self.draft_toks, self.draft_probs.transpose(0, 1)) if k else (None, None)
-            ops.verify_drafts(*drafts, self._probs(hidden).view(B, k + 1, -1), self.uniform[1], self.out_tokens, self.out_count)
+            ops.verify_drafts(*drafts, self._probs(hidden, logits=logits).view(B, k + 1, -1), self.uniform[1], self.out_tokens, self.out_count)
             n_acc, emitted = self.out_count - 1, self.out_tokens
             nxt = emitted.gather(1, n_acc.unsqueeze(1)).squeeze(1)
         else:
-            tgt = m.greedy_tokens(hidden).view(B, k + 1)
+            tgt = (m.greedy_tokens(hidden) if logits is None else ops.argmax_rows(logits)).view(B, k + 1)
             # ---- greedy rejection (spec_decode_worker.py:861-915 with temperature 0)
             match = (tgt[:, :k] == self.draft_toks).to(torch.int64)
             n_acc = match.cumprod(dim=1).sum(dim=1)                     # accepted draft tokens per sequence
@@ -183,6 +200,10 @@ class QSpecEngine:
             emitted = emitted.masked_fill(~served.unsqueeze(1), -1)
             self.out_tokens.copy_(emitted)
             self.out_count.mul_(served)
+        if logits is not None:
+            top = (self.out_top_logprobs.flatten(0, 1), self.out_top_tokens.flatten(0, 1)) if self.n_logprobs else (None, None)
+            ops.token_logprobs(logits, self.out_tokens.view(-1), self.out_logprobs.view(-1), self.out_entropy.view(-1), self.out_ranks.view(-1), *top,
+                               temperature=self.temperature or 1.0)
         count = self.out_count
         self.cur_tok.copy_(nxt)
         self.seq_len.add_(count.to(torch.int32))
@@ -249,7 +270,7 @@ class QSpecEngine:
     def _check_pages(self) -> None:
         self._behind_steps()
         if refused := self.paged.refused():
-            raise RuntimeError(f"the 8-bit cache had no page {refused} time(s) for a sequence of a step, which then emitted nothing, or for a portion of a prompt, which is not in "
+            raise RuntimeError(f"the {self.paged.bits}-bit cache had no page {refused} time(s) for a sequence of a step, which then emitted nothing, or for a portion of a prompt, which is not in "
                                f"it ({self.paged.pages} pages of {self.paged.page_tokens} tokens)")
 
     def _behind_steps(self) -> None:

@@ -46,7 +46,7 @@ class QSpecLlamaConfig:
     heads_rotation: str = "sylvester"   # o_proj rotation across heads: Sylvester FHT (2^k heads) or "had40" (:269-277)
     qk_hadamard: bool = False        # per-head FHT_128 of q and k after the rotary embedding (:279-288)
     gate_first: bool = False         # merged gate_up rows [gate ; up] (vLLM SiluAndMul, :80-86) instead of Llama's [up ; gate]
-    kv_cache: str = "f16"            # "f16": [slot, position] rows; "int8": pages of 8-bit codes (paged.PagedKV8Cache)
+    kv_cache: str = "f16"            # "f16": [slot, position] rows; "int8", "uint4": pages of 8-bit or 4-bit codes (paged.PagedKV8Cache, PagedKV4Cache)
     kv_page: int = 64                # tokens of a page
     kv_pages: Optional[int] = None   # pages of the whole cache (None: enough for every sequence at its longest)
 
@@ -165,14 +165,14 @@ class QSpecLlamaModel(torch.nn.Module):
         # KV cache shared by draft and verify (worker.py:309-326 ref_initilize_cache)
         L, S = cfg.num_hidden_layers, cfg.max_seq_len
         self.max_batch = max_batch
-        if cfg.kv_cache not in ("f16", "int8"):
-            raise ValueError(f'kv_cache must be "f16" or "int8", got {cfg.kv_cache!r}')
+        if cfg.kv_cache not in ("f16", "int8", "uint4"):
+            raise ValueError(f'kv_cache must be "f16", "int8" or "uint4", got {cfg.kv_cache!r}')
         self.paged = None
-        if cfg.kv_cache == "int8":
-            if cfg.qk_hadamard:
+        if cfg.kv_cache != "f16":
+            if cfg.qk_hadamard and cfg.kv_cache == "int8":
                 raise ValueError("the 8-bit cache has no form with the Hadamard of queries and keys behind the rotary embedding")
-            from .paged import PagedKV8Cache
-            self.paged = PagedKV8Cache(L, self.hkv, D, max_batch, S, max_tokens, self.device, cfg.kv_page, cfg.kv_pages)
+            from .paged import PagedKV4Cache, PagedKV8Cache     # (the 4-bit one has no other)
+            self.paged = (PagedKV8Cache if cfg.kv_cache == "int8" else PagedKV4Cache)(L, self.hkv, D, max_batch, S, max_tokens, self.device, cfg.kv_page, cfg.kv_pages)
             self.cache_k = self.cache_v = None
             self.buf_q = torch.empty(max_tokens, self.hq, D, dtype=torch.float16, device=self.device)     # rotated queries
             self._ended: set = set()
@@ -225,7 +225,7 @@ class QSpecLlamaModel(torch.nn.Module):
             dist.all_reduce(t, group=self.tp_group)     # RowParallelLinear.forward, layers/linear.py:1143-1144
 
     def forward(self, input_ids: torch.Tensor, positions: Optional[torch.Tensor], seq_ids: Optional[torch.Tensor], w4a4: bool, step=None) -> torch.Tensor:
-        """input_ids/positions/seq_ids: [T] int (int32 positions/seq_ids). Returns final-norm hidden [T, H]. step: the tokens' places in the 8-bit cache
+        """input_ids/positions/seq_ids: [T] int (int32 positions/seq_ids). Returns final-norm hidden [T, H]. step: the tokens' places in the paged cache
         (`paged.PagedStep`; positions and seq_ids are not read then)."""
         for _ in self.forward_stages(input_ids, positions, seq_ids, w4a4, step):
             pass
@@ -239,7 +239,7 @@ class QSpecLlamaModel(torch.nn.Module):
         T = input_ids.numel()
         assert T <= self.max_tokens
         if (step is None) != (self.paged is None):
-            raise ValueError("forward: a model with the 8-bit cache takes a step of that cache, others none")
+            raise ValueError("forward: a model with a paged cache takes a step of that cache, others none")
         D, H = cfg.head_dim, cfg.hidden_size
         x = self.buf_x[:T]
         torch.index_select(self.embed, 0, input_ids, out=x)
@@ -420,7 +420,7 @@ class QSpecLlamaModel(torch.nn.Module):
             lengths[slot], counts[slot] = first, n
         step = cache.plan(on_device(lengths), on_device(counts), meta.ntok, max(counts))
         if self.cfg.kv_pages is not None and (refused := cache.short()):   # (with the default number of pages every sequence fits)
-            raise RuntimeError(f"the 8-bit cache is full: {cache.pages} pages of {cache.page_tokens} tokens have no room for {refused} sequence(s) of this step; none of it "
+            raise RuntimeError(f"the {cache.bits}-bit cache is full: {cache.pages} pages of {cache.page_tokens} tokens have no room for {refused} sequence(s) of this step; none of it "
                                "has been taken, and once sequences have been released it can be made again")
         cache.commit()
         ids = input_ids.to(torch.int64)

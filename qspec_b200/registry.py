@@ -110,9 +110,9 @@ def _load_totatar(path, cfg, dtype, device, n_slots: int = 8, max_step_tokens: i
                                         max_seq_tokens=max_seq_tokens)
 
 
-def _load_qspec_llama(path, cfg, dtype, device, n_slots: int = 8, max_step_tokens: int = 256, **_):
+def _load_qspec_llama(path, cfg, dtype, device, n_slots: int = 8, max_step_tokens: int = 256, kv_cache: str = "f16", **_):
     """The int4 dual-mode decoder (Llama-3 / Qwen2.5 shapes) from a Hugging Face style config.json; weights from the
-    folder's QuaRot-format safetensors shards if there are any, random otherwise."""
+    folder's QuaRot-format safetensors shards if there are any, random otherwise. kv_cache: of `model.QSpecLlamaConfig`."""
     import glob
     from .checkpoint import load_qspec_checkpoint
     from .model import QSpecLlamaConfig, QSpecLlamaModel
@@ -124,7 +124,7 @@ def _load_qspec_llama(path, cfg, dtype, device, n_slots: int = 8, max_step_token
     c = base(hidden_size=cfg["hidden_size"], intermediate_size=cfg["intermediate_size"], num_attention_heads=heads,
              num_key_value_heads=cfg.get("num_key_value_heads", heads), head_dim=cfg.get("head_dim", cfg["hidden_size"] // heads),
              num_hidden_layers=cfg["num_hidden_layers"], vocab_size=cfg["vocab_size"], rms_norm_eps=cfg.get("rms_norm_eps", 1e-5),
-             rope_theta=cfg.get("rope_theta", 500000.0), max_seq_len=cfg.get("max_position_embeddings", 1024))
+             rope_theta=cfg.get("rope_theta", 500000.0), max_seq_len=cfg.get("max_position_embeddings", 1024), kv_cache=kv_cache)
     model = QSpecLlamaModel(c, max_batch=n_slots, max_tokens=max_step_tokens, device=device)
     if glob.glob(os.path.join(path, "*.safetensors")):
         load_qspec_checkpoint(model, path)

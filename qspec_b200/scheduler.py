@@ -36,6 +36,19 @@ class Request:
     fed: int = 0                                   # prompt tokens already consumed
     output: List[int] = field(default_factory=list)
     done: bool = False
+    logprobs: Optional[int] = None                 # best alternatives wanted with each token's log probability (None: neither)
+    scores: List["TokenScore"] = field(default_factory=list)
+
+
+@dataclass
+class TokenScore:
+    """What the model says of one token: its log probability, its rank (1: the likeliest), the entropy of the distribution that it comes from (nats), and the likeliest tokens
+    with their log probabilities."""
+    token: int
+    logprob: float
+    rank: int
+    entropy: float
+    top: List[Tuple[int, float]]
 
 
 class Scheduler:
@@ -124,13 +137,56 @@ class Scheduler:
             if self._release_slot is not None:
                 self._release_slot(slot)
 
+    # ---- log probabilities ------------------------------------------------------------------------------------------
+    def _scores(self, logits: torch.Tensor, tokens: Sequence[int], top: int) -> List[TokenScore]:
+        """Of tokens[i] under row i of the logits. Reads the device."""
+        n, dev = len(tokens), logits.device
+        ids = torch.tensor(tokens, dtype=torch.int64, device=dev)
+        lp, entropy, ranks = torch.empty(n, device=dev), torch.empty(n, device=dev), torch.empty(n, dtype=torch.int64, device=dev)
+        best = (torch.empty(n, top, device=dev), torch.empty(n, top, dtype=torch.int64, device=dev)) if top else (None, None)
+        ops.token_logprobs(logits, ids, lp, entropy, ranks, *best)
+        alternatives = [list(zip(t, p)) for p, t in zip(best[0].tolist(), best[1].tolist())] if top else [[] for _ in range(n)]
+        return [TokenScore(*row) for row in zip(tokens, lp.tolist(), ranks.tolist(), entropy.tolist(), alternatives)]
+
+    def score(self, texts: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenScore]]:
+        """What the model says of each text's tokens behind the first, each given those in front of it, with the `top` likeliest tokens of each place: the exponential of minus the
+        log probabilities' mean is the text's perplexity. One text after the other, a step's tokens at a time; needs a free slot."""
+        self._check_top(top)
+        results = []
+        for k, text in enumerate(texts):
+            rid, text = ("score", self.steps, k), list(text)
+            if not text:
+                raise ValueError("empty text")
+            limit = getattr(self.model, "max_seq_len", None)
+            if limit is not None and len(text) - 1 > limit:   # (before any of it is taken)
+                raise RuntimeError(f"a text of {len(text)} tokens; the cache takes {limit}")
+            scores: List[TokenScore] = []
+            try:
+                for at in range(0, len(text) - 1, self.prefill_portion):
+                    part = text[at:min(at + self.prefill_portion, len(text) - 1)]
+                    logits = self.feed([(rid, part, list(range(len(part))))])
+                    scores += self._scores(logits, text[at + 1:at + 1 + len(part)], top)
+            finally:
+                self.release(rid)
+            results.append(scores)
+        return results
+
+    def _check_top(self, top: Optional[int]) -> None:
+        if top is None:
+            return
+        most = min(ops.max_top_logprobs(), self.model.vocab_size)
+        if not 0 <= top <= most:
+            raise ValueError(f"the best 0 to {most} tokens can be had, got {top}")
+
     # ---- generation -------------------------------------------------------------------------------------------------
-    def add(self, rid: Hashable, prompt: Sequence[int], max_new_tokens: int, eos: Optional[int] = None) -> None:
+    def add(self, rid: Hashable, prompt: Sequence[int], max_new_tokens: int, eos: Optional[int] = None, logprobs: Optional[int] = None) -> None:
+        """logprobs: the request's tokens come with a `TokenScore` each (`Request.scores`), with so many alternatives."""
         if not len(prompt):
             raise ValueError("empty prompt")
+        self._check_top(logprobs)
         if rid in self.finished or any(r.rid == rid for r in list(self.waiting) + self.running):
             raise ValueError(f"request id {rid!r} is already known")
-        self.waiting.append(Request(rid, list(prompt), max_new_tokens, eos))
+        self.waiting.append(Request(rid, list(prompt), max_new_tokens, eos, logprobs=logprobs))
 
     def has_work(self) -> bool:
         return bool(self.waiting or self.running)
@@ -167,6 +223,11 @@ class Scheduler:
         self.steps += 1
         toks = ops.argmax_rows(logits).tolist() if logits.shape[0] else []
         sampled = []
+        if toks and any(r.logprobs is not None for r in owners):
+            for r, score in zip(owners, self._scores(logits, [int(t) for t in toks], max(r.logprobs or 0 for r in owners))):
+                if r.logprobs is not None:
+                    score.top = score.top[:r.logprobs]
+                    r.scores.append(score)
         for r, t in zip(owners, toks):
             r.output.append(int(t))
             sampled.append((r.rid, int(t)))
@@ -179,9 +240,13 @@ class Scheduler:
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, eos: Optional[int] = None) -> List[List[int]]:
         """Greedy continuation of every prompt; more prompts than slots queue up and run as slots come free."""
+        return [r.output for r in self.generate_requests(prompts, max_new_tokens, eos)]
+
+    def generate_requests(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, eos: Optional[int] = None, logprobs: Optional[int] = None) -> List[Request]:
+        """`generate`, with all that is known of the finished requests (`Request.scores`)."""
         ids = [("gen", self.steps, k) for k in range(len(prompts))]
         for rid, p in zip(ids, prompts):
-            self.add(rid, p, max_new_tokens, eos)
+            self.add(rid, p, max_new_tokens, eos, logprobs)
         while self.has_work():
             self.step()
-        return [self.finished.pop(rid).output for rid in ids]
+        return [self.finished.pop(rid) for rid in ids]
