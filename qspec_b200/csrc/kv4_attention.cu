@@ -25,6 +25,10 @@ namespace qspec {
 namespace kv4 {
 using namespace kv8;
 
+constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr int CTAS = 2;                          // of an SM: while one waits at a barrier the other computes
+constexpr int GRID_MOST = 320;                   // CTAs
+
 struct AttArgs : Step, Out {
   const void* q; long long q_ts; int q_hs;
   const uint8_t *k, *v;
@@ -37,15 +41,15 @@ template <int D> struct Smem {
   static constexpr int WORDS = 2 * CODES, STAGE = WORDS + 2 * UNIT * 2;   // keys, values, words of either
   static constexpr int FACTORS = 16 * 16 * 2 + 8 * 16;                    // what the words of a unit's keys come to, in the order of the products
   static constexpr int WARP = STAGES * STAGE + FACTORS;
-  static constexpr size_t RING = (size_t)WARPS * WARP;
-  static constexpr size_t Q = ROWS * D * 2;
   static constexpr int LD = D + 8;                                      // floats of a row of sums on its way between warps
-  static constexpr size_t SUMS = (size_t)WARPS * ROWS * LD * 4, PARTS = (size_t)(GRID_MOST + 1) * ROWS * 4;
-  static constexpr size_t O = SUMS > PARTS ? SUMS : PARTS;              // sums on their way between warps, or a factor for every part of an item
+  // units, or (at a segment's end) sums on their way between warps, or a factor for every part of an item
+  static constexpr size_t RING = (size_t)WARPS * WARP, SUMS = (size_t)WARPS * ROWS * LD * 4, PARTS = (size_t)(GRID_MOST + 1) * ROWS * 4;
+  static constexpr size_t ROOM = RING > SUMS ? (RING > PARTS ? RING : PARTS) : SUMS > PARTS ? SUMS : PARTS;
+  static constexpr size_t Q = ROWS * D * 2;
   static constexpr size_t ML = (size_t)WARPS * ROWS * 2 * 4;
   static constexpr size_t F = ROWS * 4;                                 // the rows' powers of two
-  static constexpr size_t TOTAL = RING + Q + O + ML + F;
-  static_assert(STAGE % 16 == 0 && WARP % 16 == 0, "16-byte boundaries");
+  static constexpr size_t TOTAL = ROOM + Q + ML + F;
+  static_assert(STAGE % 16 == 0 && WARP % 16 == 0 && ROOM % 16 == 0, "16-byte boundaries");
 };
 
 __device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -55,6 +59,10 @@ template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 // two 16 x 16 blocks of bytes, columns first: word 2 m + h of a lane has rows 4 j .. 4 j + 3 (j = lane % 4) of column lane / 4 + 8 h of block m
 __device__ __forceinline__ void load_columns(uint32_t (&w)[4], uint32_t addr) {
@@ -79,7 +87,9 @@ __device__ __forceinline__ uint32_t half_fma(uint32_t a, uint32_t b, uint32_t c)
   const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t half_bits(float x) { return __half_as_ushort(__float2half_rn(x)); }
+// (x & mask) | magic in one instruction, which two constants would make two: they are kept in registers.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) { uint32_t r; asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(r) : "r"(x), "r"(mask), "r"(magic)); return r; }
+__device__ __forceinline__ uint32_t held(uint32_t x) { uint32_t r; asm volatile("mov.b32 %0, %1;\n" : "=r"(r) : "r"(x)); return r; }
 
 // Where the 16 bytes c of a row lie in a buffer, so that neither copies nor reads of eight rows meet in a bank (a row is half a line of banks, or a quarter).
 template <int D> __device__ __forceinline__ uint32_t k_row(int row) {   // of eight lanes four read a row and four the row two behind it
@@ -89,28 +99,25 @@ template <int D> __device__ __forceinline__ uint32_t v_chunk(int row, int c) {
   return (uint32_t)(D == 128 ? row * 64 + c * 16 ^ (row >> 1 & 3) << 4 : row * 32 + c * 16 ^ (row >> 2 & 1) << 4);
 }
 
-// A unit's codes and words: 16 rows lie in one page, whatever its size. Rows behind the last key are not fetched: what the buffer holds in their place is never used but as codes, which
-// are codes like any other and meet weights of zero.
+// A unit's codes and words that lie in two pages, or are fewer than UNIT: 16 rows at a time. Rows behind the last key are not fetched: what the buffer holds in their place is never used
+// but as codes, which are codes like any other and meet weights of zero.
 template <int D>
-__device__ __forceinline__ void fetch(const AttArgs& a, const Unit& n, uint32_t dst, int lane) {
+__device__ __noinline__ void fetch_parts(const uint8_t* k, const uint8_t* v, const uint16_t* kw, const uint16_t* vw, int pshift, long long row, int have, uint32_t dst) {
   using S = Smem<D>;
   constexpr int CH = D / 32, PER = 32 / CH;       // 16-byte pieces of a row; rows per instruction
-  const int c = lane % CH, row0 = lane / CH, have = n.keys - n.key0;
-#pragma unroll
+  const int lane = threadIdx.x & 31, c = lane % CH, row0 = lane / CH;
+#pragma unroll 1
   for (int q = 0; q < UNIT / 16; ++q) {
-    const long long at = __shfl_sync(0xffffffffu, n.at, (16 * q) >> a.pshift);
+    const long long at = __shfl_sync(0xffffffffu, row, q);
     if (at < 0 || 16 * q >= have) continue;
-    const size_t first = (size_t)at + ((n.key0 + 16 * q) & ((1 << a.pshift) - 1));   // row of the cache
-    const uint8_t *ks = a.k + (first + row0) * S::ROW + c * 16, *vs = a.v + (first + row0) * S::ROW + c * 16;
-#pragma unroll
-    for (int i = 0; i < 16 / PER; ++i) {
-      const int row = 16 * q + i * PER + row0;
-      if (row < have) {
-        copy16(dst + k_row<D>(row) + c * 16, ks + i * PER * S::ROW);
-        copy16(dst + S::CODES + v_chunk<D>(row, c), vs + i * PER * S::ROW);
+    const size_t first = (size_t)at + (pshift >= 5 ? 16 * q : 0);
+#pragma unroll 1
+    for (int r = row0; r < 16; r += PER)
+      if (16 * q + r < have) {
+        copy16(dst + k_row<D>(16 * q + r) + c * 16, k + (first + r) * S::ROW + c * 16);
+        copy16(dst + S::CODES + v_chunk<D>(16 * q + r, c), v + (first + r) * S::ROW + c * 16);
       }
-    }
-    if (lane < 4) copy16(dst + S::WORDS + (lane >> 1) * UNIT * 2 + q * 32 + (lane & 1) * 16, (lane >> 1 ? a.vw : a.kw) + first + (lane & 1) * 8);
+    if (lane < 4) copy16(dst + S::WORDS + (lane >> 1) * UNIT * 2 + q * 32 + (lane & 1) * 16, (lane >> 1 ? vw : kw) + first + (lane & 1) * 8);
   }
 }
 
@@ -120,93 +127,128 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
   using S = Smem<D>;
   constexpr int NT = D / 8, W = D / 32, KT = UNIT / 8, QT = UNIT / 16;   // column tiles of the value product, words that a lane has of a key, key tiles
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ Shared s_sh;
+  __shared__ Shared<WARPS> s_sh;
+  __shared__ Stretch s_stretch;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, qi = lane >> 2, qj = lane & 3;
-  unsigned char* const s_q = smem + S::RING;
-  float* const s_o = reinterpret_cast<float*>(smem + S::RING + S::Q);
-  float* const s_ml = reinterpret_cast<float*>(smem + S::RING + S::Q + S::O);   // [warp][maximum, sum][16]
-  float* const s_f = reinterpret_cast<float*>(smem + S::RING + S::Q + S::O + S::ML);   // [16]
+  unsigned char* const s_q = smem + S::ROOM;
+  float* const s_o = reinterpret_cast<float*>(smem);
+  float* const s_ml = reinterpret_cast<float*>(smem + S::ROOM + S::Q);   // [warp][maximum, sum][16]
+  float* const s_f = reinterpret_cast<float*>(smem + S::ROOM + S::Q + S::ML);   // [16]
   const uint32_t ring = shared_addr(smem) + warp * S::WARP, factors = ring + S::STAGES * S::STAGE;
   pdl_enter();
 
+  // The stretch stays in shared memory (its place is that of the segment that all warps are in: the rest of one item): registers are what there is least of.
   unsigned long long work;
-  Stretch stretch;
-  if (!find_stretch(a, s_sh, work, stretch)) return;
-  Place cur = stretch.cur;                                  // the segment that all warps are in: (the rest of) one item
-  const int todo = stretch.todo;
+  {
+    Stretch stretch;
+    if (!find_stretch<WARPS, GRID_MOST>(a, s_sh, work, stretch)) return;
+    if (tid == 0) s_stretch = stretch;
+  }
 
   // Queries of an item: a thread's pieces of 8 values (rows behind the last one are zeros), then float16 in the order in which the products take them: word (step, lane,
   // register) of the operand. A lane's word i of a key has columns 8 (W j + i) .. + 7; step 2 i takes the first and the second of each four of them, step 2 i + 1 the
   // third and the fourth.
-  constexpr int IN_ROW = D / 8, PIECES_Q = ROWS * IN_ROW / THREADS, QROWS = THREADS / IN_ROW;
+  constexpr int IN_ROW = D / 8;
+  static_assert(ROWS * IN_ROW <= THREADS, "a piece a thread");
   const int qr = tid / IN_ROW, qc = tid % IN_ROW;
-  uint4 queries[PIECES_Q];
   auto load_q = [&](const Place& p) {
-#pragma unroll
-    for (int i = 0; i < PIECES_Q; ++i) {
-      const int row = p.tile * ROWS + qr + i * QROWS, tok = row / a.rep;
-      queries[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (tok < p.r.n)
-        queries[i] = *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(p.r.first + tok) * a.q_ts + (size_t)(p.g * a.rep + row - tok * a.rep) * a.q_hs + qc * 8);
-    }
+    const int row = p.tile * ROWS + qr, tok = row / a.rep;
+    uint4 piece = make_uint4(0u, 0u, 0u, 0u);
+    if (qr < ROWS && tok < p.r.n)
+      piece = *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(p.r.first + tok) * a.q_ts + (size_t)(p.g * a.rep + row - tok * a.rep) * a.q_hs + qc * 8);
+    return piece;
   };
-  auto store_q = [&]() {
+  auto store_q = [&](const uint4& piece) {
+    float x[8], mx = 0.f;
+    unpack8<BF16>(piece, x);
 #pragma unroll
-    for (int i = 0; i < PIECES_Q; ++i) {
-      const int row = qr + i * QROWS;
-      float x[8], mx = 0.f;
-      unpack8<BF16>(queries[i], x);
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(x[e]));
+    for (int o = IN_ROW / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    // 2^(14 - exponent of the largest), from its bits, in float32's range at both ends; none for a row of zeros or one that is not finite
+    const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+    const bool some = mx > 0.f && mx < INFINITY;
+    const int sh = some ? min(max(14 - ex, -126), 126) : 0;
+    const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
 #pragma unroll
-      for (int o = IN_ROW / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      // 2^(14 - exponent of the largest), from its bits, in float32's range at both ends; none for a row of zeros or one that is not finite
-      const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
-      const bool some = mx > 0.f && mx < INFINITY;
-      const int sh = some ? min(max(14 - ex, -126), 126) : 0;
-      const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= e & 1 ? up * 0.0625f : up;
-      if (qc == 0) s_f[row] = __uint_as_float((uint32_t)(some ? 127 - sh : 1) << 23);   // (those have no say in the tile's largest)
-      uint32_t* to = reinterpret_cast<uint32_t*>(s_q) + (qc % W) * 2 * 128 + ((row & 7) * 4 + qc / W) * 4 + (row >> 3);
-      to[0] = half_pair(x[0], x[4]);
-      to[2] = half_pair(x[1], x[5]);
-      to[128] = half_pair(x[2], x[6]);
-      to[130] = half_pair(x[3], x[7]);
-    }
+    for (int e = 0; e < 8; ++e) x[e] *= e & 1 ? up * 0.0625f : up;
+    if (qr >= ROWS) return;
+    if (qc == 0) s_f[qr] = __uint_as_float((uint32_t)(some ? 127 - sh : 1) << 23);   // (those have no say in the tile's largest)
+    uint32_t* to = reinterpret_cast<uint32_t*>(s_q) + (qc % W) * 2 * 128 + ((qr & 7) * 4 + qc / W) * 4 + (qr >> 3);
+    to[0] = half_pair(x[0], x[4]);
+    to[2] = half_pair(x[1], x[5]);
+    to[128] = half_pair(x[2], x[6]);
+    to[130] = half_pair(x[3], x[7]);
   };
 
-  // ---- the first units of this warp are on their way before anything else. Pages are looked up one unit ahead of the copies, so that these do not wait for them.
-  int next = warp;                                          // index in the stretch of the unit that is fetched next
-  Place np = cur;
-  np.forward(a, work, warp);
-  int pages = next < todo ? unit_page(a, np, lane) : -1;
-  auto take = [&]() {                                       // the unit at np, and the pages of the one behind it
-    Unit unit;
-    unit.at = pages >= 0 ? (long long)(((size_t)pages * a.G + np.g) << a.pshift) : -1ll;
-    unit.key0 = np.u * UNIT;
-    unit.keys = next < todo ? np.r.keys : 0;
-    np.forward(a, work, WARPS);
+  // ---- a segment's units: warp w's are w, w + WARPS, .., two of them under way. Pages are looked up one unit ahead of the copies, so that these do not wait for them: a unit lies in one
+  // page, or (of 16 tokens) in two, of which odd lanes have the second.
+  const int mask = (1 << a.pshift) - 1, second = a.pshift == 4 ? lane & 1 : 0;
+  const int* table;                                         // the segment's request's
+  int g, keys, next, end;                                   // its head and keys; the unit that is fetched next, the end of the segment's units
+  auto look = [&]() {
+    if (next >= end) return -1;
+    const int at = (next * UNIT >> a.pshift) + second;
+    if ((at << a.pshift) >= keys || at >= a.width) return -1;
+    const int page = table[at];
+    return (unsigned)page < (unsigned)a.npages ? page : -1;
+  };
+  int pages;
+  struct Unit4 {
+    bool there;                                             // this lane's page
+    int key0;                                               // first key
+  };
+  // a lane's places in a unit that lies in one page: 512 bytes of codes an instruction, of which its 16 are always in the same place of their rows
+  const uint32_t kdst = k_row<D>(lane / (D / 32)) + lane % (D / 32) * 16, vdst = v_chunk<D>(lane / (D / 32), lane % (D / 32));
+  const uint32_t wdst = S::WORDS + (lane & 7) * 16;
+  auto take = [&](uint32_t dst) {                           // the next unit, and the pages of the one behind it
+    Unit4 unit;
+    unit.there = pages >= 0;
+    unit.key0 = next * UNIT;
+    const int have = next < end ? keys - unit.key0 : 0;
+    const long long row = unit.there ? (long long)((((size_t)pages * a.G + g) << a.pshift) + (unit.key0 & mask)) : -1ll;
+    if (a.pshift >= 5 && have >= UNIT) {                    // (the same for all lanes)
+      if (unit.there) {
+        const long long off = row * S::ROW + lane * 16;
+        const uint8_t *ks = a.k + off, *vs = a.v + off;
+#pragma unroll
+        for (int i = 0; i < S::CODES / 512; ++i) {
+          // (what a row's number shifts its pieces by repeats after eight rows)
+          copy16(dst + kdst + i * 512, ks + i * 512);
+          copy16(dst + S::CODES + vdst + i * 512, vs + i * 512);
+        }
+        if (lane < 8) copy16(dst + wdst, (lane & 4 ? a.vw : a.kw) + row + (lane & 3) * 8);
+      }
+    } else {
+      fetch_parts<D>(a.k, a.v, a.kw, a.vw, a.pshift, row, have, dst);
+    }
+    copy_commit();
     next += WARPS;
-    pages = next < todo ? unit_page(a, np, lane) : -1;
+    pages = look();
     return unit;
   };
-  load_q(cur);
-  Unit unit0 = take();
-  fetch<D>(a, unit0, ring, lane);
-  copy_commit();
-  Unit unit1 = take();
-  fetch<D>(a, unit1, ring + S::STAGE, lane);
-  copy_commit();
-  store_q();
-  __syncthreads();
 
+  const uint32_t low4 = held(0x000f000fu), high4 = held(0x00f000f0u), magic = held(0x64006400u);
+  // where this lane's key leaves what it comes to
+  const uint32_t words = ring + S::WORDS + lane * 2, mine = factors + (((lane >> 4) * 2 + (lane & 1)) * 4 + (lane >> 2 & 3)) * 16 + (lane >> 1 & 1) * 4;
+  const uint32_t zeros = factors + 512 + ((lane >> 4) * 4 + (lane >> 2 & 3)) * 16 + (lane & 1) * 4 + (lane >> 1 & 1) * 2;
   int seg0 = 0;                                             // index in the stretch of the segment's first unit
-  int here = warp;                                          // index of the unit that is in the ring's next stage
-  uint32_t stage = 0;
-  while (seg0 < todo) {
-    const int seg_n = min(cur.r.units - cur.u, todo - seg0);
+  __syncthreads();
+  for (;;) {
+    const Place cur = s_stretch.cur;
+    const int seg_n = min(cur.r.units - cur.u, s_stretch.todo - seg0);
     const int tile = cur.tile;
+    table = a.table + (size_t)cur.b * a.width;
+    g = cur.g;
+    keys = cur.r.keys;
+    next = cur.u + warp;
+    end = cur.u + seg_n;
+    pages = look();
+    const uint4 piece = load_q(cur);
+    Unit4 unit0 = take(ring), unit1 = take(ring + S::STAGE);
+    store_q(piece);
+    __syncthreads();
+    uint32_t stage = 0;
     const uint32_t frag = shared_addr(s_q) + lane * 16;
     auto query = [&](uint32_t (&x)[4], int step) { lds128(x, frag + step * 512); };
     // The rows' powers of two: the tile's largest goes into the keys' factors, what a row is below it (at most 1) stays the row's.
@@ -229,36 +271,31 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
       query(x, i);
       mma16816(sums, x, 0x00010001u, 0x00100010u);
     }
-    const uint64_t sum2[2] = {two(sums[0], sums[0]), two(sums[2], sums[2])}, own2[2] = {two(own[0], own[0]), two(own[1], own[1])};
     float o[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
     float m[2] = {NONE, NONE};
-    uint64_t l2[2] = {0ull, 0ull};
+    uint64_t l2[2] = {0ull, 0ull};                          // sums of weights / v
 
-    while (here < seg0 + seg_n) {
+    for (int here = cur.u + warp; here < end; here += WARPS) {
       const uint32_t buf = ring + stage * S::STAGE;
-      const int key0 = unit0.key0, have = unit0.keys - key0;
+      const int key0 = unit0.key0;
       copy_wait<1>();
       __syncwarp();
       // ---- a lane a key: what its words come to. Key 16 q + 4 j + 2 b + z is column 2 j + b of score tile 2 q + z.
       {
-        const int q = lane >> 4, j = lane >> 2 & 3, b = lane >> 1 & 1, z = lane & 1;
-        const bool broken = __shfl_sync(0xffffffffu, unit0.at, (16 * q) >> a.pshift) < 0;
-        const uint32_t kw = lds16(buf + S::WORDS + lane * 2), vw = lds16(buf + S::WORDS + UNIT * 2 + lane * 2);
-        const float ks = word_scale(kw), vs = word_scale(vw);
-        float f = fmaxf(positive(ks) * factor, 1.17549435e-38f) * 16777216.f, v = positive(vs);
-        if (broken || !(ks < INFINITY) || !(vs < INFINITY)) { f = NAN; v = 1.f; }   // rows that see it are no numbers
-        if (lane >= have) { f = 0.f; v = 1.f; }
-        const uint32_t at = factors + ((q * 2 + z) * 4 + j) * 16 + b * 4;
-        sts32(at, __float_as_uint(f));
-        sts32(at + 8, __float_as_uint(-(float)(kw & 15u)));
-        sts32(at + 256, __float_as_uint(__log2f(v)));
-        sts32(at + 264, __float_as_uint(__fdividef(WEIGHT_UNIT, v)));
-        const uint32_t zat = factors + 512 + (q * 4 + j) * 16 + z * 4 + b * 2;
-        const float zero = (float)(vw & 15u);
-        sts16(zat, half_bits(-1024.f - zero));
-        sts16(zat + 8, half_bits(-64.f - zero));
+        const bool broken = !(__ballot_sync(0xffffffffu, unit0.there) >> (lane >> 4) & 1u);
+        const uint32_t kw = lds16(words + stage * S::STAGE), vw = lds16(words + stage * S::STAGE + UNIT * 2);
+        const bool bad = broken || kw >= 0xff00u || vw >= 0xff00u;   // (exponent 255: infinite, or no number)
+        float f = word_scale(kw) * factor * 16777216.f, v = fmaxf(word_scale(vw), 7.888609052210118e-31f);
+        if (bad) { f = NAN; v = 1.f; }                      // rows that see it are no numbers
+        if (key0 + lane >= keys) f = 0.f;
+        sts32(mine, __float_as_uint(f));
+        sts32(mine + 8, __float_as_uint(__uint_as_float(0xcb000000u | (kw & 15u)) + 8388608.f));   // - z
+        sts32(mine + 256, __float_as_uint(__log2f(v)));
+        sts32(mine + 264, __float_as_uint(__fdividef(WEIGHT_UNIT, v)));
+        sts16(zeros, 0xe400u + (vw & 15u));                 // -1024 - z
+        sts16(zeros + 8, 0xd400u + ((vw & 15u) << 4));      // -64 - z
       }
       // ---- scores of the unit's keys, in units of 2^-24
       float s[KT][4];
@@ -268,7 +305,6 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
         for (int n = 0; n < KT; ++n) {
           const uint32_t at = buf + k_row<D>((n >> 1) * 16 + (n & 1) + (qi >> 1) * 4 + (qi & 1) * 2) + qj * (W * 4);
           if constexpr (W == 4) lds128(w[n], at); else lds64(w[n], at);
-          s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
         }
 #pragma unroll
         for (int i = 0; i < W; ++i) {
@@ -276,27 +312,28 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
           query(x, 2 * i);
           query(y, 2 * i + 1);
 #pragma unroll
-          for (int n = 0; n < KT; ++n) mma16816(s[n], x, w[n][i] & 0x000f000fu, w[n][i] & 0x00f000f0u);
+          for (int n = 0; n < KT; ++n) {
+            if (i == 0) mma16816_first(s[n], x, w[n][i] & 0x000f000fu, w[n][i] & 0x00f000f0u);
+            else mma16816(s[n], x, w[n][i] & 0x000f000fu, w[n][i] & 0x00f000f0u);
+          }
 #pragma unroll
           for (int n = 0; n < KT; ++n) mma16816(s[n], y, w[n][i] >> 8 & 0x000f000fu, w[n][i] >> 8 & 0x00f000f0u);
         }
       }
       __syncwarp();                                         // (the factors are there)
       // ---- exponents
-      uint64_t iv2[KT];
       float mx[2] = {NONE, NONE};
 #pragma unroll
       for (int n = 0; n < KT; ++n) {
-        uint32_t x[4], y[4];
+        uint32_t x[4], y[2];
         const uint32_t at = factors + (n * 4 + qj) * 16;
         lds128(x, at);
-        lds128(y, at + 256);
+        lds64(y, at + 256);
         const uint64_t f = two(__uint_as_float(x[0]), __uint_as_float(x[1])), zero = two(__uint_as_float(x[2]), __uint_as_float(x[3])), lv = two(__uint_as_float(y[0]), __uint_as_float(y[1]));
-        iv2[n] = two(__uint_as_float(y[2]), __uint_as_float(y[3]));
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint64_t score = ffma2_rn(zero, sum2[e], two(s[n][2 * e], s[n][2 * e + 1]));
-          const float2 r = unpack_f2(ffma2_rn(score, mul2(f, own2[e]), lv));
+          const uint64_t score = ffma2_rn(zero, two(sums[2 * e], sums[2 * e]), two(s[n][2 * e], s[n][2 * e + 1]));
+          const float2 r = unpack_f2(ffma2_rn(score, mul2(f, two(own[e], own[e])), lv));
           s[n][2 * e] = r.x;
           s[n][2 * e + 1] = r.y;
         }
@@ -313,13 +350,13 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
 #pragma unroll
         for (int e = 0; e < 2; ++e) mx[e] = fmaxf(fmaxf(mx[e], s[n][2 * e]), s[n][2 * e + 1]);
       // The reference follows the maximum only where it has fallen behind: sums are seldom multiplied again.
-      if (__any_sync(0xffffffffu, mx[0] > m[0] + GROWTH_LOG2 || mx[1] > m[1] + GROWTH_LOG2 || (m[0] == NONE && mx[0] > NONE) || (m[1] == NONE && mx[1] > NONE))) {
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + GROWTH_LOG2 || mx[1] > m[1] + GROWTH_LOG2)) {   // (of a row that had seen nothing, more than minus infinity)
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
           mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-          const bool grown = mx[e] > m[e] + GROWTH_LOG2 || (m[e] == NONE && mx[e] > NONE);
+          const bool grown = mx[e] > m[e] + GROWTH_LOG2;
           f[e] = grown && m[e] != NONE ? exp2_fast(m[e] - mx[e]) : 1.f;   // (a row that had seen nothing has sums of zero)
           if (grown) m[e] = mx[e];
           l2[e] = mul2(l2[e], two(f[e], f[e]));
@@ -329,15 +366,17 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
       }
       // ---- weights
       uint32_t pa[QT][4];
+      const float ref[2] = {m[0] == NONE ? 0.f : WEIGHT_LOG2 - m[0], m[1] == NONE ? 0.f : WEIGHT_LOG2 - m[1]};
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float ref = m[e] == NONE ? 0.f : WEIGHT_LOG2 - m[e];
-        const uint64_t ref2 = two(ref, ref);
+      for (int n = 0; n < KT; ++n) {
+        uint32_t y[2];
+        lds64(y, factors + (n * 4 + qj) * 16 + 264);
+        const uint64_t iv = two(__uint_as_float(y[0]), __uint_as_float(y[1]));
 #pragma unroll
-        for (int n = 0; n < KT; ++n) {
-          const float2 x = unpack_f2(add2(two(s[n][2 * e], s[n][2 * e + 1]), ref2));
+        for (int e = 0; e < 2; ++e) {
+          const float2 x = unpack_f2(add2(two(s[n][2 * e], s[n][2 * e + 1]), two(ref[e], ref[e])));
           const float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
-          l2[e] = ffma2_rn(two(w0, w1), iv2[n], l2[e]);
+          l2[e] = ffma2_rn(two(w0, w1), iv, l2[e]);
           pa[n >> 1][(n & 1) * 2 + e] = half_pair(w0, w1);
         }
       }
@@ -353,25 +392,20 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const uint32_t u = w[t], v = w[t] >> 8;
-            mma16816(o[4 * c + 2 * t], pa[q], half_add((u & 0x000f000fu) | 0x64006400u, zero[0]), half_add((v & 0x000f000fu) | 0x64006400u, zero[1]));
-            mma16816(o[4 * c + 2 * t + 1], pa[q], half_fma((u & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, zero[2]),
-                     half_fma((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, zero[3]));   // (times 1 / 16)
+            mma16816(o[4 * c + 2 * t], pa[q], half_add(and_or(u, low4, magic), zero[0]), half_add(and_or(v, low4, magic), zero[1]));
+            mma16816(o[4 * c + 2 * t + 1], pa[q], half_fma(and_or(u, high4, magic), 0x2c002c00u, zero[2]),
+                     half_fma(and_or(v, high4, magic), 0x2c002c00u, zero[3]));   // (times 1 / 16)
           }
         }
       }
       __syncwarp();                                         // the unit behind the next takes this one's place
       unit0 = unit1;
-      unit1 = take();
-      fetch<D>(a, unit1, buf, lane);
-      copy_commit();
-      here += WARPS;
+      unit1 = take(buf);
       stage ^= 1u;
     }
+    copy_wait<0>();
+    __syncthreads();                                        // (sums take the units' place)
 
-    Place after = cur;
-    after.forward(a, work, seg_n);
-    const bool more = seg0 + seg_n < todo;
-    if (more) load_q(after);                                // the next segment's queries, on their way while sums are joined
     // ---- the warps' sums of this item together
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -390,13 +424,13 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
         for (int t = 0; t < NT; t += 2) *reinterpret_cast<float4*>(row + 8 * t) = make_float4(o[t][2 * e], o[t + 1][2 * e], o[t][2 * e + 1], o[t + 1][2 * e + 1]);
       }
     }
-    finish_segment<BF16, D, S::LD>(a, a, stretch, cur, seg0, seg_n, s_ml, s_o, s_sh);
-    if (more) store_q();                                    // (all have passed the barrier behind their last use of this item's)
-    cur = after;
+    finish_segment<BF16, D, S::LD, WARPS>(a, a, s_stretch, s_stretch.cur, seg0, seg_n, s_ml, s_o, s_sh);
     seg0 += seg_n;
-    __syncthreads();                                        // the sums have been read, the next queries are there
+    if (seg0 >= s_stretch.todo) break;
+    __syncthreads();                                        // the sums have been read, and so has the segment's place
+    if (tid == 0) s_stretch.cur.forward(a, work, seg_n);
+    __syncthreads();
   }
-  copy_wait<0>();
 }
 
 }  // namespace kv4

@@ -24,6 +24,10 @@
 namespace qspec {
 namespace kv8 {
 
+constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int CTAS = 3;                          // of an SM: while one waits at a barrier the others compute
+constexpr int GRID_MOST = 480;                   // CTAs
+
 struct AttArgs : Step, Out {
   const void* q; long long q_ts; int q_hs;
   const signed char *k, *v;
@@ -103,7 +107,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
   using S = Smem<D>;
   constexpr int NT = D / 8, CH = D / 16, KT = UNIT / 8, QT = UNIT / 16;   // column tiles of the value product, 16-byte pieces of a key (steps of the score product), key tiles
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ Shared s_sh;
+  __shared__ Shared<WARPS> s_sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, qi = lane >> 2, qj = lane & 3;
   unsigned char* const s_q = smem + S::RING;
   float* const s_o = reinterpret_cast<float*>(smem + S::RING + S::Q);
@@ -114,7 +118,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
 
   unsigned long long work;
   Stretch stretch;
-  if (!find_stretch(a, s_sh, work, stretch)) return;
+  if (!find_stretch<WARPS, GRID_MOST>(a, s_sh, work, stretch)) return;
   Place cur = stretch.cur;                                  // the segment that all warps are in: (the rest of) one item
   const int todo = stretch.todo;
 
@@ -367,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
         for (int t = 0; t < NT; ++t) *reinterpret_cast<float2*>(row + 8 * t) = make_float2(o[t][2 * e], o[t][2 * e + 1]);
       }
     }
-    finish_segment<BF16, D, S::LD>(a, a, stretch, cur, seg0, seg_n, s_ml, s_o, s_sh);
+    finish_segment<BF16, D, S::LD, WARPS>(a, a, stretch, cur, seg0, seg_n, s_ml, s_o, s_sh);
     if (more) store_q();                                    // (all have passed the barrier behind their last use of this item's)
     cur = after;
     seg0 += seg_n;

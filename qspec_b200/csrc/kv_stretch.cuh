@@ -10,10 +10,7 @@
 namespace qspec {
 namespace kv8 {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, UNIT = 32, ROWS = 16;
-constexpr int MIN_UNITS = WARPS;                 // of a stretch: one for each warp
-constexpr int CTAS = 3;                          // of an SM: while one waits at a barrier the others compute
-constexpr int GRID_MOST = 480;                   // CTAs
+constexpr int UNIT = 32, ROWS = 16;
 constexpr float NONE = -INFINITY;
 template <int D> constexpr int PART = ROWS * 2 + ROWS * D;   // floats of a part: maxima, sums, sums of values
 
@@ -74,8 +71,8 @@ struct Unit {
   long long at;                                   // -1: no such page
   int key0, keys;
 };
-// This CTA's stretch of the work. All threads of the CTA call it; its barriers are the CTA's. false: there is nothing for this CTA.
-struct Shared {
+// This CTA's stretch of the work, of WARPS warps, in a grid of GRID_MOST CTAs at most. All threads of the CTA call it; its barriers are the CTA's. false: there is nothing for this CTA.
+template <int WARPS> struct Shared {
   long long sum[WARPS];
   int place[4], items[WARPS], ctas[6][WARPS];
   Req req;
@@ -87,7 +84,9 @@ struct Stretch {
   int share, todo;                                          // units that a CTA of such an item takes; units of this stretch
   long long begin, per;
 };
-__device__ __forceinline__ bool find_stretch(const Step& a, Shared& s, unsigned long long& work_out, Stretch& out) {
+template <int WARPS, int GRID_MOST>
+__device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, unsigned long long& work_out, Stretch& out) {
+  constexpr int THREADS = WARPS * 32, MIN_UNITS = WARPS;   // units of a stretch: one for each warp
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per_thread = (a.nreq + THREADS - 1) / THREADS, b0 = tid * per_thread;
   const int requests = max(min(per_thread, a.nreq - b0), 0);
@@ -221,9 +220,10 @@ struct Out {
 };
 // The warps' sums of an item's segment (units cur.u .. cur.u + seg_n - 1, from the stretch's unit seg0 on) together: s_ml [warp][maximum, sum][16], s_o
 // [warp][16][LD] sums of values, written by the warps (not by one that saw nothing); to the rows, or, of a part of an item, into the workspace.
-template <bool BF16, int D, int LD>
-__device__ __forceinline__ void finish_segment(const Step& a, const Out& o, const Stretch& w0, const Place& cur, int seg0, int seg_n, float* s_ml, float* s_o, Shared& s) {
+template <bool BF16, int D, int LD, int WARPS>
+__device__ __forceinline__ void finish_segment(const Step& a, const Out& o, const Stretch& w0, const Place& cur, int seg0, int seg_n, float* s_ml, float* s_o, Shared<WARPS>& s) {
   using T = typename Elem16<BF16>::T;
+  constexpr int THREADS = WARPS * 32;
   const int tid = threadIdx.x;
   __syncthreads();
   constexpr int PER_ROW = THREADS / ROWS, PIECES = D / 4 / PER_ROW;   // threads of a row, float4 of a thread
