@@ -24,6 +24,7 @@ struct AppendArgs {
   uint16_t *kw, *vw;
   void* q; long long q_ts;
   int ntok, H, G, npages, pshift, rows;           // rows of a token: keys, values, and queries if they are wanted
+  int warps, steps;                               // warps of a token, rows of a warp in steps
 };
 constexpr int APPEND_WARPS = 8;
 constexpr float SCALE_FLOOR = 8.673617379884035e-19f, MOST = 8.507059173023462e37f;   // 2^-60, 2^126
@@ -58,29 +59,29 @@ __device__ __forceinline__ void butterflies(float (&x)[16], int c, uint32_t grou
   }
 }
 
-// N rows of a token per group of lanes
-template <bool BF16, int D, bool HADAMARD, int N>
-__global__ void __launch_bounds__(APPEND_WARPS * 32) kv4_append_kernel(const AppendArgs a) {
+// A warp takes `steps` times ROWS rows of a token, the next ones on their way: one look at the position and the angles for all of them. (Steps of two rows a lane, of which a warp took
+// no others, 37 us for a prompt of 4200 tokens, 40 / 8 heads; these 27; two steps ahead, and three CTAs an SM, 31.)
+template <bool BF16, int D, bool HADAMARD>
+__global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv4_append_kernel(const AppendArgs a) {
   using T = typename Elem16<BF16>::T;
   constexpr int LANES = D / 16, ROWS = 32 / LANES;          // lanes of a row, rows of a warp at a time
   const int lane = threadIdx.x & 31, c = lane % LANES, row0 = lane / LANES;
   const uint32_t group = LANES == 8 ? 0xffu << (lane & 24) : 0xfu << (lane & 28);
-  const int per_token = (a.rows + N * ROWS - 1) / (N * ROWS);   // warps of a token
   const unsigned id = blockIdx.x * APPEND_WARPS + (threadIdx.x >> 5);
-  const int t = (int)(id / (unsigned)per_token), r0 = (int)(id % (unsigned)per_token) * N * ROWS + row0;
+  const int t = (int)(id / (unsigned)a.warps), r0 = (int)(id % (unsigned)a.warps) * a.steps * ROWS + row0, end = min(r0 - row0 + a.steps * ROWS, a.rows);
   pdl_enter();
   if (t >= a.ntok) return;
   const int pos = a.positions[t], slot = a.slots[t];
   // rows of a token, in this order: keys, values, queries; they lie as queries, keys, values
-  auto column = [&](int r) { return (r < 2 * a.G ? a.H + r : r - 2 * a.G) * D; };
   const T* const from = (const T*)a.qkv + (size_t)t * a.ld + c * 8;
-  uint4 lo[N], hi[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int r = min(r0 + i * ROWS, a.rows - 1);
-    lo[i] = *reinterpret_cast<const uint4*>(from + column(r));
-    hi[i] = *reinterpret_cast<const uint4*>(from + column(r) + D / 2);
-  }
+  uint4 lo, hi;
+  auto load = [&](int r) {
+    if (r >= end) return;
+    const T* row = from + (r < 2 * a.G ? a.H + r : r - 2 * a.G) * D;
+    lo = __ldg(reinterpret_cast<const uint4*>(row));
+    hi = __ldg(reinterpret_cast<const uint4*>(row + D / 2));
+  };
+  load(r0);
   if ((unsigned)pos >= (unsigned)a.cos_rows) return;
   const bool kept = slot >= 0 && slot < a.npages << a.pshift;
   float cs[8], sn[8];
@@ -89,15 +90,13 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv4_append_kernel(const App
     unpack8<BF16>(*reinterpret_cast<const uint4*>(tab), cs);
     unpack8<BF16>(*reinterpret_cast<const uint4*>(tab + D / 2), sn);
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int r = r0 + i * ROWS;
-    if (r >= a.rows || (r < 2 * a.G && !kept)) continue;    // (the same for all lanes of a row)
+  auto row = [&](int r, const uint4& lo_r, const uint4& hi_r) {
+    if (r >= end || (r < 2 * a.G && !kept)) return;         // (the same for all lanes of a row)
     float x[16];
     {
       float l[8], h[8];
-      unpack8<BF16>(lo[i], l);
-      unpack8<BF16>(hi[i], h);
+      unpack8<BF16>(lo_r, l);
+      unpack8<BF16>(hi_r, h);
       if (r < a.G || r >= 2 * a.G) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -114,7 +113,7 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv4_append_kernel(const App
       T* to = (T*)a.q + (size_t)t * a.q_ts + (r - 2 * a.G) * D + c * 8;
       *reinterpret_cast<uint4*>(to) = pack8<BF16>(*reinterpret_cast<const float(*)[8]>(&x[0]));
       *reinterpret_cast<uint4*>(to + D / 2) = pack8<BF16>(*reinterpret_cast<const float(*)[8]>(&x[8]));
-      continue;
+      return;
     }
     float top = x[0], low = x[0];
 #pragma unroll
@@ -164,10 +163,16 @@ __global__ void __launch_bounds__(APPEND_WARPS * 32) kv4_append_kernel(const App
     *reinterpret_cast<uint32_t*>(to) = w[0];
     *reinterpret_cast<uint32_t*>(to + D / 4) = w[1];
     if (c == 0) (r < a.G ? a.kw : a.vw)[at] = (uint16_t)(bits << 4 | (uint32_t)zero);
+  };
+#pragma unroll 1
+  for (int r = r0; r - row0 < end; r += ROWS) {
+    const uint4 l = lo, h = hi;
+    load(r + ROWS);
+    row(r, l, h);
   }
 }
 
-// ---- rows back in 16 bits: out[i, g] = the values of slot i, keys and values. Eight values a thread; slots that are none give zeros.
+// ---- rows back in 16 bits: out[i, g] = the values of slot i, keys and values. Sixteen values a thread; slots that are none give zeros.
 template <bool BF16>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* k, const uint8_t* v, const uint16_t* kw, const uint16_t* vw, const int* slots, void* ko, void* vo, unsigned chunks,
                                                        int G, int dshift, int npages, int pshift) {
@@ -177,19 +182,24 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* k, const u
   const uint16_t* words = blockIdx.y ? vw : kw;
   T* out = (T*)(blockIdx.y ? vo : ko);
   for (unsigned i = blockIdx.x * 256 + threadIdx.x; i < chunks; i += gridDim.x * 256) {
-    const unsigned c = i & ((1u << (dshift - 3)) - 1u), row = i >> (dshift - 3);
-    const int g = (int)(row % (unsigned)G);
+    const unsigned c = i & ((1u << (dshift - 4)) - 1u), row = i >> (dshift - 4);
     const int s = slots[row / (unsigned)G];
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    uint2 w = make_uint2(0u, 0u);
+    uint32_t word = 0u;
     if (s >= 0 && s < npages << pshift) {
-      const size_t at = (((size_t)(s >> pshift) * G + g) << pshift) + (s & ((1 << pshift) - 1));
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + (at << (dshift - 1)) + c * 4), word = words[at];
-      const float f = word_scale(word);
-      const int zero = (int)(word & 15u);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)((int)(w >> (4 * e) & 15u) - zero), f);
+      const size_t at = (((size_t)(s >> pshift) * G + row % (unsigned)G) << pshift) + (s & ((1 << pshift) - 1));
+      w = *reinterpret_cast<const uint2*>(codes + (at << (dshift - 1)) + c * 8);
+      word = words[at];
     }
-    *reinterpret_cast<uint4*>(out + (size_t)i * 8) = pack8<BF16>(x);
+    const float f = word_scale(word), zero = 8388608.f + (float)(word & 15u);
+    uint4* to = reinterpret_cast<uint4*>(out + (size_t)i * 16);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(__uint_as_float(0x4b000000u | ((h ? w.y : w.x) >> (4 * e) & 15u)) - zero, f);   // (2^23 + c) - (2^23 + z)
+      to[h] = pack8<BF16>(x);
+    }
   }
 }
 
@@ -218,21 +228,21 @@ extern "C" int qspec_kv4_append(const void* qkv, long long ld, const void* cos_s
   QSPEC_REQUIRE(ld >= (long long)(H + 2 * G) * D && ld % 8 == 0 && (!q_out || (q_tok_stride >= (long long)H * D && q_tok_stride % 8 == 0)) && ((uintptr_t)qkv & 15) == 0 &&
                     ((uintptr_t)cos_sin & 15) == 0 && ((uintptr_t)q_out & 15) == 0,
                 QSPEC_ERR_INVALID_ARG, "kv4_append: rows must lie on 16-byte boundaries (ld=%lld)", ld);
-  const AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (uint8_t*)k, (uint8_t*)v, (uint16_t*)k_word, (uint16_t*)v_word, q_out, q_tok_stride, ntok, H, G, npages,
-                     page_shift(page_tokens), 2 * G + (q_out ? H : 0)};
-  auto run = [&](auto kern, int n) -> int {
-    const int rows = n * (D == 128 ? 4 : 8), per_token = (a.rows + rows - 1) / rows;
-    const long long warps = (long long)ntok * per_token;
-    QSPEC_REQUIRE(warps < (1ll << 31), QSPEC_ERR_UNSUPPORTED, "kv4_append: %d tokens are too many for one call", ntok);
-    QSPEC_CUDA(launch_pdl(kern, dim3((unsigned)((warps + APPEND_WARPS - 1) / APPEND_WARPS)), dim3(APPEND_WARPS * 32), 0, (cudaStream_t)stream, a));
-    QSPEC_CHECK_LAUNCH(1);
-    return QSPEC_OK;
-  };
-  const bool many = (long long)ntok * a.rows > 64ll * max(sm_count(), 1) * (D == 128 ? 4 : 8);
-#define QSPEC_KV4_APPEND(BF, DD, HH) (many ? run(kv4_append_kernel<BF, DD, HH, 2>, 2) : run(kv4_append_kernel<BF, DD, HH, 1>, 1))
-#define QSPEC_KV4_APPEND_D(BF, HH) (D == 128 ? QSPEC_KV4_APPEND(BF, 128, HH) : QSPEC_KV4_APPEND(BF, 64, HH))
-  if (dtype == QSPEC_DTYPE_F16) return hadamard ? QSPEC_KV4_APPEND_D(false, true) : QSPEC_KV4_APPEND_D(false, false);
-  return hadamard ? QSPEC_KV4_APPEND_D(true, true) : QSPEC_KV4_APPEND_D(true, false);
+  AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (uint8_t*)k, (uint8_t*)v, (uint16_t*)k_word, (uint16_t*)v_word, q_out, q_tok_stride, ntok, H, G, npages,
+               page_shift(page_tokens), 2 * G + (q_out ? H : 0), 0, 0};
+  // Steps of a warp: as few as leave about APPEND_FULL warps an SM.
+  constexpr int APPEND_FULL = 48;
+  const int rows = D == 128 ? 4 : 8, most = (a.rows + rows - 1) / rows;
+  a.steps = (int)std::min<long long>(std::max<long long>((long long)ntok * most / (APPEND_FULL * (long long)max(sm_count(), 1)), 1), most);
+  a.warps = (most + a.steps - 1) / a.steps;
+  const long long warps = (long long)ntok * a.warps;
+  QSPEC_REQUIRE(warps < (1ll << 31), QSPEC_ERR_UNSUPPORTED, "kv4_append: %d tokens are too many for one call", ntok);
+#define QSPEC_KV4_APPEND(BF) (D == 128 ? (hadamard ? kv4_append_kernel<BF, 128, true> : kv4_append_kernel<BF, 128, false>) : hadamard ? kv4_append_kernel<BF, 64, true> : kv4_append_kernel<BF, 64, false>)
+  auto kern = dtype == QSPEC_DTYPE_F16 ? QSPEC_KV4_APPEND(false) : QSPEC_KV4_APPEND(true);
+#undef QSPEC_KV4_APPEND
+  QSPEC_CUDA(launch_pdl(kern, dim3((unsigned)((warps + APPEND_WARPS - 1) / APPEND_WARPS)), dim3(APPEND_WARPS * 32), 0, (cudaStream_t)stream, a));
+  QSPEC_CHECK_LAUNCH(1);
+  return QSPEC_OK;
 }
 
 extern "C" int qspec_kv4_read(const void* k, const void* v, const void* k_word, const void* v_word, const int* slots, void* k_out, void* v_out, int rows, int G, int D, int npages,
@@ -242,8 +252,8 @@ extern "C" int qspec_kv4_read(const void* k, const void* v, const void* k_word, 
   QSPEC_REQUIRE(rows > 0 && slots && k_out && v_out, QSPEC_ERR_INVALID_ARG, "kv4_read: null pointer or rows=%d", rows);
   QSPEC_REQUIRE(dtype == QSPEC_DTYPE_F16 || dtype == QSPEC_DTYPE_BF16, QSPEC_ERR_UNSUPPORTED, "kv4_read: float16 or bfloat16 rows");
   QSPEC_REQUIRE(((uintptr_t)k_out & 15) == 0 && ((uintptr_t)v_out & 15) == 0, QSPEC_ERR_INVALID_ARG, "kv4_read: rows must lie on 16-byte boundaries");
-  const long long chunks = (long long)rows * G * (D / 8);
-  QSPEC_REQUIRE(chunks < (1ll << 31), QSPEC_ERR_UNSUPPORTED, "kv4_read: %d rows are too many for one call", rows);
+  const long long chunks = (long long)rows * G * (D / 16);
+  QSPEC_REQUIRE(chunks < (1ll << 30), QSPEC_ERR_UNSUPPORTED, "kv4_read: %d rows are too many for one call", rows);
   const int grid = (int)std::min<long long>((chunks + 255) / 256, (long long)max(sm_count(), 1) * 8);
   auto kern = dtype == QSPEC_DTYPE_F16 ? kv4_read_kernel<false> : kv4_read_kernel<true>;
   QSPEC_CUDA(launch_pdl(kern, dim3(grid, 2), dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)k, (const uint8_t*)v, (const uint16_t*)k_word, (const uint16_t*)v_word, slots, k_out,
