@@ -6,7 +6,8 @@
 // What bounds it is reading the row, once, and the exponentials. One CTA, or a cluster of up to eight, takes a row; a CTA walks its span in batches of 1024 vectors of 16 bytes, the
 // next batch's loads under way. The first batch's maximum is where exponents are counted from; only if a value is 2^60 above it the sums are multiplied again. Candidates for
 // the best are, of the first batch, the values that reach the smallest of as many groups' maxima as are asked for, or more (at least that many do, and hardly more than some
-// hundred), and later on those above the worst of the best so far, which is brought up to date whenever four times as much has been seen: a few at a time. Where there are more than there
+// hundred), and later on those above the worst of the best so far, which is brought up to date whenever four (or, of up to eight, eight) times as much has been
+// seen: a few at a time. Where there are more than there
 // is room for (rows that rise, rows of one value), the span is looked through once for each one that is asked for. Whichever way, values are ordered together with their
 // tokens as whole numbers of 64 bits, so that there is one result. Sums are made in a fixed order in float32.
 #include "seq_common.cuh"
@@ -17,7 +18,7 @@ namespace qspec {
 namespace logprob {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, MOST_TOP = 32, EACH = 4;   // EACH: vectors of a thread in a batch
-constexpr int GROUPS = 64, GROUP = THREADS / GROUPS, HITS = 256, CANDIDATES = 512;   // groups of neighbouring threads; vectors with candidates, candidates in them
+constexpr int GROUPS = 128, GROUP = THREADS / GROUPS, HITS = 256, CANDIDATES = 512;   // groups of neighbouring threads; vectors with candidates, candidates in them
 constexpr float AHEAD = 60.f;                     // a value 2^AHEAD above the reference moves it
 typedef unsigned long long u64;
 
@@ -48,7 +49,7 @@ __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32
 __device__ __forceinline__ u64 add2(u64 a, u64 b) { u64 r; asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ u64 mul2(u64 a, u64 b) { u64 r; asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b)); return r; }
 
-// A vector's values: the largest (no number if one is none), all of them, how many are above `given`.
+// A vector's values: the largest (no number if one is none), all of them, how many are above another.
 template <typename T> struct Lanes;
 template <> struct Lanes<float> {
   static __device__ __forceinline__ float largest(const uint4& w) {
@@ -57,9 +58,14 @@ template <> struct Lanes<float> {
   static __device__ __forceinline__ void values(const uint4& w, float (&x)[4]) {
     x[0] = __uint_as_float(w.x); x[1] = __uint_as_float(w.y); x[2] = __uint_as_float(w.z); x[3] = __uint_as_float(w.w);
   }
-  static __device__ __forceinline__ int above(const uint4& w, float given) {
-    return (__uint_as_float(w.x) > given) + (__uint_as_float(w.y) > given) + (__uint_as_float(w.z) > given) + (__uint_as_float(w.w) > given);
+  // how many are above `given`, of up to EACH vectors, in pairs of their own
+  typedef u64 Count;
+  static __device__ __forceinline__ Count none() { return 0ull; }
+  static __device__ __forceinline__ void above(Count& n, const uint4& w, float given) {
+    auto one = [&](uint32_t x) { return __uint_as_float(x) > given ? 1.f : 0.f; };
+    n = add2(n, add2(pack_f2(one(w.x), one(w.y)), pack_f2(one(w.z), one(w.w))));
   }
+  static __device__ __forceinline__ int total(const Count& n) { const float2 f = unpack_f2(n); return (int)(f.x + f.y); }
 };
 #define QSPEC_LANES16(T, T2, SUFFIX, UNPACK, FROM)                                                                                                               \
   template <> struct Lanes<T> {                                                                                                                                  \
@@ -70,12 +76,14 @@ template <> struct Lanes<float> {
       return max_nan(value(h.x), value(h.y));                                                                                                                    \
     }                                                                                                                                                            \
     static __device__ __forceinline__ void values(const uint4& w, float (&x)[8]) { UNPACK(w, x); }                                                                \
-    static __device__ __forceinline__ int above(const uint4& w, float given) {   /* (given is one of the row's values: exact) */                                 \
+    typedef T2 Count;                                                                                                                                            \
+    static __device__ __forceinline__ Count none() { return FROM(0.f); }                                                                                         \
+    static __device__ __forceinline__ void above(Count& n, const uint4& w, float given) {   /* (given is one of the row's values; sums to 4 EACH: exact) */      \
       const T2 g = FROM(given);                                                                                                                                  \
       const T2* h = reinterpret_cast<const T2*>(&w);                                                                                                             \
-      const T2 n = __hadd2(__hadd2(__hgt2(h[0], g), __hgt2(h[1], g)), __hadd2(__hgt2(h[2], g), __hgt2(h[3], g)));                                                \
-      return (int)(value(n.x) + value(n.y));                                                                                                                     \
+      n = __hadd2(n, __hadd2(__hadd2(__hgt2(h[0], g), __hgt2(h[1], g)), __hadd2(__hgt2(h[2], g), __hgt2(h[3], g))));                                             \
     }                                                                                                                                                            \
+    static __device__ __forceinline__ int total(const Count& n) { return (int)(value(n.x) + value(n.y)); }                                                       \
   };
 QSPEC_LANES16(__half, __half2, "f16x2", unpack_h8, __float2half2_rn)
 QSPEC_LANES16(__nv_bfloat16, __nv_bfloat162, "bf16x2", unpack_b8, __float2bfloat162_rn)
@@ -93,20 +101,58 @@ __device__ __forceinline__ float value_of(u64 key) {
 }
 __device__ __forceinline__ int index_of(u64 key) { return (int)~(uint32_t)key; }
 
-// The n-th largest of the groups' maxima (n <= GROUPS): as many values reach it, or more. Every warp finds it for itself.
+// Floats as numbers in their order.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+// A value that as many of the groups' maxima reach as are asked for (n <= GROUPS), or some more: the n-th largest, but for the lower half of its bits. Every warp finds it for itself.
 __device__ __forceinline__ float nth_largest(const float* s_group, int n) {
-  const int lane = threadIdx.x & 31;
-  const float mine[2] = {s_group[lane], s_group[lane + 32]};
-  int larger[2] = {0, 0};
-#pragma unroll 4
-  for (int j = 0; j < GROUPS; ++j) {
-    const float x = s_group[j];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) larger[e] += x > mine[e] || (x == mine[e] && j < lane + 32 * e);
+  static_assert(GROUPS == 128, "four a lane");
+  const float4 x = reinterpret_cast<const float4*>(s_group)[threadIdx.x & 31];
+  const uint32_t k[4] = {ordered(x.x) >> 16, ordered(x.y) >> 16, ordered(x.z) >> 16, ordered(x.w) >> 16};
+  uint32_t t = 0;
+#pragma unroll 1
+  for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+    const uint32_t y = t | bit;
+    if (__reduce_add_sync(0xffffffffu, (k[0] >= y) + (k[1] >= y) + (k[2] >= y) + (k[3] >= y)) >= n) t = y;
   }
-  const uint32_t first = __ballot_sync(0xffffffffu, larger[0] == n - 1), second = __ballot_sync(0xffffffffu, larger[1] == n - 1);
-  const float x = __shfl_sync(0xffffffffu, mine[0], __ffs(first | 0x80000000u) - 1), y = __shfl_sync(0xffffffffu, mine[1], __ffs(second | 0x80000000u) - 1);
-  return first ? x : second ? y : -INFINITY;
+  const uint32_t u = t << 16;
+  return t <= 0x7fu ? -INFINITY : __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);   // (0x7f: minus infinity and what is next to it)
+}
+
+// The vector at value `first` of the span's n, which may lie over its ends.
+template <typename T>
+__device__ __noinline__ uint4 edge(const T* from, int n, int first) {
+  constexpr int E = Vec<T>::N;
+  uint4 w;
+  if (first >= 0 && first + E <= n) {
+    w = __ldg(reinterpret_cast<const uint4*>(from + first));
+  } else {
+    T* const x = reinterpret_cast<T*>(&w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = first + e >= 0 && first + e < n ? from[first + e] : lowest<T>();
+  }
+  return w;
+}
+
+// The largest key below `before` of this thread's vectors; 0: there is none.
+template <typename T>
+__device__ __noinline__ u64 best_below(const T* from, int n, int shift, int lo, u64 before) {
+  constexpr int E = Vec<T>::N;
+  u64 most = 0;
+#pragma unroll 1
+  for (int first = (int)threadIdx.x * E - shift; first < n; first += THREADS * E) {
+    const uint4 w = edge<T>(from, n, first);
+    const T* const x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = first + e;
+      const u64 key = key_of(value(x[e]), lo + i);
+      if (i >= 0 && i < n && key < before && key > most) most = key;
+    }
+  }
+  return most;
 }
 
 template <typename T, int CLUSTER>
@@ -116,33 +162,34 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
   __shared__ Partial s_part;
   __shared__ u64 s_best[MOST_TOP], s_key[CANDIDATES], s_most[WARPS];
   __shared__ uint4 s_hit[HITS];
-  __shared__ float s_group[GROUPS], s_ref[WARPS], s_sum[2][WARPS];
-  __shared__ int s_above[WARPS], s_where[HITS], s_hits, s_count;
+  __shared__ __align__(16) float s_group[GROUPS];
+  __shared__ float s_ref[WARPS], s_sum[2][WARPS];
+  __shared__ int s_above[WARPS], s_where[HITS], s_hits[2], s_count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER;
-  if (tid == 0) s_hits = s_count = 0;
+  if (tid == 0) s_hits[0] = s_hits[1] = s_count = 0;
   pdl_enter();
   const T* const x_row = (const T*)a.logits + (size_t)row * a.stride;
   const int lo = min(rank * a.span, a.V), n = min(a.span, a.V - lo);
   const T* const from = x_row + lo;
   // Vectors lie on 16-byte boundaries, the first and the last may lie over the span's ends: what stands there is minus infinity instead.
   const int shift = (int)(((uintptr_t)from & 15) / sizeof(T)), vectors = n > 0 ? (n + shift + E - 1) / E : 0;
-  auto load = [&](int v) {
-    const int first = v * E - shift;
-    uint4 w;
-    if (first >= 0 && first + E <= n) {
-      w = __ldg(reinterpret_cast<const uint4*>(from + first));
-    } else {
-      T* const x = reinterpret_cast<T*>(&w);
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = first + e >= 0 && first + e < n ? from[first + e] : lowest<T>();
-    }
-    return w;
-  };
-  const int batches = (vectors + THREADS * EACH - 1) / (THREADS * EACH);
+  const uint4* const at0 = reinterpret_cast<const uint4*>(from - shift) + tid;
+  const int inner0 = shift ? 1 : 0, inner1 = (n + shift) / E;   // vectors that are the span's as a whole
+  constexpr int BATCH = THREADS * EACH;
+  const int batches = (vectors + BATCH - 1) / BATCH;
   uint4 next[EACH];
+  auto load = [&](int b) {
+    const int v = b * BATCH;
+    if (v >= inner0 && v + BATCH <= inner1) {               // (nearly always)
 #pragma unroll
-  for (int j = 0; j < EACH; ++j) next[j] = load(j * THREADS + tid);
+      for (int j = 0; j < EACH; ++j) next[j] = __ldg(at0 + v + j * THREADS);
+    } else {
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) next[j] = edge<T>(from, n, (v + j * THREADS + tid) * E - shift);
+    }
+  };
+  load(0);
   const long long token = a.tokens ? a.tokens[row] : -1;
   const bool there = token >= 0 && token < a.V;
   const float given = there ? value(x_row[token]) : INFINITY;   // (nothing is above it)
@@ -152,16 +199,14 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
   float limit = -INFINITY;                                  // what a value that is looked at more closely reaches
   auto set_limit = [&]() { limit = none ? -INFINITY : fminf(reach, ref + AHEAD / a.c); };
   u64 S2 = 0, U2 = 0;
-  int above = 0, best = 0, check = 0;                       // check: the batch behind which the best are brought up to date
+  int above = 0, best = 0, check = 0, turn = 0;             // check: the batch behind which the best are brought up to date; turn: which count of hits is in use
+  bool lost = false;                                        // there were more candidates than there is room for
   bool odd = false;                                         // there is something that is no number
   for (int b = 0; b < batches; ++b) {
     uint4 w[EACH];
 #pragma unroll
     for (int j = 0; j < EACH; ++j) w[j] = next[j];
-    if (b + 1 < batches) {
-#pragma unroll
-      for (int j = 0; j < EACH; ++j) next[j] = load(((b + 1) * EACH + j) * THREADS + tid);
-    }
+    if (b + 1 < batches) load(b + 1);
     float big[EACH];
 #pragma unroll
     for (int j = 0; j < EACH; ++j) big[j] = L::largest(w[j]);
@@ -172,7 +217,10 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
       for (int o = 1; o < GROUP; o <<= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
       if (tid % GROUP == 0) s_group[tid / GROUP] = g;
       __syncthreads();
-      ref = max_nan(s_group[lane], s_group[lane + 32]);
+      {
+        const float4 x = reinterpret_cast<const float4*>(s_group)[lane];
+        ref = max_nan(max_nan(x.x, x.y), max_nan(x.z, x.w));
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) ref = max_nan(ref, __shfl_xor_sync(0xffffffffu, ref, o));
       if (a.top) reach = nth_largest(s_group, a.top);
@@ -195,12 +243,18 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
 #pragma unroll
       for (int j = 0; j < EACH; ++j)
         if (b == 0 ? big[j] >= reach : big[j] > reach) {
-          const int at = atomicAdd(&s_hits, 1);             // (in any order: they are put in theirs)
+          const int at = atomicAdd(&s_hits[turn], 1);             // (in any order: they are put in theirs)
           if (at < HITS) {
             s_hit[at] = w[j];
             s_where[at] = ((b * EACH + j) * THREADS + tid) * E - shift;
           }
         }
+    }
+    if (a.ranks) {
+      typename L::Count larger = L::none();
+#pragma unroll
+      for (int j = 0; j < EACH; ++j) L::above(larger, w[j], given);
+      above += L::total(larger);
     }
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
@@ -216,13 +270,13 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
         S2 = add2(S2, w2);
         U2 = ffma2_rn(w2, y2, U2);
       }
-      if (a.ranks) above += L::above(w[j], given);
     }
     if (a.top && (b == check || b + 1 == batches)) {
       // ---- the best so far: of those of before, which are the first keys, and of the candidates
       __syncthreads();
-      const int hits = s_hits;
-      if (hits <= HITS) {                                   // (the same for all)
+      const int hits = s_hits[turn];
+      if (hits > HITS) lost = true;                         // (the same for all)
+      if (hits && !lost) {
         for (int i = tid; i < hits * E; i += THREADS) {
           const float y = value(reinterpret_cast<const T*>(s_hit)[i]);
           const int at = s_where[i / E] + i % E;
@@ -242,19 +296,19 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
             if (larger < a.top) s_best[larger] = key;
           }
           __syncthreads();
+          // (the next to look at these come behind a barrier; hits are counted elsewhere from here on)
           best = min(count, a.top);
           if (tid < best) s_key[tid] = s_best[tid];
-          if (tid == 0) { s_count = best; s_hits = 0; }
+          if (tid == 0) { s_count = best; s_hits[turn] = 0; }
+          turn ^= 1;
           if (best == a.top) reach = value_of(s_best[best - 1]);
         } else {
-          reach = INFINITY;                                 // too many: all of them are looked for at the end
+          lost = true;
         }
-      } else {
-        reach = INFINITY;
       }
-      check = 4 * b + 3;
+      if (lost) reach = INFINITY;                           // all of them are looked for at the end
+      check = (a.top > 8 ? 4 : 8) * (b + 1) - 1;
       set_limit();
-      __syncthreads();
     }
   }
   // ---- the threads' sums together
@@ -280,18 +334,10 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
   }
   above = __reduce_add_sync(0xffffffffu, above);
   if (lane == 0) { s_sum[0][warp] = S; s_sum[1][warp] = U; s_above[warp] = above; }
-  if (a.top && (odd || s_hits > HITS || s_count > CANDIDATES)) {             // (the same for all: the barrier above)
-    u64 before = ~0ull;                                     // (no key is that large)
-    for (best = 0; best < a.top; ++best) {
-      u64 most = 0;
-      for (int v = tid; v < vectors; v += THREADS) {
-        const int first = v * E - shift;
-#pragma unroll 1
-        for (int i = max(first, 0); i < min(first + E, n); ++i) {
-          const u64 key = key_of(value(from[i]), lo + i);
-          if (key < before && key > most) most = key;
-        }
-      }
+  if (a.top && (odd || lost)) {             // (the same for all: the barrier above)
+    u64 mine = best_below<T>(from, n, shift, lo, ~0ull);
+    for (best = 0; best < a.top; ++best) {                  // whoever had the best looks for his next
+      u64 most = mine;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const u64 other = __shfl_xor_sync(0xffffffffu, most, o);
@@ -304,8 +350,10 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
       for (int i = 1; i < WARPS; ++i) most = s_most[i] > most ? s_most[i] : most;
       __syncthreads();
       if (!most) break;
-      if (tid == 0) s_best[best] = most;
-      before = most;
+      if (mine == most) {
+        s_best[best] = most;
+        mine = best_below<T>(from, n, shift, lo, most);
+      }
     }
   }
   __syncthreads();
