@@ -4,18 +4,26 @@
 // One CTA = one or two tiles of 128 rows of one request and key/value head; a row is a (token, query head of the group) pair. Keys are walked in blocks of 128 by two
 // streams with a softmax and a sum of values of their own, so that one's products run under the other's softmax. Two tiles have a stream each, and every
 // block's codes are made ready once for both; a single tile's streams take the blocks in turn and are joined at the end.
-//   * pages: one warp looks the block's pages and words up and leaves where the codes are, the words, and the largest exponent of the keys' scales and of the values'.
+//   * pages: one warp looks the block's pages and words up (8 a lane) and leaves where the codes are, the words, and the largest exponent of the keys' scales and of the values'.
 //   * codes: four warps bring a block's keys and values from global memory, make them float16 and store them as the tensor cores want them: the cache is read once, in 4
 //     bits, and is never anywhere in 16. A code in the upper bits of the mantissa behind an exponent of 4 is 16 + c; (16 + c) s - (16 + z) s is one multiply-add of two
 //     values, and exact: s has five bits, 16 + z has five, (c - z) s nine. s is the row's scale over the block's largest power of two, times 2^10: exact
 //     down to 2^-30 of the largest. Eight codes of a word come out as 0 4 1 5 2 6 3 7: the order of the sum over a head's columns is free (queries are put in the same), and
 //     columns of the result are put right on their way out.
 //   * S = Q K^T, accumulator [128 x 128] float32 in tensor memory, one for each stream.
-//   * softmax: thread = row, four warps a stream. Scores are read twice, for the maximum and for the weights (that keeps 128 of them out of the registers).
+//   * products: a thread a stream issues them: scores once the keys are there and the stream's product before them is over (its weights lie where the scores go), the product of
+//     values once half of the weights are there, then of the other half. (One thread for both was at work the whole time: six steps of some 900 cycles a pair of blocks,
+//     for a look at a barrier takes 100 among warps that multiply and store.)
+//   * softmax: thread = row, four warps a stream. The first half of a row's scores stays in registers between the maximum and the weights; the second half is read twice.
 //     The block's power of two of the keys multiplies the scores, that of the values goes into the exponent; weights go back over the scores as float16 (off by 2^-11 of
 //     themselves or by 2^-34 of the largest, as in kv4_attention.cu; the result is rounded to 16 bits as well).
 //   * O += P V: weights from tensor memory, values from shared memory as they lie in the cache (operand "MN-major").
 // Tensor memory: S | S | O | O = 512 columns. O is multiplied again only where a row's maximum grew by more than 2^6.
+// What bounds it: 2000 tokens after 1000, 32 / 8 heads of 128, 116.8 us, 561 TFLOP/s of products (34 % of a large library product's rate). A pair of blocks takes some 5500
+// cycles; its products are 2050 (64 each), the exponentials 2050 of a scheduler's special function unit, and both streams wait for one another's: the scores of a block take
+// 800 to 1200 cycles, the softmax 2300 alone and 3400 beside the other's, the sum of values 800. Measured and not taken (us): two accumulators of 64 keys each for a stream, scores a turn
+// ahead (151: a product of 64 columns takes as long as one of 128); one thread for both streams' products (119); the streams' exponentials in turn (120), or the second stream
+// half a turn late (122: they fall into step again); 32 scores at a time, read again for the weights (118); the steps of the codes rolled into one piece of code (160).
 //
 // Every wait is bounded; a CTA whose wait runs out waits (again with a limit) for its products under way, fills its rows with NaN, counts itself
 // (qspec_attn_tile_timeouts) and frees its tensor memory.
@@ -29,7 +37,7 @@ using namespace atile;
 using namespace kv8;
 
 constexpr int SOFTMAX = 8, CONVERT = 4;                   // warps
-constexpr int W_CONVERT = SOFTMAX, W_MMA = W_CONVERT + CONVERT, W_PAGES = W_MMA + 1, NWARPS = W_PAGES + 1, NTHREADS = NWARPS * 32;
+constexpr int W_MMA = 0, W_PAGES = 2, W_CONVERT = 3, W_SOFTMAX = W_CONVERT + CONVERT, NWARPS = W_SOFTMAX + SOFTMAX, NTHREADS = NWARPS * 32;
 constexpr int FACS = 4;                                   // blocks whose pages and factors are kept
 constexpr float NONE = -INFINITY;
 
@@ -71,7 +79,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
   using Z = Sizes<D>;
   constexpr int OP = Z::OP, PARTB = Z::PART, STAGES = Z::STAGES, COLS = D / 2;
   extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ __align__(8) uint64_t b_kfull[STAGES], b_kempty[STAGES], b_vfull[STAGES], b_vempty[STAGES], b_fac[FACS], b_facfree[FACS], b_q, b_s[2], b_p[2][2], b_o[2], b_join;
+  __shared__ __align__(8) uint64_t b_kfull[STAGES], b_kempty[STAGES], b_vfull[STAGES], b_vempty[STAGES], b_fac[FACS], b_facfree[FACS], b_q, b_s[2], b_p[2][2], b_o[2], b_end[2], b_join;
   __shared__ Block s_block[FACS];
   __shared__ float s_ml[2][2][128], s_rowf[256];
   __shared__ unsigned long long s_work[NWARPS];
@@ -85,11 +93,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
     s_fail = 0;
     s_at[0] = -1;
     for (int i = 0; i < STAGES; ++i) {
-      bar_init(smem_addr(&b_kfull[i]), CONVERT); bar_init(smem_addr(&b_kempty[i]), 1);
-      bar_init(smem_addr(&b_vfull[i]), CONVERT); bar_init(smem_addr(&b_vempty[i]), 1);
+      bar_init(smem_addr(&b_kfull[i]), CONVERT);
+      bar_init(smem_addr(&b_vfull[i]), CONVERT);
     }
     for (int i = 0; i < FACS; ++i) bar_init(smem_addr(&b_fac[i]), 1);
-    for (int i = 0; i < 2; ++i) { bar_init(smem_addr(&b_s[i]), 1); bar_init(smem_addr(&b_p[i][0]), 4); bar_init(smem_addr(&b_p[i][1]), 4); bar_init(smem_addr(&b_o[i]), 1); }
+    for (int i = 0; i < 2; ++i) { bar_init(smem_addr(&b_s[i]), 1); bar_init(smem_addr(&b_p[i][0]), 4); bar_init(smem_addr(&b_p[i][1]), 4); bar_init(smem_addr(&b_o[i]), 1); bar_init(smem_addr(&b_end[i]), 1); }
     bar_init(smem_addr(&b_q), SOFTMAX);
     bar_init(smem_addr(&b_join), SOFTMAX);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -180,8 +188,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
   auto blocks_of = [&](int tokens) { const int seen = min(pos0 + tokens, reach); return seen > 0 ? (seen + 127) / 128 : 0; };
   const int blocks = blocks_of(n2);                       // keys that any row sees
   const int turns0 = both ? blocks_of(tok) : (blocks + 1) >> 1, turns1 = both ? blocks : blocks >> 1;   // blocks of the streams
-  if (tid == 0)
+  if (tid == 0) {
     for (int i = 0; i < FACS; ++i) bar_init(smem_addr(&b_facfree[i]), (both ? SOFTMAX : SOFTMAX / 2) + CONVERT);
+    for (int i = 0; i < STAGES; ++i) { bar_init(smem_addr(&b_kempty[i]), both ? 2 : 1); bar_init(smem_addr(&b_vempty[i]), both ? 2 : 1); }   // (each stream's products)
+  }
   if (warp == W_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&s_tmem)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -194,137 +204,123 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
   const uint32_t kbuf = base + 2 * OP, vbuf = kbuf + STAGES * OP;
 
   if (warp == W_PAGES) {
-    // ---- pages and words of the blocks, ahead of all others: lane i has 16 of a block's keys (i < 8: words of keys, i < 16: of values), the next block's pages on their way
+    // ---- pages and words of the blocks, ahead of all others: lane i has 8 of a block's keys (i < 16: words of keys, else of values), the next block's pages on their way
     bool ok = !(a.give_up & 8u);
     if (!ok) s_fail = 1;
-    const int part = lane & 7;
+    const int part = (lane & 15) * 8, side = lane >> 4;
     auto page_of = [&](int n) {                             // -1: none
-      const int key = n * 128 + part * 16, at = key >> a.pshift;
-      if (lane >= 16 || n >= blocks || key >= keys) return -1;
+      const int key = n * 128 + part, at = key >> a.pshift;
+      if (n >= blocks || key >= keys) return -1;
       const int page = at < a.width ? a.table[(size_t)req * a.width + at] : -1;
       return (unsigned)page < (unsigned)a.npages ? page : -1;
     };
     int page = page_of(0);
+#pragma unroll 1
     for (int n = 0; ok && n < blocks; ++n) {
-      const int slot = n % FACS, key = n * 128 + part * 16;
+      const int slot = n % FACS, key = n * 128 + part;
       const bool there = page >= 0;
       const long long row = there ? (long long)((((size_t)page * a.G + g) << a.pshift) + (key & ((1 << a.pshift) - 1))) : -1ll;
-      uint4 w[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-      if (there) {
-        const uint4* from = reinterpret_cast<const uint4*>((lane < 8 ? a.kw : a.vw) + row);
-        w[0] = __ldg(from);
-        w[1] = __ldg(from + 1);
-      }
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (there) w = __ldg(reinterpret_cast<const uint4*>((side ? a.vw : a.kw) + row));
       page = page_of(n + 1);
       if (n >= FACS) ok = bar_wait(smem_addr(&b_facfree[slot]), (uint32_t)((n / FACS) - 1) & 1u, &s_fail);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       // scales that are infinite or no number: exponent 255. (Rows behind the last key have neither say nor sight.)
-      const uint32_t x[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
-      const int have = min(max(keys - key, 0), 16);
+      uint32_t x[4] = {w.x, w.y, w.z, w.w};
+      const int have = min(max(keys - key, 0), 8);
       uint32_t bad = 0u, most = 0u;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
+      for (int e = 0; e < 8; ++e) {
         const uint32_t ex = (x[e >> 1] >> (e & 1 ? 24 : 8)) & 0xffu;
         if (e < have) {
           if (ex == 255u) bad |= 1u << e;
           else most = max(most, ex);
         }
       }
-      if (!there && have > 0) bad = (1u << have) - 1u;      // (a page that there is not)
-      bad |= __shfl_xor_sync(0xffffffffu, bad, 8);          // of the key's word, or of the value's
+      if (!there) bad = (1u << have) - 1u;                  // (a page that there is not)
+      bad |= __shfl_xor_sync(0xffffffffu, bad, 16);         // of the key's word, or of the value's
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-      if (lane < 16) {
-        Block& f = s_block[slot];
-        uint32_t* to = reinterpret_cast<uint32_t*>(lane < 8 ? f.kw : f.vw) + part * 8;
-        const uint32_t no = lane < 8 ? NO_KEY : NO_VALUE;
+      for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      const uint32_t no = side ? NO_VALUE : NO_KEY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          uint32_t y = x[e];
-          if (bad >> (2 * e) & 1u) y = (y & 0xffff0000u) | no;
-          if (bad >> (2 * e + 1) & 1u) y = (y & 0xffffu) | no << 16;
-          if (2 * e >= have) y = 0u;                        // (values that are no numbers would make a weight of zero one)
-          else if (2 * e + 1 >= have) y &= 0xffffu;
-          to[e] = y;
-        }
-        if (lane < 8) f.at[part] = row;
-        if (part == 0) (lane ? f.ve : f.ke) = max((int)most, 27);   // (2^-100)
+      for (int e = 0; e < 4; ++e) {
+        if (bad >> (2 * e) & 1u) x[e] = (x[e] & 0xffff0000u) | no;
+        if (bad >> (2 * e + 1) & 1u) x[e] = (x[e] & 0xffffu) | no << 16;
+        if (2 * e >= have) x[e] = 0u;                       // (values that are no numbers would make a weight of zero one)
+        else if (2 * e + 1 >= have) x[e] &= 0xffffu;
       }
+      Block& f = s_block[slot];
+      *reinterpret_cast<uint4*>((side ? f.vw : f.kw) + part) = make_uint4(x[0], x[1], x[2], x[3]);
+      if (!side && !(lane & 1)) f.at[lane >> 1] = row;
+      if ((lane & 15) == 0) (side ? f.ve : f.ke) = max((int)most, 27);   // (2^-100)
       __syncwarp();
       if (lane == 0) bar_arrive(smem_addr(&b_fac[slot]));
     }
-  } else if (warp == W_MMA) {
+  } else if (warp < W_PAGES) {
     if (elect()) {
+      const int z = warp - W_MMA, turns = z ? turns1 : turns0;
       bool ok = !(a.give_up & 4u);
       if (!ok) s_fail = 1;
-      int done0 = 0, done1 = 0;                           // value products that have been issued
-      // Step k: stream k % 2's turn k / 2. Pairs of tiles take every block in turn, a single tile's streams every other one.
-      const int steps = both ? 2 * blocks : blocks;
-      auto scores = [&](int k) -> bool {
-        const int z = k & 1, i = k >> 1, n = both ? i : k;
-        if (i >= (z ? turns1 : turns0)) return true;
-        if (!bar_wait(smem_addr(&b_kfull[n % STAGES]), (uint32_t)(n / STAGES) & 1u, &s_fail)) return false;
-        // these scores take the columns of the weights of the turn before: its product must be over
-        if (i && !bar_wait(smem_addr(&b_o[z]), (uint32_t)(i - 1) & 1u, &s_fail)) return false;
+      if (turns) ok = ok && bar_wait(smem_addr(&b_q), 0, &s_fail);
+      const uint64_t qd = desc_k(base + (both ? z * OP : 0));
+      const uint32_t s = tmem + z * 128, o = tmem + 256 + z * D;
+#pragma unroll 1
+      for (int j = 0; ok && j < turns; ++j) {
+        const int n = both ? j : 2 * j + z, stage = n % STAGES;
+        const uint32_t round = (uint32_t)(n / STAGES) & 1u, turn = (uint32_t)j & 1u;
+        const bool last = both && z && n >= turns0;         // tile 0 does not see this block: tile 1 says for both that it is done with it
+        ok = bar_wait(smem_addr(&b_kfull[stage]), round, &s_fail) && (!j || bar_wait(smem_addr(&b_o[z]), turn ^ 1u, &s_fail));   // (these scores take the columns of the weights before)
+        if (!ok) break;
         fence_after();
-        const uint64_t qd = desc_k(base + (both ? z * OP : 0)), kd = desc_k(kbuf + (n % STAGES) * OP);
+        const uint64_t kd = desc_k(kbuf + stage * OP);
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
           const uint32_t step = (uint32_t)((d >> 2) * (PARTB >> 4) + (d & 3) * 2);
-          mma_ss(tmem + z * 128, qd + step, kd + step, IDESC_S<D>, d ? 1u : 0u);
+          mma_ss(s, qd + step, kd + step, IDESC_S<D>, d ? 1u : 0u);
         }
         commit(smem_addr(&b_s[z]));
-        if (!both || z) commit(smem_addr(&b_kempty[n % STAGES]));   // (tile 1 sees every block that tile 0 sees)
-        return true;
-      };
-      ok = ok && (steps == 0 || (bar_wait(smem_addr(&b_q), 0, &s_fail) && scores(0) && (steps == 1 || scores(1))));
-      for (int k = 0; ok && k < steps; ++k) {
-        const int z = k & 1, i = k >> 1, n = both ? i : k;
-        if (i >= (z ? turns1 : turns0)) continue;
-        ok = bar_wait(smem_addr(&b_vfull[n % STAGES]), (uint32_t)(n / STAGES) & 1u, &s_fail);
-        const uint64_t vd = desc_mn(vbuf + (n % STAGES) * OP);
-        const uint32_t p = tmem + z * 128, o = tmem + 256 + z * D;
+        commit(smem_addr(&b_kempty[stage]));
+        if (last) commit(smem_addr(&b_kempty[stage]));
+        ok = bar_wait(smem_addr(&b_vfull[stage]), round, &s_fail);
+        if (!ok) break;
+        const uint64_t vd = desc_mn(vbuf + stage * OP);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {                     // 64 keys each
-          ok = ok && bar_wait(smem_addr(&b_p[z][h]), (uint32_t)i & 1u, &s_fail);
+        for (int h = 0; h < 2; ++h) {                       // 64 keys each
+          ok = ok && bar_wait(smem_addr(&b_p[z][h]), turn, &s_fail);
           if (!ok) break;
           fence_after();
 #pragma unroll
-          for (int d = 0; d < 4; ++d) mma_ts(o, p + h * 32 + d * 8, vd + (h * 4 + d) * (2048 >> 4), IDESC_O<D>, (i || h || d) ? 1u : 0u);
+          for (int d = 0; d < 4; ++d) mma_ts(o, s + h * 32 + d * 8, vd + (h * 4 + d) * (2048 >> 4), IDESC_O<D>, (j || h || d) ? 1u : 0u);
         }
         if (!ok) break;
         commit(smem_addr(&b_o[z]));
-        if (!both || z) commit(smem_addr(&b_vempty[n % STAGES]));
-        (z ? done1 : done0) = i + 1;
-        ok = k + 2 >= steps || scores(k + 2);
+        commit(smem_addr(&b_vempty[stage]));
+        if (last) commit(smem_addr(&b_vempty[stage]));
       }
-      // every product of either stream is over before the CTA leaves, those of a turn that was given up, too
-      if (done0) bar_drain(smem_addr(&b_o[0]), (uint32_t)(done0 - 1) & 1u);
-      if (done1) bar_drain(smem_addr(&b_o[1]), (uint32_t)(done1 - 1) & 1u);
-      if (!ok) {
-        commit(smem_addr(&b_o[0]));
-        bar_drain(smem_addr(&b_o[0]), (uint32_t)done0 & 1u);
-      }
+      // every product is over before the CTA leaves, those of a turn that was given up, too
+      commit(smem_addr(&b_end[z]));
+      bar_drain(smem_addr(&b_end[z]), 0);
     }
     __syncwarp();
-  } else if (warp >= W_CONVERT) {
+  } else if (warp < W_SOFTMAX) {
     // ---- codes: 16 bytes (32 of them) a lane
     constexpr int ROWS = CONVERT * 32 / (D / 32), STEPS = 128 / ROWS;   // rows at a time, times
     const int ct = tid - W_CONVERT * 32;
     // (eight lanes take two pieces of four rows, so that their stores meet in no bank)
     const int c = D == 128 ? (ct >> 3 & 1) * 2 + (ct & 1) : ct & 1, row0 = D == 128 ? (ct >> 4) * 4 + (ct >> 1 & 3) : ct >> 1;
     const uint32_t part = (uint32_t)(c >> 1) * PARTB;
-    uint4 kw[STEPS], vw[STEPS];
-    auto load = [&](uint4 (&w)[STEPS], const uint8_t* codes, int n) {
-      const Block& f = s_block[n % FACS];
-      const int have = keys - n * 128;
+    uint4 here[STEPS], next[STEPS];
+    auto load = [&](int t) {                                // side t % 2 (keys, values) of block t / 2
+      const Block& f = s_block[(t >> 1) % FACS];
+      const uint8_t* codes = (t & 1 ? a.v : a.k) + c * 16;
+      const int have = keys - (t >> 1) * 128;
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         const int row = i * ROWS + row0;
         const long long at = f.at[row >> 4];
-        w[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (row < have && at >= 0) w[i] = __ldg(reinterpret_cast<const uint4*>(codes + (at + (row & 15)) * (D / 2) + c * 16));
+        next[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < have && at >= 0) next[i] = __ldg(reinterpret_cast<const uint4*>(codes + (at + (row & 15)) * (D / 2)));
       }
     };
     auto store = [&](const uint4 (&w)[STEPS], uint32_t dst, const uint16_t* words, int ex) {
@@ -356,35 +352,34 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
       ok = __all_sync(0xffffffffu, ok);
     };
     if (blocks && ok) look(0);
-    if (blocks && ok) load(kw, a.k, 0);
-    for (int n = 0; ok && n < blocks; ++n) {
-      load(vw, a.v, n);
-      if (n >= STAGES) ok = bar_wait(smem_addr(&b_kempty[n % STAGES]), (uint32_t)(n / STAGES - 1) & 1u, &s_fail);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      store(kw, kbuf + (n % STAGES) * OP, s_block[n % FACS].kw, s_block[n % FACS].ke);
-      if (lane == 0) bar_arrive(smem_addr(&b_kfull[n % STAGES]));
-      if (n + 1 < blocks) {
-        look(n + 1);
+    if (blocks && ok) load(0);
+#pragma unroll 1
+    for (int t = 0; ok && t < 2 * blocks; ++t) {            // (one piece of code for keys and values)
+      const int n = t >> 1, stage = n % STAGES, side = t & 1;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) here[i] = next[i];
+      if (t + 1 < 2 * blocks) {
+        if (side) look(n + 1);
         if (!ok) break;
-        load(kw, a.k, n + 1);
+        load(t + 1);
       }
-      if (n >= STAGES) ok = bar_wait(smem_addr(&b_vempty[n % STAGES]), (uint32_t)(n / STAGES - 1) & 1u, &s_fail);
+      if (n >= STAGES) ok = bar_wait(smem_addr(side ? &b_vempty[stage] : &b_kempty[stage]), (uint32_t)(n / STAGES - 1) & 1u, &s_fail);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      store(vw, vbuf + (n % STAGES) * OP, s_block[n % FACS].vw, s_block[n % FACS].ve);
+      const Block& f = s_block[n % FACS];
+      store(here, (side ? vbuf : kbuf) + stage * OP, side ? f.vw : f.kw, side ? f.ve : f.ke);
       if (lane == 0) {
-        bar_arrive(smem_addr(&b_vfull[n % STAGES]));
-        bar_arrive(smem_addr(&b_facfree[n % FACS]));
+        bar_arrive(smem_addr(side ? &b_vfull[stage] : &b_kfull[stage]));
+        if (side) bar_arrive(smem_addr(&b_facfree[n % FACS]));
       }
     }
   } else {
     // ---- queries: as they are, 16 bytes a thread at a time; then a thread a row: bfloat16 rows times a power of two each, and the sums. (Loops that are
     // not unrolled: every CTA comes here once, and had to wait for the instructions.)
     constexpr int IN_ROW = D / 8;
-    const int tiles = both ? 2 : 1;
+    const int tiles = both ? 2 : 1, wi = warp - W_SOFTMAX, ti = tid - W_SOFTMAX * 32;
 #pragma unroll 4
-    for (int i = tid; i < tiles * 128 * IN_ROW; i += SOFTMAX * 32) {
+    for (int i = ti; i < tiles * 128 * IN_ROW; i += SOFTMAX * 32) {
       const int c = i % IN_ROW, row = i / IN_ROW, r = row & 127, tl = (row >> 7) * tok + token_of(r);
       const uint32_t to = base + (row >> 7) * OP + (c >> 3) * PARTB + r * 128 + (((c & 7) ^ (r & 7)) << 4);
       if (tl < n2 && r < tok * rep)
@@ -400,9 +395,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
     };
     asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;\n" ::: "memory");
     asm volatile("bar.sync 1, %0;\n" ::"n"(SOFTMAX * 32) : "memory");   // (behind nothing that may be given up)
-    if (tid < tiles * 128) {
-      const int r = tid & 127;
-      unsigned char* const row = gbase + (tid >> 7) * OP + r * 128;
+    if (ti < tiles * 128) {
+      const int r = ti & 127;
+      unsigned char* const row = gbase + (ti >> 7) * OP + r * 128;
       auto piece = [&](int c) { return reinterpret_cast<uint4*>(row + (c >> 3) * PARTB + (((c & 7) ^ (r & 7)) << 4)); };
       int sh = 0;
       if (BF16) {
@@ -429,12 +424,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
         // in the order in which codes come out of a word: 0 4 1 5 2 6 3 7
         *piece(c) = make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632), __byte_perm(x[1], x[3], 0x5410), __byte_perm(x[1], x[3], 0x7632));
       }
-      s_rowf[tid] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2;
+      s_rowf[ti] = __uint_as_float((uint32_t)(127 - sh) << 23) * a.scale2;
     }
     ready();
     asm volatile("bar.sync 1, %0;\n" ::"n"(SOFTMAX * 32) : "memory");   // (the factors of the rows)
     // ---- softmax: thread = row r of stream z
-    const int z = warp >> 2, r = (warp & 3) * 32 + lane, turns = z ? turns1 : turns0, zrow = both ? z * 128 : 0, ztok = both ? z * tok : 0;
+    const int z = wi >> 2, r = (warp & 3) * 32 + lane, turns = z ? turns1 : turns0, zrow = both ? z * 128 : 0, ztok = both ? z * tok : 0;
     const int tl = ztok + token_of(r);
     const bool row_in = r < tok * rep && tl < n2;
     const int limit = row_in ? min(pos0 + tl, keys - 1) : -1;   // last visible position
@@ -445,105 +440,113 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
     const float rowf = s_rowf[zrow + r];
     float m = NONE, l = 0.f;
     for (int i = 0; ok && i < turns; ++i) {
-      const int n = both ? i : 2 * i + z;
+      const int n = both ? i : 2 * i + z, j0 = n * 128;
       const uint32_t turn = (uint32_t)i & 1u;
-      const int j0 = n * 128;
       const bool plain = __all_sync(0xffffffffu, !row_in || j0 + 127 <= limit);   // (rows that stand for no token are never stored)
       ok = bar_wait(smem_addr(&b_fac[n % FACS]), (uint32_t)(n / FACS) & 1u, &s_fail) && bar_wait(smem_addr(&b_s[z]), turn, &s_fail);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
+      uint32_t x[64];
+      auto hide = [&](uint32_t* y, int count, int c0) {     // what a row does not see
+#pragma unroll
+        for (int j = 0; j < count; ++j)
+          if (j0 + c0 + j > limit) y[j] = 0xff800000u;
+      };
+      auto largest = [&](const uint32_t* y, float mx) {
+        float t = __uint_as_float(y[0]);
+#pragma unroll
+        for (int j = 1; j < 31; j += 4) {                   // (three operands: one instruction)
+          mx = fmaxf(fmaxf(mx, __uint_as_float(y[j])), __uint_as_float(y[j + 1]));
+          if (j + 3 < 32) t = fmaxf(fmaxf(t, __uint_as_float(y[j + 2])), __uint_as_float(y[j + 3]));
+        }
+        return fmaxf(fmaxf(mx, t), __uint_as_float(y[31]));
+      };
       const Block& f = s_block[n % FACS];
+      // ---- the largest exponent: of the second half, whose scores are read again, and the first, whose scores stay
+      float mn = NONE;
+#pragma unroll 1
+      for (int c0 = 64; c0 < 128; c0 += 32) {
+        ld32(st + c0, x);
+        wait_ld();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) landed8(x + 8 * j);
+        if (!plain) hide(x, 32, c0);
+        mn = largest(x, mn);
+      }
+      auto load = [&](int c0) {
+        ld32(st + c0, x);
+        ld32(st + c0 + 32, x + 32);
+        wait_ld();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) landed8(x + 8 * j);
+        if (!plain) hide(x, 64, c0);
+      };
+      load(0);
+      mn = largest(x, mn);
+      mn = largest(x + 32, mn);
       // The block's powers of two: what scores are multiplied with (not so small that it would make a hidden key's minus infinity no number), what exponents begin with
       const float k = fmaxf(rowf * __uint_as_float((uint32_t)min(max(f.ke - TOP, 1), 254) << 23), 1.17549435e-38f), lv = (float)(f.ve - 127 - TOP);
       const float iv = __uint_as_float((uint32_t)min(max(127 + 127 + TOP - f.ve, 1), 254) << 23) * WEIGHT_UNIT;
-      // Loops over 32 columns (the weights' over 64), not over all: three kinds of warps run at once, and with the block's 128 columns laid out in a row they wait for
-      // their instructions more than for anything else. What a row does not see:
-      auto hide = [&](uint32_t (&x)[32], int c0) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (j0 + c0 + j > limit) x[j] = 0xff800000u;
-      };
-      // ---- the largest exponent
-      float mn = NONE;
+      mn = fmaf(mn, k, lv);                                 // (minus infinity stays that)
+      const bool grown = mn > m + GROWTH_LOG2;              // (of a row that had seen nothing: more than minus infinity)
+      if (__any_sync(0xffffffffu, grown)) {
+        const float up = grown ? ex2(m - mn) : 1.f;         // 0 for a row that had seen nothing; other rows of the warp keep theirs
+        l *= up;
+        if (i && __any_sync(0xffffffffu, grown && m != NONE)) {   // (the scores are there: the stream's product before them is over)
 #pragma unroll 1
-      for (int c0 = 0; c0 < 128; c0 += 32) {
-        uint32_t x[32];
-        ld32(st + c0, x);
-        wait_ld();
-        landed32(x);
-        if (!plain) hide(x, c0);
-        float t[2] = {__uint_as_float(x[0]), __uint_as_float(x[1])};
+          for (int q = 0; q < D / 16; ++q) {
+            uint32_t o[16];
+            ld16(ot + q * 16, o);
+            wait_ld();
+            landed8(o);
+            landed8(o + 8);
 #pragma unroll
-        for (int j = 2; j < 32; j += 4) {                 // (three operands: one instruction)
-          t[0] = fmaxf(fmaxf(t[0], __uint_as_float(x[j])), __uint_as_float(x[j + 1]));
-          if (j + 2 < 32) t[1] = fmaxf(fmaxf(t[1], __uint_as_float(x[j + 2])), __uint_as_float(x[j + 3]));
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * up);
+            st16(ot + q * 16, o);
+          }
         }
-        mn = fmaxf(mn, fmaxf(t[0], t[1]));
+        if (grown) m = mn;
       }
-      mn = fmaf(mn, k, lv);                               // (minus infinity stays that)
-      const bool grown = mn > m + GROWTH_LOG2 || (m == NONE && mn > m);
-      const float up = grown ? ex2(m - mn) : 1.f;         // 0 for a row that had seen nothing; other rows of the warp keep theirs
-      l *= up;
-      if (i && __any_sync(0xffffffffu, grown && m != NONE)) {   // (the scores are there: the stream's product before them is over)
-#pragma unroll 1
-        for (int q = 0; q < D / 32; ++q) {
-          uint32_t o[32];
-          ld32(ot + q * 32, o);
-          wait_ld();
-          landed32(o);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * up);
-          st16(ot + q * 32, o);
-          st16(ot + q * 32 + 16, o + 16);
-        }
-      }
-      if (grown) m = mn;
       const float mu = m == NONE ? 0.f : m;
       // Exponents are taken from the products without a rounding in between, the reference and what it is joined with have one: far from zero that alone would be a
       // large exponent.
       const bool far = __any_sync(0xffffffffu, fabsf(mu) > FAR);
-      const float ref = (far ? 0.f : mu) - WEIGHT_LOG2;
-      // ---- weights
+      const float k1 = far ? 1.f : k, at1 = far ? WEIGHT_LOG2 : lv - (mu - WEIGHT_LOG2);
+      const uint64_t k2 = pair(__float_as_uint(k1), __float_as_uint(k1)), at2 = pair(__float_as_uint(at1), __float_as_uint(at1));
       uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll 2
-      for (int c0 = 0; c0 < 128; c0 += 32) {
-        uint32_t x[32], p[16];
-        ld32(st + c0, x);
-        float f1 = k, f0 = lv;
-        wait_ld();
-        landed32(x);
+      // ---- weights, 64 at a time
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        if (h) load(64);
         if (far) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]), k, lv) - mu);
-          f1 = 1.f;
-          f0 = 0.f;
+          for (int j = 0; j < 64; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]), k, lv) - mu);
+          if (!plain) hide(x, 64, h * 64);                  // (scores that a row does not see may have been infinite)
         }
-        if (!plain) hide(x, c0);                          // (behind that: scores that a row does not see may be infinite)
-        const uint64_t k2 = pair(__float_as_uint(f1), __float_as_uint(f1)), at2 = pair(__float_as_uint(f0 - ref), __float_as_uint(f0 - ref));
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          uint32_t p0, p1;
-          unpair(fma2(pair(x[2 * j], x[2 * j + 1]), k2, at2), p0, p1);
-          p0 = __float_as_uint(ex2(__uint_as_float(p0)));
-          p1 = __float_as_uint(ex2(__uint_as_float(p1)));
-          sum[j & 1] = add2(sum[j & 1], pair(p0, p1));
-          p[j] = half_pair(__uint_as_float(p0), __uint_as_float(p1));
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            uint32_t p0, p1;
+            unpair(fma2(pair(x[c * 32 + 2 * j], x[c * 32 + 2 * j + 1]), k2, at2), p0, p1);
+            p0 = __float_as_uint(ex2(__uint_as_float(p0)));
+            p1 = __float_as_uint(ex2(__uint_as_float(p1)));
+            sum[j & 1] = add2(sum[j & 1], pair(p0, p1));
+            p[j] = half_pair(__uint_as_float(p0), __uint_as_float(p1));
+          }
+          st16(st + h * 32 + c * 16, p);                    // (over scores that have been read)
         }
-        st16(st + c0 / 2, p);                             // (over scores that have been read)
-        if (c0 & 32) {                                    // 64 keys' weights are there
-          wait_st();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(smem_addr(&b_p[z][c0 >> 6]));
-        }
-      }
-      {
-        uint32_t a0, a1;
-        unpair(add2(sum[0], sum[1]), a0, a1);
-        l = fmaf(__uint_as_float(a0) + __uint_as_float(a1), iv, l);
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(smem_addr(&b_p[z][h]));
       }
       if (lane == 0) bar_arrive(smem_addr(&b_facfree[n % FACS]));
+      uint32_t a0, a1;
+      unpair(add2(sum[0], sum[1]), a0, a1);
+      l = fmaf(__uint_as_float(a0) + __uint_as_float(a1), iv, l);
     }
     if (both && z == 0)                                   // (blocks that tile 1 alone sees)
       for (int n = turns; ok && n < blocks; ++n) {
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
     // ---- out, through shared memory, 16 bytes a lane. A single tile's streams together: maxima and sums through shared memory; stream z takes half z of the
     // columns, of both sums. Of a pair either takes both halves of its own.
     constexpr int LD = COLS * 2 + 16, LANES = COLS / 8;   // bytes of half a row (and 16: no bank conflicts), lanes that take it
-    unsigned char* const rows = gbase + warp * 32 * LD;   // (queries and keys are done with)
+    unsigned char* const rows = gbase + wi * 32 * LD;   // (queries and keys are done with)
     s_ml[z][0][r] = m;
     s_ml[z][1][r] = l;
     __syncwarp();
