@@ -18,6 +18,10 @@
 // largest may lose bits). A key's scale multiplies its scores in float32. A value's scale v goes into the exponent: the weights 2^(9 + s + log2 v - m) lie below 2^15
 // whatever the scales are and are rounded to float16 for the product with the codes (by 2^-11 of themselves at most, or by 2^-34 of the largest: kv8_common.cuh); the denominator
 // is the sum of the unrounded weights / v.
+//
+// Measured: 64 requests of 4 tokens after some 3000 keys each, 32 / 8 heads of 128, 89 us, 2.3 TB/s of codes and words; one token after 131071 keys, 64 / 8 heads, 56 us, 2.4 TB/s; 4 requests of a
+// token after some 500 keys 15 us, which is launches and a chain of loads. At this many rows not the bytes bound it (a third of the time) but instructions: a unit of 32 keys takes a warp
+// some 900, of which 64 are products and a third make codes operands; an SM issues two a cycle, the tensor cores are busy 28 % of the time.
 #include "kv4_common.cuh"
 #include "kv_stretch.cuh"
 
@@ -466,13 +470,18 @@ static int attention(const void* q, long long q_tok_stride, int q_head_stride, c
   const int grid = att_grid();
   QSPEC_REQUIRE(grid <= GRID_MOST, QSPEC_ERR_UNSUPPORTED, "kv4_attention: %d SMs", sm_count());
   // Requests with many rows may go to the prompt form (to_prompt_form()), in a launch of its own in front; none do if the call's rows are too few for a third of
-  // the SMs (always: for tests).
+  // the SMs (always: for tests). Both forms measured, 32 / 8 heads of 128, us of the prompt form (of the other):
+  //   1 request, 1000 keys in front of it   32 tokens 37 (19)   128: 37 (23)   160: 38 (39)   256: 38 (51)   1024: 71 (204)
+  //   1 request, 32000 keys                 128 tokens 493 (345)   256: 499 (610)   512: 588 (1195)
+  //   4 requests, 8000 keys                 17 tokens 139 (73)   48: 143 (145)   64: 151 (180)   128: 168 (333)
+  //   16 requests, 1000 keys                17 tokens 37 (54)   64: 50 (138)   128: 88 (258)
   const int rep = H / G;
   const bool prompts = rep <= PROMPT_REP && (long long)max_tokens * rep >= PROMPT_ROWS && (always || (long long)ntok * H >= std::max(sm_count() / 3, 1) * 128ll);
   const unsigned share = always ? 1u : std::max(sm_count() / 4, 1) * 128u;
   if (prompts) {
-    // Two tiles a CTA where the rows are more than the SMs take at once with one, by a quarter.
-    const int pair = always ? give_up >> 4 & 1 : (long long)ntok * H > 160ll * sm_count();
+    // Two tiles a CTA where one would not do for all rows at once. us with one (two), a request of n tokens, 32 / 8 heads of 128: 300 after 1000 39 (53), 500: 44 (57),
+    // 600: 64 (58), 1000: 81 (71), 1500: 124 (101); 700 after 100 39 (42); 660 after 8000 280 (223)
+    const int pair = always ? give_up >> 4 & 1 : ((long long)ntok * rep + 127) / 128 * G > sm_count();
     const PromptArgs4 pa{q, q_tok_stride, q_head_stride, (const uint8_t*)k, (const uint8_t*)v, (const uint16_t*)k_word, (const uint16_t*)v_word, table, q_start, kv_len, requests, width,
                          npages, page_shift(page_tokens), ntok, G, rep, pair, share, scale * 1.4426950408889634f, out, out_tok_stride, out_head_stride, give_up};
     if (const int rc = launch_prompt(pa, D, dtype == QSPEC_DTYPE_BF16, (cudaStream_t)stream)) return rc;

@@ -60,7 +60,7 @@ __device__ __forceinline__ void butterflies(float (&x)[16], int c, uint32_t grou
 }
 
 // A warp takes `steps` times ROWS rows of a token, the next ones on their way: one look at the position and the angles for all of them. (Steps of two rows a lane, of which a warp took
-// no others, 37 us for a prompt of 4200 tokens, 40 / 8 heads; these 27; two steps ahead, and three CTAs an SM, 31.)
+// no others, 37 us for a prompt of 4200 tokens, 40 / 8 heads; these 25; two steps ahead, and three CTAs an SM, 31.)
 template <bool BF16, int D, bool HADAMARD>
 __global__ void __launch_bounds__(APPEND_WARPS * 32, 4) kv4_append_kernel(const AppendArgs a) {
   using T = typename Elem16<BF16>::T;
@@ -230,10 +230,11 @@ extern "C" int qspec_kv4_append(const void* qkv, long long ld, const void* cos_s
                 QSPEC_ERR_INVALID_ARG, "kv4_append: rows must lie on 16-byte boundaries (ld=%lld)", ld);
   AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (uint8_t*)k, (uint8_t*)v, (uint16_t*)k_word, (uint16_t*)v_word, q_out, q_tok_stride, ntok, H, G, npages,
                page_shift(page_tokens), 2 * G + (q_out ? H : 0), 0, 0};
-  // Steps of a warp: as few as leave about APPEND_FULL warps an SM.
-  constexpr int APPEND_FULL = 48;
+  // Steps of a warp: one while that makes no more than twice the warps that the SMs hold, else as few as they all hold at once (warps that come later begin a chain of loads of their own).
+  // us, 40 / 8 heads of 128, one step (as few as they hold): 256 tokens 9 (9), 512: 12 (14), 700: 15 (15), 1000: 18 (18), 1500: 24 (21), 2000: 30 (26), 4200: 56 (44), 8000: 101 (71)
   const int rows = D == 128 ? 4 : 8, most = (a.rows + rows - 1) / rows;
-  a.steps = (int)std::min<long long>(std::max<long long>((long long)ntok * most / (APPEND_FULL * (long long)max(sm_count(), 1)), 1), most);
+  const long long hold = 32ll * std::max(sm_count(), 1), at_once = std::max(hold / ntok, 1ll);   // warps; of a token
+  a.steps = (long long)ntok * most <= 2 * hold ? 1 : (int)((most + at_once - 1) / at_once);
   a.warps = (most + a.steps - 1) / a.steps;
   const long long warps = (long long)ntok * a.warps;
   QSPEC_REQUIRE(warps < (1ll << 31), QSPEC_ERR_UNSUPPORTED, "kv4_append: %d tokens are too many for one call", ntok);

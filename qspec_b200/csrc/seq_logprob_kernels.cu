@@ -460,10 +460,13 @@ extern "C" int qspec_seq_token_logprobs(const void* logits, long long row_stride
   const int size = dtype == QSPEC_DTYPE_F32 ? 4 : 2;
   QSPEC_REQUIRE(logits && (!top || (top_logprobs && top_tokens)) && (tokens || (!logprobs && !ranks)), QSPEC_ERR_INVALID_ARG, "token_logprobs: null pointer");
   QSPEC_REQUIRE((uintptr_t)logits % size == 0 && ((uintptr_t)tokens & 7) == 0, QSPEC_ERR_INVALID_ARG, "token_logprobs: logits and tokens must lie on their types' boundaries");
-  // CTAs of a row
-  const int sms = std::max(sm_count(), 1), batch = THREADS * EACH * 16 / size;
+  // CTAs of a row: two while that leaves the SMs four each at most, four while three, eight while two and a half (larger clusters find their places less well), and more than a batch
+  // each. us with 1 / 2 / 4 / 8, float16, 5 alternatives, a call alone (and calls behind one another, of which the next begins while the last rows of one are looked at):
+  //   128256 values   4 rows 20 / 16 / 13 / 12   45: 21 / 18 / 15 / 15   75: 22 / 18 / 17 / 25   148: 23 / 20 / 28 / 39   256: 28 / 30 / 36 (38 / 29 / 35)   330: (40 / 38 / 44)
+  //   32000 values    4 rows 10 / 11 / 9   100: 12 / 13 / 11   148: 12 / 13 / 19 (12 / 12 / 18)   256: 14 / 17 / 23 (17 / 16 / 22)   400: 16 / 26 / 32 (18 / 24 / 31)
+  const int sms = std::max(sm_count(), 1), batch = THREADS * EACH * 16 / size, halves[] = {8, 6, 5};
   int cluster = 1;
-  while (cluster < 8 && (long long)rows * cluster <= 2 * sms && V > cluster * batch) cluster *= 2;
+  for (int i = 0; i < 3 && 2ll * rows * (2 * cluster) <= (long long)halves[i] * sms && V > cluster * batch; ++i) cluster *= 2;
   const int span = ((V + cluster - 1) / cluster + 7) / 8 * 8;
   QSPEC_REQUIRE(V <= (1 << 24), QSPEC_ERR_UNSUPPORTED, "token_logprobs: a vocabulary of %d is too large", V);
   QSPEC_REQUIRE((long long)rows * cluster < (1ll << 31), QSPEC_ERR_UNSUPPORTED, "token_logprobs: %d rows are too many for one call", rows);
