@@ -19,8 +19,8 @@
 // whatever the scales are and are rounded to float16 for the product with the codes (by 2^-11 of themselves at most, or by 2^-34 of the largest: kv8_common.cuh); the denominator
 // is the sum of the unrounded weights / v.
 //
-// Measured: 64 requests of 4 tokens after some 3000 keys each, 32 / 8 heads of 128, 89 us, 2.3 TB/s of codes and words; one token after 131071 keys, 64 / 8 heads, 56 us, 2.4 TB/s; 4 requests of a
-// token after some 500 keys 15 us, which is launches and a chain of loads. At this many rows not the bytes bound it (a third of the time) but instructions: a unit of 32 keys takes a warp
+// Measured: 64 requests of 4 tokens after some 3000 keys each, 32 / 8 heads of 128, 86 us, 2.4 TB/s of codes and words; one token after 131071 keys, 64 / 8 heads, 56 us, 2.5 TB/s; 4 requests of a
+// token after some 680 keys 15 us, which is launches and a chain of loads. At this many rows not the bytes bound it (a third of the time) but instructions: a unit of 32 keys takes a warp
 // some 900, of which 64 are products and a third make codes operands; an SM issues two a cycle, the tensor cores are busy 28 % of the time.
 #include "kv4_common.cuh"
 #include "kv_stretch.cuh"
@@ -185,19 +185,19 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
     to[130] = half_pair(x[3], x[7]);
   };
 
-  // ---- a segment's units: warp w's are w, w + WARPS, .., two of them under way. Pages are looked up one unit ahead of the copies, so that these do not wait for them: a unit lies in one
+  // ---- a segment's units: warp w's are w, w + WARPS, .., two of them under way. Pages are looked up two units ahead of the copies, so that these do not wait for them: a unit lies in one
   // page, or (of 16 tokens) in two, of which odd lanes have the second.
   const int mask = (1 << a.pshift) - 1, second = a.pshift == 4 ? lane & 1 : 0;
   const int* table;                                         // the segment's request's
   int g, keys, next, end;                                   // its head and keys; the unit that is fetched next, the end of the segment's units
-  auto look = [&]() {
-    if (next >= end) return -1;
-    const int at = (next * UNIT >> a.pshift) + second;
+  auto look = [&](int unit) {
+    if (unit >= end) return -1;
+    const int at = (unit * UNIT >> a.pshift) + second;
     if ((at << a.pshift) >= keys || at >= a.width) return -1;
     const int page = table[at];
     return (unsigned)page < (unsigned)a.npages ? page : -1;
   };
-  int pages;
+  int pages, then;                                          // of the next unit, of the one behind it
   struct Unit4 {
     bool there;                                             // this lane's page
     int key0;                                               // first key
@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
     }
     copy_commit();
     next += WARPS;
-    pages = look();
+    pages = then;
+    then = look(next + WARPS);
     return unit;
   };
 
@@ -247,7 +248,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
     keys = cur.r.keys;
     next = cur.u + warp;
     end = cur.u + seg_n;
-    pages = look();
+    pages = look(next);
+    then = look(next + WARPS);
     const uint4 piece = load_q(cur);
     Unit4 unit0 = take(ring), unit1 = take(ring + S::STAGE);
     store_q(piece);

@@ -6,6 +6,7 @@
 // ends inside an item, through the workspace: the CTA that comes last adds the parts up in their order, so that results do not depend on which it is.
 #pragma once
 #include "kv8_common.cuh"
+#include <type_traits>
 
 namespace qspec {
 namespace kv8 {
@@ -84,11 +85,16 @@ struct Stretch {
   int share, todo;                                          // units that a CTA of such an item takes; units of this stretch
   long long begin, per;
 };
+__device__ __forceinline__ long long quotient(long long a, long long b) {   // of numbers that are not negative (in 32 bits where they fit: five times as fast)
+  return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
+}
 template <int WARPS, int GRID_MOST>
 __device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, unsigned long long& work_out, Stretch& out) {
   constexpr int THREADS = WARPS * 32, MIN_UNITS = WARPS;   // units of a stretch: one for each warp
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per_thread = (a.nreq + THREADS - 1) / THREADS, b0 = tid * per_thread;
+  // Up to 32 requests every warp looks for itself, without barriers (16 requests of 4 tokens after 2000 keys in 4 bits 29.7 -> 28.4 us).
+  const bool few = a.nreq <= 32;
+  const int lookers = few ? 32 : THREADS, per_thread = (a.nreq + lookers - 1) / lookers, b0 = (few ? lane : tid) * per_thread;
   const int requests = max(min(per_thread, a.nreq - b0), 0);
   unsigned long long work = 0;                              // that requests with rows enough for the prompt form ask for
   if (a.share) {
@@ -98,12 +104,14 @@ __device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, un
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-    if (lane == 0) s.sum[warp] = (long long)work;
-    __syncthreads();
-    work = 0;
+    if (!few) {
+      if (lane == 0) s.sum[warp] = (long long)work;
+      __syncthreads();
+      work = 0;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) work += (unsigned long long)s.sum[w];
-    __syncthreads();
+      for (int w = 0; w < WARPS; ++w) work += (unsigned long long)s.sum[w];
+      __syncthreads();
+    }
   }
   Req only{0, 0, 0, 0, 1};
   if (per_thread == 1 && b0 < a.nreq) only = request(a, b0, work);
@@ -116,9 +124,10 @@ __device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, un
       const long long w = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += w;
     }
+    before = incl - mine;
+    if (few) { total = __shfl_sync(0xffffffffu, incl, 31); return; }
     if (lane == 31) s.sum[warp] = incl;
     __syncthreads();
-    before = incl - mine;
     total = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
@@ -134,16 +143,18 @@ __device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, un
     items = min(items + (int)min((long long)r.tiles * a.G, (long long)GRID_MOST + 1), GRID_MOST + 1);
   }
   items = __reduce_add_sync(0xffffffffu, items);
-  if (lane == 0) s.items[warp] = items;
+  if (!few && lane == 0) s.items[warp] = items;
   scan(mine);
   const int grid = gridDim.x;
   long long per = max(total <= 0x7fffffff ? (long long)(((int)total - 1) / grid + 1) : (total + grid - 1) / grid, (long long)MIN_UNITS);
   // A stretch may lie over the end of an item: then the CTA joins and stores twice. With few items each gets CTAs of its own, as long as that makes no
   // stretch much longer (by a quarter and eight units at most): 4 requests of 900, 32 / 8 heads, one token each 17.0 -> 12.1 us.
   bool whole = false;
-  items = 0;
+  if (!few) {
+    items = 0;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) items += s.items[w];
+    for (int w = 0; w < WARPS; ++w) items += s.items[w];
+  }
   if (items <= grid && per < (1 << 24)) {
     constexpr int TRIES = 6;                                // lengths that are looked at
     auto length = [&](int c) { const int p = (int)per; return c == 0 ? p : c == 1 ? p + 1 : c == 2 ? p + p / 32 + 1 : c == 3 ? p + p / 16 + 2 : c == 4 ? p + p / 8 + 4 : p + p / 4 + 8; };
@@ -157,15 +168,18 @@ __device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, un
 #pragma unroll
     for (int c = 0; c < TRIES; ++c) {
       n[c] = __reduce_add_sync(0xffffffffu, n[c]);
-      if (lane == 0) s.ctas[c][warp] = n[c];
+      if (!few && lane == 0) s.ctas[c][warp] = n[c];
     }
-    __syncthreads();
+    if (!few) __syncthreads();
     int len = 0;
 #pragma unroll
     for (int c = TRIES - 1; c >= 0; --c) {
-      int sum = 0;
+      int sum = n[c];
+      if (!few) {
+        sum = 0;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) sum += s.ctas[c][w];
+        for (int w = 0; w < WARPS; ++w) sum += s.ctas[c][w];
+      }
       if (sum <= grid) len = length(c);
     }
     if (len) {
@@ -182,31 +196,49 @@ __device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, un
   // (an item's units are spread evenly over its CTAs)
   const long long begin = whole ? blockIdx.x : per * blockIdx.x;
   if (begin >= total) return false;
+  int place[4] = {-1, 0, 0, 1};                             // request, item of it (head * tiles + tile), CTA of the item or unit, how many of those
+  Req found{0, 0, 0, 0, 1};
   if (begin >= before && begin < before + mine) {
     long long at = before;
     for (int i = 0; i < requests; ++i) {
       const Req r = req(i);
-      const int each = whole ? (r.units - 1) / (int)per + 1 : r.units;   // of an item: CTAs, or units
+      const int each = whole ? (r.units - 1) / (int)per + 1 : r.units;
       const long long n = (long long)r.tiles * a.G * each;
       if (begin < at + n) {
-        s.place[0] = b0 + i;
-        s.place[1] = (int)((begin - at) / each);            // item of the request: head * tiles + tile
-        s.place[2] = (int)((begin - at) % each);
-        s.place[3] = each;
-        s.req = r;
+        place[0] = b0 + i;
+        place[1] = (int)quotient(begin - at, each);
+        place[2] = (int)(begin - at - (long long)place[1] * each);
+        place[3] = each;
+        found = r;
         break;
       }
       at += n;
     }
   }
-  __syncthreads();
+  if (few) {
+    const int who = __ffs(__ballot_sync(0xffffffffu, place[0] >= 0)) - 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) place[i] = __shfl_sync(0xffffffffu, place[i], who);
+    found = {__shfl_sync(0xffffffffu, found.first, who), __shfl_sync(0xffffffffu, found.n, who), __shfl_sync(0xffffffffu, found.keys, who), __shfl_sync(0xffffffffu, found.tiles, who),
+             __shfl_sync(0xffffffffu, found.units, who)};
+  } else {
+    if (place[0] >= 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.place[i] = place[i];
+      s.req = found;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) place[i] = s.place[i];
+    found = s.req;
+  }
   Place cur;
-  cur.b = s.place[0];
-  cur.r = s.req;
-  cur.g = s.place[1] / cur.r.tiles;
-  cur.tile = s.place[1] - cur.g * cur.r.tiles;
-  const int share = whole ? (cur.r.units - 1) / s.place[3] + 1 : 0;
-  cur.u = whole ? min(s.place[2] * share, cur.r.units) : s.place[2];
+  cur.b = place[0];
+  cur.r = found;
+  cur.g = place[1] / cur.r.tiles;
+  cur.tile = place[1] - cur.g * cur.r.tiles;
+  const int share = whole ? (cur.r.units - 1) / place[3] + 1 : 0;
+  cur.u = whole ? min(place[2] * share, cur.r.units) : place[2];
   const int todo = whole ? min(share, cur.r.units - cur.u) : (int)(min(begin + per, total) - begin);
   work_out = work;
   out = Stretch{cur, whole, share, todo, begin, per};
@@ -232,20 +264,22 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
   float4 oo[PIECES];
 #pragma unroll
   for (int c = 0; c < PIECES; ++c) oo[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto join = [&](float mw, float lw, auto&& piece) {
+  // the warps' maxima and sums first: loads that wait for none before them
+  float mw[WARPS], lw[WARPS];
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) { mw[w] = s_ml[(w * 2) * ROWS + jr]; lw[w] = s_ml[(w * 2 + 1) * ROWS + jr]; }
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
     // (a part that saw nothing has no sums; one that saw NaN has a sum that is not zero)
-    if (mw == NONE && lw == 0.f) return;
-    const float mn = fmaxf(mm, mw), f = mm == NONE ? 0.f : exp2_fast(mm - mn), h = mw == NONE ? 1.f : exp2_fast(mw - mn);
-    mm = mn;
-    ll = ll * f + lw * h;
+    const bool none = mw[w] == NONE && lw[w] == 0.f;
+    const float mn = fmaxf(mm, mw[w]), f = mm == NONE ? 0.f : exp2_fast(mm - mn), h = mw[w] == NONE ? 1.f : exp2_fast(mw[w] - mn);
+    if (!none) { mm = mn; ll = ll * f + lw[w] * h; }
 #pragma unroll
     for (int c = 0; c < PIECES; ++c) {
-      const float4 p = piece(c);
-      oo[c].x = oo[c].x * f + p.x * h; oo[c].y = oo[c].y * f + p.y * h; oo[c].z = oo[c].z * f + p.z * h; oo[c].w = oo[c].w * f + p.w * h;
+      const float4 p = *reinterpret_cast<const float4*>(s_o + (w * ROWS + jr) * LD + (col + PER_ROW * c) * 4);
+      if (!none) { oo[c].x = oo[c].x * f + p.x * h; oo[c].y = oo[c].y * f + p.y * h; oo[c].z = oo[c].z * f + p.z * h; oo[c].w = oo[c].w * f + p.w * h; }
     }
-  };
-  for (int w = 0; w < WARPS; ++w)
-    join(s_ml[(w * 2) * ROWS + jr], s_ml[(w * 2 + 1) * ROWS + jr], [&](int c) { return *reinterpret_cast<const float4*>(s_o + (w * ROWS + jr) * LD + (col + PER_ROW * c) * 4); });
+  }
   auto store_piece = [&](int r, int at, const float4& p, float f) {   // columns at .. at + 3 of the tile's row r
     const int rr = cur.tile * ROWS + r, tok = rr / a.rep;
     uint2 w;
@@ -267,7 +301,7 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
   } else {
     // ---- a part of an item: into the workspace; the item's last CTA to come adds all of them up, first part first
     const long long item0 = w0.begin + seg0 - cur.u, item1 = item0 + cur.r.units;
-    const int c0 = w0.whole ? (int)blockIdx.x - cur.u / w0.share : (int)(item0 / w0.per), c1 = w0.whole ? c0 + (cur.r.units - 1) / w0.share : (int)((item1 - 1) / w0.per);
+    const int c0 = w0.whole ? (int)blockIdx.x - cur.u / w0.share : (int)quotient(item0, w0.per), c1 = w0.whole ? c0 + (cur.r.units - 1) / w0.share : (int)quotient(item1 - 1, w0.per);
     float* part = o.parts + (size_t)(2 * blockIdx.x + (starts ? 1 : 0)) * PART<D>;
     if (col == 0) { part[jr] = mm; part[ROWS + jr] = ll; }
 #pragma unroll
@@ -318,22 +352,26 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
       if (col == 0) factor[n * ROWS + jr] = ll == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, ll);   // (no key: zeros)
       __syncthreads();
       const int rows = min(cur.r.n * a.rep - cur.tile * ROWS, ROWS);
-      for (int x = tid; x < rows * (D / 4); x += THREADS) {
-        const int r = x / (D / 4), at = x % (D / 4) * 4;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = 0; i0 < n; i0 += 32) {
-          float4 v[32];
+      auto add = [&](auto most) {                           // parts of which loads are under way
+        constexpr int MOST = decltype(most)::value;
+        for (int x = tid; x < rows * (D / 4); x += THREADS) {
+          const int r = x / (D / 4), at = x % (D / 4) * 4;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int i0 = 0; i0 < n; i0 += MOST) {
+            float4 v[MOST];
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            v[k] = i0 + k < n ? __ldcg(reinterpret_cast<const float4*>(from(i0 + k) + 2 * ROWS + r * D + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < MOST; ++k)
+              v[k] = i0 + k < n ? __ldcg(reinterpret_cast<const float4*>(from(i0 + k) + 2 * ROWS + r * D + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const float f = i0 + k < n ? factor[(i0 + k) * ROWS + r] : 0.f;
-            sum.x = fmaf(v[k].x, f, sum.x); sum.y = fmaf(v[k].y, f, sum.y); sum.z = fmaf(v[k].z, f, sum.z); sum.w = fmaf(v[k].w, f, sum.w);
+            for (int k = 0; k < MOST; ++k) {
+              const float f = i0 + k < n ? factor[(i0 + k) * ROWS + r] : 0.f;
+              sum.x = fmaf(v[k].x, f, sum.x); sum.y = fmaf(v[k].y, f, sum.y); sum.z = fmaf(v[k].z, f, sum.z); sum.w = fmaf(v[k].w, f, sum.w);
+            }
           }
+          store_piece(r, at, sum, factor[n * ROWS + r]);
         }
-        store_piece(r, at, sum, factor[n * ROWS + r]);
-      }
+      };
+      if (n <= 4) add(std::integral_constant<int, 4>{}); else add(std::integral_constant<int, 32>{});
     }
   }
 }
