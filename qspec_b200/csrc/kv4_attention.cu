@@ -1,7 +1,7 @@
 // Softmax attention over a key/value cache in pages and in 4 bits (its layout and numbers: kv4_common.cuh). Token i of the n that request b has in the step stands at
 // position kv_len[b] - n + i and sees the keys up to its own position.
 //
-// A row is a (token, query head of a group) pair; 16 rows of one key/value head are a tile of mma.sync.m16n8k16, so that the heads of a group and the
+// A row is a (token, query head of a group) pair; 16 rows of one key/value head (or 8) are a tile of mma.sync.m16n8k16, so that the heads of a group and the
 // tokens that verify a draft share every key that is read. What bounds it at these row counts is the cache: D + 4 bytes a key and head. How the work is spread over
 // the GPU, and the parts joined: kv_stretch.cuh.
 //
@@ -19,9 +19,9 @@
 // whatever the scales are and are rounded to float16 for the product with the codes (by 2^-11 of themselves at most, or by 2^-34 of the largest: kv8_common.cuh); the denominator
 // is the sum of the unrounded weights / v.
 //
-// Measured: 64 requests of 4 tokens after some 3000 keys each, 32 / 8 heads of 128, 86 us, 2.4 TB/s of codes and words; one token after 131071 keys, 64 / 8 heads, 56 us, 2.5 TB/s; 4 requests of a
-// token after some 680 keys 15 us, which is launches and a chain of loads. At this many rows not the bytes bound it (a third of the time) but instructions: a unit of 32 keys takes a warp
-// some 900, of which 64 are products and a third make codes operands; an SM issues two a cycle, the tensor cores are busy 28 % of the time.
+// Measured: 64 requests of 4 tokens after some 3000 keys each, 32 / 8 heads of 128, 77 us, 2.7 TB/s of codes and words; one token after 131071 keys, 64 / 8 heads, 49 us, 2.8 TB/s; 4 requests of a
+// token after some 680 keys 12.7 us, which is launches and a chain of loads. At this many rows not the bytes bound it (two fifths of the time) but instructions: a unit of 32 keys takes a
+// warp some 650, of which 64 are products and 250 make codes operands; the tensor cores are busy 38 % of a long walk, the units of integer arithmetic 45 %.
 #include "kv4_common.cuh"
 #include "kv_stretch.cuh"
 
@@ -29,9 +29,14 @@ namespace qspec {
 namespace kv4 {
 using namespace kv8;
 
-constexpr int WARPS = 8, THREADS = WARPS * 32;
-constexpr int CTAS = 2;                          // of an SM: while one waits at a barrier the other computes
-constexpr int GRID_MOST = 320;                   // CTAs
+// Tiles of sixteen rows (tokens x heads of a group), or of eight where no request has more: then codes are the products' first operand, rows the second, of eight columns, and half
+// of the products, exponentials and sums' registers go. us of eight (of sixteen), 32 / 8 heads of 128, one token a request: 64 requests after 3000 keys 58 (76), after 700: 22 (34);
+// 256 after 1000: 86 (106); 4 after 676: 12.2 (12.8); one after 131071, 64 / 8 heads: 51 (57); one request of 2 after 20000 26 (24).
+// CTAs of an SM (while one waits at a barrier the others compute) x warps, us of 64 requests after 3000 keys, after 700, and of one after 131071 (eight rows) or 4 tokens after 20000
+// (sixteen): eight rows 2 x 8 66, 32, 52; 3 x 4 62, 30, 46; 4 x 4 58, 22, 51; 5 x 4 67, 26, 58; sixteen rows 2 x 8 86, 40, 27; 3 x 4 77, 32, 27; 4 x 4 78, 28, 36.
+template <int TR> struct Shape {
+  static constexpr int WARPS = 4, CTAS = TR == 8 ? 4 : 3, THREADS = WARPS * 32, GRID_MOST = 160 * CTAS;
+};
 
 struct AttArgs : Step, Out {
   const void* q; long long q_ts; int q_hs;
@@ -40,18 +45,19 @@ struct AttArgs : Step, Out {
   float scale2;                                  // scale * log2(e)
 };
 
-template <int D> struct Smem {
+template <int D, int TR> struct Smem {
+  static constexpr int WARPS = Shape<TR>::WARPS, GRID_MOST = Shape<TR>::GRID_MOST;
   static constexpr int ROW = D / 2, CODES = UNIT * ROW, STAGES = 2;
   static constexpr int WORDS = 2 * CODES, STAGE = WORDS + 2 * UNIT * 2;   // keys, values, words of either
   static constexpr int FACTORS = 16 * 16 * 2 + 8 * 16;                    // what the words of a unit's keys come to, in the order of the products
   static constexpr int WARP = STAGES * STAGE + FACTORS;
   static constexpr int LD = D + 8;                                      // floats of a row of sums on its way between warps
   // units, or (at a segment's end) sums on their way between warps, or a factor for every part of an item
-  static constexpr size_t RING = (size_t)WARPS * WARP, SUMS = (size_t)WARPS * ROWS * LD * 4, PARTS = (size_t)(GRID_MOST + 1) * ROWS * 4;
+  static constexpr size_t RING = (size_t)WARPS * WARP, SUMS = (size_t)WARPS * TR * LD * 4, PARTS = (size_t)(GRID_MOST + 1) * TR * 4;
   static constexpr size_t ROOM = RING > SUMS ? (RING > PARTS ? RING : PARTS) : SUMS > PARTS ? SUMS : PARTS;
-  static constexpr size_t Q = ROWS * D * 2;
-  static constexpr size_t ML = (size_t)WARPS * ROWS * 2 * 4;
-  static constexpr size_t F = ROWS * 4;                                 // the rows' powers of two
+  static constexpr size_t Q = TR * D * 2;
+  static constexpr size_t ML = (size_t)WARPS * TR * 2 * 4;
+  static constexpr size_t F = TR * 4;                                 // the rows' powers of two
   static constexpr size_t TOTAL = ROOM + Q + ML + F;
   static_assert(STAGE % 16 == 0 && WARP % 16 == 0 && ROOM % 16 == 0, "16-byte boundaries");
 };
@@ -93,6 +99,8 @@ __device__ __forceinline__ uint32_t half_fma(uint32_t a, uint32_t b, uint32_t c)
 }
 // (x & mask) | magic in one instruction, which two constants would make two: they are kept in registers.
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) { uint32_t r; asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(r) : "r"(x), "r"(mask), "r"(magic)); return r; }
+// an 8 x 8 matrix of 16-bit values, two of a row a lane, columns for rows
+__device__ __forceinline__ uint32_t turned(uint32_t x) { uint32_t r; asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(x)); return r; }
 __device__ __forceinline__ uint32_t held(uint32_t x) { uint32_t r; asm volatile("mov.b32 %0, %1;\n" : "=r"(r) : "r"(x)); return r; }
 
 // Where the 16 bytes c of a row lie in a buffer, so that neither copies nor reads of eight rows meet in a bank (a row is half a line of banks, or a quarter).
@@ -107,7 +115,7 @@ template <int D> __device__ __forceinline__ uint32_t v_chunk(int row, int c) {
 // but as codes, which are codes like any other and meet weights of zero.
 template <int D>
 __device__ __noinline__ void fetch_parts(const uint8_t* k, const uint8_t* v, const uint16_t* kw, const uint16_t* vw, int pshift, long long row, int have, uint32_t dst) {
-  using S = Smem<D>;
+  using S = Smem<D, ROWS>;
   constexpr int CH = D / 32, PER = 32 / CH;       // 16-byte pieces of a row; rows per instruction
   const int lane = threadIdx.x & 31, c = lane % CH, row0 = lane / CH;
 #pragma unroll 1
@@ -125,11 +133,13 @@ __device__ __noinline__ void fetch_parts(const uint8_t* k, const uint8_t* v, con
   }
 }
 
-template <bool BF16, int D>
-__global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttArgs a) {
+template <bool BF16, int D, int TR>
+__global__ void __launch_bounds__(Shape<TR>::THREADS, Shape<TR>::CTAS) kv4_attention_kernel(const AttArgs a) {
   using T = typename Elem16<BF16>::T;
-  using S = Smem<D>;
-  constexpr int NT = D / 8, W = D / 32, KT = UNIT / 8, QT = UNIT / 16;   // column tiles of the value product, words that a lane has of a key, key tiles
+  using S = Smem<D, TR>;
+  constexpr bool FEW = TR == 8;
+  constexpr int WARPS = Shape<TR>::WARPS, THREADS = Shape<TR>::THREADS;
+  constexpr int NT = D / (FEW ? 16 : 8), W = D / 32, KT = UNIT / 8, QT = UNIT / 16;   // column tiles of the value product, words that a lane has of a key, key tiles
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Shared<WARPS> s_sh;
   __shared__ Stretch s_stretch;
@@ -145,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
   unsigned long long work;
   {
     Stretch stretch;
-    if (!find_stretch<WARPS, GRID_MOST>(a, s_sh, work, stretch)) return;
+    if (!find_stretch<WARPS, Shape<TR>::GRID_MOST, TR>(a, s_sh, work, stretch)) return;
     if (tid == 0) s_stretch = stretch;
   }
 
@@ -153,16 +163,18 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
   // register) of the operand. A lane's word i of a key has columns 8 (W j + i) .. + 7; step 2 i takes the first and the second of each four of them, step 2 i + 1 the
   // third and the fourth.
   constexpr int IN_ROW = D / 8;
-  static_assert(ROWS * IN_ROW <= THREADS, "a piece a thread");
+  constexpr int AT_ONCE = THREADS / IN_ROW, PIECES = (TR + AT_ONCE - 1) / AT_ONCE;   // rows; pieces of a thread
   const int qr = tid / IN_ROW, qc = tid % IN_ROW;
-  auto load_q = [&](const Place& p) {
-    const int row = p.tile * ROWS + qr, tok = row / a.rep;
-    uint4 piece = make_uint4(0u, 0u, 0u, 0u);
-    if (qr < ROWS && tok < p.r.n)
-      piece = *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(p.r.first + tok) * a.q_ts + (size_t)(p.g * a.rep + row - tok * a.rep) * a.q_hs + qc * 8);
-    return piece;
+  auto load_q = [&](const Place& p, uint4 (&pieces)[PIECES]) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int r = qr + i * AT_ONCE, row = p.tile * TR + r, tok = row / a.rep;
+      pieces[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < TR && tok < p.r.n)
+        pieces[i] = *reinterpret_cast<const uint4*>((const T*)a.q + (size_t)(p.r.first + tok) * a.q_ts + (size_t)(p.g * a.rep + row - tok * a.rep) * a.q_hs + qc * 8);
+    }
   };
-  auto store_q = [&](const uint4& piece) {
+  auto store_q = [&](const uint4& piece, int r) {
     float x[8], mx = 0.f;
     unpack8<BF16>(piece, x);
 #pragma unroll
@@ -176,20 +188,21 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
     const float up = __uint_as_float((uint32_t)(127 + sh) << 23);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= e & 1 ? up * 0.0625f : up;
-    if (qr >= ROWS) return;
-    if (qc == 0) s_f[qr] = __uint_as_float((uint32_t)(some ? 127 - sh : 1) << 23);   // (those have no say in the tile's largest)
-    uint32_t* to = reinterpret_cast<uint32_t*>(s_q) + (qc % W) * 2 * 128 + ((qr & 7) * 4 + qc / W) * 4 + (qr >> 3);
+    if (r >= TR) return;
+    if (qc == 0) s_f[r] = __uint_as_float((uint32_t)(some ? 127 - sh : 1) << 23);   // (those have no say in the tile's largest)
+    constexpr int STEP = 8 * TR, REG = TR / 8;              // words of a step; from a register of a row to the row's next
+    uint32_t* to = reinterpret_cast<uint32_t*>(s_q) + (qc % W) * 2 * STEP + ((r & 7) * 4 + qc / W) * 2 * REG + (r >> 3);
     to[0] = half_pair(x[0], x[4]);
-    to[2] = half_pair(x[1], x[5]);
-    to[128] = half_pair(x[2], x[6]);
-    to[130] = half_pair(x[3], x[7]);
+    to[REG] = half_pair(x[1], x[5]);
+    to[STEP] = half_pair(x[2], x[6]);
+    to[STEP + REG] = half_pair(x[3], x[7]);
   };
 
   // ---- a segment's units: warp w's are w, w + WARPS, .., two of them under way. Pages are looked up two units ahead of the copies, so that these do not wait for them: a unit lies in one
   // page, or (of 16 tokens) in two, of which odd lanes have the second.
   const int mask = (1 << a.pshift) - 1, second = a.pshift == 4 ? lane & 1 : 0;
   const int* table;                                         // the segment's request's
-  int g, keys, next, end;                                   // its head and keys; the unit that is fetched next, the end of the segment's units
+  int g = 0, keys = 0, next = 0, end = 0;                   // its head and keys; the unit that is fetched next, the end of the segment's units
   auto look = [&](int unit) {
     if (unit >= end) return -1;
     const int at = (unit * UNIT >> a.pshift) + second;
@@ -235,7 +248,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
 
   const uint32_t low4 = held(0x000f000fu), high4 = held(0x00f000f0u), magic = held(0x64006400u);
   // where this lane's key leaves what it comes to
-  const uint32_t words = ring + S::WORDS + lane * 2, mine = factors + (((lane >> 4) * 2 + (lane & 1)) * 4 + (lane >> 2 & 3)) * 16 + (lane >> 1 & 1) * 4;
+  const uint32_t words = ring + S::WORDS + lane * 2;
+  const uint32_t mine = FEW ? factors + (((lane >> 4) * 2 + (lane & 1)) * 8 + (lane >> 1 & 7)) * 16 : factors + (((lane >> 4) * 2 + (lane & 1)) * 4 + (lane >> 2 & 3)) * 16 + (lane >> 1 & 1) * 4;
   const uint32_t zeros = factors + 512 + ((lane >> 4) * 4 + (lane >> 2 & 3)) * 16 + (lane & 1) * 4 + (lane >> 1 & 1) * 2;
   int seg0 = 0;                                             // index in the stretch of the segment's first unit
   __syncthreads();
@@ -250,32 +264,42 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
     end = cur.u + seg_n;
     pages = look(next);
     then = look(next + WARPS);
-    const uint4 piece = load_q(cur);
+    uint4 pieces[PIECES];
+    load_q(cur, pieces);
     Unit4 unit0 = take(ring), unit1 = take(ring + S::STAGE);
-    store_q(piece);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) store_q(pieces[i], qr + i * AT_ONCE);
     __syncthreads();
     uint32_t stage = 0;
-    const uint32_t frag = shared_addr(s_q) + lane * 16;
-    auto query = [&](uint32_t (&x)[4], int step) { lds128(x, frag + step * 512); };
+    const uint32_t frag = shared_addr(s_q) + lane * TR;
+    auto query = [&](uint32_t (&x)[TR / 4], int step) { if constexpr (FEW) lds64(x, frag + step * 256); else lds128(x, frag + step * 512); };
     // The rows' powers of two: the tile's largest goes into the keys' factors, what a row is below it (at most 1) stays the row's.
     float big = s_f[0];
 #pragma unroll
-    for (int r = 1; r < ROWS; ++r) big = fmaxf(big, s_f[r]);
-    const float own[2] = {s_f[qi] / big, s_f[qi + 8] / big}, factor = big * a.scale2;
+    for (int r = 1; r < TR; ++r) big = fmaxf(big, s_f[r]);
+    const int row0 = FEW ? 2 * qj : qi, row1 = FEW ? 2 * qj + 1 : qi + 8;   // this lane's rows of the tile
+    const float own[2] = {s_f[row0] / big, s_f[row1] / big}, factor = big * a.scale2;
     int limit[2];                                           // last visible position of this lane's rows
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int tok = (tile * ROWS + qi + 8 * e) / a.rep;
+      const int tok = (tile * TR + (e ? row1 : row0)) / a.rep;
       limit[e] = tok < cur.r.n ? min(cur.r.keys - cur.r.n + tok, cur.r.keys - 1) : -1;
     }
-    const int low = cur.r.keys - cur.r.n + tile * ROWS / a.rep;   // the lowest of the tile's rows
+    const int low = cur.r.keys - cur.r.n + tile * TR / a.rep;   // the lowest of the tile's rows
     // the rows' sums, in units of 2^-24 like the scores
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
+    uint32_t qf[FEW ? 2 * W : 1][2];                        // (eight rows' queries stay in registers)
 #pragma unroll
     for (int i = 0; i < 2 * W; ++i) {
-      uint32_t x[4];
-      query(x, i);
-      mma16816(sums, x, 0x00010001u, 0x00100010u);
+      if constexpr (FEW) {
+        const uint32_t ones[4] = {0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u};
+        query(qf[i], i);
+        mma16816(sums, ones, qf[i][0], qf[i][1]);
+      } else {
+        uint32_t x[4];
+        query(x, i);
+        mma16816(sums, x, 0x00010001u, 0x00100010u);
+      }
     }
     float o[NT][4];
 #pragma unroll
@@ -296,15 +320,21 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
         float f = word_scale(kw) * factor * 16777216.f, v = fmaxf(word_scale(vw), 7.888609052210118e-31f);
         if (bad) { f = NAN; v = 1.f; }                      // rows that see it are no numbers
         if (key0 + lane >= keys) f = 0.f;
-        sts32(mine, __float_as_uint(f));
-        sts32(mine + 8, __float_as_uint(__uint_as_float(0xcb000000u | (kw & 15u)) + 8388608.f));   // - z
-        sts32(mine + 256, __float_as_uint(__log2f(v)));
-        sts32(mine + 264, __float_as_uint(__fdividef(WEIGHT_UNIT, v)));
+        const uint32_t x[4] = {__float_as_uint(f), __float_as_uint(__uint_as_float(0xcb000000u | (kw & 15u)) + 8388608.f) /* - z */, __float_as_uint(__log2f(v)),
+                               __float_as_uint(__fdividef(WEIGHT_UNIT, v))};
+        if constexpr (FEW) {
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(mine), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+        } else {
+          sts32(mine, x[0]);
+          sts32(mine + 8, x[1]);
+          sts32(mine + 256, x[2]);
+          sts32(mine + 264, x[3]);
+        }
         sts16(zeros, 0xe400u + (vw & 15u));                 // -1024 - z
         sts16(zeros + 8, 0xd400u + ((vw & 15u) << 4));      // -64 - z
       }
       // ---- scores of the unit's keys, in units of 2^-24
-      float s[KT][4];
+      float s[FEW ? QT : KT][4];                            // few rows: of 16 keys, [key 2 j + b and the next][this lane's rows]
       {
         uint32_t w[KT][W];
 #pragma unroll
@@ -312,78 +342,130 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
           const uint32_t at = buf + k_row<D>((n >> 1) * 16 + (n & 1) + (qi >> 1) * 4 + (qi & 1) * 2) + qj * (W * 4);
           if constexpr (W == 4) lds128(w[n], at); else lds64(w[n], at);
         }
+        if constexpr (FEW) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          uint32_t x[4], y[4];
-          query(x, 2 * i);
-          query(y, 2 * i + 1);
+          for (int i = 0; i < W; ++i)
 #pragma unroll
-          for (int n = 0; n < KT; ++n) {
-            if (i == 0) mma16816_first(s[n], x, w[n][i] & 0x000f000fu, w[n][i] & 0x00f000f0u);
-            else mma16816(s[n], x, w[n][i] & 0x000f000fu, w[n][i] & 0x00f000f0u);
+            for (int q = 0; q < QT; ++q) {
+              const uint32_t u = w[2 * q][i], v = w[2 * q + 1][i];
+              const uint32_t x[4] = {u & 0x000f000fu, v & 0x000f000fu, u & 0x00f000f0u, v & 0x00f000f0u};
+              const uint32_t y[4] = {u >> 8 & 0x000f000fu, v >> 8 & 0x000f000fu, u >> 8 & 0x00f000f0u, v >> 8 & 0x00f000f0u};
+              if (i == 0) mma16816_first(s[q], x, qf[0][0], qf[0][1]); else mma16816(s[q], x, qf[2 * i][0], qf[2 * i][1]);
+              mma16816(s[q], y, qf[2 * i + 1][0], qf[2 * i + 1][1]);
+            }
+        } else {
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            uint32_t x[4], y[4];
+            query(x, 2 * i);
+            query(y, 2 * i + 1);
+#pragma unroll
+            for (int n = 0; n < KT; ++n) {
+              if (i == 0) mma16816_first(s[n], x, w[n][i] & 0x000f000fu, w[n][i] & 0x00f000f0u);
+              else mma16816(s[n], x, w[n][i] & 0x000f000fu, w[n][i] & 0x00f000f0u);
+            }
+#pragma unroll
+            for (int n = 0; n < KT; ++n) mma16816(s[n], y, w[n][i] >> 8 & 0x000f000fu, w[n][i] >> 8 & 0x00f000f0u);
           }
-#pragma unroll
-          for (int n = 0; n < KT; ++n) mma16816(s[n], y, w[n][i] >> 8 & 0x000f000fu, w[n][i] >> 8 & 0x00f000f0u);
         }
       }
       __syncwarp();                                         // (the factors are there)
       // ---- exponents
       float mx[2] = {NONE, NONE};
+      uint64_t iv2[FEW ? KT : 1];                           // unit / v of this lane's keys, twice
+      if constexpr (FEW) {
 #pragma unroll
-      for (int n = 0; n < KT; ++n) {
-        uint32_t x[4], y[2];
-        const uint32_t at = factors + (n * 4 + qj) * 16;
-        lds128(x, at);
-        lds64(y, at + 256);
-        const uint64_t f = two(__uint_as_float(x[0]), __uint_as_float(x[1])), zero = two(__uint_as_float(x[2]), __uint_as_float(x[3])), lv = two(__uint_as_float(y[0]), __uint_as_float(y[1]));
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint64_t score = ffma2_rn(zero, two(sums[2 * e], sums[2 * e]), two(s[n][2 * e], s[n][2 * e + 1]));
-          const float2 r = unpack_f2(ffma2_rn(score, mul2(f, two(own[e], own[e])), lv));
-          s[n][2 * e] = r.x;
-          s[n][2 * e + 1] = r.y;
+        for (int n = 0; n < KT; ++n) {
+          uint32_t x[4];
+          lds128(x, factors + (n * 8 + qi) * 16);
+          const float f = __uint_as_float(x[0]), zero = __uint_as_float(x[1]), lv = __uint_as_float(x[2]), iv = __uint_as_float(x[3]);
+          float* const y = s[n >> 1] + (n & 1) * 2;
+          const uint64_t score = ffma2_rn(two(zero, zero), two(sums[0], sums[1]), two(y[0], y[1]));
+          const float2 r = unpack_f2(ffma2_rn(score, mul2(two(f, f), two(own[0], own[1])), two(lv, lv)));
+          y[0] = r.x;
+          y[1] = r.y;
+          iv2[n] = two(iv, iv);
         }
-      }
-      if (key0 + UNIT - 1 > low) {                          // keys that a row does not see
+        if (key0 + UNIT - 1 > low) {                        // keys that a row does not see
+#pragma unroll
+          for (int n = 0; n < KT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (key0 + (n >> 1) * 16 + (qi >> 1) * 4 + (qi & 1) * 2 + (n & 1) > limit[e]) s[n >> 1][(n & 1) * 2 + e] = NONE;
+        }
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) mx[e] = fmaxf(fmaxf(mx[e], s[q][e]), s[q][2 + e]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < KT; ++n) {
+          uint32_t x[4], y[2];
+          const uint32_t at = factors + (n * 4 + qj) * 16;
+          lds128(x, at);
+          lds64(y, at + 256);
+          const uint64_t f = two(__uint_as_float(x[0]), __uint_as_float(x[1])), zero = two(__uint_as_float(x[2]), __uint_as_float(x[3])), lv = two(__uint_as_float(y[0]), __uint_as_float(y[1]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint64_t score = ffma2_rn(zero, two(sums[2 * e], sums[2 * e]), two(s[n][2 * e], s[n][2 * e + 1]));
+            const float2 r = unpack_f2(ffma2_rn(score, mul2(f, two(own[e], own[e])), lv));
+            s[n][2 * e] = r.x;
+            s[n][2 * e + 1] = r.y;
+          }
+        }
+        if (key0 + UNIT - 1 > low) {                          // keys that a row does not see
+#pragma unroll
+          for (int n = 0; n < KT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key0 + (n >> 1) * 16 + qj * 4 + (e & 1) * 2 + (n & 1) > limit[e >> 1]) s[n][e] = NONE;
+        }
 #pragma unroll
         for (int n = 0; n < KT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (key0 + (n >> 1) * 16 + qj * 4 + (e & 1) * 2 + (n & 1) > limit[e >> 1]) s[n][e] = NONE;
+          for (int e = 0; e < 2; ++e) mx[e] = fmaxf(fmaxf(mx[e], s[n][2 * e]), s[n][2 * e + 1]);
       }
-#pragma unroll
-      for (int n = 0; n < KT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) mx[e] = fmaxf(fmaxf(mx[e], s[n][2 * e]), s[n][2 * e + 1]);
       // The reference follows the maximum only where it has fallen behind: sums are seldom multiplied again.
       if (__any_sync(0xffffffffu, mx[0] > m[0] + GROWTH_LOG2 || mx[1] > m[1] + GROWTH_LOG2)) {   // (of a row that had seen nothing, more than minus infinity)
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+#pragma unroll
+          for (int x = FEW ? 4 : 1; x < (FEW ? 32 : 4); x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
           const bool grown = mx[e] > m[e] + GROWTH_LOG2;
           f[e] = grown && m[e] != NONE ? exp2_fast(m[e] - mx[e]) : 1.f;   // (a row that had seen nothing has sums of zero)
           if (grown) m[e] = mx[e];
-          l2[e] = mul2(l2[e], two(f[e], f[e]));
+          if (!FEW) l2[e] = mul2(l2[e], two(f[e], f[e]));
         }
+        if (FEW) l2[0] = mul2(l2[0], two(f[0], f[1]));
 #pragma unroll
-        for (int t = 0; t < NT; ++t) { o[t][0] *= f[0]; o[t][1] *= f[0]; o[t][2] *= f[1]; o[t][3] *= f[1]; }
+        for (int t = 0; t < NT; ++t) { o[t][0] *= f[0]; o[t][1] *= f[FEW]; o[t][2] *= f[!FEW]; o[t][3] *= f[1]; }
       }
       // ---- weights
-      uint32_t pa[QT][4];
+      uint32_t pa[QT][TR / 4];
       const float ref[2] = {m[0] == NONE ? 0.f : WEIGHT_LOG2 - m[0], m[1] == NONE ? 0.f : WEIGHT_LOG2 - m[1]};
+      if constexpr (FEW) {
 #pragma unroll
-      for (int n = 0; n < KT; ++n) {
-        uint32_t y[2];
-        lds64(y, factors + (n * 4 + qj) * 16 + 264);
-        const uint64_t iv = two(__uint_as_float(y[0]), __uint_as_float(y[1]));
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 x = unpack_f2(add2(two(s[n][2 * e], s[n][2 * e + 1]), two(ref[e], ref[e])));
+        for (int n = 0; n < KT; ++n) {
+          const float* const y = s[n >> 1] + (n & 1) * 2;
+          const float2 x = unpack_f2(add2(two(y[0], y[1]), two(ref[0], ref[1])));
           const float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
-          l2[e] = ffma2_rn(two(w0, w1), iv, l2[e]);
-          pa[n >> 1][(n & 1) * 2 + e] = half_pair(w0, w1);
+          l2[0] = ffma2_rn(two(w0, w1), iv2[n], l2[0]);
+          pa[n >> 1][n & 1] = turned(half_pair(w0, w1));    // (a lane has two rows of a key; the product takes two keys of a row)
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < KT; ++n) {
+          uint32_t y[2];
+          lds64(y, factors + (n * 4 + qj) * 16 + 264);
+          const uint64_t iv = two(__uint_as_float(y[0]), __uint_as_float(y[1]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 x = unpack_f2(add2(two(s[n][2 * e], s[n][2 * e + 1]), two(ref[e], ref[e])));
+            const float w0 = exp2_fast(x.x), w1 = exp2_fast(x.y);
+            l2[e] = ffma2_rn(two(w0, w1), iv, l2[e]);
+            pa[n >> 1][(n & 1) * 2 + e] = half_pair(w0, w1);
+          }
         }
       }
       // ---- values
@@ -395,12 +477,25 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
         for (int c = 0; c < W; c += 2) {                    // 64 columns at a time
           uint32_t w[4];
           load_columns(w, buf + S::CODES + v_chunk<D>(q * 16 + (lane & 15), c + (lane >> 4)));
+          if constexpr (FEW) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const uint32_t u0 = w[2 * t], v0 = u0 >> 8, u1 = w[2 * t + 1], v1 = u1 >> 8;
+              const uint32_t x[4] = {half_add(and_or(u0, low4, magic), zero[0]), half_add(and_or(u1, low4, magic), zero[0]), half_add(and_or(v0, low4, magic), zero[1]),
+                                     half_add(and_or(v1, low4, magic), zero[1])};
+              mma16816(o[2 * (c + t)], x, pa[q][0], pa[q][1]);
+              const uint32_t y[4] = {half_fma(and_or(u0, high4, magic), 0x2c002c00u, zero[2]), half_fma(and_or(u1, high4, magic), 0x2c002c00u, zero[2]),
+                                     half_fma(and_or(v0, high4, magic), 0x2c002c00u, zero[3]), half_fma(and_or(v1, high4, magic), 0x2c002c00u, zero[3])};   // (times 1 / 16)
+              mma16816(o[2 * (c + t) + 1], y, pa[q][0], pa[q][1]);
+            }
+          } else {
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const uint32_t u = w[t], v = w[t] >> 8;
             mma16816(o[4 * c + 2 * t], pa[q], half_add(and_or(u, low4, magic), zero[0]), half_add(and_or(v, low4, magic), zero[1]));
             mma16816(o[4 * c + 2 * t + 1], pa[q], half_fma(and_or(u, high4, magic), 0x2c002c00u, zero[2]),
                      half_fma(and_or(v, high4, magic), 0x2c002c00u, zero[3]));   // (times 1 / 16)
+          }
           }
         }
       }
@@ -413,28 +508,37 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
     __syncthreads();                                        // (sums take the units' place)
 
     // ---- the warps' sums of this item together
+    const float2 l0 = unpack_f2(l2[0]), l1 = unpack_f2(l2[1]);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float2 both = unpack_f2(l2[e]);
-      float l = both.x + both.y;
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      if (qj == 0) {
-        s_ml[(warp * 2) * ROWS + qi + 8 * e] = m[e];
-        s_ml[(warp * 2 + 1) * ROWS + qi + 8 * e] = l;
+      float l = FEW ? (e ? l0.y : l0.x) : e ? l1.x + l1.y : l0.x + l0.y;
+#pragma unroll
+      for (int x = FEW ? 4 : 1; x < (FEW ? 32 : 4); x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+      const int r = e ? row1 : row0;
+      if ((FEW ? qi : qj) == 0) {
+        s_ml[(warp * 2) * TR + r] = m[e];
+        s_ml[(warp * 2 + 1) * TR + r] = l;
       }
       // (a warp without a unit in this segment has nothing but its maximum to tell)
       if (m[e] != NONE || l != 0.f) {
-        float* row = s_o + (warp * ROWS + qi + 8 * e) * S::LD + qj * 4;   // (bytes 2 j and 2 j + 1 of eight: four columns)
+        float* row = s_o + (warp * TR + r) * S::LD + (FEW ? qi * 2 : qj * 4);
+        if constexpr (FEW) {                                // (bytes j and j + 8 of sixteen: two columns each)
 #pragma unroll
-        for (int t = 0; t < NT; t += 2) *reinterpret_cast<float4*>(row + 8 * t) = make_float4(o[t][2 * e], o[t + 1][2 * e], o[t][2 * e + 1], o[t + 1][2 * e + 1]);
+          for (int t = 0; t < NT; t += 2) {
+            *reinterpret_cast<float2*>(row + 16 * t) = make_float2(o[t][e], o[t + 1][e]);
+            *reinterpret_cast<float2*>(row + 16 * t + 16) = make_float2(o[t][2 + e], o[t + 1][2 + e]);
+          }
+        } else {                                            // (bytes 2 j and 2 j + 1 of eight: four columns)
+#pragma unroll
+          for (int t = 0; t < NT; t += 2) *reinterpret_cast<float4*>(row + 8 * t) = make_float4(o[t][2 * e], o[t + 1][2 * e], o[t][2 * e + 1], o[t + 1][2 * e + 1]);
+        }
       }
     }
-    finish_segment<BF16, D, S::LD, WARPS>(a, a, s_stretch, s_stretch.cur, seg0, seg_n, s_ml, s_o, s_sh);
+    finish_segment<BF16, D, S::LD, WARPS, TR>(a, a, s_stretch, s_stretch.cur, seg0, seg_n, s_ml, s_o, s_sh);
     seg0 += seg_n;
     if (seg0 >= s_stretch.todo) break;
     __syncthreads();                                        // the sums have been read, and so has the segment's place
-    if (tid == 0) s_stretch.cur.forward(a, work, seg_n);
+    if (tid == 0) s_stretch.cur.forward<TR>(a, work, seg_n);
     __syncthreads();
   }
 }
@@ -445,9 +549,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
 using namespace qspec;
 using namespace qspec::kv4;
 
-static int att_grid() { return max(sm_count(), 1) * CTAS; }
+template <int TR> int att_grid() { return max(sm_count(), 1) * Shape<TR>::CTAS; }
 
-extern "C" size_t qspec_kv4_attention_workspace_bytes(void) { return 4096 + (size_t)att_grid() * 2 * PART<128> * sizeof(float); }
+extern "C" size_t qspec_kv4_attention_workspace_bytes(void) { return 4096 + std::max((size_t)att_grid<8>() * PART<128, 8>, (size_t)att_grid<16>() * PART<128>) * 2 * sizeof(float); }
 
 static int attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const void* k_word, const void* v_word, const int* table,
                      const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H, int G, int D, int npages,
@@ -469,8 +573,7 @@ static int attention(const void* q, long long q_tok_stride, int q_head_stride, c
                 QSPEC_ERR_INVALID_ARG, "kv4_attention: rows must lie on 16-byte boundaries");
   QSPEC_REQUIRE(workspace && workspace_bytes >= qspec_kv4_attention_workspace_bytes() && ((uintptr_t)workspace & 15) == 0, QSPEC_ERR_WORKSPACE,
                 "kv4_attention: %zu bytes of workspace needed, got %zu", qspec_kv4_attention_workspace_bytes(), workspace_bytes);
-  const int grid = att_grid();
-  QSPEC_REQUIRE(grid <= GRID_MOST, QSPEC_ERR_UNSUPPORTED, "kv4_attention: %d SMs", sm_count());
+  QSPEC_REQUIRE(sm_count() <= 160, QSPEC_ERR_UNSUPPORTED, "kv4_attention: %d SMs", sm_count());
   // Requests with many rows may go to the prompt form (to_prompt_form()), in a launch of its own in front; none do if the call's rows are too few for a third of
   // the SMs (always: for tests). Both forms measured, 32 / 8 heads of 128, us of the prompt form (of the other):
   //   1 request, 1000 keys in front of it   32 tokens 37 (19)   128: 37 (23)   160: 38 (39)   256: 38 (51)   1024: 71 (204)
@@ -491,16 +594,20 @@ static int attention(const void* q, long long q_tok_stride, int q_head_stride, c
   const AttArgs a{{table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok, G, rep, prompts ? share : 0u},
                   {out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)}, q, q_tok_stride, q_head_stride, (const uint8_t*)k, (const uint8_t*)v,
                   (const uint16_t*)k_word, (const uint16_t*)v_word, scale * 1.4426950408889634f};
-  auto run = [&](auto kern, size_t smem, SmemLimit& limit) -> int {
+  auto run = [&](auto kern, int grid, int threads, size_t smem, SmemLimit& limit) -> int {
     QSPEC_CUDA(limit.raise(kern, smem));
-    QSPEC_CUDA(launch_pdl(kern, dim3(grid), dim3(THREADS), smem, (cudaStream_t)stream, a));
+    QSPEC_CUDA(launch_pdl(kern, dim3(grid), dim3(threads), smem, (cudaStream_t)stream, a));
     QSPEC_CHECK_LAUNCH(1);
     return QSPEC_OK;
   };
-  static SmemLimit limits[4];
-  if (dtype == QSPEC_DTYPE_F16)
-    return D == 128 ? run(kv4_attention_kernel<false, 128>, Smem<128>::TOTAL, limits[0]) : run(kv4_attention_kernel<false, 64>, Smem<64>::TOTAL, limits[1]);
-  return D == 128 ? run(kv4_attention_kernel<true, 128>, Smem<128>::TOTAL, limits[2]) : run(kv4_attention_kernel<true, 64>, Smem<64>::TOTAL, limits[3]);
+  static SmemLimit limits[8];
+  const bool few = (long long)max_tokens * rep <= 8;
+#define QSPEC_KV4_ATTENTION(BF, D, I)                                                                                                   \
+  (few ? run(kv4_attention_kernel<BF, D, 8>, att_grid<8>(), Shape<8>::THREADS, Smem<D, 8>::TOTAL, limits[I])                            \
+       : run(kv4_attention_kernel<BF, D, 16>, att_grid<16>(), Shape<16>::THREADS, Smem<D, 16>::TOTAL, limits[4 + I]))
+  if (dtype == QSPEC_DTYPE_F16) return D == 128 ? QSPEC_KV4_ATTENTION(false, 128, 0) : QSPEC_KV4_ATTENTION(false, 64, 1);
+  return D == 128 ? QSPEC_KV4_ATTENTION(true, 128, 2) : QSPEC_KV4_ATTENTION(true, 64, 3);
+#undef QSPEC_KV4_ATTENTION
 }
 
 extern "C" int qspec_kv4_attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const void* k_word, const void* v_word, const int* table,

@@ -11,9 +11,9 @@
 namespace qspec {
 namespace kv8 {
 
-constexpr int UNIT = 32, ROWS = 16;
+constexpr int UNIT = 32, ROWS = 16;               // keys of a unit; rows of a tile (or, where a kernel says so, eight: TR)
 constexpr float NONE = -INFINITY;
-template <int D> constexpr int PART = ROWS * 2 + ROWS * D;   // floats of a part: maxima, sums, sums of values
+template <int D, int TR = ROWS> constexpr int PART = TR * 2 + TR * D;   // floats of a part: maxima, sums, sums of values
 
 // The step's requests, as all kernels of a call see them.
 struct Step {
@@ -30,13 +30,14 @@ struct Req {
   int first, n, keys, tiles, units;               // first row of q, tokens, keys, row tiles, units of an item
   __device__ __forceinline__ long long total(int G) const { return (long long)tiles * G * units; }
 };
+template <int TR = ROWS>
 __device__ __forceinline__ Req request(const Step& a, int b, unsigned long long work) {
   Req r;
   r.first = min(max(a.q_start[b], 0), a.ntok);
   r.n = max(min(a.q_start[b + 1], a.ntok) - r.first, 0);
   r.keys = max(a.kv_len[b], 0);
   const long long rows = (long long)r.n * a.rep;
-  r.tiles = to_prompt_form(r.n, r.keys, a.rep, a.share, work) ? 0 : (int)((rows + ROWS - 1) / ROWS);
+  r.tiles = to_prompt_form(r.n, r.keys, a.rep, a.share, work) ? 0 : (int)((rows + TR - 1) / TR);
   // A request without keys has a unit that shows its rows none. Behind the table's last page is nothing but a page that there is not: one unit shows that.
   r.units = max((min(r.keys, keys_at_most(a.width, a.pshift)) + UNIT - 1) / UNIT, 1);
   return r;
@@ -46,6 +47,7 @@ __device__ __forceinline__ Req request(const Step& a, int b, unsigned long long 
 struct Place {
   int b, g, tile, u;
   Req r;
+  template <int TR = ROWS>
   __device__ __forceinline__ void forward(const Step& a, unsigned long long work, int steps) {
     u += steps;
     while (b < a.nreq && u >= r.units) {
@@ -54,7 +56,7 @@ struct Place {
       tile = 0;
       if (++g < a.G) continue;
       g = 0;
-      do { if (++b >= a.nreq) return; r = request(a, b, work); } while (r.tiles == 0);
+      do { if (++b >= a.nreq) return; r = request<TR>(a, b, work); } while (r.tiles == 0);
     }
   }
 };
@@ -88,7 +90,7 @@ struct Stretch {
 __device__ __forceinline__ long long quotient(long long a, long long b) {   // of numbers that are not negative (in 32 bits where they fit: five times as fast)
   return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
 }
-template <int WARPS, int GRID_MOST>
+template <int WARPS, int GRID_MOST, int TR = ROWS>
 __device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, unsigned long long& work_out, Stretch& out) {
   constexpr int THREADS = WARPS * 32, MIN_UNITS = WARPS;   // units of a stretch: one for each warp
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -99,7 +101,7 @@ __device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, un
   unsigned long long work = 0;                              // that requests with rows enough for the prompt form ask for
   if (a.share) {
     for (int i = 0; i < requests; ++i) {
-      const Req r = request(a, b0 + i, 0);
+      const Req r = request<TR>(a, b0 + i, 0);
       work += prompt_work(r.n, r.keys, a.rep, a.G);
     }
 #pragma unroll
@@ -114,8 +116,8 @@ __device__ __forceinline__ bool find_stretch(const Step& a, Shared<WARPS>& s, un
     }
   }
   Req only{0, 0, 0, 0, 1};
-  if (per_thread == 1 && b0 < a.nreq) only = request(a, b0, work);
-  auto req = [&](int i) { return per_thread == 1 ? only : request(a, b0 + i, work); };
+  if (per_thread == 1 && b0 < a.nreq) only = request<TR>(a, b0, work);
+  auto req = [&](int i) { return per_thread == 1 ? only : request<TR>(a, b0 + i, work); };
   long long before, total;                                  // of the requests of the threads in front of this one, and of all
   auto scan = [&](long long mine) {
     long long incl = mine;
@@ -250,16 +252,17 @@ struct Out {
   void* out; long long out_ts; int out_hs;
   int* counters; float* parts;
 };
-// The warps' sums of an item's segment (units cur.u .. cur.u + seg_n - 1, from the stretch's unit seg0 on) together: s_ml [warp][maximum, sum][16], s_o
-// [warp][16][LD] sums of values, written by the warps (not by one that saw nothing); to the rows, or, of a part of an item, into the workspace.
-template <bool BF16, int D, int LD, int WARPS>
+// The warps' sums of an item's segment (units cur.u .. cur.u + seg_n - 1, from the stretch's unit seg0 on) together: s_ml [warp][maximum, sum][TR], s_o
+// [warp][TR][LD] sums of values, written by the warps (not by one that saw nothing); to the rows, or, of a part of an item, into the workspace.
+template <bool BF16, int D, int LD, int WARPS, int TR = ROWS>
 __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, const Stretch& w0, const Place& cur, int seg0, int seg_n, float* s_ml, float* s_o, Shared<WARPS>& s) {
   using T = typename Elem16<BF16>::T;
   constexpr int THREADS = WARPS * 32;
   const int tid = threadIdx.x;
   __syncthreads();
-  constexpr int PER_ROW = THREADS / ROWS, PIECES = D / 4 / PER_ROW;   // threads of a row, float4 of a thread
-  const int jr = tid / PER_ROW, col = tid % PER_ROW;
+  constexpr int PER_ROW = THREADS / TR < D / 4 ? THREADS / TR : D / 4, PIECES = D / 4 / PER_ROW;   // threads of a row, float4 of a thread
+  const int jr = min(tid / PER_ROW, TR - 1), col = tid % PER_ROW;
+  const bool spare = TR * PER_ROW < THREADS && tid >= TR * PER_ROW;   // (does what others do)
   float mm = NONE, ll = 0.f;
   float4 oo[PIECES];
 #pragma unroll
@@ -267,7 +270,7 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
   // the warps' maxima and sums first: loads that wait for none before them
   float mw[WARPS], lw[WARPS];
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) { mw[w] = s_ml[(w * 2) * ROWS + jr]; lw[w] = s_ml[(w * 2 + 1) * ROWS + jr]; }
+  for (int w = 0; w < WARPS; ++w) { mw[w] = s_ml[(w * 2) * TR + jr]; lw[w] = s_ml[(w * 2 + 1) * TR + jr]; }
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
     // (a part that saw nothing has no sums; one that saw NaN has a sum that is not zero)
@@ -276,12 +279,12 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
     if (!none) { mm = mn; ll = ll * f + lw[w] * h; }
 #pragma unroll
     for (int c = 0; c < PIECES; ++c) {
-      const float4 p = *reinterpret_cast<const float4*>(s_o + (w * ROWS + jr) * LD + (col + PER_ROW * c) * 4);
+      const float4 p = *reinterpret_cast<const float4*>(s_o + (w * TR + jr) * LD + (col + PER_ROW * c) * 4);
       if (!none) { oo[c].x = oo[c].x * f + p.x * h; oo[c].y = oo[c].y * f + p.y * h; oo[c].z = oo[c].z * f + p.z * h; oo[c].w = oo[c].w * f + p.w * h; }
     }
   }
   auto store_piece = [&](int r, int at, const float4& p, float f) {   // columns at .. at + 3 of the tile's row r
-    const int rr = cur.tile * ROWS + r, tok = rr / a.rep;
+    const int rr = cur.tile * TR + r, tok = rr / a.rep;
     uint2 w;
     if (BF16) {
       const __nv_bfloat162 x = __floats2bfloat162_rn(p.x * f, p.y * f), y = __floats2bfloat162_rn(p.z * f, p.w * f);
@@ -293,7 +296,7 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
   };
   const bool starts = cur.u == 0, ends = cur.u + seg_n == cur.r.units;
   if (starts && ends) {
-    if (cur.tile * ROWS + jr < cur.r.n * a.rep) {
+    if (cur.tile * TR + jr < cur.r.n * a.rep) {
       const float f = ll == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, ll);   // (no key: zeros)
 #pragma unroll
       for (int c = 0; c < PIECES; ++c) store_piece(jr, (col + PER_ROW * c) * 4, oo[c], f);
@@ -302,10 +305,10 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
     // ---- a part of an item: into the workspace; the item's last CTA to come adds all of them up, first part first
     const long long item0 = w0.begin + seg0 - cur.u, item1 = item0 + cur.r.units;
     const int c0 = w0.whole ? (int)blockIdx.x - cur.u / w0.share : (int)quotient(item0, w0.per), c1 = w0.whole ? c0 + (cur.r.units - 1) / w0.share : (int)quotient(item1 - 1, w0.per);
-    float* part = o.parts + (size_t)(2 * blockIdx.x + (starts ? 1 : 0)) * PART<D>;
-    if (col == 0) { part[jr] = mm; part[ROWS + jr] = ll; }
+    float* part = o.parts + (size_t)(2 * blockIdx.x + (starts ? 1 : 0)) * PART<D, TR>;
+    if (col == 0) { part[jr] = mm; part[TR + jr] = ll; }
 #pragma unroll
-    for (int c = 0; c < PIECES; ++c) *reinterpret_cast<float4*>(part + 2 * ROWS + jr * D + (col + PER_ROW * c) * 4) = oo[c];
+    for (int c = 0; c < PIECES; ++c) *reinterpret_cast<float4*>(part + 2 * TR + jr * D + (col + PER_ROW * c) * 4) = oo[c];
     __syncthreads();
     if (tid == 0) {
       __threadfence();                                    // (of what the whole CTA has stored: the barrier is in front of it)
@@ -318,7 +321,7 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
       // All maxima and sums first (eight threads a row), which gives every part its factor, then the sums of values: loads that wait for none before them.
       __threadfence();
       const int n = c1 - c0 + 1;
-      auto from = [&](int i) { return o.parts + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * PART<D>; };
+      auto from = [&](int i) { return o.parts + (size_t)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * PART<D, TR>; };
       float* const factor = s_o;                          // [part][row]: the sums on their way between warps have been read
       mm = NONE;
       ll = 0.f;
@@ -328,7 +331,7 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
         for (int k = 0; k < 8; ++k) {
           const int i = i0 + k * PER_ROW;
           mp[k] = i < n ? __ldcg(from(i) + jr) : NONE;
-          lp[k] = i < n ? __ldcg(from(i) + ROWS + jr) : 0.f;
+          lp[k] = i < n ? __ldcg(from(i) + TR + jr) : 0.f;
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -336,7 +339,7 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
           const float mn = fmaxf(mm, mp[k]);
           ll = (mm == NONE ? ll : ll * exp2_fast(mm - mn)) + (none ? lp[k] : lp[k] * exp2_fast(mp[k] - mn));
           mm = mn;
-          if (i0 + k * PER_ROW < n) factor[(i0 + k * PER_ROW) * ROWS + jr] = none && lp[k] != 0.f ? INFINITY : mp[k];
+          if (i0 + k * PER_ROW < n && !spare) factor[(i0 + k * PER_ROW) * TR + jr] = none && lp[k] != 0.f ? INFINITY : mp[k];
         }
       }
       const float own = mm;
@@ -345,13 +348,13 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
       if (own != NONE) ll *= exp2_fast(own - mm);
 #pragma unroll
       for (int x = PER_ROW / 2; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
-      for (int i = col; i < n; i += PER_ROW) {
-        const float f = factor[i * ROWS + jr];
-        factor[i * ROWS + jr] = f == NONE ? 0.f : f == INFINITY ? 1.f : exp2_fast(f - mm);
+      for (int i = col; i < n && !spare; i += PER_ROW) {
+        const float f = factor[i * TR + jr];
+        factor[i * TR + jr] = f == NONE ? 0.f : f == INFINITY ? 1.f : exp2_fast(f - mm);
       }
-      if (col == 0) factor[n * ROWS + jr] = ll == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, ll);   // (no key: zeros)
+      if (col == 0) factor[n * TR + jr] = ll == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, ll);   // (no key: zeros)
       __syncthreads();
-      const int rows = min(cur.r.n * a.rep - cur.tile * ROWS, ROWS);
+      const int rows = min(cur.r.n * a.rep - cur.tile * TR, TR);
       auto add = [&](auto most) {                           // parts of which loads are under way
         constexpr int MOST = decltype(most)::value;
         for (int x = tid; x < rows * (D / 4); x += THREADS) {
@@ -361,14 +364,14 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
             float4 v[MOST];
 #pragma unroll
             for (int k = 0; k < MOST; ++k)
-              v[k] = i0 + k < n ? __ldcg(reinterpret_cast<const float4*>(from(i0 + k) + 2 * ROWS + r * D + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+              v[k] = i0 + k < n ? __ldcg(reinterpret_cast<const float4*>(from(i0 + k) + 2 * TR + r * D + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < MOST; ++k) {
-              const float f = i0 + k < n ? factor[(i0 + k) * ROWS + r] : 0.f;
+              const float f = i0 + k < n ? factor[(i0 + k) * TR + r] : 0.f;
               sum.x = fmaf(v[k].x, f, sum.x); sum.y = fmaf(v[k].y, f, sum.y); sum.z = fmaf(v[k].z, f, sum.z); sum.w = fmaf(v[k].w, f, sum.w);
             }
           }
-          store_piece(r, at, sum, factor[n * ROWS + r]);
+          store_piece(r, at, sum, factor[n * TR + r]);
         }
       };
       if (n <= 4) add(std::integral_constant<int, 4>{}); else add(std::integral_constant<int, 32>{});

@@ -654,3 +654,56 @@ def test_scales_next_to_a_half_are_those_of_the_formula():
     for got_c, got_w, rows in ((k, kw, x[:, G:2 * G]), (v, vw, x[:, 2 * G:])):
         c, w = quantised(rows.float())
         assert torch.equal(got_w, w.view(n // P, P, G).transpose(1, 2)) and torch.equal(got_c, c.view(n // P, P, G, D // 2).transpose(1, 2))
+
+
+# ---- tiles of eight rows: calls that say that no request has more (and hold if one does) ----------------------------------------------
+@pytest.fixture
+def eights(monkeypatch):
+    """`attend` with one token as the most of a request."""
+    import sys
+    whole = attend
+    monkeypatch.setattr(sys.modules[__name__], "attend", lambda form, *args, max_tokens=None, **kw: whole(form, *args, max_tokens=1, **kw))
+
+
+@pytest.mark.parametrize("H,G,D,P,dtype", [(64, 8, 128, 16, torch.bfloat16), (32, 8, 128, 128, torch.float16), (3, 1, 128, 64, torch.bfloat16), (8, 8, 64, 32, torch.float16), (14, 2, 64, 16, torch.bfloat16)])
+@pytest.mark.parametrize("lens,counts", [([1, 2, 31, 32, 33, 700], [1] * 6), ([64, 65, 1000, 5], [2, 1, 2, 0]), ([40000, 3], [1, 2]), ([70] * 300, [1] * 300), ([900] * 33, [1] * 33),
+                                         ([130, 400, 9], [130, 17, 3])])
+def test_eights_of_requests_of_every_kind(eights, H, G, D, P, dtype, lens, counts):
+    check_attention(make_attention(31, lens, counts, H, G, D, P, dtype), D)
+
+
+def test_eights_of_rows_that_see_nothing_of_scales_and_queries_far_apart_and_of_broken_ones(eights):
+    test_attention_rows_that_see_nothing_and_rows_of_no_request("rows")
+    test_attention_of_rows_of_very_different_sizes()
+    test_attention_of_strided_queries_and_outputs("rows")
+    test_attention_walks_no_further_than_the_table("rows")
+    for counts in ([1, 2, 1], [40, 2, 70]):
+        test_attention_shows_what_is_broken_and_only_there("rows", counts)
+        test_attention_with_scales_far_apart("rows", counts)
+    for q_scale in (0.0, 1e-30, 1e30):
+        test_attention_of_queries_of_any_size(q_scale, "rows")
+    for log2 in (-112, 100, 120):
+        test_attention_of_queries_and_scales_that_make_up_for_each_other(log2, "rows")
+    test_attention_of_scores_far_from_zero("rows")
+    test_attention_of_requests_with_more_tokens_than_keys(6, 2, "rows")
+
+
+def test_eights_are_the_same_every_time_in_a_graph_and_over_their_own_queries():
+    case = make_attention(32, [5000, 333, 64, 1800], [1, 1, 1, 1], 32, 8, 128, 64, torch.float16)
+    work, out = ops.kv4_attention_workspace("cuda"), torch.empty_like(case[0])
+    want = check_attention(case, 128, max_tokens=1, workspace=work)
+    ops.kv4_attention(*case, out, 128 ** -0.5, work, max_tokens=1)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.kv4_attention(*case, out, 128 ** -0.5, work, max_tokens=1)
+    for _ in range(20):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    q = case[0].clone()
+    ops.kv4_attention(q, *case[1:], q, 128 ** -0.5, work, max_tokens=1)
+    assert torch.equal(q, want)
+    # a workspace serves calls of either kind, one after the other
+    sixteen = check_attention(case, 128, max_tokens=5, workspace=work)
+    assert torch.equal(check_attention(case, 128, max_tokens=1, workspace=work), want) and torch.equal(check_attention(case, 128, max_tokens=5, workspace=work), sixteen)
