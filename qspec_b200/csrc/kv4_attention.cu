@@ -146,8 +146,8 @@ __global__ void __launch_bounds__(Shape<TR>::THREADS, Shape<TR>::CTAS) kv4_atten
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, qi = lane >> 2, qj = lane & 3;
   unsigned char* const s_q = smem + S::ROOM;
   float* const s_o = reinterpret_cast<float*>(smem);
-  float* const s_ml = reinterpret_cast<float*>(smem + S::ROOM + S::Q);   // [warp][maximum, sum][16]
-  float* const s_f = reinterpret_cast<float*>(smem + S::ROOM + S::Q + S::ML);   // [16]
+  float* const s_ml = reinterpret_cast<float*>(smem + S::ROOM + S::Q);   // [warp][maximum, sum][TR]
+  float* const s_f = reinterpret_cast<float*>(smem + S::ROOM + S::Q + S::ML);   // [TR]
   const uint32_t ring = shared_addr(smem) + warp * S::WARP, factors = ring + S::STAGES * S::STAGE;
   pdl_enter();
 
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(Shape<TR>::THREADS, Shape<TR>::CTAS) kv4_atten
   // a lane's places in a unit that lies in one page: 512 bytes of codes an instruction, of which its 16 are always in the same place of their rows
   const uint32_t kdst = k_row<D>(lane / (D / 32)) + lane % (D / 32) * 16, vdst = v_chunk<D>(lane / (D / 32), lane % (D / 32));
   const uint32_t wdst = S::WORDS + (lane & 7) * 16;
-  auto take = [&](uint32_t dst) {                           // the next unit, and the pages of the one behind it
+  auto take = [&](uint32_t dst) {                           // the next unit, and the pages of the one two behind it
     Unit4 unit;
     unit.there = pages >= 0;
     unit.key0 = next * UNIT;

@@ -172,3 +172,25 @@ def test_what_is_refused():
                      ((x[:, :3].contiguous(), t, None, None, None, tlp, tt), {}), ((x[:, :0], t, lp), {})):
         with pytest.raises(ValueError):
             ops.token_logprobs(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("shape", ["random", "rising", "ties", "few larger ones in every batch", "up"])
+@pytest.mark.parametrize("top", [1, 5, 8, 9])
+def test_best_of_long_rows_that_a_cta_has_to_itself(shape, top, dtype):
+    """Spans of more than eight batches: the best are first brought up to date in their middle, from candidates of many batches."""
+    rows, V = 600, 140003
+    at = torch.arange(V, device="cuda")
+    x = torch.randn(V, generator=gen(5), device="cuda")
+    x = {"random": 3 * x, "rising": x + at / 30000, "ties": (3 * x).round(), "up": at / V,
+         "few larger ones in every batch": torch.where(at % 2001 == 1000, 6.0 + at // 40000 + (at // 2001 % 3) / 4, x)}[shape].to(dtype)
+    logits = x.roll(11)[None].repeat(rows, 1)
+    logits[1::2] = logits[1::2].roll(977, 1)
+    tokens = torch.randint(0, V, (rows,), generator=gen(2), device="cuda")
+    _, _, rank, tlp, tt = call(logits, tokens, top)
+    for row in (0, 1):                                        # the even rows are alike, and the odd ones
+        best = logits[row].sort(descending=True, stable=True).indices[:top]
+        assert torch.equal(tt[row::2], best.expand(rows // 2, top)), row
+        p = torch.log_softmax(logits[row].double(), -1)[best]
+        assert ((tlp[row::2] - p).abs() <= p.abs() * 2.0 ** -22 + (V / 2048 + 16) * 2.0 ** -24 + 2.0 ** -21 + 40 * 2.0 ** -23).all()
+        assert torch.equal(rank[row::2], (logits[row] > logits[row, tokens[row::2]][:, None]).sum(-1) + 1)
