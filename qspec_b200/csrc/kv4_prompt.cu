@@ -23,7 +23,9 @@
 // cycles; its products are 2050 (64 each), the exponentials 2050 of a scheduler's special function unit, and both streams wait for one another's: the scores of a block take
 // 800 to 1200 cycles, the softmax 2300 alone and 3400 beside the other's, the sum of values 800. Measured and not taken (us): two accumulators of 64 keys each for a stream, scores a turn
 // ahead (151: a product of 64 columns takes as long as one of 128); one thread for both streams' products (119); the streams' exponentials in turn (120), or the second stream
-// half a turn late (122: they fall into step again); 32 scores at a time, read again for the weights (118); the steps of the codes rolled into one piece of code (160).
+// half a turn late (122: they fall into step again); 32 scores at a time, read again for the weights (118); the steps of the codes rolled into one piece of code (160). A CTA has
+// 13 000 cycles to its first weights (its place 2 900, tensor memory 800, queries 6 000, the first scores 2 400) and 6 000 behind its last; here 108 SMs have two CTAs, 40 have one. (Queries put in
+// order by whoever brought them, and rows out by 32 columns: 1 500 cycles less, and no time.)
 //
 // Every wait is bounded; a CTA whose wait runs out waits (again with a limit) for its products under way, fills its rows with NaN, counts itself
 // (qspec_attn_tile_timeouts) and frees its tensor memory.
@@ -465,15 +467,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
       const Block& f = s_block[n % FACS];
       // ---- the largest exponent: of the second half, whose scores are read again, and the first, whose scores stay
       float mn = NONE;
-#pragma unroll 1
-      for (int c0 = 64; c0 < 128; c0 += 32) {
-        ld32(st + c0, x);
-        wait_ld();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) landed8(x + 8 * j);
-        if (!plain) hide(x, 32, c0);
-        mn = largest(x, mn);
-      }
       auto load = [&](int c0) {
         ld32(st + c0, x);
         ld32(st + c0 + 32, x + 32);
@@ -482,9 +475,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
         for (int j = 0; j < 8; ++j) landed8(x + 8 * j);
         if (!plain) hide(x, 64, c0);
       };
-      load(0);
-      mn = largest(x, mn);
-      mn = largest(x + 32, mn);
+#pragma unroll 1
+      for (int c0 = 64; c0 >= 0; c0 -= 64) {
+        load(c0);
+        mn = largest(x, mn);
+        mn = largest(x + 32, mn);
+      }
       // The block's powers of two: what scores are multiplied with (not so small that it would make a hidden key's minus infinity no number), what exponents begin with
       const float k = fmaxf(rowf * __uint_as_float((uint32_t)min(max(f.ke - TOP, 1), 254) << 23), 1.17549435e-38f), lv = (float)(f.ve - 127 - TOP);
       const float iv = __uint_as_float((uint32_t)min(max(127 + 127 + TOP - f.ve, 1), 254) << 23) * WEIGHT_UNIT;
