@@ -19,8 +19,8 @@
 // whatever the scales are and are rounded to float16 for the product with the codes (by 2^-11 of themselves at most, or by 2^-34 of the largest: kv8_common.cuh); the denominator
 // is the sum of the unrounded weights / v.
 //
-// Measured: 64 requests of 4 tokens after some 3000 keys each, 32 / 8 heads of 128, 77 us, 2.7 TB/s of codes and words; one token after 131071 keys, 64 / 8 heads, 49 us, 2.8 TB/s; 4 requests of a
-// token after some 680 keys 12.7 us, which is launches and a chain of loads. At this many rows not the bytes bound it (two fifths of the time) but instructions: a unit of 32 keys takes a
+// Measured: 64 requests of 4 tokens after some 3000 keys each, 32 / 8 heads of 128, 77 us, 2.7 TB/s of codes and words; one token after 131071 keys, 64 / 8 heads, 44 us, 3.2 TB/s; 4 requests of a
+// token after some 680 keys 12 us, which is launches and a chain of loads. At this many rows not the bytes bound it (two fifths of the time) but instructions: a unit of 32 keys takes a
 // warp some 650, of which 64 are products and 250 make codes operands; the tensor cores are busy 38 % of a long walk, the units of integer arithmetic 45 %.
 #include "kv4_common.cuh"
 #include "kv_stretch.cuh"
@@ -31,12 +31,12 @@ using namespace kv8;
 
 // Tiles of sixteen rows (tokens x heads of a group), or of eight where no request has more: then codes are the products' first operand, rows the second, of eight columns, and half
 // of the products, exponentials and sums' registers go. us of eight (of sixteen), 32 / 8 heads of 128, one token a request: 64 requests after 3000 keys 58 (76), after 700: 22 (34);
-// 256 after 1000: 86 (106); 4 after 676: 12.2 (12.8); one after 131071, 64 / 8 heads: 51 (57); one request of 2 after 20000 26 (24).
-// CTAs of an SM (while one waits at a barrier the others compute) x warps, us of 64 requests after 3000 keys, after 700, and of one after 131071 (eight rows) or 4 tokens after 20000
-// (sixteen): eight rows 2 x 8 66, 32, 52; 3 x 4 62, 30, 46; 4 x 4 58, 22, 51; 5 x 4 67, 26, 58; sixteen rows 2 x 8 86, 40, 27; 3 x 4 77, 32, 27; 4 x 4 78, 28, 36.
-template <int TR> struct Shape {
-  static constexpr int WARPS = 4, CTAS = TR == 8 ? 4 : 3, THREADS = WARPS * 32, GRID_MOST = 160 * CTAS;
-};
+// 256 after 1000: 86 (106); 4 after 676: 11.7 (12.8); one of 2 after 20000: 21 (24); one after 131071, 64 / 8 heads: 46 (57).
+// CTAs of an SM (while one waits at a barrier the others compute): three of four warps; four, for tiles of eight, where requests x heads of keys are more than three CTAs an SM, so that each
+// may still have CTAs of its own. us with three (with four), a token each: 16 requests after 3000 keys 25 (26), 32: 40 (38), 48: 45 (52), 64: 62 (58), after 700 keys 30 (22); one after
+// 131071 46 (52). Two of eight warps: 66, 32, 52; five of four: 67, 26, 58. Tiles of sixteen, 64 requests of 4 tokens after 3000, after 748 keys, one of 4 after 20000: two of eight warps 86, 40, 27; three of
+// four 77, 32, 27; four of four 78, 28, 36.
+constexpr int WARPS = 4, THREADS = WARPS * 32, SMS_MOST = 160, CTAS_MOST = 4;
 
 struct AttArgs : Step, Out {
   const void* q; long long q_ts; int q_hs;
@@ -46,14 +46,13 @@ struct AttArgs : Step, Out {
 };
 
 template <int D, int TR> struct Smem {
-  static constexpr int WARPS = Shape<TR>::WARPS, GRID_MOST = Shape<TR>::GRID_MOST;
   static constexpr int ROW = D / 2, CODES = UNIT * ROW, STAGES = 2;
   static constexpr int WORDS = 2 * CODES, STAGE = WORDS + 2 * UNIT * 2;   // keys, values, words of either
   static constexpr int FACTORS = 16 * 16 * 2 + 8 * 16;                    // what the words of a unit's keys come to, in the order of the products
   static constexpr int WARP = STAGES * STAGE + FACTORS;
   static constexpr int LD = D + 8;                                      // floats of a row of sums on its way between warps
   // units, or (at a segment's end) sums on their way between warps, or a factor for every part of an item
-  static constexpr size_t RING = (size_t)WARPS * WARP, SUMS = (size_t)WARPS * TR * LD * 4, PARTS = (size_t)(GRID_MOST + 1) * TR * 4;
+  static constexpr size_t RING = (size_t)WARPS * WARP, SUMS = (size_t)WARPS * TR * LD * 4, PARTS = (size_t)(SMS_MOST * CTAS_MOST + 1) * TR * 4;
   static constexpr size_t ROOM = RING > SUMS ? (RING > PARTS ? RING : PARTS) : SUMS > PARTS ? SUMS : PARTS;
   static constexpr size_t Q = TR * D * 2;
   static constexpr size_t ML = (size_t)WARPS * TR * 2 * 4;
@@ -133,12 +132,11 @@ __device__ __noinline__ void fetch_parts(const uint8_t* k, const uint8_t* v, con
   }
 }
 
-template <bool BF16, int D, int TR>
-__global__ void __launch_bounds__(Shape<TR>::THREADS, Shape<TR>::CTAS) kv4_attention_kernel(const AttArgs a) {
+template <bool BF16, int D, int TR, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttArgs a) {
   using T = typename Elem16<BF16>::T;
   using S = Smem<D, TR>;
   constexpr bool FEW = TR == 8;
-  constexpr int WARPS = Shape<TR>::WARPS, THREADS = Shape<TR>::THREADS;
   constexpr int NT = D / (FEW ? 16 : 8), W = D / 32, KT = UNIT / 8, QT = UNIT / 16;   // column tiles of the value product, words that a lane has of a key, key tiles
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Shared<WARPS> s_sh;
@@ -155,7 +153,7 @@ __global__ void __launch_bounds__(Shape<TR>::THREADS, Shape<TR>::CTAS) kv4_atten
   unsigned long long work;
   {
     Stretch stretch;
-    if (!find_stretch<WARPS, Shape<TR>::GRID_MOST, TR>(a, s_sh, work, stretch)) return;
+    if (!find_stretch<WARPS, SMS_MOST * CTAS, TR>(a, s_sh, work, stretch)) return;
     if (tid == 0) s_stretch = stretch;
   }
 
@@ -549,9 +547,8 @@ __global__ void __launch_bounds__(Shape<TR>::THREADS, Shape<TR>::CTAS) kv4_atten
 using namespace qspec;
 using namespace qspec::kv4;
 
-template <int TR> int att_grid() { return max(sm_count(), 1) * Shape<TR>::CTAS; }
 
-extern "C" size_t qspec_kv4_attention_workspace_bytes(void) { return 4096 + std::max((size_t)att_grid<8>() * PART<128, 8>, (size_t)att_grid<16>() * PART<128>) * 2 * sizeof(float); }
+extern "C" size_t qspec_kv4_attention_workspace_bytes(void) { return 4096 + (size_t)std::max(sm_count(), 1) * std::max(CTAS_MOST * PART<128, 8>, 3 * PART<128>) * 2 * sizeof(float); }
 
 static int attention(const void* q, long long q_tok_stride, int q_head_stride, const void* k, const void* v, const void* k_word, const void* v_word, const int* table,
                      const int* q_start, const int* kv_len, void* out, long long out_tok_stride, int out_head_stride, int ntok, int requests, int width, int H, int G, int D, int npages,
@@ -573,7 +570,7 @@ static int attention(const void* q, long long q_tok_stride, int q_head_stride, c
                 QSPEC_ERR_INVALID_ARG, "kv4_attention: rows must lie on 16-byte boundaries");
   QSPEC_REQUIRE(workspace && workspace_bytes >= qspec_kv4_attention_workspace_bytes() && ((uintptr_t)workspace & 15) == 0, QSPEC_ERR_WORKSPACE,
                 "kv4_attention: %zu bytes of workspace needed, got %zu", qspec_kv4_attention_workspace_bytes(), workspace_bytes);
-  QSPEC_REQUIRE(sm_count() <= 160, QSPEC_ERR_UNSUPPORTED, "kv4_attention: %d SMs", sm_count());
+  QSPEC_REQUIRE(sm_count() <= SMS_MOST, QSPEC_ERR_UNSUPPORTED, "kv4_attention: %d SMs", sm_count());
   // Requests with many rows may go to the prompt form (to_prompt_form()), in a launch of its own in front; none do if the call's rows are too few for a third of
   // the SMs (always: for tests). Both forms measured, 32 / 8 heads of 128, us of the prompt form (of the other):
   //   1 request, 1000 keys in front of it   32 tokens 37 (19)   128: 37 (23)   160: 38 (39)   256: 38 (51)   1024: 71 (204)
@@ -594,17 +591,18 @@ static int attention(const void* q, long long q_tok_stride, int q_head_stride, c
   const AttArgs a{{table, q_start, kv_len, requests, width, npages, page_shift(page_tokens), ntok, G, rep, prompts ? share : 0u},
                   {out, out_tok_stride, out_head_stride, (int*)workspace, (float*)((char*)workspace + 4096)}, q, q_tok_stride, q_head_stride, (const uint8_t*)k, (const uint8_t*)v,
                   (const uint16_t*)k_word, (const uint16_t*)v_word, scale * 1.4426950408889634f};
-  auto run = [&](auto kern, int grid, int threads, size_t smem, SmemLimit& limit) -> int {
+  auto run = [&](auto kern, int ctas, size_t smem, SmemLimit& limit) -> int {
     QSPEC_CUDA(limit.raise(kern, smem));
-    QSPEC_CUDA(launch_pdl(kern, dim3(grid), dim3(threads), smem, (cudaStream_t)stream, a));
+    QSPEC_CUDA(launch_pdl(kern, dim3(std::max(sm_count(), 1) * ctas), dim3(THREADS), smem, (cudaStream_t)stream, a));
     QSPEC_CHECK_LAUNCH(1);
     return QSPEC_OK;
   };
-  static SmemLimit limits[8];
-  const bool few = (long long)max_tokens * rep <= 8;
+  static SmemLimit limits[12];
+  const bool few = (long long)max_tokens * rep <= 8, many = (long long)requests * G > 3ll * sm_count();
 #define QSPEC_KV4_ATTENTION(BF, D, I)                                                                                                   \
-  (few ? run(kv4_attention_kernel<BF, D, 8>, att_grid<8>(), Shape<8>::THREADS, Smem<D, 8>::TOTAL, limits[I])                            \
-       : run(kv4_attention_kernel<BF, D, 16>, att_grid<16>(), Shape<16>::THREADS, Smem<D, 16>::TOTAL, limits[4 + I]))
+  (!few   ? run(kv4_attention_kernel<BF, D, 16, 3>, 3, Smem<D, 16>::TOTAL, limits[I])                                                   \
+   : many ? run(kv4_attention_kernel<BF, D, 8, 4>, 4, Smem<D, 8>::TOTAL, limits[4 + I])                                                 \
+          : run(kv4_attention_kernel<BF, D, 8, 3>, 3, Smem<D, 8>::TOTAL, limits[8 + I]))
   if (dtype == QSPEC_DTYPE_F16) return D == 128 ? QSPEC_KV4_ATTENTION(false, 128, 0) : QSPEC_KV4_ATTENTION(false, 64, 1);
   return D == 128 ? QSPEC_KV4_ATTENTION(true, 128, 2) : QSPEC_KV4_ATTENTION(true, 64, 3);
 #undef QSPEC_KV4_ATTENTION

@@ -707,3 +707,9 @@ def test_eights_are_the_same_every_time_in_a_graph_and_over_their_own_queries():
     # a workspace serves calls of either kind, one after the other
     sixteen = check_attention(case, 128, max_tokens=5, workspace=work)
     assert torch.equal(check_attention(case, 128, max_tokens=1, workspace=work), want) and torch.equal(check_attention(case, 128, max_tokens=5, workspace=work), sixteen)
+
+
+@pytest.mark.parametrize("R,lens", [(1, 5000), (54, 700), (55, 700), (56, 700), (75, 90), (130, 33)])
+def test_eights_around_where_there_are_more_ctas(R, lens):
+    """With eight heads of keys the rule's limit is at three requests for eight SMs."""
+    check_attention(make_attention(33, [lens - i % 7 for i in range(R)], [1] * R, 32, 8, 128, 64, torch.float16), 128, max_tokens=1)
