@@ -488,12 +488,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
             }
           } else {
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const uint32_t u = w[t], v = w[t] >> 8;
-            mma16816(o[4 * c + 2 * t], pa[q], half_add(and_or(u, low4, magic), zero[0]), half_add(and_or(v, low4, magic), zero[1]));
-            mma16816(o[4 * c + 2 * t + 1], pa[q], half_fma(and_or(u, high4, magic), 0x2c002c00u, zero[2]),
-                     half_fma(and_or(v, high4, magic), 0x2c002c00u, zero[3]));   // (times 1 / 16)
-          }
+            for (int t = 0; t < 4; ++t) {
+              const uint32_t u = w[t], v = w[t] >> 8;
+              mma16816(o[4 * c + 2 * t], pa[q], half_add(and_or(u, low4, magic), zero[0]), half_add(and_or(v, low4, magic), zero[1]));
+              mma16816(o[4 * c + 2 * t + 1], pa[q], half_fma(and_or(u, high4, magic), 0x2c002c00u, zero[2]),
+                       half_fma(and_or(v, high4, magic), 0x2c002c00u, zero[3]));   // (times 1 / 16)
+            }
           }
         }
       }
