@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
     if (a.top && (b == check || b + 1 == batches)) {
       // ---- the best so far: of those of before, which are the first keys, and of the candidates
       __syncthreads();
+      // What is counted from here on is counted elsewhere, whatever this says: there is no barrier between a warp's look at it and another warp's next batch.
       const int hits = s_hits[turn];
       if (hits > HITS) lost = true;                         // (the same for all)
       if (hits && !lost) {
@@ -310,16 +311,16 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
             if (larger < a.top) s_best[larger] = key;
           }
           __syncthreads();
-          // (the next to look at these come behind a barrier; hits are counted elsewhere from here on)
+          // (the next to look at these come behind a barrier)
           best = min(count, a.top);
           if (tid < best) s_key[tid] = s_best[tid];
           if (tid == 0) { s_count = best; s_hits[turn] = 0; }
-          turn ^= 1;
           if (best == a.top) reach = value_of(s_best[best - 1]);
         } else {
           lost = true;
         }
       }
+      turn ^= 1;                                            // (the other count is zero: nothing has been counted there since it was set to that, a barrier ago)
       if (lost) reach = INFINITY;                           // all of them are looked for at the end
       first = false;
       check = (a.top > FEW_TOP ? 4 : 8) * (b + 1) - 1;

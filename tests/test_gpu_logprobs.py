@@ -194,3 +194,25 @@ def test_best_of_long_rows_that_a_cta_has_to_itself(shape, top, dtype):
         p = torch.log_softmax(logits[row].double(), -1)[best]
         assert ((tlp[row::2] - p).abs() <= p.abs() * 2.0 ** -22 + (V / 2048 + 16) * 2.0 ** -24 + 2.0 ** -21 + 40 * 2.0 ** -23).all()
         assert torch.equal(rank[row::2], (logits[row] > logits[row, tokens[row::2]][:, None]).sum(-1) + 1)
+
+
+@pytest.mark.parametrize("dtype,V", [(F16, 128256), (BF16, 90007), (F32, 151643)])
+@pytest.mark.parametrize("top", [5, 9, 20, 32])
+def test_best_of_rows_whose_larger_values_come_after_batches_without_any(top, dtype, V):
+    """A CTA has a row to itself and walks it in batches of 16 KB. The best so far are all in the first batch, batches 1 to 3 have none (so that a look at the candidates finds nothing), larger
+    ones come from batch 4 on, in some batches and not in others."""
+    rows, batch = 600, 16384 // torch.empty(0, dtype=dtype).element_size()
+    at = torch.arange(V, device="cuda")
+    x = torch.rand(rows, V, generator=gen(13), device="cuda")
+    x[:, :batch:97] += 4
+    for b in range(4, V // batch):                            # odd rows: three in each of them; even ones: in every third
+        x[1::2, b * batch + 500:b * batch + 503] = 8 + b / 4
+        if b % 3 == 0:
+            x[::2, b * batch + batch - 40:b * batch + batch - 3] = 6 + b / 8
+    x[:, (at % 5000 == 4999) & (at > 10 * batch)] += 7.5
+    logits = x.to(dtype)
+    best = logits.sort(dim=-1, descending=True, stable=True).indices[:, :top]
+    for _ in range(5):
+        lp, h, rank, tlp, tt = call(logits, best[:, 1].contiguous(), top)
+        assert torch.equal(tt, best)
+        assert torch.equal(rank, (logits > logits.gather(1, best[:, 1:2])).sum(-1) + 1)
