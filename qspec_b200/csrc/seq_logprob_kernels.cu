@@ -4,7 +4,8 @@
 // tokens, equal ones by the lower token.
 //
 // What bounds it is reading the row, once, and the exponentials. One CTA, or a cluster of up to eight, takes a row; a CTA walks its span in batches of 1024 vectors of 16 bytes, the
-// next batch's loads under way. The first batch's maximum is where exponents are counted from; only if a value is 2^60 above it the sums are multiplied again. Candidates for
+// next batch's loads under way. Exponents are counted from the first batch's maximum, and by a thread that sees a larger value (they are few) from that one on, its sums multiplied again: no
+// exponent is above zero, the largest value's weight is 1 exactly, and a likely token's log probability is no difference of large numbers (nor above zero). Candidates for
 // the best are, of the first batch, the values that reach the smallest of as many groups' maxima as are asked for, or more (at least that many do, and hardly more than some
 // hundred), and later on those above the worst of the best so far, which is brought up to date whenever four (or, of up to eight, eight) times as much has been
 // seen: a few at a time. Where there are more than there
@@ -22,7 +23,6 @@ namespace logprob {
 constexpr int THREADS = 256, WARPS = THREADS / 32, MOST_TOP = 32, EACH = 4;   // EACH: vectors of a thread in a batch
 constexpr int GROUPS = 128, GROUP = THREADS / GROUPS, HITS = 256, CANDIDATES = 512;   // groups of neighbouring threads; vectors with candidates, candidates in them
 constexpr int FEW_TOP = 8;                        // alternatives that are few: us of 256 rows of 128256 with 5, taken like more of them 28.8, so 26.8; 4 rows 9.5, 8.3
-constexpr float AHEAD = 60.f;                     // a value 2^AHEAD above the reference moves it
 typedef unsigned long long u64;
 
 struct Args {
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
   float ref = -INFINITY, reach = INFINITY;                  // what exponents are counted from; what a candidate has to reach (of the first batch) or to exceed
   bool none = true;                                         // nothing but minus infinity so far: there is nothing to count from
   float limit = -INFINITY;                                  // what a value that is looked at more closely reaches
-  auto set_limit = [&]() { limit = none ? -INFINITY : fminf(reach, ref + AHEAD / a.c); };
+  auto set_limit = [&]() { limit = none ? -INFINITY : fminf(reach, ref); };
   u64 S2 = 0, U2 = 0;
   // (the candidates of eight batches for FEW_TOP are few)
   int above = 0, best = 0, check = a.top > FEW_TOP ? 0 : 7, turn = 0;             // check: the batch behind which the best are brought up to date; turn: which count of hits is in use
@@ -243,9 +243,9 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
       set_limit();
     }
     const float most = max_nan(max_nan(big[0], big[1]), max_nan(big[2], big[3]));
-    if (!(most < limit)) {                                  // seldom: candidates, a value far above all before it, no numbers. (Code that is short, and there once: it is cold)
+    if (!(most < limit)) {                                  // seldom: candidates, a value above all before it, no numbers. (Code that is short, and there once: it is cold)
       odd |= most != most;
-      if (none ? most > -INFINITY : most > ref + AHEAD / a.c) {
+      if (none ? most > -INFINITY : most > ref) {
         const float d = fmaxf((ref - most) * a.c, -16384.f), f = none ? 0.f : ex2(d);
         const float2 S = unpack_f2(S2), U = unpack_f2(U2);
         U2 = pack_f2(fmaf(S.x, d, U.x) * f, fmaf(S.y, d, U.y) * f);
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 4) token_logprobs_kernel(const Args a
     if (tid == 0) {
       if (a.logprobs) a.logprobs[row] = token < 0 ? 0.f : there ? logprob(given) : lse != lse ? NAN : -INFINITY;
       if (a.ranks) a.ranks[row] = there ? 1 + above : 0;
-      if (a.entropy) a.entropy[row] = nothing ? 0.f : lse != lse ? NAN : fmaxf((lse - U / S) * ln2, 0.f);
+      if (a.entropy) a.entropy[row] = nothing ? 0.f : lse != lse ? NAN : (lse - U / S) * ln2;
     }
     if (a.top) {
       int all = 0, mine = -1;                               // of the slices' best, one behind the other: how many, and which slice's this thread's is

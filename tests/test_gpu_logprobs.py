@@ -216,3 +216,31 @@ def test_best_of_rows_whose_larger_values_come_after_batches_without_any(top, dt
         lp, h, rank, tlp, tt = call(logits, best[:, 1].contiguous(), top)
         assert torch.equal(tt, best)
         assert torch.equal(rank, (logits > logits.gather(1, best[:, 1:2])).sum(-1) + 1)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows", [3, 600])
+@pytest.mark.parametrize("temperature", [1.0, 0.7])
+@pytest.mark.parametrize("gap", [8, 20, 30])
+def test_of_rows_that_are_sure_of_a_token_wherever_it_stands(gap, temperature, rows, dtype):
+    """The best token is `gap` nats above the next ones, at the begin, in the middle, at the end of a row or anywhere. Its log probability is - ln S, S = 1 + the others' weights, of which the
+    sum is R: never above zero. Off by R times the weights' errors (2^-22 of ex2.approx, and a rounding each of the difference, of c and of the product, at exponents up to 2 gap / T * 1.4427 where there is
+    weight: 2^-17 at most), by the logarithm's last place (2^-22 of itself), and by sums: 1 and more plus t, rounded to the nearest, is off by 2^-24 at most (half a last place) and by t at
+    most (1 itself is a float, and no sum rounds past it). The terms t of the thread and pair that the 1 is in are V / 256 / 2 values at most and then 21 joins with other threads and spans, and
+    together no more than R: the smaller of (V / 512 + 21) 2^-24 and R. The entropy, a sum of positive terms: by its own 2^-17 and what the logarithm is off by, and U by its roundings, 2^-24 of U each."""
+    V = 60007
+    logits = (torch.rand(rows, V, generator=gen(17), device="cuda") * 2 - 2).to(dtype)
+    at = torch.randint(0, V, (rows,), generator=gen(18), device="cuda")
+    at[:3] = torch.tensor([0, V // 2, V - 1], device="cuda")
+    logits.scatter_(1, at[:, None], torch.full_like(logits[:, :1], gap * temperature))
+    lp, h, rank, tlp, tt = call(logits, at, 5, temperature)
+    p = torch.log_softmax(logits.double() / temperature, -1)
+    top = p.gather(1, at[:, None])[:, 0]
+    R = torch.expm1(-top)
+    sums = torch.clamp(R, max=(V / 512 + 21) * 2.0 ** -24)
+    bound = R * 2.0 ** -17 + top.abs() * 2.0 ** -22 + sums
+    assert (lp <= 0).all() and (tlp <= 0).all() and (h >= 0).all() and (rank == 1).all()
+    assert ((lp - top).abs() <= bound).all(), float(((lp - top).abs() / bound).max())
+    assert torch.equal(tlp[:, 0], lp) and torch.equal(tt[:, 0], at)
+    entropy = -torch.special.xlogy(p.exp(), p.exp()).sum(-1)
+    assert ((h - entropy).abs() <= entropy * (2.0 ** -17 + (V / 512 + 21) * 2.0 ** -24) + 2 * bound).all(), float((h - entropy).abs().max())
