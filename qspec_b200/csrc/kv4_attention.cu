@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
     float o[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
-    float m[2] = {NONE, NONE};
+    float m[2] = {NONE, NONE};                              // what exponents are counted from
     uint64_t l2[2] = {0ull, 0ull};                          // sums of weights / v
 
     for (int here = cur.u + warp; here < end; here += WARPS) {
@@ -423,16 +423,19 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
 #pragma unroll
           for (int e = 0; e < 2; ++e) mx[e] = fmaxf(fmaxf(mx[e], s[n][2 * e]), s[n][2 * e + 1]);
       }
-      // The reference follows the maximum only where it has fallen behind: sums are seldom multiplied again.
-      if (__any_sync(0xffffffffu, mx[0] > m[0] + GROWTH_LOG2 || mx[1] > m[1] + GROWTH_LOG2)) {   // (of a row that had seen nothing, more than minus infinity)
+      // The reference follows the maximum only where that is 2^TOP_LOG2 and more above it: sums are seldom multiplied again. It is WEIGHT_LOG2 below the maximum, rounded up: far from zero
+      // that is less, and weights that are counted from what it is, and the comparison with their own difference, stay finite.
+      constexpr float TOP_LOG2 = WEIGHT_LOG2 + GROWTH_LOG2;
+      if (__any_sync(0xffffffffu, mx[0] - m[0] > TOP_LOG2 || mx[1] - m[1] > TOP_LOG2)) {   // (of a row that had seen nothing: infinite, or nothing again and no number)
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int x = FEW ? 4 : 1; x < (FEW ? 32 : 4); x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-          const bool grown = mx[e] > m[e] + GROWTH_LOG2;
-          f[e] = grown && m[e] != NONE ? exp2_fast(m[e] - mx[e]) : 1.f;   // (a row that had seen nothing has sums of zero)
-          if (grown) m[e] = mx[e];
+          const bool grown = mx[e] - m[e] > TOP_LOG2;
+          const float to = __fadd_ru(mx[e], -WEIGHT_LOG2);
+          f[e] = grown && m[e] != NONE ? exp2_fast(m[e] - to) : 1.f;   // (a row that had seen nothing has sums of zero)
+          if (grown) m[e] = to;
           if (!FEW) l2[e] = mul2(l2[e], two(f[e], f[e]));
         }
         if (FEW) l2[0] = mul2(l2[0], two(f[0], f[1]));
@@ -441,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
       }
       // ---- weights
       uint32_t pa[QT][TR / 4];
-      const float ref[2] = {m[0] == NONE ? 0.f : WEIGHT_LOG2 - m[0], m[1] == NONE ? 0.f : WEIGHT_LOG2 - m[1]};
+      const float ref[2] = {m[0] == NONE ? 0.f : -m[0], m[1] == NONE ? 0.f : -m[1]};
       if constexpr (FEW) {
 #pragma unroll
         for (int n = 0; n < KT; ++n) {

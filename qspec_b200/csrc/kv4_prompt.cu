@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
       const float k = fmaxf(rowf * __uint_as_float((uint32_t)min(max(f.ke - TOP, 1), 254) << 23), 1.17549435e-38f), lv = (float)(f.ve - 127 - TOP);
       const float iv = __uint_as_float((uint32_t)min(max(127 + 127 + TOP - f.ve, 1), 254) << 23) * WEIGHT_UNIT;
       mn = fmaf(mn, k, lv);                                 // (minus infinity stays that)
-      const bool grown = mn > m + GROWTH_LOG2;              // (of a row that had seen nothing: more than minus infinity)
+      const bool grown = mn - m > GROWTH_LOG2;              // (of a row that had seen nothing: infinite, or nothing again and no number; far from zero m + 6 is more than that)
       if (__any_sync(0xffffffffu, grown)) {
         const float up = grown ? ex2(m - mn) : 1.f;         // 0 for a row that had seen nothing; other rows of the warp keep theirs
         l *= up;

@@ -288,8 +288,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv8_attention_kernel(const AttA
       for (int e = 0; e < 2; ++e) {
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-        // The reference follows the maximum only where it has fallen behind: sums are seldom multiplied again.
-        grown[e] = mx[e] > m[e] + GROWTH_LOG2 || (m[e] == NONE && mx[e] > NONE);
+        // The reference follows the maximum only where it has fallen behind: sums are seldom multiplied again. (Of a row that had seen nothing: infinite, or nothing again and no number. Far
+        // from zero m + 6 is more than that.)
+        grown[e] = mx[e] - m[e] > GROWTH_LOG2;
       }
       if (__any_sync(0xffffffffu, (grown[0] && m[0] != NONE) || (grown[1] && m[1] != NONE))) {
         const float f[2] = {grown[0] ? exp2_fast(m[0] - mx[0]) : 1.f, grown[1] ? exp2_fast(m[1] - mx[1]) : 1.f};

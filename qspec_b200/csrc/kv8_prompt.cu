@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
           taken = fmaxf(taken, fabsf(at));
         }
       }
-      const bool grown = mn > m + GROWTH_LOG2 || (m == NONE && mn > m);
+      const bool grown = mn - m > GROWTH_LOG2;              // (of a row that had seen nothing: infinite, or nothing again and no number; far from zero m + 6 is more than that)
       const float up = grown ? ex2(m - mn) : 1.f;         // 0 for a row that had seen nothing; other rows of the warp keep theirs
       l *= up;
       if (i && __any_sync(0xffffffffu, grown && m != NONE)) {   // (the scores are there: the stream's product before them is over)
