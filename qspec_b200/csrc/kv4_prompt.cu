@@ -8,7 +8,8 @@
 //   * codes: four warps bring a block's keys and values from global memory, make them float16 and store them as the tensor cores want them: the cache is read once, in 4
 //     bits, and is never anywhere in 16. A code in the upper bits of the mantissa behind an exponent of 4 is 16 + c; (16 + c) s - (16 + z) s is one multiply-add of two
 //     values, and exact: s has five bits, 16 + z has five, (c - z) s nine. s is the row's scale over the block's largest power of two, times 2^10: exact
-//     down to 2^-30 of the largest. Eight codes of a word come out as 0 4 1 5 2 6 3 7: the order of the sum over a head's columns is free (queries are put in the same), and
+//     down to 2^-30 of the largest. Where a block's keys' scales are further apart, or its values' more than 2^8 (of keys that a row does not see, or that count for nothing, it must not
+//     notice that), s is 2^10, and the softmax takes each key's scales from shared memory (wide_block()). Eight codes of a word come out as 0 4 1 5 2 6 3 7: the order of the sum over a head's columns is free (queries are put in the same), and
 //     columns of the result are put right on their way out.
 //   * S = Q K^T, accumulator [128 x 128] float32 in tensor memory, one for each stream.
 //   * products: a thread a stream issues them: scores once the keys are there and the stream's product before them is over (its weights lie where the scores go), the product of
@@ -60,7 +61,14 @@ struct alignas(16) Block {                                            // what th
   uint16_t kw[128], vw[128];                              // words of its keys; a key that makes rows no numbers has the scale NaN in kw and zero in vw
   long long at[8];                                        // of each 16 of its keys: the row of the cache where their codes begin, -1: nowhere
   int ke, ve;                                             // the largest exponent (of float32, biased) of the keys' scales, of the values'
+  alignas(16) float k;                                    // for the softmax, 16 bytes together: the keys' power of two / 2^TOP, log2 of the values' / 2^TOP, and what weights are divided by that with
+  float lv, iv;
+  int wide;                                               // scales so far apart that codes stand in the operands without them; then, of each key:
+  float ks[128], lvs[128], ivs[128];                      // its scale / 2^TOP (no number: rows that see it are none either), log2 of its value's / 2^TOP, and what weights are divided by that with
 };
+// How far apart exponents of a block's scales may be. Keys': what is exact beside each other in an operand (five bits from 2^TOP down to float16's last, 2^-24). Values': their largest goes into the
+// exponents of all of the block's weights, and the reference with it; where a key that counts for nothing has it, later blocks' weights are that much closer to float16's end (2^-26 of the largest at 8).
+constexpr int APART_K = 30, APART_V = 8;
 constexpr int TOP = 10;                                   // scales over the block's largest power of two, times 2^TOP
 constexpr uint32_t NO_KEY = 0xffffu, NO_VALUE = 0u;       // words of a key that makes the rows that see it no numbers
 
@@ -73,6 +81,42 @@ __device__ __forceinline__ void ld16(uint32_t addr, uint32_t* r) {
 __device__ __forceinline__ void landed32(uint32_t (&r)[32]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) landed8(r + i * 8);
+}
+
+// A row's scores of a block whose scales are too far apart for the operands: made exponents, each by its own key's scales, and put back where they were. Gives the sum of weights / v, with
+// the reference that the row will have (m: that it has), of the block's keys up to `limit`. (Out of line: it is
+// seldom called. With every block like that 2000 tokens after 1000 take 212 us, so 118.)
+__device__ __noinline__ float wide_block(uint32_t st, const Block& f, float rowf, float m, int limit) {
+  float mn = NONE;
+#pragma unroll 1
+  for (int c0 = 0; c0 < 128; c0 += 32) {
+    uint32_t x[32];
+    ld32(st + c0, x);
+    wait_ld();
+    landed32(x);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const float k = f.ks[c0 + j] * rowf, y = fmaf(__uint_as_float(x[j]), k < 1.17549435e-38f ? 1.17549435e-38f : k, f.lvs[c0 + j]);
+      if (c0 + j <= limit) mn = fmaxf(mn, y);
+      x[j] = __float_as_uint(y);
+    }
+    st16(st + c0, x);
+    st16(st + c0 + 16, x + 16);
+  }
+  wait_st();
+  const float top = mn - m > GROWTH_LOG2 ? mn : m, mu = top == NONE ? 0.f : top;
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c0 = 0; c0 < 128; c0 += 32) {
+    uint32_t x[32];
+    ld32(st + c0, x);
+    wait_ld();
+    landed32(x);
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (c0 + j <= limit) sum = fmaf(ex2(__uint_as_float(x[j]) - mu + WEIGHT_LOG2), f.ivs[c0 + j], sum);
+  }
+  return sum;
 }
 
 template <bool BF16, int D>
@@ -225,37 +269,79 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
       uint4 w = make_uint4(0u, 0u, 0u, 0u);
       if (there) w = __ldg(reinterpret_cast<const uint4*>((side ? a.vw : a.kw) + row));
       page = page_of(n + 1);
-      if (n >= FACS) ok = bar_wait(smem_addr(&b_facfree[slot]), (uint32_t)((n / FACS) - 1) & 1u, &s_fail);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
       // scales that are infinite or no number: exponent 255. (Rows behind the last key have neither say nor sight.)
       uint32_t x[4] = {w.x, w.y, w.z, w.w};
       const int have = min(max(keys - key, 0), 8);
-      uint32_t bad = 0u, most = 0u;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t ex = (x[e >> 1] >> (e & 1 ? 24 : 8)) & 0xffu;
-        if (e < have) {
-          if (ex == 255u) bad |= 1u << e;
-          else most = max(most, ex);
-        }
-      }
-      if (!there) bad = (1u << have) - 1u;                  // (a page that there is not)
-      bad |= __shfl_xor_sync(0xffffffffu, bad, 16);         // of the key's word, or of the value's
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-      const uint32_t no = side ? NO_VALUE : NO_KEY;
+      uint32_t most = 0u, least = 0x00ff00ffu;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (bad >> (2 * e) & 1u) x[e] = (x[e] & 0xffff0000u) | no;
-        if (bad >> (2 * e + 1) & 1u) x[e] = (x[e] & 0xffffu) | no << 16;
-        if (2 * e >= have) x[e] = 0u;                       // (values that are no numbers would make a weight of zero one)
-        else if (2 * e + 1 >= have) x[e] &= 0xffffu;
+        most = __vmaxu2(most, x[e] >> 8 & 0x00ff00ffu);
+        least = __vminu2(least, x[e] >> 8 & 0x00ff00ffu);
       }
+      most = max(most & 0xffffu, most >> 16);
+      least = min(least & 0xffffu, least >> 16);
+      if (!__all_sync(0xffffffffu, there && have == 8 && most < 255u)) {   // (seldom: one by one)
+        uint32_t bad = 0u;
+        most = 0u;
+        least = 255u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t ex = (x[e >> 1] >> (e & 1 ? 24 : 8)) & 0xffu;
+          if (there && e < have) {
+            if (ex == 255u) {
+              bad |= 1u << e;
+            } else {
+              most = max(most, ex);
+              least = min(least, ex);
+            }
+          }
+        }
+        if (!there) bad = (1u << have) - 1u;                // (a page that there is not)
+        bad |= __shfl_xor_sync(0xffffffffu, bad, 16);       // of the key's word, or of the value's
+        const uint32_t no = side ? NO_VALUE : NO_KEY;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (bad >> (2 * e) & 1u) x[e] = (x[e] & 0xffff0000u) | no;
+          if (bad >> (2 * e + 1) & 1u) x[e] = (x[e] & 0xffffu) | no << 16;
+          if (2 * e >= have) x[e] = 0u;                     // (values that are no numbers would make a weight of zero one)
+          else if (2 * e + 1 >= have) x[e] &= 0xffffu;
+        }
+      }
+      uint32_t ends = (255u - max(least, 27u)) << 16 | max(most, 27u);   // (the larger of either half; 27: 2^-100, and what is below that)
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) ends = __vmaxu2(ends, __shfl_xor_sync(0xffffffffu, ends, o));
+      most = ends & 0xffffu;
+      const bool wide = __any_sync(0xffffffffu, (int)(most + (ends >> 16)) > 255 + (side ? APART_V : APART_K));
+      // (what the others wait for begins here: nothing is left but stores)
+      if (n >= FACS) ok = bar_wait(smem_addr(&b_facfree[slot]), (uint32_t)((n / FACS) - 1) & 1u, &s_fail);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       Block& f = s_block[slot];
       *reinterpret_cast<uint4*>((side ? f.vw : f.kw) + part) = make_uint4(x[0], x[1], x[2], x[3]);
       if (!side && !(lane & 1)) f.at[lane >> 1] = row;
-      if ((lane & 15) == 0) (side ? f.ve : f.ke) = max((int)most, 27);   // (2^-100)
+      if (lane == 0) {
+        f.ke = (int)most;
+        f.k = __uint_as_float((uint32_t)min(max((int)most - TOP, 1), 254) << 23);
+        f.wide = wide;
+      }
+      if (lane == 16) {
+        f.ve = (int)most;
+        f.lv = wide ? 0.f : (float)((int)most - 127 - TOP);
+        f.iv = wide ? 0.f : __uint_as_float((uint32_t)min(max(127 + 127 + TOP - (int)most, 1), 254) << 23) * WEIGHT_UNIT;
+      }
+      if (__builtin_expect(wide, 0)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float scale = word_scale(x[e >> 1] >> (e & 1 ? 16 : 0));
+          if (side) {
+            const float v = fmaxf(scale, 7.888609052210118e-31f);
+            f.lvs[part + e] = __log2f(v) - TOP;
+            f.ivs[part + e] = __fdividef(WEIGHT_UNIT * (1 << TOP) * 5.9604644775390625e-8f, v * 5.9604644775390625e-8f);   // (2^-24: a divisor above 2^126 would give zero)
+          } else {
+            f.ks[part + e] = scale * (1.f / (1 << TOP));
+          }
+        }
+      }
       __syncwarp();
       if (lane == 0) bar_arrive(smem_addr(&b_fac[slot]));
     }
@@ -325,12 +411,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
         if (row < have && at >= 0) next[i] = __ldg(reinterpret_cast<const uint4*>(codes + (at + (row & 15)) * (D / 2)));
       }
     };
-    auto store = [&](const uint4 (&w)[STEPS], uint32_t dst, const uint16_t* words, int ex) {
+    auto store = [&](const uint4 (&w)[STEPS], uint32_t dst, const uint16_t* words, int ex, bool wide) {
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
         const int row = i * ROWS + row0;
         const uint32_t word = words[row];
-        const float s = word_scale(word) * __uint_as_float((uint32_t)min(max(127 + 127 + TOP - ex, 1), 254) << 23);   // (over the block's largest power of two)
+        const float s = wide ? (float)(1 << TOP) : word_scale(word) * __uint_as_float((uint32_t)min(max(127 + 127 + TOP - ex, 1), 254) << 23);   // (over the block's largest power of two)
         const __half2 scale = __float2half2_rn(s), zero = __float2half2_rn(-(16.f + (float)(word & 15u)) * s);
         const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
         const uint32_t at = dst + part + row * 128;
@@ -369,7 +455,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const Block& f = s_block[n % FACS];
-      store(here, (side ? vbuf : kbuf) + stage * OP, side ? f.vw : f.kw, side ? f.ve : f.ke);
+      store(here, (side ? vbuf : kbuf) + stage * OP, side ? f.vw : f.kw, side ? f.ve : f.ke, f.wide);
       if (lane == 0) {
         bar_arrive(smem_addr(side ? &b_vfull[stage] : &b_kfull[stage]));
         if (side) bar_arrive(smem_addr(&b_facfree[n % FACS]));
@@ -445,7 +531,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
       const int n = both ? i : 2 * i + z, j0 = n * 128;
       const uint32_t turn = (uint32_t)i & 1u;
       const bool plain = __all_sync(0xffffffffu, !row_in || j0 + 127 <= limit);   // (rows that stand for no token are never stored)
-      ok = bar_wait(smem_addr(&b_fac[n % FACS]), (uint32_t)(n / FACS) & 1u, &s_fail) && bar_wait(smem_addr(&b_s[z]), turn, &s_fail);
+      ok = bar_wait(smem_addr(&b_fac[n % FACS]), (uint32_t)(n / FACS) & 1u, &s_fail);
+      const Block& f = s_block[n % FACS];
+      const float4 factors = *reinterpret_cast<const float4*>(&f.k);
+      const bool wide = __float_as_int(factors.w);
+      ok = ok && bar_wait(smem_addr(&b_s[z]), turn, &s_fail);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
@@ -464,7 +554,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
         }
         return fmaxf(fmaxf(mx, t), __uint_as_float(y[31]));
       };
-      const Block& f = s_block[n % FACS];
+      float own = 0.f;
+      if (__builtin_expect(wide, 0)) own = wide_block(st, f, rowf, m, limit - j0);
       // ---- the largest exponent: of the second half, whose scores are read again, and the first, whose scores stay
       float mn = NONE;
       auto load = [&](int c0) {
@@ -482,8 +573,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
         mn = largest(x + 32, mn);
       }
       // The block's powers of two: what scores are multiplied with (not so small that it would make a hidden key's minus infinity no number), what exponents begin with
-      const float k = fmaxf(rowf * __uint_as_float((uint32_t)min(max(f.ke - TOP, 1), 254) << 23), 1.17549435e-38f), lv = (float)(f.ve - 127 - TOP);
-      const float iv = __uint_as_float((uint32_t)min(max(127 + 127 + TOP - f.ve, 1), 254) << 23) * WEIGHT_UNIT;
+      const float k = wide ? 1.f : fmaxf(rowf * factors.x, 1.17549435e-38f), lv = factors.y, iv = factors.z;
       mn = fmaf(mn, k, lv);                                 // (minus infinity stays that)
       const bool grown = mn - m > GROWTH_LOG2;              // (of a row that had seen nothing: infinite, or nothing again and no number; far from zero m + 6 is more than that)
       if (__any_sync(0xffffffffu, grown)) {
@@ -542,7 +632,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
       if (lane == 0) bar_arrive(smem_addr(&b_facfree[n % FACS]));
       uint32_t a0, a1;
       unpair(add2(sum[0], sum[1]), a0, a1);
-      l = fmaf(__uint_as_float(a0) + __uint_as_float(a1), iv, l);
+      l = fmaf(__uint_as_float(a0) + __uint_as_float(a1), iv, l) + own;
     }
     if (both && z == 0)                                   // (blocks that tile 1 alone sees)
       for (int n = turns; ok && n < blocks; ++n) {

@@ -713,3 +713,85 @@ def test_eights_are_the_same_every_time_in_a_graph_and_over_their_own_queries():
 def test_eights_around_where_there_are_more_ctas(R, lens):
     """With eight heads of keys the rule's limit is at three requests for eight SMs."""
     check_attention(make_attention(33, [lens - i % 7 for i in range(R)], [1] * R, 32, 8, 128, 64, torch.float16), 128, max_tokens=1)
+
+
+# ---- scales of a block of keys that are far apart ------------------------------------------------------------------------------------------
+def rescaled(words, table, at, exponents):
+    """Words of positions `at` of a request's row of the table, with 2^exponents times their scale."""
+    P = words.shape[2]
+    pages, rows = table[at // P].long(), at % P
+    words[pages, :, rows] = ((words[pages, :, rows].to(I32) & 0xffff) + (exponents[:, None] << 8)).to(I16)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("side", ["keys", "values", "both"])
+@pytest.mark.parametrize("by", [20, 29, 31, 45, -45])
+@pytest.mark.parametrize("D,P,dtype", [(128, 32, torch.float16), (64, 16, torch.bfloat16)])
+def test_attention_of_tokens_whose_keys_are_not_the_blocks_largest(form, side, by, D, P, dtype):
+    """Keys 64 .. 127 and 300 .. 399 of a request have scales 2^by times the others': what the tokens in front of them see is exact all the same. (Those behind them see scores that far apart.)"""
+    lens, counts = [160, 500], [150, 450]
+    q, k, v, kw, vw, table, start, lens = make_attention(40, lens, counts, 8, 2, D, P, dtype)
+    for b, ranges in enumerate([[(64, 128)], [(64, 128), (300, 400)]]):
+        for lo, hi in ranges:
+            for words, name in ((kw, "keys"), (vw, "values")):
+                if side in (name, "both"):
+                    rescaled(words, table[b], torch.arange(lo, hi, device="cuda"), torch.full((hi - lo,), by if name == "keys" or dtype == torch.bfloat16 else min(by, 10), device="cuda"))
+    check_attention((q, k, v, kw, vw, table, start, lens), D, form=form)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_over_scales_of_every_size(form, dtype):
+    """Values' scales from 2^-88 to 2^2 and keys' from 2^-60 to 2^2, in any order, rows whose words are zero, and more tokens than keys."""
+    q, k, v, kw, vw, table, start, lens = make_attention(41, [400, 90, 300], [380, 100, 130], 8, 2, 128, 64, dtype)
+    g = gen(41)
+    for b, n in enumerate(lens.tolist()):
+        at = torch.arange(n, device="cuda")
+        rescaled(vw, table[b], at, torch.randint(-88, 3, (n,), generator=g, device="cuda"))
+        rescaled(kw, table[b], at, torch.randint(-60, 3, (n,), generator=g, device="cuda"))
+        some = at[at % 17 == 3]
+        vw[table[b][some // 64].long(), :, some % 64] = 0
+        kw[table[b][some // 64].long(), :, some % 64] = 0
+    out = check_attention((q, k, v, kw, vw, table, start, lens), 128, form=form)
+    assert not out[380:390].any() and out[390:].any()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_shows_broken_words_among_scales_far_apart(form):
+    q, k, v, kw, vw, table, start, lens = make_attention(42, [300, 300], [250, 290], 8, 2, 128, 32, torch.bfloat16)
+    for b in range(2):
+        rescaled(vw, table[b], torch.arange(0, 300, 3, device="cuda"), torch.full((100,), -60, device="cuda"))
+    clean = check_attention((q, k, v, kw, vw, table, start, lens), 128, form=form)
+    kw[int(table[0, 5]), 0, 5] = 0xffa3 - 65536               # position 165, head 0; and position 229 of the other request, head 1
+    vw[int(table[1, 7]), 1, 5] = 0xff03 - 65536
+    out = torch.empty_like(q)
+    attend(form, q, k, v, kw, vw, table, start, lens, out, 128 ** -0.5, ops.kv4_attention_workspace("cuda"))
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    bad[165 - 50:250, :4] = True
+    bad[250 + 229 - 10:, 4:] = True
+    assert out.isnan().all(2).equal(bad) and out.isnan().any(2).equal(bad)
+    assert torch.equal(out[~bad], clean[~bad])
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("by", [6, 9, 15, 20, 25, 29])
+def test_attention_next_to_a_key_that_counts_for_nothing(by, dtype, form):
+    """Values that are all 1, but for one key's, whose scale is 2^by times theirs; its code is the zero point, and its weight 2^-40 of the others'. The first key has as much weight as 1900 others together,
+    2^10.9 times each: so the result is 1. Off by its rounding, 2^-11 of a weight that is a normal float16, 2^-25 of one that is not where the largest weight and value scale are 2^(9 - 8) or more
+    together (half of the sum or more is the first key's: n 2^-26), and float32 sums, 1.5 n / 4 2^-23."""
+    n, G, H, D, P, T = 1900, 1, 4, 64, 64, 40
+    pages = -(-n // P)
+    ones = torch.ones(pages, G, P, device="cuda")
+    k, v = torch.full((pages, G, P, D // 2), 0x88, dtype=U8, device="cuda"), torch.full((pages, G, P, D // 2), 0x99, dtype=U8, device="cuda")
+    kw, vw = words_of(ones, 8 * ones), words_of(ones, 8 * ones)
+    k[0, 0, 0, 0], k[0, 0, 5, 0], v[0, 0, 5] = 0x89, 0x80, 0x88   # scores of 1 and (with half the scale) of -4, a value of nothing
+    kw[0, 0, 5] = int(words_of(torch.tensor(0.5), torch.tensor(8)))
+    vw[0, 0, 5] = int(words_of(torch.tensor(2.0 ** by), torch.tensor(8)))
+    q = torch.zeros(T, H, D, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1.0
+    out = torch.empty_like(q)
+    case = (q, k, v, kw, vw, torch.arange(pages, dtype=I32, device="cuda")[None], i32([0, T]), i32([n]))
+    attend(form, *case, out, 10.9 / math.log2(math.e), ops.kv4_attention_workspace("cuda"), max_tokens=T)
+    bound = torch.finfo(dtype).eps / 2 + 2.0 ** -11 + n * 2.0 ** -26 + 1.5 * n / 4 * 2.0 ** -23
+    assert ((out.double() - 1).abs() <= bound).all(), (float((out.double() - 1).abs().max()), bound)
