@@ -271,12 +271,13 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
     uint32_t stage = 0;
     const uint32_t frag = shared_addr(s_q) + lane * TR;
     auto query = [&](uint32_t (&x)[TR / 4], int step) { if constexpr (FEW) lds64(x, frag + step * 256); else lds128(x, frag + step * 512); };
-    // The rows' powers of two: the tile's largest goes into the keys' factors, what a row is below it (at most 1) stays the row's.
+    // The rows' powers of two: the tile's largest goes into the keys' factors, what a row is below it (at most 1) stays the row's,
+    // with the scores' unit: scores times that first, so that neither leaves float32 where the whole does not.
     float big = s_f[0];
 #pragma unroll
     for (int r = 1; r < TR; ++r) big = fmaxf(big, s_f[r]);
     const int row0 = FEW ? 2 * qj : qi, row1 = FEW ? 2 * qj + 1 : qi + 8;   // this lane's rows of the tile
-    const float own[2] = {s_f[row0] / big, s_f[row1] / big}, factor = big * a.scale2;
+    const float own[2] = {s_f[row0] / big * 16777216.f, s_f[row1] / big * 16777216.f}, factor = big * a.scale2;
     int limit[2];                                           // last visible position of this lane's rows
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -315,11 +316,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
         const bool broken = !(__ballot_sync(0xffffffffu, unit0.there) >> (lane >> 4) & 1u);
         const uint32_t kw = lds16(words + stage * S::STAGE), vw = lds16(words + stage * S::STAGE + UNIT * 2);
         const bool bad = broken || kw >= 0xff00u || vw >= 0xff00u;   // (exponent 255: infinite, or no number)
-        float f = word_scale(kw) * factor * 16777216.f, v = fmaxf(word_scale(vw), 7.888609052210118e-31f);
+        float f = fminf(word_scale(kw) * factor, 3.402823466e38f), v = fmaxf(word_scale(vw), 7.888609052210118e-31f);   // (a score of nothing stays that)
         if (bad) { f = NAN; v = 1.f; }                      // rows that see it are no numbers
         if (key0 + lane >= keys) f = 0.f;
         const uint32_t x[4] = {__float_as_uint(f), __float_as_uint(__uint_as_float(0xcb000000u | (kw & 15u)) + 8388608.f) /* - z */, __float_as_uint(__log2f(v)),
-                               __float_as_uint(__fdividef(WEIGHT_UNIT, v))};
+                               __float_as_uint(__fdividef(WEIGHT_UNIT * 5.9604644775390625e-8f, v * 5.9604644775390625e-8f))};   // (2^-24: a divisor above 2^126 would give zero)
         if constexpr (FEW) {
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(mine), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
         } else {
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
           const float f = __uint_as_float(x[0]), zero = __uint_as_float(x[1]), lv = __uint_as_float(x[2]), iv = __uint_as_float(x[3]);
           float* const y = s[n >> 1] + (n & 1) * 2;
           const uint64_t score = ffma2_rn(two(zero, zero), two(sums[0], sums[1]), two(y[0], y[1]));
-          const float2 r = unpack_f2(ffma2_rn(score, mul2(two(f, f), two(own[0], own[1])), two(lv, lv)));
+          const float2 r = unpack_f2(ffma2_rn(mul2(score, two(own[0], own[1])), two(f, f), two(lv, lv)));
           y[0] = r.x;
           y[1] = r.y;
           iv2[n] = two(iv, iv);
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint64_t score = ffma2_rn(zero, two(sums[2 * e], sums[2 * e]), two(s[n][2 * e], s[n][2 * e + 1]));
-            const float2 r = unpack_f2(ffma2_rn(score, mul2(f, two(own[e], own[e])), lv));
+            const float2 r = unpack_f2(ffma2_rn(mul2(score, two(own[e], own[e])), f, lv));
             s[n][2 * e] = r.x;
             s[n][2 * e + 1] = r.y;
           }

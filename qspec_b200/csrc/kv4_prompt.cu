@@ -96,7 +96,7 @@ __device__ __noinline__ float wide_block(uint32_t st, const Block& f, float rowf
     landed32(x);
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
-      const float k = f.ks[c0 + j] * rowf, y = fmaf(__uint_as_float(x[j]), k < 1.17549435e-38f ? 1.17549435e-38f : k, f.lvs[c0 + j]);
+      const float k = f.ks[c0 + j] * rowf, y = fmaf(__uint_as_float(x[j]), k < 1.17549435e-38f ? 1.17549435e-38f : k > 3.402823466e38f ? 3.402823466e38f : k, f.lvs[c0 + j]);
       if (c0 + j <= limit) mn = fmaxf(mn, y);
       x[j] = __float_as_uint(y);
     }
@@ -572,8 +572,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
         mn = largest(x, mn);
         mn = largest(x + 32, mn);
       }
-      // The block's powers of two: what scores are multiplied with (not so small that it would make a hidden key's minus infinity no number), what exponents begin with
-      const float k = wide ? 1.f : fmaxf(rowf * factors.x, 1.17549435e-38f), lv = factors.y, iv = factors.z;
+      // The block's powers of two: what scores are multiplied with (not so small that it would make a hidden key's minus infinity no number, nor so large that it would make a score of nothing one), what exponents begin with
+      const float k = wide ? 1.f : fminf(fmaxf(rowf * factors.x, 1.17549435e-38f), 3.402823466e38f), lv = factors.y, iv = factors.z;
       mn = fmaf(mn, k, lv);                                 // (minus infinity stays that)
       const bool grown = mn - m > GROWTH_LOG2;              // (of a row that had seen nothing: infinite, or nothing again and no number; far from zero m + 6 is more than that)
       if (__any_sync(0xffffffffu, grown)) {

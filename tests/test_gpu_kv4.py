@@ -795,3 +795,51 @@ def test_attention_next_to_a_key_that_counts_for_nothing(by, dtype, form):
     attend(form, *case, out, 10.9 / math.log2(math.e), ops.kv4_attention_workspace("cuda"), max_tokens=T)
     bound = torch.finfo(dtype).eps / 2 + 2.0 ** -11 + n * 2.0 ** -26 + 1.5 * n / 4 * 2.0 ** -23
     assert ((out.double() - 1).abs() <= bound).all(), (float((out.double() - 1).abs().max()), bound)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("exponent", [250, 252, 253, 254])
+@pytest.mark.parametrize("others", [None, 215])
+def test_attention_over_values_as_large_as_there_are(others, exponent, form):
+    """Value scales of up to 31 / 16 2^127 (what the writer gives ends at 2^123), alone and among others of 2^88. What weights are divided by that with is 2^-136 and more, a subnormal number that is off
+    by 2^-14 of itself at most, and so is the denominator."""
+    q, k, v, kw, vw, table, start, lens = make_attention(43, [300, 90], [40, 70], 8, 2, 128, 32, torch.bfloat16)
+    v.copy_(0x77 + torch.randint(0, 3, v.shape, generator=gen(43), device="cuda") + 16 * torch.randint(0, 3, v.shape, generator=gen(44), device="cuda"))   # (codes 7 to 9)
+    word = (exponent << 8) + (torch.randint(0, 16, vw.shape, generator=gen(45), device="cuda") << 4) + 8
+    if others:
+        word = torch.where(torch.arange(32, device="cuda") % 5 == 2, word, (word & 0xff) + (others << 8))
+    vw.copy_(word.to(I16))
+    out = torch.empty_like(q)
+    attend(form, q, k, v, kw, vw, table, start, lens, out, 128 ** -0.5, ops.kv4_attention_workspace("cuda"))
+    want, bound = attention_in_64_bits(q, k, v, kw, vw, table, start, lens, 128 ** -0.5)
+    assert torch.isfinite(out).all()
+    assert ((out.to(F64) - want).abs() <= bound + want.abs() * 2.0 ** -14).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_of_keys_as_large_as_there_are(dtype, form):
+    """Key scales of 2^123 and 2^127. Where a row's query is zero in the columns in which they are not, their scores are zero; where it is not, one of them (the largest) takes all."""
+    T, H, D, P, n = 40, 4, 128, 32, 200
+    pages = -(-n // P)
+    ones = torch.ones(pages, 1, P, device="cuda")
+    k, v = torch.full((pages, 1, P, D // 2), 0x88, dtype=U8, device="cuda"), torch.randint(0, 256, (pages, 1, P, D // 2), generator=gen(46), device="cuda").to(U8)
+    kw, vw = words_of(ones, 8 * ones), words_of(ones, 8 * ones)
+    k[..., 0] = 0x99                                          # 1 in the first two columns
+    k[0, 0, 3, 0], kw[0, 0, 3] = 0x89, (250 << 8) + 8 - 65536     # 2^123 in the first, and 2^127 for another
+    k[1, 0, 7, 0], kw[1, 0, 7] = 0x89, (254 << 8) + 8 - 65536
+    q = torch.zeros(T, H, D, dtype=dtype, device="cuda")
+    q[:, :, 1] = 1.0
+    q[T // 2:, :, 0] = 2.0 ** -9
+    case = (q, k, v, kw, vw, torch.arange(pages, dtype=I32, device="cuda")[None], i32([0, T]), i32([n]))
+    out = torch.empty_like(q)
+    attend(form, *case, out, 1.0, ops.kv4_attention_workspace("cuda"))
+    rows = values(v, vw)[:, 0].reshape(-1, D)[:n]
+    for t in (0, T // 2 - 1):
+        m = n - T + 1 + t
+        weight = torch.full((m,), math.e, dtype=F64, device="cuda")
+        weight[[3, 39]] = 1.0                                 # scores of 0, the others' are 1
+        want = (weight[:, None] * rows[:m]).sum(0) / weight.sum()
+        # weights are off by 2^-11, sums by n / 16 2^-23, the result by its rounding
+        assert ((out[t].double() - want).abs() <= 8 * (2.0 ** -10 + n / 16 * 2.0 ** -23) + want.abs() * torch.finfo(dtype).eps / 2).all()
+    assert (out[T // 2:].double() == rows[39]).all()
