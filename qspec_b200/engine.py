@@ -139,8 +139,9 @@ class QSpecEngine:
 
     # ---------------------------------------------------------------------------------------
     def _probs(self, hidden: torch.Tensor, out: Optional[torch.Tensor] = None, logits: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """softmax(logits / temperature), float32 [rows, V]."""
-        return torch.softmax((self.model.logits(hidden) if logits is None else logits).float().mul_(1.0 / self.temperature), -1, out=out)
+        """softmax(logits / temperature), float32 [rows, V]. (Logits that are given are the caller's, and stay as they are, in float32 too.)"""
+        x = (self.model.logits(hidden) if logits is None else logits).float()
+        return torch.softmax(x * (1.0 / self.temperature) if x is logits else x.mul_(1.0 / self.temperature), -1, out=out)
 
     @torch.no_grad()
     def _spec_step(self) -> None:
