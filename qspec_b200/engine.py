@@ -30,7 +30,8 @@ class QSpecEngine:
 
         logprobs: every step also leaves, on the device, what the target says of the tokens that it emits, under the distribution that they are drawn from (that of the logits if
         greedy): `out_logprobs`, `out_entropy` float32 and `out_ranks` int64 [B, k + 1], and of every place the `logprobs` best tokens, `out_top_logprobs` float32 and
-        `out_top_tokens` int64 [B, k + 1, logprobs] (0: none of these; None: nothing). Behind what is emitted (out_count) the log probability and the rank are 0. (The reference gives them
+        `out_top_tokens` int64 [B, k + 1, logprobs] (0: none of these; None: nothing); `prefill` leaves the same of the tokens that it emits (cur_tok): `first_logprobs`, `first_entropy`,
+        `first_ranks` [B], `first_top_logprobs` and `first_top_tokens` [B, logprobs]. Behind what is emitted (out_count) the log probability and the rank are 0. (The reference gives them
         with its sampler's output, vllm/spec_decode/spec_decode_worker.py.)
 
         Over a paged cache with fewer pages than all sequences may need, a step may find none for some of them: these emit nothing (out_count 0) and stay where they
@@ -70,6 +71,9 @@ class QSpecEngine:
             self.out_ranks = torch.zeros(B, k + 1, dtype=torch.int64, device=dev)
             self.out_top_logprobs = torch.zeros(B, k + 1, logprobs, device=dev)
             self.out_top_tokens = torch.zeros(B, k + 1, logprobs, dtype=torch.int64, device=dev)
+            self.first_logprobs, self.first_entropy = torch.zeros(B, device=dev), torch.zeros(B, device=dev)
+            self.first_ranks = torch.zeros(B, dtype=torch.int64, device=dev)
+            self.first_top_logprobs, self.first_top_tokens = torch.zeros(B, logprobs, device=dev), torch.zeros(B, logprobs, dtype=torch.int64, device=dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.stream = torch.cuda.Stream(device=dev)
         # pinned host mirrors for the end-to-end API
@@ -128,11 +132,14 @@ class QSpecEngine:
                                   w4a4=False)
                 if e == P:
                     last_hidden[b].copy_(h[e - s - 1])
+        logits = m.logits(last_hidden) if self.n_logprobs is not None else None
         if self.temperature:
             self.uniform.uniform_(generator=self.generator)
-            ops.sample_probs(self._probs(last_hidden), self.uniform[0, :, 0].contiguous(), self.cur_tok)
+            ops.sample_probs(self._probs(last_hidden, logits=logits), self.uniform[0, :, 0].contiguous(), self.cur_tok)
         else:
-            self.cur_tok.copy_(m.greedy_tokens(last_hidden))
+            self.cur_tok.copy_(m.greedy_tokens(last_hidden) if logits is None else ops.argmax_rows(logits))
+        if logits is not None:
+            self._score(logits, self.cur_tok, self.first_logprobs, self.first_entropy, self.first_ranks, self.first_top_logprobs, self.first_top_tokens)
         self.seq_len.fill_(P)
         self._len_bound = P
         self.counters.zero_()
@@ -142,6 +149,9 @@ class QSpecEngine:
         """softmax(logits / temperature), float32 [rows, V]. (Logits that are given are the caller's, and stay as they are, in float32 too.)"""
         x = (self.model.logits(hidden) if logits is None else logits).float()
         return torch.softmax(x * (1.0 / self.temperature) if x is logits else x.mul_(1.0 / self.temperature), -1, out=out)
+
+    def _score(self, logits, tokens, logprobs, entropy, ranks, top_logprobs, top_tokens) -> None:
+        ops.token_logprobs(logits, tokens, logprobs, entropy, ranks, *((top_logprobs, top_tokens) if self.n_logprobs else (None, None)), temperature=self.temperature or 1.0)
 
     @torch.no_grad()
     def _spec_step(self) -> None:
@@ -202,9 +212,7 @@ class QSpecEngine:
             self.out_tokens.copy_(emitted)
             self.out_count.mul_(served)
         if logits is not None:
-            top = (self.out_top_logprobs.flatten(0, 1), self.out_top_tokens.flatten(0, 1)) if self.n_logprobs else (None, None)
-            ops.token_logprobs(logits, self.out_tokens.view(-1), self.out_logprobs.view(-1), self.out_entropy.view(-1), self.out_ranks.view(-1), *top,
-                               temperature=self.temperature or 1.0)
+            self._score(logits, *(t.flatten(0, 1) for t in (self.out_tokens, self.out_logprobs, self.out_entropy, self.out_ranks, self.out_top_logprobs, self.out_top_tokens)))
         count = self.out_count
         self.cur_tok.copy_(nxt)
         self.seq_len.add_(count.to(torch.int32))

@@ -297,3 +297,31 @@ def test_what_is_refused():
     k, v = cache.read(-1, 2, 48)
     assert k.shape == v.shape == (48, 2, 64) and not k.any()
     assert ops.max_top_logprobs() == 32
+
+
+@pytest.mark.parametrize("kv_cache", ["f16", "int8", "uint4"])
+@pytest.mark.parametrize("temperature", [0.0, 0.6])
+@pytest.mark.parametrize("n", [0, 4])
+def test_the_first_token_has_scores_as_well(n, temperature, kv_cache, monkeypatch):
+    """What a prefill emits: with the steps' scores behind it, those of the whole of a generated text."""
+    B = 3
+    model = QSpecLlamaModel(config(kv_cache=kv_cache), max_batch=B, max_tokens=16, seed=5)
+    engine = QSpecEngine(model, B, 2, temperature=temperature, logprobs=n, seed=2)
+    seen, logits = [], model.logits
+    monkeypatch.setattr(model, "logits", lambda h: seen.append(logits(h)) or seen[-1])
+    for first in (0, 50):                                     # a second prefill writes over the first one's
+        engine.prefill(torch.arange(first, first + B * 5, device="cuda").view(B, 5))
+        z = seen[-1].double() / (temperature or 1.0)
+        assert z.shape[0] == B
+        p = torch.log_softmax(z, -1)
+        torch.testing.assert_close(engine.first_logprobs.double(), p.gather(1, engine.cur_tok[:, None])[:, 0], rtol=2.0 ** -20, atol=2.0 ** -18)
+        torch.testing.assert_close(engine.first_entropy.double(), -(p.exp() * p).sum(-1), rtol=2.0 ** -18, atol=2.0 ** -18)
+        assert torch.equal(engine.first_ranks, 1 + (z > z.gather(1, engine.cur_tok[:, None])).sum(-1))
+        assert torch.equal(engine.first_top_tokens, z.sort(dim=-1, descending=True, stable=True).indices[:, :n])
+        torch.testing.assert_close(engine.first_top_logprobs.double(), p.gather(1, engine.first_top_tokens), rtol=2.0 ** -20, atol=2.0 ** -18)
+        if not temperature:
+            assert (engine.first_ranks == 1).all()
+    other = QSpecEngine(QSpecLlamaModel(config(kv_cache=kv_cache), max_batch=B, max_tokens=16, seed=5), B, 2, temperature=temperature, seed=2)
+    for first in (0, 50):
+        other.prefill(torch.arange(first, first + B * 5, device="cuda").view(B, 5))
+    assert torch.equal(other.cur_tok, engine.cur_tok) and not hasattr(other, "first_logprobs")
