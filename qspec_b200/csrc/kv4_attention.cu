@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) kv4_attention_kernel(const AttA
         if (bad) { f = NAN; v = 1.f; }                      // rows that see it are no numbers
         if (key0 + lane >= keys) f = 0.f;
         const uint32_t x[4] = {__float_as_uint(f), __float_as_uint(__uint_as_float(0xcb000000u | (kw & 15u)) + 8388608.f) /* - z */, __float_as_uint(__log2f(v)),
-                               __float_as_uint(__fdividef(WEIGHT_UNIT * 5.9604644775390625e-8f, v * 5.9604644775390625e-8f))};   // (2^-24: a divisor above 2^126 would give zero)
+                               __float_as_uint(over_scale(WEIGHT_UNIT, v))};
         if constexpr (FEW) {
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(mine), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
         } else {

@@ -18,6 +18,12 @@ using kv8::page_shift;
 
 #ifdef __CUDACC__
 __device__ __forceinline__ float word_scale(uint32_t w) { return __uint_as_float((w & 0xfff0u) << 15); }
+// `unit` / v for a value's scale v >= 2^-100. (The reciprocal is that of 2^-24 v: one of less than 2^-126 would be zero.)
+__device__ __forceinline__ float over_scale(float unit, float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(v * 5.9604644775390625e-8f));
+  return r * (unit * 5.9604644775390625e-8f);
+}
 #endif
 
 struct PromptArgs4 {

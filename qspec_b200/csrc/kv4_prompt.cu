@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv4_prompt_kernel(const Args a) {
           if (side) {
             const float v = fmaxf(scale, 7.888609052210118e-31f);
             f.lvs[part + e] = __log2f(v) - TOP;
-            f.ivs[part + e] = __fdividef(WEIGHT_UNIT * (1 << TOP) * 5.9604644775390625e-8f, v * 5.9604644775390625e-8f);   // (2^-24: a divisor above 2^126 would give zero)
+            f.ivs[part + e] = over_scale(WEIGHT_UNIT * (1 << TOP), v);
           } else {
             f.ks[part + e] = scale * (1.f / (1 << TOP));
           }
