@@ -8,7 +8,7 @@
 
 `generate` takes prompts as comma-separated token ids (the framework has no tokenizer), runs them through the
 continuous-batching scheduler with greedy sampling and prints one JSON line per prompt (with --logprobs N also each token's log probability, rank, entropy and N
-alternatives). `score` prints the same of given tokens, and the text's perplexity.
+alternatives). `score` prints the same of given tokens, and the text's perplexity. Numbers that are infinite, or none, are null.
 """
 from __future__ import annotations
 
@@ -49,6 +49,16 @@ def _scheduler(args, new_tokens: int):
     return Scheduler(model, prefill_portion=args.prefill_portion), prompts
 
 
+def _print(line: dict) -> None:
+    def plain(x):
+        if isinstance(x, dict):
+            return {k: plain(v) for k, v in x.items()}
+        if isinstance(x, (list, tuple)):
+            return [plain(v) for v in x]
+        return None if isinstance(x, float) and not math.isfinite(x) else x
+    print(json.dumps(plain(line), allow_nan=False))
+
+
 def _generate(argv) -> int:
     ap = _arguments("generate")
     ap.add_argument("--max-new-tokens", type=int, default=16)
@@ -57,7 +67,7 @@ def _generate(argv) -> int:
     args = ap.parse_args(argv)
     scheduler, prompts = _scheduler(args, args.max_new_tokens)
     for p, r in zip(prompts, scheduler.generate_requests(prompts, args.max_new_tokens, args.eos, args.logprobs)):
-        print(json.dumps({"prompt": p, "tokens": r.output} | ({} if args.logprobs is None else {"scores": [asdict(s) for s in r.scores]})))
+        _print({"prompt": p, "tokens": r.output} | ({} if args.logprobs is None else {"scores": [asdict(s) for s in r.scores]}))
     return 0
 
 
@@ -67,8 +77,8 @@ def _score(argv) -> int:
     args = ap.parse_args(argv)
     scheduler, prompts = _scheduler(args, 0)
     for p, scores in zip(prompts, scheduler.score(prompts, args.top)):
-        mean = sum(s.logprob for s in scores) / len(scores) if scores else None
-        print(json.dumps({"prompt": p, "perplexity": None if mean is None else math.exp(-mean) if mean > -700 else math.inf, "scores": [asdict(s) for s in scores]}))
+        mean = sum(s.logprob for s in scores) / len(scores) if scores else math.nan
+        _print({"prompt": p, "perplexity": math.exp(-mean) if mean > -700 else None, "scores": [asdict(s) for s in scores]})
     return 0
 
 
