@@ -152,14 +152,15 @@ class Scheduler:
         """What the model says of each text's tokens behind the first, each given those in front of it, with the `top` likeliest tokens of each place: the exponential of minus the
         log probabilities' mean is the text's perplexity. One text after the other, a step's tokens at a time; needs a free slot."""
         self._check_top(top)
-        results = []
-        for k, text in enumerate(texts):
-            rid, text = ("score", self.steps, k), list(text)
+        texts, limit = [list(text) for text in texts], getattr(self.model, "max_seq_len", None)
+        for text in texts:                                     # (all of them, before any is taken)
             if not text:
                 raise ValueError("empty text")
-            limit = getattr(self.model, "max_seq_len", None)
-            if limit is not None and len(text) - 1 > limit:   # (before any of it is taken)
+            if limit is not None and len(text) - 1 > limit:
                 raise RuntimeError(f"a text of {len(text)} tokens; the cache takes {limit}")
+        results = []
+        for k, text in enumerate(texts):
+            rid = ("score", self.steps, k)
             scores: List[TokenScore] = []
             try:
                 for at in range(0, len(text) - 1, self.prefill_portion):

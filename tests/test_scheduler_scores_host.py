@@ -74,3 +74,13 @@ def test_what_is_refused():
     with pytest.raises(ValueError):
         s.score([[]])
     assert not s.has_work()
+
+
+@pytest.mark.parametrize("texts,error", [([[1, 2, 3], []], ValueError), ([[1, 2, 3], [1] * 52], RuntimeError)])
+def test_texts_are_looked_at_before_any_is_scored(texts, error):
+    model = Counting()
+    model.max_seq_len = 50
+    s = Scheduler(model)
+    with pytest.raises(error):
+        s.score(texts)
+    assert model.calls == 0 and [len(x) for x in s.score([[1] * 51, [1, 2]])] == [50, 1]
