@@ -156,6 +156,7 @@ class Scheduler:
         for text in texts:                                     # (all of them, before any is taken)
             if not text:
                 raise ValueError("empty text")
+            self._check_tokens(text)
             if limit is not None and len(text) - 1 > limit:
                 raise RuntimeError(f"a text of {len(text)} tokens; the cache takes {limit}")
         results = []
@@ -172,6 +173,11 @@ class Scheduler:
             results.append(scores)
         return results
 
+    def _check_tokens(self, tokens: Sequence[int]) -> None:
+        """Those outside the vocabulary would be looked up outside the embedding, on the device."""
+        if min(tokens) < 0 or max(tokens) >= self.model.vocab_size:
+            raise ValueError(f"tokens are 0 to {self.model.vocab_size - 1}, got {min(tokens)} to {max(tokens)}")
+
     def _check_top(self, top: Optional[int]) -> None:
         if top is None:
             return
@@ -184,6 +190,7 @@ class Scheduler:
         """logprobs: the request's tokens come with a `TokenScore` each (`Request.scores`), with so many alternatives."""
         if not len(prompt):
             raise ValueError("empty prompt")
+        self._check_tokens(prompt)
         self._check_top(logprobs)
         if rid in self.finished or any(r.rid == rid for r in list(self.waiting) + self.running):
             raise ValueError(f"request id {rid!r} is already known")
@@ -246,8 +253,13 @@ class Scheduler:
     def generate_requests(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, eos: Optional[int] = None, logprobs: Optional[int] = None) -> List[Request]:
         """`generate`, with all that is known of the finished requests (`Request.scores`)."""
         ids = [("gen", self.steps, k) for k in range(len(prompts))]
-        for rid, p in zip(ids, prompts):
-            self.add(rid, p, max_new_tokens, eos, logprobs)
+        for k, (rid, p) in enumerate(zip(ids, prompts)):
+            try:
+                self.add(rid, p, max_new_tokens, eos, logprobs)
+            except ValueError:
+                for added in ids[:k]:                          # (one that is refused leaves no others waiting)
+                    self.release(added)
+                raise
         while self.has_work():
             self.step()
         return [self.finished.pop(rid) for rid in ids]

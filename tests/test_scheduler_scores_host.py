@@ -84,3 +84,17 @@ def test_texts_are_looked_at_before_any_is_scored(texts, error):
     with pytest.raises(error):
         s.score(texts)
     assert model.calls == 0 and [len(x) for x in s.score([[1] * 51, [1, 2]])] == [50, 1]
+
+
+@pytest.mark.parametrize("tokens", [[-1], [1000], [1, 2, 1 << 40], [5, -7, 3]])
+def test_tokens_outside_the_vocabulary_are_refused(tokens):
+    model = Counting()
+    s = Scheduler(model)
+    with pytest.raises(ValueError, match="tokens are 0 to 999"):
+        s.add("x", tokens, 2)
+    with pytest.raises(ValueError, match="tokens are 0 to 999"):
+        s.score([[1, 2], tokens])
+    with pytest.raises(ValueError, match="tokens are 0 to 999"):
+        s.generate([[1], tokens], 2)
+    assert model.calls == 0 and not s.has_work() and [x.token for x in s.score([[0, 999]])[0]] == [999]
+    assert s.generate(PROMPTS, 3) == Scheduler(Counting()).generate(PROMPTS, 3)
