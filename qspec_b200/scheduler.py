@@ -138,15 +138,19 @@ class Scheduler:
                 self._release_slot(slot)
 
     # ---- log probabilities ------------------------------------------------------------------------------------------
-    def _scores(self, logits: torch.Tensor, tokens: Sequence[int], top: int) -> List[TokenScore]:
-        """Of tokens[i] under row i of the logits. Reads the device."""
+    def _scores(self, logits: torch.Tensor, tokens: torch.Tensor, top: int) -> List[TokenScore]:
+        """Of tokens[i] under row i of the logits. Reads the device, once: all results lie in one buffer."""
         n, dev = len(tokens), logits.device
-        ids = torch.tensor(tokens, dtype=torch.int64, device=dev)
-        lp, entropy, ranks = torch.empty(n, device=dev), torch.empty(n, device=dev), torch.empty(n, dtype=torch.int64, device=dev)
-        best = (torch.empty(n, top, device=dev), torch.empty(n, top, dtype=torch.int64, device=dev)) if top else (None, None)
-        ops.token_logprobs(logits, ids, lp, entropy, ranks, *best)
-        alternatives = [list(zip(t, p)) for p, t in zip(best[0].tolist(), best[1].tolist())] if top else [[] for _ in range(n)]
-        return [TokenScore(*row) for row in zip(tokens, lp.tolist(), ranks.tolist(), entropy.tolist(), alternatives)]
+        buffer = torch.empty(n * ((2 + top) * 8 + (2 + top) * 4), dtype=torch.uint8, device=dev)
+
+        def parts(of: torch.Tensor):
+            whole, real = of[:n * (2 + top) * 8].view(torch.int64), of[n * (2 + top) * 8:].view(torch.float32)
+            return whole[:n], whole[n:2 * n], whole[2 * n:].view(n, top), real[:n], real[n:2 * n], real[2 * n:].view(n, top)
+        ids, ranks, best, lp, entropy, best_lp = parts(buffer)
+        ids.copy_(tokens)
+        ops.token_logprobs(logits, ids, lp, entropy, ranks, *((best_lp, best) if top else (None, None)))
+        ids, ranks, best, lp, entropy, best_lp = (t.tolist() for t in parts(buffer.cpu()))
+        return [TokenScore(t, p, r, h, list(zip(b, q))) for t, p, r, h, b, q in zip(ids, lp, ranks, entropy, best, best_lp)]
 
     def score(self, texts: Sequence[Sequence[int]], top: int = 0) -> List[List[TokenScore]]:
         """What the model says of each text's tokens behind the first, each given those in front of it, with the `top` likeliest tokens of each place: the exponential of minus the
@@ -167,7 +171,7 @@ class Scheduler:
                 for at in range(0, len(text) - 1, self.prefill_portion):
                     part = text[at:min(at + self.prefill_portion, len(text) - 1)]
                     logits = self.feed([(rid, part, list(range(len(part))))])
-                    scores += self._scores(logits, text[at + 1:at + 1 + len(part)], top)
+                    scores += self._scores(logits, torch.tensor(text[at + 1:at + 1 + len(part)], dtype=torch.int64), top or 0)
             finally:
                 self.release(rid)
             results.append(scores)
@@ -229,13 +233,16 @@ class Scheduler:
         for r, n in portions:
             r.fed += n
         self.steps += 1
-        toks = ops.argmax_rows(logits).tolist() if logits.shape[0] else []
-        sampled = []
-        if toks and any(r.logprobs is not None for r in owners):
-            for r, score in zip(owners, self._scores(logits, [int(t) for t in toks], max(r.logprobs or 0 for r in owners))):
+        toks, sampled = ops.argmax_rows(logits) if logits.shape[0] else [], []
+        if len(toks) and any(r.logprobs is not None for r in owners):
+            scores = self._scores(logits, toks, max(r.logprobs or 0 for r in owners))
+            toks = [score.token for score in scores]
+            for r, score in zip(owners, scores):
                 if r.logprobs is not None:
                     score.top = score.top[:r.logprobs]
                     r.scores.append(score)
+        elif len(toks):
+            toks = toks.tolist()
         for r, t in zip(owners, toks):
             r.output.append(int(t))
             sampled.append((r.rid, int(t)))

@@ -325,3 +325,22 @@ def test_the_first_token_has_scores_as_well(n, temperature, kv_cache, monkeypatc
     for first in (0, 50):
         other.prefill(torch.arange(first, first + B * 5, device="cuda").view(B, 5))
     assert torch.equal(other.cur_tok, engine.cur_tok) and not hasattr(other, "first_logprobs")
+
+
+def test_scores_are_read_with_the_tokens():
+    """A step with scores reads the device as often as one without."""
+    from torch.profiler import ProfilerActivity, profile
+    reads = []
+    for n in (None, 0, 5):
+        s = Scheduler(QSpecLlamaModel(config(), max_batch=3, max_tokens=32, seed=7))
+        for i, p in enumerate(([1, 2, 3], [9, 8, 7, 6], [30] * 20)):
+            s.add(i, p, 8, logprobs=n)
+        for _ in range(3):
+            s.step()
+        torch.cuda.synchronize()
+        with profile(activities=[ProfilerActivity.CUDA]) as prof:
+            for _ in range(2):
+                s.step()
+            torch.cuda.synchronize()
+        reads.append(sum("DtoH" in e.name for e in prof.events()))
+    assert reads[0] > 0 and reads == reads[:1] * 3, reads
