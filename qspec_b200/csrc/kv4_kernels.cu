@@ -10,9 +10,9 @@ namespace kv4 {
 // is, and spreads a channel that is large in all keys over a row's columns). Of a row of keys or values, in float32:
 //   hi = max(largest, 0), lo = min(smallest, 0)   of the values that are finite; beyond 2^126 they count as 2^126
 //   s = max((hi - lo) * (1 / 15), 2^-60), rounded to five significant bits, halves up;   z = rint(-lo / s);   c = clamp(rint(x / s) + z, 0, 15)
-// All with the roundings that the formulas have (no fused multiply-adds, quotients by s correctly rounded, 1 / 15 as float32 has it, which is a little more: halves stay halves or
-// above), so that the same codes come out of every implementation in
-// float32: scales of five bits and values of eight or eleven make quotients that lie halfway between two codes common.
+// All with the roundings that the formulas have (no fused multiply-adds, quotients by s correctly rounded, a product with 1 / 15 as float32 has it, which is a little more: halves stay
+// halves or above), so that the same codes come out of every implementation of them in float32 (one that divides by 15 instead gives another scale to one row in a million): scales of
+// five bits and values of eight or eleven make quotients that lie halfway between two codes common.
 //
 // D / 16 lanes take a row; a lane holds sixteen of its values, eight of each half, so that it has both of every pair that the rotation turns, and the butterflies of the
 // Hadamard matrix need another lane for D / 16 of D's strides only. What bounds it: bytes, of a prompt (queries come and go in 16 bits); a launch and a chain of loads, of a step.

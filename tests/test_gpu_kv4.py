@@ -843,3 +843,44 @@ def test_attention_of_keys_as_large_as_there_are(dtype, form):
         # weights are off by 2^-11, sums by n / 16 2^-23, the result by its rounding
         assert ((out[t].double() - want).abs() <= 8 * (2.0 ** -10 + n / 16 * 2.0 ** -23) + want.abs() * torch.finfo(dtype).eps / 2).all()
     assert (out[T // 2:].double() == rows[39]).all()
+
+
+def test_a_scale_is_the_range_times_float32_of_a_fifteenth():
+    """A million rows of keys in float32, by a multiplication that is written as one (tests above divide by a plain number, which PyTorch makes a multiplication of on CUDA)."""
+    G, D, P, n = 8, 64, 128, 128 * 1024
+    g = gen(47)
+    x = torch.randn(n, 3 * G, D, generator=g, device="cuda").half()
+    angle = torch.rand(n, D // 2, generator=g, device="cuda") * 6.28
+    cs = torch.cat((angle.cos(), angle.sin()), -1).half()
+    k, v = (torch.zeros(n // P, G, P, D // 2, dtype=U8, device="cuda") for _ in range(2))
+    kw, vw = (torch.zeros(n // P, G, P, dtype=I16, device="cuda") for _ in range(2))
+    at = i32(range(n))
+    ops.kv4_append(x.flatten(1), cs, at, at, k, v, kw, vw, None, hadamard=True)
+    y = hadamard(rotated(x[:, G:2 * G].float(), cs.float(), F32))
+    hi, lo = y.amax(-1).clamp(min=0), y.amin(-1).clamp(max=0)
+    scale = lambda r: ((r.view(I32) + (1 << 18)) >> 19 << 19).view(F32)  # noqa: E731
+    s = scale((hi - lo) * torch.full_like(hi, 1 / 15))
+    z = (-lo / s).round()
+    got_s, got_z = scales(kw.transpose(1, 2).reshape(n, G))
+    assert torch.equal(got_s, s) and torch.equal(got_z, z)
+    assert torch.equal(unpack(k.transpose(1, 2).reshape(n, G, D // 2)).float(), ((y / s[..., None]).round() + z[..., None]).clamp(0, 15))
+
+
+def test_a_scale_is_not_the_range_divided_by_15():
+    """Rotated pairs (x cos - w sin, w cos + x sin) whose range times float32(1 / 15) reaches a border between two scales that their range / 15 does not."""
+    pairs = [(2.60546875, -0.76904296875, 0.72705078125, 0.81298828125), (2.044921875, -0.04815673828125, 0.51123046875, 0.65673828125),
+             (1.6337890625, -0.241455078125, 0.88818359375, 0.66357421875), (4.19921875, -0.9091796875, 0.66845703125, 0.02276611328125),
+             (4.1328125, 0.235595703125, 0.7529296875, 0.70849609375), (7.3671875, -0.76416015625, 0.416259765625, 0.88623046875)]
+    n, D = len(pairs), 64
+    p = torch.tensor(pairs).half().float()                     # (all are float16)
+    x, cs = torch.zeros(n, 3, D), torch.zeros(n, D)
+    x[:, 1, 0], x[:, 1, 32], cs[:, 0], cs[:, 32] = p.unbind(1)
+    a, b = p[:, 0] * p[:, 2] - p[:, 1] * p[:, 3], p[:, 1] * p[:, 2] + p[:, 0] * p[:, 3]
+    r = torch.maximum(a, b).clamp(min=0) - torch.minimum(a, b).clamp(max=0)
+    scale = lambda r: ((r.view(I32) + (1 << 18)) >> 19 << 19).view(F32)  # noqa: E731
+    want, divided = scale(r * torch.full_like(r, 1 / 15)), scale((r.double() / 15).float())   # (rounded once: 24 bits of 53)
+    assert (want > divided).all()
+    k, v = (torch.zeros(1, 1, 16, D // 2, dtype=U8, device="cuda") for _ in range(2))
+    kw, vw = (torch.zeros(1, 1, 16, dtype=I16, device="cuda") for _ in range(2))
+    ops.kv4_append(x.flatten(1).half().cuda(), cs.half().cuda(), i32(range(n)), i32(range(n)), k, v, kw, vw, None)
+    assert torch.equal(scales(kw[0, 0, :n])[0].cpu(), want)
