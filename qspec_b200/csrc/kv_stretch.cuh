@@ -261,8 +261,8 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
   const int tid = threadIdx.x;
   __syncthreads();
   constexpr int PER_ROW = THREADS / TR < D / 4 ? THREADS / TR : D / 4, PIECES = D / 4 / PER_ROW;   // threads of a row, float4 of a thread
-  const int jr = min(tid / PER_ROW, TR - 1), col = tid % PER_ROW;
-  const bool spare = TR * PER_ROW < THREADS && tid >= TR * PER_ROW;   // (does what others do)
+  static_assert(TR * PER_ROW == THREADS, "every thread has a row");
+  const int jr = tid / PER_ROW, col = tid % PER_ROW;
   float mm = NONE, ll = 0.f;
   float4 oo[PIECES];
 #pragma unroll
@@ -339,7 +339,7 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
           const float mn = fmaxf(mm, mp[k]);
           ll = (mm == NONE ? ll : ll * exp2_fast(mm - mn)) + (none ? lp[k] : lp[k] * exp2_fast(mp[k] - mn));
           mm = mn;
-          if (i0 + k * PER_ROW < n && !spare) factor[(i0 + k * PER_ROW) * TR + jr] = none && lp[k] != 0.f ? INFINITY : mp[k];
+          if (i0 + k * PER_ROW < n) factor[(i0 + k * PER_ROW) * TR + jr] = none && lp[k] != 0.f ? INFINITY : mp[k];
         }
       }
       const float own = mm;
@@ -348,7 +348,7 @@ __device__ __forceinline__ void finish_segment(const Step& a, const Out& o, cons
       if (own != NONE) ll *= exp2_fast(own - mm);
 #pragma unroll
       for (int x = PER_ROW / 2; x > 0; x >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, x);
-      for (int i = col; i < n && !spare; i += PER_ROW) {
+      for (int i = col; i < n; i += PER_ROW) {
         const float f = factor[i * TR + jr];
         factor[i * TR + jr] = f == NONE ? 0.f : f == INFINITY ? 1.f : exp2_fast(f - mm);
       }
