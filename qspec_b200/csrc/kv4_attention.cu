@@ -34,7 +34,8 @@ using namespace kv8;
 // 256 after 1000: 86 (106); 4 after 676: 11.7 (12.8); one of 2 after 20000: 21 (24); one after 131071, 64 / 8 heads: 46 (57).
 // CTAs of an SM (while one waits at a barrier the others compute): three of four warps; four, for tiles of eight, where requests x heads of keys are more than three CTAs an SM, so that each
 // may still have CTAs of its own. us with three (with four), a token each: 16 requests after 3000 keys 25 (26), 32: 40 (38), 48: 45 (52), 64: 62 (58), after 700 keys 30 (22); one after
-// 131071 46 (52). Two of eight warps: 66, 32, 52; five of four: 67, 26, 58. Tiles of sixteen, 64 requests of 4 tokens after 3000, after 748 keys, one of 4 after 20000: two of eight warps 86, 40, 27; three of
+// 131071 46 (52). Heads of 64, where four a SM spill 372 bytes, the same: 32 / 8 heads, 16 requests after 3000 keys 17.5 (19.5), 32: 23.7 (25.9), 64: 40.4 (39.9), 128: 68.4 (65.9), 64 after 700: 23.0 (15.9), 256 after
+// 1000: 65.6 (58.9), one after 60000 23.0 (29.7); 64 / 16 heads, 16 after 3000 26.8 (26.2), 32: 40.6 (38.7), 128: 121 (113), 256 after 1000: 112 (103). Two of eight warps: 66, 32, 52; five of four: 67, 26, 58. Tiles of sixteen, 64 requests of 4 tokens after 3000, after 748 keys, one of 4 after 20000: two of eight warps 86, 40, 27; three of
 // four 77, 32, 27; four of four 78, 28, 36.
 constexpr int WARPS = 4, THREADS = WARPS * 32, SMS_MOST = 160, CTAS_MOST = 4;
 

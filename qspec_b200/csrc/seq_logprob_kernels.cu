@@ -11,8 +11,8 @@
 // seen: a few at a time. Where there are more than there
 // is room for (rows that rise, rows of one value), the span is looked through once for each one that is asked for. Whichever way, values are ordered together with their
 // tokens as whole numbers of 64 bits, so that there is one result. Sums are made in a fixed order in float32.
-// Measured: 4 rows of 128256 in float16 6.3 us, with 5 alternatives 8.3; 256 rows 21.6, with 5 26.8 (2.4 TB/s: some 11 instructions a value, issue 60 %); 1000 rows of 151643 in float32 with 20
-// 118 to 124 (5 TB/s). Not taken: exponents without an end at -16384, and sums that are no number made again (a value's instruction less; 256 rows 24.4 for 21.5); three CTAs an SM (24.9).
+// Measured: 4 rows of 128256 in float16 6.3 us, with 5 alternatives 8.3; 256 rows 21.6, with 5 26.2 (2.5 TB/s: some 11 instructions a value, issue 60 %); 1000 rows of 151643 in float32 with 20
+// 118 to 125 (5 TB/s). Not taken: exponents without an end at -16384, and sums that are no number made again (a value's instruction less; 256 rows 24.4 for 21.5); three CTAs an SM (24.9).
 #include "seq_common.cuh"
 #include "../../include/qspec_b200_seq.h"
 #include <algorithm>
@@ -22,7 +22,9 @@ namespace logprob {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, MOST_TOP = 32, EACH = 4;   // EACH: vectors of a thread in a batch
 constexpr int GROUPS = 128, GROUP = THREADS / GROUPS, HITS = 256, CANDIDATES = 512;   // groups of neighbouring threads; vectors with candidates, candidates in them
-constexpr int FEW_TOP = 8;                        // alternatives that are few: us of 256 rows of 128256 with 5, taken like more of them 28.8, so 26.8; 4 rows 9.5, 8.3
+// Alternatives that are few: us taken like more of them (so), with 1, 5, 8, 9, 12, 20: 256 float16 rows of 128256 27.6 (25.0), 29.0 (27.6), 30.4 (28.9), 30.2 (29.8), 31.1 (143: more candidates
+// than there is room for), 33.3 (346); 4 rows 11.0 (9.6), 11.7 (10.4), 12.0 (10.8), 12.2 (11.1), 12.5 (11.5), 13.6 (13.5); 600 float32 rows of 151643 99 (97), 101 (99), 102 (100), 103 (101), 103 (661), 105 (1573).
+constexpr int FEW_TOP = 8;
 typedef unsigned long long u64;
 
 struct Args {
