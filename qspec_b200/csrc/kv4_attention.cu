@@ -14,8 +14,8 @@
 //   float16 1024 + c, or 1024 + 16 c in the upper half, and one addition or multiply-add makes it c - z. (Sums over values must not carry an offset: over many
 //   keys it cancels, and what the products cut off would be of the size of what is left.)
 //
-// Queries are multiplied by a power of two per row that brings their largest value to 2^14 .. 2^15 and are float16 from there on, exactly (what is below 2^-38 of the
-// largest may lose bits). A key's scale multiplies its scores in float32. A value's scale v goes into the exponent: the weights 2^(9 + s + log2 v - m) lie below 2^15
+// Queries are multiplied by a power of two per row that brings their largest value to 2^14 .. 2^15 and are float16 from there on, exactly (but for the last bits of what is below 2^-24
+// of the largest, and all of what is below 2^-34: odd columns are divided by 16). A key's scale multiplies its scores in float32. A value's scale v goes into the exponent: the weights 2^(9 + s + log2 v - m) lie below 2^15
 // whatever the scales are and are rounded to float16 for the product with the codes (by 2^-11 of themselves at most, or by 2^-34 of the largest: kv8_common.cuh); the denominator
 // is the sum of the unrounded weights / v.
 //

@@ -230,11 +230,12 @@ extern "C" int qspec_kv4_append(const void* qkv, long long ld, const void* cos_s
                 QSPEC_ERR_INVALID_ARG, "kv4_append: rows must lie on 16-byte boundaries (ld=%lld)", ld);
   AppendArgs a{qkv, ld, cos_sin, cos_rows, positions, slots, (uint8_t*)k, (uint8_t*)v, (uint16_t*)k_word, (uint16_t*)v_word, q_out, q_tok_stride, ntok, H, G, npages,
                page_shift(page_tokens), 2 * G + (q_out ? H : 0), 0, 0};
-  // Steps of a warp: one while that makes no more than twice the warps that the SMs hold, else as few as they all hold at once (warps that come later begin a chain of loads of their own).
-  // us, 40 / 8 heads of 128, one step (as few as they hold): 256 tokens 9 (9), 512: 12 (14), 700: 15 (15), 1000: 18 (18), 1500: 24 (21), 2000: 30 (26), 4200: 56 (44), 8000: 101 (71)
+  // Steps of a warp: as few as make warps that the SMs all hold at once (warps that come later begin a chain of loads of their own). us of the kernel, 40 / 8 heads of 128, one step (as few as that), without
+  // the Hadamard matrix: 256 tokens 4.9 (4.8), 512: 7.4 (6.5), 700: 8.6 (7.5), 1000: 10.8 (9.5), 1500: 14.7 (10.9), 2000: 18.3 (13.1), 4200: 35.2 (24.7), 8000: 62.3 (43.7); with it 512: 9.3 (8.5), 1000: 13.9
+  // (12.4), 4200: 44.8 (34.4). (With warps for twice the SMs' places allowed before there are two steps, 512 tokens took 7.3.)
   const int rows = D == 128 ? 4 : 8, most = (a.rows + rows - 1) / rows;
-  const long long hold = 32ll * std::max(sm_count(), 1), at_once = std::max(hold / ntok, 1ll);   // warps; of a token
-  a.steps = (long long)ntok * most <= 2 * hold ? 1 : (int)((most + at_once - 1) / at_once);
+  const long long at_once = std::max(32ll * std::max(sm_count(), 1) / ntok, 1ll);   // warps of a token
+  a.steps = (int)((most + at_once - 1) / at_once);
   a.warps = (most + a.steps - 1) / a.steps;
   const long long warps = (long long)ntok * a.warps;
   QSPEC_REQUIRE(warps < (1ll << 31), QSPEC_ERR_UNSUPPORTED, "kv4_append: %d tokens are too many for one call", ntok);
