@@ -66,6 +66,7 @@ struct alignas(16) Block {                                            // what th
   int wide;                                               // scales so far apart that codes stand in the operands without them; then, of each key:
   float ks[128], lvs[128], ivs[128];                      // its scale / 2^TOP (no number: rows that see it are none either), log2 of its value's / 2^TOP, and what weights are divided by that with
 };
+static_assert(offsetof(Block, wide) == offsetof(Block, k) + 12 && offsetof(Block, k) % 16 == 0, "read as a float4");
 // How far apart exponents of a block's scales may be. Keys': what is exact beside each other in an operand (five bits from 2^TOP down to float16's last, 2^-24). Values': their largest goes into the
 // exponents of all of the block's weights, and the reference with it; where a key that counts for nothing has it, later blocks' weights are that much closer to float16's end (2^-26 of the largest at 8).
 constexpr int APART_K = 30, APART_V = 8;

@@ -94,15 +94,16 @@ QSPEC_LANES16(__half, __half2, "f16x2", unpack_h8, __float2half2_rn)
 QSPEC_LANES16(__nv_bfloat16, __nv_bfloat162, "bf16x2", unpack_b8, __float2bfloat162_rn)
 #undef QSPEC_LANES16
 
-// Larger values first, no numbers before all, equal ones by the lower index; never 0.
+// Larger values first, no numbers before all, equal ones by the lower index; never 0, nor all ones (which best_below() begins with).
+constexpr uint32_t NO_NUMBER = 0xfffffffeu;       // (infinity is 0xff800000)
 __device__ __forceinline__ u64 key_of(float x, int index) {
   const uint32_t u = __float_as_uint(x + 0.f);              // (-0 is 0)
-  const uint32_t v = x != x ? 0xffffffffu : u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t v = x != x ? NO_NUMBER : u & 0x80000000u ? ~u : u | 0x80000000u;
   return (u64)v << 32 | (uint32_t)~index;
 }
 __device__ __forceinline__ float value_of(u64 key) {
   const uint32_t v = (uint32_t)(key >> 32);
-  return v == 0xffffffffu ? NAN : __uint_as_float(v & 0x80000000u ? v ^ 0x80000000u : ~v);
+  return v == NO_NUMBER ? NAN : __uint_as_float(v & 0x80000000u ? v ^ 0x80000000u : ~v);
 }
 __device__ __forceinline__ int index_of(u64 key) { return (int)~(uint32_t)key; }
 

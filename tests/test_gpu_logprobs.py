@@ -244,3 +244,19 @@ def test_of_rows_that_are_sure_of_a_token_wherever_it_stands(gap, temperature, r
     assert torch.equal(tlp[:, 0], lp) and torch.equal(tt[:, 0], at)
     entropy = -torch.special.xlogy(p.exp(), p.exp()).sum(-1)
     assert ((h - entropy).abs() <= entropy * (2.0 ** -17 + (V / 512 + 21) * 2.0 ** -24) + 2 * bound).all(), float((h - entropy).abs().max())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("V,top", [(1, 1), (2, 2), (7, 3), (33, 32), (5000, 8), (70000, 9)])
+def test_a_first_token_that_is_no_number_is_the_best(V, top, dtype):
+    """Like no numbers elsewhere in a row: the first one of them first; all of a row, and one of a kind."""
+    logits = torch.randn(5, V, generator=gen(19), device="cuda").to(dtype)
+    logits[0, 0] = math.nan
+    logits[1, 0], logits[1, V - 1] = math.nan, math.nan
+    logits[2] = math.nan
+    logits[3, 0] = math.inf
+    logits[4] = -math.inf
+    logits[4, 0] = math.nan
+    lp, h, rank, tlp, tt = call(logits, torch.zeros(5, dtype=I64, device="cuda"), top)
+    assert torch.equal(tt, logits.sort(dim=-1, descending=True, stable=True).indices[:, :top])
+    assert lp.isnan().all() and h.isnan().all() and tlp.isnan().all() and (rank == 1).all()
