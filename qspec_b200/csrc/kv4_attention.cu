@@ -19,7 +19,7 @@
 // whatever the scales are and are rounded to float16 for the product with the codes (by 2^-11 of themselves at most, or by 2^-34 of the largest: kv8_common.cuh); the denominator
 // is the sum of the unrounded weights / v.
 //
-// Measured: 64 requests of 4 tokens after some 3000 keys each, 32 / 8 heads of 128, 77 us, 2.7 TB/s of codes and words; one token after 131071 keys, 64 / 8 heads, 44 us, 3.2 TB/s; 4 requests of a
+// Measured: 64 requests of 4 tokens after some 3000 keys each, 32 / 8 heads of 128, 76 us, 2.7 TB/s of codes and words; one token after 131071 keys, 64 / 8 heads, 45 us, 3.1 TB/s; 4 requests of a
 // token after some 680 keys 12 us, which is launches and a chain of loads. At this many rows not the bytes bound it (two fifths of the time) but instructions: a unit of 32 keys takes a
 // warp some 650, of which 64 are products and 250 make codes operands; the tensor cores are busy 38 % of a long walk, the units of integer arithmetic 45 %.
 #include "kv4_common.cuh"
