@@ -499,7 +499,7 @@ int qspec_seq_argmax_rows(const void* logits, int rows, int V, long long row_str
 
 /* Log probabilities under softmax(logits / temperature), logits [rows, V] float16 / bfloat16 / float32 (row_stride >= V elements). tokens [rows] int64, or NULL (logprobs and ranks
  * are then NULL as well). Any of the results may be NULL:
- *   logprobs [rows]: of the given tokens; 0 where the token is negative (there is none), minus infinity where it is not in the vocabulary
+ *   logprobs [rows]: of the given tokens, never above 0; 0 where the token is negative (there is none), minus infinity where it is not in the vocabulary
  *   ranks [rows] int64: 1 + how many logits are larger than the token's; 0 where there is no token, or none of the vocabulary
  *   entropy [rows]: - sum p ln p, in nats
  *   top_logprobs, top_tokens [rows, top]: the largest log probabilities and their tokens (int64), equal ones by the lower token; top <= 32 (and <= V)

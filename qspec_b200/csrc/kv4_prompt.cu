@@ -20,7 +20,7 @@
 //     themselves or by 2^-34 of the largest, as in kv4_attention.cu; the result is rounded to 16 bits as well).
 //   * O += P V: weights from tensor memory, values from shared memory as they lie in the cache (operand "MN-major").
 // Tensor memory: S | S | O | O = 512 columns. O is multiplied again only where a row's maximum grew by more than 2^6.
-// What bounds it: 2000 tokens after 1000, 32 / 8 heads of 128, 116.8 us, 561 TFLOP/s of products (34 % of a large library product's rate). A pair of blocks takes some 5500
+// What bounds it: 2000 tokens after 1000, 32 / 8 heads of 128, 116 to 118 us, 560 TFLOP/s of products (34 % of a large library product's rate). A pair of blocks takes some 5500
 // cycles; its products are 2050 (64 each), the exponentials 2050 of a scheduler's special function unit, and both streams wait for one another's: the scores of a block take
 // 800 to 1200 cycles, the softmax 2300 alone and 3400 beside the other's, the sum of values 800. Measured and not taken (us): two accumulators of 64 keys each for a stream, scores a turn
 // ahead (151: a product of 64 columns takes as long as one of 128); one thread for both streams' products (119); the streams' exponentials in turn (120), or the second stream
