@@ -17,7 +17,7 @@
 //     for a look at a barrier takes 100 among warps that multiply and store.)
 //   * softmax: thread = row, four warps a stream. The first half of a row's scores stays in registers between the maximum and the weights; the second half is read twice.
 //     The block's power of two of the keys multiplies the scores, that of the values goes into the exponent; weights go back over the scores as float16 (off by 2^-11 of
-//     themselves or by 2^-34 of the largest, as in kv4_attention.cu; the result is rounded to 16 bits as well).
+//     themselves or by 2^-34 of the largest, as in kv4_attention.cu, or 2^-26 next to value scales that are 2^8 apart; the result is rounded to 16 bits as well).
 //   * O += P V: weights from tensor memory, values from shared memory as they lie in the cache (operand "MN-major").
 // Tensor memory: S | S | O | O = 512 columns. O is multiplied again only where a row's maximum grew by more than 2^6.
 // What bounds it: 2000 tokens after 1000, 32 / 8 heads of 128, 116 to 118 us, 560 TFLOP/s of products (34 % of a large library product's rate). A pair of blocks takes some 5500
