@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         const float mi = i ? s_ml[other][0][r] : m, li = i ? s_ml[other][1][r] : l;
         f[i] = mi == NONE ? (li == 0.f ? 0.f : 1.f) : ex2(mi - top);   // nothing seen, or no number
         if (i && both) f[i] = 0.f;
-        sum += f[i] == 0.f ? 0.f : li * f[i];
+        sum += li * f[i];                                 // (one that is no number shows whatever its part is)
       }
       const float d = sum == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, sum);  // (no key: zeros)
       const bool one = turns > 0, two = !both && __any_sync(0xffffffffu, f[1] != 0.f) && (z ? turns0 : turns1) > 0;

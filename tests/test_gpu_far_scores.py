@@ -1,4 +1,5 @@
-"""Attention over the paged caches where scores are so far from zero that a float32 has no bits left behind the point: what exponents are counted from has a rounding of its own there."""
+"""Attention over the paged caches where scores are so far from zero that a float32 has no bits left behind the point (what exponents are counted from has a rounding of its own there), or so far from
+each other that some have no weight at all."""
 import pytest
 import torch
 
@@ -81,3 +82,45 @@ def test_8_bit_cache(order, form):
                     kv8.prompt_form(*case, out, LN2, work, pairs=form == "pairs")
                 # (the prompt form joins the value scale's log2 with what the codes' 128 adds up to, 2^(E + 1): a float with half of the places)
                 check(out, (v.double() * vs.double()[..., None, None]).permute(1, 0, 2, 3).reshape(G, -1, D), T, form == "rows" or times % 2 == 0 or E < 23)
+
+
+@pytest.mark.parametrize("form", ["rows", "eights", "prompt", "pairs"])
+@pytest.mark.parametrize("cache", [4, 8])
+@pytest.mark.parametrize("high", [0, 1, 2, 5])
+@pytest.mark.parametrize("what", ["page", "key", "value"])
+def test_what_is_broken_shows_however_little_its_keys_weigh(what, high, cache, form):
+    """Keys of one block of 128 have scores 2^9 above all others'; in every other block something is broken in turn. What weighs less than 2^-127 has no part in a result, but no number has."""
+    if form == "eights" and cache == 8:
+        return
+    T = 40 if form in ("prompt", "pairs") else 2
+    k = torch.zeros(PAGES, G, P, D // 2 if cache == 4 else D, dtype=U8 if cache == 4 else torch.int8, device="cuda")
+    k[high * 4:high * 4 + 4, ..., 0] = 8                       # pages of the block
+    v = torch.ones_like(k)
+    one = torch.ones(PAGES, G, P, device="cuda") if cache == 4 else torch.ones(PAGES, G, device="cuda")
+    ks, vs = (kv4.words_of(64 * one, 0 * one), kv4.words_of(one, 0 * one)) if cache == 4 else (64 * one, one.clone())
+    table = torch.arange(PAGES, dtype=I32, device="cuda")[None]
+    q = torch.zeros(T, 8, D, dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 1.0
+    start, lens = kv4.i32([0, T]), kv4.i32([N])
+    work = ops.kv4_attention_workspace("cuda") if cache == 4 else ops.kv8_attention_workspace("cuda")
+
+    def run(ks, vs, table):
+        out, case = torch.full_like(q, 3.0), (q, k, v, ks, vs, table, start, lens)
+        if cache == 4:
+            kv4.attend("rows" if form == "eights" else form, *case, out, LN2, work, max_tokens={"rows": 20, "eights": 1}.get(form, T))
+        elif form == "rows":
+            ops.kv8_attention(*case, out, LN2, work, max_tokens=T)
+        else:
+            kv8.prompt_form(*case, out, LN2, work, pairs=form == "pairs")
+        return out
+    assert torch.isfinite(run(ks, vs, table)).all()
+    for block in range(PAGES // 4):
+        if block == high:
+            continue
+        ks2, vs2, table2 = ks.clone(), vs.clone(), table.clone()
+        page = block * 4 + 1                                   # (all tokens see it, and the other pages of its block)
+        if what == "page":
+            table2[0, page] = -1
+        else:
+            (ks2 if what == "key" else vs2)[page] = 0xff03 - 65536 if cache == 4 else float("inf")
+        assert run(ks2, vs2, table2).isnan().all(), block
