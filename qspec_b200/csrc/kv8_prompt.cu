@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     const uint32_t st = tmem + lanes + z * 128, ot = tmem + lanes + 256 + z * D;
     bool ok = !(a.give_up & 1u);
     if (!ok) s_fail = 1;
-    const float rowf = s_rowf[zrow + r], sum128 = s_sum128[zrow + r];
+    const float rowf = s_rowf[zrow + r], sum128 = limit < 0 ? 0.f : s_sum128[zrow + r];   // (a row that sees nothing has zeros, whatever its query is)
     float m = NONE, l = 0.f;
     for (int i = 0; ok && i < turns; ++i) {
       const int n = both ? i : 2 * i + z;
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
         if (i && both) f[i] = 0.f;
         sum += li * f[i];                                 // (one that is no number shows whatever its part is)
       }
-      const float d = sum == 0.f ? 0.f : __fdiv_rn(WEIGHT_UNIT, sum);  // (no key: zeros)
+      const float d = sum != 0.f ? __fdiv_rn(WEIGHT_UNIT, sum) : limit < 0 ? 0.f : NAN;  // (no key: zeros; keys that all have minus infinity, of a query that is infinite: no numbers, like any other such)
       const bool one = turns > 0, two = !both && __any_sync(0xffffffffu, f[1] != 0.f) && (z ? turns0 : turns1) > 0;
       const uint32_t stored = __ballot_sync(0xffffffffu, row_in);
       for (int half = both ? 0 : z; half <= (both ? 1 : z); ++half) {

@@ -1,5 +1,5 @@
 """Attention over the paged caches where scores are so far from zero that a float32 has no bits left behind the point (what exponents are counted from has a rounding of its own there), or so far from
-each other that some have no weight at all."""
+each other that some have no weight at all, or are no numbers."""
 import pytest
 import torch
 
@@ -124,3 +124,35 @@ def test_what_is_broken_shows_however_little_its_keys_weigh(what, high, cache, f
         else:
             (ks2 if what == "key" else vs2)[page] = 0xff03 - 65536 if cache == 4 else float("inf")
         assert run(ks2, vs2, table2).isnan().all(), block
+
+
+@pytest.mark.parametrize("form", ["rows", "eights", "prompt", "pairs"])
+@pytest.mark.parametrize("cache", [4, 8])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("query", [float("nan"), float("inf")])
+def test_rows_that_see_nothing_are_zeros_whatever_their_queries_are(query, dtype, cache, form):
+    """More tokens than keys: those in front of the first key. Others with such a query are no numbers, and their neighbours are right."""
+    make, work = (kv4.make_attention, ops.kv4_attention_workspace) if cache == 4 else (kv8.make_attention, ops.kv8_attention_workspace)
+    q, *rest = make(3, [20, 130, 0], [60, 70, 5], 8, 2, D, P, dtype)
+    outs = []
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    for spoil in (False, True):
+        x, out = q.clone(), torch.full_like(q, 3.0)
+        if spoil:
+            for at, head in ((0, 0), (7, 5), (39, 3), (40, 2), (59, 7), (100, 1), (131, 4)):   # (the first 40 tokens, and the last five, see nothing)
+                x[at, head, 5] = query
+                bad[at, head] = 40 <= at < 130
+        case = (x, *rest, out, D ** -0.5, work("cuda"))
+        if cache == 4:
+            kv4.attend("rows" if form == "eights" else form, *case, max_tokens=1 if form == "eights" else None)
+        elif form in ("rows", "eights"):
+            ops.kv8_attention(*case, max_tokens=1 if form == "eights" else None)
+        else:
+            kv8.prompt_form(*case, pairs=form == "pairs")
+        outs.append(out)
+    assert not outs[1][:40].any() and not outs[1][130:].any()
+    assert outs[1].isnan().all(2).equal(bad) and outs[1].isnan().any(2).equal(bad)
+    # (an infinite reference takes its warp's rows the way that is for references far from zero: their last bits may differ, within the bounds that either way has)
+    want, bound = (kv4 if cache == 4 else kv8).attention_in_64_bits(q, *rest, D ** -0.5)
+    assert ((outs[1].double() - want).abs() <= bound)[~bad].all()
+    assert query == float("inf") or torch.equal(outs[1][~bad], outs[0][~bad])
