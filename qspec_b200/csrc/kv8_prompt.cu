@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_prompt_kernel(const Args a) {
     const uint32_t st = tmem + lanes + z * 128, ot = tmem + lanes + 256 + z * D;
     bool ok = !(a.give_up & 1u);
     if (!ok) s_fail = 1;
-    const float rowf = s_rowf[zrow + r], sum128 = limit < 0 ? 0.f : s_sum128[zrow + r];   // (a row that sees nothing has zeros, whatever its query is)
+    const float rowf = limit < 0 ? 0.f : s_rowf[zrow + r], sum128 = limit < 0 ? 0.f : s_sum128[zrow + r];   // (a row that sees nothing has zeros, whatever its query is)
     float m = NONE, l = 0.f;
     for (int i = 0; ok && i < turns; ++i) {
       const int n = both ? i : 2 * i + z;

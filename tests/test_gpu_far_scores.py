@@ -156,3 +156,20 @@ def test_rows_that_see_nothing_are_zeros_whatever_their_queries_are(query, dtype
     want, bound = (kv4 if cache == 4 else kv8).attention_in_64_bits(q, *rest, D ** -0.5)
     assert ((outs[1].double() - want).abs() <= bound)[~bad].all()
     assert query == float("inf") or torch.equal(outs[1][~bad], outs[0][~bad])
+
+
+@pytest.mark.parametrize("form", ["rows", "eights", "prompt", "pairs"])
+@pytest.mark.parametrize("cache", [4, 8])
+def test_rows_that_see_nothing_are_zeros_over_scores_beyond_float32(cache, form):
+    make, work = (kv4.make_attention, ops.kv4_attention_workspace) if cache == 4 else (kv8.make_attention, ops.kv8_attention_workspace)
+    q, k, v, ks, vs, table, start, lens = make(4, [20, 130], [60, 70], 8, 2, D, P, torch.bfloat16, q_scale=1e30)
+    ks = ((ks.to(I32) & 0xffff) + (60 << 8)).clamp(max=0xfe00).to(torch.int16) if cache == 4 else ks * 2.0 ** 60
+    out = torch.full_like(q, 3.0)
+    case = (q, k, v, ks, vs, table, start, lens, out, D ** -0.5, work("cuda"))
+    if cache == 4:
+        kv4.attend("rows" if form == "eights" else form, *case, max_tokens=1 if form == "eights" else None)
+    elif form in ("rows", "eights"):
+        ops.kv8_attention(*case, max_tokens=1 if form == "eights" else None)
+    else:
+        kv8.prompt_form(*case, pairs=form == "pairs")
+    assert not out[:40].any()
